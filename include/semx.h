@@ -567,6 +567,52 @@ size_t semx_linoss_readout_workspace_bytes(const SemxLinossReadoutArgs* args);
 int semx_linoss_readout_fwd(const SemxLinossReadoutArgs* args, semx_stream_t stream);
 int semx_linoss_readout_bwd(const SemxLinossReadoutArgs* args, semx_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Layer normalisation over the last dimension, with an optional residual added first (the
+ * pre-norm Block's nn.LayerNorm and its residual add, create_block with rms_norm=False and
+ * fused_add_norm=True, models/mamba_block.py:303-344):
+ *   s = x + residual (x when residual is NULL), mean = mean_j(s), var = mean_j((s - mean)^2)
+ *   y[r, j] = (s[r, j] - mean) / sqrt(var + eps) * weight[j] + bias[j]
+ * in fp32. n rows of d <= 32768 contiguous elements. x, dx are bf16 when x_bf16 is set,
+ * else fp32; residual, dresidual by r_bf16; y, dy by y_bf16; sum, dsum by s_bf16. The sum is
+ * written when a residual is given (required then), and the norm is that of the sum as
+ * stored. weight (1 when NULL) and bias (0 when NULL) fp32. mean, rstd (n) fp32: written
+ * by the forward when non-NULL.
+ * Backward reads sum (x itself where there was no residual, with s_bf16 = x_bf16), mean,
+ * rstd, dy and dsum (the gradient that arrives at the sum, may be NULL), and writes dx, the
+ * same values as dresidual when non-NULL, and dweight, dbias (fp32, each may be NULL),
+ * reduced over rows in a fixed order (workspace: semx_layer_norm_workspace_bytes()).
+ * ---------------------------------------------------------------------------------- */
+typedef struct SemxLayerNormArgs {
+  uint32_t struct_size;
+  float eps;
+  int32_t x_bf16;
+  int32_t r_bf16;
+  int32_t y_bf16;
+  int32_t s_bf16;
+  int64_t n, d; /* rows, elements per row */
+  const void* x;
+  const void* residual;
+  const float* weight;
+  const float* bias;
+  void* y;
+  void* sum;
+  float* mean;
+  float* rstd;
+  const void* dy;
+  const void* dsum;
+  void* dx;
+  void* dresidual;
+  float* dweight;
+  float* dbias;
+  void* workspace;
+} SemxLayerNormArgs;
+
+size_t semx_layer_norm_args_size(void);
+size_t semx_layer_norm_workspace_bytes(const SemxLayerNormArgs* args);
+int semx_layer_norm_fwd(const SemxLayerNormArgs* args, semx_stream_t stream);
+int semx_layer_norm_bwd(const SemxLayerNormArgs* args, semx_stream_t stream);
+
 size_t semx_mimo_layer_args_size(void);
 size_t semx_mimo_layer_ckpt_bytes(const SemxMimoLayerArgs* args);
 size_t semx_mimo_layer_workspace_bytes(const SemxMimoLayerArgs* args);

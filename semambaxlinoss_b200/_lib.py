@@ -233,6 +233,21 @@ class SemxLinossReadoutArgs(ctypes.Structure):
     ] + [(n, ctypes.c_void_p) for n in ("x", "y2", "C", "D", "y", "dy", "dx", "dC", "dD", "workspace")]
 
 
+class SemxLayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("eps", ctypes.c_float),
+        ("x_bf16", ctypes.c_int32),
+        ("r_bf16", ctypes.c_int32),
+        ("y_bf16", ctypes.c_int32),
+        ("s_bf16", ctypes.c_int32),
+        ("n", ctypes.c_int64),
+        ("d", ctypes.c_int64),
+    ] + [(name, ctypes.c_void_p) for name in (
+        "x", "residual", "weight", "bias", "y", "sum", "mean", "rstd", "dy", "dsum", "dx", "dresidual",
+        "dweight", "dbias", "workspace")]
+
+
 # (python struct, C size query) for every argument struct in semx.h.
 STRUCTS = {
     "SemxLinossArgs": (SemxLinossArgs, "semx_linoss_args_size"),
@@ -245,6 +260,7 @@ STRUCTS = {
     "SemxRmsNormArgs": (SemxRmsNormArgs, "semx_rms_norm_args_size"),
     "SemxStepProjArgs": (SemxStepProjArgs, "semx_step_proj_args_size"),
     "SemxLinossReadoutArgs": (SemxLinossReadoutArgs, "semx_linoss_readout_args_size"),
+    "SemxLayerNormArgs": (SemxLayerNormArgs, "semx_layer_norm_args_size"),
 }
 
 # Every symbol semx.h declares, with its ctypes signature.
@@ -299,6 +315,10 @@ _SIGNATURES = {
     "semx_linoss_readout_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxLinossReadoutArgs)]),
     "semx_linoss_readout_fwd": (ctypes.c_int, [ctypes.POINTER(SemxLinossReadoutArgs), ctypes.c_void_p]),
     "semx_linoss_readout_bwd": (ctypes.c_int, [ctypes.POINTER(SemxLinossReadoutArgs), ctypes.c_void_p]),
+    "semx_layer_norm_args_size": (ctypes.c_size_t, []),
+    "semx_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxLayerNormArgs)]),
+    "semx_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(SemxLayerNormArgs), ctypes.c_void_p]),
+    "semx_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(SemxLayerNormArgs), ctypes.c_void_p]),
     "semx_mimo_layer_args_size": (ctypes.c_size_t, []),
     "semx_mimo_layer_ckpt_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),
     "semx_mimo_layer_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),

@@ -25,6 +25,26 @@ int check_launch(const char* what);
 // that holds the operands, whichever device the caller's own runtime has current.
 int bind_device(std::initializer_list<const void*> ptrs);
 
+// bind_device() for the length of a scope: the device that was current before is current
+// again when the scope ends.
+class DeviceScope {
+ public:
+  DeviceScope() = default;
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  ~DeviceScope() {
+    int cur = -1;
+    if (prev_ >= 0 && (cudaGetDevice(&cur) != cudaSuccess || cur != prev_)) cudaSetDevice(prev_);
+  }
+  int bind(std::initializer_list<const void*> ptrs) {
+    if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+    return bind_device(ptrs);
+  }
+
+ private:
+  int prev_ = -1;
+};
+
 inline bool aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;
 }

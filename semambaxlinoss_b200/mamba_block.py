@@ -12,6 +12,8 @@ checkout. Their documented behaviour is restated here:
   block: ``residual = x + residual`` (or ``x`` when no residual is given),
   ``h = mixer(norm(residual))``; returns ``(h, residual)``; the caller adds the final
   residual.
+* ``create_block(rms_norm=False, fused_add_norm=True)`` takes this package's ``LayerNorm``
+  (nn.LayerNorm's parameters), whose kernel adds the residual and normalises in one pass.
 * ``_init_weights(module, n_layer)``: zero every Linear bias not tagged ``_no_reinit``;
   re-draw every ``out_proj.weight`` / ``fc2.weight`` Kaiming-uniform (a = sqrt(5)) and
   divide it by sqrt(n_layer).
@@ -41,6 +43,7 @@ from torch import nn
 import torch.nn.functional as F
 
 from . import _lib
+from .layer_norm import LayerNorm
 from .layout import TokenLayout
 from .linoss import LinOSS
 from .mixer import MambaStyleMixer
@@ -103,7 +106,8 @@ class RMSNorm(nn.Module):
 
 
 class Block(nn.Module):
-    """Pre-norm residual block: returns (mixer(norm(x + residual)), x + residual)."""
+    """Pre-norm residual block: returns (mixer(norm(x + residual)), x + residual). With
+    ``fused_add_norm`` and this package's LayerNorm the sum and the norm are one kernel."""
 
     def __init__(self, dim, mixer_cls, mlp_cls=nn.Identity, norm_cls=nn.LayerNorm,
                  fused_add_norm=False, residual_in_fp32=False):
@@ -119,15 +123,29 @@ class Block(nn.Module):
             self.mlp = None
 
     def forward(self, hidden_states, residual=None, inference_params=None, **mixer_kwargs):
-        residual = hidden_states + residual if residual is not None else hidden_states
-        hidden_states = self.norm(residual.to(dtype=self.norm.weight.dtype))
+        if self.fused_add_norm and isinstance(self.norm, LayerNorm):
+            hidden_states, residual = _add_norm(self.norm, hidden_states, residual)
+        else:
+            residual = hidden_states + residual if residual is not None else hidden_states
+            hidden_states = self.norm(residual.to(dtype=self.norm.weight.dtype))
         if self.residual_in_fp32:
             residual = residual.to(torch.float32)
         hidden_states = self.mixer(hidden_states, inference_params=inference_params, **mixer_kwargs)
         if self.mlp is not None:
-            residual = hidden_states + residual
-            hidden_states = self.mlp(self.norm2(residual.to(dtype=self.norm2.weight.dtype)))
+            if self.fused_add_norm and isinstance(self.norm2, LayerNorm):
+                hidden_states, residual = _add_norm(self.norm2, hidden_states, residual)
+            else:
+                residual = hidden_states + residual
+                hidden_states = self.norm2(residual.to(dtype=self.norm2.weight.dtype))
+            hidden_states = self.mlp(hidden_states)
         return hidden_states, residual
+
+
+def _add_norm(norm: LayerNorm, x, residual):
+    """(norm(x + residual) in the norm's type, x + residual) as one kernel."""
+    if residual is None:
+        return norm(x.to(dtype=norm.weight.dtype)), x
+    return norm(x, residual, out_dtype=norm.weight.dtype)
 
 
 def _init_weights(module, n_layer, initializer_range=0.02, rescale_prenorm_residual=True,
@@ -147,6 +165,8 @@ def _init_weights(module, n_layer, initializer_range=0.02, rescale_prenorm_resid
 
 def _apply_layer_norm(x, residual, norm_layer):
     """Pre-norm add + norm: returns (norm(x + residual), x + residual)."""
+    if isinstance(norm_layer, LayerNorm):
+        return _add_norm(norm_layer, x, residual)
     residual = x + residual if residual is not None else x
     return norm_layer(residual), residual
 
@@ -257,7 +277,8 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
 def create_block(d_model, model_cfg, layer_idx=0, rms_norm=True, fused_add_norm=False,
                  residual_in_fp32=False):
     norm_eps = model_cfg.get("norm_epsilon", 1e-5)
-    norm_cls = partial(nn.LayerNorm if not rms_norm else RMSNorm, eps=norm_eps)
+    layer_norm_cls = LayerNorm if fused_add_norm else nn.LayerNorm
+    norm_cls = partial(layer_norm_cls if not rms_norm else RMSNorm, eps=norm_eps)
     if model_cfg["ssm"] == "hybrid":
         hybrid_cfg = model_cfg.get("hybrid", {})
         b1 = _build_mixer_cls(d_model, model_cfg["backbone_1"], layer_idx)(d_model)
