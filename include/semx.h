@@ -613,6 +613,116 @@ size_t semx_layer_norm_workspace_bytes(const SemxLayerNormArgs* args);
 int semx_layer_norm_fwd(const SemxLayerNormArgs* args, semx_stream_t stream);
 int semx_layer_norm_bwd(const SemxLayerNormArgs* args, semx_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Selective state mixer: a short causal convolution and a selective scan whose sequences
+ * can keep their state between calls. (The reference takes such a mixer, its "mamba"
+ * backbone, from mamba_ssm, models/mamba_block.py:105-299; the formulas are restated here.)
+ *
+ * Sequences (both operators): S sequences of L rows (cu_seqlens NULL, rows = S L, row
+ * s L + t), or `rows` packed rows with cu_seqlens (S + 1, int32, device): sequence s owns
+ * rows [cu_seqlens[s], cu_seqlens[s+1]), lengths from 0; rows from cu_seqlens[S] on belong
+ * to none: their outputs and gradients are zeros. L is ignored with cu_seqlens. The
+ * offsets must not decrease; they are clamped, so that bad ones give wrong rows and no
+ * access outside the rows.
+ * State: a pool of n_slots entries, updated in place; sequence s has entry slots[s] (int32,
+ * device; NULL: entry s). A negative slot: the sequence starts from zeros and leaves
+ * nothing. A slot >= n_slots, or one that an earlier sequence of the call has, is refused
+ * for that sequence: its outputs are NaN, its entry stays as it was. fresh (S bytes, device;
+ * NULL: none): where non-zero the sequence starts from zeros and its entry is replaced. A
+ * sequence of no rows leaves its entry (zeros if fresh). state NULL (n_slots 0): every
+ * sequence starts from zeros. Only the forward takes a state.
+ * Rows of x, dt, z, B and C are read at their own row strides (elements); y, dy and the
+ * gradients are contiguous.
+ * ---------------------------------------------------------------------------------- */
+
+/* Short causal depthwise convolution of K taps (1..8), with SiLU when `silu` is set:
+ *   y[t, c] = act(b[c] + sum_k w[c, k] x[t - (K - 1) + k, c])
+ * The state entry is the sequence's last K - 1 inputs: state (n_slots, K - 1, C) in x's type.
+ * A single token per sequence is L = 1. x, y, state, dy, dx are bf16 when `bf16` is set,
+ * else fp32; w (C, K), b (C, may be NULL), dw, db fp32. Backward writes dx, and dw / db
+ * (each may be NULL) reduced over rows in a fixed order (workspace:
+ * semx_short_conv_workspace_bytes()). */
+typedef struct SemxShortConvArgs {
+  uint32_t struct_size;
+  int32_t K;
+  int32_t silu;
+  int32_t bf16;
+  int64_t S, rows, L, C, ldx, n_slots;
+  const void* x;
+  const float* w;
+  const float* b;
+  void* y;
+  const int32_t* cu_seqlens;
+  void* state;
+  const int32_t* slots;
+  const uint8_t* fresh;
+  const void* dy;
+  void* dx;
+  float* dw;
+  float* db;
+  void* workspace;
+} SemxShortConvArgs;
+
+size_t semx_short_conv_args_size(void);
+size_t semx_short_conv_workspace_bytes(const SemxShortConvArgs* args);
+int semx_short_conv_fwd(const SemxShortConvArgs* args, semx_stream_t stream);
+int semx_short_conv_bwd(const SemxShortConvArgs* args, semx_stream_t stream);
+
+/* Selective state scan of N modes (1..128) per channel, channels in G groups that share B
+ * and C (C % G == 0):
+ *   d = dt + dt_bias[c]  (softplus of it when `softplus` is set: x above 20)
+ *   h[n] = exp(d A[c, n]) h[n] + d x B[t, g, n]          (fp32; the state entry (C, N))
+ *   v = sum_n C[t, g, n] h[n] + D[c] x;   y = v silu(z), or v without z
+ * x, z, B, C, y (and their gradients) are bf16 when `bf16` is set, else fp32; dt, ddt by
+ * dt_bf16; A, D, dt_bias (the last two may be NULL: 0) and their gradients fp32;
+ * state (n_slots, C, N) fp32. B and C rows hold (G, N) contiguously.
+ * semx_state_scan_*: whole sequences. A training forward passes ckpt
+ * (semx_state_scan_ckpt_bytes()) and, with z, v (rows, C) in x's type; the backward reads
+ * them and writes dx, ddt, dz (with z), dB, dC (rows, G, N), and dA, dD, ddt_bias (each may
+ * be NULL), all reduced in a fixed order. Workspace: semx_state_scan_workspace_bytes() with
+ * `backward` 0 or 1 (0 bytes where none is needed).
+ * semx_state_step: one row per sequence (cu_seqlens NULL, L = 1), state required. */
+typedef struct SemxStateScanArgs {
+  uint32_t struct_size;
+  int32_t softplus;
+  int32_t bf16;
+  int32_t dt_bf16;
+  int64_t S, rows, L, C, N, G, n_slots;
+  int64_t ldx, lddt, ldz, ldb, ldc;
+  const void* x;
+  const void* dt;
+  const float* A;
+  const void* B;
+  const void* Cm;
+  const float* D;
+  const void* z;
+  const float* dt_bias;
+  void* y;
+  const int32_t* cu_seqlens;
+  float* state;
+  const int32_t* slots;
+  const uint8_t* fresh;
+  void* v;
+  float* ckpt;
+  const void* dy;
+  void* dx;
+  void* ddt;
+  void* dz;
+  void* dB;
+  void* dC;
+  float* dA;
+  float* dD;
+  float* ddt_bias;
+  void* workspace;
+} SemxStateScanArgs;
+
+size_t semx_state_scan_args_size(void);
+size_t semx_state_scan_ckpt_bytes(const SemxStateScanArgs* args);
+size_t semx_state_scan_workspace_bytes(const SemxStateScanArgs* args, int32_t backward);
+int semx_state_scan_fwd(const SemxStateScanArgs* args, semx_stream_t stream);
+int semx_state_scan_bwd(const SemxStateScanArgs* args, semx_stream_t stream);
+int semx_state_step(const SemxStateScanArgs* args, semx_stream_t stream);
+
 size_t semx_mimo_layer_args_size(void);
 size_t semx_mimo_layer_ckpt_bytes(const SemxMimoLayerArgs* args);
 size_t semx_mimo_layer_workspace_bytes(const SemxMimoLayerArgs* args);

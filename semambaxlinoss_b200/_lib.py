@@ -248,6 +248,30 @@ class SemxLayerNormArgs(ctypes.Structure):
         "dweight", "dbias", "workspace")]
 
 
+class SemxShortConvArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("K", ctypes.c_int32),
+        ("silu", ctypes.c_int32),
+        ("bf16", ctypes.c_int32),
+    ] + [(name, ctypes.c_int64) for name in ("S", "rows", "L", "C", "ldx", "n_slots")] + [
+        (name, ctypes.c_void_p) for name in (
+            "x", "w", "b", "y", "cu_seqlens", "state", "slots", "fresh", "dy", "dx", "dw", "db", "workspace")]
+
+
+class SemxStateScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("softplus", ctypes.c_int32),
+        ("bf16", ctypes.c_int32),
+        ("dt_bf16", ctypes.c_int32),
+    ] + [(name, ctypes.c_int64) for name in (
+        "S", "rows", "L", "C", "N", "G", "n_slots", "ldx", "lddt", "ldz", "ldb", "ldc")] + [
+        (name, ctypes.c_void_p) for name in (
+            "x", "dt", "A", "B", "Cm", "D", "z", "dt_bias", "y", "cu_seqlens", "state", "slots", "fresh", "v",
+            "ckpt", "dy", "dx", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "workspace")]
+
+
 # (python struct, C size query) for every argument struct in semx.h.
 STRUCTS = {
     "SemxLinossArgs": (SemxLinossArgs, "semx_linoss_args_size"),
@@ -261,6 +285,8 @@ STRUCTS = {
     "SemxStepProjArgs": (SemxStepProjArgs, "semx_step_proj_args_size"),
     "SemxLinossReadoutArgs": (SemxLinossReadoutArgs, "semx_linoss_readout_args_size"),
     "SemxLayerNormArgs": (SemxLayerNormArgs, "semx_layer_norm_args_size"),
+    "SemxShortConvArgs": (SemxShortConvArgs, "semx_short_conv_args_size"),
+    "SemxStateScanArgs": (SemxStateScanArgs, "semx_state_scan_args_size"),
 }
 
 # Every symbol semx.h declares, with its ctypes signature.
@@ -319,6 +345,16 @@ _SIGNATURES = {
     "semx_layer_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxLayerNormArgs)]),
     "semx_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(SemxLayerNormArgs), ctypes.c_void_p]),
     "semx_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(SemxLayerNormArgs), ctypes.c_void_p]),
+    "semx_short_conv_args_size": (ctypes.c_size_t, []),
+    "semx_short_conv_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxShortConvArgs)]),
+    "semx_short_conv_fwd": (ctypes.c_int, [ctypes.POINTER(SemxShortConvArgs), ctypes.c_void_p]),
+    "semx_short_conv_bwd": (ctypes.c_int, [ctypes.POINTER(SemxShortConvArgs), ctypes.c_void_p]),
+    "semx_state_scan_args_size": (ctypes.c_size_t, []),
+    "semx_state_scan_ckpt_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxStateScanArgs)]),
+    "semx_state_scan_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_int32]),
+    "semx_state_scan_fwd": (ctypes.c_int, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_void_p]),
+    "semx_state_scan_bwd": (ctypes.c_int, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_void_p]),
+    "semx_state_step": (ctypes.c_int, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_void_p]),
     "semx_mimo_layer_args_size": (ctypes.c_size_t, []),
     "semx_mimo_layer_ckpt_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),
     "semx_mimo_layer_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),

@@ -28,7 +28,9 @@ place. A scan layer that cannot read a layout (the MIMO layer; a streamed
 SelectiveLRU for strided layouts) falls back to the reference's copies.
 
 Supported mixers: ``selective_lru``, ``selective_lru_mimo``, ``linoss`` (the layers on
-this package's scan path). The reference's other backbones (``mamba``, ``mamba2``,
+this package's scan path), and ``selective_state`` (the Mamba layer's formulas with packed
+sequences, prompts and single tokens; ``ssm_params``: the mixer's own keyword arguments;
+``cu_seqlens``, ``cache``, ``slots`` and ``fresh`` pass through ``Block.forward``). The reference's other backbones (``mamba``, ``mamba2``,
 ``mamba3`` from mamba_ssm, ``s4d``, ``s5``, and ``selective_linoss``, whose source the
 reference does not contain) raise NotImplementedError.
 """
@@ -48,6 +50,7 @@ from .layout import TokenLayout
 from .linoss import LinOSS
 from .mixer import MambaStyleMixer
 from .selective_lru import SelectiveLRU, SelectiveLRUMIMO
+from .selective_state import SelectiveStateMixer
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -230,6 +233,10 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
     ssm_params = model_cfg.get("ssm_params", {}) or {}
     d_state, d_conv, expand = model_cfg["d_state"], model_cfg["d_conv"], model_cfg["expand"]
     causal = model_cfg.get("causal_conv", True)
+    if ssm == "selective_state":
+        if not causal:
+            raise ValueError("the selective_state mixer's convolution is causal; causal_conv must be True")
+        return partial(SelectiveStateMixer, d_state=d_state, d_conv=d_conv, expand=expand, **ssm_params)
     if ssm == "linoss":
         layer = LinOSS(
             in_features=expand * d_model,

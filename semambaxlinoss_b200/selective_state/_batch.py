@@ -1,0 +1,96 @@
+"""Argument checks and batch description shared by the selective state operators."""
+from __future__ import annotations
+
+import torch
+
+TYPES = (torch.float32, torch.bfloat16)
+_ROW_MAX = 2 ** 31
+
+
+def rows_of(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
+    """``t`` (rows, width) or (S, L, width) as (tensor, row stride): read in place where its
+    rows lie at one stride with contiguous elements, else a contiguous copy."""
+    if t.stride(-1) == 1 or width == 1:
+        if t.dim() == 2:
+            ld = t.stride(0) if t.shape[0] > 1 else width
+        elif t.shape[1] == 1:
+            ld = t.stride(0) if t.shape[0] > 1 else width
+        elif t.shape[0] == 1 or t.stride(0) == t.shape[1] * t.stride(1):
+            ld = t.stride(1)
+        else:
+            ld = 0
+        if width <= ld < _ROW_MAX:
+            return t, ld
+    return t.contiguous(), width
+
+
+def check_same(op: str, name: str, t: torch.Tensor, shape, dtypes, device) -> None:
+    if t.shape != shape or t.dtype not in dtypes or t.device != device:
+        want = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+        raise ValueError(f"{op}: {name} must be {want} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
+
+
+def param32(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A parameter as the kernels read it: contiguous fp32 (no copy where it is that already)."""
+    if t is None:
+        return None
+    t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
+def batch(op: str, x: torch.Tensor, cu_seqlens) -> tuple[int, int, int]:
+    """(S, rows, L) of x (S, L, C), or of packed x (rows, C) with cu_seqlens (S + 1)."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{op} requires CUDA tensors.")
+    if x.dtype not in TYPES:
+        raise ValueError(f"{op}: unsupported dtype {x.dtype}")
+    if cu_seqlens is None:
+        if x.dim() != 3:
+            raise ValueError(f"{op}: x must be (batch, length, channels), or (rows, channels) with cu_seqlens, got "
+                             f"{tuple(x.shape)}")
+        return x.shape[0], x.shape[0] * x.shape[1], x.shape[1]
+    if x.dim() != 2:
+        raise ValueError(f"{op}: packed x must be (rows, channels), got {tuple(x.shape)}")
+    if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1
+            or cu_seqlens.device != x.device or not cu_seqlens.is_contiguous()):
+        raise ValueError(f"{op}: cu_seqlens must be contiguous int32 (sequences + 1,) on {x.device}, got "
+                         f"{cu_seqlens.dtype} {tuple(cu_seqlens.shape)} on {cu_seqlens.device}")
+    return cu_seqlens.shape[0] - 1, x.shape[0], 0
+
+
+def set_pool(op: str, a, S: int, device, state, shape, dtype, slots, fresh) -> None:
+    """Checks the state pool (entries of ``shape``) and its index and fills the argument struct."""
+    if state is None:
+        if slots is not None or fresh is not None:
+            raise ValueError(f"{op}: slots / fresh without a state")
+        return
+    if (state.dim() != 1 + len(shape) or state.shape[1:] != shape or state.dtype != dtype or state.device != device
+            or not state.is_contiguous()):
+        raise ValueError(f"{op}: the state must be contiguous {str(dtype)[6:]} (entries, "
+                         f"{', '.join(map(str, shape))}) on {device}, got {state.dtype} {tuple(state.shape)} on "
+                         f"{state.device}")
+    if torch.is_grad_enabled() and state.requires_grad:
+        raise ValueError(f"{op}: the state is updated in place and cannot require a gradient")
+    n = state.shape[0]
+    if slots is None:
+        if n < S:
+            raise ValueError(f"{op}: {n} state entries for {S} sequences")
+    elif slots.shape != (S,) or slots.dtype != torch.int32 or slots.device != device or not slots.is_contiguous():
+        raise ValueError(f"{op}: slots must be contiguous int32 ({S},) on {device}, got {slots.dtype} "
+                         f"{tuple(slots.shape)} on {slots.device}")
+    else:
+        a.slots = slots.data_ptr()
+    if fresh is not None:
+        if fresh.shape != (S,) or fresh.dtype != torch.bool or fresh.device != device or not fresh.is_contiguous():
+            raise ValueError(f"{op}: fresh must be contiguous bool ({S},) on {device}, got {fresh.dtype} "
+                             f"{tuple(fresh.shape)} on {fresh.device}")
+        a.fresh = fresh.data_ptr()
+    if n == 0:
+        # Every slot is behind an empty pool; the library takes a pool of none as "no state".
+        raise ValueError(f"{op}: the state has no entries")
+    a.n_slots, a.state = n, state.data_ptr()
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

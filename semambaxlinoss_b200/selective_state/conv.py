@@ -1,0 +1,130 @@
+"""Short causal depthwise convolution over sequences that can keep their last inputs
+(``semx_short_conv_fwd/bwd``).
+
+    y[t, c] = act(bias[c] + sum_k weight[c, k] x[t - (K - 1) + k, c])
+
+Unlike the convolution inside ``MambaStyleMixer`` (:mod:`semambaxlinoss_b200.mixer`), x is
+any tensor of rows (packed sequences of many lengths too), y has x's type, and a sequence
+can start from the window that an earlier call left.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool, wants_grad
+
+_ACTIVATIONS = {"silu": 1, None: 0}
+
+
+def _weight(op, weight, C):
+    """(C, K) of a weight (C, K) or (C, 1, K) (``nn.Conv1d``'s, groups = channels)."""
+    w = weight.squeeze(1) if weight.dim() == 3 and weight.shape[1] == 1 else weight
+    if w.dim() != 2 or w.shape[0] != C or not 1 <= w.shape[1] <= 8:
+        raise ValueError(f"{op}: weight must be ({C}, taps) or ({C}, 1, taps) with 1 to 8 taps, got "
+                         f"{tuple(weight.shape)}")
+    return w
+
+
+def _args(x, w, b, silu, S, rows, L, cu):
+    C = x.shape[-1]
+    xr, ld = rows_of(x, C)
+    a = _lib.new_args(_lib.SemxShortConvArgs)
+    a.K, a.silu, a.bf16 = w.shape[1], silu, x.dtype == torch.bfloat16
+    a.S, a.rows, a.L, a.C, a.ldx = S, rows, L, C, ld
+    a.x, a.w = xr.data_ptr(), w.data_ptr()
+    if b is not None:
+        a.b = b.data_ptr()
+    if cu is not None:
+        a.cu_seqlens = cu.data_ptr()
+    return a, xr
+
+
+class _ShortConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, silu, S, rows, L, cu):
+        w, b = param32(weight), param32(bias)
+        a, xr = _args(x.detach(), w, b, silu, S, rows, L, cu)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a.y = y.data_ptr()
+        _lib.call("semx_short_conv_fwd", a, x.device)
+        ctx.save_for_backward(xr, w, b, cu)
+        ctx.cfg = (silu, S, rows, L, weight.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, b, cu = ctx.saved_tensors
+        silu, S, rows, L, wdt, bdt = ctx.cfg
+        a, xr = _args(x, w, b, silu, S, rows, L, cu)
+        dy = dy.to(x.dtype).contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
+        db = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
+        a.dy, a.dx, a.dw, a.db = dy.data_ptr(), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db)
+        ws = None
+        if dw is not None or db is not None:
+            ws = _lib.empty_f32(_lib.load().semx_short_conv_workspace_bytes(a), x.device)
+            a.workspace = ws.data_ptr()
+        _lib.call("semx_short_conv_bwd", a, x.device)
+        return (dx, None if dw is None else dw.to(wdt), None if db is None else db.to(bdt), None, None, None, None,
+                None)
+
+
+def _silu_flag(op, activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{op}: activation must be 'silu' or None, got {activation!r}")
+    return _ACTIVATIONS[activation]
+
+
+def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = "silu",
+               cu_seqlens: torch.Tensor | None = None, state: torch.Tensor | None = None,
+               slots: torch.Tensor | None = None, fresh: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal depthwise convolution of the sequences in ``x``; y has x's shape and type.
+
+    x: (S, L, C), or packed (rows, C) with ``cu_seqlens`` (S + 1, int32): sequence s owns rows
+    cu_seqlens[s] .. cu_seqlens[s+1] - 1 (none, if they are equal); rows from cu_seqlens[S] on
+    belong to no sequence and come out as zeros. Rows may lie at any stride (a slice of
+    the in_proj output is read in place). weight (C, K) or (C, 1, K), K from 1 to 8, bias (C,).
+
+    Training: gradients flow to x, weight and bias, every sequence starts from zeros.
+    Prompts: ``state`` (entries, K - 1, C) in x's type holds the last K - 1 inputs of running
+    sequences and is updated in place; sequence s uses entry ``slots[s]`` (int32; entry s
+    without slots), from zeros where ``fresh[s]``. A negative slot: no entry, from zeros. A
+    slot behind the pool, or one an earlier sequence of the call has, gives NaN for that
+    sequence and leaves the entry alone. Not differentiable: refused while a gradient is
+    wanted (call it under ``torch.no_grad()``)."""
+    op = "short_conv"
+    S, rows, L = batch(op, x, cu_seqlens)
+    silu = _silu_flag(op, activation)
+    C = x.shape[-1]
+    w = _weight(op, weight, C)
+    check_same(op, "weight", w, w.shape, TYPES, x.device)
+    if bias is not None:
+        check_same(op, "bias", bias, (C,), TYPES, x.device)
+    if wants_grad(x, weight, bias):
+        if state is not None:
+            raise ValueError(f"{op}: a state is for inference; the call wants gradients")
+        if slots is not None or fresh is not None:
+            raise ValueError(f"{op}: slots / fresh without a state")
+        return _ShortConv.apply(x, w, bias, silu, S, rows, L, cu_seqlens)
+    w32, b32 = param32(w), param32(bias)
+    a, xr = _args(x.detach(), w32, b32, silu, S, rows, L, cu_seqlens)
+    if w.shape[1] > 1 or state is None:
+        set_pool(op, a, S, x.device, state, (w.shape[1] - 1, C), x.dtype, slots, fresh)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a.y = y.data_ptr()
+    _lib.call("semx_short_conv_fwd", a, x.device)
+    return y
+
+
+def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                    activation: str | None = "silu", slots: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of every sequence: x (S, C) -> y (S, C); the windows in ``state`` (entries,
+    K - 1, C) move on by one in place. Slots as in :func:`short_conv`."""
+    if x.dim() != 2:
+        raise ValueError(f"short_conv_step: x must be (sequences, channels), got {tuple(x.shape)}")
+    if state is None:
+        raise ValueError("short_conv_step: a state is needed")
+    return short_conv(x.unsqueeze(1), weight, bias, activation, None, state, slots).squeeze(1)
