@@ -416,15 +416,22 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+# The current stream's handle without building a Stream object (2.3 us -> 0.1 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
 def call(fn_name: str, args, device) -> None:
     """Runs a semx entry point on the current stream of `device`; raises on failure."""
-    lib = load()
+    lib = _lib or load()
     status = getattr(lib, fn_name)(ctypes.byref(args), stream_handle(device))
-    check(fn_name, status)
+    if status != SEMX_OK:
+        check(fn_name, status)
 
 
 def empty_f32(nbytes: int, device) -> torch.Tensor:

@@ -23,7 +23,9 @@ MAX_WIDTH = 32768
 
 
 def _param(p):
-    return None if p is None else p.detach().to(torch.float32).contiguous()
+    if p is None or (p.dtype == torch.float32 and p.is_contiguous()):
+        return p
+    return p.detach().to(torch.float32).contiguous()
 
 
 def _forward(x, weight, bias, eps, residual, out_dtype, stats):
@@ -31,7 +33,7 @@ def _forward(x, weight, bias, eps, residual, out_dtype, stats):
     unless ``stats``."""
     d = x.shape[-1]
     x = x.contiguous()
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    y = x.new_empty(x.shape, dtype=out_dtype)
     a = _lib.new_args(_lib.SemxLayerNormArgs)
     a.eps, a.n, a.d = eps, x.numel() // d, d
     a.x_bf16, a.y_bf16 = x.dtype == torch.bfloat16, out_dtype == torch.bfloat16
@@ -39,7 +41,7 @@ def _forward(x, weight, bias, eps, residual, out_dtype, stats):
     s = x
     if residual is not None:
         residual = residual.contiguous()
-        s = torch.empty(x.shape, dtype=torch.promote_types(x.dtype, residual.dtype), device=x.device)
+        s = x.new_empty(x.shape, dtype=residual.dtype if x.dtype == torch.bfloat16 else x.dtype)
         a.r_bf16, a.s_bf16 = residual.dtype == torch.bfloat16, s.dtype == torch.bfloat16
         a.residual, a.sum = residual.data_ptr(), s.data_ptr()
     if weight is not None:
@@ -59,8 +61,8 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, residual, out_dtype):
         ctx.set_materialize_grads(False)
         w, b = _param(weight), _param(bias)
-        r = None if residual is None else residual.detach()
-        y, s, mean, rstd = _forward(x.detach(), w, b, eps, r, out_dtype, True)
+        r = residual
+        y, s, mean, rstd = _forward(x, w, b, eps, r, out_dtype, True)
         ctx.save_for_backward(s, w, mean, rstd)
         ctx.cfg = (eps, out_dtype, x.dtype, None if r is None else r.dtype,
                    None if weight is None else weight.dtype, None if bias is None else bias.dtype)
@@ -117,14 +119,16 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     if d < 1:
         raise ValueError(f"layer_norm: nothing to normalise in shape {tuple(x.shape)}")
     for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None and (p.shape != (d,) or p.device != x.device):
+        if p is not None and (p.shape != (d,) or p.get_device() != x.get_device()):
             raise ValueError(f"layer_norm: {name} must be ({d},) on {x.device}, got {tuple(p.shape)} on {p.device}")
-    if residual is not None and (residual.shape != x.shape or residual.device != x.device
+    if residual is not None and (residual.shape != x.shape or residual.get_device() != x.get_device()
                                  or residual.dtype not in _TYPES):
         raise ValueError(f"layer_norm: residual must be fp32 or bf16 {tuple(x.shape)} on {x.device}, got "
                          f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
     eps = float(eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, residual, out_dtype)
     y, s, _, _ = _forward(x, _param(weight), _param(bias), eps, residual, out_dtype, False)
     return y if residual is None else (y, s)

@@ -7,16 +7,20 @@ TYPES = (torch.float32, torch.bfloat16)
 _ROW_MAX = 2 ** 31
 
 
-def rows_of(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
-    """``t`` (rows, width) or (S, L, width) as (tensor, row stride): read in place where its
-    rows lie at one stride with contiguous elements, else a contiguous copy."""
-    if t.stride(-1) == 1 or width == 1:
-        if t.dim() == 2:
-            ld = t.stride(0) if t.shape[0] > 1 else width
-        elif t.shape[1] == 1:
-            ld = t.stride(0) if t.shape[0] > 1 else width
-        elif t.shape[0] == 1 or t.stride(0) == t.shape[1] * t.stride(1):
-            ld = t.stride(1)
+def rows_of(t: torch.Tensor, width: int, inner: int = 1) -> tuple[torch.Tensor, int]:
+    """``t`` (rows, ...) or (S, L, ...) with ``inner`` dimensions of ``width`` elements in all as
+    (tensor, row stride): read in place where its rows lie at one stride with contiguous
+    elements, else a contiguous copy."""
+    if t.is_contiguous():
+        return t, width
+    shape, stride = t.shape, t.stride()
+    if (stride[-1] == 1 or shape[-1] == 1) and (inner == 1 or stride[-2] == shape[-1] or shape[-2] == 1):
+        if len(shape) == 1 + inner:
+            ld = stride[0] if shape[0] > 1 else width
+        elif shape[1] == 1:
+            ld = stride[0] if shape[0] > 1 else width
+        elif shape[0] == 1 or stride[0] == shape[1] * stride[1]:
+            ld = stride[1]
         else:
             ld = 0
         if width <= ld < _ROW_MAX:
@@ -24,19 +28,19 @@ def rows_of(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
     return t.contiguous(), width
 
 
-def check_same(op: str, name: str, t: torch.Tensor, shape, dtypes, device) -> None:
-    if t.shape != shape or t.dtype not in dtypes or t.device != device:
+def check_same(op: str, name: str, t: torch.Tensor, shape, dtypes, dev: int) -> None:
+    """``dev``: the GPU's number (``Tensor.get_device``)."""
+    if t.shape != shape or t.dtype not in dtypes or t.get_device() != dev:
         want = " or ".join(str(d).replace("torch.", "") for d in dtypes)
-        raise ValueError(f"{op}: {name} must be {want} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} "
+        raise ValueError(f"{op}: {name} must be {want} {tuple(shape)} on cuda:{dev}, got {t.dtype} {tuple(t.shape)} "
                          f"on {t.device}")
 
 
 def param32(t: torch.Tensor | None) -> torch.Tensor | None:
     """A parameter as the kernels read it: contiguous fp32 (no copy where it is that already)."""
-    if t is None:
-        return None
-    t = t.detach()
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
 
 
 def batch(op: str, x: torch.Tensor, cu_seqlens) -> tuple[int, int, int]:
@@ -59,38 +63,33 @@ def batch(op: str, x: torch.Tensor, cu_seqlens) -> tuple[int, int, int]:
     return cu_seqlens.shape[0] - 1, x.shape[0], 0
 
 
-def set_pool(op: str, a, S: int, device, state, shape, dtype, slots, fresh) -> None:
+def set_pool(op: str, a, S: int, dev: int, state, shape, dtype, slots, fresh) -> None:
     """Checks the state pool (entries of ``shape``) and its index and fills the argument struct."""
     if state is None:
         if slots is not None or fresh is not None:
             raise ValueError(f"{op}: slots / fresh without a state")
         return
-    if (state.dim() != 1 + len(shape) or state.shape[1:] != shape or state.dtype != dtype or state.device != device
-            or not state.is_contiguous()):
+    if (state.shape[1:] != shape or state.dtype != dtype or state.get_device() != dev or not state.is_contiguous()):
         raise ValueError(f"{op}: the state must be contiguous {str(dtype)[6:]} (entries, "
-                         f"{', '.join(map(str, shape))}) on {device}, got {state.dtype} {tuple(state.shape)} on "
+                         f"{', '.join(map(str, shape))}) on cuda:{dev}, got {state.dtype} {tuple(state.shape)} on "
                          f"{state.device}")
-    if torch.is_grad_enabled() and state.requires_grad:
+    if state.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{op}: the state is updated in place and cannot require a gradient")
     n = state.shape[0]
-    if slots is None:
-        if n < S:
-            raise ValueError(f"{op}: {n} state entries for {S} sequences")
-    elif slots.shape != (S,) or slots.dtype != torch.int32 or slots.device != device or not slots.is_contiguous():
-        raise ValueError(f"{op}: slots must be contiguous int32 ({S},) on {device}, got {slots.dtype} "
-                         f"{tuple(slots.shape)} on {slots.device}")
-    else:
-        a.slots = slots.data_ptr()
-    if fresh is not None:
-        if fresh.shape != (S,) or fresh.dtype != torch.bool or fresh.device != device or not fresh.is_contiguous():
-            raise ValueError(f"{op}: fresh must be contiguous bool ({S},) on {device}, got {fresh.dtype} "
-                             f"{tuple(fresh.shape)} on {fresh.device}")
-        a.fresh = fresh.data_ptr()
     if n == 0:
         # Every slot is behind an empty pool; the library takes a pool of none as "no state".
         raise ValueError(f"{op}: the state has no entries")
+    if slots is None:
+        if n < S:
+            raise ValueError(f"{op}: {n} state entries for {S} sequences")
+    else:
+        if slots.shape != (S,) or slots.dtype != torch.int32 or slots.get_device() != dev or not slots.is_contiguous():
+            raise ValueError(f"{op}: slots must be contiguous int32 ({S},) on cuda:{dev}, got {slots.dtype} "
+                             f"{tuple(slots.shape)} on {slots.device}")
+        a.slots = slots.data_ptr()
+    if fresh is not None:
+        if fresh.shape != (S,) or fresh.dtype != torch.bool or fresh.get_device() != dev or not fresh.is_contiguous():
+            raise ValueError(f"{op}: fresh must be contiguous bool ({S},) on cuda:{dev}, got {fresh.dtype} "
+                             f"{tuple(fresh.shape)} on {fresh.device}")
+        a.fresh = fresh.data_ptr()
     a.n_slots, a.state = n, state.data_ptr()
-
-
-def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

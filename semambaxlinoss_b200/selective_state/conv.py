@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool, wants_grad
+from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool
 
 _ACTIVATIONS = {"silu": 1, None: 0}
 
@@ -20,7 +20,8 @@ _ACTIVATIONS = {"silu": 1, None: 0}
 def _weight(op, weight, C):
     """(C, K) of a weight (C, K) or (C, 1, K) (``nn.Conv1d``'s, groups = channels)."""
     w = weight.squeeze(1) if weight.dim() == 3 and weight.shape[1] == 1 else weight
-    if w.dim() != 2 or w.shape[0] != C or not 1 <= w.shape[1] <= 8:
+    shape = w.shape
+    if len(shape) != 2 or shape[0] != C or not 1 <= shape[1] <= 8:
         raise ValueError(f"{op}: weight must be ({C}, taps) or ({C}, 1, taps) with 1 to 8 taps, got "
                          f"{tuple(weight.shape)}")
     return w
@@ -44,7 +45,7 @@ class _ShortConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, silu, S, rows, L, cu):
         w, b = param32(weight), param32(bias)
-        a, xr = _args(x.detach(), w, b, silu, S, rows, L, cu)
+        a, xr = _args(x, w, b, silu, S, rows, L, cu)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         a.y = y.data_ptr()
         _lib.call("semx_short_conv_fwd", a, x.device)
@@ -97,23 +98,29 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     wanted (call it under ``torch.no_grad()``)."""
     op = "short_conv"
     S, rows, L = batch(op, x, cu_seqlens)
+    return _run(op, x, weight, bias, activation, S, rows, L, cu_seqlens, state, slots, fresh)
+
+
+def _run(op, x, weight, bias, activation, S, rows, L, cu_seqlens, state, slots, fresh):
     silu = _silu_flag(op, activation)
-    C = x.shape[-1]
+    C, dev = x.shape[-1], x.get_device()
     w = _weight(op, weight, C)
-    check_same(op, "weight", w, w.shape, TYPES, x.device)
+    if w.dtype not in TYPES or w.get_device() != dev:
+        check_same(op, "weight", w, w.shape, TYPES, dev)
     if bias is not None:
-        check_same(op, "bias", bias, (C,), TYPES, x.device)
-    if wants_grad(x, weight, bias):
+        check_same(op, "bias", bias, (C,), TYPES, dev)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)):
         if state is not None:
             raise ValueError(f"{op}: a state is for inference; the call wants gradients")
         if slots is not None or fresh is not None:
             raise ValueError(f"{op}: slots / fresh without a state")
         return _ShortConv.apply(x, w, bias, silu, S, rows, L, cu_seqlens)
-    w32, b32 = param32(w), param32(bias)
-    a, xr = _args(x.detach(), w32, b32, silu, S, rows, L, cu_seqlens)
-    if w.shape[1] > 1 or state is None:
-        set_pool(op, a, S, x.device, state, (w.shape[1] - 1, C), x.dtype, slots, fresh)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    w, bias = param32(w), param32(bias)
+    a, xr = _args(x, w, bias, silu, S, rows, L, cu_seqlens)
+    K = w.shape[1]
+    if K > 1 or state is None:  # one tap keeps nothing
+        set_pool(op, a, S, dev, state, (K - 1, C), x.dtype, slots, fresh)
+    y = x.new_empty(x.shape)
     a.y = y.data_ptr()
     _lib.call("semx_short_conv_fwd", a, x.device)
     return y
@@ -123,8 +130,12 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
                     activation: str | None = "silu", slots: torch.Tensor | None = None) -> torch.Tensor:
     """One token of every sequence: x (S, C) -> y (S, C); the windows in ``state`` (entries,
     K - 1, C) move on by one in place. Slots as in :func:`short_conv`."""
-    if x.dim() != 2:
-        raise ValueError(f"short_conv_step: x must be (sequences, channels), got {tuple(x.shape)}")
+    op = "short_conv_step"
+    if not x.is_cuda:
+        raise RuntimeError(f"{op} requires CUDA tensors.")
+    if x.dim() != 2 or x.dtype not in TYPES:
+        raise ValueError(f"{op}: x must be fp32 or bf16 (sequences, channels), got {x.dtype} {tuple(x.shape)}")
     if state is None:
-        raise ValueError("short_conv_step: a state is needed")
-    return short_conv(x.unsqueeze(1), weight, bias, activation, None, state, slots).squeeze(1)
+        raise ValueError(f"{op}: a state is needed")
+    S = x.shape[0]
+    return _run(op, x, weight, bias, activation, S, S, 1, None, state, slots, None)

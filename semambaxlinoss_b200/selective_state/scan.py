@@ -17,67 +17,76 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool, wants_grad
+from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool
 
 MAX_MODES = 128
+_F32 = (torch.float32,)
 
 
 def _check(op, x, dt, A, B, C, D, z, dt_bias):
     """Shapes and types; returns (channels, modes, groups)."""
-    ch, dev = x.shape[-1], x.device
-    if A.dim() != 2 or A.shape[0] != ch or not 1 <= A.shape[1] <= MAX_MODES:
-        raise ValueError(f"{op}: A must be ({ch}, modes) with 1 to {MAX_MODES} modes, got {tuple(A.shape)}")
-    N = A.shape[1]
-    check_same(op, "A", A, A.shape, TYPES, dev)
-    check_same(op, "dt", dt, x.shape, TYPES if x.dtype != torch.float32 else (torch.float32,), dev)
-    G = B.shape[-2] if B.dim() == x.dim() + 1 else 1
-    if G < 1 or ch % max(G, 1):
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    ch = shape[-1]
+    Ashape = A.shape
+    if len(Ashape) != 2 or Ashape[0] != ch or not 1 <= Ashape[1] <= MAX_MODES:
+        raise ValueError(f"{op}: A must be ({ch}, modes) with 1 to {MAX_MODES} modes, got {tuple(Ashape)}")
+    N = Ashape[1]
+    check_same(op, "A", A, Ashape, TYPES, dev)
+    check_same(op, "dt", dt, shape, _F32 if dtype == torch.float32 else TYPES, dev)
+    grouped = B.dim() == len(shape) + 1
+    G = B.shape[-2] if grouped else 1
+    if G < 1 or ch % G:
         raise ValueError(f"{op}: {ch} channels do not fall into {G} groups")
-    for name, t in (("B", B), ("C", C)):
-        check_same(op, name, t, x.shape[:-1] + ((G, N) if B.dim() == x.dim() + 1 else (N,)), (x.dtype,), dev)
+    own = (dtype,)
+    want = shape[:-1] + ((G, N) if grouped else (N,))
+    check_same(op, "B", B, want, own, dev)
+    check_same(op, "C", C, want, own, dev)
     if z is not None:
-        check_same(op, "z", z, x.shape, (x.dtype,), dev)
-    for name, t in (("D", D), ("dt_bias", dt_bias)):
-        if t is not None:
-            check_same(op, name, t, (ch,), TYPES, dev)
+        check_same(op, "z", z, shape, own, dev)
+    if D is not None:
+        check_same(op, "D", D, (ch,), TYPES, dev)
+    if dt_bias is not None:
+        check_same(op, "dt_bias", dt_bias, (ch,), TYPES, dev)
     return ch, N, G
 
 
+def _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
+    return torch.is_grad_enabled() and (
+        x.requires_grad or dt.requires_grad or A.requires_grad or B.requires_grad or C.requires_grad
+        or (D is not None and D.requires_grad) or (z is not None and z.requires_grad)
+        or (dt_bias is not None and dt_bias.requires_grad))
+
+
 def _args(x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu, N, G):
-    """The argument struct of detached operands, and what has to outlive the call."""
+    """The argument struct, and what has to outlive the call."""
     ch = x.shape[-1]
-    lead = x.shape[:-1]
-    xr, ldx = rows_of(x, ch)
-    dr, ldd = rows_of(dt, ch)
-    if B.dim() == x.dim() + 1:
-        # (groups, modes) of a row as one run of elements: a view wherever the storage has it.
-        B, C = (t.reshape(lead + (G * N,)) for t in (B, C))
-    Br, ldb = rows_of(B, G * N)
-    Cr, ldc = rows_of(C, G * N)
+    inner = B.dim() - x.dim() + 1  # (groups, modes) or (modes,)
+    x, ldx = rows_of(x, ch)
+    dt, ldd = rows_of(dt, ch)
+    B, ldb = rows_of(B, G * N, inner)
+    C, ldc = rows_of(C, G * N, inner)
     a = _lib.new_args(_lib.SemxStateScanArgs)
     a.softplus, a.bf16, a.dt_bf16 = softplus, x.dtype == torch.bfloat16, dt.dtype == torch.bfloat16
     a.S, a.rows, a.L, a.C, a.N, a.G = S, rows, L, ch, N, G
     a.ldx, a.lddt, a.ldb, a.ldc = ldx, ldd, ldb, ldc
-    a.x, a.dt, a.A, a.B, a.Cm = xr.data_ptr(), dr.data_ptr(), A.data_ptr(), Br.data_ptr(), Cr.data_ptr()
-    zr = None
+    a.x, a.dt, a.A, a.B, a.Cm = x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr()
     if z is not None:
-        zr, a.ldz = rows_of(z, ch)
-        a.z = zr.data_ptr()
+        z, a.ldz = rows_of(z, ch)
+        a.z = z.data_ptr()
     if D is not None:
         a.D = D.data_ptr()
     if dt_bias is not None:
         a.dt_bias = dt_bias.data_ptr()
     if cu is not None:
         a.cu_seqlens = cu.data_ptr()
-    return a, (xr, dr, Br, Cr, zr)
+    return a, (x, dt, B, C, z)
 
 
 class _StateScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu, N, G):
         A32, D32, b32 = param32(A), param32(D), param32(dt_bias)
-        a, kept = _args(x.detach(), dt.detach(), A32, B.detach(), C.detach(), D32, None if z is None else z.detach(),
-                        b32, softplus, S, rows, L, cu, N, G)
+        a, kept = _args(x, dt, A32, B, C, D32, z, b32, softplus, S, rows, L, cu, N, G)
         dev = x.device
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
         v = None if z is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
@@ -143,7 +152,7 @@ def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     S, rows, L = batch(op, x, cu_seqlens)
     ch, N, G = _check(op, x, dt, A, B, C, D, z, dt_bias)
     softplus = int(bool(dt_softplus))
-    if wants_grad(x, dt, A, B, C, D, z, dt_bias):
+    if _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
         if state is not None:
             raise ValueError(f"{op}: a state is for inference; the call wants gradients")
         if slots is not None or fresh is not None:
@@ -152,8 +161,8 @@ def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     A, D, dt_bias = param32(A), param32(D), param32(dt_bias)
     a, kept = _args(x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu_seqlens, N, G)
     dev = x.device
-    set_pool(op, a, S, dev, state, (ch, N), torch.float32, slots, fresh)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    set_pool(op, a, S, x.get_device(), state, (ch, N), torch.float32, slots, fresh)
+    y = x.new_empty(x.shape)
     a.y = y.data_ptr()
     nbytes = _lib.load().semx_state_scan_workspace_bytes(a, 0)
     ws = _lib.empty_f32(nbytes, dev) if nbytes else None
@@ -177,13 +186,13 @@ def selective_state_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     if state is None:
         raise ValueError(f"{op}: a state is needed")
     ch, N, G = _check(op, x, dt, A, B, C, D, z, dt_bias)
-    if wants_grad(x, dt, A, B, C, D, z, dt_bias):
+    if _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
         raise ValueError(f"{op}: a state is for inference; the call wants gradients")
     S = x.shape[0]
     A, D, dt_bias = param32(A), param32(D), param32(dt_bias)
     a, kept = _args(x, dt, A, B, C, D, z, dt_bias, int(bool(dt_softplus)), S, S, 1, None, N, G)
-    set_pool(op, a, S, x.device, state, (ch, N), torch.float32, slots, None)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    set_pool(op, a, S, x.get_device(), state, (ch, N), torch.float32, slots, None)
+    y = x.new_empty(x.shape)
     a.y = y.data_ptr()
     _lib.call("semx_state_step", a, x.device)
     return y
