@@ -9,11 +9,11 @@
 // that evaluate them: A is scaled by log2(e) once, d and d x are evaluated once per (step,
 // channel) and shared through shared memory.
 //
-// Split: a thread owns one channel and MPT modes of it, GL neighbouring lanes a channel; a
-// CTA of 128 threads owns 128 / GL channels of one piece of a sequence and walks over it in
-// tiles of kTT steps. The tile's operands are loaded into registers while the tile before is
+// Split: a thread owns one channel and 4 modes of it (two pairs, each in one register pair
+// for the two-wide multiply-adds), GL neighbouring lanes a channel; a CTA of 128 threads
+// owns 128 / GL channels of one piece of a sequence and walks over it in tiles of steps. The tile's operands are loaded into registers while the tile before is
 // computed, converted and put into shared memory; the sums over modes go back through
-// shared memory, so that the D skip, the gate and the stores run one (step, channel) per
+// shared memory, so that the step, the D skip, the gate and the stores run two channels per
 // thread with neighbouring channels in neighbouring threads.
 //
 // Long sequences that leave the GPU idle are cut into pieces. A first pass (LOCAL) runs each
@@ -29,67 +29,98 @@ namespace {
 
 using namespace semx_scan;
 
-constexpr int kTT = 16;  // steps per tile
+// Steps per tile: at most 1024 (step, channel) pairs and 2048 (step, mode) pairs.
+template <int GL>
+constexpr int tile_steps() {
+  return GL <= 4 ? 8 * GL : GL == 8 ? 32 : 16;
+}
 
-template <int MPT, int GL, bool LOCAL>
-__global__ void __launch_bounds__(kThreads) state_scan_fwd_kernel(const ScanParams p) {
-  constexpr int NP = MPT * GL, CH = kThreads / GL, TT = kTT;
-  constexpr int E = TT * CH / kThreads > 0 ? TT * CH / kThreads : 1;  // (step, channel) pairs per thread
-  constexpr int EB = (TT * NP + kThreads - 1) / kThreads;             // (step, mode) pairs per thread
-  constexpr int RS = GL < 4 ? GL : 4;  // lanes whose sums are exchanged step by step
-  __shared__ float2 sdt[TT][CH];       // (d, d x)
-  __shared__ float sys[LOCAL ? 1 : TT][LOCAL ? 1 : CH];
+template <int GL, bool LOCAL>
+__global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kernel(const ScanParams p) {
+  constexpr int NP = 4 * GL, CH = kThreads / GL, TT = tile_steps<GL>();
+  constexpr int TS = kThreads / (CH / 2);                  // rows that the CTA loads at a time
+  constexpr int E = (TT + TS - 1) / TS;                    // (step, channel pair)s of a thread
+  constexpr int EB = (TT * NP + kThreads - 1) / kThreads;  // (step, mode)s of a thread
+  constexpr int RS = GL < 4 ? GL : 4;                      // steps whose sums are exchanged together
+  constexpr int YS = CH + 8;                               // row of sys: the RS rows fall into other banks
+  __shared__ __align__(16) float4 sdt[TT][CH];             // (d, d, d x, d x)
+  __shared__ __align__(16) float sys[LOCAL ? 1 : TT][LOCAL ? 2 : YS];
   __shared__ __align__(16) float sB[TT][NP];
   __shared__ __align__(16) float sC[LOCAL ? 1 : TT][LOCAL ? 1 : NP];
 
   const int64_t j = blockIdx.x / p.ctiles;
   const int ct = blockIdx.x % p.ctiles;
-  const int grp = ct / p.tpg;                     // group of channels that share B and C
-  const int cg0 = (ct % p.tpg) * CH;              // first channel of the tile in the group
+  const int grp = ct / p.tpg;         // group of channels that share B and C
+  const int cg0 = (ct % p.tpg) * CH;  // first channel of the tile in the group
   const int c_base = grp * p.cpg;
   const Piece q = find_piece(p.m, j);
   const int64_t slot = LOCAL || !q.live ? semx::kNone : find_slot(p.m, q.s);
   const int tid = threadIdx.x;
 
-  // The pair of this thread in loads and stores: steps tid / CH + i kThreads / CH of channel ec.
-  const int ec = tid % CH, et = tid / CH;
-  const bool eok = cg0 + ec < p.cpg;
-  const int ech = c_base + min(cg0 + ec, p.cpg - 1);
+  // The channel pair of this thread in loads and stores; its steps are et, et + TS, ...
+  const int ec = tid % (CH / 2) * 2, et = tid / (CH / 2);
+  const bool eok = cg0 + ec < p.cpg, two = cg0 + ec + 1 < p.cpg;
+  const bool vec = p.vec2 != 0;
+  const int ech = c_base + min(cg0 + ec, p.cpg - 1), ech1 = two ? ech + 1 : ech;
   if (!LOCAL && eok && et == 0)
     for (int64_t r = rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) {
-      store(p.y, r * p.C + ech, p.bf16, 0.f);
-      if (p.v != nullptr) store(p.v, r * p.C + ech, p.bf16, 0.f);
+      store_pair(p.y, r * p.C + ech, p.bf16, vec, two, 0.f, 0.f);
+      if (p.v != nullptr) store_pair(p.v, r * p.C + ech, p.bf16, vec, two, 0.f, 0.f);
     }
   if (!q.live) return;
 
   // The channel and modes of this thread in the scan.
-  const int lane_m = tid % GL, sc = tid / GL;
+  const int lm = tid % GL, sc = tid / GL;
   const bool cok = cg0 + sc < p.cpg;
   const int ch = c_base + min(cg0 + sc, p.cpg - 1);
-  const int n0 = lane_m * MPT;
-  float A2[MPT], h[MPT];
+  const int n0 = lm * 4;
   const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[q.s] != 0);
+  f2 A2[2], h[2];
+  {
+    float a[4], s[4];
 #pragma unroll
-  for (int n = 0; n < MPT; ++n) {
-    const bool ok = n0 + n < p.N;
-    A2[n] = ok ? p.A[(int64_t)ch * p.N + n0 + n] * kLog2e : 0.f;
-    h[n] = 0.f;
-    if (!LOCAL && ok) {
-      if (p.entry != nullptr) h[n] = p.entry[(j * p.C + ch) * p.N + n0 + n];
-      else if (!cold) h[n] = p.state[(slot * p.C + ch) * p.N + n0 + n];
+    for (int n = 0; n < 4; ++n) {
+      const bool ok = n0 + n < p.N;
+      a[n] = ok ? p.A[(int64_t)ch * p.N + n0 + n] * kLog2e : 0.f;
+      s[n] = 0.f;
+      if (!LOCAL && ok) {
+        if (p.entry != nullptr) s[n] = p.entry[(j * p.C + ch) * p.N + n0 + n];
+        else if (!cold) s[n] = p.state[(slot * p.C + ch) * p.N + n0 + n];
+      }
     }
+    A2[0] = pack2(a[0], a[1]); A2[1] = pack2(a[2], a[3]);
+    h[0] = pack2(s[0], s[1]); h[1] = pack2(s[2], s[3]);
   }
-  const float bias = p.dt_bias != nullptr ? p.dt_bias[ech] : 0.f;
-  const float Dc = LOCAL ? 0.f : (slot == semx::kRefused ? __int_as_float(0x7fffffff) : (p.D != nullptr ? p.D[ech] : 0.f));
-  float dsum = 0.f;
+  const f2 pole_bias = pack2(kPoleBias, kPoleBias);
+  const float bias0 = p.dt_bias != nullptr ? p.dt_bias[ech] : 0.f, bias1 = p.dt_bias != nullptr ? p.dt_bias[ech1] : 0.f;
+  float D0 = 0.f, D1 = 0.f;
+  if (!LOCAL) {
+    if (p.D != nullptr) { D0 = p.D[ech]; D1 = p.D[ech1]; }
+    if (slot == semx::kRefused) D0 = D1 = __int_as_float(0x7fffffff);
+  }
+  float dsum0 = 0.f, dsum1 = 0.f;
+  // States that a training forward keeps: of step 0 of the piece on, every kBlock steps.
+  float* ck = nullptr;
+  if (!LOCAL && p.ckpt != nullptr && cok)
+    ck = p.ckpt + ((piece_base(p.m, q.s, kBlock) + q.t0 / kBlock) * p.C + ch) * p.N + n0;
+  const int64_t ck_step = (int64_t)p.C * p.N;
+  const bool ck_vec = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.ckpt) & 15) == 0;
 
-  uint32_t rx[E], rd[E], rz[E], rB[EB], rC[EB];
+  uint2 rx[E], rd[E], rz[E];
+  uint32_t rB[EB], rC[EB];
   auto fetch = [&](int t0) {
     const int64_t row = q.row0 + t0 + et;
-    fetch_pairs<E, kThreads / CH>(rx, p.x, p.bf16, row * p.ldx + ech, (kThreads / CH) * p.ldx, t0 + et, q.t1, eok && et < TT);
-    fetch_pairs<E, kThreads / CH>(rd, p.dt, p.dt_bf16, row * p.lddt + ech, (kThreads / CH) * p.lddt, t0 + et, q.t1, eok && et < TT);
-    if (!LOCAL && p.z != nullptr)
-      fetch_pairs<E, kThreads / CH>(rz, p.z, p.bf16, row * p.ldz + ech, (kThreads / CH) * p.ldz, t0 + et, q.t1, eok && et < TT);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const bool ok = eok && et + i * TS < TT && t0 + et + i * TS < q.t1;
+      const int64_t r = row + i * TS;
+      rx[i] = rd[i] = rz[i] = make_uint2(0u, 0u);
+      if (ok) {
+        rx[i] = load_pair(p.x, r * p.ldx + ech, p.bf16, vec, two);
+        rd[i] = load_pair(p.dt, r * p.lddt + ech, p.dt_bf16, vec, two);
+        if (!LOCAL && p.z != nullptr) rz[i] = load_pair(p.z, r * p.ldz + ech, p.bf16, vec, two);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < EB; ++i) {
       const int e = tid + i * kThreads, t = e / NP, n = e % NP;
@@ -99,21 +130,30 @@ __global__ void __launch_bounds__(kThreads) state_scan_fwd_kernel(const ScanPara
       if (!LOCAL) rC[i] = ok ? load_raw(p.Cm, r * p.ldc + (int64_t)grp * p.N + n, p.bf16) : 0u;
     }
   };
-  fetch(q.t0);
+  if (q.t0 < q.t1) fetch(q.t0);
   for (int t0 = q.t0; t0 < q.t1; t0 += TT) {
-    float xv[E], zv[E];
+    float2 xv[E], zv[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int t = et + i * (kThreads / CH);
+      const int t = et + i * TS;
       if (t < TT) {
-        const float x = as_float(rx[i], p.bf16);
-        float d = as_float(rd[i], p.dt_bf16) + bias;
-        if (p.softplus) d = softplus(d);
-        if (!(t0 + t < q.t1 && eok)) d = 0.f;  // a row behind the piece: pole 1, no drive
-        sdt[t][ec] = make_float2(d, d * x);
+        const float2 x = pair_floats(rx[i], p.bf16);
+        float2 d = pair_floats(rd[i], p.dt_bf16);
+        d.x += bias0;
+        d.y += bias1;
+        if (p.softplus) {
+          d.x = softplus(d.x);
+          d.y = softplus(d.y);
+        }
+        if (t0 + t >= q.t1) d.x = d.y = 0.f;  // a row behind the piece: pole 1, no drive
+        sdt[t][ec] = make_float4(d.x, d.x, d.x * x.x, d.x * x.x);
+        sdt[t][ec + 1] = make_float4(d.y, d.y, d.y * x.y, d.y * x.y);
         xv[i] = x;
-        zv[i] = !LOCAL && p.z != nullptr ? as_float(rz[i], p.bf16) : 0.f;
-        if (LOCAL) dsum += d;
+        if (!LOCAL && p.z != nullptr) zv[i] = pair_floats(rz[i], p.bf16);
+        if (LOCAL) {
+          dsum0 += d.x;
+          dsum1 += d.y;
+        }
       }
     }
 #pragma unroll
@@ -127,66 +167,88 @@ __global__ void __launch_bounds__(kThreads) state_scan_fwd_kernel(const ScanPara
     __syncthreads();
     if (t0 + TT < q.t1) fetch(t0 + TT);
 
-#pragma unroll
-    for (int tb = 0; tb < TT; tb += RS) {
-      float acc[RS];
-#pragma unroll
-      for (int u = 0; u < RS; ++u) {
-        const int t = tb + u;
-        if (!LOCAL && p.ckpt != nullptr && t % kBlock == 0 && t0 + t < q.t1 && cok) {
-          float* o = p.ckpt + ((piece_base(p.m, q.s, kBlock) + (t0 + t) / kBlock) * p.C + ch) * p.N + n0;
-#pragma unroll
-          for (int n = 0; n < MPT; ++n)
-            if (n0 + n < p.N) o[n] = h[n];
+    const int nt = min(TT, q.t1 - t0);
+#pragma unroll 1
+    for (int tb = 0; tb < nt; tb += 4) {
+      if (!LOCAL && ck != nullptr && (tb & (kBlock - 1)) == 0) {
+        const float2 a = unpack2(h[0]), b = unpack2(h[1]);
+        if (ck_vec) {
+          if (n0 < p.N) *reinterpret_cast<float4*>(ck) = make_float4(a.x, a.y, b.x, b.y);
+        } else {
+          if (n0 < p.N) ck[0] = a.x;
+          if (n0 + 1 < p.N) ck[1] = a.y;
+          if (n0 + 2 < p.N) ck[2] = b.x;
+          if (n0 + 3 < p.N) ck[3] = b.y;
         }
-        const float2 d = sdt[t][sc];
-        acc[u] = 0.f;
+        ck += ck_step;
+      }
+      float acc[4];
 #pragma unroll
-        for (int n = 0; n < MPT; ++n) {
-          const float a = semx::ex2_approx(d.x * A2[n]);
-          h[n] = fmaf(a, h[n], d.y * sB[t][n0 + n]);
-          if (!LOCAL) acc[u] = fmaf(h[n], sC[t][n0 + n], acc[u]);
+      for (int u = 0; u < 4; ++u) {
+        const int t = tb + u;
+        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(&sdt[t][sc]);
+        const ulonglong2 Bn = *reinterpret_cast<const ulonglong2*>(&sB[t][n0]);
+        h[0] = fma2(poles2(d.x, A2[0], pole_bias), h[0], mul2(d.y, Bn.x));
+        h[1] = fma2(poles2(d.x, A2[1], pole_bias), h[1], mul2(d.y, Bn.y));
+        if (!LOCAL) {
+          const ulonglong2 Cn = *reinterpret_cast<const ulonglong2*>(&sC[t][n0]);
+          const float2 v = unpack2(fma2(h[1], Cn.y, mul2(h[0], Cn.x)));
+          acc[u] = v.x + v.y;
         }
       }
       if (!LOCAL) {
-        // Lane m (mod RS) of a channel's lanes ends with the sum of step tb + m.
-        const float s = lanes_scatter_sum<GL>(acc, lane_m);
-        if (lane_m < RS) sys[tb + lane_m][sc] = s;
+        // Lane m (mod RS) of a channel's lanes ends with the sums of steps m, m + RS, ...
+#pragma unroll
+        for (int u = 0; u < 4; u += RS) {
+          float part[RS];
+#pragma unroll
+          for (int k = 0; k < RS; ++k) part[k] = acc[u + k];
+          const float s = lanes_scatter_sum<GL, RS>(part, lm);
+          if (lm < RS) sys[tb + u + lm][sc] = s;
+        }
       }
     }
     __syncthreads();
     if (!LOCAL) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int t = et + i * (kThreads / CH);
+        const int t = et + i * TS;
         if (t < TT && t0 + t < q.t1 && eok) {
           const int64_t o = (q.row0 + t0 + t) * p.C + ech;
-          float v = fmaf(Dc, xv[i], sys[t][ec]);
-          if (p.v != nullptr) store(p.v, o, p.bf16, v);
-          if (p.z != nullptr) v *= zv[i] * sigmoid(zv[i]);
-          store(p.y, o, p.bf16, v);
+          const float2 s = *reinterpret_cast<const float2*>(&sys[t][ec]);
+          float v0 = fmaf(D0, xv[i].x, s.x), v1 = fmaf(D1, xv[i].y, s.y);
+          if (p.v != nullptr) store_pair(p.v, o, p.bf16, vec, two, v0, v1);
+          if (p.z != nullptr) {
+            v0 *= zv[i].x * sigmoid(zv[i].x);
+            v1 *= zv[i].y * sigmoid(zv[i].y);
+          }
+          store_pair(p.y, o, p.bf16, vec, two, v0, v1);
         }
       }
     }
   }
+  const float2 ha = unpack2(h[0]), hb = unpack2(h[1]);
+  const float last[4] = {ha.x, ha.y, hb.x, hb.y};
   if (LOCAL) {
     if (cok)
 #pragma unroll
-      for (int n = 0; n < MPT; ++n)
-        if (n0 + n < p.N) p.entry[(j * p.C + ch) * p.N + n0 + n] = h[n];
+      for (int n = 0; n < 4; ++n)
+        if (n0 + n < p.N) p.entry[(j * p.C + ch) * p.N + n0 + n] = last[n];
     // Sum of the steps: the threads of a channel in order.
     float* red = reinterpret_cast<float*>(&sdt[0][0]);
-    red[tid] = dsum;
     __syncthreads();
-    if (tid < CH && eok) {
+    red[et * CH + ec] = dsum0;
+    red[et * CH + ec + 1] = dsum1;
+    __syncthreads();
+    if (tid < CH && cg0 + tid < p.cpg) {
       float s = 0.f;
-      for (int i = 0; i < kThreads / CH; ++i) s += red[i * CH + tid];
-      p.dsum[j * p.C + ech] = s;
+      for (int i = 0; i < TS; ++i) s += red[i * CH + tid];
+      p.dsum[j * p.C + c_base + cg0 + tid] = s;
     }
   } else if (p.entry == nullptr && slot >= 0 && cok) {
 #pragma unroll
-    for (int n = 0; n < MPT; ++n)
-      if (n0 + n < p.N) p.state[(slot * p.C + ch) * p.N + n0 + n] = h[n];
+    for (int n = 0; n < 4; ++n)
+      if (n0 + n < p.N) p.state[(slot * p.C + ch) * p.N + n0 + n] = last[n];
   }
 }
 
@@ -216,27 +278,26 @@ __global__ void __launch_bounds__(kThreads) state_scan_join_kernel(const ScanPar
 }
 
 template <bool LOCAL>
-int launch_fwd(ScanParams& p, int mpt, cudaStream_t st) {
-  const int gl = lanes_for(p.N, mpt);
-  const int64_t ch = kThreads / gl;
-  p.tpg = (int)semx::cdiv(p.cpg, ch);
+int launch_fwd(ScanParams& p, cudaStream_t st) {
+  const int gl = lanes_for(p.N, 4);
+  p.tpg = (int)semx::cdiv(p.cpg, (int64_t)(kThreads / gl));
   p.ctiles = p.G * p.tpg;
   const int64_t grid = p.m.pieces * p.ctiles;
   if (grid == 0) return SEMX_OK;
   if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan: too many pieces");
-#define SEMX_GL(M, GV)                                                                            \
-  if (mpt == M && gl == GV) {                                                                     \
-    state_scan_fwd_kernel<M, GV, LOCAL><<<(unsigned)grid, kThreads, 0, st>>>(p);                  \
-    return semx::check_launch("state_scan_fwd_kernel");                                           \
-  }
-  SEMX_GL(16, 1)
-  SEMX_GL(4, 1)
-  SEMX_GL(4, 2)
-  SEMX_GL(4, 4)
-  SEMX_GL(4, 8)
-  SEMX_GL(4, 16)
-  SEMX_GL(4, 32)
+  switch (gl) {
+#define SEMX_GL(GV)                                                                     \
+  case GV:                                                                              \
+    state_scan_fwd_kernel<GV, LOCAL><<<(unsigned)grid, kThreads, 0, st>>>(p);           \
+    return semx::check_launch("state_scan_fwd_kernel");
+    SEMX_GL(1)
+    SEMX_GL(2)
+    SEMX_GL(4)
+    SEMX_GL(8)
+    SEMX_GL(16)
+    SEMX_GL(32)
 #undef SEMX_GL
+  }
   return semx::fail(SEMX_ERR_UNSUPPORTED, "state_scan: %d modes", p.N);
 }
 
@@ -273,6 +334,11 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
   p->x = a->x; p->dt = a->dt; p->A = a->A; p->B = a->B; p->Cm = a->Cm; p->D = a->D; p->z = a->z;
   p->dt_bias = a->dt_bias; p->y = a->y; p->state = a->state; p->v = a->v; p->ckpt = a->ckpt;
   p->dy = a->dy; p->dx = a->dx; p->ddt = a->ddt; p->dz = a->dz;
+  const uintptr_t align = a->bf16 ? 4 : 8;
+  p->vec2 = p->cpg % 2 == 0 && a->ldx % 2 == 0 && a->lddt % 2 == 0 && (a->z == nullptr || a->ldz % 2 == 0) &&
+            semx::aligned(a->dt, a->dt_bf16 ? 4 : 8) && semx::aligned(a->ddt, a->dt_bf16 ? 4 : 8);
+  for (const void* t : {a->x, a->z, (const void*)a->y, (const void*)a->v, a->dy, (const void*)a->dx, (const void*)a->dz})
+    if (!semx::aligned(t, align)) p->vec2 = 0;
   return SEMX_OK;
 }
 
@@ -280,23 +346,14 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
 
 namespace {
 
-// How a forward is run: modes per thread, and rows per piece (0: whole sequences).
-struct Plan {
-  int mpt;
-  int64_t Q;
-};
-Plan fwd_plan(const ScanParams& p) {
-  const int64_t work = (int64_t)p.m.S * p.C;
-  Plan plan = {4, 0};
-  if (p.N <= 16 && p.N > 4 && work >= 148 * 256) plan.mpt = 16;
-  const int64_t warps = work * lanes_for(p.N, plan.mpt) / 32;
+// Rows per piece of a forward (0: whole sequences).
+int64_t fwd_rows_per_piece(const ScanParams& p) {
+  const int64_t warps = (int64_t)p.m.S * p.C * lanes_for(p.N, 4) / 32;
   const int64_t rows = p.m.S > 0 ? p.m.T / p.m.S : 0;
-  if (warps < 148 * 8 && rows > 64) {
-    const int64_t cut = semx::cdiv((int64_t)148 * 16, warps > 0 ? warps : 1);
-    int64_t Q = semx::cdiv(semx::cdiv(p.m.T, p.m.S * cut), 16) * 16;
-    plan.Q = Q < 32 ? 32 : Q;
-  }
-  return plan;
+  if (warps >= 148 * 8 || rows <= 64) return 0;
+  const int64_t cut = semx::cdiv((int64_t)148 * 16, warps > 0 ? warps : 1);
+  const int64_t Q = semx::cdiv(semx::cdiv(p.m.T, p.m.S * cut), 32) * 32;
+  return Q < 32 ? 32 : Q;
 }
 
 size_t split_floats(const ScanParams& p) { return (size_t)p.m.pieces * p.C * (p.N + 1); }
@@ -322,14 +379,14 @@ int semx_state_scan_fwd(const SemxStateScanArgs* a, semx_stream_t stream) {
   rc = scope.bind({a->y, a->state});
   if (rc != SEMX_OK) return rc;
   cudaStream_t st = semx::as_stream(stream);
-  const Plan plan = fwd_plan(p);
-  semx::set_pieces(&p.m, plan.Q);
+  const int64_t Q = fwd_rows_per_piece(p);
+  semx::set_pieces(&p.m, Q);
   if (p.m.S == 0 && p.m.T > 0) p.m.pieces = 1;  // nothing but rows behind the last sequence
-  if (plan.Q > 0 && p.m.S > 0) {
+  if (Q > 0 && p.m.S > 0) {
     SEMX_REQUIRE(a->workspace != nullptr, SEMX_ERR_WORKSPACE, "state_scan: workspace is NULL");
     p.entry = reinterpret_cast<float*>(a->workspace);
     p.dsum = p.entry + (size_t)p.m.pieces * p.C * p.N;
-    rc = launch_fwd<true>(p, plan.mpt, st);
+    rc = launch_fwd<true>(p, st);
     if (rc != SEMX_OK) return rc;
     const int64_t grid = p.m.S * semx::cdiv((int64_t)p.C * p.N, kThreads);
     if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan: too many sequences");
@@ -337,7 +394,7 @@ int semx_state_scan_fwd(const SemxStateScanArgs* a, semx_stream_t stream) {
     rc = semx::check_launch("state_scan_join_kernel");
     if (rc != SEMX_OK) return rc;
   }
-  return launch_fwd<false>(p, plan.mpt, st);
+  return launch_fwd<false>(p, st);
 }
 
 size_t semx_state_scan_workspace_bytes(const SemxStateScanArgs* a, int32_t backward) {
@@ -353,9 +410,9 @@ size_t semx_state_scan_workspace_bytes(const SemxStateScanArgs* a, int32_t backw
   ScanParams p = {};
   if (scan_validate(&b, backward != 0, &p) != SEMX_OK) return 0;
   if (backward != 0) return scan_bwd_workspace(p);
-  const Plan plan = fwd_plan(p);
-  semx::set_pieces(&p.m, plan.Q);
-  return plan.Q > 0 ? split_floats(p) * sizeof(float) : 0;
+  const int64_t Q = fwd_rows_per_piece(p);
+  semx::set_pieces(&p.m, Q);
+  return Q > 0 ? split_floats(p) * sizeof(float) : 0;
 }
 
 }  // extern "C"

@@ -27,6 +27,7 @@ struct ScanParams {
   int C, N, G, cpg;      // channels, modes, groups, channels per group
   int ctiles, tpg;       // channel tiles, and tiles per group
   int bf16, dt_bf16, softplus;
+  int vec2;              // every row operand allows accesses of two neighbouring channels
   int64_t ldx, lddt, ldz, ldb, ldc;
   const void* x;
   const void* dt;
@@ -63,23 +64,105 @@ __device__ __forceinline__ void store(void* base, int64_t i, int bf16, float v) 
   else reinterpret_cast<float*>(base)[i] = v;
 }
 
-// E elements at i, i + stride, ... of steps t, t + TS, ... (0 from step t1 on).
-template <int E, int TS>
-__device__ __forceinline__ void fetch_pairs(uint32_t (&r)[E], const void* base, int bf16, int64_t i, int64_t stride,
-                                            int t, int t1, bool ok) {
+// Two neighbouring channels of a row as they are stored (bf16: x alone).
+__device__ __forceinline__ uint2 load_pair(const void* base, int64_t i, int bf16, bool vec, bool two) {
+  uint2 r = make_uint2(0u, 0u);
   if (bf16) {
-    const unsigned short* b = reinterpret_cast<const unsigned short*>(base);
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = ok && t + e * TS < t1 ? b[i + e * stride] : 0u;
+    const unsigned short* b = reinterpret_cast<const unsigned short*>(base) + i;
+    if (vec) r.x = *reinterpret_cast<const uint32_t*>(b);
+    else r.x = (uint32_t)b[0] | (two ? (uint32_t)b[1] << 16 : 0u);
   } else {
-    const uint32_t* b = reinterpret_cast<const uint32_t*>(base);
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = ok && t + e * TS < t1 ? b[i + e * stride] : 0u;
+    const uint32_t* b = reinterpret_cast<const uint32_t*>(base) + i;
+    if (vec) r = *reinterpret_cast<const uint2*>(b);
+    else r = make_uint2(b[0], two ? b[1] : 0u);
+  }
+  return r;
+}
+__device__ __forceinline__ float2 pair_floats(uint2 r, int bf16) {
+  return bf16 ? make_float2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u))
+              : make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ void store_pair(void* base, int64_t i, int bf16, bool vec, bool two, float a, float b) {
+  if (bf16) {
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + i;
+    if (vec) {
+      *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(a, b);
+    } else {
+      o[0] = __float2bfloat16(a);
+      if (two) o[1] = __float2bfloat16(b);
+    }
+  } else {
+    float* o = reinterpret_cast<float*>(base) + i;
+    if (vec) {
+      *reinterpret_cast<float2*>(o) = make_float2(a, b);
+    } else {
+      o[0] = a;
+      if (two) o[1] = b;
+    }
   }
 }
 
+// Pairs of fp32 values in one register pair: one instruction works on both.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Poles exp(d A) of two modes from d (in both halves) and A log2(e). The special-function
+// exponential of small negative arguments is measured 2e-8 low on average (rms 3.5e-8); a
+// state multiplies hundreds of poles, so that average is what reaches the results. kPoleBias
+// moves the argument by as much, inside the multiply-add that forms it.
+constexpr float kPoleBias = 3.0e-8f;
+__device__ __forceinline__ f2 poles2(f2 dd, f2 A2, f2 bias) {
+  const float2 v = unpack2(fma2(dd, A2, bias));
+  return pack2(semx::ex2_approx(v.x), semx::ex2_approx(v.y));
+}
+
 __device__ __forceinline__ float sigmoid(float v) { return semx::rcp_approx(1.f + semx::ex2_approx(-kLog2e * v)); }
-__device__ __forceinline__ float softplus(float v) { return semx::softplus(v); }
+
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|): log1p(e) / e on [0, 1] is a degree 9
+// Chebyshev interpolant (5e-9 off, 1e-7 with its roundings); e is corrected for the rounding
+// of its argument, which small steps (v near -7) would show in full. Above 20 the
+// logarithm is below half a step of v.
+__device__ __forceinline__ float softplus(float v) {
+  const float t = -fabsf(v), p = t * kLog2e;
+  const float lost = fmaf(t, kLog2e, -p) + t * 1.925963033500e-8f;  // log2(e) - float(log2(e))
+  float e = semx::ex2_approx(p);
+  e = fmaf(e, lost * 0.6931471805599453f, e);
+  float s = -0.0031760570127512695f;
+  s = fmaf(s, e, 0.019542528316378593f);
+  s = fmaf(s, e, -0.05637361481785774f);
+  s = fmaf(s, e, 0.10543623566627502f);
+  s = fmaf(s, e, -0.1526966691017151f);
+  s = fmaf(s, e, 0.1966327428817749f);
+  s = fmaf(s, e, -0.24951615929603577f);
+  s = fmaf(s, e, 0.33329710364341736f);
+  s = fmaf(s, e, -0.49999892711639404f);
+  s = fmaf(s, e, 1.0f);
+  return fmaf(s, e, fmaxf(v, 0.f));
+}
 
 // Lanes per channel for N modes, MPT per thread.
 inline int lanes_for(int N, int mpt) {
@@ -88,10 +171,10 @@ inline int lanes_for(int N, int mpt) {
   return g;
 }
 
-// v[u] summed over the GL neighbouring lanes; lane m (mod R, R = 1, 2 or 4 values) returns
-// the total of v[m mod R].
+// v summed over GL neighbouring lanes step by step: of the R = min(GL, 4) values, lane m
+// returns the total of v[m mod R].
 template <int GL, int R>
-__device__ __forceinline__ float lanes_scatter_sum(float (&v)[R], int lane) {
+__device__ __forceinline__ float lanes_scatter_sum(const float (&v)[R], int lane) {
   float s;
   if constexpr (R == 1) {
     s = v[0];

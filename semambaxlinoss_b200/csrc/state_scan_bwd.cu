@@ -33,6 +33,21 @@ using namespace semx_scan;
 constexpr int kWarps = kThreads / 32;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// E elements at i, i + stride, ... of steps t, t + TS, ... (0 from step t1 on).
+template <int E, int TS>
+__device__ __forceinline__ void fetch_pairs(uint32_t (&r)[E], const void* base, int bf16, int64_t i, int64_t stride,
+                                            int t, int t1, bool ok) {
+  if (bf16) {
+    const unsigned short* b = reinterpret_cast<const unsigned short*>(base);
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = ok && t + e * TS < t1 ? b[i + e * stride] : 0u;
+  } else {
+    const uint32_t* b = reinterpret_cast<const uint32_t*>(base);
+#pragma unroll
+    for (int e = 0; e < E; ++e) r[e] = ok && t + e * TS < t1 ? b[i + e * stride] : 0u;
+  }
+}
+
 template <int GM>
 constexpr int channels_per_thread() {
   return GM == 1 ? 1 : 2;
