@@ -9,12 +9,12 @@
 // that evaluate them: A is scaled by log2(e) once, d and d x are evaluated once per (step,
 // channel) and shared through shared memory.
 //
-// Split: a thread owns one channel and 4 modes of it (two pairs, each in one register pair
+// Split: a thread owns two channels and 4 modes of each (two pairs, each in one register pair
 // for the two-wide multiply-adds), GL neighbouring lanes a channel; a CTA of 128 threads
-// owns 128 / GL channels of one piece of a sequence and walks over it in tiles of steps. The tile's operands are loaded into registers while the tile before is
+// owns 256 / GL channels of one piece of a sequence and walks over it in tiles of steps. The tile's operands are loaded into registers while the tile before is
 // computed, converted and put into shared memory; the sums over modes go back through
-// shared memory, so that the step, the D skip, the gate and the stores run two channels per
-// thread with neighbouring channels in neighbouring threads.
+// shared memory, so that the step, the D skip, the gate and the stores run four neighbouring
+// channels per thread.
 //
 // Long sequences that leave the GPU idle are cut into pieces. A first pass (LOCAL) runs each
 // piece from zero and keeps its last state and the sum of its steps d; since all of a
@@ -29,24 +29,34 @@ namespace {
 
 using namespace semx_scan;
 
-// Steps per tile: at most 1024 (step, channel) pairs and 2048 (step, mode) pairs.
+// Channels per thread: the values of B and C that a thread reads from shared memory serve
+// both of them (with one channel per thread shared memory was the bound, at 3 to 4 cycles a
+// load: 153 us where two take less for a prompt of 8191 x 2048).
+constexpr int kCPT = 2;
+
+template <int GL>
+constexpr int channels_per_cta() {
+  return kThreads / GL * kCPT;
+}
 template <int GL>
 constexpr int tile_steps() {
-  return GL <= 4 ? 8 * GL : GL == 8 ? 32 : 16;
+  return GL >= 4 ? 16 : 8;
 }
 
-template <int GL, bool LOCAL>
+template <int GL, bool LOCAL, int ACC>
 __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kernel(const ScanParams p) {
-  constexpr int NP = 4 * GL, CH = kThreads / GL, TT = tile_steps<GL>();
-  constexpr int TS = kThreads / (CH / 2);                  // rows that the CTA loads at a time
-  constexpr int E = (TT + TS - 1) / TS;                    // (step, channel pair)s of a thread
-  constexpr int EB = (TT * NP + kThreads - 1) / kThreads;  // (step, mode)s of a thread
+  constexpr int CH = channels_per_cta<GL>(), TT = tile_steps<GL>();
+  constexpr int TS = kThreads / (CH / 4);                  // rows that the CTA loads at a time
+  constexpr int E = (TT + TS - 1) / TS;                    // (step, four channels) of a thread
+  constexpr int ML = kThreads / GL;                        // rows of B and C loaded at a time
+  constexpr int EB = (TT + ML - 1) / ML;                   // (step, four modes) of a thread
   constexpr int RS = GL < 4 ? GL : 4;                      // steps whose sums are exchanged together
-  constexpr int YS = CH + 8;                               // row of sys: the RS rows fall into other banks
-  __shared__ __align__(16) float4 sdt[TT][CH];             // (d, d, d x, d x)
-  __shared__ __align__(16) float sys[LOCAL ? 1 : TT][LOCAL ? 2 : YS];
-  __shared__ __align__(16) float sB[TT][NP];
-  __shared__ __align__(16) float sC[LOCAL ? 1 : TT][LOCAL ? 1 : NP];
+  constexpr int YS = CH + 8;                               // row of sys: RS rows fall into other banks
+  typedef typename RawQuad<ACC>::type Quad;
+  __shared__ __align__(16) float4 sdt[TT][CH / 2];         // (d, d', d x, d' x') of two channels
+  __shared__ __align__(16) float sys[LOCAL ? 1 : TT][LOCAL ? 4 : YS];
+  __shared__ __align__(16) float4 sB[TT][GL];
+  __shared__ __align__(16) float4 sC[LOCAL ? 1 : TT][LOCAL ? 1 : GL];
 
   const int64_t j = blockIdx.x / p.ctiles;
   const int ct = blockIdx.x % p.ctiles;
@@ -57,154 +67,162 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   const int64_t slot = LOCAL || !q.live ? semx::kNone : find_slot(p.m, q.s);
   const int tid = threadIdx.x;
 
-  // The channel pair of this thread in loads and stores; its steps are et, et + TS, ...
-  const int ec = tid % (CH / 2) * 2, et = tid / (CH / 2);
-  const bool eok = cg0 + ec < p.cpg, two = cg0 + ec + 1 < p.cpg;
-  const bool vec = p.vec2 != 0;
-  const int ech = c_base + min(cg0 + ec, p.cpg - 1), ech1 = two ? ech + 1 : ech;
-  if (!LOCAL && eok && et == 0)
+  // The four channels of this thread in loads and stores (en of them exist); its steps are
+  // et, et + TS, ...
+  const int ec = tid % (CH / 4) * 4, et = tid / (CH / 4);
+  const int en = min(4, p.cpg - cg0 - ec);
+  const int64_t ech = c_base + (en > 0 ? cg0 + ec : 0);
+  const bool has_z = !LOCAL && p.z != nullptr;
+  if (!LOCAL && en > 0 && et == 0)
     for (int64_t r = rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) {
-      store_pair(p.y, r * p.C + ech, p.bf16, vec, two, 0.f, 0.f);
-      if (p.v != nullptr) store_pair(p.v, r * p.C + ech, p.bf16, vec, two, 0.f, 0.f);
+      store_quad<ACC>(p.y, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (p.v != nullptr) store_quad<ACC>(p.v, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
     }
   if (!q.live) return;
 
-  // The channel and modes of this thread in the scan.
-  const int lm = tid % GL, sc = tid / GL;
-  const bool cok = cg0 + sc < p.cpg;
-  const int ch = c_base + min(cg0 + sc, p.cpg - 1);
+  // The channels and modes of this thread in the scan.
+  const int lm = tid % GL, cp = tid / GL, sc = cp * kCPT;
   const int n0 = lm * 4;
   const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[q.s] != 0);
-  f2 A2[2], h[2];
-  {
-    float a[4], s[4];
+  int nn[kCPT];          // modes of the channel that this thread holds
+  int64_t at[kCPT];      // (channel, first mode) of an array (C, N)
+  float A2[kCPT][4];
+  f2 h[kCPT][2];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const bool ok = n0 + n < p.N;
-      a[n] = ok ? p.A[(int64_t)ch * p.N + n0 + n] * kLog2e : 0.f;
-      s[n] = 0.f;
-      if (!LOCAL && ok) {
-        if (p.entry != nullptr) s[n] = p.entry[(j * p.C + ch) * p.N + n0 + n];
-        else if (!cold) s[n] = p.state[(slot * p.C + ch) * p.N + n0 + n];
-      }
+  for (int i = 0; i < kCPT; ++i) {
+    const bool ok = cg0 + sc + i < p.cpg;
+    nn[i] = ok ? min(4, p.N - n0) : 0;
+    at[i] = (int64_t)(c_base + (ok ? cg0 + sc + i : 0)) * p.N + n0;
+    const float4 a = load_params(p.A, at[i], nn[i]);
+    A2[i][0] = a.x * kLog2e; A2[i][1] = a.y * kLog2e; A2[i][2] = a.z * kLog2e; A2[i][3] = a.w * kLog2e;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!LOCAL) {
+      if (p.entry != nullptr) s = load_params(p.entry, j * p.C * p.N + at[i], nn[i]);
+      else if (!cold) s = load_params(p.state, slot * p.C * p.N + at[i], nn[i]);
     }
-    A2[0] = pack2(a[0], a[1]); A2[1] = pack2(a[2], a[3]);
-    h[0] = pack2(s[0], s[1]); h[1] = pack2(s[2], s[3]);
+    h[i][0] = pack2(s.x, s.y);
+    h[i][1] = pack2(s.z, s.w);
   }
-  const f2 pole_bias = pack2(kPoleBias, kPoleBias);
-  const float bias0 = p.dt_bias != nullptr ? p.dt_bias[ech] : 0.f, bias1 = p.dt_bias != nullptr ? p.dt_bias[ech1] : 0.f;
-  float D0 = 0.f, D1 = 0.f;
-  if (!LOCAL) {
-    if (p.D != nullptr) { D0 = p.D[ech]; D1 = p.D[ech1]; }
-    if (slot == semx::kRefused) D0 = D1 = __int_as_float(0x7fffffff);
-  }
-  float dsum0 = 0.f, dsum1 = 0.f;
+  const float4 bias = load_params(p.dt_bias, ech, en);
+  float4 D = LOCAL ? make_float4(0.f, 0.f, 0.f, 0.f) : load_params(p.D, ech, en);
+  if (slot == semx::kRefused) D.x = D.y = D.z = D.w = __int_as_float(0x7fffffff);
+  float4 dsum = make_float4(0.f, 0.f, 0.f, 0.f);
   // States that a training forward keeps: of step 0 of the piece on, every kBlock steps.
   float* ck = nullptr;
-  if (!LOCAL && p.ckpt != nullptr && cok)
-    ck = p.ckpt + ((piece_base(p.m, q.s, kBlock) + q.t0 / kBlock) * p.C + ch) * p.N + n0;
   const int64_t ck_step = (int64_t)p.C * p.N;
-  const bool ck_vec = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.ckpt) & 15) == 0;
+  if (!LOCAL && p.ckpt != nullptr) ck = p.ckpt + (piece_base(p.m, q.s, kBlock) + q.t0 / kBlock) * ck_step;
+  const bool mode_quads = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.ckpt) & 15) == 0;
 
-  uint2 rx[E], rd[E], rz[E];
-  uint32_t rB[EB], rC[EB];
-  auto fetch = [&](int t0) {
-    const int64_t row = q.row0 + t0 + et;
+  Quad rx[E], rd[E], rz[E], rB[EB], rC[EB];
+  // Element offsets of the thread's first row; they move on by a tile at a time.
+  int64_t ox = (q.row0 + q.t0 + et) * p.ldx + ech, od = (q.row0 + q.t0 + et) * p.lddt + ech;
+  int64_t oz = (q.row0 + q.t0 + et) * p.ldz + ech, oy = (q.row0 + q.t0 + et) * p.C + ech;
+  const int tb0 = tid / GL;  // its (step, four modes): steps tb0, tb0 + ML, ...
+  int64_t oB = (q.row0 + q.t0 + tb0) * p.ldb + (int64_t)grp * p.N + n0;
+  int64_t oC = (q.row0 + q.t0 + tb0) * p.ldc + (int64_t)grp * p.N + n0;
+  const int bn = min(4, p.N - n0);
+  auto fetch = [&](int left) {  // rows of the piece from this tile on
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const bool ok = eok && et + i * TS < TT && t0 + et + i * TS < q.t1;
-      const int64_t r = row + i * TS;
-      rx[i] = rd[i] = rz[i] = make_uint2(0u, 0u);
-      if (ok) {
-        rx[i] = load_pair(p.x, r * p.ldx + ech, p.bf16, vec, two);
-        rd[i] = load_pair(p.dt, r * p.lddt + ech, p.dt_bf16, vec, two);
-        if (!LOCAL && p.z != nullptr) rz[i] = load_pair(p.z, r * p.ldz + ech, p.bf16, vec, two);
+      rx[i] = rd[i] = rz[i] = Quad{};
+      if (en > 0 && et + i * TS < min(TT, left)) {
+        rx[i] = load_quad<ACC>(p.x, ox + i * TS * p.ldx, p.bf16, en);
+        rd[i] = load_quad<ACC>(p.dt, od + i * TS * p.lddt, p.dt_bf16, en);
+        if (has_z) rz[i] = load_quad<ACC>(p.z, oz + i * TS * p.ldz, p.bf16, en);
       }
     }
+    ox += TT * p.ldx;
+    od += TT * p.lddt;
+    oz += TT * p.ldz;
 #pragma unroll
     for (int i = 0; i < EB; ++i) {
-      const int e = tid + i * kThreads, t = e / NP, n = e % NP;
-      const bool ok = t < TT && n < p.N && t0 + t < q.t1;
-      const int64_t r = q.row0 + t0 + t;
-      rB[i] = ok ? load_raw(p.B, r * p.ldb + (int64_t)grp * p.N + n, p.bf16) : 0u;
-      if (!LOCAL) rC[i] = ok ? load_raw(p.Cm, r * p.ldc + (int64_t)grp * p.N + n, p.bf16) : 0u;
+      rB[i] = rC[i] = Quad{};
+      if (bn > 0 && tb0 + i * ML < min(TT, left)) {
+        rB[i] = load_quad<ACC>(p.B, oB + i * ML * p.ldb, p.bf16, bn);
+        if (!LOCAL) rC[i] = load_quad<ACC>(p.Cm, oC + i * ML * p.ldc, p.bf16, bn);
+      }
     }
+    oB += TT * p.ldb;
+    oC += TT * p.ldc;
   };
-  if (q.t0 < q.t1) fetch(q.t0);
+  if (q.t0 < q.t1) fetch(q.t1 - q.t0);
   for (int t0 = q.t0; t0 < q.t1; t0 += TT) {
-    float2 xv[E], zv[E];
+    const int left = q.t1 - t0, nt = min(TT, left);
+    float4 xv[E], zv[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int t = et + i * TS;
       if (t < TT) {
-        const float2 x = pair_floats(rx[i], p.bf16);
-        float2 d = pair_floats(rd[i], p.dt_bf16);
-        d.x += bias0;
-        d.y += bias1;
-        if (p.softplus) {
-          d.x = softplus(d.x);
-          d.y = softplus(d.y);
-        }
-        if (t0 + t >= q.t1) d.x = d.y = 0.f;  // a row behind the piece: pole 1, no drive
-        sdt[t][ec] = make_float4(d.x, d.x, d.x * x.x, d.x * x.x);
-        sdt[t][ec + 1] = make_float4(d.y, d.y, d.y * x.y, d.y * x.y);
+        const float4 x = quad_floats<ACC>(rx[i], p.bf16);
+        float4 d = quad_floats<ACC>(rd[i], p.dt_bf16);
+        d.x += bias.x; d.y += bias.y; d.z += bias.z; d.w += bias.w;
+        if (p.softplus) d = softplus4(d);
+        if (t >= nt) d = make_float4(0.f, 0.f, 0.f, 0.f);  // a row behind the piece: pole 1, no drive
+        sdt[t][ec / 2] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
+        sdt[t][ec / 2 + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
         xv[i] = x;
-        if (!LOCAL && p.z != nullptr) zv[i] = pair_floats(rz[i], p.bf16);
+        if (has_z) zv[i] = quad_floats<ACC>(rz[i], p.bf16);
         if (LOCAL) {
-          dsum0 += d.x;
-          dsum1 += d.y;
+          dsum.x += d.x; dsum.y += d.y; dsum.z += d.z; dsum.w += d.w;
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < EB; ++i) {
-      const int e = tid + i * kThreads;
-      if (e < TT * NP) {
-        (&sB[0][0])[e] = as_float(rB[i], p.bf16);
-        if (!LOCAL) (&sC[0][0])[e] = as_float(rC[i], p.bf16);
+      if (tb0 + i * ML < TT) {
+        sB[tb0 + i * ML][lm] = quad_floats<ACC>(rB[i], p.bf16);
+        if (!LOCAL) sC[tb0 + i * ML][lm] = quad_floats<ACC>(rC[i], p.bf16);
       }
     }
     __syncthreads();
-    if (t0 + TT < q.t1) fetch(t0 + TT);
+    if (left > TT) fetch(left - TT);
 
-    const int nt = min(TT, q.t1 - t0);
 #pragma unroll 1
     for (int tb = 0; tb < nt; tb += 4) {
       if (!LOCAL && ck != nullptr && (tb & (kBlock - 1)) == 0) {
-        const float2 a = unpack2(h[0]), b = unpack2(h[1]);
-        if (ck_vec) {
-          if (n0 < p.N) *reinterpret_cast<float4*>(ck) = make_float4(a.x, a.y, b.x, b.y);
-        } else {
-          if (n0 < p.N) ck[0] = a.x;
-          if (n0 + 1 < p.N) ck[1] = a.y;
-          if (n0 + 2 < p.N) ck[2] = b.x;
-          if (n0 + 3 < p.N) ck[3] = b.y;
+#pragma unroll
+        for (int i = 0; i < kCPT; ++i) {
+          const float2 a = unpack2(h[i][0]), b = unpack2(h[i][1]);
+          if (mode_quads) {
+            if (nn[i] > 0) *reinterpret_cast<float4*>(ck + at[i]) = make_float4(a.x, a.y, b.x, b.y);
+          } else {
+            store_quad<kAny>(ck, at[i], 0, nn[i], make_float4(a.x, a.y, b.x, b.y));
+          }
         }
         ck += ck_step;
       }
-      float acc[4];
+      float acc[kCPT][4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int t = tb + u;
-        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(&sdt[t][sc]);
-        const ulonglong2 Bn = *reinterpret_cast<const ulonglong2*>(&sB[t][n0]);
-        h[0] = fma2(poles2(d.x, A2[0], pole_bias), h[0], mul2(d.y, Bn.x));
-        h[1] = fma2(poles2(d.x, A2[1], pole_bias), h[1], mul2(d.y, Bn.y));
-        if (!LOCAL) {
-          const ulonglong2 Cn = *reinterpret_cast<const ulonglong2*>(&sC[t][n0]);
-          const float2 v = unpack2(fma2(h[1], Cn.y, mul2(h[0], Cn.x)));
-          acc[u] = v.x + v.y;
+        const float4 d = sdt[t][cp];
+        const float4 Bn = sB[t][lm];
+        ulonglong2 Cn;
+        if (!LOCAL) Cn = *reinterpret_cast<const ulonglong2*>(&sC[t][lm]);
+#pragma unroll
+        for (int i = 0; i < kCPT; ++i) {
+          const float dd = i == 0 ? d.x : d.y, dx = i == 0 ? d.z : d.w;
+          h[i][0] = fma2(pack2(pole(dd, A2[i][0]), pole(dd, A2[i][1])), h[i][0], pack2(dx * Bn.x, dx * Bn.y));
+          h[i][1] = fma2(pack2(pole(dd, A2[i][2]), pole(dd, A2[i][3])), h[i][1], pack2(dx * Bn.z, dx * Bn.w));
+          if (!LOCAL) {
+            const float2 v = unpack2(fma2(h[i][1], Cn.y, mul2(h[i][0], Cn.x)));
+            acc[i][u] = v.x + v.y;
+          }
         }
       }
       if (!LOCAL) {
         // Lane m (mod RS) of a channel's lanes ends with the sums of steps m, m + RS, ...
 #pragma unroll
         for (int u = 0; u < 4; u += RS) {
-          float part[RS];
+          float s[kCPT];
 #pragma unroll
-          for (int k = 0; k < RS; ++k) part[k] = acc[u + k];
-          const float s = lanes_scatter_sum<GL, RS>(part, lm);
-          if (lm < RS) sys[tb + u + lm][sc] = s;
+          for (int i = 0; i < kCPT; ++i) {
+            float part[RS];
+#pragma unroll
+            for (int k = 0; k < RS; ++k) part[k] = acc[i][u + k];
+            s[i] = lanes_scatter_sum<GL, RS>(part, lm);
+          }
+          if (lm < RS) *reinterpret_cast<float2*>(&sys[tb + u + lm][sc]) = make_float2(s[0], s[1]);
         }
       }
     }
@@ -213,42 +231,40 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int t = et + i * TS;
-        if (t < TT && t0 + t < q.t1 && eok) {
-          const int64_t o = (q.row0 + t0 + t) * p.C + ech;
-          const float2 s = *reinterpret_cast<const float2*>(&sys[t][ec]);
-          float v0 = fmaf(D0, xv[i].x, s.x), v1 = fmaf(D1, xv[i].y, s.y);
-          if (p.v != nullptr) store_pair(p.v, o, p.bf16, vec, two, v0, v1);
-          if (p.z != nullptr) {
-            v0 *= zv[i].x * sigmoid(zv[i].x);
-            v1 *= zv[i].y * sigmoid(zv[i].y);
-          }
-          store_pair(p.y, o, p.bf16, vec, two, v0, v1);
+        if (t < nt && en > 0) {
+          const int64_t o = oy + i * TS * (int64_t)p.C;
+          const float4 s = *reinterpret_cast<const float4*>(&sys[t][ec]);
+          float4 v = make_float4(fmaf(D.x, xv[i].x, s.x), fmaf(D.y, xv[i].y, s.y), fmaf(D.z, xv[i].z, s.z),
+                                 fmaf(D.w, xv[i].w, s.w));
+          if (p.v != nullptr) store_quad<ACC>(p.v, o, p.bf16, en, v);
+          if (has_z) v = gate4(v, zv[i]);
+          store_quad<ACC>(p.y, o, p.bf16, en, v);
         }
       }
+      oy += TT * (int64_t)p.C;
     }
   }
-  const float2 ha = unpack2(h[0]), hb = unpack2(h[1]);
-  const float last[4] = {ha.x, ha.y, hb.x, hb.y};
-  if (LOCAL) {
-    if (cok)
+  float* out = LOCAL ? p.entry + j * p.C * p.N : p.entry == nullptr && slot >= 0 ? p.state + slot * p.C * p.N : nullptr;
+  if (out != nullptr) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
-        if (n0 + n < p.N) p.entry[(j * p.C + ch) * p.N + n0 + n] = last[n];
-    // Sum of the steps: the threads of a channel in order.
-    float* red = reinterpret_cast<float*>(&sdt[0][0]);
-    __syncthreads();
-    red[et * CH + ec] = dsum0;
-    red[et * CH + ec + 1] = dsum1;
-    __syncthreads();
-    if (tid < CH && cg0 + tid < p.cpg) {
-      float s = 0.f;
-      for (int i = 0; i < TS; ++i) s += red[i * CH + tid];
-      p.dsum[j * p.C + c_base + cg0 + tid] = s;
+    for (int i = 0; i < kCPT; ++i) {
+      const float2 a = unpack2(h[i][0]), b = unpack2(h[i][1]);
+      store_quad<kAny>(out, at[i], 0, nn[i], make_float4(a.x, a.y, b.x, b.y));
     }
-  } else if (p.entry == nullptr && slot >= 0 && cok) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (n0 + n < p.N) p.state[(slot * p.C + ch) * p.N + n0 + n] = last[n];
+  }
+  if (LOCAL) {
+    // Sum of the steps: the threads of a channel in order.
+    __syncthreads();
+    if (et < TT) sdt[0][et * (CH / 4) + ec / 4] = dsum;  // at most TT CH / 4 entries
+    __syncthreads();
+    if (et == 0 && en > 0) {
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < (TS < TT ? TS : TT); ++i) {
+        const float4 d = sdt[0][i * (CH / 4) + ec / 4];
+        s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
+      }
+      store_quad<kAny>(p.dsum, j * p.C + ech, 0, en, s);
+    }
   }
 }
 
@@ -280,15 +296,17 @@ __global__ void __launch_bounds__(kThreads) state_scan_join_kernel(const ScanPar
 template <bool LOCAL>
 int launch_fwd(ScanParams& p, cudaStream_t st) {
   const int gl = lanes_for(p.N, 4);
-  p.tpg = (int)semx::cdiv(p.cpg, (int64_t)(kThreads / gl));
+  p.tpg = (int)semx::cdiv(p.cpg, (int64_t)(kThreads / gl * kCPT));
   p.ctiles = p.G * p.tpg;
   const int64_t grid = p.m.pieces * p.ctiles;
   if (grid == 0) return SEMX_OK;
   if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan: too many pieces");
   switch (gl) {
-#define SEMX_GL(GV)                                                                     \
-  case GV:                                                                              \
-    state_scan_fwd_kernel<GV, LOCAL><<<(unsigned)grid, kThreads, 0, st>>>(p);           \
+#define SEMX_GL(GV)                                                                                              \
+  case GV:                                                                                                       \
+    if (p.access == kBf16) state_scan_fwd_kernel<GV, LOCAL, kBf16><<<(unsigned)grid, kThreads, 0, st>>>(p);      \
+    else if (p.access == kFp32) state_scan_fwd_kernel<GV, LOCAL, kFp32><<<(unsigned)grid, kThreads, 0, st>>>(p); \
+    else state_scan_fwd_kernel<GV, LOCAL, kAny><<<(unsigned)grid, kThreads, 0, st>>>(p);                         \
     return semx::check_launch("state_scan_fwd_kernel");
     SEMX_GL(1)
     SEMX_GL(2)
@@ -334,11 +352,16 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
   p->x = a->x; p->dt = a->dt; p->A = a->A; p->B = a->B; p->Cm = a->Cm; p->D = a->D; p->z = a->z;
   p->dt_bias = a->dt_bias; p->y = a->y; p->state = a->state; p->v = a->v; p->ckpt = a->ckpt;
   p->dy = a->dy; p->dx = a->dx; p->ddt = a->ddt; p->dz = a->dz;
-  const uintptr_t align = a->bf16 ? 4 : 8;
-  p->vec2 = p->cpg % 2 == 0 && a->ldx % 2 == 0 && a->lddt % 2 == 0 && (a->z == nullptr || a->ldz % 2 == 0) &&
-            semx::aligned(a->dt, a->dt_bf16 ? 4 : 8) && semx::aligned(a->ddt, a->dt_bf16 ? 4 : 8);
-  for (const void* t : {a->x, a->z, (const void*)a->y, (const void*)a->v, a->dy, (const void*)a->dx, (const void*)a->dz})
-    if (!semx::aligned(t, align)) p->vec2 = 0;
+  // Four neighbours per access: one type, and every row, group and base on four elements.
+  p->access = kAny;
+  if ((a->bf16 != 0) == (a->dt_bf16 != 0) && p->cpg % 4 == 0 && p->N % 4 == 0 && a->ldx % 4 == 0 && a->lddt % 4 == 0 &&
+      (a->z == nullptr || a->ldz % 4 == 0) && a->ldb % 4 == 0 && a->ldc % 4 == 0) {
+    bool ok = true;
+    for (const void* t : {a->x, a->dt, a->B, a->Cm, a->z, (const void*)a->y, (const void*)a->v, a->dy,
+                          (const void*)a->dx, (const void*)a->ddt, (const void*)a->dz})
+      ok = ok && semx::aligned(t, a->bf16 ? 8 : 16);
+    if (ok) p->access = a->bf16 ? kBf16 : kFp32;
+  }
   return SEMX_OK;
 }
 
@@ -346,14 +369,16 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
 
 namespace {
 
-// Rows per piece of a forward (0: whole sequences).
+// Rows per piece of a forward (0: whole sequences). Pieces cost the exponentials twice, so
+// only batches that leave most of the GPU idle are cut, into one wave of resident CTAs.
+constexpr int64_t kResident = 148 * 4;
 int64_t fwd_rows_per_piece(const ScanParams& p) {
-  const int64_t warps = (int64_t)p.m.S * p.C * lanes_for(p.N, 4) / 32;
-  const int64_t rows = p.m.S > 0 ? p.m.T / p.m.S : 0;
-  if (warps >= 148 * 8 || rows <= 64) return 0;
-  const int64_t cut = semx::cdiv((int64_t)148 * 16, warps > 0 ? warps : 1);
-  const int64_t Q = semx::cdiv(semx::cdiv(p.m.T, p.m.S * cut), 32) * 32;
-  return Q < 32 ? 32 : Q;
+  const int64_t ch = kThreads / lanes_for(p.N, 4) * kCPT;
+  const int64_t ctas = p.m.S * p.G * semx::cdiv(p.cpg, ch);
+  const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
+  if (2 * ctas > kResident || rows <= 128) return 0;
+  const int64_t Q = semx::cdiv(semx::cdiv(rows, kResident / ctas), 16) * 16;
+  return Q < 64 ? 64 : Q;
 }
 
 size_t split_floats(const ScanParams& p) { return (size_t)p.m.pieces * p.C * (p.N + 1); }

@@ -27,7 +27,7 @@ struct ScanParams {
   int C, N, G, cpg;      // channels, modes, groups, channels per group
   int ctiles, tpg;       // channel tiles, and tiles per group
   int bf16, dt_bf16, softplus;
-  int vec2;              // every row operand allows accesses of two neighbouring channels
+  int access;            // enum Access that all row operands allow
   int64_t ldx, lddt, ldz, ldb, ldc;
   const void* x;
   const void* dt;
@@ -64,42 +64,68 @@ __device__ __forceinline__ void store(void* base, int64_t i, int bf16, float v) 
   else reinterpret_cast<float*>(base)[i] = v;
 }
 
-// Two neighbouring channels of a row as they are stored (bf16: x alone).
-__device__ __forceinline__ uint2 load_pair(const void* base, int64_t i, int bf16, bool vec, bool two) {
-  uint2 r = make_uint2(0u, 0u);
-  if (bf16) {
-    const unsigned short* b = reinterpret_cast<const unsigned short*>(base) + i;
-    if (vec) r.x = *reinterpret_cast<const uint32_t*>(b);
-    else r.x = (uint32_t)b[0] | (two ? (uint32_t)b[1] << 16 : 0u);
+// How a kernel reads and writes rows: kAny takes any type, stride, alignment and width, one
+// element at a time; kBf16 and kFp32 take four neighbours in one access (every operand of
+// that type, rows and groups that start on four elements: ScanParams::quads).
+enum Access { kAny = 0, kBf16 = 1, kFp32 = 2 };
+
+template <int ACC>
+struct RawQuad {
+  typedef uint4 type;
+};
+template <>
+struct RawQuad<kBf16> {
+  typedef uint2 type;
+};
+
+// Elements i .. i + 3 as they are stored (kAny: the first n of them).
+template <int ACC>
+__device__ __forceinline__ typename RawQuad<ACC>::type load_quad(const void* base, int64_t i, int bf16, int n) {
+  if constexpr (ACC == kBf16) {
+    return *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(base) + i);
+  } else if constexpr (ACC == kFp32) {
+    return *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(base) + i);
   } else {
-    const uint32_t* b = reinterpret_cast<const uint32_t*>(base) + i;
-    if (vec) r = *reinterpret_cast<const uint2*>(b);
-    else r = make_uint2(b[0], two ? b[1] : 0u);
+    uint4 r = make_uint4(0u, 0u, 0u, 0u);
+    if (n > 0) r.x = load_raw(base, i, bf16);
+    if (n > 1) r.y = load_raw(base, i + 1, bf16);
+    if (n > 2) r.z = load_raw(base, i + 2, bf16);
+    if (n > 3) r.w = load_raw(base, i + 3, bf16);
+    return r;
   }
-  return r;
 }
-__device__ __forceinline__ float2 pair_floats(uint2 r, int bf16) {
-  return bf16 ? make_float2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u))
-              : make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-__device__ __forceinline__ void store_pair(void* base, int64_t i, int bf16, bool vec, bool two, float a, float b) {
-  if (bf16) {
-    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + i;
-    if (vec) {
-      *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(a, b);
-    } else {
-      o[0] = __float2bfloat16(a);
-      if (two) o[1] = __float2bfloat16(b);
-    }
+template <int ACC>
+__device__ __forceinline__ float4 quad_floats(const typename RawQuad<ACC>::type& r, int bf16) {
+  if constexpr (ACC == kBf16) {
+    return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                       __uint_as_float(r.y & 0xffff0000u));
+  } else if constexpr (ACC == kFp32) {
+    return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w));
   } else {
-    float* o = reinterpret_cast<float*>(base) + i;
-    if (vec) {
-      *reinterpret_cast<float2*>(o) = make_float2(a, b);
-    } else {
-      o[0] = a;
-      if (two) o[1] = b;
-    }
+    return make_float4(as_float(r.x, bf16), as_float(r.y, bf16), as_float(r.z, bf16), as_float(r.w, bf16));
   }
+}
+template <int ACC>
+__device__ __forceinline__ void store_quad(void* base, int64_t i, int bf16, int n, float4 v) {
+  if constexpr (ACC == kBf16) {
+    uint2 q;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+    h[0] = __floats2bfloat162_rn(v.x, v.y);
+    h[1] = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = q;
+  } else if constexpr (ACC == kFp32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i) = v;
+  } else {
+    if (n > 0) store(base, i, bf16, v.x);
+    if (n > 1) store(base, i + 1, bf16, v.y);
+    if (n > 2) store(base, i + 2, bf16, v.z);
+    if (n > 3) store(base, i + 3, bf16, v.w);
+  }
+}
+// The first n of four parameters (0 for the rest and without a parameter).
+__device__ __forceinline__ float4 load_params(const float* base, int64_t i, int n) {
+  if (base == nullptr) return make_float4(0.f, 0.f, 0.f, 0.f);
+  return make_float4(n > 0 ? base[i] : 0.f, n > 1 ? base[i + 1] : 0.f, n > 2 ? base[i + 2] : 0.f, n > 3 ? base[i + 3] : 0.f);
 }
 
 // Pairs of fp32 values in one register pair: one instruction works on both.
@@ -130,38 +156,44 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
   return r;
 }
 
-// Poles exp(d A) of two modes from d (in both halves) and A log2(e). The special-function
-// exponential of small negative arguments is measured 2e-8 low on average (rms 3.5e-8); a
-// state multiplies hundreds of poles, so that average is what reaches the results. kPoleBias
-// moves the argument by as much, inside the multiply-add that forms it.
+// Pole exp(d A) from d and A log2(e). The special-function exponential of small negative
+// arguments is measured 2e-8 low on average (rms 3.5e-8); a state multiplies hundreds of
+// poles, so that average is what reaches the results. kPoleBias moves the argument by as
+// much, inside the multiply-add that forms it.
 constexpr float kPoleBias = 3.0e-8f;
-__device__ __forceinline__ f2 poles2(f2 dd, f2 A2, f2 bias) {
-  const float2 v = unpack2(fma2(dd, A2, bias));
-  return pack2(semx::ex2_approx(v.x), semx::ex2_approx(v.y));
-}
+__device__ __forceinline__ float pole(float d, float A2) { return semx::ex2_approx(fmaf(d, A2, kPoleBias)); }
 
 __device__ __forceinline__ float sigmoid(float v) { return semx::rcp_approx(1.f + semx::ex2_approx(-kLog2e * v)); }
 
-// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|): log1p(e) / e on [0, 1] is a degree 9
-// Chebyshev interpolant (5e-9 off, 1e-7 with its roundings); e is corrected for the rounding
-// of its argument, which small steps (v near -7) would show in full. Above 20 the
-// logarithm is below half a step of v.
-__device__ __forceinline__ float softplus(float v) {
-  const float t = -fabsf(v), p = t * kLog2e;
-  const float lost = fmaf(t, kLog2e, -p) + t * 1.925963033500e-8f;  // log2(e) - float(log2(e))
-  float e = semx::ex2_approx(p);
-  e = fmaf(e, lost * 0.6931471805599453f, e);
-  float s = -0.0031760570127512695f;
-  s = fmaf(s, e, 0.019542528316378593f);
-  s = fmaf(s, e, -0.05637361481785774f);
-  s = fmaf(s, e, 0.10543623566627502f);
-  s = fmaf(s, e, -0.1526966691017151f);
-  s = fmaf(s, e, 0.1966327428817749f);
-  s = fmaf(s, e, -0.24951615929603577f);
-  s = fmaf(s, e, 0.33329710364341736f);
-  s = fmaf(s, e, -0.49999892711639404f);
-  s = fmaf(s, e, 1.0f);
-  return fmaf(s, e, fmaxf(v, 0.f));
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|), of two values: log1p(e) / e on [0, 1]
+// is a degree 9 Chebyshev interpolant (5e-9 off, 1e-7 with its roundings); e is corrected for
+// the rounding of its argument, which small steps (v near -7) would show in full. Above 20
+// the logarithm is below half a step of v.
+__device__ __forceinline__ float2 softplus2(float a, float b) {
+  constexpr float kLow = 1.925963033500e-8f;  // log2(e) - float(log2(e))
+  constexpr float kLn2 = 0.6931471805599453f;
+  // exp(-150) is 0 in fp32; the bound keeps infinities out of the products below.
+  const f2 t = pack2(fmaxf(-fabsf(a), -150.f), fmaxf(-fabsf(b), -150.f)), l = pack2(kLog2e, kLog2e);
+  const f2 p = mul2(t, l);
+  const float2 pv = unpack2(p);
+  // What the product lost, and the constant's own tail.
+  const f2 lost = fma2(t, pack2(kLow, kLow), fma2(t, l, pack2(-pv.x, -pv.y)));
+  f2 e = pack2(semx::ex2_approx(pv.x), semx::ex2_approx(pv.y));
+  e = fma2(e, mul2(lost, pack2(kLn2, kLn2)), e);
+  constexpr float c[9] = {0.019542528316378593f, -0.05637361481785774f, 0.10543623566627502f, -0.1526966691017151f,
+                          0.1966327428817749f, -0.24951615929603577f, 0.33329710364341736f, -0.49999892711639404f, 1.0f};
+  f2 s = pack2(-0.0031760570127512695f, -0.0031760570127512695f);
+#pragma unroll
+  for (int i = 0; i < 9; ++i) s = fma2(s, e, pack2(c[i], c[i]));
+  return unpack2(fma2(s, e, pack2(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b)));  // a NaN stays
+}
+__device__ __forceinline__ float4 softplus4(float4 v) {
+  const float2 a = softplus2(v.x, v.y), b = softplus2(v.z, v.w);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 gate4(float4 v, float4 z) {
+  return make_float4(v.x * (z.x * sigmoid(z.x)), v.y * (z.y * sigmoid(z.y)), v.z * (z.z * sigmoid(z.z)),
+                     v.w * (z.w * sigmoid(z.w)));
 }
 
 // Lanes per channel for N modes, MPT per thread.

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) state_scan_bwd_kernel(const ScanPara
       if (t < kBlock) {
         const bool in = t0 + t < q.t1 && eok;
         const float raw = as_float(rd[i], p.dt_bf16) + bias;
-        float d = p.softplus ? softplus(raw) : raw;
+        float d = p.softplus ? softplus2(raw, raw).x : raw;
         if (!in) d = 0.f;
         float g = as_float(rg[i], p.bf16);
         if (p.z != nullptr) {
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) state_scan_bwd_kernel(const ScanPara
         const float4 s = sp[t][sc + i];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          a[t][i][n] = semx::ex2_approx(s.x * A2[i][n]);
+          a[t][i][n] = pole(s.x, A2[i][n]);
           if (!LOCAL) h[t + 1][i][n] = fmaf(a[t][i][n], h[t][i][n], s.y * Bn[n]);
         }
       }

@@ -46,11 +46,11 @@ __global__ void __launch_bounds__(kThreads) state_step_kernel(const ScanParams p
 #pragma unroll
     for (int n = 0; n < 4; ++n) h[n] = !cold && n0 + n < p.N ? st[n] : 0.f;
   }
-  if (p.softplus) d = softplus(d);
+  if (p.softplus) d = softplus2(d, d).x;
   float v = 0.f;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
-    h[n] = fmaf(semx::ex2_approx(d * A2[n]), h[n], d * x * Bn[n]);
+    h[n] = fmaf(pole(d, A2[n]), h[n], d * x * Bn[n]);
     v = fmaf(h[n], Cn[n], v);
   }
 #pragma unroll

@@ -355,6 +355,25 @@ def test_non_finite_rows_stay_in_their_sequence():
             assert torch.isfinite(p[9:20, :3]).all() and torch.isfinite(p[9:20, 4:]).all()
 
 
+def test_steps_far_out():
+    """Softplus at its ends: exact to 2 steps of fp32 from tiny steps to large ones, zero at
+    -inf (the state stays as it is), NaN at NaN. One row per sequence with x = B = C = 1, A = 0
+    and no entry state, so that y is the step itself."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, selective_state_step
+
+    v = torch.cat([torch.linspace(-30, 30, 997), torch.tensor([-100.0, -87.0, 20.0, 20.5, 88.0, 1e4, float("-inf"), float("nan")])])
+    ch = v.numel()
+    dt, one = v.to(cuda()).view(1, 1, ch), torch.ones(1, 1, ch, device=cuda())
+    BC, A = torch.ones(1, 1, 1, device=cuda()), torch.zeros(ch, 1, device=cuda())
+    want = torch.nn.functional.softplus(v.double())
+    state = torch.zeros(1, ch, 1, device=cuda())
+    for y in (selective_state_scan(one, dt, A, BC, BC), selective_state_step(one[0], dt[0], A, BC[0], BC[0], state)):
+        y = y.reshape(-1).double().cpu()
+        assert torch.isnan(y[-1])
+        # 1e-7 of the series, 4 eps of the exponential, a few roundings; below exp(-87) fp32 flushes.
+        assert ((y - want)[:-1].abs() <= 8 * EPS * want[:-1] + 2.0 ** -126).all()
+
+
 def test_bad_offsets_stay_inside():
     """Offsets that decrease, start below zero or reach behind the rows give some result
     without an access outside (they are clamped in the kernels)."""
