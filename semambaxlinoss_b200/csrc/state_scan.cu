@@ -84,21 +84,19 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   const int lm = tid % GL, cp = tid / GL, sc = cp * kCPT;
   const int n0 = lm * 4;
   const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[q.s] != 0);
-  int nn[kCPT];          // modes of the channel that this thread holds
-  int64_t at[kCPT];      // (channel, first mode) of an array (C, N)
+  int nn[kCPT];  // modes of the channel that this thread holds
+  const int64_t at0 = (int64_t)(c_base + cg0 + sc) * p.N + n0;  // (channel, first mode) of an array (C, N)
   float A2[kCPT][4];
   f2 h[kCPT][2];
 #pragma unroll
   for (int i = 0; i < kCPT; ++i) {
-    const bool ok = cg0 + sc + i < p.cpg;
-    nn[i] = ok ? min(4, p.N - n0) : 0;
-    at[i] = (int64_t)(c_base + (ok ? cg0 + sc + i : 0)) * p.N + n0;
-    const float4 a = load_params(p.A, at[i], nn[i]);
+    nn[i] = cg0 + sc + i < p.cpg ? min(4, p.N - n0) : 0;
+    const float4 a = load_params(p.A, at0 + i * p.N, nn[i]);
     A2[i][0] = a.x * kLog2e; A2[i][1] = a.y * kLog2e; A2[i][2] = a.z * kLog2e; A2[i][3] = a.w * kLog2e;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (!LOCAL) {
-      if (p.entry != nullptr) s = load_params(p.entry, j * p.C * p.N + at[i], nn[i]);
-      else if (!cold) s = load_params(p.state, slot * p.C * p.N + at[i], nn[i]);
+      if (p.entry != nullptr) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
+      else if (!cold) s = load_params(p.state, slot * p.C * p.N + at0 + i * p.N, nn[i]);
     }
     h[i][0] = pack2(s.x, s.y);
     h[i][1] = pack2(s.z, s.w);
@@ -184,9 +182,9 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
         for (int i = 0; i < kCPT; ++i) {
           const float2 a = unpack2(h[i][0]), b = unpack2(h[i][1]);
           if (mode_quads) {
-            if (nn[i] > 0) *reinterpret_cast<float4*>(ck + at[i]) = make_float4(a.x, a.y, b.x, b.y);
+            if (nn[i] > 0) *reinterpret_cast<float4*>(ck + at0 + i * p.N) = make_float4(a.x, a.y, b.x, b.y);
           } else {
-            store_quad<kAny>(ck, at[i], 0, nn[i], make_float4(a.x, a.y, b.x, b.y));
+            store_quad<kAny>(ck, at0 + i * p.N, 0, nn[i], make_float4(a.x, a.y, b.x, b.y));
           }
         }
         ck += ck_step;
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
 #pragma unroll
     for (int i = 0; i < kCPT; ++i) {
       const float2 a = unpack2(h[i][0]), b = unpack2(h[i][1]);
-      store_quad<kAny>(out, at[i], 0, nn[i], make_float4(a.x, a.y, b.x, b.y));
+      store_quad<kAny>(out, at0 + i * p.N, 0, nn[i], make_float4(a.x, a.y, b.x, b.y));
     }
   }
   if (LOCAL) {

@@ -168,8 +168,8 @@ __device__ __forceinline__ float sigmoid(float v) { return semx::rcp_approx(1.f 
 // log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|), of two values: log1p(e) / e on [0, 1]
 // is a degree 9 Chebyshev interpolant (5e-9 off, 1e-7 with its roundings); e is corrected for
 // the rounding of its argument, which small steps (v near -7) would show in full. Above 20
-// the logarithm is below half a step of v.
-__device__ __forceinline__ float2 softplus2(float a, float b) {
+// the logarithm is below half a step of v. e comes back for the derivative.
+__device__ __forceinline__ float2 softplus2(float a, float b, float2* exps = nullptr) {
   constexpr float kLow = 1.925963033500e-8f;  // log2(e) - float(log2(e))
   constexpr float kLn2 = 0.6931471805599453f;
   // exp(-150) is 0 in fp32; the bound keeps infinities out of the products below.
@@ -180,6 +180,7 @@ __device__ __forceinline__ float2 softplus2(float a, float b) {
   const f2 lost = fma2(t, pack2(kLow, kLow), fma2(t, l, pack2(-pv.x, -pv.y)));
   f2 e = pack2(semx::ex2_approx(pv.x), semx::ex2_approx(pv.y));
   e = fma2(e, mul2(lost, pack2(kLn2, kLn2)), e);
+  if (exps != nullptr) *exps = unpack2(e);
   constexpr float c[9] = {0.019542528316378593f, -0.05637361481785774f, 0.10543623566627502f, -0.1526966691017151f,
                           0.1966327428817749f, -0.24951615929603577f, 0.33329710364341736f, -0.49999892711639404f, 1.0f};
   f2 s = pack2(-0.0031760570127512695f, -0.0031760570127512695f);
@@ -191,6 +192,12 @@ __device__ __forceinline__ float4 softplus4(float4 v) {
   const float2 a = softplus2(v.x, v.y), b = softplus2(v.z, v.w);
   return make_float4(a.x, a.y, b.x, b.y);
 }
+// softplus' = 1 / (1 + exp(-v)) from e = exp(-|v|).
+__device__ __forceinline__ float softplus_slope(float v, float e) {
+  const float r = semx::rcp_approx(1.f + e);
+  return v < 0.f ? e * r : r;
+}
+
 __device__ __forceinline__ float4 gate4(float4 v, float4 z) {
   return make_float4(v.x * (z.x * sigmoid(z.x)), v.y * (z.y * sigmoid(z.y)), v.z * (z.z * sigmoid(z.z)),
                      v.w * (z.w * sigmoid(z.w)));

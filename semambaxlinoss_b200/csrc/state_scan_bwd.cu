@@ -31,30 +31,12 @@ namespace {
 using namespace semx_scan;
 
 constexpr int kWarps = kThreads / 32;
+constexpr int kCPT = 2;  // channels per thread
 constexpr float kLn2 = 0.6931471805599453f;
 
-// E elements at i, i + stride, ... of steps t, t + TS, ... (0 from step t1 on).
-template <int E, int TS>
-__device__ __forceinline__ void fetch_pairs(uint32_t (&r)[E], const void* base, int bf16, int64_t i, int64_t stride,
-                                            int t, int t1, bool ok) {
-  if (bf16) {
-    const unsigned short* b = reinterpret_cast<const unsigned short*>(base);
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = ok && t + e * TS < t1 ? b[i + e * stride] : 0u;
-  } else {
-    const uint32_t* b = reinterpret_cast<const uint32_t*>(base);
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = ok && t + e * TS < t1 ? b[i + e * stride] : 0u;
-  }
-}
-
-template <int GM>
-constexpr int channels_per_thread() {
-  return GM == 1 ? 1 : 2;
-}
 template <int GM>
 constexpr int channels_per_cta() {
-  return kWarps * (32 / GM) * channels_per_thread<GM>();
+  return kThreads / GM * kCPT;
 }
 
 // Sums v over LANES lanes that are STRIDE apart, by halving; afterwards v[0 .. NV / LANES)
@@ -80,19 +62,23 @@ __device__ __forceinline__ void halve_sum(float (&v)[NV], int lane) {
   }
 }
 
-template <int GM, bool LOCAL>
-__global__ void __launch_bounds__(kThreads) state_scan_bwd_kernel(const ScanParams p) {
-  constexpr int CPT = channels_per_thread<GM>(), CL = 32 / GM, CH = channels_per_cta<GM>(), NP = 4 * GM;
-  constexpr int TS = kThreads / CH;  // steps between a thread's (step, channel) pairs
-  constexpr int E = kBlock / TS > 0 ? kBlock / TS : 1;
-  constexpr int EB = (kBlock * NP + kThreads - 1) / kThreads;
-  constexpr int NV1 = 2 * CPT, NO1 = NV1 / GM > 0 ? NV1 / GM : 1;
+template <int GM, bool LOCAL, int ACC>
+__global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel(const ScanParams p) {
+  constexpr int CL = 32 / GM, CH = channels_per_cta<GM>(), NP = 4 * GM;
+  constexpr int TS = kThreads / (CH / 4);       // rows that the CTA loads at a time
+  constexpr int E = (kBlock + TS - 1) / TS;     // (step, four channels) of a thread
+  constexpr int ML = kThreads / GM;             // rows of B and C loaded at a time
+  constexpr int EB = (kBlock + ML - 1) / ML;    // (step, four modes) of a thread
+  constexpr int NV1 = 2 * kCPT, NO1 = NV1 / GM > 0 ? NV1 / GM : 1;
   constexpr int NO2 = 8 / CL > 0 ? 8 / CL : 1;
-  __shared__ __align__(16) float4 sp[kBlock][CH];  // (d, d x, dv, -)
-  __shared__ __align__(16) float sB[kBlock][NP];
-  __shared__ __align__(16) float sC[kBlock][NP];
-  __shared__ float2 so[LOCAL ? 1 : kBlock][LOCAL ? 1 : CH];                      // (gB, uA)
+  typedef typename RawQuad<ACC>::type Quad;
+  __shared__ __align__(16) float4 sd[kBlock][CH / 2];  // (d, d', d x, d' x') of two channels
+  __shared__ __align__(16) float2 sv[kBlock][CH / 2];  // (dv, dv')
+  __shared__ __align__(16) float4 sB[LOCAL ? 1 : kBlock][LOCAL ? 1 : GM];
+  __shared__ __align__(16) float4 sC[kBlock][GM];
+  __shared__ __align__(16) float so[LOCAL ? 1 : kBlock][LOCAL ? 4 : 2 * CH];        // (gB, uA) per channel
   __shared__ float sw[LOCAL ? 1 : kWarps][LOCAL ? 1 : kBlock][LOCAL ? 1 : 2 * NP];  // dB | dC of a warp
+  __shared__ __align__(16) float4 red[kThreads];
 
   const int64_t j = blockIdx.x / p.ctiles;
   const int ct = blockIdx.x % p.ctiles;
@@ -100,170 +86,212 @@ __global__ void __launch_bounds__(kThreads) state_scan_bwd_kernel(const ScanPara
   const Piece q = find_piece(p.m, j);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
 
-  const int ec = tid % CH, et = tid / CH;
-  const bool eok = cg0 + ec < p.cpg;
-  const int ech = c_base + min(cg0 + ec, p.cpg - 1);
-  if (!LOCAL && eok && et == 0)
+  // The four channels of this thread in loads and stores (en of them exist).
+  const int ec = tid % (CH / 4) * 4, et = tid / (CH / 4);
+  const int en = min(4, p.cpg - cg0 - ec);
+  const int64_t ech = c_base + (en > 0 ? cg0 + ec : 0);
+  const bool has_z = p.z != nullptr;
+  const float4 zero4 = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (!LOCAL && en > 0 && et == 0)
     for (int64_t r = rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) {
-      store(p.dx, r * p.C + ech, p.bf16, 0.f);
-      store(p.ddt, r * p.C + ech, p.dt_bf16, 0.f);
-      if (p.z != nullptr) store(p.dz, r * p.C + ech, p.bf16, 0.f);
+      store_quad<ACC>(p.dx, r * p.C + ech, p.bf16, en, zero4);
+      store_quad<ACC>(p.ddt, r * p.C + ech, p.dt_bf16, en, zero4);
+      if (has_z) store_quad<ACC>(p.dz, r * p.C + ech, p.bf16, en, zero4);
     }
 
-  const int lm = lane % GM, cl = lane / GM;
-  const int sc = (warp * CL + cl) * CPT;  // first of the thread's channels in the tile
-  const int n0 = lm * 4;
-  bool cok[CPT];
-  int ch[CPT];
-  float A2[CPT][4], dA[CPT][4], carry[CPT][4];
+  // The channels and modes of this thread in the scan.
+  const int lm = lane % GM, cl = lane / GM, n0 = lm * 4;
+  const int cp = warp * CL + cl, sc = cp * kCPT;
+  int nn[kCPT];  // modes of the channel that this thread holds
+  const int64_t at0 = (int64_t)(c_base + cg0 + sc) * p.N + n0;  // (channel, first mode) of an array (C, N)
+  float A2[kCPT][4];
+  f2 dA[kCPT][2], carry[kCPT][2];
 #pragma unroll
-  for (int i = 0; i < CPT; ++i) {
-    cok[i] = cg0 + sc + i < p.cpg;
-    ch[i] = c_base + min(cg0 + sc + i, p.cpg - 1);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const bool ok = n0 + n < p.N;
-      A2[i][n] = ok ? p.A[(int64_t)ch[i] * p.N + n0 + n] * kLog2e : 0.f;
-      dA[i][n] = 0.f;
-      carry[i][n] = !LOCAL && ok && q.live && p.entry != nullptr ? p.entry[(j * p.C + ch[i]) * p.N + n0 + n] : 0.f;
-    }
+  for (int i = 0; i < kCPT; ++i) {
+    nn[i] = cg0 + sc + i < p.cpg ? min(4, p.N - n0) : 0;
+    const float4 a = load_params(p.A, at0 + i * p.N, nn[i]);
+    A2[i][0] = a.x * kLog2e; A2[i][1] = a.y * kLog2e; A2[i][2] = a.z * kLog2e; A2[i][3] = a.w * kLog2e;
+    float4 s = zero4;
+    if (!LOCAL && q.live) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
+    carry[i][0] = pack2(s.x, s.y);
+    carry[i][1] = pack2(s.z, s.w);
+    dA[i][0] = dA[i][1] = 0ull;
   }
-  const float bias = p.dt_bias != nullptr ? p.dt_bias[ech] : 0.f;
-  const float Dc = p.D != nullptr ? p.D[ech] : 0.f;
-  float accD = 0.f, accb = 0.f, dsum = 0.f;
+  const float4 bias = load_params(p.dt_bias, ech, en);
+  const float4 D = load_params(p.D, ech, en);
+  float4 accD = zero4, accb = zero4;  // LOCAL: accb is the sum of the steps
+  const bool mode_quads = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.ckpt) & 15) == 0;
 
-  uint32_t rx[E], rd[E], rg[E], rz[E], rv[E], rB[EB], rC[EB];
-  float hn[CPT][4];
+  Quad rx[E], rd[E], rg[E], rz[E], rv[E], rB[EB], rC[EB];
+  float4 hn[kCPT];
   const int64_t blk0 = q.live ? piece_base(p.m, q.s, kBlock) : 0;
+  const int tb0 = tid / GM, bl = tid % GM, bn = min(4, p.N - bl * 4);
   auto fetch = [&](int t0) {
-    const int64_t row = q.row0 + t0 + et;
-    const bool ok = eok && et < kBlock;
-    fetch_pairs<E, TS>(rd, p.dt, p.dt_bf16, row * p.lddt + ech, TS * p.lddt, t0 + et, q.t1, ok);
-    fetch_pairs<E, TS>(rg, p.dy, p.bf16, row * p.C + ech, (int64_t)TS * p.C, t0 + et, q.t1, ok);
-    if (p.z != nullptr) fetch_pairs<E, TS>(rz, p.z, p.bf16, row * p.ldz + ech, TS * p.ldz, t0 + et, q.t1, ok);
-    if (!LOCAL) {
-      fetch_pairs<E, TS>(rx, p.x, p.bf16, row * p.ldx + ech, TS * p.ldx, t0 + et, q.t1, ok);
-      if (p.z != nullptr) fetch_pairs<E, TS>(rv, p.v, p.bf16, row * p.C + ech, (int64_t)TS * p.C, t0 + et, q.t1, ok);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      rx[i] = rd[i] = rg[i] = rz[i] = rv[i] = Quad{};
+      const int t = et + i * TS;
+      if (en > 0 && t < kBlock && t0 + t < q.t1) {
+        const int64_t r = q.row0 + t0 + t;
+        rd[i] = load_quad<ACC>(p.dt, r * p.lddt + ech, p.dt_bf16, en);
+        rg[i] = load_quad<ACC>(p.dy, r * p.C + ech, p.bf16, en);
+        if (has_z) rz[i] = load_quad<ACC>(p.z, r * p.ldz + ech, p.bf16, en);
+        if (!LOCAL) {
+          rx[i] = load_quad<ACC>(p.x, r * p.ldx + ech, p.bf16, en);
+          if (has_z) rv[i] = load_quad<ACC>(p.v, r * p.C + ech, p.bf16, en);
+        }
+      }
     }
 #pragma unroll
     for (int i = 0; i < EB; ++i) {
-      const int e = tid + i * kThreads, t = e / NP, n = e % NP;
-      const bool in = t < kBlock && n < p.N && t0 + t < q.t1;
-      const int64_t r = q.row0 + t0 + t;
-      if (!LOCAL) rB[i] = in ? load_raw(p.B, r * p.ldb + (int64_t)grp * p.N + n, p.bf16) : 0u;
-      rC[i] = in ? load_raw(p.Cm, r * p.ldc + (int64_t)grp * p.N + n, p.bf16) : 0u;
+      rB[i] = rC[i] = Quad{};
+      const int t = tb0 + i * ML;
+      if (bn > 0 && t < kBlock && t0 + t < q.t1) {
+        const int64_t r = q.row0 + t0 + t;
+        if (!LOCAL) rB[i] = load_quad<ACC>(p.B, r * p.ldb + (int64_t)grp * p.N + bl * 4, p.bf16, bn);
+        rC[i] = load_quad<ACC>(p.Cm, r * p.ldc + (int64_t)grp * p.N + bl * 4, p.bf16, bn);
+      }
     }
     if (!LOCAL) {
 #pragma unroll
-      for (int i = 0; i < CPT; ++i)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          hn[i][n] = n0 + n < p.N ? p.ckpt[((blk0 + t0 / kBlock) * p.C + ch[i]) * p.N + n0 + n] : 0.f;
+      for (int i = 0; i < kCPT; ++i) {
+        const float* c = p.ckpt + (blk0 + t0 / kBlock) * p.C * p.N;
+        hn[i] = zero4;
+        if (mode_quads) {
+          if (nn[i] > 0) hn[i] = *reinterpret_cast<const float4*>(c + at0 + i * p.N);
+        } else {
+          hn[i] = load_params(c, at0 + i * p.N, nn[i]);
+        }
+      }
     }
   };
 
   const int tl = q.t1 > q.t0 ? q.t0 + (q.t1 - 1 - q.t0) / kBlock * kBlock : q.t0 - kBlock;
   if (tl >= q.t0) fetch(tl);
+#pragma unroll 1
   for (int t0 = tl; t0 >= q.t0; t0 -= kBlock) {
-    float xv[E], dv[E], gv[E], sg[E];  // x, d, dv, softplus'
+    const int nt = min(kBlock, q.t1 - t0);
+    float4 sg[E];  // softplus'
+    Quad kx[E];    // x
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int t = et + i * TS;
       if (t < kBlock) {
-        const bool in = t0 + t < q.t1 && eok;
-        const float raw = as_float(rd[i], p.dt_bf16) + bias;
-        float d = p.softplus ? softplus2(raw, raw).x : raw;
-        if (!in) d = 0.f;
-        float g = as_float(rg[i], p.bf16);
-        if (p.z != nullptr) {
-          const float z = as_float(rz[i], p.bf16), s = sigmoid(z);
-          if (!LOCAL && in)
-            store(p.dz, (q.row0 + t0 + t) * p.C + ech, p.bf16,
-                  g * as_float(rv[i], p.bf16) * (s * fmaf(z, 1.f - s, 1.f)));
-          g *= z * s;
+        const bool in = t < nt && en > 0;
+        float4 d = quad_floats<ACC>(rd[i], p.dt_bf16), g = quad_floats<ACC>(rg[i], p.bf16);
+        d.x += bias.x; d.y += bias.y; d.z += bias.z; d.w += bias.w;
+        sg[i] = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (p.softplus) {
+          float2 e0, e1;
+          const float2 a = softplus2(d.x, d.y, &e0), b = softplus2(d.z, d.w, &e1);
+          if (!LOCAL)
+            sg[i] = make_float4(softplus_slope(d.x, e0.x), softplus_slope(d.y, e0.y), softplus_slope(d.z, e1.x),
+                                softplus_slope(d.w, e1.y));
+          d = make_float4(a.x, a.y, b.x, b.y);
         }
-        if (!in) g = 0.f;
-        const float x = LOCAL ? 0.f : as_float(rx[i], p.bf16);
-        sp[t][ec] = make_float4(d, d * x, g, 0.f);
-        xv[i] = x;
-        dv[i] = d;
-        gv[i] = g;
-        sg[i] = !LOCAL && p.softplus ? semx::softplus_grad(raw) : 1.f;
-        if (LOCAL) dsum += d;
+        if (has_z) {
+          const float4 z = quad_floats<ACC>(rz[i], p.bf16);
+          const float4 s = make_float4(sigmoid(z.x), sigmoid(z.y), sigmoid(z.z), sigmoid(z.w));
+          if (!LOCAL && in) {
+            const float4 v = quad_floats<ACC>(rv[i], p.bf16);
+            store_quad<ACC>(p.dz, (q.row0 + t0 + t) * p.C + ech, p.bf16, en,
+                            make_float4(g.x * v.x * (s.x * fmaf(z.x, 1.f - s.x, 1.f)),
+                                        g.y * v.y * (s.y * fmaf(z.y, 1.f - s.y, 1.f)),
+                                        g.z * v.z * (s.z * fmaf(z.z, 1.f - s.z, 1.f)),
+                                        g.w * v.w * (s.w * fmaf(z.w, 1.f - s.w, 1.f))));
+          }
+          g.x *= z.x * s.x; g.y *= z.y * s.y; g.z *= z.z * s.z; g.w *= z.w * s.w;
+        }
+        if (!in) d = g = zero4;  // a row behind the piece: pole 1, no drive, no gradient
+        const float4 x = LOCAL ? zero4 : quad_floats<ACC>(rx[i], p.bf16);
+        sd[t][ec / 2] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
+        sd[t][ec / 2 + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
+        *reinterpret_cast<float4*>(&sv[t][ec / 2]) = g;
+        kx[i] = rx[i];
+        if (LOCAL) {
+          accb.x += d.x; accb.y += d.y; accb.z += d.z; accb.w += d.w;
+        }
       }
     }
 #pragma unroll
     for (int i = 0; i < EB; ++i) {
-      const int e = tid + i * kThreads;
-      if (e < kBlock * NP) {
-        if (!LOCAL) (&sB[0][0])[e] = as_float(rB[i], p.bf16);
-        (&sC[0][0])[e] = as_float(rC[i], p.bf16);
+      if (tb0 + i * ML < kBlock) {
+        if (!LOCAL) sB[tb0 + i * ML][bl] = quad_floats<ACC>(rB[i], p.bf16);
+        sC[tb0 + i * ML][bl] = quad_floats<ACC>(rC[i], p.bf16);
       }
     }
-    float a[kBlock][CPT][4], h[kBlock + 1][CPT][4];
+    f2 a[kBlock][kCPT][2], h[kBlock + 1][kCPT][2];
     if (!LOCAL) {
 #pragma unroll
-      for (int i = 0; i < CPT; ++i)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) h[0][i][n] = hn[i][n];
+      for (int i = 0; i < kCPT; ++i) {
+        h[0][i][0] = pack2(hn[i].x, hn[i].y);
+        h[0][i][1] = pack2(hn[i].z, hn[i].w);
+      }
     }
     __syncthreads();
     if (t0 - kBlock >= q.t0) fetch(t0 - kBlock);
 #pragma unroll
     for (int t = 0; t < kBlock; ++t) {
-      float4 B4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!LOCAL) B4 = *reinterpret_cast<const float4*>(&sB[t][n0]);
-      const float Bn[4] = {B4.x, B4.y, B4.z, B4.w};
+      const float4 d = sd[t][cp];
+      float4 B = zero4;
+      if (!LOCAL) B = sB[t][lm];
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        const float4 s = sp[t][sc + i];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          a[t][i][n] = pole(s.x, A2[i][n]);
-          if (!LOCAL) h[t + 1][i][n] = fmaf(a[t][i][n], h[t][i][n], s.y * Bn[n]);
+      for (int i = 0; i < kCPT; ++i) {
+        const float dd = i == 0 ? d.x : d.y, dx = i == 0 ? d.z : d.w;
+        a[t][i][0] = pack2(pole(dd, A2[i][0]), pole(dd, A2[i][1]));
+        a[t][i][1] = pack2(pole(dd, A2[i][2]), pole(dd, A2[i][3]));
+        if (!LOCAL) {
+          h[t + 1][i][0] = fma2(a[t][i][0], h[t][i][0], pack2(dx * B.x, dx * B.y));
+          h[t + 1][i][1] = fma2(a[t][i][1], h[t][i][1], pack2(dx * B.z, dx * B.w));
         }
       }
     }
 #pragma unroll
     for (int t = kBlock - 1; t >= 0; --t) {
-      const float4 C4 = *reinterpret_cast<const float4*>(&sC[t][n0]);
-      const float Cn[4] = {C4.x, C4.y, C4.z, C4.w};
+      const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sC[t][lm]);
+      const float2 vv = sv[t][cp];
       if (LOCAL) {
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-          const float4 s = sp[t][sc + i];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) carry[i][n] = a[t][i][n] * fmaf(Cn[n], s.z, carry[i][n]);
+        for (int i = 0; i < kCPT; ++i) {
+          const f2 v = i == 0 ? pack2(vv.x, vv.x) : pack2(vv.y, vv.y);
+          carry[i][0] = mul2(a[t][i][0], fma2(C.x, v, carry[i][0]));
+          carry[i][1] = mul2(a[t][i][1], fma2(C.y, v, carry[i][1]));
         }
       } else {
-        const float4 B4 = *reinterpret_cast<const float4*>(&sB[t][n0]);
-        const float Bn[4] = {B4.x, B4.y, B4.z, B4.w};
+        const float4 d4 = sd[t][cp];
+        const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sB[t][lm]);
         float v1[NV1], v2[8];
+        f2 b0 = 0ull, b1 = 0ull, c0 = 0ull, c1 = 0ull;
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-          const float4 s = sp[t][sc + i];
-          float gB = 0.f, uA = 0.f;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float g = fmaf(Cn[n], s.z, carry[i][n]);
-            carry[i][n] = a[t][i][n] * g;
-            const float u = carry[i][n] * h[t][i][n];
-            gB = fmaf(g, Bn[n], gB);
-            uA = fmaf(u, A2[i][n], uA);
-            dA[i][n] = fmaf(u, s.x, dA[i][n]);
-            v2[n] = i == 0 ? g * s.y : fmaf(g, s.y, v2[n]);
-            v2[4 + n] = i == 0 ? h[t + 1][i][n] * s.z : fmaf(h[t + 1][i][n], s.z, v2[4 + n]);
-          }
-          v1[2 * i] = gB;
-          v1[2 * i + 1] = uA;
+        for (int i = 0; i < kCPT; ++i) {
+          const f2 v = i == 0 ? pack2(vv.x, vv.x) : pack2(vv.y, vv.y);
+          const f2 d = i == 0 ? pack2(d4.x, d4.x) : pack2(d4.y, d4.y);
+          const f2 dx = i == 0 ? pack2(d4.z, d4.z) : pack2(d4.w, d4.w);
+          const f2 g0 = fma2(C.x, v, carry[i][0]), g1 = fma2(C.y, v, carry[i][1]);
+          carry[i][0] = mul2(a[t][i][0], g0);
+          carry[i][1] = mul2(a[t][i][1], g1);
+          const f2 u0 = mul2(carry[i][0], h[t][i][0]), u1 = mul2(carry[i][1], h[t][i][1]);
+          const float2 gB = unpack2(fma2(g1, B.y, mul2(g0, B.x)));
+          const float2 uA = unpack2(fma2(u1, pack2(A2[i][2], A2[i][3]), mul2(u0, pack2(A2[i][0], A2[i][1]))));
+          v1[2 * i] = gB.x + gB.y;
+          v1[2 * i + 1] = uA.x + uA.y;
+          dA[i][0] = fma2(u0, d, dA[i][0]);
+          dA[i][1] = fma2(u1, d, dA[i][1]);
+          b0 = i == 0 ? mul2(g0, dx) : fma2(g0, dx, b0);
+          b1 = i == 0 ? mul2(g1, dx) : fma2(g1, dx, b1);
+          c0 = i == 0 ? mul2(h[t + 1][i][0], v) : fma2(h[t + 1][i][0], v, c0);
+          c1 = i == 0 ? mul2(h[t + 1][i][1], v) : fma2(h[t + 1][i][1], v, c1);
         }
+        const float2 e0 = unpack2(b0), e1 = unpack2(b1), e2 = unpack2(c0), e3 = unpack2(c1);
+        v2[0] = e0.x; v2[1] = e0.y; v2[2] = e1.x; v2[3] = e1.y;
+        v2[4] = e2.x; v2[5] = e2.y; v2[6] = e3.x; v2[7] = e3.y;
         halve_sum<NV1, GM, 1>(v1, lane);
         halve_sum<8, CL, GM>(v2, lane);
-        // Value k of (channel, {gB, uA}) is float sc * 2 + k of the step's row.
+        // Value k of (channel, {gB, uA}) is float 2 sc + k of the step's row.
         constexpr int SPARE1 = GM > NV1 ? GM / NV1 : 1;
         if (lm % SPARE1 == 0) {
 #pragma unroll
-          for (int k = 0; k < NO1; ++k) reinterpret_cast<float*>(&so[t][sc])[lm / SPARE1 * NO1 + k] = v1[k];
+          for (int k = 0; k < NO1; ++k) so[t][2 * sc + lm / SPARE1 * NO1 + k] = v1[k];
         }
         constexpr int SPARE2 = CL > 8 ? CL / 8 : 1;
         if (cl % SPARE2 == 0) {
@@ -280,19 +308,30 @@ __global__ void __launch_bounds__(kThreads) state_scan_bwd_kernel(const ScanPara
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int t = et + i * TS;
-        if (t < kBlock && t0 + t < q.t1 && eok) {
+        if (t < nt && en > 0) {
           const int64_t o = (q.row0 + t0 + t) * p.C + ech;
-          const float2 s = so[t][ec];
-          store(p.dx, o, p.bf16, fmaf(dv[i], s.x, Dc * gv[i]));
-          const float ddt = fmaf(s.y, kLn2, xv[i] * s.x) * sg[i];
-          store(p.ddt, o, p.dt_bf16, ddt);
-          accb += ddt;
-          accD = fmaf(gv[i], xv[i], accD);
+          const float4 s0 = *reinterpret_cast<const float4*>(&so[t][2 * ec]);
+          const float4 s1 = *reinterpret_cast<const float4*>(&so[t][2 * ec + 4]);
+          // d and dv as this thread put them there.
+          const float4 x = quad_floats<ACC>(kx[i], p.bf16), k = sg[i];
+          const float4 g = *reinterpret_cast<const float4*>(&sv[t][ec / 2]);
+          const float2 d01 = *reinterpret_cast<const float2*>(&sd[t][ec / 2]);
+          const float2 d23 = *reinterpret_cast<const float2*>(&sd[t][ec / 2 + 1]);
+          const float4 d = make_float4(d01.x, d01.y, d23.x, d23.y);
+          store_quad<ACC>(p.dx, o, p.bf16, en,
+                          make_float4(fmaf(d.x, s0.x, D.x * g.x), fmaf(d.y, s0.z, D.y * g.y),
+                                      fmaf(d.z, s1.x, D.z * g.z), fmaf(d.w, s1.z, D.w * g.w)));
+          const float4 ddt = make_float4(fmaf(s0.y, kLn2, x.x * s0.x) * k.x, fmaf(s0.w, kLn2, x.y * s0.z) * k.y,
+                                         fmaf(s1.y, kLn2, x.z * s1.x) * k.z, fmaf(s1.w, kLn2, x.w * s1.z) * k.w);
+          store_quad<ACC>(p.ddt, o, p.dt_bf16, en, ddt);
+          accb.x += ddt.x; accb.y += ddt.y; accb.z += ddt.z; accb.w += ddt.w;
+          accD.x = fmaf(g.x, x.x, accD.x); accD.y = fmaf(g.y, x.y, accD.y);
+          accD.z = fmaf(g.z, x.z, accD.z); accD.w = fmaf(g.w, x.w, accD.w);
         }
       }
-      for (int e = tid; e < kBlock * 2 * NP; e += kThreads) {
+      for (int e = tid; e < nt * 2 * NP; e += kThreads) {
         const int t = e / (2 * NP), v = e % (2 * NP), n = v % NP;
-        if (n < p.N && t0 + t < q.t1) {
+        if (n < p.N) {
           float s = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) s += sw[w][t][v];
@@ -301,43 +340,37 @@ __global__ void __launch_bounds__(kThreads) state_scan_bwd_kernel(const ScanPara
       }
     }
   }
-  float* red = reinterpret_cast<float*>(&sp[0][0]);
-  if (LOCAL) {
-    if (!q.live) return;
-#pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (cok[i])
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          if (n0 + n < p.N) p.entry[(j * p.C + ch[i]) * p.N + n0 + n] = carry[i][n];
-    red[tid] = dsum;
+  // Sum over the threads of four channels, in order of their rows.
+  auto rows_sum = [&](float4 v) {
     __syncthreads();
-    if (tid < CH && eok) {
-      float s = 0.f;
-      for (int i = 0; i < TS; ++i) s += red[i * CH + tid];
-      p.dsum[j * p.C + ech] = s;
-    }
-  } else if (p.part != nullptr) {
-    // Every piece index writes its row, zeros where there is no such piece.
-    float* row = p.part + j * ((int64_t)p.C * (p.N + 2));
-#pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (cok[i])
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          if (n0 + n < p.N) row[(int64_t)ch[i] * p.N + n0 + n] = dA[i][n];
+    red[tid] = v;
     __syncthreads();
-    red[tid] = accD;
-    red[kThreads + tid] = accb;
-    __syncthreads();
-    if (tid < CH && eok) {
-      float s = 0.f, b = 0.f;
+    float4 s = zero4;
+    if (et == 0)
       for (int i = 0; i < TS; ++i) {
-        s += red[i * CH + tid];
-        b += red[kThreads + i * CH + tid];
+        const float4 d = red[i * (CH / 4) + tid];
+        s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
       }
-      row[(int64_t)p.C * p.N + ech] = s;
-      row[(int64_t)p.C * (p.N + 1) + ech] = b;
+    return s;
+  };
+  if (LOCAL && !q.live) return;
+  float* out = LOCAL ? p.entry + j * p.C * p.N : p.part != nullptr ? p.part + j * ((int64_t)p.C * (p.N + 2)) : nullptr;
+  if (out != nullptr) {
+    // Without LOCAL every piece index writes its row, zeros where there is no such piece.
+#pragma unroll
+    for (int i = 0; i < kCPT; ++i) {
+      const float2 v0 = unpack2(LOCAL ? carry[i][0] : dA[i][0]), v1 = unpack2(LOCAL ? carry[i][1] : dA[i][1]);
+      store_quad<kAny>(out, at0 + i * p.N, 0, nn[i], make_float4(v0.x, v0.y, v1.x, v1.y));
+    }
+    const float4 sb = rows_sum(accb);
+    if (LOCAL) {
+      if (et == 0) store_quad<kAny>(p.dsum, j * p.C + ech, 0, en, sb);
+    } else {
+      const float4 sD = rows_sum(accD);
+      if (et == 0) {
+        store_quad<kAny>(out, (int64_t)p.C * p.N + ech, 0, en, sD);
+        store_quad<kAny>(out, (int64_t)p.C * (p.N + 1) + ech, 0, en, sb);
+      }
     }
   }
 }
@@ -377,23 +410,21 @@ __global__ void __launch_bounds__(256) state_scan_bc_kernel(const ScanParams p, 
   store(kind == 0 ? dB : dC, r * per + gn, p.bf16, s);
 }
 
-int tile_channels(int N) {
-  const int gm = lanes_for(N, 4);
-  return kWarps * (32 / gm) * (gm == 1 ? 1 : 2);
-}
+int tile_channels(int N) { return kThreads / lanes_for(N, 4) * kCPT; }
 
 void set_tiles(ScanParams& p) {
   p.tpg = (int)semx::cdiv(p.cpg, (int64_t)tile_channels(p.N));
   p.ctiles = p.G * p.tpg;
 }
 
+// Rows per piece (0: whole sequences): as in the forward, with two resident CTAs per SM.
+constexpr int64_t kResident = 148 * 2;
 int64_t bwd_rows_per_piece(const ScanParams& p) {
   const int64_t ctas = (int64_t)p.m.S * p.ctiles;
-  const int64_t rows = p.m.S > 0 ? p.m.T / p.m.S : 0;
-  if (ctas >= 148 * 2 || rows <= 64) return 0;
-  const int64_t cut = semx::cdiv((int64_t)148 * 4, ctas > 0 ? ctas : 1);
-  const int64_t Q = semx::cdiv(semx::cdiv(p.m.T, p.m.S * cut), kBlock) * kBlock;
-  return Q < 32 ? 32 : Q;
+  const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
+  if (2 * ctas > kResident || rows <= 128) return 0;
+  const int64_t Q = semx::cdiv(semx::cdiv(rows, kResident / ctas), kBlock) * kBlock;
+  return Q < 64 ? 64 : Q;
 }
 
 struct Layout {
@@ -424,9 +455,11 @@ int launch_bwd(const ScanParams& p, cudaStream_t st) {
   if (grid == 0) return SEMX_OK;
   if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan bwd: too many pieces");
   switch (gm) {
-#define SEMX_GM(V)                                                                       \
-  case V:                                                                                \
-    state_scan_bwd_kernel<V, LOCAL><<<(unsigned)grid, kThreads, 0, st>>>(p);             \
+#define SEMX_GM(V)                                                                                              \
+  case V:                                                                                                       \
+    if (p.access == kBf16) state_scan_bwd_kernel<V, LOCAL, kBf16><<<(unsigned)grid, kThreads, 0, st>>>(p);      \
+    else if (p.access == kFp32) state_scan_bwd_kernel<V, LOCAL, kFp32><<<(unsigned)grid, kThreads, 0, st>>>(p); \
+    else state_scan_bwd_kernel<V, LOCAL, kAny><<<(unsigned)grid, kThreads, 0, st>>>(p);                         \
     return semx::check_launch("state_scan_bwd_kernel");
     SEMX_GM(1)
     SEMX_GM(2)
