@@ -165,32 +165,31 @@ __device__ __forceinline__ float pole(float d, float A2) { return semx::ex2_appr
 
 __device__ __forceinline__ float sigmoid(float v) { return semx::rcp_approx(1.f + semx::ex2_approx(-kLog2e * v)); }
 
-// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|), of two values: log1p(e) / e on [0, 1]
-// is a degree 9 Chebyshev interpolant (5e-9 off, 1e-7 with its roundings); e is corrected for
-// the rounding of its argument, which small steps (v near -7) would show in full. Above 20
-// the logarithm is below half a step of v. e comes back for the derivative.
-__device__ __forceinline__ float2 softplus2(float a, float b, float2* exps = nullptr) {
-  constexpr float kLow = 1.925963033500e-8f;  // log2(e) - float(log2(e))
-  constexpr float kLn2 = 0.6931471805599453f;
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|): log1p(e) / e on [0, 1] is a degree 9
+// Chebyshev interpolant (5e-9 off, 1e-7 with its roundings); e is corrected for the rounding
+// of its argument, which small steps (v near -7) would show in full. Above 20 the logarithm
+// is below half a step of v. e comes back for the derivative.
+__device__ __forceinline__ float softplus(float v, float* exp_out = nullptr) {
   // exp(-150) is 0 in fp32; the bound keeps infinities out of the products below.
-  const f2 t = pack2(fmaxf(-fabsf(a), -150.f), fmaxf(-fabsf(b), -150.f)), l = pack2(kLog2e, kLog2e);
-  const f2 p = mul2(t, l);
-  const float2 pv = unpack2(p);
-  // What the product lost, and the constant's own tail.
-  const f2 lost = fma2(t, pack2(kLow, kLow), fma2(t, l, pack2(-pv.x, -pv.y)));
-  f2 e = pack2(semx::ex2_approx(pv.x), semx::ex2_approx(pv.y));
-  e = fma2(e, mul2(lost, pack2(kLn2, kLn2)), e);
-  if (exps != nullptr) *exps = unpack2(e);
-  constexpr float c[9] = {0.019542528316378593f, -0.05637361481785774f, 0.10543623566627502f, -0.1526966691017151f,
-                          0.1966327428817749f, -0.24951615929603577f, 0.33329710364341736f, -0.49999892711639404f, 1.0f};
-  f2 s = pack2(-0.0031760570127512695f, -0.0031760570127512695f);
-#pragma unroll
-  for (int i = 0; i < 9; ++i) s = fma2(s, e, pack2(c[i], c[i]));
-  return unpack2(fma2(s, e, pack2(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b)));  // a NaN stays
+  const float t = fmaxf(-fabsf(v), -150.f), p = t * kLog2e;
+  // What the product lost, and the constant's own tail log2(e) - float(log2(e)).
+  const float lost = fmaf(t, 1.925963033500e-8f, fmaf(t, kLog2e, -p));
+  float e = semx::ex2_approx(p);
+  e = fmaf(e, lost * 0.6931471805599453f, e);
+  if (exp_out != nullptr) *exp_out = e;
+  float s = fmaf(-0.0031760570127512695f, e, 0.019542528316378593f);
+  s = fmaf(s, e, -0.05637361481785774f);
+  s = fmaf(s, e, 0.10543623566627502f);
+  s = fmaf(s, e, -0.1526966691017151f);
+  s = fmaf(s, e, 0.1966327428817749f);
+  s = fmaf(s, e, -0.24951615929603577f);
+  s = fmaf(s, e, 0.33329710364341736f);
+  s = fmaf(s, e, -0.49999892711639404f);
+  s = fmaf(s, e, 1.0f);
+  return fmaf(s, e, v < 0.f ? 0.f : v);  // a NaN stays
 }
 __device__ __forceinline__ float4 softplus4(float4 v) {
-  const float2 a = softplus2(v.x, v.y), b = softplus2(v.z, v.w);
-  return make_float4(a.x, a.y, b.x, b.y);
+  return make_float4(softplus(v.x), softplus(v.y), softplus(v.z), softplus(v.w));
 }
 // softplus' = 1 / (1 + exp(-v)) from e = exp(-|v|).
 __device__ __forceinline__ float softplus_slope(float v, float e) {

@@ -62,8 +62,26 @@ __device__ __forceinline__ void halve_sum(float (&v)[NV], int lane) {
   }
 }
 
+template <int GM, bool LOCAL>
+struct BwdShared {
+  static constexpr int CH = channels_per_cta<GM>(), R = LOCAL ? 1 : kBlock;
+  static constexpr int TS = kThreads / (CH / 4), E = (kBlock + TS - 1) / TS;
+  float4 sd[kBlock][CH / 2];  // (d, d', d x, d' x') of two channels
+  float2 sv[kBlock][CH / 2];  // (dv, dv')
+  float4 sC[kBlock][GM];
+  float4 sB[R][LOCAL ? 1 : GM];
+  float so[R][LOCAL ? 4 : 2 * CH];                       // (gB, uA) per channel
+  float4 sw[LOCAL ? 1 : kWarps][R][LOCAL ? 1 : 2 * GM];  // dB | dC of a warp
+  float4 spar[2][CH / 4];             // dt_bias and D of the CTA's channels
+  // Values that a thread leaves for itself: its sums for dD and ddt_bias, softplus' of its
+  // rows, its states in front of the block.
+  float4 sums[2][kThreads];
+  float4 sg[LOCAL ? 1 : E][LOCAL ? 1 : kThreads];
+  float4 sh[LOCAL ? 1 : kCPT][LOCAL ? 1 : kThreads];
+};
+
 template <int GM, bool LOCAL, int ACC>
-__global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_scan_bwd_kernel(const ScanParams p) {
   constexpr int CL = 32 / GM, CH = channels_per_cta<GM>(), NP = 4 * GM;
   constexpr int TS = kThreads / (CH / 4);       // rows that the CTA loads at a time
   constexpr int E = (kBlock + TS - 1) / TS;     // (step, four channels) of a thread
@@ -71,14 +89,21 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
   constexpr int EB = (kBlock + ML - 1) / ML;    // (step, four modes) of a thread
   constexpr int NV1 = 2 * kCPT, NO1 = NV1 / GM > 0 ? NV1 / GM : 1;
   constexpr int NO2 = 8 / CL > 0 ? 8 / CL : 1;
+  constexpr int HALF = kBlock / 2;
   typedef typename RawQuad<ACC>::type Quad;
-  __shared__ __align__(16) float4 sd[kBlock][CH / 2];  // (d, d', d x, d' x') of two channels
-  __shared__ __align__(16) float2 sv[kBlock][CH / 2];  // (dv, dv')
-  __shared__ __align__(16) float4 sB[LOCAL ? 1 : kBlock][LOCAL ? 1 : GM];
-  __shared__ __align__(16) float4 sC[kBlock][GM];
-  __shared__ __align__(16) float so[LOCAL ? 1 : kBlock][LOCAL ? 4 : 2 * CH];        // (gB, uA) per channel
-  __shared__ float sw[LOCAL ? 1 : kWarps][LOCAL ? 1 : kBlock][LOCAL ? 1 : 2 * NP];  // dB | dC of a warp
-  __shared__ __align__(16) float4 red[kThreads];
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  typedef BwdShared<GM, LOCAL> Shared;
+  Shared& sm = *reinterpret_cast<Shared*>(raw_smem);
+  auto& sd = sm.sd;
+  auto& sv = sm.sv;
+  auto& sC = sm.sC;
+  auto& sB = sm.sB;
+  auto& so = sm.so;
+  auto& sw = sm.sw;
+  auto& spar = sm.spar;
+  auto& sums = sm.sums;
+  auto& sg = sm.sg;
+  auto& sh = sm.sh;
 
   const int64_t j = blockIdx.x / p.ctiles;
   const int ct = blockIdx.x % p.ctiles;
@@ -87,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
 
   // The four channels of this thread in loads and stores (en of them exist).
-  const int ec = tid % (CH / 4) * 4, et = tid / (CH / 4);
+  const int eq = tid % (CH / 4), ec = eq * 4, et = tid / (CH / 4);
   const int en = min(4, p.cpg - cg0 - ec);
   const int64_t ech = c_base + (en > 0 ? cg0 + ec : 0);
   const bool has_z = p.z != nullptr;
@@ -104,35 +129,47 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
   const int cp = warp * CL + cl, sc = cp * kCPT;
   int nn[kCPT];  // modes of the channel that this thread holds
   const int64_t at0 = (int64_t)(c_base + cg0 + sc) * p.N + n0;  // (channel, first mode) of an array (C, N)
-  float A2[kCPT][4];
-  f2 dA[kCPT][2], carry[kCPT][2];
+  f2 A2[kCPT][2], dA[kCPT][2], carry[kCPT][2];
 #pragma unroll
   for (int i = 0; i < kCPT; ++i) {
     nn[i] = cg0 + sc + i < p.cpg ? min(4, p.N - n0) : 0;
     const float4 a = load_params(p.A, at0 + i * p.N, nn[i]);
-    A2[i][0] = a.x * kLog2e; A2[i][1] = a.y * kLog2e; A2[i][2] = a.z * kLog2e; A2[i][3] = a.w * kLog2e;
+    A2[i][0] = pack2(a.x * kLog2e, a.y * kLog2e);
+    A2[i][1] = pack2(a.z * kLog2e, a.w * kLog2e);
     float4 s = zero4;
     if (!LOCAL && q.live) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
     carry[i][0] = pack2(s.x, s.y);
     carry[i][1] = pack2(s.z, s.w);
     dA[i][0] = dA[i][1] = 0ull;
   }
-  const float4 bias = load_params(p.dt_bias, ech, en);
-  const float4 D = load_params(p.D, ech, en);
-  float4 accD = zero4, accb = zero4;  // LOCAL: accb is the sum of the steps
+  if (et == 0) {
+    spar[0][eq] = load_params(p.dt_bias, ech, en);
+    spar[1][eq] = load_params(p.D, ech, en);
+  }
+  sums[0][tid] = sums[1][tid] = zero4;  // LOCAL: the second is the sum of the steps
+  __syncthreads();
   const bool mode_quads = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.ckpt) & 15) == 0;
+  const bool bc_quads = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.pBC) & 15) == 0;
+  auto poles = [&](float d, f2 A) {
+    const float2 a = unpack2(A);
+    return pack2(pole(d, a.x), pole(d, a.y));
+  };
+  auto drive = [&](float dx, f2 B) {
+    const float2 b = unpack2(B);
+    return pack2(dx * b.x, dx * b.y);
+  };
 
+  const int tl = q.t1 > q.t0 ? q.t0 + (q.t1 - 1 - q.t0) / kBlock * kBlock : q.t0 - kBlock;
+  const int tb0 = tid / GM, bl = tid % GM, bn = min(4, p.N - bl * 4);
+  const float* ck = LOCAL || !q.live ? nullptr : p.ckpt + (piece_base(p.m, q.s, kBlock) + tl / kBlock) * p.C * p.N + at0;
   Quad rx[E], rd[E], rg[E], rz[E], rv[E], rB[EB], rC[EB];
   float4 hn[kCPT];
-  const int64_t blk0 = q.live ? piece_base(p.m, q.s, kBlock) : 0;
-  const int tb0 = tid / GM, bl = tid % GM, bn = min(4, p.N - bl * 4);
-  auto fetch = [&](int t0) {
+  auto fetch = [&](int t0, int rows) {  // rows of the tile that exist
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       rx[i] = rd[i] = rg[i] = rz[i] = rv[i] = Quad{};
-      const int t = et + i * TS;
-      if (en > 0 && t < kBlock && t0 + t < q.t1) {
-        const int64_t r = q.row0 + t0 + t;
+      if (en > 0 && et + i * TS < rows) {
+        const int64_t r = q.row0 + t0 + et + i * TS;
         rd[i] = load_quad<ACC>(p.dt, r * p.lddt + ech, p.dt_bf16, en);
         rg[i] = load_quad<ACC>(p.dy, r * p.C + ech, p.bf16, en);
         if (has_z) rz[i] = load_quad<ACC>(p.z, r * p.ldz + ech, p.bf16, en);
@@ -145,49 +182,47 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
 #pragma unroll
     for (int i = 0; i < EB; ++i) {
       rB[i] = rC[i] = Quad{};
-      const int t = tb0 + i * ML;
-      if (bn > 0 && t < kBlock && t0 + t < q.t1) {
-        const int64_t r = q.row0 + t0 + t;
-        if (!LOCAL) rB[i] = load_quad<ACC>(p.B, r * p.ldb + (int64_t)grp * p.N + bl * 4, p.bf16, bn);
-        rC[i] = load_quad<ACC>(p.Cm, r * p.ldc + (int64_t)grp * p.N + bl * 4, p.bf16, bn);
+      if (bn > 0 && tb0 + i * ML < rows) {
+        const int64_t r = q.row0 + t0 + tb0 + i * ML, b = (int64_t)grp * p.N + bl * 4;
+        if (!LOCAL) rB[i] = load_quad<ACC>(p.B, r * p.ldb + b, p.bf16, bn);
+        rC[i] = load_quad<ACC>(p.Cm, r * p.ldc + b, p.bf16, bn);
       }
     }
     if (!LOCAL) {
 #pragma unroll
       for (int i = 0; i < kCPT; ++i) {
-        const float* c = p.ckpt + (blk0 + t0 / kBlock) * p.C * p.N;
         hn[i] = zero4;
         if (mode_quads) {
-          if (nn[i] > 0) hn[i] = *reinterpret_cast<const float4*>(c + at0 + i * p.N);
+          if (nn[i] > 0) hn[i] = *reinterpret_cast<const float4*>(ck + i * p.N);
         } else {
-          hn[i] = load_params(c, at0 + i * p.N, nn[i]);
+          hn[i] = load_params(ck, i * p.N, nn[i]);
         }
       }
+      ck -= (int64_t)p.C * p.N;
     }
   };
 
-  const int tl = q.t1 > q.t0 ? q.t0 + (q.t1 - 1 - q.t0) / kBlock * kBlock : q.t0 - kBlock;
-  if (tl >= q.t0) fetch(tl);
+  if (tl >= q.t0) fetch(tl, min(kBlock, q.t1 - tl));
 #pragma unroll 1
   for (int t0 = tl; t0 >= q.t0; t0 -= kBlock) {
     const int nt = min(kBlock, q.t1 - t0);
-    float4 sg[E];  // softplus'
-    Quad kx[E];    // x
+    Quad kx[E];  // x
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int t = et + i * TS;
       if (t < kBlock) {
         const bool in = t < nt && en > 0;
+        const float4 bias = spar[0][eq];
         float4 d = quad_floats<ACC>(rd[i], p.dt_bf16), g = quad_floats<ACC>(rg[i], p.bf16);
         d.x += bias.x; d.y += bias.y; d.z += bias.z; d.w += bias.w;
-        sg[i] = make_float4(1.f, 1.f, 1.f, 1.f);
+        float4 slope = make_float4(1.f, 1.f, 1.f, 1.f);
         if (p.softplus) {
-          float2 e0, e1;
-          const float2 a = softplus2(d.x, d.y, &e0), b = softplus2(d.z, d.w, &e1);
+          float4 e;
+          const float4 raw = d;
+          d = make_float4(softplus(raw.x, &e.x), softplus(raw.y, &e.y), softplus(raw.z, &e.z), softplus(raw.w, &e.w));
           if (!LOCAL)
-            sg[i] = make_float4(softplus_slope(d.x, e0.x), softplus_slope(d.y, e0.y), softplus_slope(d.z, e1.x),
-                                softplus_slope(d.w, e1.y));
-          d = make_float4(a.x, a.y, b.x, b.y);
+            slope = make_float4(softplus_slope(raw.x, e.x), softplus_slope(raw.y, e.y), softplus_slope(raw.z, e.z),
+                                softplus_slope(raw.w, e.w));
         }
         if (has_z) {
           const float4 z = quad_floats<ACC>(rz[i], p.bf16);
@@ -204,12 +239,16 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
         }
         if (!in) d = g = zero4;  // a row behind the piece: pole 1, no drive, no gradient
         const float4 x = LOCAL ? zero4 : quad_floats<ACC>(rx[i], p.bf16);
-        sd[t][ec / 2] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
-        sd[t][ec / 2 + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
-        *reinterpret_cast<float4*>(&sv[t][ec / 2]) = g;
-        kx[i] = rx[i];
-        if (LOCAL) {
-          accb.x += d.x; accb.y += d.y; accb.z += d.z; accb.w += d.w;
+        sd[t][2 * eq] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
+        sd[t][2 * eq + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
+        *reinterpret_cast<float4*>(&sv[t][2 * eq]) = g;
+        if (!LOCAL) {
+          kx[i] = rx[i];
+          sg[i][tid] = slope;
+        } else {
+          float4 s = sums[1][tid];
+          s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
+          sums[1][tid] = s;
         }
       }
     }
@@ -220,85 +259,116 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
         sC[tb0 + i * ML][bl] = quad_floats<ACC>(rC[i], p.bf16);
       }
     }
-    f2 a[kBlock][kCPT][2], h[kBlock + 1][kCPT][2];
     if (!LOCAL) {
 #pragma unroll
-      for (int i = 0; i < kCPT; ++i) {
-        h[0][i][0] = pack2(hn[i].x, hn[i].y);
-        h[0][i][1] = pack2(hn[i].z, hn[i].w);
-      }
+      for (int i = 0; i < kCPT; ++i) sh[i][tid] = hn[i];
     }
     __syncthreads();
-    if (t0 - kBlock >= q.t0) fetch(t0 - kBlock);
+    if (t0 - kBlock >= q.t0) fetch(t0 - kBlock, kBlock);
+
+    // The later half of the block first: its entry state is a run over the earlier half,
+    // whose poles and states are rebuilt afterwards. Half of a block's values in registers
+    // leave room for three CTAs per SM.
+#pragma unroll 1
+    for (int tb = HALF; tb >= 0; tb -= HALF) {
+      f2 a[HALF][kCPT][2], h[HALF + 1][kCPT][2];
+      if (!LOCAL) {
 #pragma unroll
-    for (int t = 0; t < kBlock; ++t) {
-      const float4 d = sd[t][cp];
-      float4 B = zero4;
-      if (!LOCAL) B = sB[t][lm];
+        for (int i = 0; i < kCPT; ++i) {
+          const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&sh[i][tid]);
+          h[0][i][0] = e.x;
+          h[0][i][1] = e.y;
+        }
+        if (tb > 0) {
 #pragma unroll
-      for (int i = 0; i < kCPT; ++i) {
-        const float dd = i == 0 ? d.x : d.y, dx = i == 0 ? d.z : d.w;
-        a[t][i][0] = pack2(pole(dd, A2[i][0]), pole(dd, A2[i][1]));
-        a[t][i][1] = pack2(pole(dd, A2[i][2]), pole(dd, A2[i][3]));
-        if (!LOCAL) {
-          h[t + 1][i][0] = fma2(a[t][i][0], h[t][i][0], pack2(dx * B.x, dx * B.y));
-          h[t + 1][i][1] = fma2(a[t][i][1], h[t][i][1], pack2(dx * B.z, dx * B.w));
+          for (int t = 0; t < HALF; ++t) {
+            const float4 d = sd[t][cp];
+            const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sB[t][lm]);
+#pragma unroll
+            for (int i = 0; i < kCPT; ++i) {
+              const float dd = i == 0 ? d.x : d.y, dx = i == 0 ? d.z : d.w;
+              h[0][i][0] = fma2(poles(dd, A2[i][0]), h[0][i][0], drive(dx, B.x));
+              h[0][i][1] = fma2(poles(dd, A2[i][1]), h[0][i][1], drive(dx, B.y));
+            }
+          }
         }
       }
-    }
 #pragma unroll
-    for (int t = kBlock - 1; t >= 0; --t) {
-      const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sC[t][lm]);
-      const float2 vv = sv[t][cp];
-      if (LOCAL) {
+      for (int t = 0; t < HALF; ++t) {
+        const float4 d = sd[tb + t][cp];
 #pragma unroll
         for (int i = 0; i < kCPT; ++i) {
-          const f2 v = i == 0 ? pack2(vv.x, vv.x) : pack2(vv.y, vv.y);
-          carry[i][0] = mul2(a[t][i][0], fma2(C.x, v, carry[i][0]));
-          carry[i][1] = mul2(a[t][i][1], fma2(C.y, v, carry[i][1]));
+          const float dd = i == 0 ? d.x : d.y;
+          a[t][i][0] = poles(dd, A2[i][0]);
+          a[t][i][1] = poles(dd, A2[i][1]);
         }
-      } else {
-        const float4 d4 = sd[t][cp];
-        const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sB[t][lm]);
-        float v1[NV1], v2[8];
-        f2 b0 = 0ull, b1 = 0ull, c0 = 0ull, c1 = 0ull;
+        if (!LOCAL) {
+          const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sB[tb + t][lm]);
 #pragma unroll
-        for (int i = 0; i < kCPT; ++i) {
-          const f2 v = i == 0 ? pack2(vv.x, vv.x) : pack2(vv.y, vv.y);
-          const f2 d = i == 0 ? pack2(d4.x, d4.x) : pack2(d4.y, d4.y);
-          const f2 dx = i == 0 ? pack2(d4.z, d4.z) : pack2(d4.w, d4.w);
-          const f2 g0 = fma2(C.x, v, carry[i][0]), g1 = fma2(C.y, v, carry[i][1]);
-          carry[i][0] = mul2(a[t][i][0], g0);
-          carry[i][1] = mul2(a[t][i][1], g1);
-          const f2 u0 = mul2(carry[i][0], h[t][i][0]), u1 = mul2(carry[i][1], h[t][i][1]);
-          const float2 gB = unpack2(fma2(g1, B.y, mul2(g0, B.x)));
-          const float2 uA = unpack2(fma2(u1, pack2(A2[i][2], A2[i][3]), mul2(u0, pack2(A2[i][0], A2[i][1]))));
-          v1[2 * i] = gB.x + gB.y;
-          v1[2 * i + 1] = uA.x + uA.y;
-          dA[i][0] = fma2(u0, d, dA[i][0]);
-          dA[i][1] = fma2(u1, d, dA[i][1]);
-          b0 = i == 0 ? mul2(g0, dx) : fma2(g0, dx, b0);
-          b1 = i == 0 ? mul2(g1, dx) : fma2(g1, dx, b1);
-          c0 = i == 0 ? mul2(h[t + 1][i][0], v) : fma2(h[t + 1][i][0], v, c0);
-          c1 = i == 0 ? mul2(h[t + 1][i][1], v) : fma2(h[t + 1][i][1], v, c1);
+          for (int i = 0; i < kCPT; ++i) {
+            const float dx = i == 0 ? d.z : d.w;
+            h[t + 1][i][0] = fma2(a[t][i][0], h[t][i][0], drive(dx, B.x));
+            h[t + 1][i][1] = fma2(a[t][i][1], h[t][i][1], drive(dx, B.y));
+          }
         }
-        const float2 e0 = unpack2(b0), e1 = unpack2(b1), e2 = unpack2(c0), e3 = unpack2(c1);
-        v2[0] = e0.x; v2[1] = e0.y; v2[2] = e1.x; v2[3] = e1.y;
-        v2[4] = e2.x; v2[5] = e2.y; v2[6] = e3.x; v2[7] = e3.y;
-        halve_sum<NV1, GM, 1>(v1, lane);
-        halve_sum<8, CL, GM>(v2, lane);
-        // Value k of (channel, {gB, uA}) is float 2 sc + k of the step's row.
-        constexpr int SPARE1 = GM > NV1 ? GM / NV1 : 1;
-        if (lm % SPARE1 == 0) {
+      }
 #pragma unroll
-          for (int k = 0; k < NO1; ++k) so[t][2 * sc + lm / SPARE1 * NO1 + k] = v1[k];
-        }
-        constexpr int SPARE2 = CL > 8 ? CL / 8 : 1;
-        if (cl % SPARE2 == 0) {
+      for (int t = HALF - 1; t >= 0; --t) {
+        // The compiler would load all steps' operands ahead and spill.
+        asm volatile("" ::: "memory");
+        const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sC[tb + t][lm]);
+        const float2 vv = sv[tb + t][cp];
+        if (LOCAL) {
 #pragma unroll
-          for (int k = 0; k < NO2; ++k) {
-            const int id = cl / SPARE2 * NO2 + k;  // (dB, dC) x 4 modes
-            sw[warp][t][(id / 4) * NP + n0 + id % 4] = v2[k];
+          for (int i = 0; i < kCPT; ++i) {
+            const f2 v = i == 0 ? pack2(vv.x, vv.x) : pack2(vv.y, vv.y);
+            carry[i][0] = mul2(a[t][i][0], fma2(C.x, v, carry[i][0]));
+            carry[i][1] = mul2(a[t][i][1], fma2(C.y, v, carry[i][1]));
+          }
+        } else {
+          const float4 d4 = sd[tb + t][cp];
+          const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sB[tb + t][lm]);
+          float v1[NV1], v2[8];
+          f2 b0 = 0ull, b1 = 0ull, c0 = 0ull, c1 = 0ull;
+#pragma unroll
+          for (int i = 0; i < kCPT; ++i) {
+            const f2 v = i == 0 ? pack2(vv.x, vv.x) : pack2(vv.y, vv.y);
+            const f2 d = i == 0 ? pack2(d4.x, d4.x) : pack2(d4.y, d4.y);
+            const f2 dx = i == 0 ? pack2(d4.z, d4.z) : pack2(d4.w, d4.w);
+            const f2 g0 = fma2(C.x, v, carry[i][0]), g1 = fma2(C.y, v, carry[i][1]);
+            carry[i][0] = mul2(a[t][i][0], g0);
+            carry[i][1] = mul2(a[t][i][1], g1);
+            const f2 u0 = mul2(carry[i][0], h[t][i][0]), u1 = mul2(carry[i][1], h[t][i][1]);
+            const float2 gB = unpack2(fma2(g1, B.y, mul2(g0, B.x)));
+            const float2 uA = unpack2(fma2(u1, A2[i][1], mul2(u0, A2[i][0])));
+            v1[2 * i] = gB.x + gB.y;
+            v1[2 * i + 1] = uA.x + uA.y;
+            dA[i][0] = fma2(u0, d, dA[i][0]);
+            dA[i][1] = fma2(u1, d, dA[i][1]);
+            b0 = i == 0 ? mul2(g0, dx) : fma2(g0, dx, b0);
+            b1 = i == 0 ? mul2(g1, dx) : fma2(g1, dx, b1);
+            c0 = i == 0 ? mul2(h[t + 1][i][0], v) : fma2(h[t + 1][i][0], v, c0);
+            c1 = i == 0 ? mul2(h[t + 1][i][1], v) : fma2(h[t + 1][i][1], v, c1);
+          }
+          const float2 e0 = unpack2(b0), e1 = unpack2(b1), e2 = unpack2(c0), e3 = unpack2(c1);
+          v2[0] = e0.x; v2[1] = e0.y; v2[2] = e1.x; v2[3] = e1.y;
+          v2[4] = e2.x; v2[5] = e2.y; v2[6] = e3.x; v2[7] = e3.y;
+          halve_sum<NV1, GM, 1>(v1, lane);
+          halve_sum<8, CL, GM>(v2, lane);
+          // Value k of (channel, {gB, uA}) is float 2 sc + k of the step's row.
+          constexpr int SPARE1 = GM > NV1 ? GM / NV1 : 1;
+          if (lm % SPARE1 == 0) {
+#pragma unroll
+            for (int k = 0; k < NO1; ++k) so[tb + t][2 * sc + lm / SPARE1 * NO1 + k] = v1[k];
+          }
+          constexpr int SPARE2 = CL > 8 ? CL / 8 : 1;
+          if (cl % SPARE2 == 0) {
+            float* w = reinterpret_cast<float*>(sw[warp][tb + t]);
+#pragma unroll
+            for (int k = 0; k < NO2; ++k) {
+              const int id = cl / SPARE2 * NO2 + k;  // (dB, dC) x 4 modes
+              w[(id / 4) * NP + n0 + id % 4] = v2[k];
+            }
           }
         }
       }
@@ -313,64 +383,63 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : 2) state_scan_bwd_kernel
           const float4 s0 = *reinterpret_cast<const float4*>(&so[t][2 * ec]);
           const float4 s1 = *reinterpret_cast<const float4*>(&so[t][2 * ec + 4]);
           // d and dv as this thread put them there.
-          const float4 x = quad_floats<ACC>(kx[i], p.bf16), k = sg[i];
-          const float4 g = *reinterpret_cast<const float4*>(&sv[t][ec / 2]);
-          const float2 d01 = *reinterpret_cast<const float2*>(&sd[t][ec / 2]);
-          const float2 d23 = *reinterpret_cast<const float2*>(&sd[t][ec / 2 + 1]);
-          const float4 d = make_float4(d01.x, d01.y, d23.x, d23.y);
+          const float4 x = quad_floats<ACC>(kx[i], p.bf16), k = sg[i][tid], D = spar[1][eq];
+          const float4 g = *reinterpret_cast<const float4*>(&sv[t][2 * eq]);
+          const float2 d01 = *reinterpret_cast<const float2*>(&sd[t][2 * eq]);
+          const float2 d23 = *reinterpret_cast<const float2*>(&sd[t][2 * eq + 1]);
           store_quad<ACC>(p.dx, o, p.bf16, en,
-                          make_float4(fmaf(d.x, s0.x, D.x * g.x), fmaf(d.y, s0.z, D.y * g.y),
-                                      fmaf(d.z, s1.x, D.z * g.z), fmaf(d.w, s1.z, D.w * g.w)));
+                          make_float4(fmaf(d01.x, s0.x, D.x * g.x), fmaf(d01.y, s0.z, D.y * g.y),
+                                      fmaf(d23.x, s1.x, D.z * g.z), fmaf(d23.y, s1.z, D.w * g.w)));
           const float4 ddt = make_float4(fmaf(s0.y, kLn2, x.x * s0.x) * k.x, fmaf(s0.w, kLn2, x.y * s0.z) * k.y,
                                          fmaf(s1.y, kLn2, x.z * s1.x) * k.z, fmaf(s1.w, kLn2, x.w * s1.z) * k.w);
           store_quad<ACC>(p.ddt, o, p.dt_bf16, en, ddt);
-          accb.x += ddt.x; accb.y += ddt.y; accb.z += ddt.z; accb.w += ddt.w;
-          accD.x = fmaf(g.x, x.x, accD.x); accD.y = fmaf(g.y, x.y, accD.y);
-          accD.z = fmaf(g.z, x.z, accD.z); accD.w = fmaf(g.w, x.w, accD.w);
+          float4 sD = sums[0][tid], sb = sums[1][tid];
+          sD.x = fmaf(g.x, x.x, sD.x); sD.y = fmaf(g.y, x.y, sD.y);
+          sD.z = fmaf(g.z, x.z, sD.z); sD.w = fmaf(g.w, x.w, sD.w);
+          sb.x += ddt.x; sb.y += ddt.y; sb.z += ddt.z; sb.w += ddt.w;
+          sums[0][tid] = sD;
+          sums[1][tid] = sb;
         }
       }
-      for (int e = tid; e < nt * 2 * NP; e += kThreads) {
-        const int t = e / (2 * NP), v = e % (2 * NP), n = v % NP;
-        if (n < p.N) {
-          float s = 0.f;
+      // dB | dC of the CTA's channels: the warps' sums in order.
+      for (int e = tid; e < nt * 2 * GM; e += kThreads) {
+        const int t = e / (2 * GM), v = e % (2 * GM), n = v % GM * 4;
+        float4 s = sw[0][t][v];
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) s += sw[w][t][v];
-          p.pBC[((int64_t)ct * p.m.T + q.row0 + t0 + t) * 2 * p.N + (v / NP) * p.N + n] = s;
+        for (int w = 1; w < kWarps; ++w) {
+          const float4 o = sw[w][t][v];
+          s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+        }
+        const int64_t o = ((int64_t)ct * p.m.T + q.row0 + t0 + t) * 2 * p.N + (v / GM) * p.N + n;
+        if (bc_quads) {
+          if (n < p.N) *reinterpret_cast<float4*>(p.pBC + o) = s;
+        } else {
+          store_quad<kAny>(p.pBC, o, 0, min(4, p.N - n), s);
         }
       }
     }
   }
-  // Sum over the threads of four channels, in order of their rows.
-  auto rows_sum = [&](float4 v) {
-    __syncthreads();
-    red[tid] = v;
-    __syncthreads();
-    float4 s = zero4;
-    if (et == 0)
-      for (int i = 0; i < TS; ++i) {
-        const float4 d = red[i * (CH / 4) + tid];
-        s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
-      }
-    return s;
-  };
   if (LOCAL && !q.live) return;
   float* out = LOCAL ? p.entry + j * p.C * p.N : p.part != nullptr ? p.part + j * ((int64_t)p.C * (p.N + 2)) : nullptr;
-  if (out != nullptr) {
-    // Without LOCAL every piece index writes its row, zeros where there is no such piece.
+  if (out == nullptr) return;
+  // Without LOCAL every piece index writes its row, zeros where there is no such piece.
 #pragma unroll
-    for (int i = 0; i < kCPT; ++i) {
-      const float2 v0 = unpack2(LOCAL ? carry[i][0] : dA[i][0]), v1 = unpack2(LOCAL ? carry[i][1] : dA[i][1]);
-      store_quad<kAny>(out, at0 + i * p.N, 0, nn[i], make_float4(v0.x, v0.y, v1.x, v1.y));
-    }
-    const float4 sb = rows_sum(accb);
-    if (LOCAL) {
-      if (et == 0) store_quad<kAny>(p.dsum, j * p.C + ech, 0, en, sb);
-    } else {
-      const float4 sD = rows_sum(accD);
-      if (et == 0) {
-        store_quad<kAny>(out, (int64_t)p.C * p.N + ech, 0, en, sD);
-        store_quad<kAny>(out, (int64_t)p.C * (p.N + 1) + ech, 0, en, sb);
+  for (int i = 0; i < kCPT; ++i) {
+    const float2 v0 = unpack2(LOCAL ? carry[i][0] : dA[i][0]), v1 = unpack2(LOCAL ? carry[i][1] : dA[i][1]);
+    store_quad<kAny>(out, at0 + i * p.N, 0, nn[i], make_float4(v0.x, v0.y, v1.x, v1.y));
+  }
+  // The threads of four channels in order of their rows.
+  __syncthreads();
+  if (et == 0) {
+#pragma unroll
+    for (int k = LOCAL ? 1 : 0; k < 2; ++k) {
+      float4 s = sums[k][tid];
+      for (int i = 1; i < TS; ++i) {
+        const float4 d = sums[k][i * (CH / 4) + tid];
+        s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
       }
+      if (LOCAL) store_quad<kAny>(p.dsum, j * p.C + ech, 0, en, s);
+      else store_quad<kAny>(out, (int64_t)p.C * (p.N + k) + ech, 0, en, s);
     }
   }
 }
@@ -410,15 +479,17 @@ __global__ void __launch_bounds__(256) state_scan_bc_kernel(const ScanParams p, 
   store(kind == 0 ? dB : dC, r * per + gn, p.bf16, s);
 }
 
-int tile_channels(int N) { return kThreads / lanes_for(N, 4) * kCPT; }
+// At least two lanes per channel: the tiles of one would not fit shared memory.
+int mode_lanes(int N) { return lanes_for(N, 4) < 2 ? 2 : lanes_for(N, 4); }
+int tile_channels(int N) { return kThreads / mode_lanes(N) * kCPT; }
 
 void set_tiles(ScanParams& p) {
   p.tpg = (int)semx::cdiv(p.cpg, (int64_t)tile_channels(p.N));
   p.ctiles = p.G * p.tpg;
 }
 
-// Rows per piece (0: whole sequences): as in the forward, with two resident CTAs per SM.
-constexpr int64_t kResident = 148 * 2;
+// Rows per piece (0: whole sequences): as in the forward, with three resident CTAs per SM.
+constexpr int64_t kResident = 148 * 3;
 int64_t bwd_rows_per_piece(const ScanParams& p) {
   const int64_t ctas = (int64_t)p.m.S * p.ctiles;
   const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
@@ -434,34 +505,41 @@ Layout layout(const ScanParams& p, int64_t Q) {
   Layout l = {};
   const size_t pieces = (size_t)p.m.pieces;
   size_t at = 0;
+  // Every part starts on 16 bytes of the workspace.
+  auto up = [](size_t n) { return (n + 3) / 4 * 4; };
   l.entry = at;
-  at += Q > 0 ? pieces * p.C * p.N : 0;
+  at += Q > 0 ? up(pieces * p.C * p.N) : 0;
   l.dsum = at;
-  at += Q > 0 ? pieces * p.C : 0;
+  at += Q > 0 ? up(pieces * p.C) : 0;
   l.pbc = at;
-  at += (size_t)p.ctiles * p.m.T * 2 * p.N;
+  at += up((size_t)p.ctiles * p.m.T * 2 * p.N);
   l.part = at;
-  at += pieces * p.C * (p.N + 2);
+  at += up(pieces * p.C * (p.N + 2));
   l.groups = at;
   at += semx::colsum_group_floats(p.m.pieces, (int64_t)p.C * (p.N + 2));
   l.total = at;
   return l;
 }
 
+template <int GM, bool LOCAL, int ACC>
+int launch_one(const ScanParams& p, unsigned grid, cudaStream_t st) {
+  constexpr size_t bytes = sizeof(BwdShared<GM, LOCAL>);
+  if (!semx::allow_smem(state_scan_bwd_kernel<GM, LOCAL, ACC>, bytes)) return SEMX_ERR_LAUNCH;
+  state_scan_bwd_kernel<GM, LOCAL, ACC><<<grid, kThreads, bytes, st>>>(p);
+  return semx::check_launch("state_scan_bwd_kernel");
+}
+
 template <bool LOCAL>
 int launch_bwd(const ScanParams& p, cudaStream_t st) {
-  const int gm = lanes_for(p.N, 4);
   const int64_t grid = p.m.pieces * p.ctiles;
   if (grid == 0) return SEMX_OK;
   if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan bwd: too many pieces");
-  switch (gm) {
-#define SEMX_GM(V)                                                                                              \
-  case V:                                                                                                       \
-    if (p.access == kBf16) state_scan_bwd_kernel<V, LOCAL, kBf16><<<(unsigned)grid, kThreads, 0, st>>>(p);      \
-    else if (p.access == kFp32) state_scan_bwd_kernel<V, LOCAL, kFp32><<<(unsigned)grid, kThreads, 0, st>>>(p); \
-    else state_scan_bwd_kernel<V, LOCAL, kAny><<<(unsigned)grid, kThreads, 0, st>>>(p);                         \
-    return semx::check_launch("state_scan_bwd_kernel");
-    SEMX_GM(1)
+  switch (mode_lanes(p.N)) {
+#define SEMX_GM(V)                                                                        \
+  case V:                                                                                 \
+    if (p.access == kBf16) return launch_one<V, LOCAL, kBf16>(p, (unsigned)grid, st);     \
+    if (p.access == kFp32) return launch_one<V, LOCAL, kFp32>(p, (unsigned)grid, st);     \
+    return launch_one<V, LOCAL, kAny>(p, (unsigned)grid, st);
     SEMX_GM(2)
     SEMX_GM(4)
     SEMX_GM(8)

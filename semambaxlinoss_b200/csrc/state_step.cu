@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) state_step_kernel(const ScanParams p
 #pragma unroll
     for (int n = 0; n < 4; ++n) h[n] = !cold && n0 + n < p.N ? st[n] : 0.f;
   }
-  if (p.softplus) d = softplus2(d, d).x;
+  if (p.softplus) d = softplus(d);
   float v = 0.f;
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
