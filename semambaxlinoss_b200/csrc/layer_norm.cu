@@ -54,51 +54,58 @@ __device__ __forceinline__ int col(int t, int i) {
   return VEC ? ((i >> 3) * TPR + t) * 8 + (i & 7) : i * TPR + t;
 }
 
+// A thread's part of a row as it is stored: loaded a row ahead, converted when it is used.
+template <int V>
+struct RawRow {
+  uint4 q[2 * V];
+};
+
 template <int TPR, int V, bool VEC>
-__device__ __forceinline__ void load_row(const void* base, int64_t off, int bf16, int t, int d, float (&v)[8 * V]) {
+__device__ __forceinline__ void load_row(const void* base, int64_t off, int bf16, int t, int d, RawRow<V>& r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r.q);
   if (VEC) {
     if (bf16) {
-      uint4 q[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int c = col<TPR, VEC>(t, 8 * k);
-        q[k] = make_uint4(0, 0, 0, 0);
-        if (c < d) q[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + off + c);
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const uint32_t u[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[8 * k + 2 * j] = __uint_as_float(u[j] << 16);
-          v[8 * k + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-        }
+        r.q[k] = make_uint4(0, 0, 0, 0);
+        if (c < d) r.q[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + off + c);
       }
     } else {
-      float4 q[2 * V];
 #pragma unroll
       for (int k = 0; k < 2 * V; ++k) {
         const int c = col<TPR, VEC>(t, 4 * k);
-        q[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < d) q[k] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + off + c);
-      }
-#pragma unroll
-      for (int k = 0; k < 2 * V; ++k) {
-        v[4 * k] = q[k].x; v[4 * k + 1] = q[k].y; v[4 * k + 2] = q[k].z; v[4 * k + 3] = q[k].w;
+        r.q[k] = make_uint4(0, 0, 0, 0);
+        if (c < d) r.q[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + off + c);
       }
     }
   } else if (bf16) {
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) {
       const int c = col<TPR, VEC>(t, i);
-      v[i] = c < d ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[off + c]) : 0.f;
+      u[i] = c < d ? (uint32_t) reinterpret_cast<const unsigned short*>(base)[off + c] : 0u;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) {
       const int c = col<TPR, VEC>(t, i);
-      v[i] = c < d ? reinterpret_cast<const float*>(base)[off + c] : 0.f;
+      u[i] = c < d ? reinterpret_cast<const uint32_t*>(base)[off + c] : 0u;
     }
+  }
+}
+
+template <int V, bool VEC>
+__device__ __forceinline__ void to_floats(const RawRow<V>& r, int bf16, float (&v)[8 * V]) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(r.q);
+  if (VEC && bf16) {
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8 * V; ++i) v[i] = __uint_as_float(bf16 ? u[i] << 16 : u[i]);
   }
 }
 
@@ -138,6 +145,47 @@ __device__ __forceinline__ void store_row(void* base, int64_t off, int bf16, int
   }
 }
 
+// Parameters of the thread's 8 V columns (0 beyond the row, `none` where there is no parameter).
+template <int TPR, int V, bool VEC>
+__device__ __forceinline__ void load_param(const float* p, int t, int d, float none, float (&v)[8 * V]) {
+  if (VEC) {
+#pragma unroll
+    for (int k = 0; k < 2 * V; ++k) {
+      const int c = col<TPR, VEC>(t, 4 * k);
+      float4 q = make_float4(none, none, none, none);
+      if (p != nullptr) q = c < d ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[4 * k] = q.x; v[4 * k + 1] = q.y; v[4 * k + 2] = q.z; v[4 * k + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8 * V; ++i) {
+      const int c = col<TPR, VEC>(t, i);
+      v[i] = p == nullptr ? none : c < d ? p[c] : 0.f;
+    }
+  }
+}
+
+// Rows of at most 512 elements keep the parameters in registers from row to row; wider ones
+// read them again from L1, which leaves registers for two CTAs of 512 threads per SM.
+template <int TPR>
+constexpr bool keeps_params() {
+  return TPR <= 32;
+}
+// Whether the next row is loaded while this one is worked on: not where a thread's part of
+// a row is so long that it would spill.
+template <int TPR, int V>
+constexpr bool loads_ahead() {
+  return V <= 2 || TPR <= 32;
+}
+template <int TPR>
+constexpr int cta_threads() {
+  return TPR < 128 ? 128 : TPR;
+}
+template <int TPR, int V>
+constexpr int ctas_per_sm() {
+  return TPR < 128 ? 4 : TPR * V <= 1024 ? 1024 / (TPR * V) : 1;
+}
+
 template <int W>
 __device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
@@ -157,7 +205,7 @@ __device__ __forceinline__ int warp_count(int q, int d) {
 }
 
 template <int TPR, int V, bool VEC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_fwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(cta_threads<TPR>(), ctas_per_sm<TPR, V>()) layer_norm_fwd_kernel(const LnParams p) {
   constexpr int NT = TPR < 128 ? 128 : TPR;
   constexpr int ROWS = NT / TPR;
   constexpr int LW = TPR < 32 ? TPR : 32;  // lanes of a warp that share a row
@@ -165,24 +213,35 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_fwd_kernel(c
   __shared__ float2 red[2][WPR];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, d = p.d;
   float w[8 * V], b[8 * V];
-#pragma unroll
-  for (int i = 0; i < 8 * V; ++i) {
-    const int c = col<TPR, VEC>(t, i);
-    w[i] = p.w != nullptr ? (c < d ? p.w[c] : 0.f) : 1.f;
-    b[i] = p.b != nullptr && c < d ? p.b[c] : 0.f;
+  if (keeps_params<TPR>()) {
+    load_param<TPR, V, VEC>(p.w, t, d, 1.f, w);
+    load_param<TPR, V, VEC>(p.b, t, d, 0.f, b);
   }
   const float inv_d = 1.f / (float)d;
+  // Elements of a row that this warp holds, and those of the warp that this lane joins.
+  const int lane = threadIdx.x & 31;
+  const float own_inv = WPR == 1 ? inv_d : 1.f / (float)max(1, warp_count<TPR, V, VEC>(t / 32, d));
+  const float lane_n = lane < WPR ? (float)warp_count<TPR, V, VEC>(lane, d) : 0.f;
+  const float lane_inv = lane_n > 0.f ? 1.f / lane_n : 0.f;
   int par = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.n; r0 += (int64_t)gridDim.x * ROWS, par ^= 1) {
+  RawRow<V> nx, nr;
+  auto fetch = [&](int64_t row) {
+    const int dd = row < p.n ? d : 0;  // a slot behind the last row loads and stores nothing
+    load_row<TPR, V, VEC>(p.x, row * d, p.x_bf16, t, dd, nx);
+    if (p.r != nullptr) load_row<TPR, V, VEC>(p.r, row * d, p.r_bf16, t, dd, nr);
+  };
+  const int64_t hop = (int64_t)gridDim.x * ROWS;
+  fetch((int64_t)blockIdx.x * ROWS + slot);
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.n; r0 += hop, par ^= 1) {
     const int64_t row = r0 + slot;
     const bool ok = row < p.n;
-    const int dd = ok ? d : 0;  // a slot behind the last row loads and stores nothing
+    const int dd = ok ? d : 0;
     const int64_t off = row * d;
-    float v[8 * V];
-    load_row<TPR, V, VEC>(p.x, off, p.x_bf16, t, dd, v);
+    float v[8 * V], r[8 * V];
+    to_floats<V, VEC>(nx, p.x_bf16, v);
+    if (p.r != nullptr) to_floats<V, VEC>(nr, p.r_bf16, r);
+    if (loads_ahead<TPR, V>() && r0 + hop < p.n) fetch(row + hop);
     if (p.r != nullptr) {
-      float r[8 * V];
-      load_row<TPR, V, VEC>(p.r, off, p.r_bf16, t, dd, r);
 #pragma unroll
       for (int i = 0; i < 8 * V; ++i) {
         v[i] += r[i];
@@ -195,12 +254,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_fwd_kernel(c
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) sum += v[i];
     sum = lane_sum<LW>(sum);
-    float mean, sq = 0.f;
-    if (WPR == 1) {
-      mean = sum * inv_d;
-    } else {
-      mean = sum / (float)max(1, warp_count<TPR, V, VEC>(t / 32, d));
-    }
+    float mean = sum * own_inv, sq = 0.f;
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) {
       const float e = col<TPR, VEC>(t, i) < d ? v[i] - mean : 0.f;
@@ -210,34 +264,31 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_fwd_kernel(c
     if (WPR > 1) {
       if ((t & 31) == 0) red[par][t / 32] = make_float2(sum, sq);
       __syncthreads();
-      // Total of the warps' sums, then the squares about the common mean:
+      // Lane q joins warp q: the total of the sums, then the squares about the common mean,
       // sum (e - m)^2 = sum (e - m_q)^2 + n_q (m_q - m)^2.
-      float all = 0.f;
-#pragma unroll
-      for (int q = 0; q < WPR; ++q) all += red[par][q].x;
-      mean = all * inv_d;
-      sq = 0.f;
-#pragma unroll
-      for (int q = 0; q < WPR; ++q) {
-        const float nq = (float)warp_count<TPR, V, VEC>(q, d);
-        const float2 e = red[par][q];
-        const float dm = nq > 0.f ? e.x / nq - mean : 0.f;
-        sq += fmaf(nq * dm, dm, e.y);
-      }
+      const float2 e = lane < WPR ? red[par][lane] : make_float2(0.f, 0.f);
+      mean = lane_sum<32>(e.x) * inv_d;
+      const float dm = lane_n > 0.f ? e.x * lane_inv - mean : 0.f;
+      sq = lane_sum<32>(fmaf(lane_n * dm, dm, e.y));
     }
     const float rstd = 1.f / sqrtf(fmaf(sq, inv_d, p.eps));
     if (ok && t == 0 && p.mean != nullptr) {
       p.mean[row] = mean;
       p.rstd[row] = rstd;
     }
+    if (!keeps_params<TPR>()) {
+      load_param<TPR, V, VEC>(p.w, t, d, 1.f, w);
+      load_param<TPR, V, VEC>(p.b, t, d, 0.f, b);
+    }
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) v[i] = fmaf((v[i] - mean) * rstd, w[i], b[i]);
     store_row<TPR, V, VEC>(p.y, off, p.y_bf16, t, dd, v);
+    if (!loads_ahead<TPR, V>() && r0 + hop < p.n) fetch(row + hop);
   }
 }
 
 template <int TPR, int V, bool VEC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_bwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(cta_threads<TPR>(), ctas_per_sm<TPR, V>()) layer_norm_bwd_kernel(const LnParams p) {
   constexpr int NT = TPR < 128 ? 128 : TPR;
   constexpr int ROWS = NT / TPR;
   constexpr int LW = TPR < 32 ? TPR : 32;
@@ -246,23 +297,35 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_bwd_kernel(c
   __shared__ float join[ROWS > 1 ? NT : 1][ROWS > 1 ? 16 * V + 1 : 1];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR, d = p.d;
   float w[8 * V], dw[8 * V], db[8 * V];
+  if (keeps_params<TPR>()) load_param<TPR, V, VEC>(p.w, t, d, 1.f, w);
 #pragma unroll
-  for (int i = 0; i < 8 * V; ++i) {
-    const int c = col<TPR, VEC>(t, i);
-    w[i] = p.w != nullptr ? (c < d ? p.w[c] : 0.f) : 1.f;
-    dw[i] = db[i] = 0.f;
-  }
+  for (int i = 0; i < 8 * V; ++i) dw[i] = db[i] = 0.f;
   const float inv_d = 1.f / (float)d;
   int par = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.n; r0 += (int64_t)gridDim.x * ROWS, par ^= 1) {
+  RawRow<V> nx, ng, ns;
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t row) {
+    const bool in = row < p.n;
+    const int dd = in ? d : 0;
+    load_row<TPR, V, VEC>(p.x, row * d, p.s_bf16, t, dd, nx);
+    load_row<TPR, V, VEC>(p.dy, row * d, p.y_bf16, t, dd, ng);
+    nmean = in ? p.mean[row] : 0.f;
+    nrstd = in ? p.rstd[row] : 0.f;
+  };
+  const int64_t hop = (int64_t)gridDim.x * ROWS;
+  fetch((int64_t)blockIdx.x * ROWS + slot);
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < p.n; r0 += hop, par ^= 1) {
     const int64_t row = r0 + slot;
     const bool ok = row < p.n;
     const int dd = ok ? d : 0;
     const int64_t off = row * d;
     float v[8 * V], g[8 * V];
-    load_row<TPR, V, VEC>(p.x, off, p.s_bf16, t, dd, v);
-    load_row<TPR, V, VEC>(p.dy, off, p.y_bf16, t, dd, g);
-    const float mean = ok ? p.mean[row] : 0.f, rstd = ok ? p.rstd[row] : 0.f;
+    to_floats<V, VEC>(nx, p.s_bf16, v);
+    to_floats<V, VEC>(ng, p.y_bf16, g);
+    const float mean = nmean, rstd = nrstd;
+    if (p.ds != nullptr) load_row<TPR, V, VEC>(p.ds, off, p.s_bf16, t, dd, ns);
+    if (loads_ahead<TPR, V>() && r0 + hop < p.n) fetch(row + hop);
+    if (!keeps_params<TPR>()) load_param<TPR, V, VEC>(p.w, t, d, 1.f, w);
     float a = 0.f, c = 0.f;
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) {
@@ -279,24 +342,23 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_bwd_kernel(c
     if (WPR > 1) {
       if ((t & 31) == 0) red[par][t / 32] = make_float2(a, c);
       __syncthreads();
-      a = c = 0.f;
-#pragma unroll
-      for (int q = 0; q < WPR; ++q) {
-        a += red[par][q].x;
-        c += red[par][q].y;
-      }
+      const int lane = threadIdx.x & 31;
+      const float2 e = lane < WPR ? red[par][lane] : make_float2(0.f, 0.f);
+      a = lane_sum<32>(e.x);
+      c = lane_sum<32>(e.y);
     }
     a *= inv_d;
     c *= inv_d;
 #pragma unroll
     for (int i = 0; i < 8 * V; ++i) v[i] = rstd * (g[i] - a - v[i] * c);
     if (p.ds != nullptr) {
-      load_row<TPR, V, VEC>(p.ds, off, p.s_bf16, t, dd, g);
+      to_floats<V, VEC>(ns, p.s_bf16, g);
 #pragma unroll
       for (int i = 0; i < 8 * V; ++i) v[i] += g[i];
     }
     store_row<TPR, V, VEC>(p.dx, off, p.x_bf16, t, dd, v);
     if (p.dr != nullptr) store_row<TPR, V, VEC>(p.dr, off, p.r_bf16, t, dd, v);
+    if (!loads_ahead<TPR, V>() && r0 + hop < p.n) fetch(row + hop);
   }
   if (p.part == nullptr) return;
   if (ROWS > 1) {
@@ -326,40 +388,46 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) layer_norm_bwd_kernel(c
   }
 }
 
-// CTAs of a launch: enough to fill the GPU, few enough that a CTA sees many rows.
-constexpr int kFwdCtas = 148 * 8;
-constexpr int kBwdCtas = 148 * 4;
-
-int rows_per_cta(int64_t d) { return d <= 64 ? 16 : d <= 128 ? 8 : d <= 1024 ? 4 : 1; }
+// CTAs of a launch: one wave of what an SM holds, so that a CTA sees many rows and leaves
+// one row of partial sums for all of them (8192 x 4096: two waves 127 us, one 110 us).
+constexpr int kFwdCtas = 148 * 4;
+int rows_per_cta(int64_t d) { return d <= 64 ? 16 : d <= 128 ? 8 : d <= 512 ? 4 : 1; }
 int64_t bwd_ctas(int64_t n, int64_t d) {
-  const int64_t want = semx::cdiv(n, rows_per_cta(d));
-  return want < kBwdCtas ? want : kBwdCtas;
+  const int64_t want = semx::cdiv(n, rows_per_cta(d)), most = 148 * (d <= 2048 ? 4 : d <= 4096 ? 2 : 1);
+  return want < most ? want : most;
 }
 
 template <bool VEC>
 int launch_ln(bool bwd, const LnParams& p, cudaStream_t st) {
   const int64_t rows = rows_per_cta(p.d), want = semx::cdiv(p.n, rows);
   const unsigned grid = (unsigned)(bwd ? bwd_ctas(p.n, p.d) : want < kFwdCtas ? want : kFwdCtas);
-  // A row's threads: 8 V elements each. Wide rows take more threads before more elements,
-  // so that a thread's row, w, dw and db stay in registers.
-#define SEMX_LN(DMAX, TPR, V)                                                                 \
-  if (p.d <= DMAX) {                                                                          \
-    constexpr int NT = TPR < 128 ? 128 : TPR;                                                 \
-    if (bwd) layer_norm_bwd_kernel<TPR, V, VEC><<<grid, NT, 0, st>>>(p);                      \
-    else layer_norm_fwd_kernel<TPR, V, VEC><<<grid, NT, 0, st>>>(p);                          \
-    return semx::check_launch(bwd ? "layer_norm_bwd_kernel" : "layer_norm_fwd_kernel");       \
+  // A row's threads, 8 V elements each: more threads before more elements in the forward; the
+  // backward, which also keeps dw and db, takes two steps' elements per thread and half the
+  // threads.
+#define SEMX_LN(DMAX, TPR, V)                                                                             \
+  if (p.d <= DMAX) {                                                                                      \
+    if (bwd) layer_norm_bwd_kernel<TPR, V, VEC><<<grid, cta_threads<TPR>(), 0, st>>>(p);                  \
+    else layer_norm_fwd_kernel<TPR, V, VEC><<<grid, cta_threads<TPR>(), 0, st>>>(p);                      \
+    return semx::check_launch(bwd ? "layer_norm_bwd_kernel" : "layer_norm_fwd_kernel");                   \
+  }
+#define SEMX_LN2(DMAX, TPR, BTPR, BV)                                                                     \
+  if (p.d <= DMAX) {                                                                                      \
+    if (bwd) layer_norm_bwd_kernel<BTPR, BV, VEC><<<grid, cta_threads<BTPR>(), 0, st>>>(p);               \
+    else layer_norm_fwd_kernel<TPR, 1, VEC><<<grid, cta_threads<TPR>(), 0, st>>>(p);                      \
+    return semx::check_launch(bwd ? "layer_norm_bwd_kernel" : "layer_norm_fwd_kernel");                   \
   }
   SEMX_LN(64, 8, 1)
   SEMX_LN(128, 16, 1)
   SEMX_LN(256, 32, 1)
   SEMX_LN(512, 32, 2)
-  SEMX_LN(1024, 32, 4)
-  SEMX_LN(2048, 128, 2)
-  SEMX_LN(4096, 256, 2)
-  SEMX_LN(8192, 512, 2)
+  SEMX_LN(1024, 128, 1)
+  SEMX_LN2(2048, 256, 128, 2)
+  SEMX_LN2(4096, 512, 256, 2)
+  SEMX_LN2(8192, 1024, 512, 2)
   SEMX_LN(16384, 1024, 2)
   SEMX_LN(32768, 1024, 4)
 #undef SEMX_LN
+#undef SEMX_LN2
   return semx::fail(SEMX_ERR_UNSUPPORTED, "layer_norm: width %d", p.d);
 }
 
@@ -406,7 +474,7 @@ size_t semx_layer_norm_args_size(void) { return sizeof(SemxLayerNormArgs); }
 size_t semx_layer_norm_workspace_bytes(const SemxLayerNormArgs* a) {
   if (a == nullptr || a->n < 0 || a->d < 1 || a->d > kMaxD) return 0;
   const int64_t rows = bwd_ctas(a->n, a->d);
-  return ((size_t)rows * 2 * a->d + semx::colsum_group_floats(rows, 2 * a->d)) * sizeof(float);
+  return (size_t)rows * 2 * a->d * sizeof(float);
 }
 
 int semx_layer_norm_fwd(const SemxLayerNormArgs* a, semx_stream_t stream) {
@@ -418,7 +486,7 @@ int semx_layer_norm_fwd(const SemxLayerNormArgs* a, semx_stream_t stream) {
   if (rc != SEMX_OK) return rc;
   const LnParams p = ln_params(a);
   cudaStream_t st = semx::as_stream(stream);
-  return vec_ok(a->d, {p.x, p.r, p.y, p.s}) ? launch_ln<true>(false, p, st) : launch_ln<false>(false, p, st);
+  return vec_ok(a->d, {p.x, p.r, p.y, p.s, p.w, p.b}) ? launch_ln<true>(false, p, st) : launch_ln<false>(false, p, st);
 }
 
 int semx_layer_norm_bwd(const SemxLayerNormArgs* a, semx_stream_t stream) {
@@ -436,7 +504,7 @@ int semx_layer_norm_bwd(const SemxLayerNormArgs* a, semx_stream_t stream) {
   float* ws = reinterpret_cast<float*>(a->workspace);
   p.part = params ? ws : nullptr;
   if (a->n > 0) {
-    rc = vec_ok(a->d, {p.x, p.dy, p.ds, p.dx, p.dr}) ? launch_ln<true>(true, p, st) : launch_ln<false>(true, p, st);
+    rc = vec_ok(a->d, {p.x, p.dy, p.ds, p.dx, p.dr, p.w}) ? launch_ln<true>(true, p, st) : launch_ln<false>(true, p, st);
     if (rc != SEMX_OK) return rc;
   }
   if (!params) return SEMX_OK;
@@ -447,7 +515,7 @@ int semx_layer_norm_bwd(const SemxLayerNormArgs* a, semx_stream_t stream) {
   seg.out[1] = a->dbias;
   seg.len[0] = seg.len[1] = a->d;
   // No rows: the sum over none of them is zero.
-  return semx::colsum(ws, rows, 2 * a->d, ws + (size_t)rows * 2 * a->d, seg, st);
+  return semx::colsum_once(ws, rows, 2 * a->d, seg, st);
 }
 
 }  // extern "C"

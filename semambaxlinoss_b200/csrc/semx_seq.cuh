@@ -104,6 +104,32 @@ __device__ __forceinline__ int64_t find_slot(const SeqMap& m, int64_t s) {
   return twice || mine >= m.n_slots ? kRefused : mine;
 }
 
+// Entries of sequences [s0, s0 + n), n at most RUN <= blockDim.x, into out (shared memory). Called by
+// all threads of the CTA; ends with a barrier.
+template <int RUN>
+__device__ __forceinline__ void find_slots(const SeqMap& m, int64_t s0, int n, int64_t* out) {
+  const int tid = threadIdx.x;
+  if (m.n_slots == 0 || m.slots == nullptr) {
+    if (tid < n) out[tid] = m.n_slots == 0 ? kNone : s0 + tid < m.n_slots ? s0 + tid : kRefused;
+    __syncthreads();
+    return;
+  }
+  __shared__ int32_t run[RUN];
+  if (tid < n) {
+    const int32_t mine = m.slots[s0 + tid];
+    run[tid] = mine;
+    out[tid] = mine < 0 ? kNone : mine >= m.n_slots ? kRefused : mine;
+  }
+  __syncthreads();
+  // Every earlier slot against the run's. Threads that find a pair write the same value.
+  for (int64_t i = tid; i < s0 + n; i += blockDim.x) {
+    const int32_t v = m.slots[i];
+    for (int k = (int)max((int64_t)0, i - s0 + 1); k < n; ++k)
+      if (v >= 0 && run[k] == v) out[k] = kRefused;
+  }
+  __syncthreads();
+}
+
 // Host: fills the sequence fields for pieces of Q rows (Q <= 0: one piece per sequence).
 inline void set_pieces(SeqMap* m, int64_t Q) {
   if (Q <= 0) Q = (int64_t)1 << 31;  // longer than any sequence

@@ -8,11 +8,13 @@
 // state pool), or zeros.
 //
 // Bound: HBM (2 K + 5 flops per 2 elements moved). A thread owns V neighbouring channels
-// (one 16-byte access) and walks over a piece of a sequence with the K inputs of the window
+// and walks over a piece of a sequence with the K inputs of the window
 // in registers, so every input is read once but for the K - 1 rows in front of a piece. It
-// loads kU rows at a time before it uses them. The backward walks the same way: dpre of the
-// K - 1 rows behind the piece is recomputed there. dw and db are summed per thread over the
-// piece, written as one row per piece and reduced over pieces by the fixed-order column sum.
+// loads U rows at a time; in the backward U rows are on their way while it uses the U before
+// them (in the forward the registers for that cost more threads than it hid: 18 -> 38 us).
+// The backward walks the same way: dpre of the K - 1 rows behind the piece is recomputed
+// there. dw and db are summed per thread over the piece, written as one row per piece and
+// reduced over pieces by the fixed-order column sum.
 //
 // The window is read and replaced by the thread that runs the sequence's first piece: the
 // pool entry is written after that thread has read it, and no other piece looks at it
@@ -28,6 +30,10 @@ namespace {
 
 constexpr int kT = 128;
 constexpr int kMaxK = 8;
+// Channels per thread. More of them, up to 16-byte accesses, leave too few threads to hide the
+// latency and need twice the registers (backward 404 x 321 x 256 fp32: four 108 us, two
+// 93 us; forward 6151 x 2048 bf16: eight 23 us, two 18 us).
+constexpr int kWidth = 2;
 
 struct CvParams {
   semx::SeqMap m;
@@ -48,15 +54,15 @@ struct Raw {
   typedef uint32_t type;
 };
 template <>
-struct Raw<true, 8> {
-  typedef uint4 type;
-};
-template <>
 struct Raw<false, 4> {
   typedef uint4 type;
 };
 template <>
 struct Raw<true, 4> {
+  typedef uint2 type;
+};
+template <>
+struct Raw<false, 2> {
   typedef uint2 type;
 };
 
@@ -71,17 +77,24 @@ __device__ __forceinline__ typename Raw<BF16, V>::type ld_raw(const void* base, 
   }
 }
 template <bool BF16, int V>
+__device__ __forceinline__ void st_raw(void* base, int64_t i, const typename Raw<BF16, V>::type& r) {
+  if constexpr (V > 1) {
+    *reinterpret_cast<typename Raw<BF16, V>::type*>(reinterpret_cast<char*>(base) + i * (BF16 ? 2 : 4)) = r;
+  } else if constexpr (BF16) {
+    reinterpret_cast<unsigned short*>(base)[i] = (unsigned short)r;
+  } else {
+    reinterpret_cast<uint32_t*>(base)[i] = r;
+  }
+}
+template <bool BF16, int V>
 __device__ __forceinline__ void unpack(const typename Raw<BF16, V>::type& r, float (&v)[V]) {
-  if constexpr (V == 8) {
-    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(u[j] << 16);
-      v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-    }
-  } else if constexpr (V == 4 && BF16) {
+  if constexpr (V == 4 && BF16) {
     v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
     v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
+  } else if constexpr (V == 2 && BF16) {
+    v[0] = __uint_as_float(r << 16); v[1] = __uint_as_float(r & 0xffff0000u);
+  } else if constexpr (V == 2) {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
   } else if constexpr (V == 4) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
     v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
@@ -93,18 +106,16 @@ __device__ __forceinline__ void unpack(const typename Raw<BF16, V>::type& r, flo
 }
 template <bool BF16, int V>
 __device__ __forceinline__ void st_vec(void* base, int64_t i, const float (&v)[V]) {
-  if constexpr (V == 8) {
-    uint4 q;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = q;
-  } else if constexpr (V == 4 && BF16) {
+  if constexpr (V == 4 && BF16) {
     uint2 q;
     __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
     h[0] = __floats2bfloat162_rn(v[0], v[1]);
     h[1] = __floats2bfloat162_rn(v[2], v[3]);
     *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = q;
+  } else if constexpr (V == 2 && BF16) {
+    *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = __floats2bfloat162_rn(v[0], v[1]);
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(reinterpret_cast<float*>(base) + i) = make_float2(v[0], v[1]);
   } else if constexpr (V == 4) {
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i) = make_float4(v[0], v[1], v[2], v[3]);
   } else if constexpr (BF16) {
@@ -130,12 +141,40 @@ __device__ __forceinline__ void input(const CvParams& p, const semx::Piece& q, i
   }
 }
 
+// The CTA's weights (a run of w) go through shared memory, where a thread's V K values are
+// one run too: read from global memory they cost as much as 32 rows of x. PAD keeps the
+// runs of neighbouring threads in other banks.
+template <int V, int K>
+struct Weights {
+  static constexpr int RUN = V * K, PAD = RUN % 32 == 0 ? 4 : 0;
+  float v[kT * (RUN + PAD)];
+};
+template <int V, int K>
+__device__ __forceinline__ void stage_weights(Weights<V, K>& s, const float* w, int c0, int C) {
+  constexpr int RUN = V * K, PAD = Weights<V, K>::PAD;
+  const int n = min((int)blockDim.x * V, C - c0) * K;
+  const float* src = w + (int64_t)c0 * K;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) s.v[i + i / RUN * PAD] = src[i];
+}
+template <int V, int K>
+__device__ __forceinline__ void own_weights(const Weights<V, K>& s, float (&w)[K][V]) {
+  constexpr int RUN = V * K, PAD = Weights<V, K>::PAD;
+  const float* mine = s.v + threadIdx.x * (RUN + PAD);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][i] = mine[i * K + k];
+}
+
 template <bool BF16, int V, int K, int U>
 __global__ void __launch_bounds__(kT) short_conv_fwd_kernel(const CvParams p) {
+  __shared__ Weights<V, K> sw;
   const int64_t j = blockIdx.x / p.ctiles;
-  const int c = ((blockIdx.x % p.ctiles) * blockDim.x + threadIdx.x) * V;
+  const int c0 = (blockIdx.x % p.ctiles) * blockDim.x * V, c = c0 + threadIdx.x * V;
+  stage_weights(sw, p.w, c0, p.C);
   const semx::Piece q = semx::find_piece(p.m, j);
   const int64_t slot = q.live ? semx::find_slot(p.m, q.s) : semx::kNone;
+  __syncthreads();
   if (c >= p.C) return;
   float zero[V];
 #pragma unroll
@@ -144,10 +183,9 @@ __global__ void __launch_bounds__(kT) short_conv_fwd_kernel(const CvParams p) {
   if (!q.live) return;
   const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[q.s] != 0);
   float w[K][V], b[V];
+  own_weights(sw, w);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) w[k][i] = p.w[(int64_t)(c + i) * K + k];
     b[i] = p.b != nullptr ? p.b[c + i] : 0.f;
     if (slot == semx::kRefused) b[i] = __int_as_float(0x7fffffff);
   }
@@ -214,22 +252,23 @@ __global__ void __launch_bounds__(kT) short_conv_fwd_kernel(const CvParams p) {
 // only feed dx), and dx[t - (K - 1)] once dpre[t] is there.
 template <bool BF16, int V, int K, int U>
 __global__ void __launch_bounds__(kT) short_conv_bwd_kernel(const CvParams p) {
+  __shared__ Weights<V, K> sw;
   const int64_t j = blockIdx.x / p.ctiles;
-  const int c = ((blockIdx.x % p.ctiles) * blockDim.x + threadIdx.x) * V;
+  const int c0 = (blockIdx.x % p.ctiles) * blockDim.x * V, c = c0 + threadIdx.x * V;
+  stage_weights(sw, p.w, c0, p.C);
   const semx::Piece q = semx::find_piece(p.m, j);
+  __syncthreads();
   if (c >= p.C) return;
   float zero[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) zero[i] = 0.f;
   for (int64_t r = semx::rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) st_vec<BF16, V>(p.dx, r * p.C + c, zero);
   float w[K][V], b[V], dw[K][V], db[V];
+  own_weights(sw, w);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      w[k][i] = p.w[(int64_t)(c + i) * K + k];
-      dw[k][i] = 0.f;
-    }
+    for (int k = 0; k < K; ++k) dw[k][i] = 0.f;
     b[i] = p.b != nullptr ? p.b[c + i] : 0.f;
     db[i] = 0.f;
   }
@@ -242,14 +281,26 @@ __global__ void __launch_bounds__(kT) short_conv_bwd_kernel(const CvParams p) {
   }
   const int end = q.t1 > q.t0 ? q.t1 + K - 1 : 0;  // a piece without rows has no steps
   typedef typename Raw<BF16, V>::type R;
+  R nx[U], ng[U];  // U rows are always on their way
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u < end) {
+        const int tt = min(t + u, q.len - 1);  // rows behind the sequence load its last row and count nothing
+        nx[u] = ld_raw<BF16, V>(p.x, (q.row0 + tt) * p.ldx + c);
+        ng[u] = ld_raw<BF16, V>(p.dy, (q.row0 + tt) * p.C + c);
+      }
+    }
+  };
+  fetch(q.t0);
   for (int t = q.t0; t < end; t += U) {
     R rx[U], rg[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int tt = min(t + u, q.len - 1);  // rows behind the sequence load its last row and count nothing
-      rx[u] = ld_raw<BF16, V>(p.x, (q.row0 + tt) * p.ldx + c);
-      rg[u] = ld_raw<BF16, V>(p.dy, (q.row0 + tt) * p.C + c);
+      rx[u] = nx[u];
+      rg[u] = ng[u];
     }
+    fetch(t + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (t + u < end) {
@@ -306,12 +357,95 @@ __global__ void __launch_bounds__(kT) short_conv_bwd_kernel(const CvParams p) {
   }
 }
 
+// One row per sequence. Two channels per thread (one where they do not pair up): with few
+// sequences the threads are what hides the latency, and a warp's weights are one run of
+// memory. A CTA takes a run of sequences, so that the weights are read once for all of them,
+// and loads kAhead rows and windows before it uses them.
+constexpr int kAhead = 4;
+constexpr int kStepRows = 16;  // sequences per CTA at most
+
+template <bool BF16, int V, int K>
+__global__ void __launch_bounds__(kT) short_conv_step_kernel(const CvParams p, int rows) {
+  typedef typename Raw<BF16, V>::type R;
+  __shared__ int64_t slots[kStepRows];
+  const int64_t s0 = (int64_t)(blockIdx.x / p.ctiles) * rows;
+  const int n = (int)min((int64_t)rows, p.m.S - s0);
+  const int c = ((blockIdx.x % p.ctiles) * kT + threadIdx.x) * V;
+  float w[V][K], b[V];
+  if (c < p.C) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) w[i][k] = p.w[(int64_t)(c + i) * K + k];
+      b[i] = p.b != nullptr ? p.b[c + i] : 0.f;
+    }
+  }
+  semx::find_slots<kStepRows>(p.m, s0, n, slots);
+  if (c >= p.C) return;
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    R rx[kAhead][K];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u < n) {
+        const int64_t s = s0 + i0 + u, slot = slots[i0 + u];
+        rx[u][K - 1] = ld_raw<BF16, V>(p.x, s * p.ldx + c);
+        const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[s] != 0);
+#pragma unroll
+        for (int k = 0; k + 1 < K; ++k)
+          rx[u][k] = cold ? R{} : ld_raw<BF16, V>(p.state, (slot * (K - 1) + k) * p.C + c);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u < n) {
+        const int64_t s = s0 + i0 + u, slot = slots[i0 + u];
+        float a[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[i] = slot == semx::kRefused ? __int_as_float(0x7fffffff) : b[i];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float x[V];
+          unpack<BF16, V>(rx[u][k], x);
+#pragma unroll
+          for (int i = 0; i < V; ++i) a[i] = fmaf(w[i][k], x[i], a[i]);
+        }
+        if (p.silu) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) a[i] *= sigmoid(a[i]);
+        }
+        st_vec<BF16, V>(p.y, s * p.C + c, a);
+        if (slot >= 0) {
+#pragma unroll
+          for (int k = 0; k + 1 < K; ++k) st_raw<BF16, V>(p.state, (slot * (K - 1) + k) * p.C + c, rx[u][k + 1]);
+        }
+      }
+    }
+  }
+}
+
+template <bool BF16, int V, int K0>
+int launch_step(int K, CvParams& p, cudaStream_t st) {
+  if constexpr (K0 <= kMaxK) {
+    if (K != K0) return launch_step<BF16, V, K0 + 1>(K, p, st);
+    p.ctiles = (int)semx::cdiv(p.C, (int64_t)kT * V);
+    // Sequences per CTA: as many as leave four CTAs per SM.
+    int rows = kStepRows;
+    while (rows > 1 && semx::cdiv(p.m.S, rows) * p.ctiles < 148 * 4) rows /= 2;
+    const int64_t grid = semx::cdiv(p.m.S, rows) * p.ctiles;
+    if (grid == 0) return SEMX_OK;
+    if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "short_conv: too many sequences");
+    short_conv_step_kernel<BF16, V, K0><<<(unsigned)grid, kT, 0, st>>>(p, rows);
+    return semx::check_launch("short_conv_step_kernel");
+  }
+  return semx::fail(SEMX_ERR_UNSUPPORTED, "short_conv: %d taps", K);
+}
+
 // Rows of a piece: long pieces re-read few rows (K - 1 in front, and K - 1 behind in the
 // backward) and leave few rows of partial sums; short ones fill the GPU.
-constexpr int64_t kFill = 148 * 1024;
-int64_t piece_rows(int64_t T, int64_t C, int64_t V, bool bwd) {
+constexpr int64_t kFill = 148 * 512;  // threads
+int64_t piece_rows(int64_t T, int64_t C, bool bwd) {
   int64_t Q = bwd ? 64 : 32;
-  while (Q > 8 && semx::cdiv(T, Q) * semx::cdiv(C, V) < kFill) Q /= 2;
+  while (Q > 8 && semx::cdiv(T, Q) * semx::cdiv(C, (int64_t)kWidth) < kFill) Q /= 2;
   return Q;
 }
 
@@ -335,25 +469,21 @@ int cv_validate(const SemxShortConvArgs* a, bool bwd, CvParams* p) {
   return SEMX_OK;
 }
 
-// Channels per thread: one 16-byte access, except that the K-step windows of 8 channels no
-// longer fit the registers above 4 taps.
-int64_t cv_width(const SemxShortConvArgs* a) { return a->bf16 && a->K <= 4 ? 8 : 4; }
-
-bool cv_vec(const SemxShortConvArgs* a) {
-  const int64_t V = cv_width(a);
+// Whether every row allows accesses of V neighbouring channels.
+bool cv_allows(const SemxShortConvArgs* a, int64_t V) {
   if (a->C % V != 0 || a->ldx % V != 0) return false;
   for (const void* q : {a->x, (const void*)a->y, (const void*)a->state, a->dy, (const void*)a->dx})
-    if (!semx::aligned(q, 16)) return false;
+    if (!semx::aligned(q, V * (a->bf16 ? 2 : 4))) return false;
   return true;
 }
 
 int64_t cv_pieces(const SemxShortConvArgs* a, semx::SeqMap* m) {
   // The partial rows' number must not depend on alignment: both paths cut alike.
-  semx::set_pieces(m, piece_rows(a->rows, a->C, cv_width(a), true));
+  semx::set_pieces(m, piece_rows(a->rows, a->C, true));
   return m->pieces;
 }
 
-template <bool BF16, int V, int K0, int K1>
+template <bool BF16, int V, int K0>
 int launch_cv(bool bwd, int K, CvParams& p, cudaStream_t st) {
   // Narrow tensors take narrow CTAs.
   const int nt = (int)semx::cdiv(p.C, (int64_t)V) >= kT ? kT : (int)semx::cdiv(semx::cdiv(p.C, (int64_t)V), 32) * 32;
@@ -361,22 +491,25 @@ int launch_cv(bool bwd, int K, CvParams& p, cudaStream_t st) {
   const int64_t grid = p.m.pieces * p.ctiles;
   if (grid == 0) return SEMX_OK;
   if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "short_conv: too many pieces");
-  if constexpr (K0 <= K1) {
+  if constexpr (K0 <= kMaxK) {
     if (K == K0) {
-      constexpr int U = V > 1 ? 4 : 8;  // rows loaded ahead
-      if (bwd) short_conv_bwd_kernel<BF16, V, K0, U><<<(unsigned)grid, nt, 0, st>>>(p);
-      else short_conv_fwd_kernel<BF16, V, K0, U><<<(unsigned)grid, nt, 0, st>>>(p);
+      if (bwd) short_conv_bwd_kernel<BF16, V, K0, 4><<<(unsigned)grid, nt, 0, st>>>(p);
+      else short_conv_fwd_kernel<BF16, V, K0, 4><<<(unsigned)grid, nt, 0, st>>>(p);
       return semx::check_launch(bwd ? "short_conv_bwd_kernel" : "short_conv_fwd_kernel");
     }
-    return launch_cv<BF16, V, K0 + 1, K1>(bwd, K, p, st);
+    return launch_cv<BF16, V, K0 + 1>(bwd, K, p, st);
   }
   return semx::fail(SEMX_ERR_UNSUPPORTED, "short_conv: %d taps", K);
 }
 
 int dispatch_cv(const SemxShortConvArgs* a, bool bwd, CvParams& p, cudaStream_t st) {
-  if (!cv_vec(a)) return a->bf16 ? launch_cv<true, 1, 1, 8>(bwd, a->K, p, st) : launch_cv<false, 1, 1, 8>(bwd, a->K, p, st);
-  if (!a->bf16) return launch_cv<false, 4, 1, 8>(bwd, a->K, p, st);
-  return a->K <= 4 ? launch_cv<true, 8, 1, 4>(bwd, a->K, p, st) : launch_cv<true, 4, 5, 8>(bwd, a->K, p, st);
+  if (!bwd && p.m.cu == nullptr && p.m.L == 1) {
+    if (cv_allows(a, 2)) return a->bf16 ? launch_step<true, 2, 1>(a->K, p, st) : launch_step<false, 2, 1>(a->K, p, st);
+    return a->bf16 ? launch_step<true, 1, 1>(a->K, p, st) : launch_step<false, 1, 1>(a->K, p, st);
+  }
+  if (!cv_allows(a, kWidth))
+    return a->bf16 ? launch_cv<true, 1, 1>(bwd, a->K, p, st) : launch_cv<false, 1, 1>(bwd, a->K, p, st);
+  return a->bf16 ? launch_cv<true, kWidth, 1>(bwd, a->K, p, st) : launch_cv<false, kWidth, 1>(bwd, a->K, p, st);
 }
 
 }  // namespace
@@ -394,7 +527,7 @@ size_t semx_short_conv_workspace_bytes(const SemxShortConvArgs* a) {
   b.dx = reinterpret_cast<void*>(256);
   if (cv_validate(&b, true, &p) != SEMX_OK) return 0;
   const int64_t rows = cv_pieces(a, &p.m), cols = a->C * (a->K + 1);
-  return ((size_t)rows * cols + semx::colsum_group_floats(rows, cols)) * sizeof(float);
+  return (size_t)rows * cols * sizeof(float);
 }
 
 int semx_short_conv_fwd(const SemxShortConvArgs* a, semx_stream_t stream) {
@@ -405,7 +538,7 @@ int semx_short_conv_fwd(const SemxShortConvArgs* a, semx_stream_t stream) {
   semx::DeviceScope scope;
   rc = scope.bind({a->y, a->state});
   if (rc != SEMX_OK) return rc;
-  semx::set_pieces(&p.m, piece_rows(a->rows, a->C, cv_vec(a) ? cv_width(a) : 1, false));
+  semx::set_pieces(&p.m, piece_rows(a->rows, a->C, false));
   // Without a sequence every row is a row behind the last one.
   if (p.m.S == 0 && p.m.T > 0) p.m.pieces = p.m.T;
   return dispatch_cv(a, false, p, semx::as_stream(stream));
@@ -437,7 +570,7 @@ int semx_short_conv_bwd(const SemxShortConvArgs* a, semx_stream_t stream) {
   seg.out[1] = a->db;
   seg.len[0] = a->C * a->K;
   seg.len[1] = a->C;
-  return semx::colsum(ws, a->rows > 0 && a->S > 0 ? rows : 0, cols, ws + (size_t)rows * cols, seg, st);
+  return semx::colsum_once(ws, a->rows > 0 && a->S > 0 ? rows : 0, cols, seg, st);
 }
 
 }  // extern "C"

@@ -499,7 +499,7 @@ int64_t bwd_rows_per_piece(const ScanParams& p) {
 }
 
 struct Layout {
-  size_t entry, dsum, pbc, part, groups, total;
+  size_t entry, dsum, pbc, part, total;
 };
 Layout layout(const ScanParams& p, int64_t Q) {
   Layout l = {};
@@ -515,8 +515,6 @@ Layout layout(const ScanParams& p, int64_t Q) {
   at += up((size_t)p.ctiles * p.m.T * 2 * p.N);
   l.part = at;
   at += up(pieces * p.C * (p.N + 2));
-  l.groups = at;
-  at += semx::colsum_group_floats(p.m.pieces, (int64_t)p.C * (p.N + 2));
   l.total = at;
   return l;
 }
@@ -613,7 +611,7 @@ int semx_state_scan_bwd(const SemxStateScanArgs* a, semx_stream_t stream) {
   seg.out[2] = a->ddt_bias;
   seg.len[0] = a->C * a->N;
   seg.len[1] = seg.len[2] = a->C;
-  return semx::colsum(ws + l.part, p.m.T > 0 ? p.m.pieces : 0, a->C * (a->N + 2), ws + l.groups, seg, st);
+  return semx::colsum_once(ws + l.part, p.m.T > 0 ? p.m.pieces : 0, a->C * (a->N + 2), seg, st);
 }
 
 }  // extern "C"
