@@ -439,6 +439,16 @@ def empty_f32(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max((nbytes + 3) // 4, 1), dtype=torch.float32, device=device)
 
 
+def scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    """As :func:`empty_f32`, on the GPU of ``like``."""
+    return like.new_empty((max((nbytes + 3) // 4, 1),), dtype=torch.float32)
+
+
+def cast(grad: torch.Tensor | None, dtype) -> torch.Tensor | None:
+    """A gradient in its parameter's type."""
+    return grad if grad is None or grad.dtype == dtype else grad.to(dtype)
+
+
 def new_args(cls):
     a = cls()
     a.struct_size = ctypes.sizeof(cls)

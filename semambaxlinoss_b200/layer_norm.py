@@ -29,8 +29,8 @@ def _param(p):
 
 
 def _forward(x, weight, bias, eps, residual, out_dtype, stats):
-    """Runs the forward on detached tensors; returns (y, s, mean, rstd), mean and rstd None
-    unless ``stats``."""
+    """Runs the forward; returns (y, s, kept): kept (2, rows) holds mean and 1 / sqrt(var + eps)
+    where ``stats``, else None."""
     d = x.shape[-1]
     x = x.contiguous()
     y = x.new_empty(x.shape, dtype=out_dtype)
@@ -48,56 +48,65 @@ def _forward(x, weight, bias, eps, residual, out_dtype, stats):
         a.weight = weight.data_ptr()
     if bias is not None:
         a.bias = bias.data_ptr()
-    mean = rstd = None
+    kept = None
     if stats:
-        mean, rstd = torch.empty((2, a.n), dtype=torch.float32, device=x.device).unbind(0)
-        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+        kept = x.new_empty((2, x.numel() // d), dtype=torch.float32)
+        at = kept.data_ptr()
+        a.mean, a.rstd = at, at + 4 * a.n
     _lib.call("semx_layer_norm_fwd", a, x.device)
-    return y, s, mean, rstd
+    return y, s, kept
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual, out_dtype):
         ctx.set_materialize_grads(False)
-        w, b = _param(weight), _param(bias)
-        r = residual
-        y, s, mean, rstd = _forward(x, w, b, eps, r, out_dtype, True)
-        ctx.save_for_backward(s, w, mean, rstd)
-        ctx.cfg = (eps, out_dtype, x.dtype, None if r is None else r.dtype,
+        w = _param(weight)
+        y, s, kept = _forward(x, w, _param(bias), eps, residual, out_dtype, True)
+        ctx.save_for_backward(s, w, kept)
+        ctx.cfg = (eps, out_dtype, x.dtype, None if residual is None else residual.dtype,
                    None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        return y if r is None else (y, s)
+        return y if residual is None else (y, s)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
-        s, w, mean, rstd = ctx.saved_tensors
+        s, w, kept = ctx.saved_tensors
         eps, ydt, xdt, rdt, wdt, bdt = ctx.cfg
         if dy is None and dsum is None:
             return None, None, None, None, None, None
-        dev, d = s.device, s.shape[-1]
-        dy = torch.zeros(s.shape, dtype=ydt, device=dev) if dy is None else dy.to(ydt).contiguous()
-        dsum = None if dsum is None else dsum.to(s.dtype).contiguous()
-        dx = torch.empty(s.shape, dtype=xdt, device=dev)
+        shape = s.shape
+        d = shape[-1]
+        dy = s.new_zeros(shape, dtype=ydt) if dy is None else _as(dy, ydt)
+        dsum = None if dsum is None else _as(dsum, s.dtype)
+        dx = s.new_empty(shape, dtype=xdt)
         a = _lib.new_args(_lib.SemxLayerNormArgs)
-        a.eps, a.n, a.d = eps, s.numel() // d, d
+        a.eps, a.n, a.d = eps, kept.shape[1], d
         a.x_bf16, a.y_bf16, a.s_bf16 = xdt == torch.bfloat16, ydt == torch.bfloat16, s.dtype == torch.bfloat16
-        a.sum, a.mean, a.rstd, a.weight = s.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _lib.ptr(w)
+        at = kept.data_ptr()
+        a.sum, a.mean, a.rstd, a.weight = s.data_ptr(), at, at + 4 * a.n, _lib.ptr(w)
         a.dy, a.dsum, a.dx = dy.data_ptr(), _lib.ptr(dsum), dx.data_ptr()
+        need = ctx.needs_input_grad
         dr = dx if rdt == xdt else None
-        if rdt is not None and ctx.needs_input_grad[4] and dr is None:
-            dr = torch.empty(s.shape, dtype=rdt, device=dev)
+        if rdt is not None and need[4] and dr is None:
+            dr = s.new_empty(shape, dtype=rdt)
             a.r_bf16, a.dresidual = rdt == torch.bfloat16, dr.data_ptr()
-        dw = torch.empty(d, dtype=torch.float32, device=dev) if wdt is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty(d, dtype=torch.float32, device=dev) if bdt is not None and ctx.needs_input_grad[2] else None
+        dw = s.new_empty(d, dtype=torch.float32) if wdt is not None and need[1] else None
+        db = s.new_empty(d, dtype=torch.float32) if bdt is not None and need[2] else None
         ws = None
         if dw is not None or db is not None:
             a.dweight, a.dbias = _lib.ptr(dw), _lib.ptr(db)
-            ws = _lib.empty_f32(_lib.load().semx_layer_norm_workspace_bytes(a), dev)
+            ws = _lib.scratch(_lib.load().semx_layer_norm_workspace_bytes(a), s)
             a.workspace = ws.data_ptr()
-        _lib.call("semx_layer_norm_bwd", a, dev)
-        return (dx, None if dw is None else dw.to(wdt), None if db is None else db.to(bdt), None,
-                dr if rdt is not None else None, None)
+        _lib.call("semx_layer_norm_bwd", a, s.device)
+        return (dx, _lib.cast(dw, wdt), _lib.cast(db, bdt), None, dr if rdt is not None else None, None)
+
+
+def _as(t, dtype):
+    """t contiguous in ``dtype``, itself where it is that already."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -130,7 +139,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
             x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
             or (residual is not None and residual.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, residual, out_dtype)
-    y, s, _, _ = _forward(x, _param(weight), _param(bias), eps, residual, out_dtype, False)
+    y, s, _ = _forward(x, _param(weight), _param(bias), eps, residual, out_dtype, False)
     return y if residual is None else (y, s)
 
 

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool
+from ._batch import TYPES, as_rows, batch, check_same, param32, rows_of, set_pool
 
 _ACTIVATIONS = {"silu": 1, None: 0}
 
@@ -46,7 +46,7 @@ class _ShortConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, silu, S, rows, L, cu):
         w, b = param32(weight), param32(bias)
         a, xr = _args(x, w, b, silu, S, rows, L, cu)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = x.new_empty(x.shape)
         a.y = y.data_ptr()
         _lib.call("semx_short_conv_fwd", a, x.device)
         ctx.save_for_backward(xr, w, b, cu)
@@ -59,18 +59,17 @@ class _ShortConv(torch.autograd.Function):
         x, w, b, cu = ctx.saved_tensors
         silu, S, rows, L, wdt, bdt = ctx.cfg
         a, xr = _args(x, w, b, silu, S, rows, L, cu)
-        dy = dy.to(x.dtype).contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dy = as_rows(dy, x.dtype)
+        dx = x.new_empty(x.shape)
         dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
         a.dy, a.dx, a.dw, a.db = dy.data_ptr(), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db)
         ws = None
         if dw is not None or db is not None:
-            ws = _lib.empty_f32(_lib.load().semx_short_conv_workspace_bytes(a), x.device)
+            ws = _lib.scratch(_lib.load().semx_short_conv_workspace_bytes(a), x)
             a.workspace = ws.data_ptr()
         _lib.call("semx_short_conv_bwd", a, x.device)
-        return (dx, None if dw is None else dw.to(wdt), None if db is None else db.to(bdt), None, None, None, None,
-                None)
+        return dx, _lib.cast(dw, wdt), _lib.cast(db, bdt), None, None, None, None, None
 
 
 def _silu_flag(op, activation):

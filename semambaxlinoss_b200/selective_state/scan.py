@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._batch import TYPES, batch, check_same, param32, rows_of, set_pool
+from ._batch import TYPES, as_rows, batch, check_same, param32, rows_of, set_pool
 
 MAX_MODES = 128
 _F32 = (torch.float32,)
@@ -88,12 +88,12 @@ class _StateScan(torch.autograd.Function):
         A32, D32, b32 = param32(A), param32(D), param32(dt_bias)
         a, kept = _args(x, dt, A32, B, C, D32, z, b32, softplus, S, rows, L, cu, N, G)
         dev = x.device
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        v = None if z is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        ckpt = _lib.empty_f32(_lib.load().semx_state_scan_ckpt_bytes(a), dev)
+        y = x.new_empty(x.shape)
+        v = None if z is None else x.new_empty(x.shape)
+        ckpt = _lib.scratch(_lib.load().semx_state_scan_ckpt_bytes(a), x)
         a.y, a.v, a.ckpt = y.data_ptr(), _lib.ptr(v), ckpt.data_ptr()
         nbytes = _lib.load().semx_state_scan_workspace_bytes(a, 0)
-        ws = _lib.empty_f32(nbytes, dev) if nbytes else None
+        ws = _lib.scratch(nbytes, x) if nbytes else None
         a.workspace = _lib.ptr(ws)
         _lib.call("semx_state_scan_fwd", a, dev)
         xr, dr, Br, Cr, zr = kept
@@ -108,11 +108,10 @@ class _StateScan(torch.autograd.Function):
         softplus, S, rows, L, N, G, Bshape, (Adt, Ddt, bdt) = ctx.cfg
         a, kept = _args(x, dt, A, B, C, D, z, bias, softplus, S, rows, L, cu, N, G)
         dev = x.device
-        dy = dy.to(x.dtype).contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        ddt = torch.empty(x.shape, dtype=dt.dtype, device=dev)
-        dz = None if z is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dB, dC = (torch.empty(Bshape, dtype=x.dtype, device=dev) for _ in range(2))
+        dy = as_rows(dy, x.dtype)
+        dx, ddt = x.new_empty(x.shape), dt.new_empty(x.shape)
+        dz = None if z is None else x.new_empty(x.shape)
+        dB, dC = x.new_empty(Bshape), x.new_empty(Bshape)
         need = ctx.needs_input_grad
         dA = torch.empty_like(A) if need[2] else None
         dD = torch.empty_like(D) if D is not None and need[5] else None
@@ -120,15 +119,12 @@ class _StateScan(torch.autograd.Function):
         a.v, a.ckpt, a.dy, a.dx, a.ddt, a.dz = (_lib.ptr(v), ckpt.data_ptr(), dy.data_ptr(), dx.data_ptr(),
                                                 ddt.data_ptr(), _lib.ptr(dz))
         a.dB, a.dC, a.dA, a.dD, a.ddt_bias = dB.data_ptr(), dC.data_ptr(), _lib.ptr(dA), _lib.ptr(dD), _lib.ptr(db)
-        ws = _lib.empty_f32(_lib.load().semx_state_scan_workspace_bytes(a, 1), dev)
+        ws = _lib.scratch(_lib.load().semx_state_scan_workspace_bytes(a, 1), x)
         a.workspace = ws.data_ptr()
         _lib.call("semx_state_scan_bwd", a, dev)
 
-        def cast(g, dtype):
-            return None if g is None else g.to(dtype)
-
-        return (dx, ddt, cast(dA, Adt), dB, dC, cast(dD, Ddt), dz, cast(db, bdt), None, None, None, None, None, None,
-                None)
+        return (dx, ddt, _lib.cast(dA, Adt), dB, dC, _lib.cast(dD, Ddt), dz, _lib.cast(db, bdt), None, None, None, None,
+                None, None, None)
 
 
 def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
@@ -165,7 +161,7 @@ def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     y = x.new_empty(x.shape)
     a.y = y.data_ptr()
     nbytes = _lib.load().semx_state_scan_workspace_bytes(a, 0)
-    ws = _lib.empty_f32(nbytes, dev) if nbytes else None
+    ws = _lib.scratch(nbytes, x) if nbytes else None
     a.workspace = _lib.ptr(ws)
     _lib.call("semx_state_scan_fwd", a, dev)
     return y
