@@ -282,11 +282,23 @@ __global__ void __launch_bounds__(kThreads) state_scan_join_kernel(const ScanPar
   const int64_t base = piece_base(p.m, s, p.m.Q), n = (len + p.m.Q - 1) / p.m.Q;
   const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[s] != 0);
   float h = cold ? 0.f : p.state[slot * per + i];
-  for (int64_t k = 0; k < n; ++k) {
-    const int64_t j = base + k;
-    const float local = p.entry[j * per + i];
-    p.entry[j * per + i] = h;
-    h = fmaf(semx::ex2_approx(p.dsum[j * p.C + c] * A2), h, local);
+  // Batches of loads ahead of the chain: entry is written where it was read.
+  constexpr int U = 8;
+  for (int64_t k = 0; k < n; k += U) {
+    float local[U], decay[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t j = base + k + u;
+      local[u] = k + u < n ? p.entry[j * per + i] : 0.f;
+      decay[u] = k + u < n ? p.dsum[j * p.C + c] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k + u < n) {
+        p.entry[(base + k + u) * per + i] = h;
+        h = fmaf(semx::ex2_approx(decay[u] * A2), h, local[u]);
+      }
+    }
   }
   if (slot >= 0) p.state[slot * per + i] = h;
 }

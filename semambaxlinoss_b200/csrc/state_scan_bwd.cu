@@ -458,25 +458,52 @@ __global__ void __launch_bounds__(kThreads) state_scan_join_back_kernel(const Sc
   const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;
   const int64_t base = piece_base(p.m, s, p.m.Q), n = (len + p.m.Q - 1) / p.m.Q;
   float carry = 0.f;
-  for (int64_t k = n - 1; k >= 0; --k) {
-    const int64_t j = base + k;
-    const float local = p.entry[j * per + i];
-    p.entry[j * per + i] = carry;
-    carry = fmaf(semx::ex2_approx(p.dsum[j * p.C + c] * A2), carry, local);
+  constexpr int U = 8;  // loads ahead of the chain: entry is written where it was read
+  for (int64_t k = n - 1; k >= 0; k -= U) {
+    float local[U], decay[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t j = base + k - u;
+      local[u] = k - u >= 0 ? p.entry[j * per + i] : 0.f;
+      decay[u] = k - u >= 0 ? p.dsum[j * p.C + c] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k - u >= 0) {
+        p.entry[(base + k - u) * per + i] = carry;
+        carry = fmaf(semx::ex2_approx(decay[u] * A2), carry, local[u]);
+      }
+    }
   }
 }
 
-// dB and dC: the channel tiles' sums in tile order.
+// dB and dC: the channel tiles' sums in tile order. A thread takes four neighbouring modes of
+// one (row, group, kind); a CTA a run of rows, so that a thread's place in the row is found once.
+constexpr int kBcRows = 32;
+template <int ACC>
 __global__ void __launch_bounds__(256) state_scan_bc_kernel(const ScanParams p, void* dB, void* dC) {
-  const int64_t per = (int64_t)p.G * p.N;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= 2 * per * p.m.T) return;
-  const int64_t kind = e / (per * p.m.T), r = e % (per * p.m.T) / per, gn = e % per;
-  const int64_t g = gn / p.N, n = gn % p.N;
-  float s = 0.f;
-  if (r < rows_end(p.m))
-    for (int i = 0; i < p.tpg; ++i) s += p.pBC[((g * p.tpg + i) * p.m.T + r) * 2 * p.N + kind * p.N + n];
-  store(kind == 0 ? dB : dC, r * per + gn, p.bf16, s);
+  const int nq = (p.N + 3) / 4, per = 2 * p.G * nq;  // fours of a row: (kind, group, modes)
+  const int64_t r0 = (int64_t)blockIdx.x * kBcRows;
+  const int rows = (int)min((int64_t)kBcRows, p.m.T - r0);
+  const int64_t end = rows_end(p.m);
+  const int64_t tile = p.m.T * 2 * p.N;
+  for (int e = threadIdx.x; e < rows * per; e += blockDim.x) {
+    const int t = e / per, f = e % per, kind = f / (p.G * nq), g = f / nq % p.G, n = f % nq * 4;
+    const int64_t r = r0 + t;
+    const int cnt = min(4, p.N - n);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < end) {
+      const float* src = p.pBC + (int64_t)g * p.tpg * tile + r * 2 * p.N + kind * p.N + n;
+#pragma unroll 4
+      for (int i = 0; i < p.tpg; ++i, src += tile) {
+        float4 v;
+        if (ACC != kAny) v = *reinterpret_cast<const float4*>(src);
+        else v = load_params(src, 0, cnt);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+    }
+    store_quad<ACC>(kind == 0 ? dB : dC, r * p.G * p.N + (int64_t)g * p.N + n, p.bf16, cnt, s);
+  }
 }
 
 // At least two lanes per channel: the tiles of one would not fit shared memory.
@@ -597,9 +624,12 @@ int semx_state_scan_bwd(const SemxStateScanArgs* a, semx_stream_t stream) {
     }
     rc = launch_bwd<false>(p, st);
     if (rc != SEMX_OK) return rc;
-    const int64_t grid = semx::cdiv(2 * (int64_t)p.G * p.N * p.m.T, 256);
-    if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan bwd: too many rows");
-    state_scan_bc_kernel<<<(unsigned)grid, 256, 0, st>>>(p, a->dB, a->dC);
+    const unsigned grid = (unsigned)semx::cdiv(p.m.T, (int64_t)kBcRows);
+    const uintptr_t align = a->bf16 ? 8 : 16;
+    const bool fours = p.N % 4 == 0 && semx::aligned(p.pBC, 16) && semx::aligned(a->dB, align) && semx::aligned(a->dC, align);
+    if (!fours) state_scan_bc_kernel<kAny><<<grid, 256, 0, st>>>(p, a->dB, a->dC);
+    else if (a->bf16) state_scan_bc_kernel<kBf16><<<grid, 256, 0, st>>>(p, a->dB, a->dC);
+    else state_scan_bc_kernel<kFp32><<<grid, 256, 0, st>>>(p, a->dB, a->dC);
     rc = semx::check_launch("state_scan_bc_kernel");
     if (rc != SEMX_OK) return rc;
   }
