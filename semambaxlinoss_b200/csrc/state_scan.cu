@@ -380,14 +380,16 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
 namespace {
 
 // Rows per piece of a forward (0: whole sequences). Pieces cost the exponentials twice, so
-// only batches that leave most of the GPU idle are cut, into one wave of resident CTAs.
+// only batches that leave half of the GPU idle are cut (4 x 2047 x 2048: whole 275 us, in
+// pieces 216 us), into two waves of the four CTAs that an SM holds: the second evens out
+// what the first leaves uneven (one wave 235 us, three 212 us, but of shorter pieces).
 constexpr int64_t kResident = 148 * 4;
 int64_t fwd_rows_per_piece(const ScanParams& p) {
   const int64_t ch = kThreads / lanes_for(p.N, 4) * kCPT;
   const int64_t ctas = p.m.S * p.G * semx::cdiv(p.cpg, ch);
   const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
   if (2 * ctas > kResident || rows <= 128) return 0;
-  const int64_t Q = semx::cdiv(semx::cdiv(rows, kResident / ctas), 16) * 16;
+  const int64_t Q = semx::cdiv(semx::cdiv(rows, 2 * kResident / ctas), 16) * 16;
   return Q < 64 ? 64 : Q;
 }
 
