@@ -632,7 +632,8 @@ int semx_layer_norm_bwd(const SemxLayerNormArgs* args, semx_stream_t stream);
  * sequence of no rows leaves its entry (zeros if fresh). state NULL (n_slots 0): every
  * sequence starts from zeros. Only the forward takes a state.
  * Rows of x, dt, z, B and C are read at their own row strides (elements); y, dy and the
- * gradients are contiguous.
+ * gradients are contiguous. Pointers lie on their elements (SEMX_ERR_ALIGN); every operand
+ * on 16 bytes with rows that are multiples of 4 elements is the fast case, not a requirement.
  * ---------------------------------------------------------------------------------- */
 
 /* Short causal depthwise convolution of K taps (1..8), with SiLU when `silu` is set:

@@ -436,6 +436,12 @@ int ln_validate(const SemxLayerNormArgs* a, bool bwd) {
   SEMX_REQUIRE(a->d <= kMaxD, SEMX_ERR_UNSUPPORTED, "layer_norm: width %lld > %d", (long long)a->d, kMaxD);
   SEMX_REQUIRE(a->n <= INT64_MAX / kMaxD / 8, SEMX_ERR_SHAPE, "layer_norm: n=%lld", (long long)a->n);
   SEMX_REQUIRE(a->eps >= 0.f, SEMX_ERR_SHAPE, "layer_norm: eps < 0");
+  SEMX_REQUIRE(semx::all_aligned({a->x, a->dx}, a->x_bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->residual, a->dresidual}, a->r_bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->y, a->dy}, a->y_bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->sum, a->dsum}, a->s_bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->weight, a->bias, a->mean, a->rstd, a->dweight, a->dbias, a->workspace}, 4),
+               SEMX_ERR_ALIGN, "layer_norm: a pointer is not on an element");
   if (a->n == 0) return SEMX_OK;
   if (!bwd) {
     SEMX_REQUIRE(a->x && a->y, SEMX_ERR_NULL, "layer_norm: x / y is NULL");

@@ -49,6 +49,13 @@ inline bool aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;
 }
 
+// Whether every pointer lies on an element of `bytes` (NULL does).
+inline bool all_aligned(std::initializer_list<const void*> ptrs, uintptr_t bytes) {
+  for (const void* p : ptrs)
+    if (!aligned(p, bytes)) return false;
+  return true;
+}
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline cudaStream_t as_stream(semx_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }

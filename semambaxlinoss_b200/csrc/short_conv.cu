@@ -463,6 +463,9 @@ int cv_validate(const SemxShortConvArgs* a, bool bwd, CvParams* p) {
   SEMX_REQUIRE(a->w && (a->rows == 0 || a->x), SEMX_ERR_NULL, "short_conv: x / w is NULL");
   if (!bwd) SEMX_REQUIRE(a->rows == 0 || a->y, SEMX_ERR_NULL, "short_conv: y is NULL");
   else SEMX_REQUIRE(a->rows == 0 || (a->dy && a->dx), SEMX_ERR_NULL, "short_conv bwd: dy / dx is NULL");
+  SEMX_REQUIRE(semx::all_aligned({a->x, a->y, a->state, a->dy, a->dx}, a->bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->w, a->b, a->cu_seqlens, a->slots, a->dw, a->db, a->workspace}, 4),
+               SEMX_ERR_ALIGN, "short_conv: a pointer is not on an element");
   p->C = (int)a->C; p->silu = a->silu; p->ldx = a->ldx;
   p->x = a->x; p->w = a->w; p->b = a->b; p->y = a->y; p->state = a->state;
   p->dy = a->dy; p->dx = a->dx;

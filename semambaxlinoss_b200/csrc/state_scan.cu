@@ -356,6 +356,11 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
                  "state_scan bwd: dy / dx / ddt / dB / dC / ckpt is NULL");
     SEMX_REQUIRE(none || a->z == nullptr || (a->dz && a->v), SEMX_ERR_NULL, "state_scan bwd: dz / v is NULL");
   }
+  SEMX_REQUIRE(semx::all_aligned({a->x, a->B, a->Cm, a->z, a->y, a->v, a->dy, a->dx, a->dz, a->dB, a->dC}, a->bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->dt, a->ddt}, a->dt_bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->A, a->D, a->dt_bias, a->cu_seqlens, a->state, a->slots, a->ckpt, a->dA, a->dD,
+                                      a->ddt_bias, a->workspace}, 4),
+               SEMX_ERR_ALIGN, "state_scan: a pointer is not on an element");
   p->C = (int)a->C; p->N = (int)a->N; p->G = (int)a->G; p->cpg = (int)(a->C / a->G);
   p->bf16 = a->bf16; p->dt_bf16 = a->dt_bf16; p->softplus = a->softplus;
   p->ldx = a->ldx; p->lddt = a->lddt; p->ldz = a->ldz; p->ldb = a->ldb; p->ldc = a->ldc;

@@ -169,6 +169,32 @@ def test_views_types_missing_parameters_and_gradients_asked_for():
 
 
 @pytest.mark.gpu
+def test_gradients_against_differences():
+    """The operator's own outputs, moved along one direction of every operand by 2^-7: the slope
+    to about 4 (2^-7)^2 of the terms' size, and the outputs' rounding, 64 2^-24, over the step."""
+    from semambaxlinoss_b200.layer_norm import layer_norm
+
+    dev, g = cuda(), gen(77)
+    t = [randn(s, g).float().to(dev) for s in ((9, 130), (130,), (130,), (9, 130))]
+    move = [randn(u.shape, g, scale=0.3).float().to(dev) for u in t]
+    cy, cs = (randn((9, 130), g).float().to(dev) for _ in range(2))
+
+    def value(x, w, b, r):
+        y, s = layer_norm(x, w, b, residual=r)
+        return (y.double() * cy).sum() + (s.double() * cs).sum(), y, s
+
+    leaves = [u.clone().requires_grad_() for u in t]
+    _, y, s = value(*leaves)
+    grads = torch.autograd.grad((y, s), leaves, (cy, cs))
+    slope = sum((p.double() * m.double()).sum() for p, m in zip(grads, move))
+    size = sum((p.double() * m.double()).abs().sum() for p, m in zip(grads, move))
+    h = 2.0 ** -7
+    up, down = (value(*[u + k * h * m for u, m in zip(t, move)])[0] for k in (1, -1))
+    noise = 64 * EPS32 / h * ((y.double() * cy).abs().sum() + (s.double() * cs).abs().sum())
+    assert ((up - down) / (2 * h) - slope).abs() <= 4 * h * h * size + noise
+
+
+@pytest.mark.gpu
 def test_other_stream_and_captured_graph():
     from semambaxlinoss_b200.layer_norm import layer_norm
 
@@ -226,6 +252,8 @@ def test_refusals():
     assert status("semx_layer_norm_fwd", n=2 ** 62) == _lib.SEMX_ERR_SHAPE
     assert status("semx_layer_norm_fwd", eps=-1.0) == _lib.SEMX_ERR_SHAPE
     assert status("semx_layer_norm_fwd", x=256, y=256, residual=256) == _lib.SEMX_ERR_NULL
+    assert status("semx_layer_norm_fwd", x=258, y=256) == _lib.SEMX_ERR_ALIGN
+    assert status("semx_layer_norm_fwd", x=257, y=256, x_bf16=1) == _lib.SEMX_ERR_ALIGN
     assert status("semx_layer_norm_bwd", sum=256) == _lib.SEMX_ERR_NULL
     assert status("semx_layer_norm_bwd", sum=256, mean=256, rstd=256, dy=256, dx=256, dweight=256) == _lib.SEMX_ERR_WORKSPACE
 

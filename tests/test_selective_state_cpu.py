@@ -98,6 +98,9 @@ def test_conv_status_codes():
         assert fwd(**ptr, **bad) == _lib.SEMX_ERR_SHAPE, bad
     for bad in (dict(state=256), dict(n_slots=2), dict(slots=256), dict(fresh=256)):
         assert fwd(**ptr, **bad) == _lib.SEMX_ERR_NULL, bad
+    for bad in (dict(x=257), dict(y=258), dict(w=258), dict(slots=257, state=256, n_slots=2)):
+        assert fwd(**{**ptr, **bad}) == _lib.SEMX_ERR_ALIGN, bad
+    assert fwd(**{**ptr, "x": 257}, bf16=1) == _lib.SEMX_ERR_ALIGN
     assert bwd(**ptr, dy=256) == _lib.SEMX_ERR_NULL
     assert bwd(**ptr, dy=256, dx=256, dw=256) == _lib.SEMX_ERR_WORKSPACE
     assert bwd(**ptr, dy=256, dx=256, state=256, n_slots=2) == _lib.SEMX_ERR_UNSUPPORTED
@@ -115,6 +118,8 @@ def test_scan_status_codes():
     for bad in (dict(C=0), dict(G=3), dict(G=0), dict(ldx=7), dict(ldb=7), dict(z=256, ldz=7), dict(rows=9),
                 dict(state=256, n_slots=1)):
         assert fwd(**ptr, **bad) == _lib.SEMX_ERR_SHAPE, bad
+    for bad in (dict(x=258), dict(dt=257, dt_bf16=1), dict(A=258), dict(state=258, n_slots=2)):
+        assert fwd(**{**ptr, **bad}) == _lib.SEMX_ERR_ALIGN, bad
     assert _status("semx_state_scan_bwd", cls, base, **ptr, dy=256) == _lib.SEMX_ERR_NULL
     back = dict(ptr, dy=256, dx=256, ddt=256, dB=256, dC=256, ckpt=256)
     assert _status("semx_state_scan_bwd", cls, base, **back) == _lib.SEMX_ERR_WORKSPACE

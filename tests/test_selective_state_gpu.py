@@ -392,6 +392,30 @@ def test_bad_offsets_stay_inside():
         torch.cuda.synchronize()
 
 
+def test_offsets_past_32_bits():
+    """Operands that are slices of rows 2^20 elements long: row 2500 begins behind element 2^31.
+    The same values as with rows of their own, bit for bit."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, short_conv
+
+    rows, ch, N = 2600, 32, 16
+    wide = torch.empty(rows, 1 << 20, dtype=torch.bfloat16, device=cuda())
+    part = wide[:, -(3 * ch + 2 * N):]
+    part.normal_()
+    x, dt, z, B, C = part.split([ch, ch, ch, N, N], -1)
+    A = -torch.rand(ch, N, device=cuda()) - 0.1
+    w = torch.randn(ch, 4, device=cuda())
+    cu = torch.tensor([0, 700, 2590], dtype=torch.int32, device=cuda())
+
+    def run(x, dt, z, B, C):
+        leaves = [t.detach().requires_grad_() for t in (x, dt, z, B, C)]
+        u = short_conv(leaves[0], w, cu_seqlens=cu)
+        y = selective_state_scan(u, leaves[1], A, leaves[3], leaves[4], z=leaves[2], cu_seqlens=cu)
+        return [y] + list(torch.autograd.grad(y, leaves, torch.ones_like(y)))
+
+    for p, q in zip(run(x, dt, z, B, C), run(*[t.contiguous() for t in (x, dt, z, B, C)])):
+        assert torch.equal(p, q)
+
+
 def test_no_sequences_and_no_rows():
     from semambaxlinoss_b200.selective_state import selective_state_scan, selective_state_step, short_conv
 
