@@ -166,7 +166,7 @@ __device__ __forceinline__ void load_param(const float* p, int t, int d, float n
 }
 
 // Rows of at most 512 elements keep the parameters in registers from row to row; wider ones
-// read them again from L1, which leaves registers for two CTAs of 512 threads per SM.
+// read them again from L1, which leaves registers for the row that is on its way.
 template <int TPR>
 constexpr bool keeps_params() {
   return TPR <= 32;
@@ -388,32 +388,23 @@ __global__ void __launch_bounds__(cta_threads<TPR>(), ctas_per_sm<TPR, V>()) lay
   }
 }
 
-// CTAs of a launch: one wave of what an SM holds, so that a CTA sees many rows and leaves
-// one row of partial sums for all of them (8192 x 4096: two waves 127 us, one 110 us).
-constexpr int kFwdCtas = 148 * 4;
+// CTAs of a launch: one wave of what an SM holds, so that a CTA sees many rows, always has
+// the next one on its way and leaves one row of partial sums for all of them (8192 x 4096:
+// backward in two waves 127 us, one 110 us; forward 83 and 73 us).
 int rows_per_cta(int64_t d) { return d <= 64 ? 16 : d <= 128 ? 8 : d <= 512 ? 4 : 1; }
-int64_t bwd_ctas(int64_t n, int64_t d) {
+int64_t ln_ctas(int64_t n, int64_t d) {
   const int64_t want = semx::cdiv(n, rows_per_cta(d)), most = 148 * (d <= 2048 ? 4 : d <= 4096 ? 2 : 1);
   return want < most ? want : most;
 }
 
 template <bool VEC>
 int launch_ln(bool bwd, const LnParams& p, cudaStream_t st) {
-  const int64_t rows = rows_per_cta(p.d), want = semx::cdiv(p.n, rows);
-  const unsigned grid = (unsigned)(bwd ? bwd_ctas(p.n, p.d) : want < kFwdCtas ? want : kFwdCtas);
-  // A row's threads, 8 V elements each: more threads before more elements in the forward; the
-  // backward, which also keeps dw and db, takes two steps' elements per thread and half the
-  // threads.
+  const unsigned grid = (unsigned)ln_ctas(p.n, p.d);
+  // A row's threads, 8 V elements each.
 #define SEMX_LN(DMAX, TPR, V)                                                                             \
   if (p.d <= DMAX) {                                                                                      \
     if (bwd) layer_norm_bwd_kernel<TPR, V, VEC><<<grid, cta_threads<TPR>(), 0, st>>>(p);                  \
     else layer_norm_fwd_kernel<TPR, V, VEC><<<grid, cta_threads<TPR>(), 0, st>>>(p);                      \
-    return semx::check_launch(bwd ? "layer_norm_bwd_kernel" : "layer_norm_fwd_kernel");                   \
-  }
-#define SEMX_LN2(DMAX, TPR, BTPR, BV)                                                                     \
-  if (p.d <= DMAX) {                                                                                      \
-    if (bwd) layer_norm_bwd_kernel<BTPR, BV, VEC><<<grid, cta_threads<BTPR>(), 0, st>>>(p);               \
-    else layer_norm_fwd_kernel<TPR, 1, VEC><<<grid, cta_threads<TPR>(), 0, st>>>(p);                      \
     return semx::check_launch(bwd ? "layer_norm_bwd_kernel" : "layer_norm_fwd_kernel");                   \
   }
   SEMX_LN(64, 8, 1)
@@ -421,13 +412,12 @@ int launch_ln(bool bwd, const LnParams& p, cudaStream_t st) {
   SEMX_LN(256, 32, 1)
   SEMX_LN(512, 32, 2)
   SEMX_LN(1024, 128, 1)
-  SEMX_LN2(2048, 256, 128, 2)
-  SEMX_LN2(4096, 512, 256, 2)
-  SEMX_LN2(8192, 1024, 512, 2)
+  SEMX_LN(2048, 128, 2)
+  SEMX_LN(4096, 256, 2)
+  SEMX_LN(8192, 512, 2)
   SEMX_LN(16384, 1024, 2)
   SEMX_LN(32768, 1024, 4)
 #undef SEMX_LN
-#undef SEMX_LN2
   return semx::fail(SEMX_ERR_UNSUPPORTED, "layer_norm: width %d", p.d);
 }
 
@@ -479,7 +469,7 @@ size_t semx_layer_norm_args_size(void) { return sizeof(SemxLayerNormArgs); }
 
 size_t semx_layer_norm_workspace_bytes(const SemxLayerNormArgs* a) {
   if (a == nullptr || a->n < 0 || a->d < 1 || a->d > kMaxD) return 0;
-  const int64_t rows = bwd_ctas(a->n, a->d);
+  const int64_t rows = ln_ctas(a->n, a->d);
   return (size_t)rows * 2 * a->d * sizeof(float);
 }
 
@@ -514,7 +504,7 @@ int semx_layer_norm_bwd(const SemxLayerNormArgs* a, semx_stream_t stream) {
     if (rc != SEMX_OK) return rc;
   }
   if (!params) return SEMX_OK;
-  const int64_t rows = bwd_ctas(a->n, a->d);
+  const int64_t rows = ln_ctas(a->n, a->d);
   semx::Segments seg = {};
   seg.n = 2;
   seg.out[0] = a->dweight;

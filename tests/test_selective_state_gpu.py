@@ -374,6 +374,23 @@ def test_steps_far_out():
         assert ((y - want)[:-1].abs() <= 8 * EPS * want[:-1] + 2.0 ** -126).all()
 
 
+@pytest.mark.parametrize("L", [1, 3, 16, 18])
+def test_a_step_of_zero_keeps_the_state(L):
+    """dt = -inf is a step of exactly zero: pole 1, no drive; the entry keeps its bits, at lengths
+    that end inside a tile too (rows behind the end are steps of zero)."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, selective_state_step
+
+    ch, N = 70, 16
+    A, BC = -torch.rand(ch, N, device=cuda()) * 20, torch.randn(2, L, N, device=cuda())
+    x, dt = torch.randn(2, L, ch, device=cuda()), torch.full((2, L, ch), float("-inf"), device=cuda())
+    state = torch.randn(2, ch, N, device=cuda())
+    kept = state.clone()
+    y = selective_state_scan(x, dt, A, BC, BC, state=state)
+    assert torch.equal(state, kept) and torch.isfinite(y).all()
+    selective_state_step(x[:, 0], dt[:, 0], A, BC[:, 0], BC[:, 0], state)
+    assert torch.equal(state, kept)
+
+
 def test_bad_offsets_stay_inside():
     """Offsets that decrease, start below zero or reach behind the rows give some result
     without an access outside (they are clamped in the kernels)."""
