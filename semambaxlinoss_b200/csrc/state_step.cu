@@ -16,7 +16,7 @@ namespace {
 using namespace semx_scan;
 
 constexpr int kAhead = 4;
-constexpr int kStepRows = 16;  // sequences per CTA at most
+constexpr int kStepRows = 8;  // sequences per CTA at most
 
 // ACC: how B and C are read; the state is read four modes at a time unless ACC is kAny.
 template <int GL, int ACC>

@@ -26,27 +26,31 @@ _F32 = (torch.float32,)
 def _check(op, x, dt, A, B, C, D, z, dt_bias):
     """Shapes and types; returns (channels, modes, groups)."""
     shape, dtype, dev = x.shape, x.dtype, x.get_device()
-    ch = shape[-1]
-    Ashape = A.shape
+    ch, Ashape = shape[-1], A.shape
     if len(Ashape) != 2 or Ashape[0] != ch or not 1 <= Ashape[1] <= MAX_MODES:
         raise ValueError(f"{op}: A must be ({ch}, modes) with 1 to {MAX_MODES} modes, got {tuple(Ashape)}")
-    N = Ashape[1]
-    check_same(op, "A", A, Ashape, TYPES, dev)
-    check_same(op, "dt", dt, shape, _F32 if dtype == torch.float32 else TYPES, dev)
-    grouped = B.dim() == len(shape) + 1
-    G = B.shape[-2] if grouped else 1
+    N, Bshape = Ashape[1], B.shape
+    grouped = len(Bshape) == len(shape) + 1
+    G = Bshape[-2] if grouped else 1
     if G < 1 or ch % G:
         raise ValueError(f"{op}: {ch} channels do not fall into {G} groups")
-    own = (dtype,)
     want = shape[:-1] + ((G, N) if grouped else (N,))
-    check_same(op, "B", B, want, own, dev)
-    check_same(op, "C", C, want, own, dev)
-    if z is not None:
-        check_same(op, "z", z, shape, own, dev)
-    if D is not None:
-        check_same(op, "D", D, (ch,), TYPES, dev)
-    if dt_bias is not None:
-        check_same(op, "dt_bias", dt_bias, (ch,), TYPES, dev)
+    types = _F32 if dtype == torch.float32 else TYPES
+    # One expression for the calls that are right, which a decoding loop makes thousands of.
+    if not (dt.shape == shape and Bshape == want and C.shape == want and dt.dtype in types and A.dtype in TYPES
+            and B.dtype == dtype and C.dtype == dtype and dt.get_device() == dev and A.get_device() == dev
+            and B.get_device() == dev and C.get_device() == dev
+            and (z is None or (z.shape == shape and z.dtype == dtype and z.get_device() == dev))
+            and (D is None or (D.shape == (ch,) and D.dtype in TYPES and D.get_device() == dev))
+            and (dt_bias is None or (dt_bias.shape == (ch,) and dt_bias.dtype in TYPES and dt_bias.get_device() == dev))):
+        check_same(op, "A", A, Ashape, TYPES, dev)
+        check_same(op, "dt", dt, shape, types, dev)
+        for name, t, s in (("B", B, want), ("C", C, want), ("z", z, shape)):
+            if t is not None:
+                check_same(op, name, t, s, (dtype,), dev)
+        for name, t in (("D", D), ("dt_bias", dt_bias)):
+            if t is not None:
+                check_same(op, name, t, (ch,), TYPES, dev)
     return ch, N, G
 
 
@@ -59,7 +63,7 @@ def _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
 
 def _args(x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu, N, G):
     """The argument struct, and what has to outlive the call."""
-    ch = x.shape[-1]
+    ch = A.shape[0]
     inner = B.dim() - x.dim() + 1  # (groups, modes) or (modes,)
     x, ldx = rows_of(x, ch)
     dt, ldd = rows_of(dt, ch)
