@@ -50,7 +50,7 @@ __global__ void colsum_stage2(const float* __restrict__ group_sums, int64_t G, i
 // One-launch form for tall, narrow partial sums: a CTA takes COLS columns, its 1024 / COLS
 // row lanes every (1024 / COLS)-th row each, and the lanes' sums are added in lane order. The
 // order is fixed too, but it is another one than colsum's, so the two do not give the same
-// bits. 2424 rows of 1280: 16 us in two launches, 5 us in this one.
+// bits. 2424 rows of 1280: 16 us in two launches, 8 us in this one.
 template <int COLS>
 __global__ void __launch_bounds__(1024) colsum_once_kernel(const float* __restrict__ rows, int64_t S, int64_t K,
                                                            Segments seg) {
@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(1024) colsum_once_kernel(const float* __restri
 
 inline int colsum_once(const float* rows, int64_t S, int64_t K, const Segments& seg, cudaStream_t st) {
   if (K <= 0) return SEMX_OK;
-  // Few columns: narrower CTAs, so that they still fill the GPU.
+  // Few columns: narrower CTAs, so that they still fill the GPU (2424 rows of 1280 columns: 32
+  // columns per CTA 22.8 us, 8 columns 10.8 with 4 rows loaded ahead, 8 with 8).
   if (K < 32 * 148) colsum_once_kernel<8><<<(unsigned)cdiv(K, 8), 1024, 0, st>>>(rows, S, K, seg);
   else colsum_once_kernel<32><<<(unsigned)cdiv(K, 32), 1024, 0, st>>>(rows, S, K, seg);
   return check_launch("colsum_once_kernel");

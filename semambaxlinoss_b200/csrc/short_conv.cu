@@ -441,7 +441,9 @@ int launch_step(int K, CvParams& p, cudaStream_t st) {
 }
 
 // Rows of a piece: long pieces re-read few rows (K - 1 in front, and K - 1 behind in the
-// backward) and leave few rows of partial sums; short ones fill the GPU.
+// backward) and leave few rows of partial sums; short ones fill the GPU. Always long against
+// this rule, bf16, 4 taps: 600 x 1024 forward 7.8 and 6.4 us, training pass 26.7 and 17.7;
+// 150 x 256 7.8 and 6.1, 26.2 and 15.2; 6151 x 2048 the same.
 constexpr int64_t kFill = 148 * 512;  // threads
 int64_t piece_rows(int64_t T, int64_t C, bool bwd) {
   int64_t Q = bwd ? 64 : 32;

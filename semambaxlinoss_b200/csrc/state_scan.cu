@@ -387,15 +387,18 @@ namespace {
 // Rows per piece of a forward (0: whole sequences). Pieces cost the exponentials twice, so
 // only batches that leave half of the GPU idle are cut (4 x 2047 x 2048: whole 275 us, in
 // pieces 216 us), into two waves of the four CTAs that an SM holds: the second evens out
-// what the first leaves uneven (one wave 235 us, three 212 us, but of shorter pieces).
+// what the first leaves uneven (one wave 235 us, three 212 us, but of shorter pieces). Three
+// launches against one pay from about 100 rows on (one sequence of 256 channels: 100 rows
+// 15.9 us whole and 15.7 in pieces, 256 rows 34.8 and 15.9), and pieces of 32 rows still do
+// (512 rows: pieces of at least 64 rows 22.0 us, 32 rows 16.6).
 constexpr int64_t kResident = 148 * 4;
 int64_t fwd_rows_per_piece(const ScanParams& p) {
   const int64_t ch = kThreads / lanes_for(p.N, 4) * kCPT;
   const int64_t ctas = p.m.S * p.G * semx::cdiv(p.cpg, ch);
   const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
-  if (2 * ctas > kResident || rows <= 128) return 0;
+  if (2 * ctas > kResident || rows <= 96) return 0;
   const int64_t Q = semx::cdiv(semx::cdiv(rows, 2 * kResident / ctas), 16) * 16;
-  return Q < 64 ? 64 : Q;
+  return Q < 32 ? 32 : Q;
 }
 
 size_t split_floats(const ScanParams& p) { return (size_t)p.m.pieces * p.C * (p.N + 1); }

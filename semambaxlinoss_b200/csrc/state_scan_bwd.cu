@@ -516,14 +516,16 @@ void set_tiles(ScanParams& p) {
 }
 
 // Rows per piece (0: whole sequences): as in the forward, with three resident CTAs per SM and
-// about five waves (4 x 2047 x 2048: whole 590 us, one wave 475 us, five 408 us).
+// about five waves (4 x 2047 x 2048: whole 590 us, one wave 475 us, five 408 us). One sequence
+// of 100 rows and 256 channels, training pass: whole 56.5 us, in pieces 45.9; of 512 rows:
+// whole 177 us, pieces of at least 64 rows 63.3, of 32 rows 52.1.
 constexpr int64_t kResident = 148 * 3;
 int64_t bwd_rows_per_piece(const ScanParams& p) {
   const int64_t ctas = (int64_t)p.m.S * p.ctiles;
   const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
-  if (2 * ctas > kResident || rows <= 128) return 0;
+  if (2 * ctas > kResident || rows <= 64) return 0;
   const int64_t Q = semx::cdiv(semx::cdiv(rows, 5 * kResident / ctas), kBlock) * kBlock;
-  return Q < 64 ? 64 : Q;
+  return Q < 32 ? 32 : Q;
 }
 
 struct Layout {

@@ -131,7 +131,8 @@ int semx_state_step(const SemxStateScanArgs* a, semx_stream_t stream) {
   cudaStream_t st = semx::as_stream(stream);
   const int gl = lanes_for(p.N, 4);
   p.ctiles = (int)semx::cdiv(p.C, (int64_t)(kThreads / gl));
-  // Sequences per CTA: as many as leave eight CTAs per SM.
+  // Sequences per CTA: as many as leave eight CTAs per SM (192 x 4096, cold state: at most 4
+  // 31.7 us, 8 28.6, 16 31.7).
   int rows = kStepRows;
   while (rows > 1 && semx::cdiv(p.m.S, rows) * p.ctiles < 148 * 8) rows /= 2;
   const int64_t grid = semx::cdiv(p.m.S, rows) * p.ctiles;
