@@ -78,7 +78,10 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
       store_quad<ACC>(p.y, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
       if (p.v != nullptr) store_quad<ACC>(p.v, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
     }
-  if (!q.live) return;
+  // A sequence of one piece needs neither a first pass nor joining: its piece starts from the
+  // pool's entry and leaves its state there.
+  const bool split = p.entry != nullptr && q.len > p.m.Q;
+  if (!q.live || (LOCAL && !split)) return;
 
   // The channels and modes of this thread in the scan.
   const int lm = tid % GL, cp = tid / GL, sc = cp * kCPT;
@@ -95,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
     A2[i][0] = a.x * kLog2e; A2[i][1] = a.y * kLog2e; A2[i][2] = a.z * kLog2e; A2[i][3] = a.w * kLog2e;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (!LOCAL) {
-      if (p.entry != nullptr) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
+      if (split) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
       else if (!cold) s = load_params(p.state, slot * p.C * p.N + at0 + i * p.N, nn[i]);
     }
     h[i][0] = pack2(s.x, s.y);
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
       oy += TT * (int64_t)p.C;
     }
   }
-  float* out = LOCAL ? p.entry + j * p.C * p.N : p.entry == nullptr && slot >= 0 ? p.state + slot * p.C * p.N : nullptr;
+  float* out = LOCAL ? p.entry + j * p.C * p.N : !split && slot >= 0 ? p.state + slot * p.C * p.N : nullptr;
   if (out != nullptr) {
 #pragma unroll
     for (int i = 0; i < kCPT; ++i) {
@@ -266,41 +269,44 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   }
 }
 
-// Joins the pieces of a sequence: entry[j] becomes the state in front of piece j, the last
-// state goes to the pool. One thread per (sequence, channel, mode).
+// Joins the pieces of the sequences that have more than one: entry[j] becomes the state in
+// front of piece j, the last state goes to the pool. A thread owns a (channel, mode); a CTA
+// walks over every gridDim.y-th sequence.
 __global__ void __launch_bounds__(kThreads) state_scan_join_kernel(const ScanParams p) {
   const int64_t per = (int64_t)p.C * p.N;
-  const int64_t tiles = (per + kThreads - 1) / kThreads;
-  const int64_t s = blockIdx.x / tiles;
-  const int64_t i = (blockIdx.x % tiles) * kThreads + threadIdx.x;
-  const int64_t slot = find_slot(p.m, s);
-  if (i >= per) return;
-  const int64_t c = i / p.N;
-  const float A2 = p.A[i] * kLog2e;
-  const int64_t row0 = seq_start(p.m, s);
-  const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;
-  const int64_t base = piece_base(p.m, s, p.m.Q), n = (len + p.m.Q - 1) / p.m.Q;
-  const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[s] != 0);
-  float h = cold ? 0.f : p.state[slot * per + i];
-  // Batches of loads ahead of the chain: entry is written where it was read.
-  constexpr int U = 8;
-  for (int64_t k = 0; k < n; k += U) {
-    float local[U], decay[U];
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (!any_split(p.m)) return;
+  const int64_t c = min(i, per - 1) / p.N;
+  const float A2 = p.A[min(i, per - 1)] * kLog2e;
+  for (int64_t s = blockIdx.y; s < p.m.S; s += gridDim.y) {
+    const int64_t row0 = seq_start(p.m, s);
+    const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;
+    if (len <= p.m.Q) continue;
+    const int64_t slot = find_slot(p.m, s);
+    if (i >= per) continue;
+    const int64_t base = piece_base(p.m, s, p.m.Q), n = (len + p.m.Q - 1) / p.m.Q;
+    const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[s] != 0);
+    float h = cold ? 0.f : p.state[slot * per + i];
+    // Batches of loads ahead of the chain: entry is written where it was read.
+    constexpr int U = 8;
+    for (int64_t k = 0; k < n; k += U) {
+      float local[U], decay[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t j = base + k + u;
-      local[u] = k + u < n ? p.entry[j * per + i] : 0.f;
-      decay[u] = k + u < n ? p.dsum[j * p.C + c] : 0.f;
-    }
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = base + k + u;
+        local[u] = k + u < n ? p.entry[j * per + i] : 0.f;
+        decay[u] = k + u < n ? p.dsum[j * p.C + c] : 0.f;
+      }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (k + u < n) {
-        p.entry[(base + k + u) * per + i] = h;
-        h = fmaf(semx::ex2_approx(decay[u] * A2), h, local[u]);
+      for (int u = 0; u < U; ++u) {
+        if (k + u < n) {
+          p.entry[(base + k + u) * per + i] = h;
+          h = fmaf(semx::ex2_approx(decay[u] * A2), h, local[u]);
+        }
       }
     }
+    if (slot >= 0) p.state[slot * per + i] = h;
   }
-  if (slot >= 0) p.state[slot * per + i] = h;
 }
 
 template <bool LOCAL>
@@ -390,13 +396,15 @@ namespace {
 // what the first leaves uneven (one wave 235 us, three 212 us, but of shorter pieces). Three
 // launches against one pay from about 100 rows on (one sequence of 256 channels: 100 rows
 // 15.9 us whole and 15.7 in pieces, 256 rows 34.8 and 15.9), and pieces of 32 rows still do
-// (512 rows: pieces of at least 64 rows 22.0 us, 32 rows 16.6).
+// (512 rows: pieces of at least 64 rows 22.0 us, 32 rows 16.6). Batches that fill the GPU are
+// cut at outlier_rows() if their lengths are not known to be equal.
 constexpr int64_t kResident = 148 * 4;
 int64_t fwd_rows_per_piece(const ScanParams& p) {
   const int64_t ch = kThreads / lanes_for(p.N, 4) * kCPT;
   const int64_t ctas = p.m.S * p.G * semx::cdiv(p.cpg, ch);
   const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
-  if (2 * ctas > kResident || rows <= 96) return 0;
+  if (2 * ctas > kResident) return p.m.cu != nullptr && p.m.S > 1 ? outlier_rows(rows) : 0;
+  if (rows <= 96) return 0;
   const int64_t Q = semx::cdiv(semx::cdiv(rows, 2 * kResident / ctas), 16) * 16;
   return Q < 32 ? 32 : Q;
 }
@@ -433,9 +441,7 @@ int semx_state_scan_fwd(const SemxStateScanArgs* a, semx_stream_t stream) {
     p.dsum = p.entry + (size_t)p.m.pieces * p.C * p.N;
     rc = launch_fwd<true>(p, st);
     if (rc != SEMX_OK) return rc;
-    const int64_t grid = p.m.S * semx::cdiv((int64_t)p.C * p.N, kThreads);
-    if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan: too many sequences");
-    state_scan_join_kernel<<<(unsigned)grid, kThreads, 0, st>>>(p);
+    state_scan_join_kernel<<<join_grid(p), kThreads, 0, st>>>(p);
     rc = semx::check_launch("state_scan_join_kernel");
     if (rc != SEMX_OK) return rc;
   }

@@ -202,6 +202,35 @@ __device__ __forceinline__ float4 gate4(float4 v, float4 z) {
                      v.w * (z.w * sigmoid(z.w)));
 }
 
+// Rows at which a sequence of a packed batch is cut although the batch as a whole fills the
+// GPU: one far longer than the mean (a prompt beside single tokens) would run on alone. The
+// others stay whole and cost the two additional launches. 8192 rows of 1024 channels in 64
+// sequences: one of 7940 rows and 63 of 4, whole 979 us, cut at 4 times the mean 191 us; all of
+// 128 rows, 64 us and 70.
+inline int64_t outlier_rows(int64_t mean) {
+  const int64_t Q = (4 * mean + 15) / 16 * 16;
+  return Q < 128 ? 128 : Q;
+}
+
+// CTAs that join pieces: the (channel, mode)s across, a few of the sequences at a time down.
+inline dim3 join_grid(const ScanParams& p) {
+  const int64_t tiles = semx::cdiv((int64_t)p.C * p.N, kThreads);
+  int64_t down = semx::cdiv((int64_t)148 * 16, tiles);
+  if (down > p.m.S) down = p.m.S;
+  return dim3((unsigned)tiles, (unsigned)(down < 1 ? 1 : down > 65535 ? 65535 : down));
+}
+
+// Whether one of the sequences that the CTA walks over (every gridDim.y-th) has more than one
+// piece. Called by all threads of the CTA.
+__device__ __forceinline__ bool any_split(const semx::SeqMap& m) {
+  int found = 0;
+  for (int64_t s = blockIdx.y + (int64_t)threadIdx.x * gridDim.y; s < m.S; s += (int64_t)blockDim.x * gridDim.y) {
+    const int64_t row0 = seq_start(m, s);
+    found |= (m.cu == nullptr ? m.L : seq_start(m, s + 1) - row0) > m.Q;
+  }
+  return __syncthreads_or(found) != 0;
+}
+
 // Lanes per channel for N modes, MPT per thread.
 inline int lanes_for(int N, int mpt) {
   int g = 1;

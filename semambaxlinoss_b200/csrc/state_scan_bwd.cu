@@ -110,6 +110,9 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_s
   const int grp = ct / p.tpg, cg0 = (ct % p.tpg) * CH, c_base = grp * p.cpg;
   const Piece q = find_piece(p.m, j);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+  // A sequence of one piece needs neither a first pass nor joining.
+  const bool split = p.entry != nullptr && q.live && q.len > p.m.Q;
+  if (LOCAL && !split) return;
 
   // The four channels of this thread in loads and stores (en of them exist).
   const int eq = tid % (CH / 4), ec = eq * 4, et = tid / (CH / 4);
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_s
     A2[i][0] = pack2(a.x * kLog2e, a.y * kLog2e);
     A2[i][1] = pack2(a.z * kLog2e, a.w * kLog2e);
     float4 s = zero4;
-    if (!LOCAL && q.live) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
+    if (!LOCAL && split) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
     carry[i][0] = pack2(s.x, s.y);
     carry[i][1] = pack2(s.z, s.w);
     dA[i][0] = dA[i][1] = 0ull;
@@ -419,7 +422,6 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_s
       }
     }
   }
-  if (LOCAL && !q.live) return;
   float* out = LOCAL ? p.entry + j * p.C * p.N : p.part != nullptr ? p.part + j * ((int64_t)p.C * (p.N + 2)) : nullptr;
   if (out == nullptr) return;
   // Without LOCAL every piece index writes its row, zeros where there is no such piece.
@@ -444,34 +446,36 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_s
   }
 }
 
-// Joins the pieces' carries from the last piece of a sequence: entry[j] becomes the gradient
-// of the state behind piece j. One thread per (sequence, channel, mode).
+// Joins the carries of the pieces of the sequences that have more than one, from the last
+// piece: entry[j] becomes the gradient of the state behind piece j. Threads as in the forward.
 __global__ void __launch_bounds__(kThreads) state_scan_join_back_kernel(const ScanParams p) {
   const int64_t per = (int64_t)p.C * p.N;
-  const int64_t tiles = (per + kThreads - 1) / kThreads;
-  const int64_t s = blockIdx.x / tiles;
-  const int64_t i = (blockIdx.x % tiles) * kThreads + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (!any_split(p.m)) return;
   if (i >= per) return;
   const int64_t c = i / p.N;
   const float A2 = p.A[i] * kLog2e;
-  const int64_t row0 = seq_start(p.m, s);
-  const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;
-  const int64_t base = piece_base(p.m, s, p.m.Q), n = (len + p.m.Q - 1) / p.m.Q;
-  float carry = 0.f;
-  constexpr int U = 8;  // loads ahead of the chain: entry is written where it was read
-  for (int64_t k = n - 1; k >= 0; k -= U) {
-    float local[U], decay[U];
+  for (int64_t s = blockIdx.y; s < p.m.S; s += gridDim.y) {
+    const int64_t row0 = seq_start(p.m, s);
+    const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;
+    if (len <= p.m.Q) continue;
+    const int64_t base = piece_base(p.m, s, p.m.Q), n = (len + p.m.Q - 1) / p.m.Q;
+    float carry = 0.f;
+    constexpr int U = 8;  // loads ahead of the chain: entry is written where it was read
+    for (int64_t k = n - 1; k >= 0; k -= U) {
+      float local[U], decay[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t j = base + k - u;
-      local[u] = k - u >= 0 ? p.entry[j * per + i] : 0.f;
-      decay[u] = k - u >= 0 ? p.dsum[j * p.C + c] : 0.f;
-    }
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = base + k - u;
+        local[u] = k - u >= 0 ? p.entry[j * per + i] : 0.f;
+        decay[u] = k - u >= 0 ? p.dsum[j * p.C + c] : 0.f;
+      }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (k - u >= 0) {
-        p.entry[(base + k - u) * per + i] = carry;
-        carry = fmaf(semx::ex2_approx(decay[u] * A2), carry, local[u]);
+      for (int u = 0; u < U; ++u) {
+        if (k - u >= 0) {
+          p.entry[(base + k - u) * per + i] = carry;
+          carry = fmaf(semx::ex2_approx(decay[u] * A2), carry, local[u]);
+        }
       }
     }
   }
@@ -523,7 +527,8 @@ constexpr int64_t kResident = 148 * 3;
 int64_t bwd_rows_per_piece(const ScanParams& p) {
   const int64_t ctas = (int64_t)p.m.S * p.ctiles;
   const int64_t rows = p.m.S > 0 ? semx::cdiv(p.m.T, p.m.S) : 0;
-  if (2 * ctas > kResident || rows <= 64) return 0;
+  if (2 * ctas > kResident) return p.m.cu != nullptr && p.m.S > 1 ? outlier_rows(rows) : 0;
+  if (rows <= 64) return 0;
   const int64_t Q = semx::cdiv(semx::cdiv(rows, 5 * kResident / ctas), kBlock) * kBlock;
   return Q < 32 ? 32 : Q;
 }
@@ -619,9 +624,7 @@ int semx_state_scan_bwd(const SemxStateScanArgs* a, semx_stream_t stream) {
       p.dsum = ws + l.dsum;
       rc = launch_bwd<true>(p, st);
       if (rc != SEMX_OK) return rc;
-      const int64_t grid = p.m.S * semx::cdiv((int64_t)p.C * p.N, kThreads);
-      if (grid >= ((int64_t)1 << 31)) return semx::fail(SEMX_ERR_SHAPE, "state_scan bwd: too many sequences");
-      state_scan_join_back_kernel<<<(unsigned)grid, kThreads, 0, st>>>(p);
+      state_scan_join_back_kernel<<<join_grid(p), kThreads, 0, st>>>(p);
       rc = semx::check_launch("state_scan_join_back_kernel");
       if (rc != SEMX_OK) return rc;
     }

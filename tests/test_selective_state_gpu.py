@@ -252,6 +252,54 @@ def test_long_sequences_in_pieces_equal_whole_ones():
     assert (one - two).abs().max() <= (8 * L + 64) * EPS * 4 * one.abs().max()
 
 
+def test_a_long_prompt_among_short_ones():
+    """A packed batch that fills the GPU with one sequence far longer than the others, which is
+    then cut while they stay whole: outputs, states and gradients of every sequence are those
+    of the sequence alone, within both ways' rounding; a refused slot and an absent one too."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan
+
+    g, ch, N = gen(17), 520, 16
+    lens = [3, 900, 1, 0] + [2 + i % 7 for i in range(50)]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    rows, S = cu[-1] + 5, len(lens)
+    t = {k: u.to(cuda()) for k, u in _scan_problem(rows, ch, N, 1, g, torch.float32).items()}
+    cud = torch.tensor(cu, dtype=torch.int32, device=cuda())
+    par = {k: t[k] for k in ("D", "dt_bias")}
+    units = (16 * 900 + 128) * EPS * 4
+
+    def run(sel, **kw):
+        v = {k: t[k][sel].clone().requires_grad_() for k in ("x", "dt", "B", "C", "z")}
+        y = selective_state_scan(v["x"], v["dt"], t["A"], v["B"], v["C"], z=v["z"], **par, **kw)
+        return [y] + list(torch.autograd.grad(y, list(v.values()), torch.ones_like(y)))
+
+    whole = run(slice(None), cu_seqlens=cud)
+    pool = torch.randn(S + 1, ch, N, device=cuda())
+    slots = torch.randperm(S + 1, generator=g)[:S].to(torch.int32)
+    slots[0], slots[4] = -1, slots[1]  # no entry; the long prompt's entry again
+    after = pool.clone()
+    with torch.no_grad():
+        y = selective_state_scan(t["x"], t["dt"], t["A"], t["B"], t["C"], z=t["z"], **par, cu_seqlens=cud, state=after,
+                                 slots=slots.to(cuda()))
+    assert torch.isnan(y[cu[4]:cu[5]]).all()
+    for s in (0, 1, 2, 5, S - 1):
+        sel = slice(cu[s], cu[s + 1])
+        one = torch.tensor([0, lens[s]], dtype=torch.int32, device=cuda())
+        for p, q in zip(whole, run(sel, cu_seqlens=one)):
+            assert (p[sel] - q).abs().max() <= units * q.abs().max(), s
+        state = pool[slots[s].clamp(min=0)][None].clone() if slots[s] >= 0 else torch.zeros(1, ch, N, device=cuda())
+        with torch.no_grad():
+            want = selective_state_scan(t["x"][sel], t["dt"][sel], t["A"], t["B"][sel], t["C"][sel], z=t["z"][sel], **par,
+                                        cu_seqlens=one, state=state)
+        assert (y[sel] - want).abs().max() <= units * want.abs().max(), s
+        if slots[s] >= 0:
+            assert (after[slots[s]] - state[0]).abs().max() <= units * state.abs().max(), s
+    for e in [i for i in range(S + 1) if i not in slots.tolist()] + [int(slots[3])]:
+        assert torch.equal(after[e], pool[e])
+    assert not y[cu[-1]:].any() and not whole[1][cu[-1]:].any()
+
+
 @pytest.mark.parametrize("S", [1, 5, 150])
 @pytest.mark.parametrize("ch,N,G,K", [(8, 4, 1, 4), (65, 16, 1, 4), (24, 3, 2, 2), (12, 128, 2, 3), (520, 16, 1, 8)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
