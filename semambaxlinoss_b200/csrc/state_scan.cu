@@ -7,7 +7,9 @@
 // clock per SM) and 4 N multiply-adds, against 8 to 16 bytes moved. So every exponential is
 // evaluated once where the batch fills the GPU, and everything else is kept off the units
 // that evaluate them: A is scaled by log2(e) once, d and d x are evaluated once per (step,
-// channel) and shared through shared memory.
+// channel) and shared through shared memory. Measured: 404 x 321 x 256 fp32 training forward
+// 243 us (exponentials alone 114, its bytes 142); in 4 x 2047 x 2048 bf16 the unit is busy 58 %
+// of the main pass and 77 % of the first one (profiles/selective_state_scan.md).
 //
 // Split: a thread owns two channels and 4 modes of each (two pairs, each in one register pair
 // for the two-wide multiply-adds), GL neighbouring lanes a channel; a CTA of 128 threads

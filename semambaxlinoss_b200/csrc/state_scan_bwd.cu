@@ -7,10 +7,12 @@
 //   dx = d gB + D dv, dd = uA + x gB, ddt = dd softplus'(dt + bias), dz = dy v silu'(z),
 //   dD += dv x, ddt_bias += ddt
 //
-// Bound: instruction issue, then the special-function unit. The forward left the state in
-// front of every kBlock steps, so a block's states and poles are rebuilt from it in
-// registers and the adjoint runs back through them: every exponential is evaluated once
-// (one that kept fewer states would evaluate them twice).
+// Bound: instructions (24 per (step, channel, mode) of a warp, a quarter of them the exchanges
+// between lanes) and shared memory's path to the registers, at 59 % and 61 % of their rates in
+// 4 x 2047 x 2048 bf16 (305 us of 410 with its first pass; profiles/selective_state_scan.md).
+// The forward left the state in front of every kBlock steps; a block's states and poles are
+// rebuilt from it in registers, half a block at a time, and the adjoint runs back through
+// them: one and a half exponentials per (step, channel, mode).
 //
 // Split: a thread owns kCPT channels and 4 modes of them, GM neighbouring lanes the modes
 // of a channel. Sums over modes (gB, uA) are exchanged between those lanes, sums over
@@ -80,8 +82,16 @@ struct BwdShared {
   float4 sh[LOCAL ? 1 : kCPT][LOCAL ? 1 : kThreads];
 };
 
+// CTAs per SM that the registers are cut for: three where a thread's next rows are bf16, two
+// where they are twice as long and three would spill (4 x 2047 x 2048 bf16: two 358 us,
+// three 305; 404 x 321 x 256 fp32: three 752 us, two 700).
 template <int GM, bool LOCAL, int ACC>
-__global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_scan_bwd_kernel(const ScanParams p) {
+__host__ __device__ constexpr int bwd_ctas() {
+  return LOCAL ? 4 : ACC == kBf16 && GM >= 4 ? 3 : 2;
+}
+
+template <int GM, bool LOCAL, int ACC>
+__global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_scan_bwd_kernel(const ScanParams p) {
   constexpr int CL = 32 / GM, CH = channels_per_cta<GM>(), NP = 4 * GM;
   constexpr int TS = kThreads / (CH / 4);       // rows that the CTA loads at a time
   constexpr int E = (kBlock + TS - 1) / TS;     // (step, four channels) of a thread
@@ -270,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, LOCAL ? 4 : GM >= 4 ? 3 : 2) state_s
     if (t0 - kBlock >= q.t0) fetch(t0 - kBlock, kBlock);
 
     // The later half of the block first: its entry state is a run over the earlier half,
-    // whose poles and states are rebuilt afterwards. Half of a block's values in registers
-    // leave room for three CTAs per SM.
+    // whose poles and states are rebuilt afterwards. A whole block's values would take every
+    // register of two CTAs per SM (4 x 2047 x 2048 bf16: 365 us against 346).
 #pragma unroll 1
     for (int tb = HALF; tb >= 0; tb -= HALF) {
       f2 a[HALF][kCPT][2], h[HALF + 1][kCPT][2];
