@@ -30,9 +30,10 @@ SelectiveLRU for strided layouts) falls back to the reference's copies.
 Supported mixers: ``selective_lru``, ``selective_lru_mimo``, ``linoss`` (the layers on
 this package's scan path), and ``selective_state`` (the Mamba layer's formulas with packed
 sequences, prompts and single tokens; ``ssm_params``: the mixer's own keyword arguments;
-``cu_seqlens``, ``cache``, ``slots`` and ``fresh`` pass through ``Block.forward``). The reference's other backbones (``mamba``, ``mamba2``,
-``mamba3`` from mamba_ssm, ``s4d``, ``s5``, and ``selective_linoss``, whose source the
-reference does not contain) raise NotImplementedError.
+``cu_seqlens``, ``cache``, ``slots`` and ``fresh`` pass through ``Block.forward``). The
+reference's other backbones (``mamba``, ``mamba2``, ``mamba3`` from mamba_ssm, ``s4d``,
+``s5``, and ``selective_linoss``, whose source the reference does not contain) raise
+NotImplementedError.
 """
 from __future__ import annotations
 
