@@ -36,7 +36,7 @@ struct Piece {
   bool live;         // false: no such piece. A sequence without rows has piece 0.
 };
 
-// Ckpt / piece index of the first piece of Q rows of sequence s.
+// First row of sequence s, and the index of its first piece of Q rows.
 __device__ __forceinline__ int64_t seq_start(const SeqMap& m, int64_t s) {
   return m.cu == nullptr ? s * m.L : min(max((int64_t)m.cu[s], (int64_t)0), m.T);
 }

@@ -13,10 +13,10 @@
 //
 // Split: a thread owns two channels and 4 modes of each (two pairs, each in one register pair
 // for the two-wide multiply-adds), GL neighbouring lanes a channel; a CTA of 128 threads
-// owns 256 / GL channels of one piece of a sequence and walks over it in tiles of steps. The tile's operands are loaded into registers while the tile before is
-// computed, converted and put into shared memory; the sums over modes go back through
-// shared memory, so that the step, the D skip, the gate and the stores run four neighbouring
-// channels per thread.
+// owns 256 / GL channels of one piece of a sequence and walks over it in tiles of steps. The
+// tile's operands are loaded into registers while the tile before is computed, converted and
+// put into shared memory; the sums over modes go back through shared memory, so that the
+// step, the D skip, the gate and the stores run four neighbouring channels per thread.
 //
 // Long sequences that leave the GPU idle are cut into pieces. A first pass (LOCAL) runs each
 // piece from zero and keeps its last state and the sum of its steps d; since all of a
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   for (int i = 0; i < kCPT; ++i) {
     nn[i] = cg0 + sc + i < p.cpg ? min(4, p.N - n0) : 0;
     const float4 a = load_params(p.A, at0 + i * p.N, nn[i]);
-    A2[i][0] = a.x * kLog2e; A2[i][1] = a.y * kLog2e; A2[i][2] = a.z * kLog2e; A2[i][3] = a.w * kLog2e;
+    A2[i][0] = log2_rate(a.x); A2[i][1] = log2_rate(a.y); A2[i][2] = log2_rate(a.z); A2[i][3] = log2_rate(a.w);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (!LOCAL) {
       if (split) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) state_scan_join_kernel(const ScanPar
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (!any_split(p.m)) return;
   const int64_t c = min(i, per - 1) / p.N;
-  const float A2 = p.A[min(i, per - 1)] * kLog2e;
+  const float A2 = log2_rate(p.A[min(i, per - 1)]);
   for (int64_t s = blockIdx.y; s < p.m.S; s += gridDim.y) {
     const int64_t row0 = seq_start(p.m, s);
     const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;

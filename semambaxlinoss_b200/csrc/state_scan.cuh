@@ -66,7 +66,7 @@ __device__ __forceinline__ void store(void* base, int64_t i, int bf16, float v) 
 
 // How a kernel reads and writes rows: kAny takes any type, stride, alignment and width, one
 // element at a time; kBf16 and kFp32 take four neighbours in one access (every operand of
-// that type, rows and groups that start on four elements: ScanParams::quads).
+// that type, rows and groups that start on four elements: ScanParams::access).
 enum Access { kAny = 0, kBf16 = 1, kFp32 = 2 };
 
 template <int ACC>
@@ -150,17 +150,19 @@ __device__ __forceinline__ f2 mul2(f2 a, f2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // Pole exp(d A) from d and A log2(e). The special-function exponential of small negative
 // arguments is measured 2e-8 low on average (rms 3.5e-8); a state multiplies hundreds of
 // poles, so that average is what reaches the results. kPoleBias moves the argument by as
 // much, inside the multiply-add that forms it.
 constexpr float kPoleBias = 3.0e-8f;
+// A log2(e). An A of -inf becomes the lowest finite value: the rows that fill up a tile have
+// d = 0, and 0 times -inf would put a NaN into the state (a step with d > 0 still forgets all).
+__device__ __forceinline__ float log2_rate(float A) {
+  constexpr float kLowest = -3.4028234663852886e38f;
+  const float a = A * kLog2e;
+  return a < kLowest ? kLowest : a;
+}
 __device__ __forceinline__ float pole(float d, float A2) { return semx::ex2_approx(fmaf(d, A2, kPoleBias)); }
 
 __device__ __forceinline__ float sigmoid(float v) { return semx::rcp_approx(1.f + semx::ex2_approx(-kLog2e * v)); }

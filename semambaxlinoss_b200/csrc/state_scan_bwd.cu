@@ -9,7 +9,7 @@
 //
 // Bound: instructions (24 per (step, channel, mode) of a warp, a quarter of them the exchanges
 // between lanes) and shared memory's path to the registers, at 59 % and 61 % of their rates in
-// 4 x 2047 x 2048 bf16 (305 us of 410 with its first pass; profiles/selective_state_scan.md).
+// 4 x 2047 x 2048 bf16 (307 us of 420 with its first pass and the join; profiles/selective_state_scan.md).
 // The forward left the state in front of every kBlock steps; a block's states and poles are
 // rebuilt from it in registers, half a block at a time, and the adjoint runs back through
 // them: one and a half exponentials per (step, channel, mode).
@@ -147,8 +147,8 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   for (int i = 0; i < kCPT; ++i) {
     nn[i] = cg0 + sc + i < p.cpg ? min(4, p.N - n0) : 0;
     const float4 a = load_params(p.A, at0 + i * p.N, nn[i]);
-    A2[i][0] = pack2(a.x * kLog2e, a.y * kLog2e);
-    A2[i][1] = pack2(a.z * kLog2e, a.w * kLog2e);
+    A2[i][0] = pack2(log2_rate(a.x), log2_rate(a.y));
+    A2[i][1] = pack2(log2_rate(a.z), log2_rate(a.w));
     float4 s = zero4;
     if (!LOCAL && split) s = load_params(p.entry, j * p.C * p.N + at0 + i * p.N, nn[i]);
     carry[i][0] = pack2(s.x, s.y);
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kThreads) state_scan_join_back_kernel(const Sc
   if (!any_split(p.m)) return;
   if (i >= per) return;
   const int64_t c = i / p.N;
-  const float A2 = p.A[i] * kLog2e;
+  const float A2 = log2_rate(p.A[i]);
   for (int64_t s = blockIdx.y; s < p.m.S; s += gridDim.y) {
     const int64_t row0 = seq_start(p.m, s);
     const int64_t len = p.m.cu == nullptr ? p.m.L : max(seq_start(p.m, s + 1), row0) - row0;

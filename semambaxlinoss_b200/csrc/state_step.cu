@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kThreads) state_step_kernel(const ScanParams p
   const int cc = min(c, p.C - 1), g = cc / p.cpg;
   const int nn = min(4, p.N - n0);
   const float4 a4 = load_params(p.A, (int64_t)cc * p.N + n0, nn);
-  const float A2[4] = {a4.x * kLog2e, a4.y * kLog2e, a4.z * kLog2e, a4.w * kLog2e};
+  const float A2[4] = {log2_rate(a4.x), log2_rate(a4.y), log2_rate(a4.z), log2_rate(a4.w)};
   const float bias = p.dt_bias != nullptr ? p.dt_bias[cc] : 0.f;
   const float D = p.D != nullptr ? p.D[cc] : 0.f;
   semx::find_slots<kStepRows>(p.m, s0, n, slots);

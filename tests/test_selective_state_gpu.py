@@ -439,6 +439,34 @@ def test_a_step_of_zero_keeps_the_state(L):
     assert torch.equal(state, kept)
 
 
+@pytest.mark.parametrize("L", [1, 3, 18, 300])
+def test_a_rate_of_minus_infinity_forgets(L):
+    """A = -inf (its logarithm ran away) is a pole of zero: every mode holds its last drive, no
+    NaN comes up at lengths that end inside a tile, and the gradients are those of a finite
+    rate whose poles are zero too (1e30 with steps above 1e-3)."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, selective_state_step
+
+    g = gen(11)
+    ch, N = 40, 16
+    t = {k: u.to(cuda()) for k, u in _scan_problem(2 * L, ch, N, 1, g, torch.float32).items()}
+    rows = {k: t[k].reshape(2, L, *t[k].shape[1:]) for k in ("x", "dt", "B", "C", "z")}
+    rows["dt"] = rows["dt"].abs()
+
+    def run(rate):
+        A = t["A"].clone()
+        A[3:9, 1::3] = rate
+        state = torch.zeros(2, ch, N, device=cuda())
+        with torch.no_grad():
+            y = selective_state_scan(rows["x"], rows["dt"], A, rows["B"], rows["C"], t["D"], rows["z"], state=state)
+            last = selective_state_step(*(rows[k][:, 0] for k in ("x", "dt")), A, rows["B"][:, 0], rows["C"][:, 0], state)
+        v = {k: u.detach().clone().requires_grad_() for k, u in rows.items()}
+        out = selective_state_scan(v["x"], v["dt"], A, v["B"], v["C"], t["D"], v["z"])
+        return [y, state, last, out.detach()] + list(torch.autograd.grad(out.square().sum(), list(v.values())))
+
+    for got, want in zip(run(float("-inf")), run(-1e30)):
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+
+
 def test_bad_offsets_stay_inside():
     """Offsets that decrease, start below zero or reach behind the rows give some result
     without an access outside (they are clamped in the kernels)."""
