@@ -64,8 +64,26 @@ __device__ __forceinline__ void halve_sum(float (&v)[NV], int lane) {
   }
 }
 
-template <int GM, bool LOCAL>
+// fp32 rows fetch x, v, z and the block's entry states for the next tile straight into shared
+// memory, every thread into slots of its own: in registers they leave room for two CTAs per SM
+// only (404 x 321 x 256 fp32: in registers 704 us, three CTAs that spill 752, this way 614).
+template <int GM, bool LOCAL, int ACC>
+__host__ __device__ constexpr bool stages() {
+  return !LOCAL && ACC == kFp32 && GM >= 4;
+}
+
+// 16 bytes into shared memory (zeros where there is nothing to copy), on their way until
+// copies_done(). The thread that asked for them reads them.
+__device__ __forceinline__ void copy16(void* to, const void* from, bool any) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from),
+               "r"(any ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <int GM, bool LOCAL, int ACC>
 struct BwdShared {
+  static constexpr bool STAGE = stages<GM, LOCAL, ACC>();
   static constexpr int CH = channels_per_cta<GM>(), R = LOCAL ? 1 : kBlock;
   static constexpr int TS = kThreads / (CH / 4), E = (kBlock + TS - 1) / TS;
   float4 sd[kBlock][CH / 2];  // (d, d', d x, d' x') of two channels
@@ -79,15 +97,14 @@ struct BwdShared {
   // rows, its states in front of the block.
   float4 sums[2][kThreads];
   float4 sg[LOCAL ? 1 : E][LOCAL ? 1 : kThreads];
-  float4 sh[LOCAL ? 1 : kCPT][LOCAL ? 1 : kThreads];
+  float4 sh[STAGE ? 2 : 1][LOCAL ? 1 : kCPT][LOCAL ? 1 : kThreads];
+  float4 rows[STAGE ? 2 : 1][STAGE ? 3 : 1][STAGE ? kThreads : 1];  // x, v, z of this tile and the next
 };
 
-// CTAs per SM that the registers are cut for: three where a thread's next rows are bf16, two
-// where they are twice as long and three would spill (4 x 2047 x 2048 bf16: two 358 us,
-// three 305; 404 x 321 x 256 fp32: three 752 us, two 700).
+// CTAs per SM that the registers are cut for (4 x 2047 x 2048 bf16: two 358 us, three 305).
 template <int GM, bool LOCAL, int ACC>
 __host__ __device__ constexpr int bwd_ctas() {
-  return LOCAL ? 4 : ACC == kBf16 && GM >= 4 ? 3 : 2;
+  return LOCAL ? 4 : ACC != kAny && GM >= 4 ? 3 : 2;
 }
 
 template <int GM, bool LOCAL, int ACC>
@@ -102,7 +119,9 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   constexpr int HALF = kBlock / 2;
   typedef typename RawQuad<ACC>::type Quad;
   extern __shared__ __align__(16) unsigned char raw_smem[];
-  typedef BwdShared<GM, LOCAL> Shared;
+  typedef BwdShared<GM, LOCAL, ACC> Shared;
+  constexpr bool STAGE = Shared::STAGE;
+  static_assert(!STAGE || E == 1, "one row of a tile per thread");
   Shared& sm = *reinterpret_cast<Shared*>(raw_smem);
   auto& sd = sm.sd;
   auto& sv = sm.sv;
@@ -177,7 +196,20 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   const float* ck = LOCAL || !q.live ? nullptr : p.ckpt + (piece_base(p.m, q.s, kBlock) + tl / kBlock) * p.C * p.N + at0;
   Quad rx[E], rd[E], rg[E], rz[E], rv[E], rB[EB], rC[EB];
   float4 hn[kCPT];
+  int par = 0;  // STAGE: which of the two buffers the next fetch fills
   auto fetch = [&](int t0, int rows) {  // rows of the tile that exist
+    if constexpr (STAGE) {
+      const bool in = en > 0 && et < rows;
+      const int64_t r = q.row0 + t0 + (in ? et : 0);
+      copy16(&sm.rows[par][0][tid], reinterpret_cast<const float*>(p.x) + r * p.ldx + ech, in);
+      if (has_z) {
+        copy16(&sm.rows[par][1][tid], reinterpret_cast<const float*>(p.v) + r * p.C + ech, in);
+        copy16(&sm.rows[par][2][tid], reinterpret_cast<const float*>(p.z) + r * p.ldz + ech, in);
+      }
+#pragma unroll
+      for (int i = 0; i < kCPT; ++i) copy16(&sh[par][i][tid], nn[i] > 0 ? ck + i * p.N : p.ckpt, nn[i] > 0);
+      par ^= 1;
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       rx[i] = rd[i] = rg[i] = rz[i] = rv[i] = Quad{};
@@ -185,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
         const int64_t r = q.row0 + t0 + et + i * TS;
         rd[i] = load_quad<ACC>(p.dt, r * p.lddt + ech, p.dt_bf16, en);
         rg[i] = load_quad<ACC>(p.dy, r * p.C + ech, p.bf16, en);
-        if (has_z) rz[i] = load_quad<ACC>(p.z, r * p.ldz + ech, p.bf16, en);
-        if (!LOCAL) {
+        if (has_z && !STAGE) rz[i] = load_quad<ACC>(p.z, r * p.ldz + ech, p.bf16, en);
+        if (!LOCAL && !STAGE) {
           rx[i] = load_quad<ACC>(p.x, r * p.ldx + ech, p.bf16, en);
           if (has_z) rv[i] = load_quad<ACC>(p.v, r * p.C + ech, p.bf16, en);
         }
@@ -201,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
         rC[i] = load_quad<ACC>(p.Cm, r * p.ldc + b, p.bf16, bn);
       }
     }
-    if (!LOCAL) {
+    if (!LOCAL && !STAGE) {
 #pragma unroll
       for (int i = 0; i < kCPT; ++i) {
         hn[i] = zero4;
@@ -211,8 +243,8 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
           hn[i] = load_params(ck, i * p.N, nn[i]);
         }
       }
-      ck -= (int64_t)p.C * p.N;
     }
+    if (!LOCAL) ck -= (int64_t)p.C * p.N;
   };
 
   if (tl >= q.t0) fetch(tl, min(kBlock, q.t1 - tl));
@@ -220,6 +252,8 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   for (int t0 = tl; t0 >= q.t0; t0 -= kBlock) {
     const int nt = min(kBlock, q.t1 - t0);
     Quad kx[E];  // x
+    const int now = STAGE ? par ^ 1 : 0;  // the buffer of this tile
+    if constexpr (STAGE) copies_done();
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int t = et + i * TS;
@@ -238,10 +272,14 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
                                 softplus_slope(raw.w, e.w));
         }
         if (has_z) {
-          const float4 z = quad_floats<ACC>(rz[i], p.bf16);
+          float4 z;
+          if constexpr (STAGE) z = sm.rows[now][2][tid];
+          else z = quad_floats<ACC>(rz[i], p.bf16);
           const float4 s = make_float4(sigmoid(z.x), sigmoid(z.y), sigmoid(z.z), sigmoid(z.w));
           if (!LOCAL && in) {
-            const float4 v = quad_floats<ACC>(rv[i], p.bf16);
+            float4 v;
+            if constexpr (STAGE) v = sm.rows[now][1][tid];
+            else v = quad_floats<ACC>(rv[i], p.bf16);
             store_quad<ACC>(p.dz, (q.row0 + t0 + t) * p.C + ech, p.bf16, en,
                             make_float4(g.x * v.x * (s.x * fmaf(z.x, 1.f - s.x, 1.f)),
                                         g.y * v.y * (s.y * fmaf(z.y, 1.f - s.y, 1.f)),
@@ -251,12 +289,14 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
           g.x *= z.x * s.x; g.y *= z.y * s.y; g.z *= z.z * s.z; g.w *= z.w * s.w;
         }
         if (!in) d = g = zero4;  // a row behind the piece: pole 1, no drive, no gradient
-        const float4 x = LOCAL ? zero4 : quad_floats<ACC>(rx[i], p.bf16);
+        float4 x;
+        if constexpr (STAGE) x = sm.rows[now][0][tid];
+        else x = LOCAL ? zero4 : quad_floats<ACC>(rx[i], p.bf16);
         sd[t][2 * eq] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
         sd[t][2 * eq + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
         *reinterpret_cast<float4*>(&sv[t][2 * eq]) = g;
         if (!LOCAL) {
-          kx[i] = rx[i];
+          if (!STAGE) kx[i] = rx[i];
           sg[i][tid] = slope;
         } else {
           float4 s = sums[1][tid];
@@ -272,9 +312,9 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
         sC[tb0 + i * ML][bl] = quad_floats<ACC>(rC[i], p.bf16);
       }
     }
-    if (!LOCAL) {
+    if (!LOCAL && !STAGE) {
 #pragma unroll
-      for (int i = 0; i < kCPT; ++i) sh[i][tid] = hn[i];
+      for (int i = 0; i < kCPT; ++i) sh[0][i][tid] = hn[i];
     }
     __syncthreads();
     if (t0 - kBlock >= q.t0) fetch(t0 - kBlock, kBlock);
@@ -288,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
       if (!LOCAL) {
 #pragma unroll
         for (int i = 0; i < kCPT; ++i) {
-          const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&sh[i][tid]);
+          const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&sh[now][i][tid]);
           h[0][i][0] = e.x;
           h[0][i][1] = e.y;
         }
@@ -396,7 +436,10 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
           const float4 s0 = *reinterpret_cast<const float4*>(&so[t][2 * ec]);
           const float4 s1 = *reinterpret_cast<const float4*>(&so[t][2 * ec + 4]);
           // d and dv as this thread put them there.
-          const float4 x = quad_floats<ACC>(kx[i], p.bf16), k = sg[i][tid], D = spar[1][eq];
+          float4 x;
+          if constexpr (STAGE) x = sm.rows[now][0][tid];
+          else x = quad_floats<ACC>(kx[i], p.bf16);
+          const float4 k = sg[i][tid], D = spar[1][eq];
           const float4 g = *reinterpret_cast<const float4*>(&sv[t][2 * eq]);
           const float2 d01 = *reinterpret_cast<const float2*>(&sd[t][2 * eq]);
           const float2 d23 = *reinterpret_cast<const float2*>(&sd[t][2 * eq + 1]);
@@ -566,7 +609,7 @@ Layout layout(const ScanParams& p, int64_t Q) {
 
 template <int GM, bool LOCAL, int ACC>
 int launch_one(const ScanParams& p, unsigned grid, cudaStream_t st) {
-  constexpr size_t bytes = sizeof(BwdShared<GM, LOCAL>);
+  constexpr size_t bytes = sizeof(BwdShared<GM, LOCAL, ACC>);
   if (!semx::allow_smem(state_scan_bwd_kernel<GM, LOCAL, ACC>, bytes)) return SEMX_ERR_LAUNCH;
   state_scan_bwd_kernel<GM, LOCAL, ACC><<<grid, kThreads, bytes, st>>>(p);
   return semx::check_launch("state_scan_bwd_kernel");
@@ -626,6 +669,7 @@ int semx_state_scan_bwd(const SemxStateScanArgs* a, semx_stream_t stream) {
   const Layout l = layout(p, Q);
   float* ws = reinterpret_cast<float*>(a->workspace);
   p.pBC = ws + l.pbc;
+  if (!semx::aligned(a->ckpt, 16)) p.access = kAny;  // the states are read four at a time, too
   const bool params = a->dA != nullptr || a->dD != nullptr || a->ddt_bias != nullptr;
   p.part = params ? ws + l.part : nullptr;
   if (p.m.T > 0) {
