@@ -8,15 +8,15 @@
 // evaluated once where the batch fills the GPU, and everything else is kept off the units
 // that evaluate them: A is scaled by log2(e) once, d and d x are evaluated once per (step,
 // channel) and shared through shared memory. Measured: 404 x 321 x 256 fp32 training forward
-// 243 us (exponentials alone 114, its bytes 142); in 4 x 2047 x 2048 bf16 the unit is busy 58 %
+// 232 us (exponentials alone 114, its bytes 142); in 4 x 2047 x 2048 bf16 the unit is busy 58 %
 // of the main pass and 77 % of the first one (profiles/selective_state_scan.md).
 //
 // Split: a thread owns two channels and 4 modes of each (two pairs, each in one register pair
 // for the two-wide multiply-adds), GL neighbouring lanes a channel; a CTA of 128 threads
 // owns 256 / GL channels of one piece of a sequence and walks over it in tiles of steps. The
-// tile's operands are loaded into registers while the tile before is computed, converted and
-// put into shared memory; the sums over modes go back through shared memory, so that the
-// step, the D skip, the gate and the stores run four neighbouring channels per thread.
+// tile's operands are loaded while the tile before is computed, converted and put into shared
+// memory; the sums over modes go back through shared memory, so that the step, the D skip,
+// the gate and the stores run four neighbouring channels per thread.
 //
 // Long sequences that leave the GPU idle are cut into pieces. A first pass (LOCAL) runs each
 // piece from zero and keeps its last state and the sum of its steps d; since all of a
@@ -45,6 +45,16 @@ constexpr int tile_steps() {
   return GL >= 4 ? 16 : 8;
 }
 
+// Rows that are read four elements at a time go straight into shared memory, every thread's
+// into slots of its own, where x and z stay until the tile's results need them again (404 x
+// 321 x 256 fp32: through registers 243 us, this way 232; with the registers cut for five CTAs
+// per SM instead of four 250). The first pass needs them once and is faster without (4 x 2047
+// x 2048 bf16: 89 us and 91).
+template <int GL, bool LOCAL, int ACC>
+__host__ __device__ constexpr bool stages() {
+  return !LOCAL && ACC != kAny && GL >= 4;
+}
+
 template <int GL, bool LOCAL, int ACC>
 __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kernel(const ScanParams p) {
   constexpr int CH = channels_per_cta<GL>(), TT = tile_steps<GL>();
@@ -59,6 +69,8 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   __shared__ __align__(16) float sys[LOCAL ? 1 : TT][LOCAL ? 4 : YS];
   __shared__ __align__(16) float4 sB[TT][GL];
   __shared__ __align__(16) float4 sC[LOCAL ? 1 : TT][LOCAL ? 1 : GL];
+  constexpr bool STAGE = stages<GL, LOCAL, ACC>();
+  __shared__ __align__(16) Quad rows[STAGE ? 2 : 1][STAGE ? 3 : 1][STAGE ? E : 1][STAGE ? kThreads : 1];  // x, dt, z
 
   const int64_t j = blockIdx.x / p.ctiles;
   const int ct = blockIdx.x % p.ctiles;
@@ -124,9 +136,17 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   int64_t oB = (q.row0 + q.t0 + tb0) * p.ldb + (int64_t)grp * p.N + n0;
   int64_t oC = (q.row0 + q.t0 + tb0) * p.ldc + (int64_t)grp * p.N + n0;
   const int bn = min(4, p.N - n0);
+  int par = 0;  // STAGE: which of the two buffers the next fetch fills
   auto fetch = [&](int left) {  // rows of the piece from this tile on
 #pragma unroll
     for (int i = 0; i < E; ++i) {
+      if constexpr (STAGE) {
+        const bool in = en > 0 && et + i * TS < min(TT, left);
+        copy_quad<ACC>(&rows[par][0][i][tid], p.x, ox + i * TS * p.ldx, in);
+        copy_quad<ACC>(&rows[par][1][i][tid], p.dt, od + i * TS * p.lddt, in);
+        if (has_z) copy_quad<ACC>(&rows[par][2][i][tid], p.z, oz + i * TS * p.ldz, in);
+        continue;
+      }
       rx[i] = rd[i] = rz[i] = Quad{};
       if (en > 0 && et + i * TS < min(TT, left)) {
         rx[i] = load_quad<ACC>(p.x, ox + i * TS * p.ldx, p.bf16, en);
@@ -134,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
         if (has_z) rz[i] = load_quad<ACC>(p.z, oz + i * TS * p.ldz, p.bf16, en);
       }
     }
+    par ^= 1;
     ox += TT * p.ldx;
     od += TT * p.lddt;
     oz += TT * p.ldz;
@@ -152,10 +173,16 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   for (int t0 = q.t0; t0 < q.t1; t0 += TT) {
     const int left = q.t1 - t0, nt = min(TT, left);
     float4 xv[E], zv[E];
+    const int now = STAGE ? par ^ 1 : 0;  // the buffer of this tile
+    if constexpr (STAGE) copies_done();
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int t = et + i * TS;
       if (t < TT) {
+        if constexpr (STAGE) {
+          rx[i] = rows[now][0][i][tid];
+          rd[i] = rows[now][1][i][tid];
+        }
         const float4 x = quad_floats<ACC>(rx[i], p.bf16);
         float4 d = quad_floats<ACC>(rd[i], p.dt_bf16);
         d.x += bias.x; d.y += bias.y; d.z += bias.z; d.w += bias.w;
@@ -163,8 +190,10 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
         if (t >= nt) d = make_float4(0.f, 0.f, 0.f, 0.f);  // a row behind the piece: pole 1, no drive
         sdt[t][ec / 2] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
         sdt[t][ec / 2 + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
-        xv[i] = x;
-        if (has_z) zv[i] = quad_floats<ACC>(rz[i], p.bf16);
+        if constexpr (!STAGE) {
+          xv[i] = x;
+          if (has_z) zv[i] = quad_floats<ACC>(rz[i], p.bf16);
+        }
         if (LOCAL) {
           dsum.x += d.x; dsum.y += d.y; dsum.z += d.z; dsum.w += d.w;
         }
@@ -237,6 +266,10 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
         if (t < nt && en > 0) {
           const int64_t o = oy + i * TS * (int64_t)p.C;
           const float4 s = *reinterpret_cast<const float4*>(&sys[t][ec]);
+          if constexpr (STAGE) {
+            xv[i] = quad_floats<ACC>(rows[now][0][i][tid], p.bf16);
+            if (has_z) zv[i] = quad_floats<ACC>(rows[now][2][i][tid], p.bf16);
+          }
           float4 v = make_float4(fmaf(D.x, xv[i].x, s.x), fmaf(D.y, xv[i].y, s.y), fmaf(D.z, xv[i].z, s.z),
                                  fmaf(D.w, xv[i].w, s.w));
           if (p.v != nullptr) store_quad<ACC>(p.v, o, p.bf16, en, v);

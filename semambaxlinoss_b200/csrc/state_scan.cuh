@@ -122,6 +122,19 @@ __device__ __forceinline__ void store_quad(void* base, int64_t i, int bf16, int 
     if (n > 3) store(base, i + 3, bf16, v.w);
   }
 }
+// Four elements from base[i] on (kBf16, kFp32) into shared memory, zeros where there are none to
+// copy; on their way until copies_done(). Only the thread that asked for them reads them.
+template <int ACC>
+__device__ __forceinline__ void copy_quad(typename RawQuad<ACC>::type* to, const void* base, int64_t i, bool any) {
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  const char* from = reinterpret_cast<const char*>(base) + (any ? i * (ACC == kBf16 ? 2 : 4) : 0);
+  if constexpr (ACC == kBf16)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(any ? 8 : 0) : "memory");
+  else
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(any ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // The first n of four parameters (0 for the rest and without a parameter).
 __device__ __forceinline__ float4 load_params(const float* base, int64_t i, int n) {
   if (base == nullptr) return make_float4(0.f, 0.f, 0.f, 0.f);

@@ -72,15 +72,6 @@ __host__ __device__ constexpr bool stages() {
   return !LOCAL && ACC == kFp32 && GM >= 4;
 }
 
-// 16 bytes into shared memory (zeros where there is nothing to copy), on their way until
-// copies_done(). The thread that asked for them reads them.
-__device__ __forceinline__ void copy16(void* to, const void* from, bool any) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from),
-               "r"(any ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 template <int GM, bool LOCAL, int ACC>
 struct BwdShared {
   static constexpr bool STAGE = stages<GM, LOCAL, ACC>();
@@ -98,7 +89,7 @@ struct BwdShared {
   float4 sums[2][kThreads];
   float4 sg[LOCAL ? 1 : E][LOCAL ? 1 : kThreads];
   float4 sh[STAGE ? 2 : 1][LOCAL ? 1 : kCPT][LOCAL ? 1 : kThreads];
-  float4 rows[STAGE ? 2 : 1][STAGE ? 3 : 1][STAGE ? kThreads : 1];  // x, v, z of this tile and the next
+  uint4 rows[STAGE ? 2 : 1][STAGE ? 3 : 1][STAGE ? kThreads : 1];  // x, v, z of this tile and the next
 };
 
 // CTAs per SM that the registers are cut for (4 x 2047 x 2048 bf16: two 358 us, three 305).
@@ -200,14 +191,15 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   auto fetch = [&](int t0, int rows) {  // rows of the tile that exist
     if constexpr (STAGE) {
       const bool in = en > 0 && et < rows;
-      const int64_t r = q.row0 + t0 + (in ? et : 0);
-      copy16(&sm.rows[par][0][tid], reinterpret_cast<const float*>(p.x) + r * p.ldx + ech, in);
+      const int64_t r = q.row0 + t0 + et;
+      copy_quad<kFp32>(&sm.rows[par][0][tid], p.x, r * p.ldx + ech, in);
       if (has_z) {
-        copy16(&sm.rows[par][1][tid], reinterpret_cast<const float*>(p.v) + r * p.C + ech, in);
-        copy16(&sm.rows[par][2][tid], reinterpret_cast<const float*>(p.z) + r * p.ldz + ech, in);
+        copy_quad<kFp32>(&sm.rows[par][1][tid], p.v, r * p.C + ech, in);
+        copy_quad<kFp32>(&sm.rows[par][2][tid], p.z, r * p.ldz + ech, in);
       }
 #pragma unroll
-      for (int i = 0; i < kCPT; ++i) copy16(&sh[par][i][tid], nn[i] > 0 ? ck + i * p.N : p.ckpt, nn[i] > 0);
+      for (int i = 0; i < kCPT; ++i)
+        copy_quad<kFp32>(reinterpret_cast<uint4*>(&sh[par][i][tid]), nn[i] > 0 ? ck : p.ckpt, i * p.N, nn[i] > 0);
       par ^= 1;
     }
 #pragma unroll
@@ -273,12 +265,12 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
         }
         if (has_z) {
           float4 z;
-          if constexpr (STAGE) z = sm.rows[now][2][tid];
+          if constexpr (STAGE) z = quad_floats<kFp32>(sm.rows[now][2][tid], 0);
           else z = quad_floats<ACC>(rz[i], p.bf16);
           const float4 s = make_float4(sigmoid(z.x), sigmoid(z.y), sigmoid(z.z), sigmoid(z.w));
           if (!LOCAL && in) {
             float4 v;
-            if constexpr (STAGE) v = sm.rows[now][1][tid];
+            if constexpr (STAGE) v = quad_floats<kFp32>(sm.rows[now][1][tid], 0);
             else v = quad_floats<ACC>(rv[i], p.bf16);
             store_quad<ACC>(p.dz, (q.row0 + t0 + t) * p.C + ech, p.bf16, en,
                             make_float4(g.x * v.x * (s.x * fmaf(z.x, 1.f - s.x, 1.f)),
@@ -290,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
         }
         if (!in) d = g = zero4;  // a row behind the piece: pole 1, no drive, no gradient
         float4 x;
-        if constexpr (STAGE) x = sm.rows[now][0][tid];
+        if constexpr (STAGE) x = quad_floats<kFp32>(sm.rows[now][0][tid], 0);
         else x = LOCAL ? zero4 : quad_floats<ACC>(rx[i], p.bf16);
         sd[t][2 * eq] = make_float4(d.x, d.y, d.x * x.x, d.y * x.y);
         sd[t][2 * eq + 1] = make_float4(d.z, d.w, d.z * x.z, d.w * x.w);
@@ -437,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
           const float4 s1 = *reinterpret_cast<const float4*>(&so[t][2 * ec + 4]);
           // d and dv as this thread put them there.
           float4 x;
-          if constexpr (STAGE) x = sm.rows[now][0][tid];
+          if constexpr (STAGE) x = quad_floats<kFp32>(sm.rows[now][0][tid], 0);
           else x = quad_floats<ACC>(kx[i], p.bf16);
           const float4 k = sg[i][tid], D = spar[1][eq];
           const float4 g = *reinterpret_cast<const float4*>(&sv[t][2 * eq]);
