@@ -743,6 +743,40 @@ def test_prompts_and_tokens_equal_the_whole_sequence(dtype):
         assert pos == [n + new for n in lens]
 
 
+@pytest.mark.parametrize("width,modes,taps,groups", [(24, 8, 1, 2), (15, 5, 8, 3), (33, 16, 2, 1)])
+def test_mixer_widths_and_captured_tokens(width, modes, taps, groups):
+    """One tap (no window to keep), many taps, groups, widths that leave rows unaligned: a prompt,
+    then tokens from a replayed graph, against the whole sequence (fp32: the repository's 1e-4)."""
+    from semambaxlinoss_b200.selective_state import SelectiveStateMixer
+
+    torch.manual_seed(3)
+    mixer = SelectiveStateMixer(width, modes, taps, 2, n_groups=groups).to(cuda())
+    x = torch.randn(2, 12, width, device=cuda())
+    slots = torch.tensor([2, 0], dtype=torch.int32, device=cuda())
+    with torch.no_grad():
+        whole = mixer(x)
+        tol = 1e-4 * whole.abs().max()
+        cache = mixer.allocate_cache(3)
+        y = mixer(x[:, :7], cache=cache, slots=slots, fresh=torch.ones(2, dtype=torch.bool, device=cuda()))
+        assert (y - whole[:, :7]).abs().max() <= tol
+        token = x[:, 7].clone()
+        kept = [t.clone() for t in (cache.window, cache.state)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            mixer.step(token, cache, slots)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mixer.step(token, cache, slots)
+        for t, k in zip((cache.window, cache.state), kept):
+            t.copy_(k)
+        for i in range(7, 12):
+            token.copy_(x[:, i])
+            graph.replay()
+            assert (out - whole[:, i]).abs().max() <= tol
+
+
 def test_bidirectional_block_and_autocast():
     """The factory's mixer inside MambaBlock: both directions, and bf16 autocast end to end."""
     from semambaxlinoss_b200.mamba_block import MambaBlock
