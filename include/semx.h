@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define SEMX_ABI_VERSION 2
+#define SEMX_ABI_VERSION 3
 
 typedef void* semx_stream_t; /* cudaStream_t */
 
@@ -678,7 +678,7 @@ int semx_short_conv_bwd(const SemxShortConvArgs* args, semx_stream_t stream);
  * dt_bf16; A, D, dt_bias (the last two may be NULL: 0) and their gradients fp32;
  * state (n_slots, C, N) fp32. B and C rows hold (G, N) contiguously.
  * semx_state_scan_*: whole sequences. A training forward passes ckpt
- * (semx_state_scan_ckpt_bytes()) and, with z, v (rows, C) in x's type; the backward reads
+ * (semx_state_scan_ckpt_bytes()) and, with z, v (rows, C) in fp32; the backward reads
  * them and writes dx, ddt, dz (with z), dB, dC (rows, G, N), and dA, dD, ddt_bias (each may
  * be NULL), all reduced in a fixed order. Workspace: semx_state_scan_workspace_bytes() with
  * `backward` 0 or 1 (0 bytes where none is needed).
@@ -703,7 +703,7 @@ typedef struct SemxStateScanArgs {
   float* state;
   const int32_t* slots;
   const uint8_t* fresh;
-  void* v;
+  float* v;
   float* ckpt;
   const void* dy;
   void* dx;

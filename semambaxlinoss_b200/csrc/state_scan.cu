@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   if (!LOCAL && en > 0 && et == 0)
     for (int64_t r = rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) {
       store_quad<ACC>(p.y, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
-      if (p.v != nullptr) store_quad<ACC>(p.v, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (p.v != nullptr) store_quad<fp32_beside(ACC)>(p.v, r * p.C + ech, 0, en, make_float4(0.f, 0.f, 0.f, 0.f));
     }
   // A sequence of one piece needs neither a first pass nor joining: its piece starts from the
   // pool's entry and leaves its state there.
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
           }
           float4 v = make_float4(fmaf(D.x, xv[i].x, s.x), fmaf(D.y, xv[i].y, s.y), fmaf(D.z, xv[i].z, s.z),
                                  fmaf(D.w, xv[i].w, s.w));
-          if (p.v != nullptr) store_quad<ACC>(p.v, o, p.bf16, en, v);
+          if (p.v != nullptr) store_quad<fp32_beside(ACC)>(p.v, o, 0, en, v);
           if (has_z) v = gate4(v, zv[i]);
           store_quad<ACC>(p.y, o, p.bf16, en, v);
         }
@@ -397,9 +397,9 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
                  "state_scan bwd: dy / dx / ddt / dB / dC / ckpt is NULL");
     SEMX_REQUIRE(none || a->z == nullptr || (a->dz && a->v), SEMX_ERR_NULL, "state_scan bwd: dz / v is NULL");
   }
-  SEMX_REQUIRE(semx::all_aligned({a->x, a->B, a->Cm, a->z, a->y, a->v, a->dy, a->dx, a->dz, a->dB, a->dC}, a->bf16 ? 2 : 4) &&
+  SEMX_REQUIRE(semx::all_aligned({a->x, a->B, a->Cm, a->z, a->y, a->dy, a->dx, a->dz, a->dB, a->dC}, a->bf16 ? 2 : 4) &&
                    semx::all_aligned({a->dt, a->ddt}, a->dt_bf16 ? 2 : 4) &&
-                   semx::all_aligned({a->A, a->D, a->dt_bias, a->cu_seqlens, a->state, a->slots, a->ckpt, a->dA, a->dD,
+                   semx::all_aligned({a->A, a->D, a->dt_bias, a->cu_seqlens, a->state, a->slots, a->v, a->ckpt, a->dA, a->dD,
                                       a->ddt_bias, a->workspace}, 4),
                SEMX_ERR_ALIGN, "state_scan: a pointer is not on an element");
   p->C = (int)a->C; p->N = (int)a->N; p->G = (int)a->G; p->cpg = (int)(a->C / a->G);
@@ -412,9 +412,9 @@ int scan_validate(const SemxStateScanArgs* a, bool bwd, ScanParams* p) {
   p->access = kAny;
   if ((a->bf16 != 0) == (a->dt_bf16 != 0) && p->cpg % 4 == 0 && p->N % 4 == 0 && a->ldx % 4 == 0 && a->lddt % 4 == 0 &&
       (a->z == nullptr || a->ldz % 4 == 0) && a->ldb % 4 == 0 && a->ldc % 4 == 0) {
-    bool ok = true;
-    for (const void* t : {a->x, a->dt, a->B, a->Cm, a->z, (const void*)a->y, (const void*)a->v, a->dy,
-                          (const void*)a->dx, (const void*)a->ddt, (const void*)a->dz})
+    bool ok = semx::aligned(a->v, 16);
+    for (const void* t : {a->x, a->dt, a->B, a->Cm, a->z, (const void*)a->y, a->dy, (const void*)a->dx,
+                          (const void*)a->ddt, (const void*)a->dz})
       ok = ok && semx::aligned(t, a->bf16 ? 8 : 16);
     if (ok) p->access = a->bf16 ? kBf16 : kFp32;
   }
@@ -491,8 +491,8 @@ size_t semx_state_scan_workspace_bytes(const SemxStateScanArgs* a, int32_t backw
   b.A = any;
   b.y = any;
   b.dy = any;
-  b.dx = b.ddt = b.dz = b.dB = b.dC = b.v = any;
-  b.ckpt = any;
+  b.dx = b.ddt = b.dz = b.dB = b.dC = any;
+  b.v = b.ckpt = any;
   ScanParams p = {};
   if (scan_validate(&b, backward != 0, &p) != SEMX_OK) return 0;
   if (backward != 0) return scan_bwd_workspace(p);

@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   const int tl = q.t1 > q.t0 ? q.t0 + (q.t1 - 1 - q.t0) / kBlock * kBlock : q.t0 - kBlock;
   const int tb0 = tid / GM, bl = tid % GM, bn = min(4, p.N - bl * 4);
   const float* ck = LOCAL || !q.live ? nullptr : p.ckpt + (piece_base(p.m, q.s, kBlock) + tl / kBlock) * p.C * p.N + at0;
-  Quad rx[E], rd[E], rg[E], rz[E], rv[E], rB[EB], rC[EB];
+  Quad rx[E], rd[E], rg[E], rz[E], rB[EB], rC[EB];
+  uint4 rv[E];  // fp32 whatever the rows' type
   float4 hn[kCPT];
   int par = 0;  // STAGE: which of the two buffers the next fetch fills
   auto fetch = [&](int t0, int rows) {  // rows of the tile that exist
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      rx[i] = rd[i] = rg[i] = rz[i] = rv[i] = Quad{};
+      rx[i] = rd[i] = rg[i] = rz[i] = Quad{};
+      rv[i] = uint4{};
       if (en > 0 && et + i * TS < rows) {
         const int64_t r = q.row0 + t0 + et + i * TS;
         rd[i] = load_quad<ACC>(p.dt, r * p.lddt + ech, p.dt_bf16, en);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
         if (has_z && !STAGE) rz[i] = load_quad<ACC>(p.z, r * p.ldz + ech, p.bf16, en);
         if (!LOCAL && !STAGE) {
           rx[i] = load_quad<ACC>(p.x, r * p.ldx + ech, p.bf16, en);
-          if (has_z) rv[i] = load_quad<ACC>(p.v, r * p.C + ech, p.bf16, en);
+          if (has_z) rv[i] = load_quad<fp32_beside(ACC)>(p.v, r * p.C + ech, 0, en);
         }
       }
     }
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
           if (!LOCAL && in) {
             float4 v;
             if constexpr (STAGE) v = quad_floats<kFp32>(sm.rows[now][1][tid], 0);
-            else v = quad_floats<ACC>(rv[i], p.bf16);
+            else v = quad_floats<fp32_beside(ACC)>(rv[i], 0);
             store_quad<ACC>(p.dz, (q.row0 + t0 + t) * p.C + ech, p.bf16, en,
                             make_float4(g.x * v.x * (s.x * fmaf(z.x, 1.f - s.x, 1.f)),
                                         g.y * v.y * (s.y * fmaf(z.y, 1.f - s.y, 1.f)),

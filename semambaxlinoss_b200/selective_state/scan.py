@@ -93,7 +93,7 @@ class _StateScan(torch.autograd.Function):
         a, kept = _args(x, dt, A32, B, C, D32, z, b32, softplus, S, rows, L, cu, N, G)
         dev = x.device
         y = x.new_empty(x.shape)
-        v = None if z is None else x.new_empty(x.shape)
+        v = None if z is None else x.new_empty(x.shape, dtype=torch.float32)
         ckpt = _lib.scratch(_lib.load().semx_state_scan_ckpt_bytes(a), x)
         a.y, a.v, a.ckpt = y.data_ptr(), _lib.ptr(v), ckpt.data_ptr()
         nbytes = _lib.load().semx_state_scan_workspace_bytes(a, 0)
@@ -145,8 +145,8 @@ def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     beside bf16. Rows may lie at any stride.
 
     Training: gradients flow to every operand, every sequence starts from zeros; the forward
-    keeps the state of every 8th step in fp32 and, with z, the value in front of the gate in
-    x's type. Prompts: ``state`` (entries, C, N) fp32 is read and updated in place; refused
+    keeps the state of every 8th step and, with z, the value in front of the gate, both in
+    fp32. Prompts: ``state`` (entries, C, N) fp32 is read and updated in place; refused
     while a gradient is wanted."""
     op = "selective_state_scan"
     S, rows, L = batch(op, x, cu_seqlens)
