@@ -1,7 +1,8 @@
 // Sequences of a batch and their pieces, for the operators that keep a state per sequence.
 //
 // A batch is S sequences of L rows each (row s L + t), or packed rows with offsets cu
-// (S + 1): sequence s owns rows [cu[s], cu[s+1]) and rows from cu[S] on belong to none.
+// (S + 1): sequence s owns rows [cu[s], cu[s+1]); rows in front of cu[0] and from cu[S] on
+// belong to none.
 // Every sequence is cut into pieces of Q rows; piece j of the batch is piece k = j - base(s)
 // of sequence s with base(s) = s ceil(L / Q), or cu[s] / Q + s for packed rows (rounded
 // down): consecutive bases are at least ceil(len / Q) apart, so the pieces of two sequences
@@ -84,9 +85,20 @@ __device__ __forceinline__ Piece find_piece(const SeqMap& m, int64_t j) {
   return q;
 }
 
-// First row behind the last sequence.
+// First row of the first sequence, and first row behind the last one.
+__device__ __forceinline__ int64_t rows_begin(const SeqMap& m) {
+  return m.S > 0 && m.cu != nullptr ? seq_start(m, 0) : 0;
+}
 __device__ __forceinline__ int64_t rows_end(const SeqMap& m) {
   return m.S > 0 ? (m.cu == nullptr ? m.S * m.L : seq_start(m, m.S)) : 0;
+}
+
+// Calls f(row) for every pieces-th of the rows that belong to no sequence, from number j on: those
+// in front of the first sequence, then those behind the last.
+template <class F>
+__device__ __forceinline__ void for_unused_rows(const SeqMap& m, int64_t j, F f) {
+  const int64_t front = rows_begin(m), count = front + m.T - rows_end(m);
+  for (int64_t i = j; i < count; i += m.pieces) f(i < front ? i : m.T - count + i);
 }
 
 // Entry of sequence s in the pool: >= 0, or kNone (no entry), or kRefused. Called by all

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kT) short_conv_fwd_kernel(const CvParams p) {
   float zero[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) zero[i] = 0.f;
-  for (int64_t r = semx::rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) st_vec<BF16, V>(p.y, r * p.C + c, zero);
+  semx::for_unused_rows(p.m, j, [&](int64_t r) { st_vec<BF16, V>(p.y, r * p.C + c, zero); });
   if (!q.live) return;
   const bool cold = slot < 0 || (p.m.fresh != nullptr && p.m.fresh[q.s] != 0);
   float w[K][V], b[V];
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kT) short_conv_bwd_kernel(const CvParams p) {
   float zero[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) zero[i] = 0.f;
-  for (int64_t r = semx::rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) st_vec<BF16, V>(p.dx, r * p.C + c, zero);
+  semx::for_unused_rows(p.m, j, [&](int64_t r) { st_vec<BF16, V>(p.dx, r * p.C + c, zero); });
   float w[K][V], b[V], dw[K][V], db[V];
   own_weights(sw, w);
 #pragma unroll

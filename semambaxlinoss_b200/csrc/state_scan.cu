@@ -88,10 +88,10 @@ __global__ void __launch_bounds__(kThreads, GL >= 4 ? 4 : 2) state_scan_fwd_kern
   const int64_t ech = c_base + (en > 0 ? cg0 + ec : 0);
   const bool has_z = !LOCAL && p.z != nullptr;
   if (!LOCAL && en > 0 && et == 0)
-    for (int64_t r = rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) {
+    for_unused_rows(p.m, j, [&](int64_t r) {
       store_quad<ACC>(p.y, r * p.C + ech, p.bf16, en, make_float4(0.f, 0.f, 0.f, 0.f));
       if (p.v != nullptr) store_quad<fp32_beside(ACC)>(p.v, r * p.C + ech, 0, en, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
+    });
   // A sequence of one piece needs neither a first pass nor joining: its piece starts from the
   // pool's entry and leaves its state there.
   const bool split = p.entry != nullptr && q.len > p.m.Q;
@@ -469,7 +469,7 @@ int semx_state_scan_fwd(const SemxStateScanArgs* a, semx_stream_t stream) {
   cudaStream_t st = semx::as_stream(stream);
   const int64_t Q = fwd_rows_per_piece(p);
   semx::set_pieces(&p.m, Q);
-  if (p.m.S == 0 && p.m.T > 0) p.m.pieces = 1;  // nothing but rows behind the last sequence
+  if (p.m.S == 0 && p.m.T > 0) p.m.pieces = 1;  // nothing but unused rows
   if (Q > 0 && p.m.S > 0) {
     SEMX_REQUIRE(a->workspace != nullptr, SEMX_ERR_WORKSPACE, "state_scan: workspace is NULL");
     p.entry = reinterpret_cast<float*>(a->workspace);

@@ -12,8 +12,10 @@ namespace semx_scan {
 
 using semx::find_piece;
 using semx::find_slot;
+using semx::for_unused_rows;
 using semx::Piece;
 using semx::piece_base;
+using semx::rows_begin;
 using semx::rows_end;
 using semx::seq_start;
 

@@ -142,11 +142,11 @@ __global__ void __launch_bounds__(kThreads, (bwd_ctas<GM, LOCAL, ACC>())) state_
   const bool has_z = p.z != nullptr;
   const float4 zero4 = make_float4(0.f, 0.f, 0.f, 0.f);
   if (!LOCAL && en > 0 && et == 0)
-    for (int64_t r = rows_end(p.m) + j; r < p.m.T; r += p.m.pieces) {
+    for_unused_rows(p.m, j, [&](int64_t r) {
       store_quad<ACC>(p.dx, r * p.C + ech, p.bf16, en, zero4);
       store_quad<ACC>(p.ddt, r * p.C + ech, p.dt_bf16, en, zero4);
       if (has_z) store_quad<ACC>(p.dz, r * p.C + ech, p.bf16, en, zero4);
-    }
+    });
 
   // The channels and modes of this thread in the scan.
   const int lm = lane % GM, cl = lane / GM, n0 = lm * 4;
@@ -537,14 +537,14 @@ __global__ void __launch_bounds__(256) state_scan_bc_kernel(const ScanParams p, 
   const int nq = (p.N + 3) / 4, per = 2 * p.G * nq;  // fours of a row: (kind, group, modes)
   const int64_t r0 = (int64_t)blockIdx.x * kBcRows;
   const int rows = (int)min((int64_t)kBcRows, p.m.T - r0);
-  const int64_t end = rows_end(p.m);
+  const int64_t begin = rows_begin(p.m), end = rows_end(p.m);
   const int64_t tile = p.m.T * 2 * p.N;
   for (int e = threadIdx.x; e < rows * per; e += blockDim.x) {
     const int t = e / per, f = e % per, kind = f / (p.G * nq), g = f / nq % p.G, n = f % nq * 4;
     const int64_t r = r0 + t;
     const int cnt = min(4, p.N - n);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < end) {
+    if (r >= begin && r < end) {
       const float* src = p.pBC + (int64_t)g * p.tpg * tile + r * 2 * p.N + kind * p.N + n;
 #pragma unroll 4
       for (int i = 0; i < p.tpg; ++i, src += tile) {

@@ -84,8 +84,8 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """Causal depthwise convolution of the sequences in ``x``; y has x's shape and type.
 
     x: (S, L, C), or packed (rows, C) with ``cu_seqlens`` (S + 1, int32): sequence s owns rows
-    cu_seqlens[s] .. cu_seqlens[s+1] - 1 (none, if they are equal); rows from cu_seqlens[S] on
-    belong to no sequence and come out as zeros. Rows may lie at any stride (a slice of
+    cu_seqlens[s] .. cu_seqlens[s+1] - 1 (none, if they are equal); rows in front of cu_seqlens[0]
+    and from cu_seqlens[S] on belong to no sequence and come out as zeros. Rows may lie at any stride (a slice of
     the in_proj output is read in place). weight (C, K) or (C, 1, K), K from 1 to 8, bias (C,).
 
     Training: gradients flow to x, weight and bias, every sequence starts from zeros.

@@ -34,3 +34,75 @@ def test_gate_gradient_is_rounded_once(kind, ch, N, G, pad, dtt):
     out, size = oss.scan(*args, dy=dy.double()), oss.scan(*args, dy=dy.double(), absolute=True)
     longest = max(b - a for a, b in zip(cu[:-1], cu[1:]))
     _near(dz, out["dz"], size["dz"], 16 * longest + 128, torch.bfloat16, "dz")
+
+
+@pytest.fixture
+def poisoned():
+    """Every fresh allocation starts as NaN, so that what a kernel leaves unwritten shows."""
+    before = torch.are_deterministic_algorithms_enabled(), torch.utils.deterministic.fill_uninitialized_memory
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    torch.utils.deterministic.fill_uninitialized_memory = True
+    yield
+    torch.use_deterministic_algorithms(before[0])
+    torch.utils.deterministic.fill_uninitialized_memory = before[1]
+
+
+# Offsets that begin above 0: short sequences, more unused rows than pieces, sequences that are cut
+# into pieces, a batch of which one sequence is cut (it fills the GPU), none at all.
+FRONT = {"short": ([5, 12, 20], 24), "far": ([700, 701, 703, 703, 720], 900), "pieces": ([37, 437, 440], 443),
+         "outlier": ([3, 303] + [303 + 3 * i for i in range(1, 310)], 1235), "none": ([4, 4], 9), "end": ([9, 9, 9], 9)}
+
+
+@pytest.mark.parametrize("kind", FRONT)
+@pytest.mark.parametrize("ch,N,G", [(40, 16, 1), (33, 5, 3), (8, 128, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_in_front_of_the_first_sequence(kind, ch, N, G, dtype, poisoned):
+    """A slice of a larger batch: rows that no sequence owns, in front and behind, come out as
+    zeros in outputs and gradients, and reach nothing else."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, short_conv
+
+    cu, rows = FRONT[kind]
+    S, g = len(cu) - 1, gen(ch + N)
+    t = _scan_problem(rows, ch, N, G, g, dtype)
+    w, b, dy = randn((ch, 4), g, scale=0.5).float(), randn((ch,), g).float(), randn((rows, ch), g).to(dtype)
+    cud = torch.tensor(cu, dtype=torch.int32, device=cuda())
+    unused = torch.tensor([i < cu[0] or i >= cu[-1] for i in range(rows)])
+    t["x"][unused], dy[unused] = float("nan"), float("nan")
+    v = {k: u.to(cuda()).requires_grad_() for k, u in dict(t, w=w, b=b).items()}
+    clean = {k: torch.where(unused.view((-1,) + (1,) * (u.dim() - 1)), torch.zeros_like(u), u) if u.shape[0] == rows and k not in ("A", "D", "dt_bias")
+             else u for k, u in t.items()}
+    d = {k: u.double() for k, u in clean.items()}
+    dy64 = torch.where(unused[:, None], torch.zeros_like(dy), dy).double()
+
+    y = short_conv(v["x"], v["w"], v["b"], cu_seqlens=cud)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, (v["x"], v["w"], v["b"]), dy.to(cuda()))), y=y)
+    out = oss.conv(d["x"], w.double(), b.double(), cu, dy=dy64)
+    size = oss.conv(d["x"].abs(), w.double().abs(), b.double().abs(), cu, False, dy=dy64.abs())
+    grow = 1.1 + size["y"].amax()
+    _near(got["y"], out["y"], size["y"], 64, dtype, "conv y")
+    _near(got["dx"], out["dx"], size["dx"] * grow, 64, dtype, "conv dx")
+    _near(got["dw"], out["dw"], size["aw"] * grow, 64 + min(rows, 64) + 64, torch.float32, "conv dw")
+    _near(got["db"], out["db"], size["ab"] * grow, 64 + min(rows, 64) + 64, torch.float32, "conv db")
+    for k in ("y", "dx"):
+        assert not got[k].cpu()[unused].any(), k  # NaN counts as true
+
+    names = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")
+    y = selective_state_scan(*[v[k] for k in names[:5]], D=v["D"], z=v["z"], dt_bias=v["dt_bias"], cu_seqlens=cud)
+    got = dict(zip(names, torch.autograd.grad(y, [v[k] for k in names], dy.to(cuda()))))
+    args = (d["x"], d["dt"], d["A"], d["B"], d["C"], cu, d["D"], d["z"], d["dt_bias"])
+    out, size = oss.scan(*args, dy=dy64), oss.scan(*args, dy=dy64, absolute=True)
+    longest = max(q - p for p, q in zip(cu[:-1], cu[1:]))
+    _near(y, out["y"], size["y"], 8 * longest + 64, dtype, "y")
+    assert not y.cpu()[unused].any()
+    for k in names:
+        n = 16 * longest + 128 + (ch if k in ("B", "C") else rows if k in ("A", "D", "dt_bias") else 0)
+        _near(got[k], out["d" + k], size["d" + k], n, got[k].dtype, "d" + k)
+        assert k in ("A", "D", "dt_bias") or not got[k].cpu()[unused].any(), k
+
+    with torch.no_grad():
+        for call, shape, dt in ((lambda p: short_conv(v["x"], v["w"], v["b"], cu_seqlens=cud, state=p), (3, ch), dtype),
+                                (lambda p: selective_state_scan(*[v[k] for k in names[:5]], D=v["D"], z=v["z"],
+                                                                dt_bias=v["dt_bias"], cu_seqlens=cud, state=p), (ch, N),
+                                 torch.float32)):
+            y = call(torch.zeros((S,) + shape, dtype=dt, device=cuda())).cpu()
+            assert not y[unused].any() and bool(torch.isfinite(y).all())
