@@ -150,6 +150,10 @@ inline void set_pieces(SeqMap* m, int64_t Q) {
   m->pieces = m->cu == nullptr ? m->S * m->per : m->T / Q + m->S;
 }
 
+// Host: a forward without rows and without a pool has no output. It returns before it looks for its
+// GPU, which only an output's address could tell.
+inline bool nothing_to_do(const SeqMap& m) { return m.T == 0 && (m.S == 0 || m.n_slots == 0); }
+
 // Host: checks the sequence fields shared by the argument structs.
 inline int check_seqs(const char* what, int64_t S, int64_t T, int64_t L, const int32_t* cu, const void* state,
                       const int32_t* slots, const uint8_t* fresh, int64_t n_slots, SeqMap* m) {

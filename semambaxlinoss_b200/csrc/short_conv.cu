@@ -539,7 +539,7 @@ int semx_short_conv_fwd(const SemxShortConvArgs* a, semx_stream_t stream) {
   SEMX_CHECK_ARGS(a, SemxShortConvArgs);
   CvParams p = {};
   int rc = cv_validate(a, false, &p);
-  if (rc != SEMX_OK) return rc;
+  if (rc != SEMX_OK || semx::nothing_to_do(p.m)) return rc;
   semx::DeviceScope scope;
   rc = scope.bind({a->y, a->state});
   if (rc != SEMX_OK) return rc;

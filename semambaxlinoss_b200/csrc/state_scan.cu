@@ -462,7 +462,7 @@ int semx_state_scan_fwd(const SemxStateScanArgs* a, semx_stream_t stream) {
   SEMX_CHECK_ARGS(a, SemxStateScanArgs);
   ScanParams p = {};
   int rc = scan_validate(a, false, &p);
-  if (rc != SEMX_OK) return rc;
+  if (rc != SEMX_OK || semx::nothing_to_do(p.m)) return rc;
   semx::DeviceScope scope;
   rc = scope.bind({a->y, a->state});
   if (rc != SEMX_OK) return rc;
