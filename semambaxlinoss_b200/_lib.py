@@ -12,6 +12,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 import os
 
@@ -447,6 +448,16 @@ def scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
 def cast(grad: torch.Tensor | None, dtype) -> torch.Tensor | None:
     """A gradient in its parameter's type."""
     return grad if grad is None or grad.dtype == dtype else grad.to(dtype)
+
+
+def refuse_tangents(op: str, *operands: torch.Tensor | None) -> None:
+    """Refuses operands that carry a forward-mode tangent. They need no gradient, so a call would
+    go past its autograd function, which has no jvp either, and lose the tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level: no tangents (60 ns a call)
+        return
+    for t in operands:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{op}: forward-mode derivatives are not implemented")
 
 
 def new_args(cls):

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from semambaxlinoss_b200 import _lib
 from tests.test_selective_state_cpu import _status
@@ -21,3 +22,18 @@ def test_an_empty_forward_launches_nothing(S, cu):
     assert _status("semx_state_scan_fwd", _lib.SemxStateScanArgs, scan) == _lib.SEMX_OK
     assert _status("semx_state_scan_bwd", _lib.SemxStateScanArgs, scan, workspace=256) == _lib.SEMX_OK
     assert _lib.launch_count() == before
+
+
+def test_tangents_are_refused_inside_a_dual_level_only():
+    from torch.autograd import forward_ad
+
+    x, w = torch.randn(3), torch.randn(3)
+    _lib.refuse_tangents("op", x, None, w)
+    with forward_ad.dual_level():
+        _lib.refuse_tangents("op", x, None, w)
+        d = forward_ad.make_dual(x, torch.ones(3))
+        for operands in ((d,), (w, None, d), (w, d[1:])):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="^op: "):
+                    _lib.refuse_tangents("op", *operands)
+    _lib.refuse_tangents("op", d)  # outside of its level a dual tensor is a plain one

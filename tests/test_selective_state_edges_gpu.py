@@ -106,3 +106,33 @@ def test_rows_in_front_of_the_first_sequence(kind, ch, N, G, dtype, poisoned):
                                  torch.float32)):
             y = call(torch.zeros((S,) + shape, dtype=dt, device=cuda())).cpu()
             assert not y[unused].any() and bool(torch.isfinite(y).all())
+
+
+def test_forward_mode_tangents_are_refused():
+    """Every operand of every operator: a tangent is refused, not lost, and no state moves."""
+    from torch.autograd import forward_ad
+
+    from semambaxlinoss_b200.layer_norm import LayerNorm, layer_norm
+    from semambaxlinoss_b200.selective_state import (selective_state_scan, selective_state_step, short_conv,
+                                                     short_conv_step)
+
+    dev, ch, N = cuda(), 8, 4
+    r = lambda *s: torch.randn(*s, device=dev)  # noqa: E731
+    x, BC, vec = r(2, 5, ch), r(2, 5, N), r(ch)
+    conv = dict(x=x, weight=r(ch, 4), bias=vec)
+    scan = dict(x=x, dt=x.clone(), A=-r(ch, N).abs(), B=BC, C=BC.clone(), D=vec, z=x.clone(), dt_bias=vec.clone())
+    one = {k: u[:, 0] if k in ("x", "dt", "B", "C", "z") else u for k, u in scan.items()}
+    window, state = torch.zeros(2, 3, ch, device=dev), torch.zeros(2, ch, N, device=dev)
+    calls = [(short_conv, conv), (short_conv, dict(conv, state=window)), (selective_state_scan, scan),
+             (selective_state_scan, dict(scan, state=state)), (selective_state_step, dict(one, state=state)),
+             (short_conv_step, dict(conv, x=x[:, 0], state=window)),
+             (layer_norm, dict(x=x, weight=vec, bias=vec.clone(), residual=x.clone())),
+             (LayerNorm(ch, device=dev), dict(x=x, residual=x.clone()))]
+    for call, kw in calls:
+        with torch.no_grad():
+            call(**kw)
+        window.zero_(), state.zero_()
+        for name in kw:
+            with forward_ad.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
+                call(**dict(kw, **{name: forward_ad.make_dual(kw[name], torch.ones_like(kw[name]))}))
+            assert not window.any() and not state.any(), (call, name)
