@@ -450,14 +450,18 @@ def cast(grad: torch.Tensor | None, dtype) -> torch.Tensor | None:
     return grad if grad is None or grad.dtype == dtype else grad.to(dtype)
 
 
+def has_tangents(*operands: torch.Tensor | None) -> bool:
+    """Whether one of the operands carries a forward-mode tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level: no tangents (60 ns a call)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands)
+
+
 def refuse_tangents(op: str, *operands: torch.Tensor | None) -> None:
     """Refuses operands that carry a forward-mode tangent. They need no gradient, so a call would
     go past its autograd function, which has no jvp either, and lose the tangent."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level: no tangents (60 ns a call)
-        return
-    for t in operands:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError(f"{op}: forward-mode derivatives are not implemented")
+    if has_tangents(*operands):
+        raise NotImplementedError(f"{op}: forward-mode derivatives are not implemented")
 
 
 def new_args(cls):

@@ -4,7 +4,7 @@
   ``y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias`` over the last dimension, in
   fp32 arithmetic, with gradients for every input.
 * :class:`LayerNorm` — the module: parameters, names and initial values of
-  ``nn.LayerNorm(d, eps)``, forward through the operator. ``create_block`` builds it with
+  ``nn.LayerNorm(d, eps)``, which it is, forward through the operator. ``create_block`` builds it with
   ``rms_norm=False, fused_add_norm=True``, and the pre-norm ``Block`` then runs its
   residual add and its norm as one kernel.
 
@@ -144,16 +144,36 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
     return y if residual is None else (y, s)
 
 
-class LayerNorm(nn.Module):
-    """Layer norm over the last dimension with a learned gain and offset (``nn.LayerNorm``'s
-    parameters and state dict), through :func:`layer_norm`. ``forward(x, residual)`` adds the
-    residual first and returns (y, x + residual)."""
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` over the last dimension, with its parameters and state dict, through
+    :func:`layer_norm`. ``forward(x, residual)`` adds the residual first and returns
+    (y, x + residual)."""
 
     def __init__(self, hidden_size: int, eps: float = 1e-5, device=None, dtype=None):
-        super().__init__()
-        self.eps = eps
-        self.weight = nn.Parameter(torch.ones(hidden_size, device=device, dtype=dtype))
-        self.bias = nn.Parameter(torch.zeros(hidden_size, device=device, dtype=dtype))
+        super().__init__(hidden_size, eps, device=device, dtype=dtype)
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None):
+    def takes(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> bool:
+        """Whether ``self(x, residual, out_dtype=weight.dtype)`` is a call of the operator's."""
+        w = self.weight
+        return (x.is_cuda and x.dtype in _TYPES and w.dtype in _TYPES and w.get_device() == x.get_device()
+                and w.shape[0] <= MAX_WIDTH and not _lib.has_tangents(x, residual, w, self.bias)
+                and (residual is None or (residual.dtype in _TYPES and residual.shape == x.shape
+                                          and residual.get_device() == x.get_device())))
+
+    def add(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """(the norm of x + residual in the weight's type, x + residual), in one kernel where the
+        operator takes the tensors, else as ``nn.LayerNorm`` behind an addition."""
+        dtype = self.weight.dtype
+        if residual is None:
+            rows = x.to(dtype=dtype)
+            return self(rows, plain=not self.takes(rows)), x
+        if self.takes(x, residual):
+            return self(x, residual, out_dtype=dtype)
+        residual = x + residual
+        return self(residual.to(dtype=dtype), plain=True), residual
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                plain: bool = False):
+        if plain:  # as nn.LayerNorm, for what the operator does not take (see add)
+            return super().forward(x)
         return layer_norm(x, self.weight, self.bias, self.eps, residual, out_dtype)

@@ -13,7 +13,8 @@ checkout. Their documented behaviour is restated here:
   ``h = mixer(norm(residual))``; returns ``(h, residual)``; the caller adds the final
   residual.
 * ``create_block(rms_norm=False, fused_add_norm=True)`` takes this package's ``LayerNorm``
-  (nn.LayerNorm's parameters), whose kernel adds the residual and normalises in one pass.
+  (an nn.LayerNorm), whose kernel adds the residual and normalises in one pass; tensors that
+  the kernel does not take (CPU, other types, wider rows) run as nn.LayerNorm behind an addition.
 * ``_init_weights(module, n_layer)``: zero every Linear bias not tagged ``_no_reinit``;
   re-draw every ``out_proj.weight`` / ``fc2.weight`` Kaiming-uniform (a = sqrt(5)) and
   divide it by sqrt(n_layer).
@@ -111,7 +112,8 @@ class RMSNorm(nn.Module):
 
 class Block(nn.Module):
     """Pre-norm residual block: returns (mixer(norm(x + residual)), x + residual). With
-    ``fused_add_norm`` and this package's LayerNorm the sum and the norm are one kernel."""
+    ``fused_add_norm`` and this package's LayerNorm the sum and the norm are one kernel where
+    it takes the tensors."""
 
     def __init__(self, dim, mixer_cls, mlp_cls=nn.Identity, norm_cls=nn.LayerNorm,
                  fused_add_norm=False, residual_in_fp32=False):
@@ -128,7 +130,7 @@ class Block(nn.Module):
 
     def forward(self, hidden_states, residual=None, inference_params=None, **mixer_kwargs):
         if self.fused_add_norm and isinstance(self.norm, LayerNorm):
-            hidden_states, residual = _add_norm(self.norm, hidden_states, residual)
+            hidden_states, residual = self.norm.add(hidden_states, residual)
         else:
             residual = hidden_states + residual if residual is not None else hidden_states
             hidden_states = self.norm(residual.to(dtype=self.norm.weight.dtype))
@@ -137,19 +139,12 @@ class Block(nn.Module):
         hidden_states = self.mixer(hidden_states, inference_params=inference_params, **mixer_kwargs)
         if self.mlp is not None:
             if self.fused_add_norm and isinstance(self.norm2, LayerNorm):
-                hidden_states, residual = _add_norm(self.norm2, hidden_states, residual)
+                hidden_states, residual = self.norm2.add(hidden_states, residual)
             else:
                 residual = hidden_states + residual
                 hidden_states = self.norm2(residual.to(dtype=self.norm2.weight.dtype))
             hidden_states = self.mlp(hidden_states)
         return hidden_states, residual
-
-
-def _add_norm(norm: LayerNorm, x, residual):
-    """(norm(x + residual) in the norm's type, x + residual) as one kernel."""
-    if residual is None:
-        return norm(x.to(dtype=norm.weight.dtype)), x
-    return norm(x, residual, out_dtype=norm.weight.dtype)
 
 
 def _init_weights(module, n_layer, initializer_range=0.02, rescale_prenorm_residual=True,
@@ -170,7 +165,7 @@ def _init_weights(module, n_layer, initializer_range=0.02, rescale_prenorm_resid
 def _apply_layer_norm(x, residual, norm_layer):
     """Pre-norm add + norm: returns (norm(x + residual), x + residual)."""
     if isinstance(norm_layer, LayerNorm):
-        return _add_norm(norm_layer, x, residual)
+        return norm_layer.add(x, residual)
     residual = x + residual if residual is not None else x
     return norm_layer(residual), residual
 
