@@ -98,6 +98,8 @@ class SelectiveStateMixer(nn.Module):
         # ``inference_params`` is accepted for the pre-norm Block's calling convention; the
         # state of running sequences is in ``cache``.
         del inference_params
+        if cache is None and (slots is not None or fresh is not None):
+            raise ValueError("SelectiveStateMixer: slots / fresh without a cache")
         if cache is not None and fresh is None and cu_seqlens is None and x.dim() == 3 and x.shape[1] == 1:
             return self.step(x[:, 0], cache, slots).unsqueeze(1)
         xz = self.in_proj(x)

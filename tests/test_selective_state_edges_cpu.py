@@ -37,3 +37,13 @@ def test_tangents_are_refused_inside_a_dual_level_only():
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="^op: "):
                     _lib.refuse_tangents("op", *operands)
     _lib.refuse_tangents("op", d)  # outside of its level a dual tensor is a plain one
+
+
+def test_the_mixer_refuses_slots_without_a_cache():
+    """As the operators below it do without a state; neither is dropped."""
+    from semambaxlinoss_b200.selective_state import SelectiveStateMixer
+
+    mixer, x = SelectiveStateMixer(8), torch.randn(2, 5, 8)
+    for bad in (dict(slots=torch.zeros(2, dtype=torch.int32)), dict(fresh=torch.ones(2, dtype=torch.bool))):
+        with pytest.raises(ValueError, match="without a cache"):
+            mixer(x, **bad)
