@@ -81,7 +81,7 @@ class SelectiveStateMixer(nn.Module):
         w = self.in_proj.weight
         dev = w.device if device is None else device
         return MixerCache(torch.zeros(entries, self.d_conv - 1, self.inner_dim, device=dev, dtype=dtype or w.dtype),
-                          torch.zeros(entries, self.inner_dim, self.d_state, device=dev))
+                          torch.zeros(entries, self.inner_dim, self.d_state, device=dev, dtype=torch.float32))
 
     def _operands(self, u):
         """(dt, B, C) of the convolved rows u."""

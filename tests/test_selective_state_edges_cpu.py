@@ -47,3 +47,19 @@ def test_the_mixer_refuses_slots_without_a_cache():
     for bad in (dict(slots=torch.zeros(2, dtype=torch.int32)), dict(fresh=torch.ones(2, dtype=torch.bool))):
         with pytest.raises(ValueError, match="without a cache"):
             mixer(x, **bad)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_the_state_is_fp32_under_any_default_type(default):
+    """A model built under torch.set_default_dtype gets the cache that the scan takes."""
+    from semambaxlinoss_b200.selective_state import SelectiveStateMixer
+
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        mixer = SelectiveStateMixer(8)
+        cache = mixer.allocate_cache(3)
+    finally:
+        torch.set_default_dtype(before)
+    assert mixer.in_proj.weight.dtype == cache.window.dtype == default
+    assert cache.state.dtype == torch.float32 and not cache.state.any()
