@@ -267,12 +267,13 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
     elif ssm in _OUT_OF_SCOPE:
         raise NotImplementedError(
             f"mixer {ssm!r} is not part of this package (only the selective-LRU and LinOSS "
-            "scan layers are)"
+            "scan layers and the selective state mixer are)"
+            + ("; 'selective_state' has that layer's formulas and parameter names" if ssm == "mamba" else "")
         )
     else:
         raise ValueError(
             f"Unknown mixer {ssm!r}; expected 'mamba', 'mamba2', 'mamba3', "
-            "'linoss', 'selective_lru', 'selective_lru_mimo', 's4d', or 's5'."
+            "'linoss', 'selective_lru', 'selective_lru_mimo', 'selective_state', 's4d', or 's5'."
         )
     return partial(MambaStyleMixer, ssm=layer, expand=expand, d_conv=d_conv, causal_conv=causal)
 

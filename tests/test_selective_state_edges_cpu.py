@@ -63,3 +63,15 @@ def test_the_state_is_fp32_under_any_default_type(default):
         torch.set_default_dtype(before)
     assert mixer.in_proj.weight.dtype == cache.window.dtype == default
     assert cache.state.dtype == torch.float32 and not cache.state.any()
+
+
+def test_the_factory_names_the_selective_state_mixer():
+    from semambaxlinoss_b200.mamba_block import create_block
+
+    cfg = {"d_state": 4, "d_conv": 4, "expand": 2}
+    for name in ("mamba", "s4d"):
+        with pytest.raises(NotImplementedError, match="selective state mixer") as e:
+            create_block(8, dict(cfg, ssm=name))
+        assert ("'selective_state'" in str(e.value)) == (name == "mamba")
+    with pytest.raises(ValueError, match="'selective_state'"):
+        create_block(8, dict(cfg, ssm="unknown"))
