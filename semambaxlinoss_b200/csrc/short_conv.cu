@@ -54,14 +54,6 @@ struct Raw {
   typedef uint32_t type;
 };
 template <>
-struct Raw<false, 4> {
-  typedef uint4 type;
-};
-template <>
-struct Raw<true, 4> {
-  typedef uint2 type;
-};
-template <>
 struct Raw<false, 2> {
   typedef uint2 type;
 };
@@ -88,16 +80,10 @@ __device__ __forceinline__ void st_raw(void* base, int64_t i, const typename Raw
 }
 template <bool BF16, int V>
 __device__ __forceinline__ void unpack(const typename Raw<BF16, V>::type& r, float (&v)[V]) {
-  if constexpr (V == 4 && BF16) {
-    v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
-    v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
-  } else if constexpr (V == 2 && BF16) {
+  if constexpr (V == 2 && BF16) {
     v[0] = __uint_as_float(r << 16); v[1] = __uint_as_float(r & 0xffff0000u);
   } else if constexpr (V == 2) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
-  } else if constexpr (V == 4) {
-    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
-    v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
   } else if constexpr (BF16) {
     v[0] = __uint_as_float(r << 16);
   } else {
@@ -106,18 +92,10 @@ __device__ __forceinline__ void unpack(const typename Raw<BF16, V>::type& r, flo
 }
 template <bool BF16, int V>
 __device__ __forceinline__ void st_vec(void* base, int64_t i, const float (&v)[V]) {
-  if constexpr (V == 4 && BF16) {
-    uint2 q;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
-    h[0] = __floats2bfloat162_rn(v[0], v[1]);
-    h[1] = __floats2bfloat162_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = q;
-  } else if constexpr (V == 2 && BF16) {
+  if constexpr (V == 2 && BF16) {
     *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = __floats2bfloat162_rn(v[0], v[1]);
   } else if constexpr (V == 2) {
     *reinterpret_cast<float2*>(reinterpret_cast<float*>(base) + i) = make_float2(v[0], v[1]);
-  } else if constexpr (V == 4) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i) = make_float4(v[0], v[1], v[2], v[3]);
   } else if constexpr (BF16) {
     reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16(v[0]);
   } else {
@@ -142,24 +120,20 @@ __device__ __forceinline__ void input(const CvParams& p, const semx::Piece& q, i
 }
 
 // The CTA's weights (a run of w) go through shared memory, where a thread's V K values are
-// one run too: read from global memory they cost as much as 32 rows of x. PAD keeps the
-// runs of neighbouring threads in other banks.
+// one run too: read from global memory they cost as much as 32 rows of x.
 template <int V, int K>
 struct Weights {
-  static constexpr int RUN = V * K, PAD = RUN % 32 == 0 ? 4 : 0;
-  float v[kT * (RUN + PAD)];
+  float v[kT * V * K];
 };
 template <int V, int K>
 __device__ __forceinline__ void stage_weights(Weights<V, K>& s, const float* w, int c0, int C) {
-  constexpr int RUN = V * K, PAD = Weights<V, K>::PAD;
   const int n = min((int)blockDim.x * V, C - c0) * K;
   const float* src = w + (int64_t)c0 * K;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) s.v[i + i / RUN * PAD] = src[i];
+  for (int i = threadIdx.x; i < n; i += blockDim.x) s.v[i] = src[i];
 }
 template <int V, int K>
 __device__ __forceinline__ void own_weights(const Weights<V, K>& s, float (&w)[K][V]) {
-  constexpr int RUN = V * K, PAD = Weights<V, K>::PAD;
-  const float* mine = s.v + threadIdx.x * (RUN + PAD);
+  const float* mine = s.v + threadIdx.x * (V * K);
 #pragma unroll
   for (int i = 0; i < V; ++i)
 #pragma unroll
