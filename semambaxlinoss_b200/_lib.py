@@ -445,6 +445,20 @@ def scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
     return like.new_empty((max((nbytes + 3) // 4, 1),), dtype=torch.float32)
 
 
+def param32(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A parameter as the kernels read it: contiguous fp32 (no copy where it is that already)."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
+
+
+def as_rows(t: torch.Tensor, dtype) -> torch.Tensor:
+    """An arriving gradient, contiguous in ``dtype``: itself where it is that already."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def cast(grad: torch.Tensor | None, dtype) -> torch.Tensor | None:
     """A gradient in its parameter's type."""
     return grad if grad is None or grad.dtype == dtype else grad.to(dtype)

@@ -22,12 +22,6 @@ _TYPES = (torch.float32, torch.bfloat16)
 MAX_WIDTH = 32768
 
 
-def _param(p):
-    if p is None or (p.dtype == torch.float32 and p.is_contiguous()):
-        return p
-    return p.detach().to(torch.float32).contiguous()
-
-
 def _forward(x, weight, bias, eps, residual, out_dtype, stats):
     """Runs the forward; returns (y, s, kept): kept (2, rows) holds mean and 1 / sqrt(var + eps)
     where ``stats``, else None."""
@@ -61,8 +55,8 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual, out_dtype):
         ctx.set_materialize_grads(False)
-        w = _param(weight)
-        y, s, kept = _forward(x, w, _param(bias), eps, residual, out_dtype, True)
+        w = _lib.param32(weight)
+        y, s, kept = _forward(x, w, _lib.param32(bias), eps, residual, out_dtype, True)
         ctx.save_for_backward(s, w, kept)
         ctx.cfg = (eps, out_dtype, x.dtype, None if residual is None else residual.dtype,
                    None if weight is None else weight.dtype, None if bias is None else bias.dtype)
@@ -77,8 +71,8 @@ class _LayerNorm(torch.autograd.Function):
             return None, None, None, None, None, None
         shape = s.shape
         d = shape[-1]
-        dy = s.new_zeros(shape, dtype=ydt) if dy is None else _as(dy, ydt)
-        dsum = None if dsum is None else _as(dsum, s.dtype)
+        dy = s.new_zeros(shape, dtype=ydt) if dy is None else _lib.as_rows(dy, ydt)
+        dsum = None if dsum is None else _lib.as_rows(dsum, s.dtype)
         dx = s.new_empty(shape, dtype=xdt)
         a = _lib.new_args(_lib.SemxLayerNormArgs)
         a.eps, a.n, a.d = eps, kept.shape[1], d
@@ -100,13 +94,6 @@ class _LayerNorm(torch.autograd.Function):
             a.workspace = ws.data_ptr()
         _lib.call("semx_layer_norm_bwd", a, s.device)
         return (dx, _lib.cast(dw, wdt), _lib.cast(db, bdt), None, dr if rdt is not None else None, None)
-
-
-def _as(t, dtype):
-    """t contiguous in ``dtype``, itself where it is that already."""
-    if t.dtype != dtype:
-        t = t.to(dtype)
-    return t if t.is_contiguous() else t.contiguous()
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -140,7 +127,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
             x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
             or (residual is not None and residual.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, residual, out_dtype)
-    y, s, _ = _forward(x, _param(weight), _param(bias), eps, residual, out_dtype, False)
+    y, s, _ = _forward(x, _lib.param32(weight), _lib.param32(bias), eps, residual, out_dtype, False)
     return y if residual is None else (y, s)
 
 

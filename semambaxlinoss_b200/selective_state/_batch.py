@@ -36,20 +36,6 @@ def check_same(op: str, name: str, t: torch.Tensor, shape, dtypes, dev: int) -> 
                          f"on {t.device}")
 
 
-def param32(t: torch.Tensor | None) -> torch.Tensor | None:
-    """A parameter as the kernels read it: contiguous fp32 (no copy where it is that already)."""
-    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
-        return t
-    return t.detach().to(torch.float32).contiguous()
-
-
-def as_rows(t: torch.Tensor, dtype) -> torch.Tensor:
-    """An arriving gradient, contiguous in ``dtype``: itself where it is that already."""
-    if t.dtype != dtype:
-        t = t.to(dtype)
-    return t if t.is_contiguous() else t.contiguous()
-
-
 def batch(op: str, x: torch.Tensor, cu_seqlens) -> tuple[int, int, int]:
     """(S, rows, L) of x (S, L, C), or of packed x (rows, C) with cu_seqlens (S + 1)."""
     if not x.is_cuda:

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._batch import TYPES, as_rows, batch, check_same, param32, rows_of, set_pool
+from ._batch import TYPES, batch, check_same, rows_of, set_pool
 
 _ACTIVATIONS = {"silu": 1, None: 0}
 
@@ -44,7 +44,7 @@ def _args(x, w, b, silu, S, rows, L, cu):
 class _ShortConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, silu, S, rows, L, cu):
-        w, b = param32(weight), param32(bias)
+        w, b = _lib.param32(weight), _lib.param32(bias)
         a, xr = _args(x, w, b, silu, S, rows, L, cu)
         y = x.new_empty(x.shape)
         a.y = y.data_ptr()
@@ -59,7 +59,7 @@ class _ShortConv(torch.autograd.Function):
         x, w, b, cu = ctx.saved_tensors
         silu, S, rows, L, wdt, bdt = ctx.cfg
         a, xr = _args(x, w, b, silu, S, rows, L, cu)
-        dy = as_rows(dy, x.dtype)
+        dy = _lib.as_rows(dy, x.dtype)
         dx = x.new_empty(x.shape)
         dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
@@ -115,7 +115,7 @@ def _run(op, x, weight, bias, activation, S, rows, L, cu_seqlens, state, slots, 
         if slots is not None or fresh is not None:
             raise ValueError(f"{op}: slots / fresh without a state")
         return _ShortConv.apply(x, w, bias, silu, S, rows, L, cu_seqlens)
-    w, bias = param32(w), param32(bias)
+    w, bias = _lib.param32(w), _lib.param32(bias)
     a, xr = _args(x, w, bias, silu, S, rows, L, cu_seqlens)
     K = w.shape[1]
     if K > 1 or state is None:  # one tap keeps nothing

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._batch import TYPES, as_rows, batch, check_same, param32, rows_of, set_pool
+from ._batch import TYPES, batch, check_same, rows_of, set_pool
 
 MAX_MODES = 128
 _F32 = (torch.float32,)
@@ -89,7 +89,7 @@ def _args(x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu, N, G):
 class _StateScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu, N, G):
-        A32, D32, b32 = param32(A), param32(D), param32(dt_bias)
+        A32, D32, b32 = _lib.param32(A), _lib.param32(D), _lib.param32(dt_bias)
         a, kept = _args(x, dt, A32, B, C, D32, z, b32, softplus, S, rows, L, cu, N, G)
         dev = x.device
         y = x.new_empty(x.shape)
@@ -112,7 +112,7 @@ class _StateScan(torch.autograd.Function):
         softplus, S, rows, L, N, G, Bshape, (Adt, Ddt, bdt) = ctx.cfg
         a, kept = _args(x, dt, A, B, C, D, z, bias, softplus, S, rows, L, cu, N, G)
         dev = x.device
-        dy = as_rows(dy, x.dtype)
+        dy = _lib.as_rows(dy, x.dtype)
         dx, ddt = x.new_empty(x.shape), dt.new_empty(x.shape)
         dz = None if z is None else x.new_empty(x.shape)
         dB, dC = x.new_empty(Bshape), x.new_empty(Bshape)
@@ -159,7 +159,7 @@ def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
         if slots is not None or fresh is not None:
             raise ValueError(f"{op}: slots / fresh without a state")
         return _StateScan.apply(x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu_seqlens, N, G)
-    A, D, dt_bias = param32(A), param32(D), param32(dt_bias)
+    A, D, dt_bias = _lib.param32(A), _lib.param32(D), _lib.param32(dt_bias)
     a, kept = _args(x, dt, A, B, C, D, z, dt_bias, softplus, S, rows, L, cu_seqlens, N, G)
     dev = x.device
     set_pool(op, a, S, x.get_device(), state, (ch, N), torch.float32, slots, fresh)
@@ -191,7 +191,7 @@ def selective_state_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     if _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
         raise ValueError(f"{op}: a state is for inference; the call wants gradients")
     S = x.shape[0]
-    A, D, dt_bias = param32(A), param32(D), param32(dt_bias)
+    A, D, dt_bias = _lib.param32(A), _lib.param32(D), _lib.param32(dt_bias)
     a, kept = _args(x, dt, A, B, C, D, z, dt_bias, int(bool(dt_softplus)), S, S, 1, None, N, G)
     set_pool(op, a, S, x.get_device(), state, (ch, N), torch.float32, slots, None)
     y = x.new_empty(x.shape)
