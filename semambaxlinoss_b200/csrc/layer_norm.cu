@@ -10,7 +10,8 @@
 // Bound: HBM. Forward reads x (and r) once and writes y (and s) once; backward reads s, dy
 // (and the gradient of s) once and writes dx (and dr) once. A row therefore stays in the
 // registers of its TPR threads (8 V elements each) between the statistics and the result,
-// and a CTA walks over many rows so that w, b and the sums dw, db stay in registers too.
+// and a CTA walks over many rows so that the sums dw, db stay in registers too, and w and b
+// where a row is narrow (keeps_params).
 // The statistics are two-step (mean, then squares about it): a warp does both by shuffles,
 // and the warps of a wide row join their (mean, squares) pairs with the exact update for
 // the mean of two samples, so a wide row costs one barrier. All arithmetic is fp32.

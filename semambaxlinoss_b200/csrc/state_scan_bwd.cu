@@ -558,7 +558,8 @@ __global__ void __launch_bounds__(256) state_scan_bc_kernel(const ScanParams p, 
   }
 }
 
-// At least two lanes per channel: the tiles of one would not fit shared memory.
+// At least two lanes per channel: with one, a thread would hold four rows of every operand of a tile
+// beside a CTA's 60 KB of shared memory. So up to 4 modes leave half of the lanes without any.
 int mode_lanes(int N) { return lanes_for(N, 4) < 2 ? 2 : lanes_for(N, 4); }
 int tile_channels(int N) { return kThreads / mode_lanes(N) * kCPT; }
 
