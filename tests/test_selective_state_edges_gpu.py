@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import tests.test_selective_state_gpu as base
 from oracle import selective_state as oss
 from tests.parity import cuda, gen, randn
 from tests.test_selective_state_gpu import _batched, _near, _scan_problem, _seqs, _strided
@@ -136,3 +137,126 @@ def test_forward_mode_tangents_are_refused():
             with forward_ad.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
                 call(**dict(kw, **{name: forward_ad.make_dual(kw[name], torch.ones_like(kw[name]))}))
             assert not window.any() and not state.any(), (call, name)
+
+
+# Rows, groups and modes on four elements, so that every operand is read four at a time, with 8, 16
+# and 32 lanes per channel (a lane holds four modes), full and partly used, and the gate.
+VECTORS = [(264, 32, 1, 4), (48, 28, 2, 0), (16, 64, 1, 0), (40, 36, 1, 8), (24, 128, 2, 8), (32, 100, 1, 0)]
+
+
+@pytest.mark.parametrize("kind", ["one", "short", "even", "ragged", "long"])
+@pytest.mark.parametrize("ch,N,G,pad", VECTORS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_vector_rows_of_many_modes_training(kind, ch, N, G, pad, dtype):
+    base.test_scan_training(kind, ch, N, G, pad, True, True, True, dtype, None)
+
+
+@pytest.mark.parametrize("kind", ["one", "short", "even", "ragged", "long", "many"])
+@pytest.mark.parametrize("ch,N,G", [v[:3] for v in VECTORS])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_vector_rows_of_many_modes_prompts(kind, ch, N, G, dtype):
+    base.test_scan_prompts(kind, ch, N, G, dtype)
+
+
+@pytest.mark.parametrize("S", [1, 9, 150])
+@pytest.mark.parametrize("ch,N,G", [v[:3] for v in VECTORS])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_vector_rows_of_many_modes_tokens(S, ch, N, G, dtype):
+    base.test_single_tokens(S, ch, N, G, 4, dtype)
+
+
+DIFF = ("x", "w", "b", "dt", "A", "B", "C", "D", "z", "dt_bias")
+
+
+def _difference_problem():
+    g, rows, ch, N = gen(11), 24, 40, 16
+    t = _scan_problem(rows, ch, N, 2, g, torch.float32)
+    t |= {"w": randn((ch, 4), g).float(), "b": randn((ch,), g).float()}
+    return t, randn((rows, ch), g).float(), [0, 7, 7, 20]
+
+
+def _allowed(slope, y, weight, h):
+    """Difference against slope: (8 len + 64) 2^-24 of the outputs' terms, 4 for sums that cancel, over the
+    step; and the third derivative. A direction of size 0.3 in every step and rate moves the
+    logarithm of 13 poles' product by at most 13 x 0.3 = 4, so it is at most 4^3 / 6 of the slope's terms
+    in h^2; the products with the other operands double it a few times: 64."""
+    return (8 * 13 + 64) * 2.0 ** -24 / h * 4 * (y.abs() * weight.abs()).sum() + 64 * h * h * slope
+
+
+@pytest.mark.parametrize("name", DIFF)
+def test_each_gradient_against_differences(name):
+    """The operators' own outputs moved along the sign of one operand's gradient, where the slope is the sum
+    of its absolute values: without the gradient, or with a quarter of it wrong, the test fails."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, short_conv
+
+    t, weight, cu = _difference_problem()
+    t, weight, cud = {k: u.to(cuda()) for k, u in t.items()}, weight.to(cuda()), torch.tensor(cu, dtype=torch.int32, device=cuda())
+
+    def value(v):
+        u = short_conv(v["x"], v["w"], v["b"], cu_seqlens=cud)
+        return selective_state_scan(u, v["dt"], v["A"], v["B"], v["C"], v["D"], v["z"], v["dt_bias"], cu_seqlens=cud)
+
+    leaf = t[name].clone().requires_grad_()
+    (grad,) = torch.autograd.grad(value(dict(t, **{name: leaf})), leaf, weight)
+    move, h = 0.3 * grad.sign(), 2.0 ** -7
+    slope = (grad.double() * move.double()).sum()
+    up, down = (value(dict(t, **{name: t[name] + s * h * move})).double() for s in (1, -1))
+    tol = _allowed(slope, up, weight, h)
+    assert tol < 0.25 * slope
+    assert (((up - down) * weight).sum() / (2 * h) - slope).abs() <= tol
+
+
+def test_pieces_hold_the_precision_of_one_pass():
+    """One sequence of 500 rows, cut into pieces both ways, against 64 bits in the 2-norm. Steps of 0.13
+    and rates of 1 keep a state for about 10 steps: 10 roundings of the state, 4 eps of each pole,
+    the same again in the adjoint, in the 2-norm below 32 eps; a piece that starts from a wrong
+    state is off by hundredths."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan
+
+    g, L, ch, N = gen(29), 500, 96, 16
+    t = _scan_problem(L, ch, N, 1, g, torch.float32)
+    dy = randn((L, ch), g).float()
+    names = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")
+    v = {k: (u[None] if k in ("x", "dt", "B", "C", "z") else u).to(cuda()).requires_grad_() for k, u in t.items()}
+    y = selective_state_scan(*[v[k] for k in names[:5]], D=v["D"], z=v["z"], dt_bias=v["dt_bias"])
+    grads = torch.autograd.grad(y, [v[k] for k in names], dy[None].to(cuda()))
+    d = {k: u.double() for k, u in t.items()}
+    out = oss.scan(d["x"], d["dt"], d["A"], d["B"], d["C"], [0, L], d["D"], d["z"], d["dt_bias"], dy=dy.double())
+    for name, got in zip(("y",) + tuple("d" + k for k in names), (y,) + grads):
+        want = out[name]
+        off = (got.detach().double().cpu().reshape(want.shape) - want).norm() / want.norm()
+        assert off <= 32 * 2.0 ** -24, (name, off)
+
+
+@pytest.mark.parametrize("width,groups", [(64, 1), (128, 2)])
+def test_block_with_vector_rows(width, groups):
+    """The block as a whole where the projections' rows allow four elements at a time (dt_rank 4 and 8), with
+    every gradient; 1e-4 of the largest value as for the other block tests."""
+    from semambaxlinoss_b200.mamba_block import create_block
+
+    torch.manual_seed(width)
+    cfg = {"ssm": "selective_state", "d_state": 16, "d_conv": 4, "expand": 2, "ssm_params": {"n_groups": groups}}
+    block = create_block(width, cfg, rms_norm=False, fused_add_norm=True)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.add_(torch.randn(p.shape) * 0.05)
+    block, rank, GN = block.to(cuda()), width // 16, groups * 16
+    g, cu = gen(width), [2, 19, 20, 60]
+    x, r, dy, ds = (randn((61, width), g).float() for _ in range(4))
+    p = {k: u.detach().double().cpu().requires_grad_() for k, u in block.named_parameters()}
+    x64, r64 = x.double().requires_grad_(), r.double().requires_grad_()
+    s64 = x64 + r64
+    xz = torch.nn.functional.layer_norm(s64, (width,), p["norm.weight"], p["norm.bias"]) @ p["mixer.in_proj.weight"].t()
+    u, z = xz.chunk(2, -1)
+    u = oss.conv(u, p["mixer.conv1d.weight"][:, 0], p["mixer.conv1d.bias"], cu)["y"]
+    rows = u @ p["mixer.x_proj.weight"].t()
+    B, C = (rows[:, rank + i * GN:rank + (i + 1) * GN].unflatten(-1, (groups, 16)) for i in range(2))
+    y64 = oss.scan(u, rows[:, :rank] @ p["mixer.dt_proj.weight"].t(), -torch.exp(p["mixer.A_log"]), B, C, cu, p["mixer.D"], z,
+                   p["mixer.dt_proj.bias"])["y"] @ p["mixer.out_proj.weight"].t()
+    want = torch.autograd.grad((y64 * dy).sum() + (s64 * ds).sum(), [x64, r64] + list(p.values()))
+    xd, rd = x.to(cuda()).requires_grad_(), r.to(cuda()).requires_grad_()
+    y, s = block(xd, rd, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=cuda()))
+    got = torch.autograd.grad((y, s), [xd, rd] + list(block.parameters()), (dy.to(cuda()), ds.to(cuda())))
+    for name, a, b in zip(["y", "s", "x", "r"] + list(p), (y, s) + got, (y64, s64) + want):
+        err = (a.detach().double().cpu() - b.detach()).abs().max() / b.detach().abs().max()
+        assert err <= 1e-4, (name, err)
