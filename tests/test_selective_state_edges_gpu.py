@@ -260,3 +260,115 @@ def test_block_with_vector_rows(width, groups):
     for name, a, b in zip(["y", "s", "x", "r"] + list(p), (y, s) + got, (y64, s64) + want):
         err = (a.detach().double().cpu() - b.detach()).abs().max() / b.detach().abs().max()
         assert err <= 1e-4, (name, err)
+
+
+@pytest.mark.parametrize("ch,N,G", [(64, 16, 1), (33, 5, 3)])
+def test_fp32_steps_beside_bf16_rows(ch, N, G):
+    """Prompts and single tokens whose step projection stayed in fp32."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, selective_state_step
+
+    S, L, g = 5, 9, gen(ch)
+    t = _scan_problem(S * L, ch, N, G, g, torch.bfloat16, torch.float32)
+    start, cu = randn((S, ch, N), g).float(), [L * s for s in range(S + 1)]
+    v = {k: (u.view((S, L) + u.shape[1:]) if k in ("x", "dt", "B", "C", "z") else u).to(cuda()) for k, u in t.items()}
+    d = {k: u.double() for k, u in t.items()}
+    state = start.to(cuda())
+    y = selective_state_scan(*[v[k] for k in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")], state=state)
+    args = (d["x"], d["dt"], d["A"], d["B"], d["C"], cu, d["D"], d["z"], d["dt_bias"])
+    h0 = [u.double() for u in start]
+    out, size = oss.scan(*args, h0=h0), oss.scan(*args, h0=h0, absolute=True)
+    _near(y, out["y"], size["y"], 8 * L + 64, torch.bfloat16, "y")
+    _near(state, torch.stack(out["h"]), torch.stack(size["h"]), 8 * L + 64, torch.float32, "state")
+    one = {k: u[:, 0] if k in ("x", "dt", "B", "C", "z") else u for k, u in v.items()}  # rows at L times the stride
+    state = start.to(cuda())
+    y = selective_state_step(*[one[k] for k in ("x", "dt", "A", "B", "C")], state, one["D"], one["z"], one["dt_bias"])
+    first = {k: u[::L] if k in ("x", "dt", "B", "C", "z") else u for k, u in d.items()}
+    args = (first["x"], first["dt"], first["A"], first["B"], first["C"], list(range(S + 1)), first["D"], first["z"], first["dt_bias"])
+    out, size = oss.scan(*args, h0=h0), oss.scan(*args, h0=h0, absolute=True)
+    _near(y, out["y"], size["y"], 72, torch.bfloat16, "token")
+    _near(state, torch.stack(out["h"]), torch.stack(size["h"]), 72, torch.float32, "token state")
+
+
+def test_slots_named_again_far_behind():
+    """Two sequences of one slot that different CTAs run: the first has it, the later ones are refused."""
+    S, dev = 700, cuda()
+    again = {350: 3, 699: 3, 698: 697, 17: 16}
+    for name, call, shape in base._ops(S):
+        pool = torch.randn((S,) + shape, device=dev)
+        good = torch.arange(S, dtype=torch.int32, device=dev)
+        bad = good.clone()
+        for s, other in again.items():
+            bad[s] = other
+        p0, p1 = pool.clone(), pool.clone()
+        want, got = call(p0, good), call(p1, bad)
+        for s in range(S):
+            p0[s] = pool[s] if s in again else p0[s]
+        refused = torch.tensor([s in again for s in range(S)], device=dev)
+        assert torch.isnan(got[refused]).all() and torch.equal(got[~refused], want[~refused]), name
+        assert torch.equal(p0, p1), name
+
+
+def test_no_steps_and_inference_mode():
+    from semambaxlinoss_b200.selective_state import selective_state_scan, short_conv
+
+    dev, ch, N = cuda(), 16, 4
+    x, B = torch.empty(3, 0, ch, device=dev, requires_grad=True), torch.empty(3, 0, N, device=dev)
+    A, w = (-torch.rand(ch, N, device=dev)).requires_grad_(), torch.rand(ch, 4, device=dev, requires_grad=True)
+    y = selective_state_scan(short_conv(x, w), x, A, B, B, z=x)
+    assert y.shape == x.shape
+    dx, dA, dw = torch.autograd.grad(y, (x, A, w), torch.empty_like(y))
+    assert dx.shape == x.shape and not dA.any() and not dw.any()
+    state = torch.ones(3, ch, N, device=dev)
+    with torch.no_grad():
+        selective_state_scan(x, x, A, B, B, state=state, fresh=torch.tensor([True, False, True], device=dev))
+    assert not state[[0, 2]].any() and bool((state[1] == 1).all())
+    x, B = torch.randn(2, 9, ch, device=dev), torch.randn(2, 9, N, device=dev)
+    with torch.no_grad():
+        want = selective_state_scan(short_conv(x, w), x, A, B, B)
+    with torch.inference_mode():
+        assert torch.equal(selective_state_scan(short_conv(x, w), x, A, B, B), want)
+
+
+def test_a_captured_prompt_takes_other_offsets():
+    """A packed prompt captured once and replayed with other offsets, slots and fresh flags (a long sequence
+    where short ones were, rows in front of the first): what plain calls give, bit for bit."""
+    from semambaxlinoss_b200.selective_state import selective_state_scan, short_conv
+
+    g, rows, S, ch, N, dev = gen(31), 700, 6, 72, 16, cuda()
+    t = {k: u.to(dev) for k, u in _scan_problem(rows, ch, N, 1, g, torch.bfloat16).items()}
+    w = torch.randn(ch, 4, device=dev)
+    plans = [([0, 5, 9, 9, 30, 600, 690], [3, 0, 7, 1, 2, 5], [1, 0, 1, 0, 0, 1]),
+             ([4, 650, 651, 652, 652, 652, 655], [7, 6, 5, 4, -1, 0], [0, 0, 0, 0, 1, 1]),
+             ([0, 100, 200, 300, 400, 500, 700], [0, 1, 2, 2, 4, 9], [0] * 6)]
+    cu, slots = (torch.zeros(n, dtype=torch.int32, device=dev) for n in (S + 1, S))
+    fresh = torch.zeros(S, dtype=torch.bool, device=dev)
+    window, state = torch.randn(8, 3, ch, device=dev).bfloat16(), torch.randn(8, ch, N, device=dev)
+
+    def prompt(window, state):
+        u = short_conv(t["x"], w, cu_seqlens=cu, state=window, slots=slots, fresh=fresh)
+        return selective_state_scan(u, *[t[k] for k in ("dt", "A", "B", "C", "D", "z", "dt_bias")], cu_seqlens=cu,
+                                    state=state, slots=slots, fresh=fresh)
+
+    def plan(i):
+        for buf, values in zip((cu, slots, fresh), plans[i]):
+            buf.copy_(torch.tensor(values).to(buf.dtype))
+
+    plan(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        prompt(window.clone(), state.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    kept = window.clone(), state.clone()
+    with torch.cuda.graph(graph):
+        y = prompt(window, state)
+    window.copy_(kept[0]), state.copy_(kept[1])
+    for i in (0, 1, 2, 0):
+        plan(i)
+        w2, s2 = window.clone(), state.clone()
+        graph.replay()
+        want = prompt(w2, s2)
+        assert torch.equal(torch.nan_to_num(y, 77.0), torch.nan_to_num(want, 77.0))
+        assert torch.isnan(y).any() == (i == 2)
+        assert torch.equal(window, w2) and torch.equal(state, s2)
