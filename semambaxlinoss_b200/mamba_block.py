@@ -14,7 +14,7 @@ checkout. Their documented behaviour is restated here:
   residual.
 * ``create_block(rms_norm=False, fused_add_norm=True)`` takes this package's ``LayerNorm``
   (an nn.LayerNorm), whose kernel adds the residual and normalises in one pass; tensors that
-  the kernel does not take (CPU, other types, wider rows) run as nn.LayerNorm behind an addition.
+  the kernel does not take (CPU, other types, rows above 8192 elements) run as nn.LayerNorm behind an addition.
 * ``_init_weights(module, n_layer)``: zero every Linear bias not tagged ``_no_reinit``;
   re-draw every ``out_proj.weight`` / ``fc2.weight`` Kaiming-uniform (a = sqrt(5)) and
   divide it by sqrt(n_layer).
