@@ -26,11 +26,11 @@ BLOCK_WIDTH = 8192
 
 
 def _forward(x, weight, bias, eps, residual, out_dtype, stats):
-    """Runs the forward; returns (y, s, kept): kept (2, rows) holds mean and 1 / sqrt(var + eps)
+    """Runs the forward; returns (y, s, kept): kept (2 rows) holds mean and 1 / sqrt(var + eps)
     where ``stats``, else None."""
     d = x.shape[-1]
     x = x.contiguous()
-    y = x.new_empty(x.shape, dtype=out_dtype)
+    y = torch.empty_like(x, dtype=out_dtype)
     a = _lib.new_args(_lib.SemxLayerNormArgs)
     a.eps, a.n, a.d = eps, x.numel() // d, d
     a.x_bf16, a.y_bf16 = x.dtype == torch.bfloat16, out_dtype == torch.bfloat16
@@ -38,7 +38,7 @@ def _forward(x, weight, bias, eps, residual, out_dtype, stats):
     s = x
     if residual is not None:
         residual = residual.contiguous()
-        s = x.new_empty(x.shape, dtype=residual.dtype if x.dtype == torch.bfloat16 else x.dtype)
+        s = torch.empty_like(residual if x.dtype == torch.bfloat16 else x)  # the wider type
         a.r_bf16, a.s_bf16 = residual.dtype == torch.bfloat16, s.dtype == torch.bfloat16
         a.residual, a.sum = residual.data_ptr(), s.data_ptr()
     if weight is not None:
@@ -47,7 +47,7 @@ def _forward(x, weight, bias, eps, residual, out_dtype, stats):
         a.bias = bias.data_ptr()
     kept = None
     if stats:
-        kept = x.new_empty((2, x.numel() // d), dtype=torch.float32)
+        kept = x.new_empty(2 * a.n, dtype=torch.float32)
         at = kept.data_ptr()
         a.mean, a.rstd = at, at + 4 * a.n
     _lib.call("semx_layer_norm_fwd", a, x.device)
@@ -66,7 +66,7 @@ class _LayerNorm(torch.autograd.Function):
         return y if residual is None else (y, s)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy, dsum=None):
         s, w, kept = ctx.saved_tensors
         eps, ydt, xdt, rdt, wdt, bdt = ctx.cfg
@@ -76,9 +76,9 @@ class _LayerNorm(torch.autograd.Function):
         d = shape[-1]
         dy = s.new_zeros(shape, dtype=ydt) if dy is None else _lib.as_rows(dy, ydt)
         dsum = None if dsum is None else _lib.as_rows(dsum, s.dtype)
-        dx = s.new_empty(shape, dtype=xdt)
+        dx = torch.empty_like(s, dtype=xdt)
         a = _lib.new_args(_lib.SemxLayerNormArgs)
-        a.eps, a.n, a.d = eps, kept.shape[1], d
+        a.eps, a.n, a.d = eps, kept.shape[0] // 2, d
         a.x_bf16, a.y_bf16, a.s_bf16 = xdt == torch.bfloat16, ydt == torch.bfloat16, s.dtype == torch.bfloat16
         at = kept.data_ptr()
         a.sum, a.mean, a.rstd, a.weight = s.data_ptr(), at, at + 4 * a.n, _lib.ptr(w)
@@ -86,7 +86,7 @@ class _LayerNorm(torch.autograd.Function):
         need = ctx.needs_input_grad
         dr = dx if rdt == xdt else None
         if rdt is not None and need[4] and dr is None:
-            dr = s.new_empty(shape, dtype=rdt)
+            dr = torch.empty_like(s, dtype=rdt)
             a.r_bf16, a.dresidual = rdt == torch.bfloat16, dr.data_ptr()
         dw = s.new_empty(d, dtype=torch.float32) if wdt is not None and need[1] else None
         db = s.new_empty(d, dtype=torch.float32) if bdt is not None and need[2] else None

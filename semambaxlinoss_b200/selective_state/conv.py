@@ -54,7 +54,7 @@ class _ShortConv(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy):
         x, w, b, cu = ctx.saved_tensors
         silu, S, rows, L, wdt, bdt = ctx.cfg

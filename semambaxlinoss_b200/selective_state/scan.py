@@ -106,7 +106,7 @@ class _StateScan(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy):
         x, dt, A, B, C, D, z, bias, v, ckpt, cu = ctx.saved_tensors
         softplus, S, rows, L, N, G, Bshape, (Adt, Ddt, bdt) = ctx.cfg
