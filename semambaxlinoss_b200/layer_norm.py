@@ -124,7 +124,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor 
                                  or residual.dtype not in _TYPES):
         raise ValueError(f"layer_norm: residual must be fp32 or bf16 {tuple(x.shape)} on {x.device}, got "
                          f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
-    _lib.refuse_tangents("layer_norm", x, weight, bias, residual)
+    if _lib.in_dual_level():
+        _lib.refuse_tangents("layer_norm", x, weight, bias, residual)
     eps = float(eps)
     if torch.is_grad_enabled() and (
             x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)

@@ -102,7 +102,8 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 def _run(op, x, weight, bias, activation, S, rows, L, cu_seqlens, state, slots, fresh):
     silu = _silu_flag(op, activation)
-    _lib.refuse_tangents(op, x, weight, bias, state)
+    if _lib.in_dual_level():
+        _lib.refuse_tangents(op, x, weight, bias, state)
     C, dev = x.shape[-1], x.get_device()
     w = _weight(op, weight, C)
     if w.dtype not in TYPES or w.get_device() != dev:

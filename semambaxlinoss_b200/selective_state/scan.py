@@ -150,7 +150,8 @@ def selective_state_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     while a gradient is wanted."""
     op = "selective_state_scan"
     S, rows, L = batch(op, x, cu_seqlens)
-    _lib.refuse_tangents(op, x, dt, A, B, C, D, z, dt_bias, state)
+    if _lib.in_dual_level():
+        _lib.refuse_tangents(op, x, dt, A, B, C, D, z, dt_bias, state)
     ch, N, G = _check(op, x, dt, A, B, C, D, z, dt_bias)
     softplus = int(bool(dt_softplus))
     if _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
@@ -186,7 +187,8 @@ def selective_state_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
         raise ValueError(f"{op}: x must be fp32 or bf16 (sequences, channels), got {x.dtype} {tuple(x.shape)}")
     if state is None:
         raise ValueError(f"{op}: a state is needed")
-    _lib.refuse_tangents(op, x, dt, A, B, C, state, D, z, dt_bias)
+    if _lib.in_dual_level():
+        _lib.refuse_tangents(op, x, dt, A, B, C, state, D, z, dt_bias)
     ch, N, G = _check(op, x, dt, A, B, C, D, z, dt_bias)
     if _grads_wanted(x, dt, A, B, C, D, z, dt_bias):
         raise ValueError(f"{op}: a state is for inference; the call wants gradients")
