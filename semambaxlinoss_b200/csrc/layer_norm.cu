@@ -184,7 +184,7 @@ constexpr int cta_threads() {
 }
 // CTAs per SM that the registers are cut for: what a launch puts there (ln_ctas) at most. Cut for eight
 // where four are launched, rows of 513 to 1024 elements spilled (64 M elements of 1024 fp32: forward 152
-// us, cut for four 134; backward 284 and 173).
+// us, cut for four 134; backward 293 and 173).
 template <int TPR, int V>
 constexpr int ctas_per_sm() {
   return TPR * V <= 256 ? 4 : TPR * V <= 1024 ? 1024 / (TPR * V) : 1;

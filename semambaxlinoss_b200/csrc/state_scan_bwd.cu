@@ -9,7 +9,7 @@
 //
 // Bound: instructions (24 per (step, channel, mode) of a warp, a quarter of them the exchanges
 // between lanes) and shared memory's path to the registers, at 59 % and 61 % of their rates in
-// 4 x 2047 x 2048 bf16 (307 us of 420 with its first pass and the join; profiles/selective_state_scan.md).
+// 4 x 2047 x 2048 bf16 (312 us of 425 with its first pass and the join; profiles/selective_state_scan.md).
 // The forward left the state in front of every kBlock steps; a block's states and poles are
 // rebuilt from it in registers, half a block at a time, and the adjoint runs back through
 // them: one and a half exponentials per (step, channel, mode).
@@ -67,7 +67,8 @@ __device__ __forceinline__ void halve_sum(float (&v)[NV], int lane) {
 // fp32 rows fetch x, v, z and the block's entry states for the next tile straight into shared
 // memory, every thread into slots of its own: in registers they leave room for two CTAs per SM
 // only (404 x 321 x 256 fp32: in registers 704 us, three CTAs that spill 752, this way 614).
-// bf16 rows take half of the registers (4 x 2047 x 2048: in registers 307 us, this way 312).
+// bf16 rows take half of the registers (4 x 2047 x 2048: in registers 307 us, this way 312, both
+// before v was fp32).
 template <int GM, bool LOCAL, int ACC>
 __host__ __device__ constexpr bool stages() {
   return !LOCAL && ACC == kFp32 && GM >= 4;
@@ -571,7 +572,8 @@ void set_tiles(ScanParams& p) {
 // Rows per piece (0: whole sequences): as in the forward, with three resident CTAs per SM and
 // about five waves (4 x 2047 x 2048: whole 590 us, one wave 475 us, five 408 us). One sequence
 // of 100 rows and 256 channels, training pass: whole 56.5 us, in pieces 45.9; of 512 rows:
-// whole 177 us, pieces of at least 64 rows 63.3, of 32 rows 52.1.
+// whole 177 us, pieces of at least 64 rows 63.3, of 32 rows 52.1. The forward's exception holds here too, at
+// 64 rows a sequence (training pass of 63 sequences of 4 rows and one of 4000: 602 us; that one alone 102).
 constexpr int64_t kResident = 148 * 3;
 int64_t bwd_rows_per_piece(const ScanParams& p) {
   const int64_t ctas = (int64_t)p.m.S * p.ctiles;
