@@ -621,9 +621,9 @@ int semx_layer_norm_bwd(const SemxLayerNormArgs* args, semx_stream_t stream);
  * Sequences (both operators): S sequences of L rows (cu_seqlens NULL, rows = S L, row
  * s L + t), or `rows` packed rows with cu_seqlens (S + 1, int32, device): sequence s owns
  * rows [cu_seqlens[s], cu_seqlens[s+1]), lengths from 0; rows in front of cu_seqlens[0] and
- * from cu_seqlens[S] on belong to none: their outputs and gradients are zeros. L is ignored with cu_seqlens. The
- * offsets must not decrease; they are clamped, so that bad ones give wrong rows and no
- * access outside the rows.
+ * from cu_seqlens[S] on belong to none: their outputs and gradients are zeros. L is ignored
+ * with cu_seqlens. The offsets must not decrease; they are clamped, so that bad ones give
+ * wrong rows and no access outside the rows.
  * State: a pool of n_slots entries, updated in place; sequence s has entry slots[s] (int32,
  * device; NULL: entry s). A negative slot: the sequence starts from zeros and leaves
  * nothing. A slot >= n_slots, or one that an earlier sequence of the call has, is refused

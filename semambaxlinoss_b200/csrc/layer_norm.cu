@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(cta_threads<TPR>(), ctas_per_sm<TPR, V>()) lay
 
 // CTAs of a launch: one wave of what an SM holds, so that a CTA sees many rows, always has
 // the next one on its way and leaves one row of partial sums for all of them (8192 x 4096:
-// backward in two waves 127 us, one 110 us; forward 83 and 73 us).
+// backward in two waves 127 us, one 110 us, both before its partial sums left as whole lines, 104 since;
+// forward 83 and 73 us).
 int rows_per_cta(int64_t d) { return d <= 64 ? 16 : d <= 128 ? 8 : d <= 512 ? 4 : 1; }
 int64_t ln_ctas(int64_t n, int64_t d) {
   const int64_t want = semx::cdiv(n, rows_per_cta(d)), most = 148 * (d <= 2048 ? 4 : d <= 4096 ? 2 : 1);
