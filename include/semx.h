@@ -67,9 +67,10 @@ const char* semx_last_error(void);
  * threads and devices together (a monotonically increasing counter). No counterpart in
  * the reference; it lets a caller count the device launches of a region of its own. */
 uint64_t semx_launch_count(void);
-/* Number of tensor-core completion waits, on the current GPU, that ran out of time in this
- * process (the kernel then stops and leaves the rest of its outputs unwritten); 0 in a
- * healthy run. Synchronises with that GPU. No counterpart in the reference. */
+/* Number of tensor-core completion waits, and of waits of one tile of the gated recurrence on
+ * another, on the current GPU, that ran out of time in this process (the kernel then stops and
+ * leaves the rest of its outputs unwritten, or NaN in the recurrence); 0 in a healthy run.
+ * Synchronises with that GPU. No counterpart in the reference. */
 int semx_tc_timeouts(uint32_t* count);
 
 /* ------------------------------------------------------------------------------------
@@ -723,6 +724,61 @@ size_t semx_state_scan_workspace_bytes(const SemxStateScanArgs* args, int32_t ba
 int semx_state_scan_fwd(const SemxStateScanArgs* args, semx_stream_t stream);
 int semx_state_scan_bwd(const SemxStateScanArgs* args, semx_stream_t stream);
 int semx_state_step(const SemxStateScanArgs* args, semx_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Gated linear recurrence: one real mode per channel whose decay and input are gated per
+ * token. Sequences, state pool and row strides as in the section above; the state entry is
+ * (C) fp32.
+ *   rho = sigmoid(r + r_bias), iota = sigmoid(i + i_bias)
+ *   a = exp(-rate_scale softplus(rate) rho), gain = sqrt(max(1 - a^2, 1e-6))
+ *   h_t = a_t h_{t-1} + gain_t iota_t x_t (fp32);   y = h silu(z), or h without z
+ * x, r, i, z, y (and their gradients) are bf16 when `bf16` is set, else fp32; rate, r_bias,
+ * i_bias (the last two may be NULL: 0) and their gradients fp32. rate_scale > 0.
+ * semx_gated_lru_*: whole sequences. A training forward passes ckpt
+ * (semx_gated_lru_ckpt_bytes()); the backward reads it and writes dx, d_r, d_i, dz (with z),
+ * and drate, dr_bias, di_bias (each may be NULL), reduced in a fixed order. Where 1 - a^2 is
+ * at its least value no gradient goes through the gain. Workspace (8-byte aligned, of this
+ * call alone): semx_gated_lru_workspace_bytes() with `backward` 0 or 1 (0 bytes where none is
+ * needed).
+ * semx_gated_lru_step: one row per sequence (cu_seqlens NULL, L = 1), state required, no
+ * fresh flags. */
+typedef struct SemxGatedLruArgs {
+  uint32_t struct_size;
+  int32_t bf16;
+  float rate_scale;
+  int32_t reserved;
+  int64_t S, rows, L, C, n_slots;
+  int64_t ldx, ldr, ldi, ldz;
+  const void* x;
+  const void* r;
+  const void* i;
+  const void* z;
+  const float* rate;
+  const float* r_bias;
+  const float* i_bias;
+  void* y;
+  const int32_t* cu_seqlens;
+  float* state;
+  const int32_t* slots;
+  const uint8_t* fresh;
+  float* ckpt;
+  const void* dy;
+  void* dx;
+  void* d_r;
+  void* d_i;
+  void* dz;
+  float* drate;
+  float* dr_bias;
+  float* di_bias;
+  void* workspace;
+} SemxGatedLruArgs;
+
+size_t semx_gated_lru_args_size(void);
+size_t semx_gated_lru_ckpt_bytes(const SemxGatedLruArgs* args);
+size_t semx_gated_lru_workspace_bytes(const SemxGatedLruArgs* args, int32_t backward);
+int semx_gated_lru_fwd(const SemxGatedLruArgs* args, semx_stream_t stream);
+int semx_gated_lru_bwd(const SemxGatedLruArgs* args, semx_stream_t stream);
+int semx_gated_lru_step(const SemxGatedLruArgs* args, semx_stream_t stream);
 
 size_t semx_mimo_layer_args_size(void);
 size_t semx_mimo_layer_ckpt_bytes(const SemxMimoLayerArgs* args);

@@ -275,6 +275,18 @@ class SemxStateScanArgs(ctypes.Structure):
             "ckpt", "dy", "dx", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "workspace")]
 
 
+class SemxGatedLruArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("bf16", ctypes.c_int32),
+        ("rate_scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ] + [(name, ctypes.c_int64) for name in ("S", "rows", "L", "C", "n_slots", "ldx", "ldr", "ldi", "ldz")] + [
+        (name, ctypes.c_void_p) for name in (
+            "x", "r", "i", "z", "rate", "r_bias", "i_bias", "y", "cu_seqlens", "state", "slots", "fresh", "ckpt",
+            "dy", "dx", "d_r", "d_i", "dz", "drate", "dr_bias", "di_bias", "workspace")]
+
+
 # (python struct, C size query) for every argument struct in semx.h.
 STRUCTS = {
     "SemxLinossArgs": (SemxLinossArgs, "semx_linoss_args_size"),
@@ -290,6 +302,7 @@ STRUCTS = {
     "SemxLayerNormArgs": (SemxLayerNormArgs, "semx_layer_norm_args_size"),
     "SemxShortConvArgs": (SemxShortConvArgs, "semx_short_conv_args_size"),
     "SemxStateScanArgs": (SemxStateScanArgs, "semx_state_scan_args_size"),
+    "SemxGatedLruArgs": (SemxGatedLruArgs, "semx_gated_lru_args_size"),
 }
 
 # Every symbol semx.h declares, with its ctypes signature.
@@ -358,6 +371,12 @@ _SIGNATURES = {
     "semx_state_scan_fwd": (ctypes.c_int, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_void_p]),
     "semx_state_scan_bwd": (ctypes.c_int, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_void_p]),
     "semx_state_step": (ctypes.c_int, [ctypes.POINTER(SemxStateScanArgs), ctypes.c_void_p]),
+    "semx_gated_lru_args_size": (ctypes.c_size_t, []),
+    "semx_gated_lru_ckpt_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxGatedLruArgs)]),
+    "semx_gated_lru_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_int32]),
+    "semx_gated_lru_fwd": (ctypes.c_int, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_void_p]),
+    "semx_gated_lru_bwd": (ctypes.c_int, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_void_p]),
+    "semx_gated_lru_step": (ctypes.c_int, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_void_p]),
     "semx_mimo_layer_args_size": (ctypes.c_size_t, []),
     "semx_mimo_layer_ckpt_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),
     "semx_mimo_layer_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),

@@ -2455,7 +2455,10 @@ int semx_tc_timeouts(uint32_t* count) {
   unsigned int v = 0;
   const cudaError_t e = cudaMemcpyFromSymbol(&v, g_tc_timeouts, sizeof(v));
   if (e != cudaSuccess) return semx::fail(SEMX_ERR_LAUNCH, "semx_tc_timeouts: %s", cudaGetErrorString(e));
-  *count = v;
+  uint32_t links = 0;
+  const int rc = semx::link_timeouts(&links);
+  if (rc != SEMX_OK) return rc;
+  *count = v + links;
   return SEMX_OK;
 }
 

@@ -45,6 +45,10 @@ class DeviceScope {
   int prev_ = -1;
 };
 
+// Waits of the gated recurrence's tiles on one another that gave up, on the current device
+// (a part of semx_tc_timeouts()).
+int link_timeouts(uint32_t* count);
+
 inline bool aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;
 }

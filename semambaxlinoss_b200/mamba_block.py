@@ -29,9 +29,10 @@ place. A scan layer that cannot read a layout (the MIMO layer; a streamed
 SelectiveLRU for strided layouts) falls back to the reference's copies.
 
 Supported mixers: ``selective_lru``, ``selective_lru_mimo``, ``linoss`` (the layers on
-this package's scan path), and ``selective_state`` (the Mamba layer's formulas with packed
-sequences, prompts and single tokens; ``ssm_params``: the mixer's own keyword arguments;
-``cu_seqlens``, ``cache``, ``slots`` and ``fresh`` pass through ``Block.forward``). The
+this package's scan path), ``selective_state`` (the Mamba layer's formulas) and ``gated_lru``
+(one gated real mode per channel). The last two take packed sequences, prompts and single
+tokens (``ssm_params``: the mixer's own keyword arguments; ``cu_seqlens``, ``cache``, ``slots``
+and ``fresh`` pass through ``Block.forward``). The
 reference's other backbones (``mamba``, ``mamba2``, ``mamba3`` from mamba_ssm, ``s4d``,
 ``s5``, and ``selective_linoss``, whose source the reference does not contain) raise
 NotImplementedError.
@@ -47,6 +48,7 @@ from torch import nn
 import torch.nn.functional as F
 
 from . import _lib
+from .gated_lru import GatedLruMixer
 from .layer_norm import LayerNorm
 from .layout import TokenLayout
 from .linoss import LinOSS
@@ -233,6 +235,10 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
         if not causal:
             raise ValueError("the selective_state mixer's convolution is causal; causal_conv must be True")
         return partial(SelectiveStateMixer, d_state=d_state, d_conv=d_conv, expand=expand, **ssm_params)
+    if ssm == "gated_lru":
+        if not causal:
+            raise ValueError("the gated_lru mixer's convolution is causal; causal_conv must be True")
+        return partial(GatedLruMixer, d_conv=d_conv, expand=expand, **ssm_params)
     if ssm == "linoss":
         layer = LinOSS(
             in_features=expand * d_model,
@@ -267,13 +273,13 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
     elif ssm in _OUT_OF_SCOPE:
         raise NotImplementedError(
             f"mixer {ssm!r} is not part of this package (only the selective-LRU and LinOSS "
-            "scan layers and the selective state mixer are)"
+            "scan layers and the selective state and gated recurrence mixers are)"
             + ("; 'selective_state' has that layer's formulas and parameter names" if ssm == "mamba" else "")
         )
     else:
         raise ValueError(
             f"Unknown mixer {ssm!r}; expected 'mamba', 'mamba2', 'mamba3', "
-            "'linoss', 'selective_lru', 'selective_lru_mimo', 'selective_state', 's4d', or 's5'."
+            "'linoss', 'selective_lru', 'selective_lru_mimo', 'selective_state', 'gated_lru', 's4d', or 's5'."
         )
     return partial(MambaStyleMixer, ssm=layer, expand=expand, d_conv=d_conv, causal_conv=causal)
 
