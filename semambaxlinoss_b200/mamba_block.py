@@ -273,7 +273,7 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
     elif ssm in _OUT_OF_SCOPE:
         raise NotImplementedError(
             f"mixer {ssm!r} is not part of this package (only the selective-LRU and LinOSS "
-            "scan layers and the selective state and gated recurrence mixers are)"
+            "scan layers, the selective state mixer and the gated recurrence mixer are)"
             + ("; 'selective_state' has that layer's formulas and parameter names" if ssm == "mamba" else "")
         )
     else:
