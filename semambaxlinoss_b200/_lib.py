@@ -287,6 +287,16 @@ class SemxGatedLruArgs(ctypes.Structure):
             "dy", "dx", "d_r", "d_i", "dz", "drate", "dr_bias", "di_bias", "workspace")]
 
 
+class SemxGatedLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("bf16", ctypes.c_int32),
+        ("act", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ] + [(name, ctypes.c_int64) for name in ("rows", "D", "H", "ldx")] + [
+        (name, ctypes.c_void_p) for name in ("x", "w", "bias", "h", "saved", "dh", "dx", "dw", "db", "workspace")]
+
+
 # (python struct, C size query) for every argument struct in semx.h.
 STRUCTS = {
     "SemxLinossArgs": (SemxLinossArgs, "semx_linoss_args_size"),
@@ -303,6 +313,7 @@ STRUCTS = {
     "SemxShortConvArgs": (SemxShortConvArgs, "semx_short_conv_args_size"),
     "SemxStateScanArgs": (SemxStateScanArgs, "semx_state_scan_args_size"),
     "SemxGatedLruArgs": (SemxGatedLruArgs, "semx_gated_lru_args_size"),
+    "SemxGatedLinearArgs": (SemxGatedLinearArgs, "semx_gated_linear_args_size"),
 }
 
 # Every symbol semx.h declares, with its ctypes signature.
@@ -377,6 +388,11 @@ _SIGNATURES = {
     "semx_gated_lru_fwd": (ctypes.c_int, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_void_p]),
     "semx_gated_lru_bwd": (ctypes.c_int, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_void_p]),
     "semx_gated_lru_step": (ctypes.c_int, [ctypes.POINTER(SemxGatedLruArgs), ctypes.c_void_p]),
+    "semx_gated_linear_args_size": (ctypes.c_size_t, []),
+    "semx_gated_linear_saved_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxGatedLinearArgs)]),
+    "semx_gated_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxGatedLinearArgs), ctypes.c_int32]),
+    "semx_gated_linear_fwd": (ctypes.c_int, [ctypes.POINTER(SemxGatedLinearArgs), ctypes.c_void_p]),
+    "semx_gated_linear_bwd": (ctypes.c_int, [ctypes.POINTER(SemxGatedLinearArgs), ctypes.c_void_p]),
     "semx_mimo_layer_args_size": (ctypes.c_size_t, []),
     "semx_mimo_layer_ckpt_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),
     "semx_mimo_layer_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SemxMimoLayerArgs)]),

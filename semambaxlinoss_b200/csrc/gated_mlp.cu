@@ -1,0 +1,950 @@
+// Gated projection of a feed-forward block, forward and backward, for sm_100a.
+//
+//   [u | g] = x W^T + b  (W: H rows of the value, then H rows of the gate);  h = u act(g)
+//   du = dh act(g), dg = dh u act'(g);  dx = du Wu + dg Wg,  dW = [du | dg]^T x,  db = column sums
+//
+// Forward: one kernel does both products, the activation and the last product. A tile is 128 rows of
+// x by the same columns of u and g side by side in one accumulator, so the epilogue has both.
+// Backward: an elementwise pass makes du and dg from what the forward kept (u and g in fp32: rounded
+// to bf16 they would put their rounding into dx and dW on top of that of du and dg), then two
+// products run on the same kernel with other operand orders.
+//
+// Products: tcgen05 (one CTA per SM, persistent; one warp loads tiles by TMA, one issues the
+// products into tensor memory, four write the accumulators out; two accumulators, so that writing
+// a tile overlaps the next one's products). fp32 operands are split into three bf16 parts whose sum
+// is the value up to its last bit; six of the nine products of parts (all above 2^-24 of the
+// result) run one behind the other into the same accumulator.
+// Few rows (up to 8): the weights' bytes are the bound, and a warp per pair of columns streams them.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <atomic>
+
+#include "semx_reduce.cuh"
+#include "semx_tc.cuh"
+#include "state_scan.cuh"
+
+namespace {
+
+using semx::cdiv;
+using semx_scan::sigmoid;
+
+constexpr int kM = 128, kK = 64;  // rows of a tile, depth of a stage (128 bytes of bf16)
+constexpr int kGemmT = 192;       // warps 0 to 3 write out, 4 loads, 5 issues products
+constexpr int kSms = 148;
+constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
+constexpr int kBufRow = 36;       // floats of a row of a warp's 32 x 32 exchange buffer
+constexpr int kParts = 3;         // bf16 parts of an fp32 value
+
+__device__ unsigned int g_gemm_timeouts;
+
+enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
+
+// Parts of A and B in the order of their products, small ones first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
+__device__ __forceinline__ int part_a(int pair) { return (0x001102 >> (4 * pair)) & 0xf; }
+__device__ __forceinline__ int part_b(int pair) { return (0x010120 >> (4 * pair)) & 0xf; }
+
+struct GemmParams {
+  int64_t M, N;           // rows and columns of the result (kFwd: N = H; kDw: M = H, once per half)
+  int tiles_m, tiles_n;   // kDw: tiles_m of one half
+  int tiles;              // in all
+  int kper, khalf;        // stages of one pair of parts, and of one half of them (kDx: u, then g)
+  int pairs, splits;      // products of parts; slices of the depth
+  void* out;              // kFwd: h
+  int64_t ldo;
+  int out_bf16;
+  float* u;               // kFwd: u and g in front of the activation, or NULL
+  float* g;
+  int64_t ldu;
+  const float* bias;      // (2 H) or NULL
+  int gelu;
+  float* part;            // with splits: (splits, result) sums, kFwd: (splits, 2, M, N)
+};
+
+__device__ __forceinline__ float act_of(float g, int gelu) {
+  return gelu ? g * (0.5f * erfcf(g * -0.70710678118654752f)) : g * sigmoid(g);
+}
+__device__ __forceinline__ float act_slope(float g, int gelu) {
+  if (gelu) {
+    const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
+    return fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), cdf);
+  }
+  const float s = sigmoid(g);
+  return s * fmaf(g, 1.f - s, 1.f);
+}
+
+// -- tensor core plumbing -----------------------------------------------------------------------
+
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          semx::tc::smem_addr(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(semx::tc::smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(semx::tc::smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(semx::tc::smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// Descriptor of an operand in 128-byte rows with the 128-byte swizzle. K-major: a row is 64 values of
+// the depth, 8-row groups 1024 bytes apart. MN-major: a row is 64 neighbouring M or N values at one
+// depth, 8-row groups 1024 bytes apart, the next 64 values 64 rows (8192 bytes) on.
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  const uint64_t lead = MN ? 8192 >> 4 : 1;
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (lead << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+constexpr uint32_t idesc_bf16(int M, int N, bool a_mn, bool b_mn) {
+  return (1u << 4)                    // fp32 accumulator
+         | (1u << 7) | (1u << 10)     // bf16 A and B
+         | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// Waits for a phase of bar, some two seconds at most.
+__device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  if (semx::tc::mbar_wait(bar, parity, 16)) return true;
+  const long long from = clock64();
+  do {
+    if (semx::tc::mbar_wait(bar, parity, 64)) return true;
+    if (dead != nullptr && *dead) return false;
+  } while (clock64() - from < kPatience);
+  return false;
+}
+// The same; false when it gave up or another role has.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  if (wait_some(bar, parity, dead)) return true;
+  if (*dead) return false;
+  if (atomicExch((int*)dead, 1) == 0) atomicAdd(&g_gemm_timeouts, 1u);
+  return false;
+}
+
+constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
+constexpr int stage_bytes(int bn) { return (kM + bn) * kK * 2; }
+constexpr size_t gemm_smem(int bn) {
+  return 1024 + (size_t)stages_of(bn) * stage_bytes(bn) + 4 * 32 * kBufRow * sizeof(float);
+}
+
+struct Tile {
+  int m, n, half, split;
+};
+__device__ __forceinline__ Tile tile_at(const GemmParams& p, int w) {
+  Tile t;
+  t.split = w % p.splits;
+  int i = w / p.splits;
+  t.half = 0;
+  const int per_half = p.tiles_m * p.tiles_n;
+  if (i >= per_half) {
+    t.half = 1;
+    i -= per_half;
+  }
+  // Eight tiles down, then one across: the operands of the tiles that run together stay in L2.
+  const int per = 8 * p.tiles_n, grp = i / per, r = i % per;
+  const int down = min(8, p.tiles_m - grp * 8);
+  t.m = grp * 8 + r % down;
+  t.n = r / down;
+  return t;
+}
+
+// 32 x 32 values, a lane's row each, to out[row0 ..][col0 ..] through the warp's buffer, so that a
+// row's values leave as whole sectors. rows, cols: how many of them exist.
+__device__ __forceinline__ void write_block(float* buf, const float (&v)[32], void* out, int64_t ld, int64_t row0, int64_t col0,
+                                            int rows, int cols, int bf16) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    *reinterpret_cast<float4*>(&buf[lane * kBufRow + i]) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  __syncwarp();
+  if (bf16) {
+    __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(out) + row0 * ld + col0;
+    if (cols >= 32 && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      const int c = lane % 4 * 8;
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + lane / 4;
+        const float4 a = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c]);
+        const float4 b = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c + 4]);
+        uint4 q;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+        h[0] = __floats2bfloat162_rn(a.x, a.y);
+        h[1] = __floats2bfloat162_rn(a.z, a.w);
+        h[2] = __floats2bfloat162_rn(b.x, b.y);
+        h[3] = __floats2bfloat162_rn(b.z, b.w);
+        if (r < rows) *reinterpret_cast<uint4*>(to + r * ld + c) = q;
+      }
+    } else {
+      for (int r = 0; r < rows; ++r)
+        if (lane < cols) to[r * ld + lane] = __float2bfloat16(buf[r * kBufRow + lane]);
+    }
+  } else {
+    float* to = reinterpret_cast<float*>(out) + row0 * ld + col0;
+    if (cols >= 32 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      const int c = lane % 8 * 4;
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int r = it * 4 + lane / 8;
+        const float4 a = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c]);
+        if (r < rows) *reinterpret_cast<float4*>(to + r * ld + c) = a;
+      }
+    } else {
+      for (int r = 0; r < rows; ++r)
+        if (lane < cols) to[r * ld + lane] = buf[r * kBufRow + lane];
+    }
+  }
+  __syncwarp();
+}
+
+// Result of one mode. BN: columns of the accumulator (kFwd: BN / 2 of u, then as many of g).
+template <int MODE, int BN>
+__global__ void __launch_bounds__(kGemmT, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                         const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
+  constexpr int ST = stages_of(BN), BYTES = stage_bytes(BN), ABYTES = kM * kK * 2;
+  constexpr bool A_MN = MODE == kDw, B_MN = MODE != kFwd;
+  constexpr int CN = MODE == kFwd ? BN / 2 : BN;  // columns of the result in a tile
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int dead;
+  uint8_t* stage0 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  float* bufs = reinterpret_cast<float*>(stage0 + ST * BYTES);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      semx::tc::mbar_init(&full[s], 1);
+      semx::tc::mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      semx::tc::mbar_init(&acc_full[b], 1);
+      semx::tc::mbar_init(&acc_empty[b], 4);
+    }
+    semx::tc::mbar_init(&drained, 1);
+    dead = 0;
+  }
+  if (warp == 0) semx::tc::tmem_alloc(&tmem_slot, 2 * BN);
+  semx::tc::fence_before_sync();
+  __syncthreads();
+  semx::tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int works = p.tiles * p.splits, depth = p.kper * p.pairs;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < works && ok; w += gridDim.x) {
+        const Tile t = tile_at(p, w);
+        const int k0 = (int)((int64_t)depth * t.split / p.splits), k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % ST;
+          ok = wait_phase(&empty[s], ((it / ST) & 1) ^ 1, &dead);
+          if (!ok) break;
+          expect_bytes(&full[s], BYTES);
+          uint8_t *sa = stage0 + s * BYTES, *sb = sa + ABYTES;
+          const int pair = k / p.kper, in = k % p.kper, kh = in / p.khalf, kk = (in % p.khalf) * kK;
+          const int pa = p.pairs > 1 ? part_a(pair) : 0, pb = p.pairs > 1 ? part_b(pair) : 0;
+          if (MODE == kDw) {
+            for (int b = 0; b < kM / 64; ++b) tma_load(sa + b * 8192, &map_a, t.m * kM + b * 64, kk, t.half, pa, &full[s]);
+            for (int b = 0; b < BN / 64; ++b) tma_load(sb + b * 8192, &map_b, t.n * BN + b * 64, kk, 0, pb, &full[s]);
+          } else if (MODE == kDx) {
+            tma_load(sa, &map_a, kk, t.m * kM, kh, pa, &full[s]);
+            for (int b = 0; b < BN / 64; ++b) tma_load(sb + b * 8192, &map_b, t.n * BN + b * 64, kk, kh, pb, &full[s]);
+          } else {
+            tma_load(sa, &map_a, kk, t.m * kM, 0, pa, &full[s]);
+            tma_load(sb, &map_b, kk, t.n * CN, 0, pb, &full[s]);
+            tma_load(sb + CN * 128, &map_b, kk, t.n * CN, 1, pb, &full[s]);
+          }
+        }
+      }
+      // After a wait that gave up: the copies on their way land before the CTA ends.
+      if (!ok)
+        for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) wait_some(&full[i % ST], (i / ST) & 1, nullptr);
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(kM, BN, A_MN, B_MN);
+      constexpr uint32_t a_step = (A_MN ? 2048 : 32), b_step = (B_MN ? 2048 : 32);  // 16 of the depth
+      uint32_t it = 0, acc = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < works && ok; w += gridDim.x, ++acc) {
+        const Tile t = tile_at(p, w);
+        const int k0 = (int)((int64_t)depth * t.split / p.splits), k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
+        const uint32_t b = acc & 1, d = tmem + b * BN;
+        ok = wait_phase(&acc_empty[b], ((acc >> 1) & 1) ^ 1, &dead);
+        if (!ok) break;
+        semx::tc::fence_after_sync();
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % ST;
+          ok = wait_phase(&full[s], (it / ST) & 1, &dead);
+          if (!ok) break;
+          semx::tc::fence_after_sync();
+          const uint32_t sa = semx::tc::smem_addr(stage0 + s * BYTES), sb = sa + ABYTES;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            mma_bf16(d, operand_desc<A_MN>(sa + q * a_step), operand_desc<B_MN>(sb + q * b_step), idesc, k > k0 || q > 0);
+          semx::tc::mma_commit(&empty[s]);
+        }
+        if (ok) semx::tc::mma_commit(&acc_full[b]);
+      }
+      if (!ok) {  // products on their way end before tensor memory is given back
+        semx::tc::mma_commit(&drained);
+        wait_some(&drained, 0, nullptr);
+      }
+    }
+  } else {
+    float* buf = bufs + warp * 32 * kBufRow;
+    const uint32_t lanes = (uint32_t)warp << 21;  // this warp's 32 lanes of tensor memory
+    uint32_t acc = 0;
+    for (int w = blockIdx.x; w < works; w += gridDim.x, ++acc) {
+      const Tile t = tile_at(p, w);
+      const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
+      const bool ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      semx::tc::fence_after_sync();
+      const int64_t row0 = (int64_t)t.m * kM + warp * 32;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
+#pragma unroll 1
+      for (int c = 0; c < CN; c += 32) {
+        const int64_t col0 = (int64_t)t.n * CN + c;
+        const int cols = (int)max((int64_t)0, min((int64_t)32, p.N - col0));
+        float v[32];
+        semx::tc::tmem_ld32(d + c, v);
+        if (MODE == kFwd) {
+          float g[32];
+          semx::tc::tmem_ld32(d + CN + c, g);
+          if (c + 32 >= CN) {
+            semx::tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(&acc_empty[b]);
+          }
+          if (p.splits > 1) {
+            float* to = p.part + (int64_t)t.split * 2 * p.M * p.N;
+            write_block(buf, v, to, p.N, row0, col0, rows, cols, 0);
+            write_block(buf, g, to + p.M * p.N, p.N, row0, col0, rows, cols, 0);
+            continue;
+          }
+          if (p.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < cols) {
+                v[i] += p.bias[col0 + i];
+                g[i] += p.bias[p.N + col0 + i];
+              }
+          }
+          if (p.u != nullptr) {
+            write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
+            write_block(buf, g, p.g, p.ldu, row0, col0, rows, cols, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= act_of(g[i], p.gelu);
+          write_block(buf, v, p.out, p.ldo, row0, col0, rows, cols, p.out_bf16);
+        } else {
+          if (c + 32 >= CN) {
+            semx::tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(&acc_empty[b]);
+          }
+          const int64_t half0 = (int64_t)t.half * p.M;
+          if (p.splits > 1) {
+            const int64_t all = (MODE == kDw ? 2 : 1) * p.M * p.N;
+            write_block(buf, v, p.part + t.split * all + half0 * p.N, p.N, row0, col0, rows, cols, 0);
+          } else {
+            write_block(buf, v, p.out, p.ldo, half0 + row0, col0, rows, cols, p.out_bf16);
+          }
+        }
+      }
+    }
+  }
+  semx::tc::fence_before_sync();
+  __syncthreads();
+  semx::tc::fence_after_sync();
+  if (warp == 0) semx::tc::tmem_dealloc(tmem, 2 * BN);
+}
+
+// Sums of the slices of the depth, in their order, and what the epilogue does with them.
+__global__ void __launch_bounds__(256) join_plain_kernel(const float* part, int splits, int64_t n, void* out, int bf16) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < splits; ++k) s += part[k * n + i];
+  semx_scan::store(out, i, bf16, s);
+}
+__global__ void __launch_bounds__(256) join_gated_kernel(const GemmParams p) {
+  const int64_t n = p.M * p.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t row = i / p.N, col = i % p.N;
+  float u = 0.f, g = 0.f;
+  for (int k = 0; k < p.splits; ++k) {
+    u += p.part[2 * k * n + i];
+    g += p.part[(2 * k + 1) * n + i];
+  }
+  if (p.bias != nullptr) {
+    u += p.bias[col];
+    g += p.bias[p.N + col];
+  }
+  if (p.u != nullptr) {
+    p.u[row * p.ldu + col] = u;
+    p.g[row * p.ldu + col] = g;
+  }
+  semx_scan::store(p.out, row * p.ldo + col, p.out_bf16, u * act_of(g, p.gelu));
+}
+
+// -- operands as the products read them -----------------------------------------------------------
+
+// Value n of the parts of v: v rounded to bf16, then what is left, each rounded. What no bf16 holds
+// (infinities, NaN) stays in the first; a value that would round to infinity is cut instead.
+__device__ __forceinline__ void parts_of(float v, __nv_bfloat16 (&part)[kParts]) {
+  part[0] = __float2bfloat16(v);
+  float rest = 0.f;
+  if (fabsf(v) <= 3.4028234663852886e38f) {
+    if (fabsf(v) >= 3.3961775292304608e38f) part[0] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16));
+    rest = v - __bfloat162float(part[0]);
+  }
+  part[1] = __float2bfloat16(rest);
+  part[2] = __float2bfloat16(rest - __bfloat162float(part[1]));
+}
+
+// rows x cols values at row stride ld into (parts, rows, ldp) bf16, ldp a multiple of 8; a thread has
+// 8 neighbours. Columns behind the last one are left: the tensor map ends in front of them.
+__global__ void __launch_bounds__(256) lay_kernel(const void* src, int64_t ld, int bf16, int64_t rows, int64_t cols,
+                                                  __nv_bfloat16* dst, int64_t ldp, int parts) {
+  const int64_t per = ldp / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, c = i % per * 8;
+    float v[8];
+    if (bf16) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? semx_scan::load(src, row * ld + c + k, 1) : 0.f;
+    } else {
+      const float* s = reinterpret_cast<const float*>(src) + row * ld + c;
+      if (c + 8 <= cols && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
+        const float4 a = *reinterpret_cast<const float4*>(s), b = *reinterpret_cast<const float4*>(s + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? s[k] : 0.f;
+      }
+    }
+    __align__(16) __nv_bfloat16 out[kParts][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      __nv_bfloat16 q[kParts];
+      parts_of(v[k], q);
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) out[n][k] = q[n];
+    }
+#pragma unroll
+    for (int n = 0; n < kParts; ++n)
+      if (n < parts) *reinterpret_cast<uint4*>(dst + (n * rows + row) * ldp + c) = *reinterpret_cast<const uint4*>(out[n]);
+  }
+}
+
+// du and dg from u, g (fp32, rows of ldu) and dh, as parts (parts, 2, rows, ldp); column sums of 64
+// rows each into sums (row blocks, 2 H) where wanted. A thread has 4 columns of every 4th row.
+constexpr int kDzRows = 64;
+__global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const float* g, int64_t ldu, const void* dh, int bf16,
+                                                        int64_t rows, int64_t H, int gelu, __nv_bfloat16* dz, int64_t ldp,
+                                                        int parts, float* sums) {
+  __shared__ float red[2][4][256];
+  const int lane = threadIdx.x % 64, down = threadIdx.x / 64;
+  const int64_t c = (int64_t)blockIdx.y * 256 + lane * 4, r0 = (int64_t)blockIdx.x * kDzRows;
+  const int nn = (int)min((int64_t)4, H - c);
+  const bool wide = H % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (bf16 ? 7 : 15)) == 0;
+  float su[4] = {}, sg[4] = {};
+  if (nn > 0)
+    for (int64_t r = r0 + down; r < min(r0 + kDzRows, rows); r += 4) {
+      const float4 u4 = *reinterpret_cast<const float4*>(u + r * ldu + c), g4 = *reinterpret_cast<const float4*>(g + r * ldu + c);
+      const float uu[4] = {u4.x, u4.y, u4.z, u4.w}, gg[4] = {g4.x, g4.y, g4.z, g4.w};
+      float d[4] = {};
+      if (wide) {
+        const float4 q = bf16 ? semx_scan::quad_floats<semx_scan::kBf16>(semx_scan::load_quad<semx_scan::kBf16>(dh, r * H + c, 1, 4), 1)
+                              : semx_scan::quad_floats<semx_scan::kFp32>(semx_scan::load_quad<semx_scan::kFp32>(dh, r * H + c, 0, 4), 0);
+        d[0] = q.x; d[1] = q.y; d[2] = q.z; d[3] = q.w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < nn) d[k] = semx_scan::load(dh, r * H + c + k, bf16);
+      }
+      __align__(8) __nv_bfloat16 pu[kParts][4], pg[kParts][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool in = k < nn;
+        const float du = in ? d[k] * act_of(gg[k], gelu) : 0.f, dg = in ? d[k] * uu[k] * act_slope(gg[k], gelu) : 0.f;
+        su[k] += du;
+        sg[k] += dg;
+        __nv_bfloat16 q[kParts];
+        parts_of(du, q);
+        for (int n = 0; n < kParts; ++n) pu[n][k] = q[n];
+        parts_of(dg, q);
+        for (int n = 0; n < kParts; ++n) pg[n][k] = q[n];
+      }
+#pragma unroll
+      for (int n = 0; n < kParts; ++n)
+        if (n < parts) {
+          *reinterpret_cast<uint2*>(dz + ((2 * n) * rows + r) * ldp + c) = *reinterpret_cast<const uint2*>(pu[n]);
+          *reinterpret_cast<uint2*>(dz + ((2 * n + 1) * rows + r) * ldp + c) = *reinterpret_cast<const uint2*>(pg[n]);
+        }
+    }
+  if (sums == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    red[0][down][lane * 4 + k] = su[k];
+    red[1][down][lane * 4 + k] = sg[k];
+  }
+  __syncthreads();
+  const int64_t cc = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  if (cc < H) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      sums[(int64_t)blockIdx.x * 2 * H + n * H + cc] =
+          red[n][0][threadIdx.x] + red[n][1][threadIdx.x] + red[n][2][threadIdx.x] + red[n][3][threadIdx.x];
+  }
+}
+
+// -- few rows ---------------------------------------------------------------------------------
+
+// Up to R rows of x. A warp has two columns (four rows of W); x lies in shared memory in fp32, kDepth
+// values of each row at a time. Its lanes take 8 neighbouring weights of every 256.
+constexpr int kDepth = 2048, kFewT = 256, kFew = 8;
+// Place of value k in a row in shared memory: of every 256, the first halves of the lanes' eights, then
+// the second ones, so that lanes side by side read side by side.
+__device__ __forceinline__ int spread(int k) { return (k & ~255) | (k & 4) << 5 | (k & 248) >> 1 | (k & 3); }
+template <int R, bool BF16, bool VEC>
+__global__ void __launch_bounds__(kFewT) few_rows_kernel(const void* x, int64_t ldx, const void* w, int64_t D, int64_t H, int rows,
+                                                         const GemmParams p) {
+  extern __shared__ float xs[];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const int64_t h0 = ((int64_t)blockIdx.x * (kFewT / 32) + warp) * 2;
+  semx_scan::f2 acc[4][R];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[q][r] = semx_scan::pack2(0.f, 0.f);
+  int64_t at[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) at[q] = (min(h0 + (q & 1), H - 1) + (q >> 1) * H) * D;
+  for (int64_t d0 = 0; d0 < D; d0 += kDepth) {
+    const int n = (int)min((int64_t)kDepth, D - d0), n8 = (n + 7) / 8 * 8;
+    if (d0 > 0) __syncthreads();
+    for (int i = tid; i < R * n8; i += kFewT) {
+      const int r = i / n8, k = i % n8;
+      xs[r * kDepth + spread(k)] = r < rows && k < n ? semx_scan::load(x, r * ldx + d0 + k, BF16) : 0.f;
+    }
+    __syncthreads();
+    if (h0 < H)
+#pragma unroll 2
+      for (int k = lane * 8; k < n; k += 256) {
+        semx_scan::f2 wv[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t i = at[q] + d0 + k;
+          float f[8];
+          if constexpr (VEC && BF16) {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(w) + i));
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f[2 * j] = __uint_as_float(e[j] << 16);
+              f[2 * j + 1] = __uint_as_float(e[j] & 0xffff0000u);
+            }
+          } else if constexpr (VEC) {
+            const float4 a = __ldcs(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + i));
+            const float4 b = __ldcs(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + i + 4));
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = k + j < n ? semx_scan::load(w, i + j, BF16) : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wv[q][j] = semx_scan::pack2(f[2 * j], f[2 * j + 1]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float4 a = *reinterpret_cast<const float4*>(&xs[r * kDepth + spread(k)]);
+          const float4 b = *reinterpret_cast<const float4*>(&xs[r * kDepth + spread(k) + 128]);
+          const semx_scan::f2 xv[4] = {semx_scan::pack2(a.x, a.y), semx_scan::pack2(a.z, a.w), semx_scan::pack2(b.x, b.y),
+                                       semx_scan::pack2(b.z, b.w)};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[q][r] = semx_scan::fma2(wv[q][j], xv[j], acc[q][r]);
+        }
+      }
+  }
+  if (h0 >= H) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 s = semx_scan::unpack2(acc[q][r]);
+      v[q] = s.x + s.y;
+#pragma unroll
+      for (int m = 16; m >= 1; m /= 2) v[q] += __shfl_xor_sync(0xffffffffu, v[q], m);
+    }
+    if (lane < 2 && r < rows && h0 + lane < H) {
+      const int64_t h = h0 + lane;
+      float u = lane ? v[1] : v[0], g = lane ? v[3] : v[2];
+      if (p.bias != nullptr) {
+        u += p.bias[h];
+        g += p.bias[H + h];
+      }
+      if (p.u != nullptr) {
+        p.u[r * p.ldu + h] = u;
+        p.g[r * p.ldu + h] = g;
+      }
+      semx_scan::store(p.out, r * p.ldo + h, BF16, u * act_of(g, p.gelu));
+    }
+  }
+}
+
+// -- host ---------------------------------------------------------------------------------------
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static std::atomic<void*> found{nullptr};
+  void* f = found.load(std::memory_order_acquire);
+  if (f == nullptr) {
+    cudaDriverEntryPointQueryResult how;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &how) != cudaSuccess ||
+        how != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    found.store(f, std::memory_order_release);
+  }
+  return reinterpret_cast<EncodeFn>(f);
+}
+
+// An operand in memory: (parts, halves, rows, cols) bf16 with 16-byte aligned rows.
+struct Operand {
+  const void* base;
+  int64_t cols, rows, halves, parts;
+  int64_t ld, half_stride, part_stride;  // elements
+};
+
+// box_rows: rows of a copy (64 columns each).
+int make_map(CUtensorMap* map, const Operand& o, int box_rows) {
+  EncodeFn encode = encode_fn();
+  SEMX_REQUIRE(encode != nullptr, SEMX_ERR_UNSUPPORTED, "gated_linear: the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[4] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.halves, (cuuint64_t)o.parts};
+  const cuuint64_t strides[3] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.halves > 1 ? o.half_stride : o.ld) * 2,
+                                 (cuuint64_t)(o.parts > 1 ? o.part_stride : o.ld) * 2};
+  const cuuint32_t box[4] = {kK, (cuuint32_t)box_rows, 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(o.base), dims, strides, box, steps,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  SEMX_REQUIRE(rc == CUDA_SUCCESS, SEMX_ERR_SHAPE, "gated_linear: cuTensorMapEncodeTiled refused %lld x %lld, stride %lld (%d)",
+               (long long)o.rows, (long long)o.cols, (long long)o.ld, (int)rc);
+  return SEMX_OK;
+}
+
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// What one product needs: tile width, slices of the depth, bytes of their sums.
+struct Plan {
+  int mode, bn, splits;
+  GemmParams p;
+  size_t part_bytes;
+};
+
+// M, N: the result; K: the depth of one pair of parts and half.
+Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
+  Plan q = {};
+  q.mode = mode;
+  GemmParams& p = q.p;
+  p.M = M;
+  p.N = N;
+  p.khalf = (int)cdiv(K, (int64_t)kK);
+  p.kper = p.khalf * (mode == kDx ? 2 : 1);
+  p.pairs = parts > 1 ? 6 : 1;
+  const int64_t wide = mode == kFwd ? 2 * N : N;
+  const int64_t down = cdiv(M, (int64_t)kM) * (mode == kDw ? 2 : 1);
+  q.bn = wide > 128 ? 256 : wide > 64 ? 128 : 64;
+  // Narrower tiles where wide ones leave SMs idle.
+  while (q.bn > 64 && down * cdiv(wide, (int64_t)q.bn) < kSms && cdiv(wide, (int64_t)q.bn / 2) > cdiv(wide, (int64_t)q.bn)) q.bn /= 2;
+  p.tiles_m = (int)cdiv(M, (int64_t)kM);
+  p.tiles_n = (int)cdiv(wide, (int64_t)q.bn);
+  p.tiles = p.tiles_m * p.tiles_n * (mode == kDw ? 2 : 1);
+  // Slices of the depth where tiles alone leave half of the SMs idle, of 8 stages at least.
+  const int64_t depth = (int64_t)p.kper * p.pairs;
+  int64_t s = kSms / p.tiles;
+  if (s > depth / 8) s = depth / 8;
+  if (s > 64) s = 64;
+  p.splits = q.splits = s < 2 ? 1 : (int)s;
+  const int64_t result = M * N * (mode == kDx ? 1 : 2);
+  q.part_bytes = p.splits > 1 ? up256((size_t)p.splits * result * sizeof(float)) : 0;
+  return q;
+}
+
+template <int MODE, int BN>
+int launch_tiles(const Plan& q, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t st) {
+  if (!semx::allow_smem(gemm_kernel<MODE, BN>, gemm_smem(BN))) return SEMX_ERR_LAUNCH;
+  const int works = q.p.tiles * q.p.splits;
+  gemm_kernel<MODE, BN><<<works < kSms ? works : kSms, kGemmT, gemm_smem(BN), st>>>(a, b, q.p);
+  return semx::check_launch("gated_linear gemm_kernel");
+}
+
+template <int MODE>
+int launch_gemm(const Plan& q, const Operand& A, const Operand& B, cudaStream_t st) {
+  CUtensorMap a, b;
+  int rc = make_map(&a, A, MODE == kDw ? 64 : kM);
+  if (rc != SEMX_OK) return rc;
+  rc = make_map(&b, B, MODE == kFwd ? q.bn / 2 : 64);
+  if (rc != SEMX_OK) return rc;
+  rc = q.bn == 256 ? launch_tiles<MODE, 256>(q, a, b, st)
+       : q.bn == 128 ? launch_tiles<MODE, 128>(q, a, b, st) : launch_tiles<MODE, 64>(q, a, b, st);
+  if (rc != SEMX_OK || q.splits == 1) return rc;
+  const int64_t n = q.p.M * q.p.N * (MODE == kDw ? 2 : 1);
+  const unsigned grid = (unsigned)cdiv(n, (int64_t)256);
+  if (MODE == kFwd) join_gated_kernel<<<grid, 256, 0, st>>>(q.p);
+  else join_plain_kernel<<<grid, 256, 0, st>>>(q.p.part, q.splits, n, q.p.out, q.p.out_bf16);
+  return semx::check_launch("gated_linear join");
+}
+
+int lay(const void* src, int64_t ld, int bf16, int64_t rows, int64_t cols, void* dst, int64_t ldp, int parts, cudaStream_t st) {
+  const int64_t n = cdiv(rows * (ldp / 8), (int64_t)256);
+  lay_kernel<<<(unsigned)(n < kSms * 16 ? n : kSms * 16), 256, 0, st>>>(src, ld, bf16, rows, cols,
+                                                                     reinterpret_cast<__nv_bfloat16*>(dst), ldp, parts);
+  return semx::check_launch("gated_linear lay_kernel");
+}
+
+int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
+  const int64_t top = (int64_t)1 << 31;
+  SEMX_REQUIRE(a->rows >= 0 && a->rows < top && a->D >= 1 && a->D < (1 << 23) && a->H >= 1 && a->H < (1 << 23),
+               SEMX_ERR_SHAPE, "gated_linear: rows=%lld, D=%lld, H=%lld", (long long)a->rows, (long long)a->D, (long long)a->H);
+  SEMX_REQUIRE(a->ldx >= a->D && a->ldx < top, SEMX_ERR_SHAPE, "gated_linear: row stride %lld for %lld columns",
+               (long long)a->ldx, (long long)a->D);
+  SEMX_REQUIRE(a->act == 0 || a->act == 1, SEMX_ERR_UNSUPPORTED, "gated_linear: activation %d", a->act);
+  // Tiles and their numbers fit 31 bits.
+  SEMX_REQUIRE(cdiv(a->rows, (int64_t)64) * cdiv(a->H > a->D ? a->H : a->D, (int64_t)32) < ((int64_t)1 << 30) &&
+                   cdiv(a->D, (int64_t)64) * cdiv(a->H, (int64_t)32) < ((int64_t)1 << 30) &&
+                   cdiv(a->rows, (int64_t)kK) * 6 < top,
+               SEMX_ERR_SHAPE, "gated_linear: rows=%lld, D=%lld, H=%lld", (long long)a->rows, (long long)a->D, (long long)a->H);
+  if (a->rows == 0 && !bwd) return SEMX_OK;
+  SEMX_REQUIRE(a->w && (a->rows == 0 || a->x), SEMX_ERR_NULL, "gated_linear: x / w is NULL");
+  if (!bwd) SEMX_REQUIRE(a->h, SEMX_ERR_NULL, "gated_linear: h is NULL");
+  else SEMX_REQUIRE(a->rows == 0 || (a->dh && a->saved), SEMX_ERR_NULL, "gated_linear bwd: dh / saved is NULL");
+  SEMX_REQUIRE(semx::all_aligned({a->x, a->w, a->h, a->dh, a->dx, a->dw}, a->bf16 ? 2 : 4) &&
+                   semx::all_aligned({a->bias, a->db}, 4) && semx::all_aligned({a->saved, a->workspace}, 16),
+               SEMX_ERR_ALIGN, "gated_linear: a pointer is not on an element");
+  return SEMX_OK;
+}
+
+// Whether TMA reads rows of n bf16 at stride ld from base.
+bool in_place(const void* base, int64_t ld, int bf16) { return bf16 && ld % 8 == 0 && semx::aligned(base, 16); }
+
+// Workspace of one call: parts of x, of W, of du | dg, sums of slices, column sums.
+struct Layout {
+  int parts;
+  bool few, lay_x, lay_w;
+  size_t x, w, dz, part, sums, total;
+  Plan fwd, dx, dw;
+};
+
+Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
+  Layout l = {};
+  l.parts = a->bf16 ? 1 : kParts;
+  l.few = !bwd && a->rows <= kFew;
+  if (a->rows == 0 || l.few) return l;
+  // Laid out anew wherever the sizes allow a misaligned base: the query has no addresses that count.
+  l.lay_x = !in_place(a->x, a->ldx, a->bf16);
+  l.lay_w = !in_place(a->w, a->D, a->bf16);
+  const int64_t Dp = up8(a->D), Hp = up8(a->H);
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t was = at;
+    at += up256(bytes);
+    return was;
+  };
+  const bool need_x = !bwd || a->dw != nullptr, need_w = !bwd || a->dx != nullptr;
+  l.x = take(l.lay_x && need_x ? (size_t)l.parts * a->rows * Dp * 2 : 0);
+  l.w = take(l.lay_w && need_w ? (size_t)l.parts * 2 * a->H * Dp * 2 : 0);
+  if (!bwd) {
+    l.fwd = plan_gemm(kFwd, a->rows, a->H, a->D, l.parts);
+    l.part = take(l.fwd.part_bytes);
+  } else {
+    l.dz = take((size_t)l.parts * 2 * a->rows * Hp * 2);
+    l.dx = plan_gemm(kDx, a->rows, a->D, a->H, l.parts);
+    l.dw = plan_gemm(kDw, a->H, a->D, a->rows, l.parts);
+    const size_t p1 = need_w ? l.dx.part_bytes : 0, p2 = need_x ? l.dw.part_bytes : 0;
+    l.part = take(p1 > p2 ? p1 : p2);
+    l.sums = take(a->db != nullptr ? (size_t)cdiv(a->rows, (int64_t)kDzRows) * 2 * a->H * sizeof(float) : 0);
+  }
+  l.total = at;
+  return l;
+}
+
+template <int R>
+int launch_few(const SemxGatedLinearArgs* a, const GemmParams& p, cudaStream_t st) {
+  const size_t smem = (size_t)R * kDepth * sizeof(float);
+  const unsigned grid = (unsigned)cdiv(a->H, (int64_t)(kFewT / 32) * 2);
+  const int rows = (int)a->rows;
+  const bool vec = a->D % 8 == 0 && semx::aligned(a->w, 16);
+#define SEMX_FEW(B, V)                                                                                      \
+  do {                                                                                                      \
+    if (!semx::allow_smem(few_rows_kernel<R, B, V>, smem)) return SEMX_ERR_LAUNCH;                          \
+    few_rows_kernel<R, B, V><<<grid, kFewT, smem, st>>>(a->x, a->ldx, a->w, a->D, a->H, rows, p);           \
+  } while (0)
+  if (a->bf16) {
+    if (vec) SEMX_FEW(true, true);
+    else SEMX_FEW(true, false);
+  } else {
+    if (vec) SEMX_FEW(false, true);
+    else SEMX_FEW(false, false);
+  }
+#undef SEMX_FEW
+  return semx::check_launch("gated_linear few_rows_kernel");
+}
+
+// x and W as the products read them.
+int lay_operands(const SemxGatedLinearArgs* a, const Layout& l, bool need_x, bool need_w, char* ws, cudaStream_t st, Operand* x,
+                 Operand* w) {
+  const int64_t Dp = up8(a->D);
+  *x = Operand{a->x, a->D, a->rows, 1, 1, a->ldx, 0, 0};
+  *w = Operand{a->w, a->D, a->H, 2, 1, a->D, a->H * a->D, 0};
+  if (need_x && l.lay_x) {
+    const int rc = lay(a->x, a->ldx, a->bf16, a->rows, a->D, ws + l.x, Dp, l.parts, st);
+    if (rc != SEMX_OK) return rc;
+    *x = Operand{ws + l.x, a->D, a->rows, 1, l.parts, Dp, 0, a->rows * Dp};
+  }
+  if (need_w && l.lay_w) {
+    const int rc = lay(a->w, a->D, a->bf16, 2 * a->H, a->D, ws + l.w, Dp, l.parts, st);
+    if (rc != SEMX_OK) return rc;
+    *w = Operand{ws + l.w, a->D, a->H, 2, l.parts, Dp, a->H * Dp, 2 * a->H * Dp};
+  }
+  return SEMX_OK;
+}
+
+}  // namespace
+
+namespace semx {
+int gemm_timeouts(uint32_t* count) {
+  unsigned v = 0;
+  const cudaError_t e = cudaMemcpyFromSymbol(&v, g_gemm_timeouts, sizeof(v));
+  if (e != cudaSuccess) return fail(SEMX_ERR_LAUNCH, "gemm_timeouts: %s", cudaGetErrorString(e));
+  *count = v;
+  return SEMX_OK;
+}
+}  // namespace semx
+
+extern "C" {
+
+size_t semx_gated_linear_args_size(void) { return sizeof(SemxGatedLinearArgs); }
+
+size_t semx_gated_linear_saved_bytes(const SemxGatedLinearArgs* a) {
+  return a == nullptr || a->rows < 0 || a->H < 0 ? 0 : (size_t)2 * a->rows * up8(a->H) * sizeof(float);
+}
+
+size_t semx_gated_linear_workspace_bytes(const SemxGatedLinearArgs* a, int32_t backward) {
+  if (a == nullptr || a->rows < 0 || a->D < 1 || a->H < 1) return 0;
+  return layout_of(a, backward != 0).total;
+}
+
+int semx_gated_linear_fwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
+  SEMX_CHECK_ARGS(a, SemxGatedLinearArgs);
+  int rc = gl_check(a, false);
+  if (rc != SEMX_OK || a->rows == 0) return rc;
+  semx::DeviceScope scope;
+  rc = scope.bind({a->h});
+  if (rc != SEMX_OK) return rc;
+  cudaStream_t st = semx::as_stream(stream);
+  const Layout l = layout_of(a, false);
+  Plan q = l.fwd;
+  q.p.out = a->h;
+  q.p.ldo = a->H;
+  q.p.out_bf16 = a->bf16;
+  q.p.ldu = up8(a->H);
+  q.p.u = a->saved;
+  q.p.g = a->saved == nullptr ? nullptr : a->saved + a->rows * q.p.ldu;
+  q.p.bias = a->bias;
+  q.p.gelu = a->act;
+  if (l.few) {
+    if (a->rows == 1) return launch_few<1>(a, q.p, st);
+    if (a->rows == 2) return launch_few<2>(a, q.p, st);
+    if (a->rows <= 4) return launch_few<4>(a, q.p, st);
+    return launch_few<8>(a, q.p, st);
+  }
+  SEMX_REQUIRE(l.total == 0 || a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_linear: workspace is NULL");
+  char* ws = reinterpret_cast<char*>(a->workspace);
+  q.p.part = reinterpret_cast<float*>(ws + l.part);
+  Operand x, w;
+  rc = lay_operands(a, l, true, true, ws, st, &x, &w);
+  if (rc != SEMX_OK) return rc;
+  return launch_gemm<kFwd>(q, x, w, st);
+}
+
+int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
+  SEMX_CHECK_ARGS(a, SemxGatedLinearArgs);
+  int rc = gl_check(a, true);
+  if (rc != SEMX_OK) return rc;
+  semx::DeviceScope scope;
+  rc = scope.bind({a->dw, a->dx, a->db});
+  if (rc != SEMX_OK) return rc;
+  cudaStream_t st = semx::as_stream(stream);
+  if (a->rows == 0) {
+    cudaError_t e = cudaSuccess;
+    if (a->dw != nullptr) e = cudaMemsetAsync(a->dw, 0, (size_t)2 * a->H * a->D * (a->bf16 ? 2 : 4), st);
+    if (e == cudaSuccess && a->db != nullptr) e = cudaMemsetAsync(a->db, 0, (size_t)2 * a->H * sizeof(float), st);
+    SEMX_REQUIRE(e == cudaSuccess, SEMX_ERR_LAUNCH, "gated_linear bwd: cudaMemsetAsync: %s", cudaGetErrorString(e));
+    return SEMX_OK;
+  }
+  const bool need_x = a->dw != nullptr, need_w = a->dx != nullptr;
+  if (!need_x && !need_w && a->db == nullptr) return SEMX_OK;
+  const Layout l = layout_of(a, true);
+  SEMX_REQUIRE(a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_linear bwd: workspace is NULL");
+  char* ws = reinterpret_cast<char*>(a->workspace);
+  const int64_t Hp = up8(a->H), blocks = cdiv(a->rows, (int64_t)kDzRows);
+  float* sums = a->db != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
+  __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + l.dz);
+  const float *u = a->saved, *g = a->saved + a->rows * Hp;
+  gate_grad_kernel<<<dim3((unsigned)blocks, (unsigned)cdiv(a->H, (int64_t)256)), 256, 0, st>>>(
+      u, g, Hp, a->dh, a->bf16, a->rows, a->H, a->act, dz, Hp, l.parts, sums);
+  rc = semx::check_launch("gated_linear gate_grad_kernel");
+  if (rc != SEMX_OK) return rc;
+  Operand x, w;
+  rc = lay_operands(a, l, need_x, need_w, ws, st, &x, &w);
+  if (rc != SEMX_OK) return rc;
+  const Operand d = {dz, a->H, a->rows, 2, l.parts, Hp, a->rows * Hp, 2 * a->rows * Hp};
+  if (need_w) {
+    Plan q = l.dx;
+    q.p.out = a->dx;
+    q.p.ldo = a->D;
+    q.p.out_bf16 = a->bf16;
+    q.p.part = reinterpret_cast<float*>(ws + l.part);
+    rc = launch_gemm<kDx>(q, d, w, st);
+    if (rc != SEMX_OK) return rc;
+  }
+  if (need_x) {
+    Plan q = l.dw;
+    q.p.out = a->dw;
+    q.p.ldo = a->D;
+    q.p.out_bf16 = a->bf16;
+    q.p.part = reinterpret_cast<float*>(ws + l.part);
+    rc = launch_gemm<kDw>(q, d, x, st);
+    if (rc != SEMX_OK) return rc;
+  }
+  if (a->db == nullptr) return SEMX_OK;
+  semx::Segments seg = {};
+  seg.n = 1;
+  seg.out[0] = a->db;
+  seg.len[0] = 2 * a->H;
+  return semx::colsum_once(sums, blocks, 2 * a->H, seg, st);
+}
+
+}  // extern "C"

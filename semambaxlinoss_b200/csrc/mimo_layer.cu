@@ -2455,10 +2455,11 @@ int semx_tc_timeouts(uint32_t* count) {
   unsigned int v = 0;
   const cudaError_t e = cudaMemcpyFromSymbol(&v, g_tc_timeouts, sizeof(v));
   if (e != cudaSuccess) return semx::fail(SEMX_ERR_LAUNCH, "semx_tc_timeouts: %s", cudaGetErrorString(e));
-  uint32_t links = 0;
-  const int rc = semx::link_timeouts(&links);
+  uint32_t links = 0, gemms = 0;
+  int rc = semx::link_timeouts(&links);
+  if (rc == SEMX_OK) rc = semx::gemm_timeouts(&gemms);
   if (rc != SEMX_OK) return rc;
-  *count = v + links;
+  *count = v + links + gemms;
   return SEMX_OK;
 }
 

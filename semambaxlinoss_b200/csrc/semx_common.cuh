@@ -48,6 +48,8 @@ class DeviceScope {
 // Waits of the gated recurrence's tiles on one another that gave up, on the current device
 // (a part of semx_tc_timeouts()).
 int link_timeouts(uint32_t* count);
+// The same of the gated projection's roles.
+int gemm_timeouts(uint32_t* count);
 
 inline bool aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;

@@ -32,7 +32,9 @@ Supported mixers: ``selective_lru``, ``selective_lru_mimo``, ``linoss`` (the lay
 this package's scan path), ``selective_state`` (the Mamba layer's formulas) and ``gated_lru``
 (one gated real mode per channel). The last two take packed sequences, prompts and single
 tokens (``ssm_params``: the mixer's own keyword arguments; ``cu_seqlens``, ``cache``, ``slots``
-and ``fresh`` pass through ``Block.forward``). The
+and ``fresh`` pass through ``Block.forward``). With ``mlp`` (the keyword arguments of
+``GatedMLP``, an empty dict for its defaults) in the configuration the block has a gated
+feed-forward half behind a second norm. The
 reference's other backbones (``mamba``, ``mamba2``, ``mamba3`` from mamba_ssm, ``s4d``,
 ``s5``, and ``selective_linoss``, whose source the reference does not contain) raise
 NotImplementedError.
@@ -49,6 +51,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from .gated_lru import GatedLruMixer
+from .gated_mlp import GatedMLP
 from .layer_norm import LayerNorm
 from .layout import TokenLayout
 from .linoss import LinOSS
@@ -290,6 +293,8 @@ def create_block(d_model, model_cfg, layer_idx=0, rms_norm=True, fused_add_norm=
     layer_norm_cls = LayerNorm if fused_add_norm else nn.LayerNorm
     norm_cls = partial(layer_norm_cls if not rms_norm else RMSNorm, eps=norm_eps)
     if model_cfg["ssm"] == "hybrid":
+        if model_cfg.get("mlp", None) is not None:
+            raise ValueError("a hybrid block has no feed-forward half; mlp must be absent")
         hybrid_cfg = model_cfg.get("hybrid", {})
         b1 = _build_mixer_cls(d_model, model_cfg["backbone_1"], layer_idx)(d_model)
         b2 = _build_mixer_cls(d_model, model_cfg["backbone_2"], layer_idx)(d_model)
@@ -299,7 +304,9 @@ def create_block(d_model, model_cfg, layer_idx=0, rms_norm=True, fused_add_norm=
         block.layer_idx = layer_idx
         return block
     mixer_cls = _build_mixer_cls(d_model, model_cfg, layer_idx)
-    block = Block(d_model, mixer_cls, nn.Identity, norm_cls=norm_cls,
+    mlp = model_cfg.get("mlp", None)
+    mlp_cls = nn.Identity if mlp is None else partial(GatedMLP, **mlp)
+    block = Block(d_model, mixer_cls, mlp_cls, norm_cls=norm_cls,
                   fused_add_norm=fused_add_norm, residual_in_fp32=residual_in_fp32)
     block.layer_idx = layer_idx
     return block
@@ -319,7 +326,8 @@ class MambaBlock(nn.Module):
         self.forward_blocks = nn.ModuleList(create_block(in_channels, cfg) for _ in range(n_layer))
         if self.bidirectional:
             self.backward_blocks = nn.ModuleList(create_block(in_channels, cfg) for _ in range(n_layer))
-        self.apply(partial(_init_weights, n_layer=n_layer))
+        self.apply(partial(_init_weights, n_layer=n_layer,
+                           n_residuals_per_layer=1 if cfg.get("mlp", None) is None else 2))
 
     def accepts_layout(self, layout: TokenLayout) -> bool:
         """Whether forward(x, layout=layout) reads x in place: the forward blocks take
