@@ -737,7 +737,7 @@ int semx_state_step(const SemxStateScanArgs* args, semx_stream_t stream);
  * semx_gated_lru_*: whole sequences. A training forward passes ckpt
  * (semx_gated_lru_ckpt_bytes()); the backward reads it and writes dx, d_r, d_i, dz (with z),
  * and drate, dr_bias, di_bias (each may be NULL), reduced in a fixed order. Where 1 - a^2 is
- * at its least value no gradient goes through the gain. Workspace (8-byte aligned, of this
+ * at its least value no gradient goes through the gain. Workspace (16-byte aligned, of this
  * call alone): semx_gated_lru_workspace_bytes() with `backward` 0 or 1 (0 bytes where none is
  * needed).
  * semx_gated_lru_step: one row per sequence (cu_seqlens NULL, L = 1), state required, no

@@ -9,19 +9,22 @@
 //   dla = g a h_{t-1} - (left > 1e-6) g iota x a^2 / gain, dr = -speed dla rho (1 - rho)
 // with speed = rate_scale softplus(rate).
 //
-// Bound: HBM (5 values per element forward, 9 backward); what each element needs of the
-// special-function unit (7 to 14 operations) comes next.
+// Bound: HBM (5 values per element forward, 9 backward); the special-function unit (6 operations per
+// element forward) comes next.
 //
-// Split: a tile is 64 steps of one sequence by 64 channels; a CTA reads it once. A thread has
-// kSeg neighbouring steps of four neighbouring channels (whole sectors of a row per warp), so the
-// recurrence inside a tile is 16 segments: each thread folds its steps into one map
-// h -> A h + B, 64 threads (one per channel) fold the segments and find the tile's entry state,
-// and each thread runs its steps again from its segment's entry state, on registers.
-// Tiles of a sequence are linked inside the one launch: each leaves its map (A, B), and takes the
-// maps of the tiles in front of it in its group of 16 and the state that the last tile of the group
-// before left. Which maps are folded in which order depends on the numbers alone, so results do
-// not change from run to run. Tickets number the tiles in the order in which CTAs start, so a tile
-// only waits for tiles that run already. The backward runs the same from the last tile on.
+// Split: a tile is 64 steps (bf16; fp32 32) of one sequence by 32 channels; a CTA of four warps reads
+// it once. A thread has a segment of 4 (2) neighbouring steps of four neighbouring channels: it folds
+// them into one map h -> A h + B, one warp (a lane per channel) folds the 16 segments' maps and finds
+// the tile's entry state, and each thread runs its steps again from its segment's entry state, on
+// registers. CTAs stay and take tile after tile; the next tile's rows are on their way while this
+// one's entry state is looked for.
+// Many sequences: a CTA walks one after another, the state stays in registers. Few or packed ones:
+// tiles are linked through global memory inside the one launch: each leaves its map (A, B) and the
+// state behind it, and takes the maps of the tiles in front of it in its group of 8 and the state that
+// the group before left. Which maps are folded in which order depends on the numbers alone, so
+// results do not change from run to run. Tickets number the tiles in the order in which CTAs take
+// them, so a tile only waits for tiles that are under way. The backward runs the same from the last
+// tile on.
 #include "semx_reduce.cuh"
 #include "state_scan.cuh"
 
@@ -29,12 +32,18 @@ namespace {
 
 using namespace semx_scan;
 
-constexpr int kT = 256;
-constexpr int kSegs = 16, kSeg = 4, kRows = kSegs * kSeg;  // segments, steps of each, steps of a tile
-constexpr int kCh = 64;                                    // channels of a tile
-constexpr int kGroup = 16;                                 // tiles between two states handed on
-constexpr unsigned kPolls = 1u << 22;
-constexpr float kLeast = 1e-6f;  // of 1 - a^2, as the gamma gain of the selective-LRU scans has it
+constexpr int kSms = 148;
+constexpr int kT = 128;
+constexpr int kCh = 32;             // channels of a tile: eight lanes of four
+constexpr int kSegs = kT * 4 / kCh; // segments of a tile
+constexpr int kFwdCtas = 5, kBwdCtas = 4;  // per SM
+constexpr int kGroup = 8;           // tiles between two states handed on
+constexpr float kLeastGain = 1e-3f;  // sqrt(1e-6), as the gamma gain of the selective-LRU scans has it
+constexpr float kNear = 0.35f;      // -la up to which the polynomials below hold
+constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
+
+// Steps of a segment: the rows of a tile in shared memory are as many bytes in either type.
+__host__ __device__ constexpr int seg_steps(bool bf16) { return bf16 ? 4 : 2; }
 
 __device__ unsigned int g_link_timeouts;
 
@@ -58,443 +67,703 @@ struct GlParams {
   void* dr;
   void* di;
   void* dz;
-  float* part;   // (tiles, 3, C) partial drate | dr_bias | di_bias
-  int* ticket;   // NULL: no sequence has more than one tile
-  int* flags;    // (tiles, ctiles, 2): 1 the tile's map is there, 2 the state behind it too
-  float2* maps;  // (tiles, C)
-  float* left;   // (tiles, C) state behind the last tile of each group
+  float* part;     // (tiles, or sequences where a CTA walks them; 3, C) partial drate | dr_bias | di_bias
+  int* ticket;     // linked: the next tile's number
+  ulonglong2* maps;         // linked: (tiles, C) map (A, B) of each tile, kHere in the upper half of both
+  unsigned long long* left; // linked: (tiles, C) state behind each tile, kHere in the upper half
 };
 
-// exp(la) - 1 for -0.35 <= la <= 0: Taylor's series up to la^7 (the rest is 1.6e-8 of it).
-__device__ __forceinline__ float expm1_near(float la) {
-  float q = fmaf(la, 1.f / 5040.f, 1.f / 720.f);
-  q = fmaf(q, la, 1.f / 120.f);
-  q = fmaf(q, la, 1.f / 24.f);
-  q = fmaf(q, la, 1.f / 6.f);
-  q = fmaf(q, la, 0.5f);
-  return fmaf(la * la, q, la);
+// Special-function results in pairs.
+__device__ __forceinline__ f2 ex2_2(f2 v) {
+  const float2 t = unpack2(v);
+  return pack2(semx::ex2_approx(t.x), semx::ex2_approx(t.y));
+}
+__device__ __forceinline__ f2 rcp_2(f2 v) {
+  const float2 t = unpack2(v);
+  return pack2(semx::rcp_approx(t.x), semx::rcp_approx(t.y));
+}
+__device__ __forceinline__ f2 rsqrt_2(f2 v) {
+  const float2 t = unpack2(v);
+  return pack2(semx::rsqrt_approx(t.x), semx::rsqrt_approx(t.y));
+}
+__device__ __forceinline__ f2 both(float c) { return pack2(c, c); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// Decay a and 1 - a^2. The series near 0 keeps the decay exact to its rounding (a state
-// multiplies hundreds of them) and 1 - a^2 = -e (2 + e) free of cancellation; the special-function
-// exponential is 2 steps off, which a decay below 0.7 forgets at once.
-__device__ __forceinline__ void decay(float la, bool slow, float* a, float* left) {
-  float e = expm1_near(la);
-  *a = 1.f + e;
-  *left = -e * (2.f + e);
-  if (!slow) {
-    const float f = semx::ex2_approx(la * kLog2e);
-    const bool far = la < -0.35f;
-    if (far) {
-      *a = f;
-      *left = fmaf(-f, f, 1.f);
-    }
+// With m = -la in [0, 0.35] (Chebyshev interpolants of degree 5, 4.4e-8 off with their coefficients'
+// roundings; 2e-9 by themselves):
+//   (1 - exp(-m)) / m, sqrt((1 - exp(-2 m)) / (2 m)), and the latter's inverse.
+__device__ __forceinline__ f2 horner5(f2 m, float c0, float c1, float c2, float c3, float c4, float c5) {
+  f2 v = fma2(both(c5), m, both(c4));
+  v = fma2(v, m, both(c3));
+  v = fma2(v, m, both(c2));
+  v = fma2(v, m, both(c1));
+  return fma2(v, m, both(c0));
+}
+__device__ __forceinline__ f2 loss_near(f2 m) {
+  return horner5(m, 1.0f, -0.4999999701976776f, 0.16666558384895325f, -0.04165346175432205f, 0.008259650319814682f,
+                 -0.0011966862948611379f);
+}
+__device__ __forceinline__ f2 root_near(f2 m) {
+  return horner5(m, 1.0f, -0.4999999403953552f, 0.2083314210176468f, -0.06247641518712044f, 0.013583178631961346f,
+                 -0.0019963912200182676f);
+}
+__device__ __forceinline__ f2 inverse_root_near(f2 m) {
+  return horner5(m, 1.0f, 0.5f, 0.04166705161333084f, -0.020837461575865746f, -0.0015454931417480111f,
+                 0.0016374377300962806f);
+}
+
+// What a channel's rates come to, one float per channel of the tile.
+struct Rates {
+  float speed[kCh];  // rate_scale softplus(rate)
+  float root[kCh];   // sqrt(2 speed)
+  float inverse[kCh];
+  float slope[kCh];  // d speed / d rate
+  float r2[kCh], i2[kCh];  // biases, times -log2(e)
+};
+__device__ __forceinline__ void load_rates(const GlParams& p, int ct, int lane, Rates* to) {
+  const int c = min(ct * kCh + lane, p.C - 1);
+  const float rate = p.rate[c];
+  float e, s = p.scale * softplus(rate, &e);
+  to->slope[lane] = p.scale * softplus_slope(rate, e);
+  s = s > 1e37f ? 1e37f : s;  // an infinite one times a closed gate is no number
+  to->speed[lane] = s;
+  const float inverse = semx::rsqrt_approx(2.f * s);
+  to->inverse[lane] = inverse;
+  to->root[lane] = s > 0.f ? 2.f * s * inverse : 2.f * s;
+  to->r2[lane] = p.r_bias != nullptr ? -kLog2e * p.r_bias[c] : 0.f;
+  to->i2[lane] = p.i_bias != nullptr ? -kLog2e * p.i_bias[c] : 0.f;
+}
+__device__ __forceinline__ f2 shared_pair(const float* row, int c) {
+  return *reinterpret_cast<const f2*>(row + c);
+}
+
+// Channels 2 h and 2 h + 1 of four.
+template <int ACC>
+__device__ __forceinline__ f2 pair_of(const typename RawQuad<ACC>::type& q, int h, int bf16) {
+  if constexpr (ACC == kBf16) {
+    const uint32_t w = h ? q.y : q.x;
+    return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    const uint32_t a = h ? q.z : q.x, b = h ? q.w : q.y;
+    return ACC == kFp32 ? pack2(__uint_as_float(a), __uint_as_float(b)) : pack2(as_float(a, bf16), as_float(b, bf16));
   }
 }
 
-// sigmoid(v) and 1 - sigmoid(v), the latter free of cancellation.
-__device__ __forceinline__ void sigmoids(float v, float* s, float* rest) {
-  const float e = semx::ex2_approx(-kLog2e * v);
-  *s = semx::rcp_approx(1.f + e);
-  *rest = v < -80.f ? 1.f : e * *s;
+// Decay and gain of a pair of channels. The decay gate's reciprocal root q gives both the gate
+// rho = q^2 and the gain: with m = -la = speed rho, sqrt(1 - exp(-2 m)) = sqrt(2 speed) q root(m).
+// Near m = 0 the decay is exact to its rounding (a state multiplies hundreds of them) and nothing
+// cancels; far from it the special-function exponential is 2 steps off, which a decay below 0.7
+// forgets at once. gain: not yet at its least value.
+__device__ __forceinline__ void decay2(f2 q, f2 speed, f2 root, bool slow, f2* rho, f2* m, f2* a, f2* gain) {
+  *rho = mul2(q, q);
+  *m = mul2(*rho, speed);
+  *a = fma2(mul2(*m, both(-1.f)), loss_near(*m), both(1.f));
+  *gain = mul2(mul2(q, root), root_near(*m));
+  if (!slow) {
+    const float2 mm = unpack2(*m);
+    float2 aa = unpack2(*a), gg = unpack2(*gain);
+    if (mm.x > kNear) {
+      aa.x = semx::ex2_approx(-kLog2e * mm.x);
+      gg.x = sqrtf(fmaf(-aa.x, aa.x, 1.f));
+    }
+    if (mm.y > kNear) {
+      aa.y = semx::ex2_approx(-kLog2e * mm.y);
+      gg.y = sqrtf(fmaf(-aa.y, aa.y, 1.f));
+    }
+    *a = pack2(aa.x, aa.y);
+    *gain = pack2(gg.x, gg.y);
+  }
 }
+__device__ __forceinline__ f2 least2(f2 gain) {
+  const float2 g = unpack2(gain);
+  return pack2(fmaxf(g.x, kLeastGain), fmaxf(g.y, kLeastGain));
+}
+// Far up the exponential of a closed gate ends, so that its product with what it closes is 1.
+__device__ __forceinline__ f2 end2(f2 v) {
+  const float2 t = unpack2(v);
+  return pack2(t.x > 126.f ? 126.f : t.x, t.y > 126.f ? 126.f : t.y);
+}
+__device__ __forceinline__ f2 gate_arg(f2 v, f2 bias) { return fma2(v, both(-kLog2e), bias); }
 
-struct Quad {
-  float v[4];
-};
-__device__ __forceinline__ Quad quad(float4 f) { return Quad{{f.x, f.y, f.z, f.w}}; }
+// -- links between the tiles of a sequence --------------------------------------------------------
 
-__device__ __forceinline__ int load_flag(const int* f) {
-  int v;
-  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
-  return v;
-}
-__device__ __forceinline__ void store_flag(int* f, int v) {
-  asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(f), "r"(v) : "memory");
-}
+constexpr unsigned long long kHere = 1ull << 32;
 
 // Where tile number `at` in the order of the recurrence is among the pieces: j0 + dir at.
 struct Chain {
   int64_t j0;
   int dir, at;
-  bool next;  // a tile follows
 };
 
-// One warp, a lane per channel (c, or none: ok false). (A, B): the tile's map; the first tile of a
-// sequence has its entry state in it (A = 0). Returns the state in front of the tile.
-__device__ float link_in(const GlParams& p, const Chain& q, int ct, int half, int c, bool ok, float A, float B) {
-  const int lane = threadIdx.x & 31;
-  const int64_t me = q.j0 + (int64_t)q.dir * q.at;
-  int* flag = p.flags + (me * p.ctiles + ct) * 2 + half;
-  if (q.next) {
-    if (ok) __stcg(&p.maps[me * p.C + c], make_float2(A, B));
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) store_flag(flag, 1);
-  }
-  if (q.at == 0) return 0.f;
+__device__ __forceinline__ ulonglong2 peek_map(const ulonglong2* p) {
+  ulonglong2 v;
+  asm volatile("ld.relaxed.gpu.global.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long peek(const unsigned long long* p) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+// Every number comes with the mark that it is there (64 bits are one access), so that no fence
+// stands between a tile and the next.
+__device__ __forceinline__ unsigned long long marked(float v) { return kHere | __float_as_uint(v); }
+__device__ __forceinline__ void leave_map(const GlParams& p, int64_t j, int c, float A, float B) {
+  asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};" ::"l"(&p.maps[j * p.C + c]), "l"(marked(A)), "l"(marked(B)) : "memory");
+}
+__device__ __forceinline__ void leave_state(const GlParams& p, int64_t j, int c, float h) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(&p.left[j * p.C + c]), "l"(marked(h)) : "memory");
+}
+
+// State in front of the tile for channel c (a lane each; ok false: none): the maps of the tiles in
+// front in its group, folded in their order, applied to the state that the group before left. The
+// first tile of a sequence has its entry state in its map (A = 0).
+__device__ __forceinline__ float link_in(const GlParams& p, const Chain& q, int c, bool ok) {
   const int g0 = q.at / kGroup * kGroup, n = q.at - g0;
-  // Lanes below n wait for the maps of the tiles in front in the group, lane kGroup for the state
-  // that the group before left.
-  const bool waits = lane < n || (lane == kGroup && g0 > 0);
-  const int64_t of = q.j0 + (int64_t)q.dir * (lane < n ? g0 + lane : g0 - 1);
   // Offsets that decrease can name a piece that is none.
-  const bool there = waits && of >= 0 && of < p.m.pieces;
-  const int* theirs = p.flags + (of * p.ctiles + ct) * 2 + half;
-  const int want = lane < n ? 1 : 2;
-  bool done = false;
-  for (unsigned tries = 0; tries < kPolls && !done; ++tries)
-    done = __all_sync(0xffffffffu, !there || load_flag(theirs) >= want);
-  if (!done && lane == 0) atomicAdd(&g_link_timeouts, 1u);
-  __syncwarp();
+  auto index = [&](int at) {
+    const int64_t j = q.j0 + (int64_t)q.dir * at;
+    return ok && j >= 0 && j < p.m.pieces ? j : (int64_t)-1;
+  };
+  ulonglong2 m[kGroup - 1];
+  unsigned long long before = kHere;
+  const int64_t jb = g0 > 0 ? index(g0 - 1) : -1;
+  const long long from = clock64();
+  bool done;
+  do {
+    done = true;
+#pragma unroll
+    for (int e = 0; e < kGroup - 1; ++e) {
+      const int64_t j = e < n ? index(g0 + e) : -1;
+      m[e] = j >= 0 ? peek_map(&p.maps[j * p.C + c]) : make_ulonglong2(marked(1.f), marked(0.f));
+    }
+    if (jb >= 0) before = peek(&p.left[jb * p.C + c]);
+#pragma unroll
+    for (int e = 0; e < kGroup - 1; ++e) done = done && (m[e].x & kHere) != 0 && (m[e].y & kHere) != 0;
+    done = done && (before & kHere) != 0;
+  } while (!done && clock64() - from < kPatience);
+  if (!done) {
+    atomicAdd(&g_link_timeouts, 1u);
+    return __int_as_float(0x7fffffff);
+  }
   float a = 1.f, b = 0.f;
-#pragma unroll 1
-  for (int e = 0; e < n; e += 5) {  // 15 maps at most, 5 on their way at a time
-    float2 m[5];
 #pragma unroll
-    for (int u = 0; u < 5; ++u) {
-      const int64_t j = q.j0 + (int64_t)q.dir * (g0 + e + u);
-      m[u] = e + u < n && ok && j >= 0 && j < p.m.pieces ? __ldcg(&p.maps[j * p.C + c]) : make_float2(1.f, 0.f);
+  for (int e = 0; e < kGroup - 1; ++e) {
+    const float A = __uint_as_float((unsigned)m[e].x), B = __uint_as_float((unsigned)m[e].y);
+    b = fmaf(A, b, B);
+    a *= A;
+  }
+  return jb >= 0 ? fmaf(a, __uint_as_float((unsigned)before), b) : b;
+}
+
+// -- the order of a CTA's tiles -------------------------------------------------------------------
+
+// A tile: rows [row, row + n) of the batch, number k of `tiles` of sequence s, piece j of the batch.
+struct Tile {
+  int64_t row;
+  int n, k, tiles, s, j, ct;
+  bool any, live;  // any: there is one; live: it is a part of a sequence (one without rows has tile 0)
+};
+
+__device__ __forceinline__ int start_of(const semx::SeqMap& m, int s) {
+  return m.cu == nullptr ? s * (int)m.L : min(max(m.cu[s], 0), (int)m.T);
+}
+// Piece j of Q rows, as semx::find_piece has it, in 32 bits with Q known.
+template <int Q>
+__device__ __forceinline__ void find_tile(const semx::SeqMap& m, int j, Tile* t) {
+  int start, len;
+  if (m.cu == nullptr) {
+    t->s = (int)((unsigned)j / (unsigned)m.per);
+    t->k = j - t->s * (int)m.per;
+    start = t->s * (int)m.L;
+    len = (int)m.L;
+  } else {
+    int lo = 0, n = (int)m.S;
+    const int lane = threadIdx.x & 31;
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const int at = lo + lane * step;
+      const bool ok = lane * step < n && start_of(m, at) / Q + at <= j;
+      const unsigned hit = __ballot_sync(0xffffffffu, ok);
+      const int w = hit == 0u ? 0 : 31 - __clz((int)hit);
+      lo += w * step;
+      n = min(step, n - w * step);
     }
-#pragma unroll
-    for (int u = 0; u < 5; ++u) {
-      b = fmaf(m[u].x, b, m[u].y);
-      a *= m[u].x;
-    }
+    t->s = lo;
+    start = start_of(m, lo);
+    len = max(start_of(m, lo + 1), start) - start;
+    t->k = j - (start / Q + lo);
   }
-  float h = 0.f;
-  if (g0 > 0) {
-    const int64_t j = q.j0 + (int64_t)q.dir * (g0 - 1);
-    if (ok && j >= 0 && j < p.m.pieces) h = __ldcg(&p.left[j * p.C + c]);
-  }
-  if (!done) return __int_as_float(0x7fffffff);
-  // A sequence's first tile (A = 0) leaves no way for what stands in front of it.
-  return g0 > 0 ? fmaf(a, h, b) : b;
+  t->tiles = (len + Q - 1) / Q;
+  t->live = t->k >= 0 && (t->k == 0 || t->k < t->tiles);
+  t->row = start + (t->live ? t->k * Q : 0);
+  t->n = t->live ? min(len - t->k * Q, Q) : 0;
 }
 
-// Hands on the state behind the tile: the last tile of a group writes it. Every tile raises its
-// flag, so that nothing waits for long whatever the offsets are.
-__device__ __forceinline__ void link_out(const GlParams& p, const Chain& q, int ct, int half, int c, bool ok, float h) {
-  const int64_t me = q.j0 + (int64_t)q.dir * q.at;
-  if (q.next && q.at % kGroup == kGroup - 1) {
-    if (ok) __stcg(&p.left[me * p.C + c], h);
-    __threadfence();
+// LINK: tiles in the order of their tickets. Else the CTA walks whole sequences of equal lengths, all
+// tiles of one behind one another. BACK: from the last one on. `n`: the ticket, or the walked
+// sequence's number among (sequences, channel tiles).
+template <bool LINK, bool BACK, int Q>
+__device__ __forceinline__ Tile tile_at(const GlParams& p, int n, int step) {
+  Tile t;
+  const int total = (int)((LINK ? p.m.pieces : p.m.S) * p.ctiles);
+  t.any = n < total;
+  t.live = false;
+  t.j = t.ct = t.k = t.n = t.s = t.tiles = 0;
+  t.row = 0;
+  if (!t.any) return t;
+  const unsigned i = LINK && BACK ? total - 1 - n : n;
+  const int of = (int)(i / (unsigned)p.ctiles);
+  t.ct = (int)i - of * p.ctiles;
+  if (LINK) {
+    t.j = of;
+    if (p.m.S > 0) find_tile<Q>(p.m, of, &t);
+  } else {
+    t.s = of;
+    t.tiles = (int)p.m.per;
+    t.k = BACK ? t.tiles - 1 - step : step;
+    t.j = of * t.tiles + t.k;
+    t.row = (int64_t)of * p.m.L + t.k * Q;
+    t.n = min((int)p.m.L - t.k * Q, Q);
+    t.live = true;
   }
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) store_flag(p.flags + (me * p.ctiles + ct) * 2 + half, 2);
+  return t;
 }
 
-// Number of the tile that this CTA takes.
-__device__ __forceinline__ int64_t take_tile(const GlParams& p, int* slot) {
-  if (p.ticket == nullptr) return blockIdx.x;
-  if (threadIdx.x == 0) *slot = atomicAdd(p.ticket, 1);
-  __syncthreads();
-  return *slot;
-}
-
-// Per channel of the tile: speed = rate_scale softplus(rate), both biases, and with SLOPE the
-// derivative of speed.
-template <bool SLOPE>
-__device__ __forceinline__ void tile_params(const GlParams& p, int c0, float (*par)[kCh]) {
-  if (threadIdx.x < kCh) {
-    const int c = min(c0 + (int)threadIdx.x, p.C - 1);
-    const float rate = p.rate[c], s = p.scale * semx::softplus(rate);
-    par[0][threadIdx.x] = s > 3.4e38f ? 3.4e38f : s;  // an infinite one times a closed gate is no number
-    par[1][threadIdx.x] = p.r_bias != nullptr ? p.r_bias[c] : 0.f;
-    par[2][threadIdx.x] = p.i_bias != nullptr ? p.i_bias[c] : 0.f;
-    if (SLOPE) par[3][threadIdx.x] = p.scale * semx::softplus_grad(rate);
+// The rows that belong to no sequence, shared out over all threads: f(row, channel, channels).
+template <class F>
+__device__ __forceinline__ void unused_rows(const GlParams& p, F f) {
+  if (p.m.cu == nullptr) return;
+  const int64_t front = rows_begin(p.m), count = front + p.m.T - rows_end(p.m);
+  const int quads = (p.C + 3) / 4;
+  for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < count * quads; i += (int64_t)gridDim.x * kT) {
+    const int64_t r = i / quads;
+    const int c = (int)(i - r * quads) * 4;
+    f(r < front ? r : p.m.T - count + r, c, min(4, p.C - c));
   }
 }
-__device__ __forceinline__ Quad shared_quad(const float* row, int c) {
-  return quad(*reinterpret_cast<const float4*>(row + c));
-}
 
-// LINK: sequences of several tiles.
-template <int ACC, bool LINK>
-__global__ void __launch_bounds__(kT, 3) gated_lru_fwd_kernel(const GlParams p) {
+template <int ACC, int SEG, int OPS>
+struct Stage {
+  typename RawQuad<ACC>::type v[OPS][SEG][kT];
+};
+
+// LINK: sequences of several tiles, linked through global memory. Else: walked.
+template <int ACC, int SEG, bool LINK>
+__global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlParams p) {
   typedef typename RawQuad<ACC>::type Raw;
-  __shared__ __align__(16) float par[3][kCh];
+  extern __shared__ __align__(16) unsigned char raw[];
+  Stage<ACC, SEG, 4>& st = *reinterpret_cast<Stage<ACC, SEG, 4>*>(raw);
   __shared__ __align__(16) float mA[kSegs][kCh], mB[kSegs][kCh];
+  __shared__ __align__(16) Rates rates[2];
   __shared__ int ticket;
-  const int tid = threadIdx.x;
-  const int64_t tile = LINK ? take_tile(p, &ticket) : (int64_t)blockIdx.x;
-  const int64_t j = tile / p.ctiles;
-  const int ct = (int)(tile % p.ctiles), c0 = ct * kCh;
-  const int seg = tid / 16, lc = tid % 16 * 4, nn = min(4, p.C - c0 - lc);
-  const int64_t ch = nn > 0 ? c0 + lc : 0;
-  const Piece q = find_piece(p.m, j);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const int seg = tid / (kCh / 4), lc = tid % (kCh / 4) * 4;
   const bool gated = p.z != nullptr;
-  if (seg == 0 && nn > 0)
-    for_unused_rows(p.m, j, [&](int64_t row) {
-      store_quad<ACC>(p.y, row * p.C + ch, p.bf16, nn, make_float4(0.f, 0.f, 0.f, 0.f));
-    });
-  if (!q.live) {
-    if (LINK && tid < 2) store_flag(p.flags + (j * p.ctiles + ct) * 2 + tid, 2);
-    return;
+  int n = blockIdx.x;
+  if (LINK) {
+    if (tid == 0) ticket = atomicAdd(p.ticket, 1);
+    __syncthreads();
+    n = ticket;
+    __syncthreads();
   }
-  const int t0 = q.t0 + seg * kSeg;
-  Raw rx[kSeg], rr[kSeg], ri[kSeg], rz[kSeg];
+  auto fetch = [&](const Tile& w) {  // the thread's own rows, on their way into its own places
+    const int nn = p.C - w.ct * kCh - lc, most = min(w.n - seg * SEG, SEG);
+    const int64_t ch = nn > 0 ? w.ct * kCh + lc : 0, row = most > 0 ? w.row + seg * SEG : 0;
+    auto bring = [&](int op, const void* from, int64_t ld) {
+      int64_t at = row * ld + ch;
 #pragma unroll
-  for (int u = 0; u < kSeg; ++u) {
-    rx[u] = rr[u] = ri[u] = rz[u] = Raw{};
-    if (t0 + u < q.t1 && nn > 0) {
-      const int64_t row = q.row0 + t0 + u;
-      rr[u] = load_quad<ACC>(p.r, row * p.ldr + ch, p.bf16, nn);
-      ri[u] = load_quad<ACC>(p.i, row * p.ldi + ch, p.bf16, nn);
-      rx[u] = load_quad<ACC>(p.x, row * p.ldx + ch, p.bf16, nn);
-      if (gated) rz[u] = load_quad<ACC>(p.z, row * p.ldz + ch, p.bf16, nn);
+      for (int u = 0; u < SEG; ++u, at += ld) {
+        const bool in = u < most && nn > 0;
+        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(from, at, p.bf16, in ? min(nn, 4) : 0);
+        else copy_quad<ACC>(&st.v[op][u][tid], from, at, in);
+      }
+    };
+    bring(0, p.x, p.ldx);
+    bring(1, p.r, p.ldr);
+    bring(2, p.i, p.ldi);
+    if (gated) bring(3, p.z, p.ldz);
+  };
+  int step = 0, turn = 0;
+  constexpr int Q = kSegs * SEG;
+  Tile w = tile_at<LINK, false, Q>(p, n, 0);
+  fetch(w);
+  if (w.any && warp == 1) load_rates(p, w.ct, lane, &rates[0]);
+  unused_rows(p, [&](int64_t row, int c, int k) {
+    store_quad<ACC>(p.y, row * p.C + c, p.bf16, k, make_float4(0.f, 0.f, 0.f, 0.f));
+  });
+  float carry = 0.f;  // warp 0: the walked sequence's state
+  while (w.any) {
+    const int c0 = w.ct * kCh, nn = min(4, p.C - c0 - lc);
+    const bool first = w.k == 0, last = w.k + 1 >= w.tiles;
+    int64_t slot = semx::kNone;
+    if (p.m.n_slots > 0 && w.live && (first || last)) slot = find_slot(p.m, w.s);
+    if (LINK && tid == 0) ticket = atomicAdd(p.ticket, 1);
+    __syncthreads();  // rates; the maps of the tile before have been read
+    const Rates& rt = rates[turn];
+    f2 a[SEG][2], b[SEG][2];
+    f2 A[2] = {both(1.f), both(1.f)}, B[2] = {both(0.f), both(0.f)};
+    Raw rz[SEG];
+    copies_done();
+    const int most = w.n - seg * SEG;  // steps of the thread that exist
+    if (warp * (kSegs / 4) * SEG < w.n) {
+      const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[lc]);
+      const bool slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+#pragma unroll
+      for (int u = 0; u < SEG; ++u) {
+        const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid];
+        if (gated) rz[u] = st.v[3][u][tid];
+        else rz[u] = Raw{};
+        const bool in = u < most;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
+          f2 rho, m, gain;
+          decay2(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h), shared_pair(rt.root, lc + 2 * h), slow,
+                 &rho, &m, &a[u][h], &gain);
+          const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
+          b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
+          if (!in) a[u][h] = both(1.f), b[u][h] = both(0.f);  // rows behind the last one keep the state
+          A[h] = mul2(A[h], a[u][h]);
+          B[h] = fma2(a[u][h], B[h], b[u][h]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < SEG; ++u) {
+        rz[u] = Raw{};
+        a[u][0] = a[u][1] = both(1.f);
+        b[u][0] = b[u][1] = both(0.f);
+      }
     }
-  }
-  tile_params<false>(p, c0, par);
-  const bool first = q.k == 0, last = q.t1 == q.len;
-  int64_t slot = semx::kNone;
-  if (p.m.n_slots > 0 && (first || last)) slot = find_slot(p.m, q.s);
-  __syncthreads();
-  const Quad speed = shared_quad(par[0], lc), rb = shared_quad(par[1], lc), ib = shared_quad(par[2], lc);
-  const bool slow = fmaxf(fmaxf(speed.v[0], speed.v[1]), fmaxf(speed.v[2], speed.v[3])) <= 0.35f;
-  float a[kSeg][4], b[kSeg][4];
-  float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < kSeg; ++u) {
-    const Quad x = quad(quad_floats<ACC>(rx[u], p.bf16)), r = quad(quad_floats<ACC>(rr[u], p.bf16)),
-               i = quad(quad_floats<ACC>(ri[u], p.bf16));
-    const bool in = t0 + u < q.t1;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float left;
-      decay(-speed.v[k] * sigmoid(r.v[k] + rb.v[k]), slow, &a[u][k], &left);
-      left = left < kLeast ? kLeast : left;
-      b[u][k] = left * semx::rsqrt_approx(left) * sigmoid(i.v[k] + ib.v[k]) * x.v[k];
-      if (!in) a[u][k] = 1.f, b[u][k] = 0.f;  // rows behind the last one keep the state
-      A[k] *= a[u][k];
-      B[k] = fmaf(a[u][k], B[k], b[u][k]);
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<f2*>(&mA[seg][lc + 2 * h]) = A[h];
+      *reinterpret_cast<f2*>(&mB[seg][lc + 2 * h]) = B[h];
     }
-  }
-  *reinterpret_cast<float4*>(&mA[seg][lc]) = make_float4(A[0], A[1], A[2], A[3]);
-  *reinterpret_cast<float4*>(&mB[seg][lc]) = make_float4(B[0], B[1], B[2], B[3]);
-  __syncthreads();
-  if (tid < kCh) {
-    const int c = c0 + tid;
+    __syncthreads();
+    // The next tile's rows set out while this one's state is on its way.
+    if (LINK) {
+      n = ticket;
+    } else if (++step == w.tiles) {
+      step = 0;
+      n += gridDim.x;
+    }
+    const int c = c0 + lane;
     const bool ok = c < p.C;
+    const Chain link = {w.j - w.k, 1, w.k};
     float h = 0.f;
-    if (first && ok && slot != semx::kNone) {
-      const bool fresh = p.m.fresh != nullptr && p.m.fresh[q.s] != 0;
-      h = slot == semx::kRefused ? __int_as_float(0x7fffffff) : fresh ? 0.f : p.state[slot * p.C + c];
+    if (warp == 0) {
+      if (first && ok && slot != semx::kNone) {
+        const bool fresh = p.m.fresh != nullptr && p.m.fresh[w.s] != 0;
+        h = slot == semx::kRefused ? __int_as_float(0x7fffffff) : fresh ? 0.f : p.state[slot * p.C + c];
+      }
+      if (LINK && ok) {
+        float fA = 1.f, fB = h;
+#pragma unroll
+        for (int s = 0; s < kSegs; ++s) {
+          fA *= mA[s][lane];
+          fB = fmaf(mA[s][lane], fB, mB[s][lane]);
+        }
+        leave_map(p, w.j, c, first ? 0.f : fA, fB);
+      }
     }
-    Chain link = {j - q.k, 1, q.k, !last};
-    if (LINK && q.len > p.m.Q) {
-      float fA = 1.f, fB = h;
+    const Tile next = tile_at<LINK, false, Q>(p, n, step);
+    fetch(next);
+    const bool other = next.any && next.ct != w.ct;
+    if (other && warp == 1) load_rates(p, next.ct, lane, &rates[turn ^ 1]);
+    if (warp == 0) {
+      if (!first) h = !LINK ? carry : w.live ? link_in(p, link, c, ok) : 0.f;
+      if (p.ckpt != nullptr && ok && w.live) p.ckpt[(int64_t)w.j * p.C + c] = h;
 #pragma unroll
       for (int s = 0; s < kSegs; ++s) {
-        fA *= mA[s][tid];
-        fB = fmaf(mA[s][tid], fB, mB[s][tid]);
+        const float after = fmaf(mA[s][lane], h, mB[s][lane]);
+        mB[s][lane] = h;  // from here on the segment's entry state
+        h = after;
       }
-      const float in = link_in(p, link, ct, tid / 32, c, ok, first ? 0.f : fA, fB);
-      if (!first) h = in;
+      carry = h;
+      // Every tile leaves its state, so that nothing waits for long whatever the offsets are.
+      if (LINK && ok) leave_state(p, w.j, c, h);
+      if (w.live && last && ok && slot >= 0) p.state[slot * p.C + c] = h;
     }
-    if (p.ckpt != nullptr && ok) p.ckpt[j * p.C + c] = h;
+    __syncthreads();
+    f2 hs[2] = {shared_pair(mB[seg], lc), shared_pair(mB[seg], lc + 2)};
+    const int64_t out = (w.row + seg * SEG) * p.C + c0 + lc;
 #pragma unroll
-    for (int s = 0; s < kSegs; ++s) {
-      const float next = fmaf(mA[s][tid], h, mB[s][tid]);
-      mB[s][tid] = h;  // from here on the segment's entry state
-      h = next;
+    for (int u = 0; u < SEG; ++u) {
+      f2 y[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        hs[k] = fma2(a[u][k], hs[k], b[u][k]);
+        y[k] = hs[k];
+        if (gated) {
+          const f2 z = pair_of<ACC>(rz[u], k, p.bf16);
+          const f2 s = rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)));
+          y[k] = mul2(y[k], mul2(z, s));
+        }
+      }
+      if (u < most && nn > 0) {
+        const float2 lo = unpack2(y[0]), hi = unpack2(y[1]);
+        store_quad<ACC>(p.y, out + u * p.C, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
+      }
     }
-    if (LINK) link_out(p, link, ct, tid / 32, c, ok, h);
-    if (last && ok && slot >= 0) p.state[slot * p.C + c] = h;
-  }
-  __syncthreads();
-  Quad h = shared_quad(mB[seg], lc);
-#pragma unroll
-  for (int u = 0; u < kSeg; ++u) {
-    Quad y;
-    const Quad z = quad(quad_floats<ACC>(rz[u], p.bf16));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h.v[k] = fmaf(a[u][k], h.v[k], b[u][k]);
-      y.v[k] = gated ? h.v[k] * (z.v[k] * sigmoid(z.v[k])) : h.v[k];
-    }
-    if (t0 + u < q.t1 && nn > 0)
-      store_quad<ACC>(p.y, (q.row0 + t0 + u) * p.C + ch, p.bf16, nn, make_float4(y.v[0], y.v[1], y.v[2], y.v[3]));
+    w = next;
+    turn ^= other;
   }
 }
 
-template <int ACC, bool LINK>
-__global__ void __launch_bounds__(kT, 2) gated_lru_bwd_kernel(const GlParams p) {
+template <int ACC, int SEG, bool LINK>
+__global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlParams p) {
   typedef typename RawQuad<ACC>::type Raw;
-  __shared__ __align__(16) float par[4][kCh];
+  extern __shared__ __align__(16) unsigned char raw[];
+  Stage<ACC, SEG, 5>* stages = reinterpret_cast<Stage<ACC, SEG, 5>*>(raw);  // this tile's and the next one's
   __shared__ __align__(16) float mA[kSegs][kCh], mB[kSegs][kCh], mG[kSegs][kCh];
+  __shared__ __align__(16) Rates rates[2];
   __shared__ int ticket;
-  const int tid = threadIdx.x;
-  const int64_t total = p.m.pieces * p.ctiles;
-  const int64_t tile = LINK ? total - 1 - take_tile(p, &ticket) : (int64_t)blockIdx.x;
-  const int64_t j = tile / p.ctiles;
-  const int ct = (int)(tile % p.ctiles), c0 = ct * kCh;
-  const int seg = tid / 16, lc = tid % 16 * 4, nn = min(4, p.C - c0 - lc);
-  const int64_t ch = nn > 0 ? c0 + lc : 0;
-  const Piece q = find_piece(p.m, j);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const int seg = tid / (kCh / 4), lc = tid % (kCh / 4) * 4;
   const bool gated = p.z != nullptr;
-  if (seg == 0 && nn > 0)
-    for_unused_rows(p.m, j, [&](int64_t row) {
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-      store_quad<ACC>(p.dx, row * p.C + ch, p.bf16, nn, zero);
-      store_quad<ACC>(p.dr, row * p.C + ch, p.bf16, nn, zero);
-      store_quad<ACC>(p.di, row * p.C + ch, p.bf16, nn, zero);
-      if (gated) store_quad<ACC>(p.dz, row * p.C + ch, p.bf16, nn, zero);
-    });
-  if (!q.live || q.len == 0) {
-    if (LINK && tid < 2) store_flag(p.flags + (j * p.ctiles + ct) * 2 + tid, 2);
-    if (p.part != nullptr && tid < kCh && c0 + tid < p.C)
-      for (int n = 0; n < 3; ++n) p.part[(j * 3 + n) * p.C + c0 + tid] = 0.f;
-    return;
+  int n = blockIdx.x;
+  if (LINK) {
+    if (tid == 0) ticket = atomicAdd(p.ticket, 1);
+    __syncthreads();
+    n = ticket;
+    __syncthreads();
   }
-  const int t0 = q.t0 + seg * kSeg;
-  Raw rx[kSeg], rr[kSeg], ri[kSeg], rz[kSeg], rg[kSeg];
+  auto fetch = [&](const Tile& w, Stage<ACC, SEG, 5>& st) {  // the thread's own rows, on their way into its own places
+    const int nn = p.C - w.ct * kCh - lc, most = min(w.n - seg * SEG, SEG);
+    const int64_t ch = nn > 0 ? w.ct * kCh + lc : 0, row = most > 0 ? w.row + seg * SEG : 0;
+    auto bring = [&](int op, const void* from, int64_t ld) {
+      int64_t at = row * ld + ch;
 #pragma unroll
-  for (int u = 0; u < kSeg; ++u) {
-    rx[u] = rr[u] = ri[u] = rz[u] = rg[u] = Raw{};
-    if (t0 + u < q.t1 && nn > 0) {
-      const int64_t row = q.row0 + t0 + u;
-      rr[u] = load_quad<ACC>(p.r, row * p.ldr + ch, p.bf16, nn);
-      ri[u] = load_quad<ACC>(p.i, row * p.ldi + ch, p.bf16, nn);
-      rx[u] = load_quad<ACC>(p.x, row * p.ldx + ch, p.bf16, nn);
-      if (gated) rz[u] = load_quad<ACC>(p.z, row * p.ldz + ch, p.bf16, nn);
-      rg[u] = load_quad<ACC>(p.dy, row * p.C + ch, p.bf16, nn);
+      for (int u = 0; u < SEG; ++u, at += ld) {
+        const bool in = u < most && nn > 0;
+        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(from, at, p.bf16, in ? min(nn, 4) : 0);
+        else copy_quad<ACC>(&st.v[op][u][tid], from, at, in);
+      }
+    };
+    bring(0, p.x, p.ldx);
+    bring(1, p.r, p.ldr);
+    bring(2, p.i, p.ldi);
+    bring(4, p.dy, p.C);
+    if (gated) bring(3, p.z, p.ldz);
+  };
+  int step = 0, turn = 0, at = 0;
+  constexpr int Q = kSegs * SEG;
+  Tile w = tile_at<LINK, true, Q>(p, n, 0);
+  fetch(w, stages[0]);
+  if (w.any && warp == 1) load_rates(p, w.ct, lane, &rates[0]);
+  unused_rows(p, [&](int64_t row, int c, int k) {
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    store_quad<ACC>(p.dx, row * p.C + c, p.bf16, k, zero);
+    store_quad<ACC>(p.dr, row * p.C + c, p.bf16, k, zero);
+    store_quad<ACC>(p.di, row * p.C + c, p.bf16, k, zero);
+    if (gated) store_quad<ACC>(p.dz, row * p.C + c, p.bf16, k, zero);
+  });
+  float carry = 0.f;  // warp 0: what reaches the walked sequence's tile from behind
+  f2 sum[3][2];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) sum[k][0] = sum[k][1] = both(0.f);
+  while (w.any) {
+    const int c0 = w.ct * kCh, nn = min(4, p.C - c0 - lc);
+    const bool end = w.k + 1 >= w.tiles;  // nothing behind it
+    const bool busy = warp * (kSegs / 4) * SEG < w.n;
+    const int most = w.n - seg * SEG;  // steps of the thread that exist
+    if (LINK && tid == 0) ticket = atomicAdd(p.ticket, 1);
+    const float entry = warp == 0 && w.live && c0 + lane < p.C ? p.ckpt[(int64_t)w.j * p.C + c0 + lane] : 0.f;
+    __syncthreads();  // rates; the maps of the tile before have been read
+    const Rates& rt = rates[turn];
+    const Stage<ACC, SEG, 5>& st = stages[at];
+    const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[lc]);
+    const bool slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+    // b: gain iota x, later the state in front of the step; d: the gradient that reaches h from y.
+    f2 a[SEG][2], b[SEG][2], d[SEG][2];
+    f2 A[2] = {both(1.f), both(1.f)}, B[2] = {both(0.f), both(0.f)}, G[2] = {both(0.f), both(0.f)};
+    copies_done();
+    if (busy) {
+#pragma unroll
+      for (int u = 0; u < SEG; ++u) {
+        const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
+        const bool in = u < most;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
+          f2 rho, m, gain;
+          decay2(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h), shared_pair(rt.root, lc + 2 * h), slow,
+                 &rho, &m, &a[u][h], &gain);
+          const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
+          b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
+          d[u][h] = pair_of<ACC>(rg, h, p.bf16);
+          if (gated) {
+            const f2 z = pair_of<ACC>(st.v[3][u][tid], h, p.bf16);
+            const f2 s = rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)));
+            d[u][h] = mul2(d[u][h], mul2(z, s));
+          }
+          if (!in) a[u][h] = both(1.f), b[u][h] = d[u][h] = both(0.f);
+          A[h] = mul2(A[h], a[u][h]);
+          B[h] = fma2(a[u][h], B[h], b[u][h]);
+        }
+      }
+      // What reaches the step in front of the segment: a_t (d_t + what reaches step t from behind).
+#pragma unroll
+      for (int u = SEG - 1; u >= 0; --u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) G[h] = mul2(a[u][h], add2(d[u][h], G[h]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < SEG; ++u) {
+        a[u][0] = a[u][1] = both(1.f);
+        b[u][0] = b[u][1] = d[u][0] = d[u][1] = both(0.f);
+      }
     }
-  }
-  tile_params<true>(p, c0, par);
-  __syncthreads();
-  const Quad speed = shared_quad(par[0], lc), rb = shared_quad(par[1], lc), ib = shared_quad(par[2], lc);
-  const bool slow = fmaxf(fmaxf(speed.v[0], speed.v[1]), fmaxf(speed.v[2], speed.v[3])) <= 0.35f;
-  float a[kSeg][4], b[kSeg][4], d[kSeg][4];  // b: gain iota x; d: the gradient that reaches h from y
-  float A[4] = {1.f, 1.f, 1.f, 1.f}, B[4] = {0.f, 0.f, 0.f, 0.f}, G[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < kSeg; ++u) {
-    const Quad x = quad(quad_floats<ACC>(rx[u], p.bf16)), r = quad(quad_floats<ACC>(rr[u], p.bf16)),
-               i = quad(quad_floats<ACC>(ri[u], p.bf16)), z = quad(quad_floats<ACC>(rz[u], p.bf16)),
-               dy = quad(quad_floats<ACC>(rg[u], p.bf16));
-    const bool in = t0 + u < q.t1;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float left;
-      decay(-speed.v[k] * sigmoid(r.v[k] + rb.v[k]), slow, &a[u][k], &left);
-      left = left < kLeast ? kLeast : left;
-      b[u][k] = left * semx::rsqrt_approx(left) * sigmoid(i.v[k] + ib.v[k]) * x.v[k];
-      d[u][k] = gated ? dy.v[k] * (z.v[k] * sigmoid(z.v[k])) : dy.v[k];
-      if (!in) a[u][k] = 1.f, b[u][k] = 0.f;
-      A[k] *= a[u][k];
-      B[k] = fmaf(a[u][k], B[k], b[u][k]);
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<f2*>(&mA[seg][lc + 2 * h]) = A[h];
+      *reinterpret_cast<f2*>(&mB[seg][lc + 2 * h]) = B[h];
+      *reinterpret_cast<f2*>(&mG[seg][lc + 2 * h]) = G[h];
     }
-  }
-  // What reaches the step in front of the segment: a_t (d_t + what reaches step t from behind).
-#pragma unroll
-  for (int u = kSeg - 1; u >= 0; --u)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) G[k] = a[u][k] * (d[u][k] + G[k]);
-  *reinterpret_cast<float4*>(&mA[seg][lc]) = make_float4(A[0], A[1], A[2], A[3]);
-  *reinterpret_cast<float4*>(&mB[seg][lc]) = make_float4(B[0], B[1], B[2], B[3]);
-  *reinterpret_cast<float4*>(&mG[seg][lc]) = make_float4(G[0], G[1], G[2], G[3]);
-  __syncthreads();
-  if (tid < kCh) {
-    const int c = c0 + tid;
-    const bool ok = c < p.C;
-    float h = ok ? p.ckpt[j * p.C + c] : 0.f, g = 0.f;
+    __syncthreads();
     if (LINK) {
-      const int tiles = (int)((q.len + p.m.Q - 1) / p.m.Q);
-      const Chain link = {j - q.k + tiles - 1, -1, tiles - 1 - q.k, q.k > 0};
-      float fA = 1.f, fG = 0.f;
+      n = ticket;
+    } else if (++step == w.tiles) {
+      step = 0;
+      n += gridDim.x;
+    }
+    const int c = c0 + lane;
+    const bool ok = c < p.C;
+    const Chain link = {w.j - w.k + w.tiles - 1, -1, w.tiles - 1 - w.k};
+    float fA = 1.f, fG = 0.f;
+    if (LINK && warp == 0) {
 #pragma unroll
       for (int s = kSegs - 1; s >= 0; --s) {
-        fA *= mA[s][tid];
-        fG = fmaf(mA[s][tid], fG, mG[s][tid]);
+        fA *= mA[s][lane];
+        fG = fmaf(mA[s][lane], fG, mG[s][lane]);
       }
-      if (tiles > 1) g = link_in(p, link, ct, tid / 32, c, ok, link.at == 0 ? 0.f : fA, fG);
-      link_out(p, link, ct, tid / 32, c, ok, fmaf(fA, g, fG));
+      if (ok) leave_map(p, w.j, c, end ? 0.f : fA, fG);
     }
+    const Tile next = tile_at<LINK, true, Q>(p, n, step);
+    fetch(next, stages[at ^ 1]);
+    const bool other = next.any && next.ct != w.ct;
+    if (other && warp == 1) load_rates(p, next.ct, lane, &rates[turn ^ 1]);
+    if (warp == 0) {
+      float h = entry;
 #pragma unroll
-    for (int s = 0; s < kSegs; ++s) {
-      const float next = fmaf(mA[s][tid], h, mB[s][tid]);
-      mB[s][tid] = h;
-      h = next;
-    }
-#pragma unroll
-    for (int s = kSegs - 1; s >= 0; --s) {
-      const float next = fmaf(mA[s][tid], g, mG[s][tid]);
-      mG[s][tid] = g;  // from here on what reaches the segment's last step from behind
-      g = next;
-    }
-  }
-  __syncthreads();
-  {
-    Quad h = shared_quad(mB[seg], lc);
-#pragma unroll
-    for (int u = 0; u < kSeg; ++u)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float next = fmaf(a[u][k], h.v[k], b[u][k]);
-        b[u][k] = h.v[k];  // from here on h_{t-1}
-        h.v[k] = next;
+      for (int s = 0; s < kSegs; ++s) {
+        const float after = fmaf(mA[s][lane], h, mB[s][lane]);
+        mB[s][lane] = h;
+        h = after;
       }
-  }
-  Quad g = shared_quad(mG[seg], lc);
-  float sum[3][4] = {};
+      float g = end ? 0.f : !LINK ? carry : w.live ? link_in(p, link, c, ok) : 0.f;
+      if (LINK && ok) leave_state(p, w.j, c, fmaf(fA, g, fG));
 #pragma unroll
-  for (int u = kSeg - 1; u >= 0; --u) {
-    const Quad x = quad(quad_floats<ACC>(rx[u], p.bf16)), r = quad(quad_floats<ACC>(rr[u], p.bf16)),
-               i = quad(quad_floats<ACC>(ri[u], p.bf16)), z = quad(quad_floats<ACC>(rz[u], p.bf16)),
-               dy = quad(quad_floats<ACC>(rg[u], p.bf16));
-    const bool in = t0 + u < q.t1;
-    Quad dx, dr, di, dz;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float gt = d[u][k] + g.v[k];
-      float rho, shut_r, iota, shut_i;
-      sigmoids(r.v[k] + rb.v[k], &rho, &shut_r);
-      sigmoids(i.v[k] + ib.v[k], &iota, &shut_i);
-      float at, left;
-      decay(-speed.v[k] * rho, slow, &at, &left);
-      const bool open = left > kLeast;
-      left = left < kLeast ? kLeast : left;
-      const float inv = semx::rsqrt_approx(left), gain = left * inv;
-      const float ah = at * b[u][k];
-      if (gated) {
-        float s, rest;
-        sigmoids(z.v[k], &s, &rest);
-        const float h = fmaf(gain * iota, x.v[k], ah);
-        dz.v[k] = dy.v[k] * h * (s * fmaf(z.v[k], rest, 1.f));
+      for (int s = kSegs - 1; s >= 0; --s) {
+        const float before = fmaf(mA[s][lane], g, mG[s][lane]);
+        mG[s][lane] = g;  // from here on what reaches the segment's last step from behind
+        g = before;
       }
-      const float gi = gt * iota;
-      dx.v[k] = gi * gain;
-      di.v[k] = dx.v[k] * x.v[k] * shut_i;
-      const float dla = gt * ah - (open ? gi * x.v[k] * (at * at) * inv : 0.f);
-      dr.v[k] = -speed.v[k] * dla * rho * shut_r;
-      g.v[k] = in ? at * gt : g.v[k];
-      if (in) {
-        sum[0][k] = fmaf(rho, dla, sum[0][k]);
-        sum[1][k] += dr.v[k];
-        sum[2][k] += di.v[k];
+      carry = g;
+    }
+    __syncthreads();
+    if (busy) {
+      f2 hs[2] = {shared_pair(mB[seg], lc), shared_pair(mB[seg], lc + 2)};
+#pragma unroll
+      for (int u = 0; u < SEG; ++u)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const f2 after = fma2(a[u][k], hs[k], b[u][k]);
+          b[u][k] = hs[k];
+          hs[k] = after;
+        }
+      const int64_t out = (w.row + seg * SEG) * p.C + c0 + lc;
+      f2 gs[2] = {shared_pair(mG[seg], lc), shared_pair(mG[seg], lc + 2)};
+#pragma unroll
+      for (int u = SEG - 1; u >= 0; --u) {
+        const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
+        const bool in = u < most;
+        f2 dx[2], dr[2], di[2], dz[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const f2 x = pair_of<ACC>(rx, k, p.bf16), speed = shared_pair(rt.speed, lc + 2 * k);
+          const f2 gt = add2(d[u][k], gs[k]);
+          const f2 er = ex2_2(end2(gate_arg(pair_of<ACC>(rr, k, p.bf16), shared_pair(rt.r2, lc + 2 * k))));
+          const f2 er1 = add2(er, both(1.f)), qr = rsqrt_2(er1);
+          f2 rho, m, at, gain;
+          decay2(qr, speed, shared_pair(rt.root, lc + 2 * k), slow, &rho, &m, &at, &gain);
+          // 1 / gain: 1 / q = (1 + er) q.
+          f2 inv = mul2(mul2(mul2(er1, qr), shared_pair(rt.inverse, lc + 2 * k)), inverse_root_near(m));
+          float2 gg = unpack2(gain), iv = unpack2(inv);
+          if (!slow) {
+            const float2 mm = unpack2(m);
+            if (mm.x > kNear) iv.x = 1.f / gg.x;
+            if (mm.y > kNear) iv.y = 1.f / gg.y;
+          }
+          iv.x = gg.x > kLeastGain ? iv.x : 0.f;  // at its least value no gradient goes through the gain
+          iv.y = gg.y > kLeastGain ? iv.y : 0.f;
+          inv = pack2(iv.x, iv.y);
+          gain = least2(gain);
+          const f2 ei = ex2_2(end2(gate_arg(pair_of<ACC>(ri, k, p.bf16), shared_pair(rt.i2, lc + 2 * k))));
+          const f2 iota = rcp_2(add2(ei, both(1.f)));
+          const f2 ah = mul2(a[u][k], b[u][k]);
+          if (gated) {
+            const f2 z = pair_of<ACC>(st.v[3][u][tid], k, p.bf16);
+            const f2 ez = ex2_2(end2(mul2(z, both(-kLog2e)))), s = rcp_2(add2(ez, both(1.f)));
+            const f2 h = fma2(mul2(gain, iota), x, ah);
+            // silu'(z) = s (1 + z (1 - s)), 1 - s = ez s
+            dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, mul2(ez, s), both(1.f))));
+          }
+          const f2 gi = mul2(gt, iota);
+          dx[k] = mul2(gi, gain);
+          di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
+          const f2 through = mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv));
+          const f2 dla = fma2(gt, ah, mul2(through, both(-1.f)));
+          const f2 rd = mul2(rho, dla);
+          dr[k] = mul2(mul2(rd, mul2(er, rho)), mul2(speed, both(-1.f)));
+          gs[k] = mul2(a[u][k], gt);
+          if (in) {
+            sum[0][k] = add2(sum[0][k], rd);
+            sum[1][k] = add2(sum[1][k], dr[k]);
+            sum[2][k] = add2(sum[2][k], di[k]);
+          }
+        }
+        if (in && nn > 0) {
+          const int64_t o = out + u * p.C;
+          auto put = [&](void* to, const f2 (&v)[2]) {
+            const float2 lo = unpack2(v[0]), hi = unpack2(v[1]);
+            store_quad<ACC>(to, o, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
+          };
+          put(p.dx, dx);
+          put(p.dr, dr);
+          put(p.di, di);
+          if (gated) put(p.dz, dz);
+        }
       }
     }
-    if (in && nn > 0) {
-      const int64_t o = (q.row0 + t0 + u) * p.C + ch;
-      store_quad<ACC>(p.dx, o, p.bf16, nn, make_float4(dx.v[0], dx.v[1], dx.v[2], dx.v[3]));
-      store_quad<ACC>(p.dr, o, p.bf16, nn, make_float4(dr.v[0], dr.v[1], dr.v[2], dr.v[3]));
-      store_quad<ACC>(p.di, o, p.bf16, nn, make_float4(di.v[0], di.v[1], di.v[2], di.v[3]));
-      if (gated) store_quad<ACC>(p.dz, o, p.bf16, nn, make_float4(dz.v[0], dz.v[1], dz.v[2], dz.v[3]));
-    }
-  }
-  if (p.part == nullptr) return;
-  __syncthreads();
-  *reinterpret_cast<float4*>(&mA[seg][lc]) = make_float4(sum[0][0], sum[0][1], sum[0][2], sum[0][3]);
-  *reinterpret_cast<float4*>(&mB[seg][lc]) = make_float4(sum[1][0], sum[1][1], sum[1][2], sum[1][3]);
-  *reinterpret_cast<float4*>(&mG[seg][lc]) = make_float4(sum[2][0], sum[2][1], sum[2][2], sum[2][3]);
-  __syncthreads();
-  if (tid < 3 * kCh) {
-    const int n = tid / kCh, k = tid % kCh;
-    float(*m)[kCh] = n == 0 ? mA : n == 1 ? mB : mG;
-    float acc = 0.f;
+    if (p.part != nullptr && (LINK || w.k == 0)) {
+      __syncthreads();
 #pragma unroll
-    for (int s = 0; s < kSegs; ++s) acc += m[s][k];
-    if (c0 + k < p.C) p.part[(j * 3 + n) * p.C + c0 + k] = n == 0 ? -par[3][k] * acc : acc;
+      for (int k = 0; k < 2; ++k) {
+        *reinterpret_cast<f2*>(&mA[seg][lc + 2 * k]) = sum[0][k];
+        *reinterpret_cast<f2*>(&mB[seg][lc + 2 * k]) = sum[1][k];
+        *reinterpret_cast<f2*>(&mG[seg][lc + 2 * k]) = sum[2][k];
+        sum[0][k] = sum[1][k] = sum[2][k] = both(0.f);
+      }
+      __syncthreads();
+      if (warp < 3 && ok) {
+        float(*m)[kCh] = warp == 0 ? mA : warp == 1 ? mB : mG;
+        float acc = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSegs; ++s) acc += m[s][lane];
+        const int64_t row = LINK ? w.j : w.s;
+        p.part[(row * 3 + warp) * p.C + c] = warp == 0 ? -rt.slope[lane] * acc : acc;
+      }
+    }
+    w = next;
+    turn ^= other;
+    at ^= 1;
   }
 }
 
@@ -510,14 +779,15 @@ __global__ void __launch_bounds__(kStepT) gated_lru_step_kernel(const GlParams p
   const int n = (int)min((int64_t)rows, p.m.S - s0);
   const int64_t c = ((int64_t)(blockIdx.x % p.ctiles) * kStepT + threadIdx.x) * 4;
   const int nn = (int)min((int64_t)4, p.C - c);
-  float speed[4] = {}, rb[4] = {}, ib[4] = {};
+  float speed[4] = {}, root[4] = {}, r2[4] = {}, i2[4] = {};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < nn) {
       const float s = p.scale * semx::softplus(p.rate[c + k]);
-      speed[k] = s > 3.4e38f ? 3.4e38f : s;
-      if (p.r_bias != nullptr) rb[k] = p.r_bias[c + k];
-      if (p.i_bias != nullptr) ib[k] = p.i_bias[c + k];
+      speed[k] = s > 1e37f ? 1e37f : s;
+      root[k] = sqrtf(2.f * speed[k]);
+      if (p.r_bias != nullptr) r2[k] = -kLog2e * p.r_bias[c + k];
+      if (p.i_bias != nullptr) i2[k] = -kLog2e * p.i_bias[c + k];
     }
   semx::find_slots<kStepRows>(p.m, s0, n, slots);
   if (nn <= 0) return;
@@ -540,26 +810,26 @@ __global__ void __launch_bounds__(kStepT) gated_lru_step_kernel(const GlParams p
     for (int u = 0; u < kAhead; ++u)
       if (n0 + u < n) {
         const int64_t s = s0 + n0 + u, slot = slots[n0 + u];
-        const Quad x = quad(quad_floats<ACC>(rx[u], p.bf16)), r = quad(quad_floats<ACC>(rr[u], p.bf16)),
-                   i = quad(quad_floats<ACC>(ri[u], p.bf16));
-        Quad h = quad(old[u]), y;
+        const float4 o = old[u];
+        f2 hs[2] = {pack2(o.x, o.y), pack2(o.z, o.w)}, ys[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float a, left;
-          decay(-speed[k] * sigmoid(r.v[k] + rb[k]), false, &a, &left);
-          left = left < kLeast ? kLeast : left;
-          h.v[k] = fmaf(a, h.v[k], left * semx::rsqrt_approx(left) * sigmoid(i.v[k] + ib[k]) * x.v[k]);
-          if (slot == semx::kRefused) h.v[k] = __int_as_float(0x7fffffff);
-          y.v[k] = h.v[k];
+        for (int k = 0; k < 2; ++k) {
+          const f2 q = rsqrt_2(add2(ex2_2(gate_arg(pair_of<ACC>(rr[u], k, p.bf16), pack2(r2[2 * k], r2[2 * k + 1]))), both(1.f)));
+          f2 rho, m, a, gain;
+          decay2(q, pack2(speed[2 * k], speed[2 * k + 1]), pack2(root[2 * k], root[2 * k + 1]), false, &rho, &m, &a, &gain);
+          const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri[u], k, p.bf16), pack2(i2[2 * k], i2[2 * k + 1]))), both(1.f)));
+          hs[k] = fma2(a, hs[k], mul2(mul2(iota, pair_of<ACC>(rx[u], k, p.bf16)), least2(gain)));
+          if (slot == semx::kRefused) hs[k] = both(__int_as_float(0x7fffffff));
+          ys[k] = hs[k];
+          if (p.z != nullptr) {
+            const f2 z = pair_of<ACC>(rz[u], k, p.bf16);
+            ys[k] = mul2(ys[k], mul2(z, rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)))));
+          }
         }
-        if (p.z != nullptr) {
-          const Quad z = quad(quad_floats<ACC>(rz[u], p.bf16));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) y.v[k] *= z.v[k] * sigmoid(z.v[k]);
-        }
+        const float2 h0 = unpack2(hs[0]), h1 = unpack2(hs[1]), y0 = unpack2(ys[0]), y1 = unpack2(ys[1]);
         if (slot >= 0)
-          store_quad<F>(p.state, slot * p.C + c, 0, nn, make_float4(h.v[0], h.v[1], h.v[2], h.v[3]));
-        store_quad<ACC>(p.y, s * p.C + c, p.bf16, nn, make_float4(y.v[0], y.v[1], y.v[2], y.v[3]));
+          store_quad<F>(p.state, slot * p.C + c, 0, nn, make_float4(h0.x, h0.y, h1.x, h1.y));
+        store_quad<ACC>(p.y, s * p.C + c, p.bf16, nn, make_float4(y0.x, y0.y, y1.x, y1.y));
       }
   }
 }
@@ -588,7 +858,7 @@ int gl_validate(const SemxGatedLruArgs* a, bool bwd, GlParams* p) {
   SEMX_REQUIRE(semx::all_aligned({a->x, a->r, a->i, a->z, a->y, a->dy, a->dx, a->d_r, a->d_i, a->dz}, a->bf16 ? 2 : 4) &&
                    semx::all_aligned({a->rate, a->r_bias, a->i_bias, a->cu_seqlens, a->state, a->slots, a->ckpt,
                                       a->drate, a->dr_bias, a->di_bias}, 4) &&
-                   semx::aligned(a->workspace, 8),
+                   semx::aligned(a->workspace, 16),
                SEMX_ERR_ALIGN, "gated_lru: a pointer is not on an element");
   p->C = (int)a->C; p->bf16 = a->bf16; p->scale = a->rate_scale;
   p->ctiles = (int)semx::cdiv(a->C, (int64_t)kCh);
@@ -603,56 +873,65 @@ int gl_validate(const SemxGatedLruArgs* a, bool bwd, GlParams* p) {
       semx::all_aligned({a->x, a->r, a->i, a->z, a->y, a->dy, a->dx, a->d_r, a->d_i, a->dz}, a->bf16 ? 8 : 16) &&
       semx::aligned(a->state, 16))
     p->access = a->bf16 ? kBf16 : kFp32;
-  semx::set_pieces(&p->m, kRows);
+  semx::set_pieces(&p->m, kSegs * seg_steps(a->bf16 != 0));
   return SEMX_OK;
 }
 
-// Whether a sequence can have more than one tile.
-bool gl_linked(const GlParams& p) { return p.m.cu != nullptr ? p.m.T > kRows : p.m.L > kRows; }
-
-size_t round8(size_t n) { return (n + 7) / 8 * 8; }
-size_t link_ints(const GlParams& p) { return round8(1 + (size_t)p.m.pieces * p.ctiles * 2); }
-size_t link_bytes(const GlParams& p) {
-  return gl_linked(p) ? link_ints(p) * sizeof(int) + (size_t)p.m.pieces * p.C * (sizeof(float2) + sizeof(float)) : 0;
+// Whether tiles are linked: packed sequences, whose lengths the host does not know, and sequences too
+// few to give each SM four CTAs that walk them.
+bool gl_linked(const GlParams& p) {
+  if (p.m.cu != nullptr) return true;
+  return p.m.per > 1 && p.m.S * p.ctiles < kSms * 4;
 }
 
-// Lays the links into the workspace and clears ticket and flags.
+size_t link_bytes(const GlParams& p) {
+  return gl_linked(p) ? 16 + (size_t)p.m.pieces * p.C * (sizeof(ulonglong2) + sizeof(unsigned long long)) : 0;
+}
+int64_t part_rows(const GlParams& p) { return gl_linked(p) ? p.m.pieces : p.m.S; }
+
+// Lays the links into the workspace and clears them.
 int set_links(GlParams* p, void* workspace, cudaStream_t st) {
-  if (!gl_linked(*p)) return SEMX_OK;
+  const size_t bytes = link_bytes(*p);
+  if (bytes == 0) return SEMX_OK;
   SEMX_REQUIRE(workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_lru: workspace is NULL");
-  const size_t ints = link_ints(*p);
-  p->ticket = reinterpret_cast<int*>(workspace);
-  p->flags = p->ticket + 1;
-  p->maps = reinterpret_cast<float2*>(p->ticket + ints);
-  p->left = reinterpret_cast<float*>(p->maps + (size_t)p->m.pieces * p->C);
-  const cudaError_t e = cudaMemsetAsync(workspace, 0, ints * sizeof(int), st);
+  p->maps = reinterpret_cast<ulonglong2*>(workspace);
+  p->left = reinterpret_cast<unsigned long long*>(p->maps + (size_t)p->m.pieces * p->C);
+  p->ticket = reinterpret_cast<int*>(p->left + (size_t)p->m.pieces * p->C);
+  const cudaError_t e = cudaMemsetAsync(workspace, 0, bytes, st);
   SEMX_REQUIRE(e == cudaSuccess, SEMX_ERR_LAUNCH, "gated_lru: cudaMemsetAsync: %s", cudaGetErrorString(e));
   return SEMX_OK;
 }
 
-template <int ACC>
+template <int ACC, int SEG>
 int launch_gl(bool bwd, const GlParams& p, cudaStream_t st) {
-  const int64_t grid = p.m.pieces * p.ctiles;
-  if (grid == 0) return SEMX_OK;
-  if (grid >= ((int64_t)1 << 30)) return semx::fail(SEMX_ERR_SHAPE, "gated_lru: too many tiles");
-  const unsigned n = (unsigned)grid;
   const bool linked = p.ticket != nullptr;
-  if (!bwd) {
-    if (linked) gated_lru_fwd_kernel<ACC, true><<<n, kT, 0, st>>>(p);
-    else gated_lru_fwd_kernel<ACC, false><<<n, kT, 0, st>>>(p);
-    return semx::check_launch("gated_lru_fwd_kernel");
-  }
-  if (linked) gated_lru_bwd_kernel<ACC, true><<<n, kT, 0, st>>>(p);
-  else gated_lru_bwd_kernel<ACC, false><<<n, kT, 0, st>>>(p);
-  return semx::check_launch("gated_lru_bwd_kernel");
+  const int64_t works = (linked ? p.m.pieces : p.m.S) * p.ctiles;
+  if (works == 0) return SEMX_OK;
+  if (works >= ((int64_t)1 << 30)) return semx::fail(SEMX_ERR_SHAPE, "gated_lru: too many tiles");
+  // As many CTAs as run at once: each takes tile after tile, and fetches the next one's rows early.
+  const int64_t most = kSms * (bwd ? kBwdCtas : kFwdCtas);
+  const unsigned n = (unsigned)(works < most ? works : most);
+#define SEMX_GL(KERNEL, STAGES)                                      \
+  do {                                                               \
+    if (!semx::allow_smem(KERNEL, STAGES)) return SEMX_ERR_LAUNCH;   \
+    KERNEL<<<n, kT, STAGES, st>>>(p);                                \
+    return semx::check_launch("gated_lru kernel");                   \
+  } while (0)
+  constexpr size_t fwd = sizeof(Stage<ACC, SEG, 4>), back = 2 * sizeof(Stage<ACC, SEG, 5>);
+  if (!bwd && linked) SEMX_GL((gated_lru_fwd_kernel<ACC, SEG, true>), fwd);
+  if (!bwd) SEMX_GL((gated_lru_fwd_kernel<ACC, SEG, false>), fwd);
+  if (linked) SEMX_GL((gated_lru_bwd_kernel<ACC, SEG, true>), back);
+  SEMX_GL((gated_lru_bwd_kernel<ACC, SEG, false>), back);
+#undef SEMX_GL
 }
 
 int dispatch_gl(bool bwd, const GlParams& p, cudaStream_t st) {
-  if (p.access == kBf16) return launch_gl<kBf16>(bwd, p, st);
-  if (p.access == kFp32) return launch_gl<kFp32>(bwd, p, st);
-  return launch_gl<kAny>(bwd, p, st);
+  if (p.access == kBf16) return launch_gl<kBf16, seg_steps(true)>(bwd, p, st);
+  if (p.access == kFp32) return launch_gl<kFp32, seg_steps(false)>(bwd, p, st);
+  return p.bf16 ? launch_gl<kAny, seg_steps(true)>(bwd, p, st) : launch_gl<kAny, seg_steps(false)>(bwd, p, st);
 }
 
+// (The sizes do not depend on addresses.)
 GlParams gl_sizes(const SemxGatedLruArgs* a, bool bwd, int* rc) {
   SemxGatedLruArgs b = *a;
   float* any = reinterpret_cast<float*>(256);
@@ -664,6 +943,7 @@ GlParams gl_sizes(const SemxGatedLruArgs* a, bool bwd, int* rc) {
   b.ckpt = any;
   GlParams p = {};
   *rc = gl_validate(&b, bwd, &p);
+  if (p.m.S == 0 && p.m.T > 0 && p.m.pieces == 0) p.m.pieces = 1;
   return p;
 }
 
@@ -695,7 +975,7 @@ size_t semx_gated_lru_workspace_bytes(const SemxGatedLruArgs* a, int32_t backwar
   int rc;
   const GlParams p = gl_sizes(a, backward != 0, &rc);
   if (rc != SEMX_OK) return 0;
-  return link_bytes(p) + (backward != 0 ? (size_t)p.m.pieces * 3 * p.C * sizeof(float) : 0);
+  return link_bytes(p) + (backward != 0 ? (size_t)part_rows(p) * 3 * p.C * sizeof(float) : 0);
 }
 
 int semx_gated_lru_fwd(const SemxGatedLruArgs* a, semx_stream_t stream) {
@@ -707,10 +987,10 @@ int semx_gated_lru_fwd(const SemxGatedLruArgs* a, semx_stream_t stream) {
   rc = scope.bind({a->y, a->state});
   if (rc != SEMX_OK) return rc;
   cudaStream_t st = semx::as_stream(stream);
-  rc = set_links(&p, a->workspace, st);
-  if (rc != SEMX_OK) return rc;
   // Without a sequence every row is a row behind the last one.
   if (p.m.S == 0 && p.m.T > 0 && p.m.pieces == 0) p.m.pieces = 1;
+  rc = set_links(&p, a->workspace, st);
+  if (rc != SEMX_OK) return rc;
   return dispatch_gl(false, p, st);
 }
 
@@ -724,17 +1004,17 @@ int semx_gated_lru_bwd(const SemxGatedLruArgs* a, semx_stream_t stream) {
   rc = scope.bind({a->dx, a->drate, a->dr_bias, a->di_bias});
   if (rc != SEMX_OK) return rc;
   cudaStream_t st = semx::as_stream(stream);
+  int64_t rows = 0;
   if (p.m.T > 0) {
+    if (p.m.S == 0 && p.m.pieces == 0) p.m.pieces = 1;
     rc = set_links(&p, a->workspace, st);
     if (rc != SEMX_OK) return rc;
     if (params) {
       SEMX_REQUIRE(a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_lru bwd: workspace is NULL");
       p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + link_bytes(p));
+      rows = part_rows(p);
     }
-    const int64_t pieces = p.m.pieces;
-    if (p.m.S == 0 && pieces == 0) p.m.pieces = 1, p.part = nullptr;
     rc = dispatch_gl(true, p, st);
-    p.m.pieces = pieces;
     if (rc != SEMX_OK) return rc;
   }
   if (!params) return SEMX_OK;
@@ -744,7 +1024,7 @@ int semx_gated_lru_bwd(const SemxGatedLruArgs* a, semx_stream_t stream) {
   seg.out[1] = a->dr_bias;
   seg.out[2] = a->di_bias;
   seg.len[0] = seg.len[1] = seg.len[2] = a->C;
-  return semx::colsum_once(p.part, p.m.T > 0 ? p.m.pieces : 0, 3 * a->C, seg, st);
+  return semx::colsum_once(p.part, rows, 3 * a->C, seg, st);
 }
 
 int semx_gated_lru_step(const SemxGatedLruArgs* a, semx_stream_t stream) {

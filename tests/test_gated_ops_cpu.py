@@ -68,13 +68,18 @@ def test_recurrence_arguments_are_checked_on_the_host():
 def test_recurrence_sizes():
     lib = _lib.load()
     a = _lru_args()
-    assert lib.semx_gated_lru_ckpt_bytes(ctypes.byref(a)) == 2 * 2 * 12 * 4  # two tiles of 64 steps each
-    ints = 1 + 4 * 1 * 2
-    links = (ints + 7) // 8 * 8 * 4 + 4 * 12 * 12
+    # fp32: four tiles of 32 steps each, linked: a map (16 bytes) and a state (8) per tile and channel.
+    assert lib.semx_gated_lru_ckpt_bytes(ctypes.byref(a)) == 2 * 4 * 12 * 4
+    links = 16 + 8 * 12 * 24
     assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == links
-    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 1) == links + 4 * 3 * 12 * 4
-    a.L, a.S = 50, 4
-    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == 0  # one tile each
+    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 1) == links + 8 * 3 * 12 * 4
+    a.bf16 = 1  # tiles of 64 steps
+    assert lib.semx_gated_lru_ckpt_bytes(ctypes.byref(a)) == 2 * 2 * 12 * 4
+    a.S, a.rows = 1000, 100000  # sequences enough to walk them
+    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == 0
+    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 1) == 1000 * 3 * 12 * 4
+    a.S, a.rows, a.L = 4, 200, 50  # one tile each
+    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == 0
 
 
 def test_projection_arguments_are_checked_on_the_host():
