@@ -39,7 +39,7 @@ constexpr int kSegs = kT * 4 / kCh; // segments of a tile
 constexpr int kFwdCtas = 5, kBwdCtas = 4;  // per SM
 constexpr int kGroup = 8;           // tiles between two states handed on
 constexpr float kLeastGain = 1e-3f;  // sqrt(1e-6), as the gamma gain of the selective-LRU scans has it
-constexpr float kNear = 0.35f;      // -la up to which the polynomials below hold
+constexpr float kNear = 0.125f;     // -la up to which the polynomials below hold
 constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
 
 // Steps of a segment: the rows of a tile in shared memory are as many bytes in either type.
@@ -93,27 +93,22 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
   return r;
 }
 
-// With m = -la in [0, 0.35] (Chebyshev interpolants of degree 5, 4.4e-8 off with their coefficients'
-// roundings; 2e-9 by themselves):
-//   (1 - exp(-m)) / m, sqrt((1 - exp(-2 m)) / (2 m)), and the latter's inverse.
-__device__ __forceinline__ f2 horner5(f2 m, float c0, float c1, float c2, float c3, float c4, float c5) {
-  f2 v = fma2(both(c5), m, both(c4));
-  v = fma2(v, m, both(c3));
-  v = fma2(v, m, both(c2));
+// With m = -la in [0, 0.125] (Chebyshev interpolants of degree 3 in m, at most 2.6e-8 off; fewer
+// coefficients matter because a pair of equal constants takes two instructions to make):
+//   exp(-m), sqrt((1 - exp(-2 m)) / (2 m)), and the latter's inverse.
+__device__ __forceinline__ f2 horner3(f2 m, float c0, float c1, float c2, float c3) {
+  f2 v = fma2(both(c3), m, both(c2));
   v = fma2(v, m, both(c1));
   return fma2(v, m, both(c0));
 }
-__device__ __forceinline__ f2 loss_near(f2 m) {
-  return horner5(m, 1.0f, -0.4999999701976776f, 0.16666558384895325f, -0.04165346175432205f, 0.008259650319814682f,
-                 -0.0011966862948611379f);
+__device__ __forceinline__ f2 decay_near(f2 m) {
+  return fma2(horner3(m, -1.0f, 0.4999960958957672f, -0.16650986671447754f, 0.03964177519083023f), m, both(1.f));
 }
 __device__ __forceinline__ f2 root_near(f2 m) {
-  return horner5(m, 1.0f, -0.4999999403953552f, 0.2083314210176468f, -0.06247641518712044f, 0.013583178631961346f,
-                 -0.0019963912200182676f);
+  return horner3(m, 1.0f, -0.49999356269836426f, 0.20807549357414246f, -0.05916960909962654f);
 }
 __device__ __forceinline__ f2 inverse_root_near(f2 m) {
-  return horner5(m, 1.0f, 0.5f, 0.04166705161333084f, -0.020837461575865746f, -0.0015454931417480111f,
-                 0.0016374377300962806f);
+  return horner3(m, 1.0f, 0.49999943375587463f, 0.04168989136815071f, -0.021152695640921593f);
 }
 
 // What a channel's rates come to, one float per channel of the tile.
@@ -156,14 +151,15 @@ __device__ __forceinline__ f2 pair_of(const typename RawQuad<ACC>::type& q, int 
 // Decay and gain of a pair of channels. The decay gate's reciprocal root q gives both the gate
 // rho = q^2 and the gain: with m = -la = speed rho, sqrt(1 - exp(-2 m)) = sqrt(2 speed) q root(m).
 // Near m = 0 the decay is exact to its rounding (a state multiplies hundreds of them) and nothing
-// cancels; far from it the special-function exponential is 2 steps off, which a decay below 0.7
-// forgets at once. gain: not yet at its least value.
-__device__ __forceinline__ void decay2(f2 q, f2 speed, f2 root, bool slow, f2* rho, f2* m, f2* a, f2* gain) {
+// cancels; far from it the special-function exponential is 2 steps off, which a decay below 0.89
+// forgets in tens of steps. gain: not yet at its least value. SLOW: no channel gets far.
+template <bool SLOW>
+__device__ __forceinline__ void decay2(f2 q, f2 speed, f2 root, f2* rho, f2* m, f2* a, f2* gain) {
   *rho = mul2(q, q);
   *m = mul2(*rho, speed);
-  *a = fma2(mul2(*m, both(-1.f)), loss_near(*m), both(1.f));
+  *a = decay_near(*m);
   *gain = mul2(mul2(q, root), root_near(*m));
-  if (!slow) {
+  if constexpr (!SLOW) {
     const float2 mm = unpack2(*m);
     float2 aa = unpack2(*a), gg = unpack2(*gain);
     if (mm.x > kNear) {
@@ -347,6 +343,11 @@ __device__ __forceinline__ void unused_rows(const GlParams& p, F f) {
   }
 }
 
+template <bool V>
+struct Is {
+  static constexpr bool value = V;
+};
+
 template <int ACC, int SEG, int OPS>
 struct Stage {
   typename RawQuad<ACC>::type v[OPS][SEG][kT];
@@ -412,22 +413,29 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
     const int most = w.n - seg * SEG;  // steps of the thread that exist
     if (warp * (kSegs / 4) * SEG < w.n) {
       const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[lc]);
-      const bool slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+      auto steps = [&](auto slow) {
+#pragma unroll
+        for (int u = 0; u < SEG; ++u) {
+          const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
+            f2 rho, m, gain;
+            decay2<decltype(slow)::value>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h),
+                                          shared_pair(rt.root, lc + 2 * h), &rho, &m, &a[u][h], &gain);
+            const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
+            b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
+          }
+        }
+      };
+      if (fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear) steps(Is<true>());
+      else steps(Is<false>());
 #pragma unroll
       for (int u = 0; u < SEG; ++u) {
-        const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid];
-        if (gated) rz[u] = st.v[3][u][tid];
-        else rz[u] = Raw{};
-        const bool in = u < most;
+        rz[u] = gated ? st.v[3][u][tid] : Raw{};
+        if (u >= most) a[u][0] = a[u][1] = both(1.f), b[u][0] = b[u][1] = both(0.f);  // rows behind the last one keep the state
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
-          f2 rho, m, gain;
-          decay2(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h), shared_pair(rt.root, lc + 2 * h), slow,
-                 &rho, &m, &a[u][h], &gain);
-          const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
-          b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
-          if (!in) a[u][h] = both(1.f), b[u][h] = both(0.f);  // rows behind the last one keep the state
           A[h] = mul2(A[h], a[u][h]);
           B[h] = fma2(a[u][h], B[h], b[u][h]);
         }
@@ -579,31 +587,42 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
     const Rates& rt = rates[turn];
     const Stage<ACC, SEG, 5>& st = stages[at];
     const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[lc]);
-    const bool slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+    const bool is_slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
     // b: gain iota x, later the state in front of the step; d: the gradient that reaches h from y.
     f2 a[SEG][2], b[SEG][2], d[SEG][2];
     f2 A[2] = {both(1.f), both(1.f)}, B[2] = {both(0.f), both(0.f)}, G[2] = {both(0.f), both(0.f)};
     copies_done();
     if (busy) {
+      auto steps = [&](auto slow) {
+#pragma unroll
+        for (int u = 0; u < SEG; ++u) {
+          const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
+            f2 rho, m, gain;
+            decay2<decltype(slow)::value>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h),
+                                          shared_pair(rt.root, lc + 2 * h), &rho, &m, &a[u][h], &gain);
+            const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
+            b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
+            d[u][h] = pair_of<ACC>(rg, h, p.bf16);
+            if (gated) {
+              const f2 z = pair_of<ACC>(st.v[3][u][tid], h, p.bf16);
+              d[u][h] = mul2(d[u][h], mul2(z, rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)))));
+            }
+          }
+        }
+      };
+      if (is_slow) steps(Is<true>());
+      else steps(Is<false>());
 #pragma unroll
       for (int u = 0; u < SEG; ++u) {
-        const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
-        const bool in = u < most;
+        if (u >= most) {
+          a[u][0] = a[u][1] = both(1.f);
+          b[u][0] = b[u][1] = d[u][0] = d[u][1] = both(0.f);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
-          f2 rho, m, gain;
-          decay2(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h), shared_pair(rt.root, lc + 2 * h), slow,
-                 &rho, &m, &a[u][h], &gain);
-          const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
-          b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
-          d[u][h] = pair_of<ACC>(rg, h, p.bf16);
-          if (gated) {
-            const f2 z = pair_of<ACC>(st.v[3][u][tid], h, p.bf16);
-            const f2 s = rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)));
-            d[u][h] = mul2(d[u][h], mul2(z, s));
-          }
-          if (!in) a[u][h] = both(1.f), b[u][h] = d[u][h] = both(0.f);
           A[h] = mul2(A[h], a[u][h]);
           B[h] = fma2(a[u][h], B[h], b[u][h]);
         }
@@ -680,67 +699,70 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
         }
       const int64_t out = (w.row + seg * SEG) * p.C + c0 + lc;
       f2 gs[2] = {shared_pair(mG[seg], lc), shared_pair(mG[seg], lc + 2)};
+      auto steps = [&](auto slow) {
 #pragma unroll
-      for (int u = SEG - 1; u >= 0; --u) {
-        const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
-        const bool in = u < most;
-        f2 dx[2], dr[2], di[2], dz[2];
+        for (int u = SEG - 1; u >= 0; --u) {
+          if (u >= most) continue;
+          const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
+          f2 dx[2], dr[2], di[2], dz[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const f2 x = pair_of<ACC>(rx, k, p.bf16), speed = shared_pair(rt.speed, lc + 2 * k);
-          const f2 gt = add2(d[u][k], gs[k]);
-          const f2 er = ex2_2(end2(gate_arg(pair_of<ACC>(rr, k, p.bf16), shared_pair(rt.r2, lc + 2 * k))));
-          const f2 er1 = add2(er, both(1.f)), qr = rsqrt_2(er1);
-          f2 rho, m, at, gain;
-          decay2(qr, speed, shared_pair(rt.root, lc + 2 * k), slow, &rho, &m, &at, &gain);
-          // 1 / gain: 1 / q = (1 + er) q.
-          f2 inv = mul2(mul2(mul2(er1, qr), shared_pair(rt.inverse, lc + 2 * k)), inverse_root_near(m));
-          float2 gg = unpack2(gain), iv = unpack2(inv);
-          if (!slow) {
-            const float2 mm = unpack2(m);
-            if (mm.x > kNear) iv.x = 1.f / gg.x;
-            if (mm.y > kNear) iv.y = 1.f / gg.y;
-          }
-          iv.x = gg.x > kLeastGain ? iv.x : 0.f;  // at its least value no gradient goes through the gain
-          iv.y = gg.y > kLeastGain ? iv.y : 0.f;
-          inv = pack2(iv.x, iv.y);
-          gain = least2(gain);
-          const f2 ei = ex2_2(end2(gate_arg(pair_of<ACC>(ri, k, p.bf16), shared_pair(rt.i2, lc + 2 * k))));
-          const f2 iota = rcp_2(add2(ei, both(1.f)));
-          const f2 ah = mul2(a[u][k], b[u][k]);
-          if (gated) {
-            const f2 z = pair_of<ACC>(st.v[3][u][tid], k, p.bf16);
-            const f2 ez = ex2_2(end2(mul2(z, both(-kLog2e)))), s = rcp_2(add2(ez, both(1.f)));
-            const f2 h = fma2(mul2(gain, iota), x, ah);
-            // silu'(z) = s (1 + z (1 - s)), 1 - s = ez s
-            dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, mul2(ez, s), both(1.f))));
-          }
-          const f2 gi = mul2(gt, iota);
-          dx[k] = mul2(gi, gain);
-          di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
-          const f2 through = mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv));
-          const f2 dla = fma2(gt, ah, mul2(through, both(-1.f)));
-          const f2 rd = mul2(rho, dla);
-          dr[k] = mul2(mul2(rd, mul2(er, rho)), mul2(speed, both(-1.f)));
-          gs[k] = mul2(a[u][k], gt);
-          if (in) {
+          for (int k = 0; k < 2; ++k) {
+            const f2 x = pair_of<ACC>(rx, k, p.bf16), speed = shared_pair(rt.speed, lc + 2 * k);
+            const f2 gt = add2(d[u][k], gs[k]);
+            const f2 er = ex2_2(end2(gate_arg(pair_of<ACC>(rr, k, p.bf16), shared_pair(rt.r2, lc + 2 * k))));
+            const f2 er1 = add2(er, both(1.f)), qr = rsqrt_2(er1);
+            f2 rho, m, at, gain;
+            decay2<decltype(slow)::value>(qr, speed, shared_pair(rt.root, lc + 2 * k), &rho, &m, &at, &gain);
+            // 1 / gain: 1 / q = (1 + er) q.
+            f2 inv = mul2(mul2(mul2(er1, qr), shared_pair(rt.inverse, lc + 2 * k)), inverse_root_near(m));
+            const float2 gg = unpack2(gain);
+            float2 iv = unpack2(inv);
+            if constexpr (!decltype(slow)::value) {
+              const float2 mm = unpack2(m);
+              if (mm.x > kNear) iv.x = 1.f / gg.x;
+              if (mm.y > kNear) iv.y = 1.f / gg.y;
+            }
+            iv.x = gg.x > kLeastGain ? iv.x : 0.f;  // at its least value no gradient goes through the gain
+            iv.y = gg.y > kLeastGain ? iv.y : 0.f;
+            inv = pack2(iv.x, iv.y);
+            gain = least2(gain);
+            const f2 ei = ex2_2(end2(gate_arg(pair_of<ACC>(ri, k, p.bf16), shared_pair(rt.i2, lc + 2 * k))));
+            const f2 iota = rcp_2(add2(ei, both(1.f)));
+            const f2 ah = mul2(a[u][k], b[u][k]);
+            if (gated) {
+              const f2 z = pair_of<ACC>(st.v[3][u][tid], k, p.bf16);
+              const f2 ez = ex2_2(end2(mul2(z, both(-kLog2e)))), s = rcp_2(add2(ez, both(1.f)));
+              const f2 h = fma2(mul2(gain, iota), x, ah);
+              // silu'(z) = s (1 + z (1 - s)), 1 - s = ez s
+              dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, mul2(ez, s), both(1.f))));
+            }
+            const f2 gi = mul2(gt, iota);
+            dx[k] = mul2(gi, gain);
+            di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
+            const f2 through = mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv));
+            const f2 dla = fma2(gt, ah, mul2(through, both(-1.f)));
+            const f2 rd = mul2(rho, dla);
+            dr[k] = mul2(mul2(rd, mul2(er, rho)), mul2(speed, both(-1.f)));
+            gs[k] = mul2(a[u][k], gt);
             sum[0][k] = add2(sum[0][k], rd);
             sum[1][k] = add2(sum[1][k], dr[k]);
             sum[2][k] = add2(sum[2][k], di[k]);
           }
+          if (nn > 0) {
+            const int64_t o = out + u * p.C;
+            auto put = [&](void* to, const f2 (&v)[2]) {
+              const float2 lo = unpack2(v[0]), hi = unpack2(v[1]);
+              store_quad<ACC>(to, o, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
+            };
+            put(p.dx, dx);
+            put(p.dr, dr);
+            put(p.di, di);
+            if (gated) put(p.dz, dz);
+          }
         }
-        if (in && nn > 0) {
-          const int64_t o = out + u * p.C;
-          auto put = [&](void* to, const f2 (&v)[2]) {
-            const float2 lo = unpack2(v[0]), hi = unpack2(v[1]);
-            store_quad<ACC>(to, o, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
-          };
-          put(p.dx, dx);
-          put(p.dr, dr);
-          put(p.di, di);
-          if (gated) put(p.dz, dz);
-        }
-      }
+      };
+      if (is_slow) steps(Is<true>());
+      else steps(Is<false>());
     }
     if (p.part != nullptr && (LINK || w.k == 0)) {
       __syncthreads();
@@ -816,7 +838,7 @@ __global__ void __launch_bounds__(kStepT) gated_lru_step_kernel(const GlParams p
         for (int k = 0; k < 2; ++k) {
           const f2 q = rsqrt_2(add2(ex2_2(gate_arg(pair_of<ACC>(rr[u], k, p.bf16), pack2(r2[2 * k], r2[2 * k + 1]))), both(1.f)));
           f2 rho, m, a, gain;
-          decay2(q, pack2(speed[2 * k], speed[2 * k + 1]), pack2(root[2 * k], root[2 * k + 1]), false, &rho, &m, &a, &gain);
+          decay2<false>(q, pack2(speed[2 * k], speed[2 * k + 1]), pack2(root[2 * k], root[2 * k + 1]), &rho, &m, &a, &gain);
           const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri[u], k, p.bf16), pack2(i2[2 * k], i2[2 * k + 1]))), both(1.f)));
           hs[k] = fma2(a, hs[k], mul2(mul2(iota, pair_of<ACC>(rx[u], k, p.bf16)), least2(gain)));
           if (slot == semx::kRefused) hs[k] = both(__int_as_float(0x7fffffff));
