@@ -260,8 +260,7 @@ __device__ __forceinline__ float link_in(const GlParams& p, const Chain& q, int 
 
 // A tile: rows [row, row + n) of the batch, number k of `tiles` of sequence s, piece j of the batch.
 struct Tile {
-  int64_t row;
-  int n, k, tiles, s, j, ct;
+  int row, n, k, tiles, s, j, ct;
   bool any, live;  // any: there is one; live: it is a part of a sequence (one without rows has tile 0)
 };
 
@@ -323,7 +322,7 @@ __device__ __forceinline__ Tile tile_at(const GlParams& p, int n, int step) {
     t.tiles = (int)p.m.per;
     t.k = BACK ? t.tiles - 1 - step : step;
     t.j = of * t.tiles + t.k;
-    t.row = (int64_t)of * p.m.L + t.k * Q;
+    t.row = of * (int)p.m.L + t.k * Q;
     t.n = min((int)p.m.L - t.k * Q, Q);
     t.live = true;
   }
@@ -341,6 +340,20 @@ __device__ __forceinline__ void unused_rows(const GlParams& p, F f) {
     const int c = (int)(i - r * quads) * 4;
     f(r < front ? r : p.m.T - count + r, c, min(4, p.C - c));
   }
+}
+
+// Bytes of an element of a row.
+__device__ __forceinline__ int element(int acc, int bf16) { return acc == kBf16 || (acc == kAny && bf16) ? 2 : 4; }
+
+// Four elements into shared memory, zeros where there are none; on their way until copies_done(). Only
+// the thread that asked for them reads them. (from may lie anywhere where `any` is false.)
+template <int ACC>
+__device__ __forceinline__ void bring_quad(typename RawQuad<ACC>::type* to, const char* from, bool any) {
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (ACC == kBf16)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(any ? 8 : 0) : "memory");
+  else
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(any ? 16 : 0) : "memory");
 }
 
 template <bool V>
@@ -373,15 +386,15 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
     __syncthreads();
   }
   auto fetch = [&](const Tile& w) {  // the thread's own rows, on their way into its own places
-    const int nn = p.C - w.ct * kCh - lc, most = min(w.n - seg * SEG, SEG);
-    const int64_t ch = nn > 0 ? w.ct * kCh + lc : 0, row = most > 0 ? w.row + seg * SEG : 0;
+    const int nn = min(p.C - w.ct * kCh - lc, 4), most = nn > 0 ? w.n - seg * SEG : 0;
+    const int row = most > 0 ? w.row + seg * SEG : 0, ch = most > 0 ? w.ct * kCh + lc : 0;
     auto bring = [&](int op, const void* from, int64_t ld) {
-      int64_t at = row * ld + ch;
+      const char* at = reinterpret_cast<const char*>(from) + ((int64_t)row * (int)ld + ch) * element(ACC, p.bf16);
+      const int64_t step = ld * element(ACC, p.bf16);
 #pragma unroll
-      for (int u = 0; u < SEG; ++u, at += ld) {
-        const bool in = u < most && nn > 0;
-        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(from, at, p.bf16, in ? min(nn, 4) : 0);
-        else copy_quad<ACC>(&st.v[op][u][tid], from, at, in);
+      for (int u = 0; u < SEG; ++u, at += step) {
+        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(at, 0, p.bf16, u < most ? nn : 0);
+        else bring_quad<ACC>(&st.v[op][u][tid], at, u < most);
       }
     };
     bring(0, p.x, p.ldx);
@@ -500,7 +513,9 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
     }
     __syncthreads();
     f2 hs[2] = {shared_pair(mB[seg], lc), shared_pair(mB[seg], lc + 2)};
-    const int64_t out = (w.row + seg * SEG) * p.C + c0 + lc;
+    char* out = reinterpret_cast<char*>(p.y) + ((int64_t)(w.row + seg * SEG) * p.C + c0 + lc) * element(ACC, p.bf16);
+    const int64_t row = (int64_t)p.C * element(ACC, p.bf16);
+    const int end = nn > 0 ? most : 0;
 #pragma unroll
     for (int u = 0; u < SEG; ++u) {
       f2 y[2];
@@ -514,9 +529,9 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
           y[k] = mul2(y[k], mul2(z, s));
         }
       }
-      if (u < most && nn > 0) {
+      if (u < end) {
         const float2 lo = unpack2(y[0]), hi = unpack2(y[1]);
-        store_quad<ACC>(p.y, out + u * p.C, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
+        store_quad<ACC>(out + u * row, 0, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
       }
     }
     w = next;
@@ -543,15 +558,15 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
     __syncthreads();
   }
   auto fetch = [&](const Tile& w, Stage<ACC, SEG, 5>& st) {  // the thread's own rows, on their way into its own places
-    const int nn = p.C - w.ct * kCh - lc, most = min(w.n - seg * SEG, SEG);
-    const int64_t ch = nn > 0 ? w.ct * kCh + lc : 0, row = most > 0 ? w.row + seg * SEG : 0;
+    const int nn = min(p.C - w.ct * kCh - lc, 4), most = nn > 0 ? w.n - seg * SEG : 0;
+    const int row = most > 0 ? w.row + seg * SEG : 0, ch = most > 0 ? w.ct * kCh + lc : 0;
     auto bring = [&](int op, const void* from, int64_t ld) {
-      int64_t at = row * ld + ch;
+      const char* at = reinterpret_cast<const char*>(from) + ((int64_t)row * (int)ld + ch) * element(ACC, p.bf16);
+      const int64_t step = ld * element(ACC, p.bf16);
 #pragma unroll
-      for (int u = 0; u < SEG; ++u, at += ld) {
-        const bool in = u < most && nn > 0;
-        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(from, at, p.bf16, in ? min(nn, 4) : 0);
-        else copy_quad<ACC>(&st.v[op][u][tid], from, at, in);
+      for (int u = 0; u < SEG; ++u, at += step) {
+        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(at, 0, p.bf16, u < most ? nn : 0);
+        else bring_quad<ACC>(&st.v[op][u][tid], at, u < most);
       }
     };
     bring(0, p.x, p.ldx);
@@ -697,7 +712,8 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
           b[u][k] = hs[k];
           hs[k] = after;
         }
-      const int64_t out = (w.row + seg * SEG) * p.C + c0 + lc;
+      const int64_t out = ((int64_t)(w.row + seg * SEG) * p.C + c0 + lc) * element(ACC, p.bf16);
+      const int64_t row = (int64_t)p.C * element(ACC, p.bf16);
       f2 gs[2] = {shared_pair(mG[seg], lc), shared_pair(mG[seg], lc + 2)};
       auto steps = [&](auto slow) {
 #pragma unroll
@@ -749,10 +765,10 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
             sum[2][k] = add2(sum[2][k], di[k]);
           }
           if (nn > 0) {
-            const int64_t o = out + u * p.C;
+            const int64_t o = out + u * row;
             auto put = [&](void* to, const f2 (&v)[2]) {
               const float2 lo = unpack2(v[0]), hi = unpack2(v[1]);
-              store_quad<ACC>(to, o, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
+              store_quad<ACC>(reinterpret_cast<char*>(to) + o, 0, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
             };
             put(p.dx, dx);
             put(p.dr, dr);
