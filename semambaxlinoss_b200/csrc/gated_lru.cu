@@ -12,7 +12,7 @@
 // Bound: HBM (5 values per element forward, 9 backward); the special-function unit (6 operations per
 // element forward) comes next.
 //
-// Split: a tile is 64 steps (bf16; fp32 32) of one sequence by 32 channels; a CTA of four warps reads
+// Split: a tile is 64 steps (backward 32) of one sequence by 32 channels; a CTA of four warps reads
 // it once. A thread has a segment of 4 (2) neighbouring steps of four neighbouring channels: it folds
 // them into one map h -> A h + B, one warp (a lane per channel) folds the 16 segments' maps and finds
 // the tile's entry state, and each thread runs its steps again from its segment's entry state, on
@@ -20,10 +20,10 @@
 // one's entry state is looked for.
 // Many sequences: a CTA walks one after another, the state stays in registers. Few or packed ones:
 // tiles are linked through global memory inside the one launch: each leaves its map (A, B) and the
-// state behind it, and takes the maps of the tiles in front of it in its group of 8 and the state that
+// state behind it, and takes the maps of the tiles in front of it in its group of 16 and the state that
 // the group before left. Which maps are folded in which order depends on the numbers alone, so
 // results do not change from run to run. Tickets number the tiles in the order in which CTAs take
-// them, so a tile only waits for tiles that are under way. The backward runs the same from the last
+// them, one count for each 32 channels, so a tile only waits for tiles that are under way. The backward runs the same from the last
 // tile on.
 #include "semx_reduce.cuh"
 #include "state_scan.cuh"
@@ -37,13 +37,15 @@ constexpr int kT = 128;
 constexpr int kCh = 32;             // channels of a tile: eight lanes of four
 constexpr int kSegs = kT * 4 / kCh; // segments of a tile
 constexpr int kFwdCtas = 5, kBwdCtas = 4;  // per SM
-constexpr int kGroup = 8;           // tiles between two states handed on
+constexpr int kGroup = 16;          // tiles between two states handed on
 constexpr float kLeastGain = 1e-3f;  // sqrt(1e-6), as the gamma gain of the selective-LRU scans has it
 constexpr float kNear = 0.125f;     // -la up to which the polynomials below hold
 constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
 
-// Steps of a segment: the rows of a tile in shared memory are as many bytes in either type.
-__host__ __device__ constexpr int seg_steps(bool bf16) { return bf16 ? 4 : 2; }
+// Steps of a segment. The backward has more to keep per step, and its unrolled steps leave the
+// instruction cache (404 x 321 x 256 bf16, two or four steps: forward 100 and 84 us, backward 186 and 229).
+constexpr int kFwdSeg = 4, kBwdSeg = 2;
+constexpr int kUnit = kSegs * kBwdSeg;  // steps between two states that a training forward keeps
 
 __device__ unsigned int g_link_timeouts;
 
@@ -61,14 +63,14 @@ struct GlParams {
   const float* i_bias;
   void* y;
   float* state;
-  float* ckpt;  // (tiles, C) state in front of each tile
+  float* ckpt;  // (units, C) state in front of every 32nd step
   const void* dy;
   void* dx;
   void* dr;
   void* di;
   void* dz;
   float* part;     // (tiles, or sequences where a CTA walks them; 3, C) partial drate | dr_bias | di_bias
-  int* ticket;     // linked: the next tile's number
+  int* ticket;     // linked: the number of each channel tile's next piece
   ulonglong2* maps;         // linked: (tiles, C) map (A, B) of each tile, kHere in the upper half of both
   unsigned long long* left; // linked: (tiles, C) state behind each tile, kHere in the upper half
 };
@@ -119,8 +121,8 @@ struct Rates {
   float slope[kCh];  // d speed / d rate
   float r2[kCh], i2[kCh];  // biases, times -log2(e)
 };
-__device__ __forceinline__ void load_rates(const GlParams& p, int ct, int lane, Rates* to) {
-  const int c = min(ct * kCh + lane, p.C - 1);
+__device__ __forceinline__ void load_rates(const GlParams& p, int c0, int lane, Rates* to) {
+  const int c = min(c0 + lane, p.C - 1);
   const float rate = p.rate[c];
   float e, s = p.scale * softplus(rate, &e);
   to->slope[lane] = p.scale * softplus_slope(rate, e);
@@ -191,8 +193,7 @@ constexpr unsigned long long kHere = 1ull << 32;
 
 // Where tile number `at` in the order of the recurrence is among the pieces: j0 + dir at.
 struct Chain {
-  int64_t j0;
-  int dir, at;
+  int j0, dir, at;
 };
 
 __device__ __forceinline__ ulonglong2 peek_map(const ulonglong2* p) {
@@ -216,51 +217,62 @@ __device__ __forceinline__ void leave_state(const GlParams& p, int64_t j, int c,
 }
 
 // State in front of the tile for channel c (a lane each; ok false: none): the maps of the tiles in
-// front in its group, folded in their order, applied to the state that the group before left. The
-// first tile of a sequence has its entry state in its map (A = 0).
+// front in its group, folded in their order, applied to the state that the group before left (looked for
+// last: it comes last). The first tile of a sequence has its entry state in its map (A = 0).
 __device__ __forceinline__ float link_in(const GlParams& p, const Chain& q, int c, bool ok) {
-  const int g0 = q.at / kGroup * kGroup, n = q.at - g0;
-  // Offsets that decrease can name a piece that is none.
-  auto index = [&](int at) {
-    const int64_t j = q.j0 + (int64_t)q.dir * at;
-    return ok && j >= 0 && j < p.m.pieces ? j : (int64_t)-1;
-  };
-  ulonglong2 m[kGroup - 1];
-  unsigned long long before = kHere;
-  const int64_t jb = g0 > 0 ? index(g0 - 1) : -1;
+  const int g0 = q.at / kGroup * kGroup, n = ok ? q.at - g0 : 0;
   const long long from = clock64();
-  bool done;
-  do {
-    done = true;
+  bool given_up = false;
+  float a = 1.f, b = 0.f;
+  constexpr int kAhead = 5;  // maps on their way
+#pragma unroll 1
+  for (int e0 = 0; e0 < n; e0 += kAhead) {
+    ulonglong2 m[kAhead];
+    bool done;
+    do {
+      done = true;
 #pragma unroll
-    for (int e = 0; e < kGroup - 1; ++e) {
-      const int64_t j = e < n ? index(g0 + e) : -1;
-      m[e] = j >= 0 ? peek_map(&p.maps[j * p.C + c]) : make_ulonglong2(marked(1.f), marked(0.f));
+      for (int e = 0; e < kAhead; ++e) {
+        const int j = q.j0 + q.dir * (g0 + e0 + e);
+        // Offsets that decrease can name a piece that is none.
+        const bool there = e0 + e < n && j >= 0 && j < (int)p.m.pieces;
+        m[e] = there ? peek_map(&p.maps[(int64_t)j * p.C + c]) : make_ulonglong2(marked(1.f), marked(0.f));
+      }
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) done = done && (m[e].x & kHere) != 0 && (m[e].y & kHere) != 0;
+      given_up = !done && clock64() - from > kPatience;
+    } while (!done && !given_up);
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const float A = __uint_as_float((unsigned)m[e].x), B = __uint_as_float((unsigned)m[e].y);
+      b = fmaf(A, b, B);
+      a *= A;
     }
-    if (jb >= 0) before = peek(&p.left[jb * p.C + c]);
-#pragma unroll
-    for (int e = 0; e < kGroup - 1; ++e) done = done && (m[e].x & kHere) != 0 && (m[e].y & kHere) != 0;
-    done = done && (before & kHere) != 0;
-  } while (!done && clock64() - from < kPatience);
-  if (!done) {
+    if (given_up) break;
+  }
+  const int jb = q.j0 + q.dir * (g0 - 1);
+  if (ok && g0 > 0 && jb >= 0 && jb < (int)p.m.pieces && !given_up) {
+    const unsigned long long* at = &p.left[(int64_t)jb * p.C + c];
+    unsigned long long before;
+    do {
+      before = peek(at);
+      given_up = (before & kHere) == 0 && clock64() - from > kPatience;
+    } while ((before & kHere) == 0 && !given_up);
+    b = fmaf(a, __uint_as_float((unsigned)before), b);
+  }
+  if (given_up) {
     atomicAdd(&g_link_timeouts, 1u);
     return __int_as_float(0x7fffffff);
   }
-  float a = 1.f, b = 0.f;
-#pragma unroll
-  for (int e = 0; e < kGroup - 1; ++e) {
-    const float A = __uint_as_float((unsigned)m[e].x), B = __uint_as_float((unsigned)m[e].y);
-    b = fmaf(A, b, B);
-    a *= A;
-  }
-  return jb >= 0 ? fmaf(a, __uint_as_float((unsigned)before), b) : b;
+  return b;
 }
 
 // -- the order of a CTA's tiles -------------------------------------------------------------------
 
-// A tile: rows [row, row + n) of the batch, number k of `tiles` of sequence s, piece j of the batch.
+// A tile: rows [row, row + n) of the batch, number k of `tiles` of sequence s, piece j of the batch; the
+// state in front of its first step is kept as number `unit`.
 struct Tile {
-  int row, n, k, tiles, s, j, ct;
+  int row, n, k, tiles, s, j, unit;
   bool any, live;  // any: there is one; live: it is a part of a sequence (one without rows has tile 0)
 };
 
@@ -296,34 +308,30 @@ __device__ __forceinline__ void find_tile(const semx::SeqMap& m, int j, Tile* t)
   t->tiles = (len + Q - 1) / Q;
   t->live = t->k >= 0 && (t->k == 0 || t->k < t->tiles);
   t->row = start + (t->live ? t->k * Q : 0);
+  t->unit = (m.cu == nullptr ? t->s * ((int)(m.L + kUnit - 1) / kUnit) : start / kUnit + t->s) + t->k * (Q / kUnit);
   t->n = t->live ? min(len - t->k * Q, Q) : 0;
 }
 
-// LINK: tiles in the order of their tickets. Else the CTA walks whole sequences of equal lengths, all
-// tiles of one behind one another. BACK: from the last one on. `n`: the ticket, or the walked
-// sequence's number among (sequences, channel tiles).
+// LINK: piece number n of the batch, the ticket of the CTA's channel tile. Else tile number `step` of
+// sequence n of equal lengths. BACK: from the last one on.
 template <bool LINK, bool BACK, int Q>
 __device__ __forceinline__ Tile tile_at(const GlParams& p, int n, int step) {
   Tile t;
-  const int total = (int)((LINK ? p.m.pieces : p.m.S) * p.ctiles);
-  t.any = n < total;
+  t.any = n < (int)(LINK ? p.m.pieces : p.m.S);
   t.live = false;
-  t.j = t.ct = t.k = t.n = t.s = t.tiles = 0;
-  t.row = 0;
+  t.j = t.k = t.n = t.s = t.tiles = t.row = t.unit = 0;
   if (!t.any) return t;
-  const unsigned i = LINK && BACK ? total - 1 - n : n;
-  const int of = (int)(i / (unsigned)p.ctiles);
-  t.ct = (int)i - of * p.ctiles;
   if (LINK) {
-    t.j = of;
-    if (p.m.S > 0) find_tile<Q>(p.m, of, &t);
+    t.j = BACK ? (int)p.m.pieces - 1 - n : n;
+    if (p.m.S > 0) find_tile<Q>(p.m, t.j, &t);
   } else {
-    t.s = of;
+    t.s = n;
     t.tiles = (int)p.m.per;
     t.k = BACK ? t.tiles - 1 - step : step;
-    t.j = of * t.tiles + t.k;
-    t.row = of * (int)p.m.L + t.k * Q;
+    t.j = n * t.tiles + t.k;
+    t.row = n * (int)p.m.L + t.k * Q;
     t.n = min((int)p.m.L - t.k * Q, Q);
+    t.unit = n * ((int)(p.m.L + kUnit - 1) / kUnit) + t.k * (Q / kUnit);
     t.live = true;
   }
   return t;
@@ -366,125 +374,147 @@ struct Stage {
   typename RawQuad<ACC>::type v[OPS][SEG][kT];
 };
 
-// LINK: sequences of several tiles, linked through global memory. Else: walked.
+// What both kernels' CTAs have: their channel tile, and the order of their tiles. LINK: the tickets of the
+// channel tile. Else they walk sequences, every (CTAs per channel tile)-th.
+struct Place {
+  int ct, c0, nn, lc, seg;  // channel tile, its first channel; the thread's channels, first of them in the tile, segment
+  int walk;                 // sequences between two of the CTA's
+};
+__device__ __forceinline__ Place place_of(const GlParams& p) {
+  Place at;
+  at.ct = blockIdx.x % (unsigned)p.ctiles;
+  at.c0 = at.ct * kCh;
+  at.lc = threadIdx.x % (kCh / 4) * 4;
+  at.seg = threadIdx.x / (kCh / 4);
+  at.nn = max(0, min(p.C - at.c0 - at.lc, 4));
+  at.walk = gridDim.x / (unsigned)p.ctiles;
+  return at;
+}
+
+// The thread's rows of one operand, on their way into its own places.
+template <int ACC, int SEG, int OPS>
+__device__ __forceinline__ void bring(const GlParams& p, const Place& at, const Tile& w, Stage<ACC, SEG, OPS>& st, int op,
+                                      const void* from, int64_t ld) {
+  const int most = at.nn > 0 ? w.n - at.seg * SEG : 0;
+  const int row = most > 0 ? w.row + at.seg * SEG : 0, ch = at.nn > 0 ? at.c0 + at.lc : 0;
+  const int size = element(ACC, p.bf16);
+  const char* src = reinterpret_cast<const char*>(from) + ((int64_t)row * (int)ld + ch) * size;
+  const int64_t step = ld * size;
+#pragma unroll
+  for (int u = 0; u < SEG; ++u, src += step) {
+    if constexpr (ACC == kAny) st.v[op][u][threadIdx.x] = load_quad<ACC>(src, 0, p.bf16, u < most ? at.nn : 0);
+    else bring_quad<ACC>(&st.v[op][u][threadIdx.x], src, u < most);
+  }
+}
+
+// Decay a and input b = gain iota x of the thread's steps.
+template <int ACC, int SEG, bool SLOW, int OPS>
+__device__ __forceinline__ void gate_steps(const GlParams& p, const Rates& rt, int lc, const Stage<ACC, SEG, OPS>& st, f2 (&a)[SEG][2],
+                                           f2 (&b)[SEG][2]) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < SEG; ++u) {
+    const typename RawQuad<ACC>::type rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = lc + 2 * h;
+      const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, c)));
+      f2 rho, m, gain;
+      decay2<SLOW>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, c), shared_pair(rt.root, c), &rho, &m, &a[u][h], &gain);
+      const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, c))), both(1.f)));
+      b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
+    }
+  }
+}
+
+// LINK: tiles linked through global memory. Else: sequences walked. Two barriers a tile: the maps are
+// there; the segments' entry states are there.
 template <int ACC, int SEG, bool LINK>
 __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlParams p) {
   typedef typename RawQuad<ACC>::type Raw;
+  constexpr int Q = kSegs * SEG;
   extern __shared__ __align__(16) unsigned char raw[];
   Stage<ACC, SEG, 4>& st = *reinterpret_cast<Stage<ACC, SEG, 4>*>(raw);
-  __shared__ __align__(16) float mA[kSegs][kCh], mB[kSegs][kCh];
-  __shared__ __align__(16) Rates rates[2];
+  __shared__ __align__(16) float maps[2][2][kSegs][kCh];  // this tile's and the one's before: A, B
+  __shared__ __align__(16) Rates rt;
   __shared__ int ticket;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-  const int seg = tid / (kCh / 4), lc = tid % (kCh / 4) * 4;
+  const Place at = place_of(p);
   const bool gated = p.z != nullptr;
-  int n = blockIdx.x;
-  if (LINK) {
-    if (tid == 0) ticket = atomicAdd(p.ticket, 1);
-    __syncthreads();
-    n = ticket;
-    __syncthreads();
-  }
-  auto fetch = [&](const Tile& w) {  // the thread's own rows, on their way into its own places
-    const int nn = min(p.C - w.ct * kCh - lc, 4), most = nn > 0 ? w.n - seg * SEG : 0;
-    const int row = most > 0 ? w.row + seg * SEG : 0, ch = most > 0 ? w.ct * kCh + lc : 0;
-    auto bring = [&](int op, const void* from, int64_t ld) {
-      const char* at = reinterpret_cast<const char*>(from) + ((int64_t)row * (int)ld + ch) * element(ACC, p.bf16);
-      const int64_t step = ld * element(ACC, p.bf16);
-#pragma unroll
-      for (int u = 0; u < SEG; ++u, at += step) {
-        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(at, 0, p.bf16, u < most ? nn : 0);
-        else bring_quad<ACC>(&st.v[op][u][tid], at, u < most);
-      }
-    };
-    bring(0, p.x, p.ldx);
-    bring(1, p.r, p.ldr);
-    bring(2, p.i, p.ldi);
-    if (gated) bring(3, p.z, p.ldz);
-  };
-  int step = 0, turn = 0;
-  constexpr int Q = kSegs * SEG;
-  Tile w = tile_at<LINK, false, Q>(p, n, 0);
-  fetch(w);
-  if (w.any && warp == 1) load_rates(p, w.ct, lane, &rates[0]);
+  if (LINK && tid == 0) ticket = atomicAdd(&p.ticket[at.ct], 1);
+  if (warp == 1) load_rates(p, at.c0, lane, &rt);
   unused_rows(p, [&](int64_t row, int c, int k) {
     store_quad<ACC>(p.y, row * p.C + c, p.bf16, k, make_float4(0.f, 0.f, 0.f, 0.f));
   });
+  __syncthreads();
+  int n = LINK ? ticket : (int)(blockIdx.x / (unsigned)p.ctiles), step = 0, buf = 0;
+  __syncthreads();
+  auto fetch = [&](const Tile& w) {
+    bring(p, at, w, st, 0, p.x, p.ldx);
+    bring(p, at, w, st, 1, p.r, p.ldr);
+    bring(p, at, w, st, 2, p.i, p.ldi);
+    if (gated) bring(p, at, w, st, 3, p.z, p.ldz);
+  };
+  const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[at.lc]);
+  const bool slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+  const int c = at.c0 + lane;  // warp 0: a lane per channel
+  const bool ok = c < p.C;
+  Tile w = tile_at<LINK, false, Q>(p, n, 0);
+  fetch(w);
   float carry = 0.f;  // warp 0: the walked sequence's state
   while (w.any) {
-    const int c0 = w.ct * kCh, nn = min(4, p.C - c0 - lc);
     const bool first = w.k == 0, last = w.k + 1 >= w.tiles;
     int64_t slot = semx::kNone;
     if (p.m.n_slots > 0 && w.live && (first || last)) slot = find_slot(p.m, w.s);
-    if (LINK && tid == 0) ticket = atomicAdd(p.ticket, 1);
-    __syncthreads();  // rates; the maps of the tile before have been read
-    const Rates& rt = rates[turn];
+    int drawn = 0;  // on its way while the tile's steps are folded
+    if (LINK && tid == 0) drawn = atomicAdd(&p.ticket[at.ct], 1);
+    float(*mA)[kCh] = maps[buf][0], (*mB)[kCh] = maps[buf][1];
     f2 a[SEG][2], b[SEG][2];
     f2 A[2] = {both(1.f), both(1.f)}, B[2] = {both(0.f), both(0.f)};
     Raw rz[SEG];
     copies_done();
-    const int most = w.n - seg * SEG;  // steps of the thread that exist
+    const int most = w.n - at.seg * SEG;  // steps of the thread that exist
     if (warp * (kSegs / 4) * SEG < w.n) {
-      const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[lc]);
-      auto steps = [&](auto slow) {
+      if (slow) gate_steps<ACC, SEG, true>(p, rt, at.lc, st, a, b);
+      else gate_steps<ACC, SEG, false>(p, rt, at.lc, st, a, b);
+      if (gated) {
 #pragma unroll
-        for (int u = 0; u < SEG; ++u) {
-          const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
-            f2 rho, m, gain;
-            decay2<decltype(slow)::value>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h),
-                                          shared_pair(rt.root, lc + 2 * h), &rho, &m, &a[u][h], &gain);
-            const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
-            b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
-          }
-        }
-      };
-      if (fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear) steps(Is<true>());
-      else steps(Is<false>());
-#pragma unroll
-      for (int u = 0; u < SEG; ++u) {
-        rz[u] = gated ? st.v[3][u][tid] : Raw{};
-        if (u >= most) a[u][0] = a[u][1] = both(1.f), b[u][0] = b[u][1] = both(0.f);  // rows behind the last one keep the state
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          A[h] = mul2(A[h], a[u][h]);
-          B[h] = fma2(a[u][h], B[h], b[u][h]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < SEG; ++u) {
-        rz[u] = Raw{};
-        a[u][0] = a[u][1] = both(1.f);
-        b[u][0] = b[u][1] = both(0.f);
+        for (int u = 0; u < SEG; ++u) rz[u] = st.v[3][u][tid];
       }
     }
+    if (most < SEG) {  // rows behind the last one keep the state
+#pragma unroll
+      for (int u = 0; u < SEG; ++u)
+        if (u >= most) a[u][0] = a[u][1] = both(1.f), b[u][0] = b[u][1] = both(0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < SEG; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        A[h] = mul2(A[h], a[u][h]);
+        B[h] = fma2(a[u][h], B[h], b[u][h]);
+      }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      *reinterpret_cast<f2*>(&mA[seg][lc + 2 * h]) = A[h];
-      *reinterpret_cast<f2*>(&mB[seg][lc + 2 * h]) = B[h];
+      *reinterpret_cast<f2*>(&mA[at.seg][at.lc + 2 * h]) = A[h];
+      *reinterpret_cast<f2*>(&mB[at.seg][at.lc + 2 * h]) = B[h];
     }
+    if (LINK && tid == 0) ticket = drawn;
     __syncthreads();
-    // The next tile's rows set out while this one's state is on its way.
     if (LINK) {
       n = ticket;
     } else if (++step == w.tiles) {
       step = 0;
-      n += gridDim.x;
+      n += at.walk;
     }
-    const int c = c0 + lane;
-    const bool ok = c < p.C;
-    const Chain link = {w.j - w.k, 1, w.k};
-    float h = 0.f;
+    float h = 0.f, fA = 1.f, fB = 0.f;
     if (warp == 0) {
       if (first && ok && slot != semx::kNone) {
         const bool fresh = p.m.fresh != nullptr && p.m.fresh[w.s] != 0;
         h = slot == semx::kRefused ? __int_as_float(0x7fffffff) : fresh ? 0.f : p.state[slot * p.C + c];
       }
       if (LINK && ok) {
-        float fA = 1.f, fB = h;
+        fB = h;
 #pragma unroll
         for (int s = 0; s < kSegs; ++s) {
           fA *= mA[s][lane];
@@ -493,31 +523,35 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
         leave_map(p, w.j, c, first ? 0.f : fA, fB);
       }
     }
+    // The next tile's rows set out while this one's state is on its way; warp 0 has the state to find
+    // first, unless it waits for others.
     const Tile next = tile_at<LINK, false, Q>(p, n, step);
-    fetch(next);
-    const bool other = next.any && next.ct != w.ct;
-    if (other && warp == 1) load_rates(p, next.ct, lane, &rates[turn ^ 1]);
+    if (LINK || warp != 0) fetch(next);
     if (warp == 0) {
-      if (!first) h = !LINK ? carry : w.live ? link_in(p, link, c, ok) : 0.f;
-      if (p.ckpt != nullptr && ok && w.live) p.ckpt[(int64_t)w.j * p.C + c] = h;
+      if (!first) h = !LINK ? carry : w.live ? link_in(p, Chain{w.j - w.k, 1, w.k}, c, ok) : 0.f;
+      // Every tile leaves its state, so that nothing waits for long whatever the offsets are; at once, for
+      // the next group waits.
+      if (LINK && ok) leave_state(p, w.j, c, first ? fB : fmaf(fA, h, fB));
+      const bool keeps = p.ckpt != nullptr && ok && w.live;
 #pragma unroll
       for (int s = 0; s < kSegs; ++s) {
+        if (s % (kUnit / SEG) == 0 && keeps && (s == 0 || s * SEG < w.n)) p.ckpt[((int64_t)w.unit + s * SEG / kUnit) * p.C + c] = h;
         const float after = fmaf(mA[s][lane], h, mB[s][lane]);
         mB[s][lane] = h;  // from here on the segment's entry state
         h = after;
       }
       carry = h;
-      // Every tile leaves its state, so that nothing waits for long whatever the offsets are.
-      if (LINK && ok) leave_state(p, w.j, c, h);
       if (w.live && last && ok && slot >= 0) p.state[slot * p.C + c] = h;
     }
     __syncthreads();
-    f2 hs[2] = {shared_pair(mB[seg], lc), shared_pair(mB[seg], lc + 2)};
-    char* out = reinterpret_cast<char*>(p.y) + ((int64_t)(w.row + seg * SEG) * p.C + c0 + lc) * element(ACC, p.bf16);
+    if (!LINK && warp == 0) fetch(next);
+    f2 hs[2] = {shared_pair(mB[at.seg], at.lc), shared_pair(mB[at.seg], at.lc + 2)};
+    char* out = reinterpret_cast<char*>(p.y) + ((int64_t)(w.row + at.seg * SEG) * p.C + at.c0 + at.lc) * element(ACC, p.bf16);
     const int64_t row = (int64_t)p.C * element(ACC, p.bf16);
-    const int end = nn > 0 ? most : 0;
+    const int end = at.nn > 0 ? most : 0;
 #pragma unroll
     for (int u = 0; u < SEG; ++u) {
+      if (u >= end) break;
       f2 y[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -525,61 +559,107 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
         y[k] = hs[k];
         if (gated) {
           const f2 z = pair_of<ACC>(rz[u], k, p.bf16);
-          const f2 s = rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)));
-          y[k] = mul2(y[k], mul2(z, s));
+          y[k] = mul2(y[k], mul2(z, rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)))));
         }
       }
-      if (u < end) {
-        const float2 lo = unpack2(y[0]), hi = unpack2(y[1]);
-        store_quad<ACC>(out + u * row, 0, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
-      }
+      const float2 lo = unpack2(y[0]), hi = unpack2(y[1]);
+      store_quad<ACC>(out + u * row, 0, p.bf16, at.nn, make_float4(lo.x, lo.y, hi.x, hi.y));
     }
     w = next;
-    turn ^= other;
+    buf ^= 1;
+  }
+}
+
+// The gradients of the thread's steps, from the last one on. a: decays, b: the states in front, d: the
+// gradients that reach h from y; gs: what reaches the last step from behind; sums over the steps of
+// rho dla, dr and di are added to `sum`.
+template <int ACC, int SEG, bool SLOW>
+__device__ __forceinline__ void gradient_steps(const GlParams& p, const Rates& rt, const Place& at, const Stage<ACC, SEG, 5>& st, int most,
+                                               int row0, const f2 (&a)[SEG][2], const f2 (&b)[SEG][2], const f2 (&d)[SEG][2],
+                                               f2 (&gs)[2], f2 (&sum)[3][2]) {
+  typedef typename RawQuad<ACC>::type Raw;
+  const int tid = threadIdx.x;
+  const bool gated = p.z != nullptr;
+  const int64_t out = ((int64_t)(row0 + at.seg * SEG) * p.C + at.c0 + at.lc) * element(ACC, p.bf16);
+  const int64_t row = (int64_t)p.C * element(ACC, p.bf16);
+#pragma unroll
+  for (int u = SEG - 1; u >= 0; --u) {
+    if (u >= most) continue;
+    const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
+    f2 dx[2], dr[2], di[2], dz[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = at.lc + 2 * k;
+      const f2 x = pair_of<ACC>(rx, k, p.bf16), speed = shared_pair(rt.speed, c);
+      const f2 gt = add2(d[u][k], gs[k]);
+      const f2 er = ex2_2(end2(gate_arg(pair_of<ACC>(rr, k, p.bf16), shared_pair(rt.r2, c))));
+      const f2 er1 = add2(er, both(1.f)), qr = rsqrt_2(er1);
+      f2 rho, m, same, gain;
+      decay2<SLOW>(qr, speed, shared_pair(rt.root, c), &rho, &m, &same, &gain);
+      // 1 / gain: 1 / q = (1 + er) q.
+      f2 inv = mul2(mul2(mul2(er1, qr), shared_pair(rt.inverse, c)), inverse_root_near(m));
+      const float2 gg = unpack2(gain);
+      float2 iv = unpack2(inv);
+      if constexpr (!SLOW) {
+        const float2 mm = unpack2(m);
+        if (mm.x > kNear) iv.x = 1.f / gg.x;
+        if (mm.y > kNear) iv.y = 1.f / gg.y;
+      }
+      iv.x = gg.x > kLeastGain ? iv.x : 0.f;  // at its least value no gradient goes through the gain
+      iv.y = gg.y > kLeastGain ? iv.y : 0.f;
+      inv = pack2(iv.x, iv.y);
+      gain = least2(gain);
+      const f2 ei = ex2_2(end2(gate_arg(pair_of<ACC>(ri, k, p.bf16), shared_pair(rt.i2, c))));
+      const f2 iota = rcp_2(add2(ei, both(1.f)));
+      const f2 ah = mul2(a[u][k], b[u][k]);
+      if (gated) {
+        const f2 z = pair_of<ACC>(st.v[3][u][tid], k, p.bf16);
+        const f2 ez = ex2_2(end2(mul2(z, both(-kLog2e)))), s = rcp_2(add2(ez, both(1.f)));
+        const f2 h = fma2(mul2(gain, iota), x, ah);
+        // silu'(z) = s (1 + z (1 - s)), 1 - s = ez s
+        dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, mul2(ez, s), both(1.f))));
+      }
+      const f2 gi = mul2(gt, iota);
+      dx[k] = mul2(gi, gain);
+      di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
+      const f2 through = mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv));
+      const f2 dla = fma2(gt, ah, mul2(through, both(-1.f)));
+      const f2 rd = mul2(rho, dla);
+      dr[k] = mul2(mul2(rd, mul2(er, rho)), mul2(speed, both(-1.f)));
+      gs[k] = mul2(a[u][k], gt);
+      sum[0][k] = add2(sum[0][k], rd);
+      sum[1][k] = add2(sum[1][k], dr[k]);
+      sum[2][k] = add2(sum[2][k], di[k]);
+    }
+    if (at.nn > 0) {
+      const int64_t o = out + u * row;
+      auto put = [&](void* to, const f2 (&v)[2]) {
+        const float2 lo = unpack2(v[0]), hi = unpack2(v[1]);
+        store_quad<ACC>(reinterpret_cast<char*>(to) + o, 0, p.bf16, at.nn, make_float4(lo.x, lo.y, hi.x, hi.y));
+      };
+      put(p.dx, dx);
+      put(p.dr, dr);
+      put(p.di, di);
+      if (gated) put(p.dz, dz);
+    }
   }
 }
 
 template <int ACC, int SEG, bool LINK>
 __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlParams p) {
   typedef typename RawQuad<ACC>::type Raw;
+  constexpr int Q = kSegs * SEG;
   extern __shared__ __align__(16) unsigned char raw[];
   Stage<ACC, SEG, 5>* stages = reinterpret_cast<Stage<ACC, SEG, 5>*>(raw);  // this tile's and the next one's
-  __shared__ __align__(16) float mA[kSegs][kCh], mB[kSegs][kCh], mG[kSegs][kCh];
-  __shared__ __align__(16) Rates rates[2];
+  __shared__ __align__(16) float maps[2][3][kSegs][kCh];  // A, B, and B of the adjoint's map
+  __shared__ __align__(16) float sums[4][3][kCh];         // a tile's (or a walked sequence's) sums, one row per warp
+  __shared__ __align__(16) Rates rt;
   __shared__ int ticket;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-  const int seg = tid / (kCh / 4), lc = tid % (kCh / 4) * 4;
+  const Place at = place_of(p);
   const bool gated = p.z != nullptr;
-  int n = blockIdx.x;
-  if (LINK) {
-    if (tid == 0) ticket = atomicAdd(p.ticket, 1);
-    __syncthreads();
-    n = ticket;
-    __syncthreads();
-  }
-  auto fetch = [&](const Tile& w, Stage<ACC, SEG, 5>& st) {  // the thread's own rows, on their way into its own places
-    const int nn = min(p.C - w.ct * kCh - lc, 4), most = nn > 0 ? w.n - seg * SEG : 0;
-    const int row = most > 0 ? w.row + seg * SEG : 0, ch = most > 0 ? w.ct * kCh + lc : 0;
-    auto bring = [&](int op, const void* from, int64_t ld) {
-      const char* at = reinterpret_cast<const char*>(from) + ((int64_t)row * (int)ld + ch) * element(ACC, p.bf16);
-      const int64_t step = ld * element(ACC, p.bf16);
-#pragma unroll
-      for (int u = 0; u < SEG; ++u, at += step) {
-        if constexpr (ACC == kAny) st.v[op][u][tid] = load_quad<ACC>(at, 0, p.bf16, u < most ? nn : 0);
-        else bring_quad<ACC>(&st.v[op][u][tid], at, u < most);
-      }
-    };
-    bring(0, p.x, p.ldx);
-    bring(1, p.r, p.ldr);
-    bring(2, p.i, p.ldi);
-    bring(4, p.dy, p.C);
-    if (gated) bring(3, p.z, p.ldz);
-  };
-  int step = 0, turn = 0, at = 0;
-  constexpr int Q = kSegs * SEG;
-  Tile w = tile_at<LINK, true, Q>(p, n, 0);
-  fetch(w, stages[0]);
-  if (w.any && warp == 1) load_rates(p, w.ct, lane, &rates[0]);
+  if (LINK && tid == 0) ticket = atomicAdd(&p.ticket[at.ct], 1);
+  if (warp == 1) load_rates(p, at.c0, lane, &rt);
   unused_rows(p, [&](int64_t row, int c, int k) {
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     store_quad<ACC>(p.dx, row * p.C + c, p.bf16, k, zero);
@@ -587,89 +667,98 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
     store_quad<ACC>(p.di, row * p.C + c, p.bf16, k, zero);
     if (gated) store_quad<ACC>(p.dz, row * p.C + c, p.bf16, k, zero);
   });
+  __syncthreads();
+  int n = LINK ? ticket : (int)(blockIdx.x / (unsigned)p.ctiles), step = 0, buf = 0;
+  __syncthreads();
+  auto fetch = [&](const Tile& w, Stage<ACC, SEG, 5>& st) {
+    bring(p, at, w, st, 0, p.x, p.ldx);
+    bring(p, at, w, st, 1, p.r, p.ldr);
+    bring(p, at, w, st, 2, p.i, p.ldi);
+    bring(p, at, w, st, 4, p.dy, p.C);
+    if (gated) bring(p, at, w, st, 3, p.z, p.ldz);
+  };
+  const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[at.lc]);
+  const bool slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+  const int c = at.c0 + lane;  // warp 0: a lane per channel
+  const bool ok = c < p.C;
+  Tile w = tile_at<LINK, true, Q>(p, n, 0);
+  fetch(w, stages[0]);
   float carry = 0.f;  // warp 0: what reaches the walked sequence's tile from behind
+  int summed = -1;    // row of partial sums that waits in shared memory
+  auto write_sums = [&]() {
+    if (summed < 0 || warp == 0 || !ok) return;
+    const int k = warp - 1;
+    const float v = sums[0][k][lane] + sums[1][k][lane] + sums[2][k][lane] + sums[3][k][lane];
+    p.part[((int64_t)summed * 3 + k) * p.C + c] = k == 0 ? -rt.slope[lane] * v : v;
+  };
   f2 sum[3][2];
 #pragma unroll
   for (int k = 0; k < 3; ++k) sum[k][0] = sum[k][1] = both(0.f);
   while (w.any) {
-    const int c0 = w.ct * kCh, nn = min(4, p.C - c0 - lc);
     const bool end = w.k + 1 >= w.tiles;  // nothing behind it
+    const int most = w.n - at.seg * SEG;  // steps of the thread that exist
     const bool busy = warp * (kSegs / 4) * SEG < w.n;
-    const int most = w.n - seg * SEG;  // steps of the thread that exist
-    if (LINK && tid == 0) ticket = atomicAdd(p.ticket, 1);
-    const float entry = warp == 0 && w.live && c0 + lane < p.C ? p.ckpt[(int64_t)w.j * p.C + c0 + lane] : 0.f;
-    __syncthreads();  // rates; the maps of the tile before have been read
-    const Rates& rt = rates[turn];
-    const Stage<ACC, SEG, 5>& st = stages[at];
-    const float4 sp = *reinterpret_cast<const float4*>(&rt.speed[lc]);
-    const bool is_slow = fmaxf(fmaxf(sp.x, sp.y), fmaxf(sp.z, sp.w)) <= kNear;
+    int drawn = 0;  // on its way while the tile's steps are folded
+    if (LINK && tid == 0) drawn = atomicAdd(&p.ticket[at.ct], 1);
+    const float entry = warp == 0 && w.live && ok ? p.ckpt[(int64_t)w.unit * p.C + c] : 0.f;
+    const Stage<ACC, SEG, 5>& st = stages[buf];
+    float(*mA)[kCh] = maps[buf][0], (*mB)[kCh] = maps[buf][1], (*mG)[kCh] = maps[buf][2];
     // b: gain iota x, later the state in front of the step; d: the gradient that reaches h from y.
     f2 a[SEG][2], b[SEG][2], d[SEG][2];
     f2 A[2] = {both(1.f), both(1.f)}, B[2] = {both(0.f), both(0.f)}, G[2] = {both(0.f), both(0.f)};
     copies_done();
     if (busy) {
-      auto steps = [&](auto slow) {
-#pragma unroll
-        for (int u = 0; u < SEG; ++u) {
-          const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, lc + 2 * h)));
-            f2 rho, m, gain;
-            decay2<decltype(slow)::value>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, lc + 2 * h),
-                                          shared_pair(rt.root, lc + 2 * h), &rho, &m, &a[u][h], &gain);
-            const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, lc + 2 * h))), both(1.f)));
-            b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
-            d[u][h] = pair_of<ACC>(rg, h, p.bf16);
-            if (gated) {
-              const f2 z = pair_of<ACC>(st.v[3][u][tid], h, p.bf16);
-              d[u][h] = mul2(d[u][h], mul2(z, rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)))));
-            }
-          }
-        }
-      };
-      if (is_slow) steps(Is<true>());
-      else steps(Is<false>());
+      if (slow) gate_steps<ACC, SEG, true>(p, rt, at.lc, st, a, b);
+      else gate_steps<ACC, SEG, false>(p, rt, at.lc, st, a, b);
 #pragma unroll
       for (int u = 0; u < SEG; ++u) {
+        const Raw rg = st.v[4][u][tid];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          d[u][h] = pair_of<ACC>(rg, h, p.bf16);
+          if (gated) {
+            const f2 z = pair_of<ACC>(st.v[3][u][tid], h, p.bf16);
+            d[u][h] = mul2(d[u][h], mul2(z, rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)))));
+          }
+        }
+      }
+    }
+    if (most < SEG) {  // rows behind the last one keep the state
+#pragma unroll
+      for (int u = 0; u < SEG; ++u)
         if (u >= most) {
           a[u][0] = a[u][1] = both(1.f);
           b[u][0] = b[u][1] = d[u][0] = d[u][1] = both(0.f);
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          A[h] = mul2(A[h], a[u][h]);
-          B[h] = fma2(a[u][h], B[h], b[u][h]);
-        }
-      }
-      // What reaches the step in front of the segment: a_t (d_t + what reaches step t from behind).
-#pragma unroll
-      for (int u = SEG - 1; u >= 0; --u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) G[h] = mul2(a[u][h], add2(d[u][h], G[h]));
-    } else {
-#pragma unroll
-      for (int u = 0; u < SEG; ++u) {
-        a[u][0] = a[u][1] = both(1.f);
-        b[u][0] = b[u][1] = d[u][0] = d[u][1] = both(0.f);
-      }
     }
+#pragma unroll
+    for (int u = 0; u < SEG; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        A[h] = mul2(A[h], a[u][h]);
+        B[h] = fma2(a[u][h], B[h], b[u][h]);
+      }
+    // What reaches the step in front of the segment: a_t (d_t + what reaches step t from behind).
+#pragma unroll
+    for (int u = SEG - 1; u >= 0; --u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) G[h] = mul2(a[u][h], add2(d[u][h], G[h]));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      *reinterpret_cast<f2*>(&mA[seg][lc + 2 * h]) = A[h];
-      *reinterpret_cast<f2*>(&mB[seg][lc + 2 * h]) = B[h];
-      *reinterpret_cast<f2*>(&mG[seg][lc + 2 * h]) = G[h];
+      *reinterpret_cast<f2*>(&mA[at.seg][at.lc + 2 * h]) = A[h];
+      *reinterpret_cast<f2*>(&mB[at.seg][at.lc + 2 * h]) = B[h];
+      *reinterpret_cast<f2*>(&mG[at.seg][at.lc + 2 * h]) = G[h];
     }
+    if (LINK && tid == 0) ticket = drawn;
     __syncthreads();
+    write_sums();  // of the tile before
+    summed = -1;
     if (LINK) {
       n = ticket;
     } else if (++step == w.tiles) {
       step = 0;
-      n += gridDim.x;
+      n += at.walk;
     }
-    const int c = c0 + lane;
-    const bool ok = c < p.C;
-    const Chain link = {w.j - w.k + w.tiles - 1, -1, w.tiles - 1 - w.k};
     float fA = 1.f, fG = 0.f;
     if (LINK && warp == 0) {
 #pragma unroll
@@ -680,9 +769,7 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
       if (ok) leave_map(p, w.j, c, end ? 0.f : fA, fG);
     }
     const Tile next = tile_at<LINK, true, Q>(p, n, step);
-    fetch(next, stages[at ^ 1]);
-    const bool other = next.any && next.ct != w.ct;
-    if (other && warp == 1) load_rates(p, next.ct, lane, &rates[turn ^ 1]);
+    if (LINK || warp != 0) fetch(next, stages[buf ^ 1]);
     if (warp == 0) {
       float h = entry;
 #pragma unroll
@@ -691,7 +778,8 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
         mB[s][lane] = h;
         h = after;
       }
-      float g = end ? 0.f : !LINK ? carry : w.live ? link_in(p, link, c, ok) : 0.f;
+      float g = 0.f;
+      if (!end) g = !LINK ? carry : w.live ? link_in(p, Chain{w.j - w.k + w.tiles - 1, -1, w.tiles - 1 - w.k}, c, ok) : 0.f;
       if (LINK && ok) leave_state(p, w.j, c, fmaf(fA, g, fG));
 #pragma unroll
       for (int s = kSegs - 1; s >= 0; --s) {
@@ -702,8 +790,9 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
       carry = g;
     }
     __syncthreads();
+    if (!LINK && warp == 0) fetch(next, stages[buf ^ 1]);
     if (busy) {
-      f2 hs[2] = {shared_pair(mB[seg], lc), shared_pair(mB[seg], lc + 2)};
+      f2 hs[2] = {shared_pair(mB[at.seg], at.lc), shared_pair(mB[at.seg], at.lc + 2)};
 #pragma unroll
       for (int u = 0; u < SEG; ++u)
 #pragma unroll
@@ -712,97 +801,32 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
           b[u][k] = hs[k];
           hs[k] = after;
         }
-      const int64_t out = ((int64_t)(w.row + seg * SEG) * p.C + c0 + lc) * element(ACC, p.bf16);
-      const int64_t row = (int64_t)p.C * element(ACC, p.bf16);
-      f2 gs[2] = {shared_pair(mG[seg], lc), shared_pair(mG[seg], lc + 2)};
-      auto steps = [&](auto slow) {
-#pragma unroll
-        for (int u = SEG - 1; u >= 0; --u) {
-          if (u >= most) continue;
-          const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
-          f2 dx[2], dr[2], di[2], dz[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const f2 x = pair_of<ACC>(rx, k, p.bf16), speed = shared_pair(rt.speed, lc + 2 * k);
-            const f2 gt = add2(d[u][k], gs[k]);
-            const f2 er = ex2_2(end2(gate_arg(pair_of<ACC>(rr, k, p.bf16), shared_pair(rt.r2, lc + 2 * k))));
-            const f2 er1 = add2(er, both(1.f)), qr = rsqrt_2(er1);
-            f2 rho, m, at, gain;
-            decay2<decltype(slow)::value>(qr, speed, shared_pair(rt.root, lc + 2 * k), &rho, &m, &at, &gain);
-            // 1 / gain: 1 / q = (1 + er) q.
-            f2 inv = mul2(mul2(mul2(er1, qr), shared_pair(rt.inverse, lc + 2 * k)), inverse_root_near(m));
-            const float2 gg = unpack2(gain);
-            float2 iv = unpack2(inv);
-            if constexpr (!decltype(slow)::value) {
-              const float2 mm = unpack2(m);
-              if (mm.x > kNear) iv.x = 1.f / gg.x;
-              if (mm.y > kNear) iv.y = 1.f / gg.y;
-            }
-            iv.x = gg.x > kLeastGain ? iv.x : 0.f;  // at its least value no gradient goes through the gain
-            iv.y = gg.y > kLeastGain ? iv.y : 0.f;
-            inv = pack2(iv.x, iv.y);
-            gain = least2(gain);
-            const f2 ei = ex2_2(end2(gate_arg(pair_of<ACC>(ri, k, p.bf16), shared_pair(rt.i2, lc + 2 * k))));
-            const f2 iota = rcp_2(add2(ei, both(1.f)));
-            const f2 ah = mul2(a[u][k], b[u][k]);
-            if (gated) {
-              const f2 z = pair_of<ACC>(st.v[3][u][tid], k, p.bf16);
-              const f2 ez = ex2_2(end2(mul2(z, both(-kLog2e)))), s = rcp_2(add2(ez, both(1.f)));
-              const f2 h = fma2(mul2(gain, iota), x, ah);
-              // silu'(z) = s (1 + z (1 - s)), 1 - s = ez s
-              dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, mul2(ez, s), both(1.f))));
-            }
-            const f2 gi = mul2(gt, iota);
-            dx[k] = mul2(gi, gain);
-            di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
-            const f2 through = mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv));
-            const f2 dla = fma2(gt, ah, mul2(through, both(-1.f)));
-            const f2 rd = mul2(rho, dla);
-            dr[k] = mul2(mul2(rd, mul2(er, rho)), mul2(speed, both(-1.f)));
-            gs[k] = mul2(a[u][k], gt);
-            sum[0][k] = add2(sum[0][k], rd);
-            sum[1][k] = add2(sum[1][k], dr[k]);
-            sum[2][k] = add2(sum[2][k], di[k]);
-          }
-          if (nn > 0) {
-            const int64_t o = out + u * row;
-            auto put = [&](void* to, const f2 (&v)[2]) {
-              const float2 lo = unpack2(v[0]), hi = unpack2(v[1]);
-              store_quad<ACC>(reinterpret_cast<char*>(to) + o, 0, p.bf16, nn, make_float4(lo.x, lo.y, hi.x, hi.y));
-            };
-            put(p.dx, dx);
-            put(p.dr, dr);
-            put(p.di, di);
-            if (gated) put(p.dz, dz);
-          }
-        }
-      };
-      if (is_slow) steps(Is<true>());
-      else steps(Is<false>());
+      f2 gs[2] = {shared_pair(mG[at.seg], at.lc), shared_pair(mG[at.seg], at.lc + 2)};
+      if (slow) gradient_steps<ACC, SEG, true>(p, rt, at, st, most, w.row, a, b, d, gs, sum);
+      else gradient_steps<ACC, SEG, false>(p, rt, at, st, most, w.row, a, b, d, gs, sum);
     }
     if (p.part != nullptr && (LINK || w.k == 0)) {
-      __syncthreads();
+      // The four segments of the warp, then (behind the next barrier) the warps.
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        *reinterpret_cast<f2*>(&mA[seg][lc + 2 * k]) = sum[0][k];
-        *reinterpret_cast<f2*>(&mB[seg][lc + 2 * k]) = sum[1][k];
-        *reinterpret_cast<f2*>(&mG[seg][lc + 2 * k]) = sum[2][k];
-        sum[0][k] = sum[1][k] = sum[2][k] = both(0.f);
-      }
-      __syncthreads();
-      if (warp < 3 && ok) {
-        float(*m)[kCh] = warp == 0 ? mA : warp == 1 ? mB : mG;
-        float acc = 0.f;
+      for (int k = 0; k < 3; ++k)
 #pragma unroll
-        for (int s = 0; s < kSegs; ++s) acc += m[s][lane];
-        const int64_t row = LINK ? w.j : w.s;
-        p.part[(row * 3 + warp) * p.C + c] = warp == 0 ? -rt.slope[lane] * acc : acc;
-      }
+        for (int h = 0; h < 2; ++h) {
+          float2 v = unpack2(sum[k][h]);
+#pragma unroll
+          for (int m = kCh / 4; m < 32; m *= 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, m);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, m);
+          }
+          if (lane < kCh / 4) *reinterpret_cast<float2*>(&sums[warp][k][at.lc + 2 * h]) = v;
+          sum[k][h] = both(0.f);
+        }
+      summed = LINK ? w.j : w.s;
     }
     w = next;
-    turn ^= other;
-    at ^= 1;
+    buf ^= 1;
   }
+  __syncthreads();
+  write_sums();
 }
 
 // One token per sequence: a thread has four channels of one, a CTA a run of sequences (their slots
@@ -911,7 +935,7 @@ int gl_validate(const SemxGatedLruArgs* a, bool bwd, GlParams* p) {
       semx::all_aligned({a->x, a->r, a->i, a->z, a->y, a->dy, a->dx, a->d_r, a->d_i, a->dz}, a->bf16 ? 8 : 16) &&
       semx::aligned(a->state, 16))
     p->access = a->bf16 ? kBf16 : kFp32;
-  semx::set_pieces(&p->m, kSegs * seg_steps(a->bf16 != 0));
+  semx::set_pieces(&p->m, kSegs * (bwd ? kBwdSeg : kFwdSeg));
   return SEMX_OK;
 }
 
@@ -923,7 +947,8 @@ bool gl_linked(const GlParams& p) {
 }
 
 size_t link_bytes(const GlParams& p) {
-  return gl_linked(p) ? 16 + (size_t)p.m.pieces * p.C * (sizeof(ulonglong2) + sizeof(unsigned long long)) : 0;
+  const size_t tickets = ((size_t)p.ctiles * sizeof(int) + 15) / 16 * 16;
+  return gl_linked(p) ? tickets + (size_t)p.m.pieces * p.C * (sizeof(ulonglong2) + sizeof(unsigned long long)) : 0;
 }
 int64_t part_rows(const GlParams& p) { return gl_linked(p) ? p.m.pieces : p.m.S; }
 
@@ -940,33 +965,36 @@ int set_links(GlParams* p, void* workspace, cudaStream_t st) {
   return SEMX_OK;
 }
 
-template <int ACC, int SEG>
+template <int ACC>
 int launch_gl(bool bwd, const GlParams& p, cudaStream_t st) {
   const bool linked = p.ticket != nullptr;
-  const int64_t works = (linked ? p.m.pieces : p.m.S) * p.ctiles;
+  const int64_t works = linked ? p.m.pieces : p.m.S;  // of each channel tile
   if (works == 0) return SEMX_OK;
-  if (works >= ((int64_t)1 << 30)) return semx::fail(SEMX_ERR_SHAPE, "gated_lru: too many tiles");
-  // As many CTAs as run at once: each takes tile after tile, and fetches the next one's rows early.
-  const int64_t most = kSms * (bwd ? kBwdCtas : kFwdCtas);
-  const unsigned n = (unsigned)(works < most ? works : most);
+  // As many CTAs as run at once, the same number for each channel tile: each takes tile after tile, and
+  // fetches the next one's rows early.
+  int64_t each = kSms * (bwd ? kBwdCtas : kFwdCtas) / p.ctiles;
+  if (each > works) each = works;
+  if (each < 1) each = 1;
+  const unsigned n = (unsigned)(each * p.ctiles);
+  constexpr size_t kStatic = 15 * 1024;  // shared memory of fixed size, at most
 #define SEMX_GL(KERNEL, STAGES)                                      \
   do {                                                               \
-    if (!semx::allow_smem(KERNEL, STAGES)) return SEMX_ERR_LAUNCH;   \
+    if ((STAGES) + kStatic > 48 * 1024 && !semx::allow_smem(KERNEL, (STAGES) + 48 * 1024)) return SEMX_ERR_LAUNCH; \
     KERNEL<<<n, kT, STAGES, st>>>(p);                                \
     return semx::check_launch("gated_lru kernel");                   \
   } while (0)
-  constexpr size_t fwd = sizeof(Stage<ACC, SEG, 4>), back = 2 * sizeof(Stage<ACC, SEG, 5>);
-  if (!bwd && linked) SEMX_GL((gated_lru_fwd_kernel<ACC, SEG, true>), fwd);
-  if (!bwd) SEMX_GL((gated_lru_fwd_kernel<ACC, SEG, false>), fwd);
-  if (linked) SEMX_GL((gated_lru_bwd_kernel<ACC, SEG, true>), back);
-  SEMX_GL((gated_lru_bwd_kernel<ACC, SEG, false>), back);
+  constexpr size_t fwd = sizeof(Stage<ACC, kFwdSeg, 4>), back = 2 * sizeof(Stage<ACC, kBwdSeg, 5>);
+  if (!bwd && linked) SEMX_GL((gated_lru_fwd_kernel<ACC, kFwdSeg, true>), fwd);
+  if (!bwd) SEMX_GL((gated_lru_fwd_kernel<ACC, kFwdSeg, false>), fwd);
+  if (linked) SEMX_GL((gated_lru_bwd_kernel<ACC, kBwdSeg, true>), back);
+  SEMX_GL((gated_lru_bwd_kernel<ACC, kBwdSeg, false>), back);
 #undef SEMX_GL
 }
 
 int dispatch_gl(bool bwd, const GlParams& p, cudaStream_t st) {
-  if (p.access == kBf16) return launch_gl<kBf16, seg_steps(true)>(bwd, p, st);
-  if (p.access == kFp32) return launch_gl<kFp32, seg_steps(false)>(bwd, p, st);
-  return p.bf16 ? launch_gl<kAny, seg_steps(true)>(bwd, p, st) : launch_gl<kAny, seg_steps(false)>(bwd, p, st);
+  if (p.access == kBf16) return launch_gl<kBf16>(bwd, p, st);
+  if (p.access == kFp32) return launch_gl<kFp32>(bwd, p, st);
+  return launch_gl<kAny>(bwd, p, st);
 }
 
 // (The sizes do not depend on addresses.)
@@ -1004,7 +1032,8 @@ size_t semx_gated_lru_args_size(void) { return sizeof(SemxGatedLruArgs); }
 size_t semx_gated_lru_ckpt_bytes(const SemxGatedLruArgs* a) {
   if (a == nullptr) return 0;
   int rc;
-  const GlParams p = gl_sizes(a, false, &rc);
+  GlParams p = gl_sizes(a, false, &rc);
+  semx::set_pieces(&p.m, kUnit);
   return rc == SEMX_OK ? (size_t)p.m.pieces * p.C * sizeof(float) : 0;
 }
 

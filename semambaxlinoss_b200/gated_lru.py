@@ -135,7 +135,7 @@ def gated_lru_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, rate: torc
     and fresh), of one type, bf16 or fp32, at any row stride. rate, r_bias, i_bias: (C,).
 
     Training: gradients flow to every operand, every sequence starts from zeros; the forward keeps
-    the state of every 64th (fp32: 32nd) step in fp32. Prompts: ``state`` (entries, C) fp32 is read and updated
+    the state of every 32nd step in fp32. Prompts: ``state`` (entries, C) fp32 is read and updated
     in place; refused while a gradient is wanted."""
     op = "gated_lru_scan"
     S, rows, L = batch(op, x, cu_seqlens)

@@ -68,17 +68,15 @@ def test_recurrence_arguments_are_checked_on_the_host():
 def test_recurrence_sizes():
     lib = _lib.load()
     a = _lru_args()
-    # fp32: four tiles of 32 steps each, linked: a map (16 bytes) and a state (8) per tile and channel.
+    # A kept state every 32 steps. Linked: a map (16 bytes) and a state (8) per tile of 64 steps (backward
+    # 32) and channel, and a ticket per 32 channels.
     assert lib.semx_gated_lru_ckpt_bytes(ctypes.byref(a)) == 2 * 4 * 12 * 4
-    links = 16 + 8 * 12 * 24
-    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == links
-    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 1) == links + 8 * 3 * 12 * 4
-    a.bf16 = 1  # tiles of 64 steps
-    assert lib.semx_gated_lru_ckpt_bytes(ctypes.byref(a)) == 2 * 2 * 12 * 4
+    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == 16 + 4 * 12 * 24
+    assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 1) == 16 + 8 * 12 * 24 + 8 * 3 * 12 * 4
     a.S, a.rows = 1000, 100000  # sequences enough to walk them
     assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == 0
     assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 1) == 1000 * 3 * 12 * 4
-    a.S, a.rows, a.L = 4, 200, 50  # one tile each
+    a.S, a.rows, a.L = 10, 200, 20  # one tile each
     assert lib.semx_gated_lru_workspace_bytes(ctypes.byref(a), 0) == 0
 
 
