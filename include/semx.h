@@ -784,8 +784,8 @@ int semx_gated_lru_step(const SemxGatedLruArgs* args, semx_stream_t stream);
  * Gated projection of a feed-forward block: both projections, the activation and their product.
  *   [u | g] = x W^T + bias;  h = u act(g)   (act 0: silu, 1: gelu with the normal distribution)
  * x (rows, D) at row stride ldx, w (2 H, D) contiguous (the value's rows, then the gate's), h, dh
- * (rows, H), dx (rows, D) and dw contiguous; all bf16 when `bf16` is set, else fp32. bias, db
- * (2 H, each may be NULL) fp32. Sums are fp32; fp32 operands keep 2^-24 of each product (as three
+ * (rows, H), dx (rows, D) and dw contiguous; all bf16 when `bf16` is set, else fp32. bias
+ * (2 H, may be NULL) by bias_bf16, db (2 H, may be NULL) fp32. Sums are fp32; fp32 operands keep 2^-24 of each product (as three
  * bf16 parts; an infinity among them gives NaN).
  * A training forward passes saved (semx_gated_linear_saved_bytes(): u and g in fp32, 16-byte
  * aligned); the backward reads it and writes dx, dw and db (each may be NULL), sums in a fixed
@@ -795,11 +795,11 @@ typedef struct SemxGatedLinearArgs {
   uint32_t struct_size;
   int32_t bf16;
   int32_t act;
-  int32_t reserved;
+  int32_t bias_bf16;
   int64_t rows, D, H, ldx;
   const void* x;
   const void* w;
-  const float* bias;
+  const void* bias;
   void* h;
   float* saved;
   const void* dh;

@@ -292,7 +292,7 @@ class SemxGatedLinearArgs(ctypes.Structure):
         ("struct_size", ctypes.c_uint32),
         ("bf16", ctypes.c_int32),
         ("act", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
+        ("bias_bf16", ctypes.c_int32),
     ] + [(name, ctypes.c_int64) for name in ("rows", "D", "H", "ldx")] + [
         (name, ctypes.c_void_p) for name in ("x", "w", "bias", "h", "saved", "dh", "dx", "dw", "db", "workspace")]
 

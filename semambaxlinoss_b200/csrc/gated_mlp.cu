@@ -9,11 +9,15 @@
 // to bf16 they would put their rounding into dx and dW on top of that of du and dg), then two
 // products run on the same kernel with other operand orders.
 //
-// Products: tcgen05 (one CTA per SM, persistent; one warp loads tiles by TMA, one issues the
-// products into tensor memory, four write the accumulators out; two accumulators, so that writing
-// a tile overlaps the next one's products). fp32 operands are split into three bf16 parts whose sum
-// is the value up to its last bit; six of the nine products of parts (all above 2^-24 of the
-// result) run one behind the other into the same accumulator.
+// Products: tcgen05 on pairs of SMs (a cluster of two CTAs has 256 rows of the result, each CTA's tensor
+// memory its 128; each brings its rows of A and half of B's by TMA, and one thread of the pair issues the
+// products for both). Persistent: in each CTA one warp loads and eight write the accumulators out; two
+// accumulators, so that writing a tile overlaps the next one's products.
+// fp32 operands are split into three bf16 parts whose sum is the value up to its last bit; six of the nine
+// products of parts are taken (the others are below 2^-24 of the result). The tensor cores cut where
+// an addition rounds, which shows over thousands of additions: so the large products (first parts) are
+// summed in tensor memory over 128 of the depth at a time, and those sums in registers; the small ones
+// have an accumulator of their own.
 // Few rows (up to 8): the weights' bytes are the bound, and a warp per pair of columns streams them.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -29,34 +33,33 @@ namespace {
 using semx::cdiv;
 using semx_scan::sigmoid;
 
-constexpr int kM = 128, kK = 64;  // rows of a tile, depth of a stage (128 bytes of bf16)
-constexpr int kGemmT = 192;       // warps 0 to 3 write out, 4 loads, 5 issues products
-constexpr int kSms = 148;
+constexpr int kM = 128, kK = 64;    // rows of a CTA's tile, depth of a stage (128 bytes of bf16)
+constexpr int kEpi = 8;             // warps that write out: two for each quarter of the rows
+constexpr int kGemmT = (kEpi + 2) * 32;  // then one that loads and one that issues products
+constexpr int kSms = 148, kPairs = kSms / 2;
 constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
-constexpr int kBufRow = 36;       // floats of a row of a warp's 32 x 32 exchange buffer
-constexpr int kParts = 3;         // bf16 parts of an fp32 value
+constexpr int kBufRow = 36;         // floats of a row of a warp's 32 x 32 exchange buffer
+constexpr int kParts = 3;           // bf16 parts of an fp32 value
+constexpr int kDrain = 2;           // stages whose large products one accumulator takes (fp32)
 
 __device__ unsigned int g_gemm_timeouts;
 
 enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
 
-// Parts of A and B in the order of their products, small ones first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
-__device__ __forceinline__ int part_a(int pair) { return (0x001102 >> (4 * pair)) & 0xf; }
-__device__ __forceinline__ int part_b(int pair) { return (0x010120 >> (4 * pair)) & 0xf; }
-
 struct GemmParams {
   int64_t M, N;           // rows and columns of the result (kFwd: N = H; kDw: M = H, once per half)
   int tiles_m, tiles_n;   // kDw: tiles_m of one half
   int tiles;              // in all
-  int kper, khalf;        // stages of one pair of parts, and of one half of them (kDx: u, then g)
-  int pairs, splits;      // products of parts; slices of the depth
+  int depth, khalf;       // stages in all, and of one half of the depth (kDx: u, then g)
+  int splits;             // slices of the depth
   void* out;              // kFwd: h
   int64_t ldo;
   int out_bf16;
   float* u;               // kFwd: u and g in front of the activation, or NULL
   float* g;
   int64_t ldu;
-  const float* bias;      // (2 H) or NULL
+  const void* bias;       // (2 H) or NULL
+  int bias_bf16;
   int gelu;
   float* part;            // with splits: (splits, result) sums, kFwd: (splits, 2, M, N)
 };
@@ -75,26 +78,57 @@ __device__ __forceinline__ float act_slope(float g, int gelu) {
 
 // -- tensor core plumbing -----------------------------------------------------------------------
 
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+// A copy into this CTA's shared memory that reports to `bar`, a barrier of the pair (its address in the
+// cluster's window).
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
           semx::tc::smem_addr(dst)),
-      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(semx::tc::smem_addr(bar))
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
+}
+// Address of CTA `rank`'s copy of a shared variable in the cluster's window.
+__device__ __forceinline__ uint32_t in_cluster(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(semx::tc::smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 __device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(semx::tc::smem_addr(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(semx::tc::smem_addr(bar)) : "memory");
+__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
+}
+// Arrives on this barrier of both CTAs once every product issued before has completed.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   semx::tc::smem_addr(bar)),
+               "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(semx::tc::smem_addr(slot)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
 }
 // Descriptor of an operand in 128-byte rows with the 128-byte swizzle. K-major: a row is 64 values of
 // the depth, 8-row groups 1024 bytes apart. MN-major: a row is 64 neighbouring M or N values at one
@@ -129,10 +163,11 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
   return false;
 }
 
-constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
-constexpr int stage_bytes(int bn) { return (kM + bn) * kK * 2; }
+// Shared memory is a ring of slots: one part of a stage's rows of A (128) and of B (half of the tile's).
+constexpr int slot_bytes(int bn) { return (kM + bn / 2) * kK * 2; }
+constexpr int slots_of(int bn) { return bn == 256 ? 5 : bn == 128 ? 7 : 8; }
 constexpr size_t gemm_smem(int bn) {
-  return 1024 + (size_t)stages_of(bn) * stage_bytes(bn) + 4 * 32 * kBufRow * sizeof(float);
+  return 1024 + (size_t)slots_of(bn) * slot_bytes(bn) + kEpi * 32 * kBufRow * sizeof(float);
 }
 
 struct Tile {
@@ -204,170 +239,269 @@ __device__ __forceinline__ void write_block(float* buf, const float (&v)[32], vo
   __syncwarp();
 }
 
-// Result of one mode. BN: columns of the accumulator (kFwd: BN / 2 of u, then as many of g).
-template <int MODE, int BN>
-__global__ void __launch_bounds__(kGemmT, 1) gemm_kernel(const __grid_constant__ CUtensorMap map_a,
-                                                         const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
-  constexpr int ST = stages_of(BN), BYTES = stage_bytes(BN), ABYTES = kM * kK * 2;
+// Result of one mode. BN: columns of the accumulator (kFwd: BN / 2 of u, then as many of g). PARTS: 1
+// (bf16), or 3 (fp32; BN 128).
+template <int MODE, int BN, int PARTS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
+  constexpr int ST = slots_of(BN), BYTES = slot_bytes(BN), ABYTES = kM * kK * 2;
   constexpr bool A_MN = MODE == kDw, B_MN = MODE != kFwd;
-  constexpr int CN = MODE == kFwd ? BN / 2 : BN;  // columns of the result in a tile
+  constexpr int CN = MODE == kFwd ? BN / 2 : BN;        // columns of the result in a tile
+  constexpr int COLS = (PARTS > 1 ? 4 : 2) * BN;        // of tensor memory: two accumulators, fp32 two more for the small products
+  static_assert(COLS <= 512, "tensor memory");
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drained;
+  __shared__ uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], small_full[2], small_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
-  uint8_t* stage0 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  float* bufs = reinterpret_cast<float*>(stage0 + ST * BYTES);
+  uint8_t* slot0 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  float* bufs = reinterpret_cast<float*>(slot0 + ST * BYTES);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
-      semx::tc::mbar_init(&full[s], 1);
+      semx::tc::mbar_init(&full[s], 1);   // of CTA 0: both CTAs' copies
       semx::tc::mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       semx::tc::mbar_init(&acc_full[b], 1);
-      semx::tc::mbar_init(&acc_empty[b], 4);
+      semx::tc::mbar_init(&acc_empty[b], 2 * kEpi);  // of CTA 0: both CTAs' warps
+      semx::tc::mbar_init(&small_full[b], 1);
+      semx::tc::mbar_init(&small_empty[b], 2 * kEpi);
     }
     semx::tc::mbar_init(&drained, 1);
     dead = 0;
   }
-  if (warp == 0) semx::tc::tmem_alloc(&tmem_slot, 2 * BN);
+  if (warp == 0) tmem_alloc_pair(&tmem_slot, COLS);
   semx::tc::fence_before_sync();
   __syncthreads();
+  cluster_sync();
   semx::tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const int works = p.tiles * p.splits, depth = p.kper * p.pairs;
+  const int works = p.tiles * p.splits, pair0 = blockIdx.x / 2, pairs = gridDim.x / 2;
+  auto slice = [&](const Tile& t, int* k0, int* k1) {
+    *k0 = (int)((int64_t)p.depth * t.split / p.splits);
+    *k1 = (int)((int64_t)p.depth * (t.split + 1) / p.splits);
+  };
 
-  if (warp == 4) {
+  if (warp == kEpi) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int w = blockIdx.x; w < works && ok; w += gridDim.x) {
+      for (int w = pair0; w < works && ok; w += pairs) {
         const Tile t = tile_at(p, w);
-        const int k0 = (int)((int64_t)depth * t.split / p.splits), k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % ST;
-          ok = wait_phase(&empty[s], ((it / ST) & 1) ^ 1, &dead);
-          if (!ok) break;
-          expect_bytes(&full[s], BYTES);
-          uint8_t *sa = stage0 + s * BYTES, *sb = sa + ABYTES;
-          const int pair = k / p.kper, in = k % p.kper, kh = in / p.khalf, kk = (in % p.khalf) * kK;
-          const int pa = p.pairs > 1 ? part_a(pair) : 0, pb = p.pairs > 1 ? part_b(pair) : 0;
-          if (MODE == kDw) {
-            for (int b = 0; b < kM / 64; ++b) tma_load(sa + b * 8192, &map_a, t.m * kM + b * 64, kk, t.half, pa, &full[s]);
-            for (int b = 0; b < BN / 64; ++b) tma_load(sb + b * 8192, &map_b, t.n * BN + b * 64, kk, 0, pb, &full[s]);
-          } else if (MODE == kDx) {
-            tma_load(sa, &map_a, kk, t.m * kM, kh, pa, &full[s]);
-            for (int b = 0; b < BN / 64; ++b) tma_load(sb + b * 8192, &map_b, t.n * BN + b * 64, kk, kh, pb, &full[s]);
-          } else {
-            tma_load(sa, &map_a, kk, t.m * kM, 0, pa, &full[s]);
-            tma_load(sb, &map_b, kk, t.n * CN, 0, pb, &full[s]);
-            tma_load(sb + CN * 128, &map_b, kk, t.n * CN, 1, pb, &full[s]);
+        int k0, k1;
+        slice(t, &k0, &k1);
+        const int m0 = t.m * 2 * kM + (int)rank * kM, n0 = t.n * BN + (int)rank * (BN / 2);
+        for (int k = k0; k < k1 && ok; ++k) {
+          const int kh = k / p.khalf, kk = (k % p.khalf) * kK;
+          for (int part = 0; part < PARTS; ++part, ++it) {
+            const int s = it % ST;
+            ok = wait_phase(&empty[s], ((it / ST) & 1) ^ 1, &dead);
+            if (!ok) break;
+            if (rank == 0) expect_bytes(&full[s], 2 * BYTES);
+            const uint32_t bar = in_cluster(&full[s], 0);
+            uint8_t *sa = slot0 + s * BYTES, *sb = sa + ABYTES;
+            if (MODE == kDw) {
+              for (int b = 0; b < kM / 64; ++b) tma_load(sa + b * 8192, &map_a, m0 + b * 64, kk, t.half, part, bar);
+              for (int b = 0; b < BN / 128; ++b) tma_load(sb + b * 8192, &map_b, n0 + b * 64, kk, 0, part, bar);
+            } else if (MODE == kDx) {
+              tma_load(sa, &map_a, kk, m0, kh, part, bar);
+              for (int b = 0; b < BN / 128; ++b) tma_load(sb + b * 8192, &map_b, n0 + b * 64, kk, kh, part, bar);
+            } else {  // CTA 0 brings u's rows of W, CTA 1 g's
+              tma_load(sa, &map_a, kk, m0, 0, part, bar);
+              tma_load(sb, &map_b, kk, t.n * CN, (int)rank, part, bar);
+            }
           }
         }
       }
-      // After a wait that gave up: the copies on their way land before the CTA ends.
-      if (!ok)
+      // After a wait that gave up: the copies on their way land before the CTAs end (CTA 0 sees both CTAs').
+      if (!ok && rank == 0)
         for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) wait_some(&full[i % ST], (i / ST) & 1, nullptr);
     }
-  } else if (warp == 5) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16(kM, BN, A_MN, B_MN);
+  } else if (warp == kEpi + 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_bf16(2 * kM, BN, A_MN, B_MN);
       constexpr uint32_t a_step = (A_MN ? 2048 : 32), b_step = (B_MN ? 2048 : 32);  // 16 of the depth
-      uint32_t it = 0, acc = 0;
+      uint32_t it = 0, acc = 0, tiles = 0;
       bool ok = true;
-      for (int w = blockIdx.x; w < works && ok; w += gridDim.x, ++acc) {
-        const Tile t = tile_at(p, w);
-        const int k0 = (int)((int64_t)depth * t.split / p.splits), k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
-        const uint32_t b = acc & 1, d = tmem + b * BN;
-        ok = wait_phase(&acc_empty[b], ((acc >> 1) & 1) ^ 1, &dead);
-        if (!ok) break;
+      auto multiply = [&](uint32_t d, int sa, int sb, bool accumulate) {
+        const uint32_t a = semx::tc::smem_addr(slot0 + sa * BYTES), b = semx::tc::smem_addr(slot0 + sb * BYTES) + ABYTES;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          mma_pair(d, operand_desc<A_MN>(a + q * a_step), operand_desc<B_MN>(b + q * b_step), idesc, accumulate || q > 0);
+      };
+      auto ready = [&](uint32_t i) {
+        ok = ok && wait_phase(&full[i % ST], (i / ST) & 1, &dead);
         semx::tc::fence_after_sync();
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % ST;
-          ok = wait_phase(&full[s], (it / ST) & 1, &dead);
+        return ok;
+      };
+      for (int w = pair0; w < works && ok; w += pairs, ++tiles) {
+        const Tile t = tile_at(p, w);
+        int k0, k1;
+        slice(t, &k0, &k1);
+        const uint32_t small = tmem + 2 * BN + (tiles & 1) * BN;
+        if (PARTS > 1) {
+          ok = wait_phase(&small_empty[tiles & 1], ((tiles >> 1) & 1) ^ 1, &dead);
+          if (!ok) break;
+        }
+        const int drain = PARTS > 1 ? kDrain : k1 - k0;
+        for (int c0 = k0; c0 < k1 && ok; c0 += drain, ++acc) {
+          const uint32_t b = acc & 1, d = tmem + b * BN;
+          ok = wait_phase(&acc_empty[b], ((acc >> 1) & 1) ^ 1, &dead);
           if (!ok) break;
           semx::tc::fence_after_sync();
-          const uint32_t sa = semx::tc::smem_addr(stage0 + s * BYTES), sb = sa + ABYTES;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mma_bf16(d, operand_desc<A_MN>(sa + q * a_step), operand_desc<B_MN>(sb + q * b_step), idesc, k > k0 || q > 0);
-          semx::tc::mma_commit(&empty[s]);
+          const int c1 = min(k1, c0 + drain);
+          for (int k = c0; k < c1; ++k, it += PARTS) {
+            const int s0 = it % ST;
+            if (!ready(it)) break;
+            multiply(d, s0, s0, k > c0);
+            if (PARTS > 1) {
+              const int s1 = (it + 1) % ST, s2 = (it + 2) % ST;
+              if (!ready(it + 1)) break;
+              multiply(small, s0, s1, k > k0);
+              multiply(small, s1, s0, true);
+              multiply(small, s1, s1, true);
+              if (!ready(it + 2)) break;
+              multiply(small, s0, s2, true);
+              multiply(small, s2, s0, true);
+              commit_pair(&empty[s0]);
+              commit_pair(&empty[s1]);
+              commit_pair(&empty[s2]);
+            } else {
+              commit_pair(&empty[s0]);
+            }
+          }
+          if (ok) commit_pair(&acc_full[b]);
         }
-        if (ok) semx::tc::mma_commit(&acc_full[b]);
+        if (PARTS > 1 && ok) commit_pair(&small_full[tiles & 1]);
       }
       if (!ok) {  // products on their way end before tensor memory is given back
-        semx::tc::mma_commit(&drained);
+        commit_pair(&drained);
         wait_some(&drained, 0, nullptr);
       }
     }
   } else {
     float* buf = bufs + warp * 32 * kBufRow;
-    const uint32_t lanes = (uint32_t)warp << 21;  // this warp's 32 lanes of tensor memory
-    uint32_t acc = 0;
-    for (int w = blockIdx.x; w < works; w += gridDim.x, ++acc) {
-      const Tile t = tile_at(p, w);
-      const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
-      const bool ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      semx::tc::fence_after_sync();
-      const int64_t row0 = (int64_t)t.m * kM + warp * 32;
-      const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0));
-#pragma unroll 1
-      for (int c = 0; c < CN; c += 32) {
-        const int64_t col0 = (int64_t)t.n * CN + c;
-        const int cols = (int)max((int64_t)0, min((int64_t)32, p.N - col0));
-        float v[32];
-        semx::tc::tmem_ld32(d + c, v);
-        if (MODE == kFwd) {
-          float g[32];
-          semx::tc::tmem_ld32(d + CN + c, g);
-          if (c + 32 >= CN) {
-            semx::tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(&acc_empty[b]);
-          }
-          if (p.splits > 1) {
-            float* to = p.part + (int64_t)t.split * 2 * p.M * p.N;
-            write_block(buf, v, to, p.N, row0, col0, rows, cols, 0);
-            write_block(buf, g, to + p.M * p.N, p.N, row0, col0, rows, cols, 0);
-            continue;
-          }
-          if (p.bias != nullptr) {
+    const int quarter = warp % 4, side = warp / 4;  // rows; columns (the first or the second half of u's and g's, or of the tile)
+    const uint32_t lanes = (uint32_t)quarter << 21;
+    // Columns of the result that a warp has; of 32 the first four warps have all.
+    constexpr int WC = CN > 32 ? CN / 2 : CN;
+    const bool idle = CN <= 32 && side > 0;
+    constexpr int VALUES = MODE == kFwd ? 2 * WC : WC;  // of the accumulator
+    const uint32_t acc_e0 = in_cluster(&acc_empty[0], 0), acc_e1 = in_cluster(&acc_empty[1], 0);
+    const uint32_t small_e0 = in_cluster(&small_empty[0], 0), small_e1 = in_cluster(&small_empty[1], 0);
+    auto release = [&](uint32_t bar) {
+      semx::tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_in_cluster(bar);
+    };
+    // Column (of the accumulator) of value i of this warp.
+    auto column = [&](int i) { return MODE == kFwd ? (i / WC) * CN + side * WC + i % WC : side * WC + i; };
+    // What becomes of 32 columns from c of the result on: v (and g, kFwd).
+    auto write = [&](const Tile& t, int c, float (&v)[32], float (&g)[32]) {
+      const int64_t row0 = ((int64_t)t.m * 2 + rank) * kM + quarter * 32, col0 = (int64_t)t.n * CN + side * WC + c;
+      const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0)), cols = (int)max((int64_t)0, min((int64_t)32, p.N - col0));
+      if (rows == 0 || cols == 0) return;
+      if (MODE == kFwd) {
+        if (p.splits > 1) {
+          float* to = p.part + (int64_t)t.split * 2 * p.M * p.N;
+          write_block(buf, v, to, p.N, row0, col0, rows, cols, 0);
+          write_block(buf, g, to + p.M * p.N, p.N, row0, col0, rows, cols, 0);
+          return;
+        }
+        if (p.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < cols) {
-                v[i] += p.bias[col0 + i];
-                g[i] += p.bias[p.N + col0 + i];
-              }
-          }
-          if (p.u != nullptr) {
-            write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
-            write_block(buf, g, p.g, p.ldu, row0, col0, rows, cols, 0);
-          }
+          for (int i = 0; i < 32; ++i)
+            if (i < cols) {
+              v[i] += semx_scan::load(p.bias, col0 + i, p.bias_bf16);
+              g[i] += semx_scan::load(p.bias, p.N + col0 + i, p.bias_bf16);
+            }
+        }
+        if (p.u != nullptr) {
+          write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
+          write_block(buf, g, p.g, p.ldu, row0, col0, rows, cols, 0);
+        }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= act_of(g[i], p.gelu);
-          write_block(buf, v, p.out, p.ldo, row0, col0, rows, cols, p.out_bf16);
+        for (int i = 0; i < 32; ++i) v[i] *= act_of(g[i], p.gelu);
+        write_block(buf, v, p.out, p.ldo, row0, col0, rows, cols, p.out_bf16);
+      } else {
+        const int64_t half0 = (int64_t)t.half * p.M;
+        if (p.splits > 1) {
+          const int64_t all = (MODE == kDw ? 2 : 1) * p.M * p.N;
+          write_block(buf, v, p.part + t.split * all + half0 * p.N, p.N, row0, col0, rows, cols, 0);
         } else {
-          if (c + 32 >= CN) {
-            semx::tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(&acc_empty[b]);
+          write_block(buf, v, p.out, p.ldo, half0 + row0, col0, rows, cols, p.out_bf16);
+        }
+      }
+    };
+    uint32_t acc = 0, tiles = 0;
+    for (int w = pair0; w < works; w += pairs, ++tiles) {
+      const Tile t = tile_at(p, w);
+      if constexpr (PARTS == 1) {
+        const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
+        const bool ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        semx::tc::fence_after_sync();
+        if (idle) release(b ? acc_e1 : acc_e0);
+#pragma unroll 1
+        for (int c = 0; c < WC && !idle; c += 32) {
+          float v[32], g[32];
+          semx::tc::tmem_ld32(d + column(c), v);
+          if (MODE == kFwd) semx::tc::tmem_ld32(d + column(WC + c), g);
+          if (c + 32 >= WC) release(b ? acc_e1 : acc_e0);
+          write(t, c, v, g);
+        }
+        ++acc;
+      } else {
+        int k0, k1;
+        slice(t, &k0, &k1);
+        float sum[VALUES];
+        bool ok = true;
+        for (int c0 = k0; c0 < k1; c0 += kDrain, ++acc) {
+          const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
+          ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          semx::tc::fence_after_sync();
+#pragma unroll
+          for (int i = 0; i < VALUES; i += 32) {
+            float v[32];
+            semx::tc::tmem_ld32(d + column(i), v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[i + j] = c0 == k0 ? v[j] : sum[i + j] + v[j];
           }
-          const int64_t half0 = (int64_t)t.half * p.M;
-          if (p.splits > 1) {
-            const int64_t all = (MODE == kDw ? 2 : 1) * p.M * p.N;
-            write_block(buf, v, p.part + t.split * all + half0 * p.N, p.N, row0, col0, rows, cols, 0);
-          } else {
-            write_block(buf, v, p.out, p.ldo, half0 + row0, col0, rows, cols, p.out_bf16);
+          release(b ? acc_e1 : acc_e0);
+        }
+        if (!ok) break;
+        ok = wait_phase(&small_full[tiles & 1], (tiles >> 1) & 1, &dead);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        semx::tc::fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < VALUES; i += 32) {
+          float v[32];
+          semx::tc::tmem_ld32(tmem + 2 * BN + (tiles & 1) * BN + lanes + column(i), v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[i + j] += v[j];
+        }
+        release((tiles & 1) ? small_e1 : small_e0);
+#pragma unroll
+        for (int c = 0; c < WC; c += 32) {
+          float v[32], g[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[j] = sum[c + j];
+            if (MODE == kFwd) g[j] = sum[WC + c + j];
           }
+          write(t, c, v, g);
         }
       }
     }
   }
   semx::tc::fence_before_sync();
   __syncthreads();
+  cluster_sync();  // neither CTA's barriers and shared memory end before the other is done with them
   semx::tc::fence_after_sync();
-  if (warp == 0) semx::tc::tmem_dealloc(tmem, 2 * BN);
+  if (warp == 0) tmem_dealloc_pair(tmem, COLS);
 }
 
 // Sums of the slices of the depth, in their order, and what the epilogue does with them.
@@ -388,8 +522,8 @@ __global__ void __launch_bounds__(256) join_gated_kernel(const GemmParams p) {
     g += p.part[(2 * k + 1) * n + i];
   }
   if (p.bias != nullptr) {
-    u += p.bias[col];
-    g += p.bias[p.N + col];
+    u += semx_scan::load(p.bias, col, p.bias_bf16);
+    g += semx_scan::load(p.bias, p.N + col, p.bias_bf16);
   }
   if (p.u != nullptr) {
     p.u[row * p.ldu + col] = u;
@@ -597,8 +731,8 @@ __global__ void __launch_bounds__(kFewT) few_rows_kernel(const void* x, int64_t 
       const int64_t h = h0 + lane;
       float u = lane ? v[1] : v[0], g = lane ? v[3] : v[2];
       if (p.bias != nullptr) {
-        u += p.bias[h];
-        g += p.bias[H + h];
+        u += semx_scan::load(p.bias, h, p.bias_bf16);
+        g += semx_scan::load(p.bias, H + h, p.bias_bf16);
       }
       if (p.u != nullptr) {
         p.u[r * p.ldu + h] = u;
@@ -663,7 +797,7 @@ struct Plan {
   size_t part_bytes;
 };
 
-// M, N: the result; K: the depth of one pair of parts and half.
+// M, N: the result; K: the depth of one half.
 Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   Plan q = {};
   q.mode = mode;
@@ -671,32 +805,36 @@ Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   p.M = M;
   p.N = N;
   p.khalf = (int)cdiv(K, (int64_t)kK);
-  p.kper = p.khalf * (mode == kDx ? 2 : 1);
-  p.pairs = parts > 1 ? 6 : 1;
+  p.depth = p.khalf * (mode == kDx ? 2 : 1);
   const int64_t wide = mode == kFwd ? 2 * N : N;
-  const int64_t down = cdiv(M, (int64_t)kM) * (mode == kDw ? 2 : 1);
-  q.bn = wide > 128 ? 256 : wide > 64 ? 128 : 64;
-  // Narrower tiles where wide ones leave SMs idle.
-  while (q.bn > 64 && down * cdiv(wide, (int64_t)q.bn) < kSms && cdiv(wide, (int64_t)q.bn / 2) > cdiv(wide, (int64_t)q.bn)) q.bn /= 2;
-  p.tiles_m = (int)cdiv(M, (int64_t)kM);
+  const int64_t down = cdiv(M, (int64_t)2 * kM) * (mode == kDw ? 2 : 1);
+  // The tile width that takes the least time in rounds of all pairs of SMs: a round costs its products
+  // and, in columns, about 32 of its own. (The operands read along the result need 128.)
+  int64_t least = 0;
+  for (int bn = 256; bn >= (mode == kFwd ? 64 : 128); bn /= 2) {
+    if (parts > 1 && bn != 128) continue;
+    const int64_t cost = cdiv(down * cdiv(wide, (int64_t)bn), (int64_t)kPairs) * (bn + 32);
+    if (q.bn == 0 || cost < least) q.bn = bn, least = cost;
+  }
+  p.tiles_m = (int)cdiv(M, (int64_t)2 * kM);
   p.tiles_n = (int)cdiv(wide, (int64_t)q.bn);
   p.tiles = p.tiles_m * p.tiles_n * (mode == kDw ? 2 : 1);
-  // Slices of the depth where tiles alone leave half of the SMs idle, of 8 stages at least.
-  const int64_t depth = (int64_t)p.kper * p.pairs;
-  int64_t s = kSms / p.tiles;
-  if (s > depth / 8) s = depth / 8;
-  if (s > 64) s = 64;
+  // Slices of the depth where tiles alone leave half of the SMs idle, of 8 stages (fp32: 4, each of them
+  // six products) at least.
+  int64_t s = kPairs / p.tiles;
+  const int64_t most = p.depth / (parts > 1 ? 4 : 8);
+  if (s > most) s = most;
   p.splits = q.splits = s < 2 ? 1 : (int)s;
   const int64_t result = M * N * (mode == kDx ? 1 : 2);
   q.part_bytes = p.splits > 1 ? up256((size_t)p.splits * result * sizeof(float)) : 0;
   return q;
 }
 
-template <int MODE, int BN>
+template <int MODE, int BN, int PARTS>
 int launch_tiles(const Plan& q, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t st) {
-  if (!semx::allow_smem(gemm_kernel<MODE, BN>, gemm_smem(BN))) return SEMX_ERR_LAUNCH;
+  if (!semx::allow_smem(gemm_kernel<MODE, BN, PARTS>, gemm_smem(BN))) return SEMX_ERR_LAUNCH;
   const int works = q.p.tiles * q.p.splits;
-  gemm_kernel<MODE, BN><<<works < kSms ? works : kSms, kGemmT, gemm_smem(BN), st>>>(a, b, q.p);
+  gemm_kernel<MODE, BN, PARTS><<<2 * (works < kPairs ? works : kPairs), kGemmT, gemm_smem(BN), st>>>(a, b, q.p);
   return semx::check_launch("gated_linear gemm_kernel");
 }
 
@@ -707,8 +845,16 @@ int launch_gemm(const Plan& q, const Operand& A, const Operand& B, cudaStream_t 
   if (rc != SEMX_OK) return rc;
   rc = make_map(&b, B, MODE == kFwd ? q.bn / 2 : 64);
   if (rc != SEMX_OK) return rc;
-  rc = q.bn == 256 ? launch_tiles<MODE, 256>(q, a, b, st)
-       : q.bn == 128 ? launch_tiles<MODE, 128>(q, a, b, st) : launch_tiles<MODE, 64>(q, a, b, st);
+  if (A.parts > 1) {
+    rc = launch_tiles<MODE, 128, kParts>(q, a, b, st);
+  } else if (q.bn == 256) {
+    rc = launch_tiles<MODE, 256, 1>(q, a, b, st);
+  } else if (q.bn == 128) {
+    rc = launch_tiles<MODE, 128, 1>(q, a, b, st);
+  } else {
+    if constexpr (MODE == kFwd) rc = launch_tiles<MODE, 64, 1>(q, a, b, st);
+    else rc = semx::fail(SEMX_ERR_UNSUPPORTED, "gated_linear: tile of %d", q.bn);
+  }
   if (rc != SEMX_OK || q.splits == 1) return rc;
   const int64_t n = q.p.M * q.p.N * (MODE == kDw ? 2 : 1);
   const unsigned grid = (unsigned)cdiv(n, (int64_t)256);
@@ -741,7 +887,8 @@ int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
   if (!bwd) SEMX_REQUIRE(a->h, SEMX_ERR_NULL, "gated_linear: h is NULL");
   else SEMX_REQUIRE(a->rows == 0 || (a->dh && a->saved), SEMX_ERR_NULL, "gated_linear bwd: dh / saved is NULL");
   SEMX_REQUIRE(semx::all_aligned({a->x, a->w, a->h, a->dh, a->dx, a->dw}, a->bf16 ? 2 : 4) &&
-                   semx::all_aligned({a->bias, a->db}, 4) && semx::all_aligned({a->saved, a->workspace}, 16),
+                   semx::aligned(a->bias, a->bias_bf16 ? 2 : 4) && semx::aligned(a->db, 4) &&
+                   semx::all_aligned({a->saved, a->workspace}, 16),
                SEMX_ERR_ALIGN, "gated_linear: a pointer is not on an element");
   return SEMX_OK;
 }
@@ -873,6 +1020,7 @@ int semx_gated_linear_fwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   q.p.u = a->saved;
   q.p.g = a->saved == nullptr ? nullptr : a->saved + a->rows * q.p.ldu;
   q.p.bias = a->bias;
+  q.p.bias_bf16 = a->bias_bf16;
   q.p.gelu = a->act;
   if (l.few) {
     if (a->rows == 1) return launch_few<1>(a, q.p, st);

@@ -26,7 +26,9 @@ def _args(x, weight, bias, act):
     a.bf16, a.act = x.dtype == torch.bfloat16, act
     a.rows, a.D, a.H = x.shape[0], x.shape[1], weight.shape[0] // 2
     a.ldx = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    a.x, a.w, a.bias = x.data_ptr(), weight.data_ptr(), _lib.ptr(bias)
+    a.x, a.w = x.data_ptr(), weight.data_ptr()
+    if bias is not None:
+        a.bias, a.bias_bf16 = bias.data_ptr(), bias.dtype == torch.bfloat16
     return a
 
 
@@ -51,9 +53,8 @@ def _forward(x, weight, bias, act, keep):
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act):
-        b = _lib.param32(bias)
         w = weight.contiguous()
-        h, saved = _forward(x, w, b, act, True)
+        h, saved = _forward(x, w, None if bias is None else bias.contiguous(), act, True)
         ctx.save_for_backward(x, w, saved)
         ctx.cfg = (act, None if bias is None else bias.dtype)
         return h
@@ -113,7 +114,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         rows = rows if rows_of(rows, D)[0] is rows else rows.contiguous()
         h = _GatedLinear.apply(rows, weight, bias, act)
     else:
-        h, _ = _forward(rows_of(rows, D)[0], weight.contiguous(), _lib.param32(bias), act, False)
+        h, _ = _forward(rows_of(rows, D)[0], weight.contiguous(), None if bias is None else bias.contiguous(), act, False)
     return h if x.dim() == 2 else h.view(lead + (h.shape[-1],))
 
 
