@@ -39,6 +39,7 @@ constexpr int kGemmT = (kEpi + 2) * 32;  // then one that loads and one that iss
 constexpr int kSms = 148, kPairs = kSms / 2;
 constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
 constexpr int kBufRow = 36;         // floats of a row of a warp's 32 x 32 exchange buffer
+constexpr int kBuf = 32 * kBufRow + 64;  // floats of the buffer, and of u's and g's biases behind it
 constexpr int kParts = 3;           // bf16 parts of an fp32 value
 constexpr int kDrain = 2;           // stages whose large products one accumulator takes (fp32)
 
@@ -64,16 +65,40 @@ struct GemmParams {
   float* part;            // with splits: (splits, result) sums, kFwd: (splits, 2, M, N)
 };
 
-__device__ __forceinline__ float act_of(float g, int gelu) {
-  return gelu ? g * (0.5f * erfcf(g * -0.70710678118654752f)) : g * sigmoid(g);
+// Half of erfc(|g| / sqrt(2)) and e = exp(-g^2 / 2): erfc(z) = t q(t) exp(-z^2) with t = 1 / (1 + z / 2); q is a
+// polynomial of degree 8, fitted to the least largest relative error for z up to 9.5 (4e-8, 2.6e-7 with its
+// roundings; further out the exponential is 0).
+__device__ __forceinline__ float normal_tail(float g, float* e) {
+  const float t = semx::rcp_approx(fmaf(fabsf(g), 0.35355339059327379f, 1.f));
+  *e = semx::ex2_approx(-0.72134752044448170f * g * g);
+  float q = fmaf(-0.029445456340909004f, t, 0.1418512910604477f);
+  q = fmaf(q, t, -0.24269245564937592f);
+  q = fmaf(q, t, 0.13798969984054565f);
+  q = fmaf(q, t, -0.012589219957590103f);
+  q = fmaf(q, t, 0.10103505849838257f);
+  q = fmaf(q, t, 0.1216304749250412f);
+  q = fmaf(q, t, 0.1411767452955246f);
+  q = fmaf(q, t, 0.14104384183883667f);
+  return t * q * *e;
 }
-__device__ __forceinline__ float act_slope(float g, int gelu) {
+__device__ __forceinline__ float act_of(float g, int gelu) {
+  if (!gelu) return g * sigmoid(g);
+  float e;
+  const float tail = normal_tail(g, &e);
+  return g * (g < 0.f ? tail : 1.f - tail);
+}
+// act(g) and act'(g).
+__device__ __forceinline__ void act_and_slope(float g, int gelu, float* act, float* slope) {
   if (gelu) {
-    const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
-    return fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), cdf);
+    float e;
+    const float tail = normal_tail(g, &e), cdf = g < 0.f ? tail : 1.f - tail;
+    *act = g * cdf;
+    *slope = fmaf(g * 0.3989422804014327f, e, cdf);
+  } else {
+    const float s = sigmoid(g);
+    *act = g * s;
+    *slope = s * fmaf(g, 1.f - s, 1.f);
   }
-  const float s = sigmoid(g);
-  return s * fmaf(g, 1.f - s, 1.f);
 }
 
 // -- tensor core plumbing -----------------------------------------------------------------------
@@ -104,8 +129,10 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(semx::tc::smem_addr(bar)), "r"(bytes) : "memory");
 }
+// (Relaxed: it says that tensor memory has been read, which has ended by then, and hands on nothing in
+// memory. A release waits for the tile's stores: 4 of 19 cycles between two instructions.)
 __device__ __forceinline__ void arrive_in_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
@@ -167,7 +194,7 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
 constexpr int slot_bytes(int bn) { return (kM + bn / 2) * kK * 2; }
 constexpr int slots_of(int bn) { return bn == 256 ? 5 : bn == 128 ? 7 : 8; }
 constexpr size_t gemm_smem(int bn) {
-  return 1024 + (size_t)slots_of(bn) * slot_bytes(bn) + kEpi * 32 * kBufRow * sizeof(float);
+  return 1024 + (size_t)slots_of(bn) * slot_bytes(bn) + kEpi * kBuf * sizeof(float);
 }
 
 struct Tile {
@@ -381,7 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
       }
     }
   } else {
-    float* buf = bufs + warp * 32 * kBufRow;
+    float* buf = bufs + warp * kBuf;
     const int quarter = warp % 4, side = warp / 4;  // rows; columns (the first or the second half of u's and g's, or of the tile)
     const uint32_t lanes = (uint32_t)quarter << 21;
     // Columns of the result that a warp has; of 32 the first four warps have all.
@@ -410,12 +437,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           return;
         }
         if (p.bias != nullptr) {
+          float* at = buf + 32 * kBufRow;
+          at[lane] = lane < cols ? semx_scan::load(p.bias, col0 + lane, p.bias_bf16) : 0.f;
+          at[32 + lane] = lane < cols ? semx_scan::load(p.bias, p.N + col0 + lane, p.bias_bf16) : 0.f;
+          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < cols) {
-              v[i] += semx_scan::load(p.bias, col0 + i, p.bias_bf16);
-              g[i] += semx_scan::load(p.bias, p.N + col0 + i, p.bias_bf16);
-            }
+          for (int i = 0; i < 32; i += 4) {
+            const float4 bu = *reinterpret_cast<const float4*>(at + i), bg = *reinterpret_cast<const float4*>(at + 32 + i);
+            v[i] += bu.x; v[i + 1] += bu.y; v[i + 2] += bu.z; v[i + 3] += bu.w;
+            g[i] += bg.x; g[i + 1] += bg.y; g[i + 2] += bg.z; g[i + 3] += bg.w;
+          }
+          __syncwarp();
         }
         if (p.u != nullptr) {
           write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
@@ -583,51 +615,76 @@ __global__ void __launch_bounds__(256) lay_kernel(const void* src, int64_t ld, i
   }
 }
 
-// du and dg from u, g (fp32, rows of ldu) and dh, as parts (parts, 2, rows, ldp); column sums of 64
-// rows each into sums (row blocks, 2 H) where wanted. A thread has 4 columns of every 4th row.
+// du and dg from u, g (fp32, rows of ldu) and dh, as parts (PARTS, 2, rows, ldp); column sums of 64
+// rows each into sums (row blocks, 2 H) where wanted. A thread has 4 columns of every 4th row, four rows
+// on their way at a time.
 constexpr int kDzRows = 64;
-__global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const float* g, int64_t ldu, const void* dh, int bf16,
+template <int PARTS>
+__global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const float* g, int64_t ldu, const void* dh,
                                                         int64_t rows, int64_t H, int gelu, __nv_bfloat16* dz, int64_t ldp,
-                                                        int parts, float* sums) {
+                                                        float* sums) {
+  constexpr bool BF16 = PARTS == 1;
+  constexpr int ACC = BF16 ? semx_scan::kBf16 : semx_scan::kFp32, AHEAD = 4;
   __shared__ float red[2][4][256];
   const int lane = threadIdx.x % 64, down = threadIdx.x / 64;
   const int64_t c = (int64_t)blockIdx.y * 256 + lane * 4, r0 = (int64_t)blockIdx.x * kDzRows;
-  const int nn = (int)min((int64_t)4, H - c);
-  const bool wide = H % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (bf16 ? 7 : 15)) == 0;
+  const int nn = (int)max((int64_t)0, min((int64_t)4, H - c)), most = (int)min((int64_t)kDzRows, rows - r0);
+  const bool wide = H % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (BF16 ? 7 : 15)) == 0;
   float su[4] = {}, sg[4] = {};
   if (nn > 0)
-    for (int64_t r = r0 + down; r < min(r0 + kDzRows, rows); r += 4) {
-      const float4 u4 = *reinterpret_cast<const float4*>(u + r * ldu + c), g4 = *reinterpret_cast<const float4*>(g + r * ldu + c);
-      const float uu[4] = {u4.x, u4.y, u4.z, u4.w}, gg[4] = {g4.x, g4.y, g4.z, g4.w};
-      float d[4] = {};
-      if (wide) {
-        const float4 q = bf16 ? semx_scan::quad_floats<semx_scan::kBf16>(semx_scan::load_quad<semx_scan::kBf16>(dh, r * H + c, 1, 4), 1)
-                              : semx_scan::quad_floats<semx_scan::kFp32>(semx_scan::load_quad<semx_scan::kFp32>(dh, r * H + c, 0, 4), 0);
-        d[0] = q.x; d[1] = q.y; d[2] = q.z; d[3] = q.w;
-      } else {
+    for (int i0 = down; i0 < most; i0 += 4 * AHEAD) {
+      float4 u4[AHEAD], g4[AHEAD];
+      float d4[AHEAD][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k < nn) d[k] = semx_scan::load(dh, r * H + c + k, bf16);
-      }
-      __align__(8) __nv_bfloat16 pu[kParts][4], pg[kParts][4];
+      for (int a = 0; a < AHEAD; ++a) {
+        const int i = i0 + 4 * a;
+        u4[a] = g4[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+        d4[a][0] = d4[a][1] = d4[a][2] = d4[a][3] = 0.f;
+        if (i >= most) continue;
+        const int64_t r = r0 + i;
+        u4[a] = __ldcs(reinterpret_cast<const float4*>(u + r * ldu + c));
+        g4[a] = __ldcs(reinterpret_cast<const float4*>(g + r * ldu + c));
+        if (wide) {
+          const float4 q = semx_scan::quad_floats<ACC>(semx_scan::load_quad<ACC>(dh, r * H + c, BF16, 4), BF16);
+          d4[a][0] = q.x; d4[a][1] = q.y; d4[a][2] = q.z; d4[a][3] = q.w;
+        } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool in = k < nn;
-        const float du = in ? d[k] * act_of(gg[k], gelu) : 0.f, dg = in ? d[k] * uu[k] * act_slope(gg[k], gelu) : 0.f;
-        su[k] += du;
-        sg[k] += dg;
-        __nv_bfloat16 q[kParts];
-        parts_of(du, q);
-        for (int n = 0; n < kParts; ++n) pu[n][k] = q[n];
-        parts_of(dg, q);
-        for (int n = 0; n < kParts; ++n) pg[n][k] = q[n];
+          for (int k = 0; k < 4; ++k)
+            if (k < nn) d4[a][k] = semx_scan::load(dh, r * H + c + k, BF16);
+        }
       }
 #pragma unroll
-      for (int n = 0; n < kParts; ++n)
-        if (n < parts) {
+      for (int a = 0; a < AHEAD; ++a) {
+        const int i = i0 + 4 * a;
+        if (i >= most) continue;
+        const int64_t r = r0 + i;
+        const float uu[4] = {u4[a].x, u4[a].y, u4[a].z, u4[a].w}, gg[4] = {g4[a].x, g4[a].y, g4[a].z, g4[a].w};
+        __align__(8) __nv_bfloat16 pu[PARTS][4], pg[PARTS][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float act, slope;
+          act_and_slope(gg[k], gelu, &act, &slope);
+          const bool in = k < nn;
+          const float du = in ? d4[a][k] * act : 0.f, dg = in ? d4[a][k] * uu[k] * slope : 0.f;
+          su[k] += du;
+          sg[k] += dg;
+          if constexpr (BF16) {
+            pu[0][k] = __float2bfloat16(du);
+            pg[0][k] = __float2bfloat16(dg);
+          } else {
+            __nv_bfloat16 q[kParts];
+            parts_of(du, q);
+            for (int n = 0; n < kParts; ++n) pu[n][k] = q[n];
+            parts_of(dg, q);
+            for (int n = 0; n < kParts; ++n) pg[n][k] = q[n];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) {
           *reinterpret_cast<uint2*>(dz + ((2 * n) * rows + r) * ldp + c) = *reinterpret_cast<const uint2*>(pu[n]);
           *reinterpret_cast<uint2*>(dz + ((2 * n + 1) * rows + r) * ldp + c) = *reinterpret_cast<const uint2*>(pg[n]);
         }
+      }
     }
   if (sums == nullptr) return;
 #pragma unroll
@@ -797,6 +854,10 @@ struct Plan {
   size_t part_bytes;
 };
 
+// Of a tile, in columns: what it costs beside them. Narrow tiles bring more of A per product (8192 x 5504 x
+// 2048, 4 rounds of 256 columns or 7 of 128: 358 and 422 us).
+constexpr int kTileCost = 96;
+
 // M, N: the result; K: the depth of one half.
 Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   Plan q = {};
@@ -808,12 +869,11 @@ Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   p.depth = p.khalf * (mode == kDx ? 2 : 1);
   const int64_t wide = mode == kFwd ? 2 * N : N;
   const int64_t down = cdiv(M, (int64_t)2 * kM) * (mode == kDw ? 2 : 1);
-  // The tile width that takes the least time in rounds of all pairs of SMs: a round costs its products
-  // and, in columns, about 32 of its own. (The operands read along the result need 128.)
+  // The tile width that takes the least time in rounds of all pairs of SMs. (The operands read along the result need 128.)
   int64_t least = 0;
   for (int bn = 256; bn >= (mode == kFwd ? 64 : 128); bn /= 2) {
     if (parts > 1 && bn != 128) continue;
-    const int64_t cost = cdiv(down * cdiv(wide, (int64_t)bn), (int64_t)kPairs) * (bn + 32);
+    const int64_t cost = cdiv(down * cdiv(wide, (int64_t)bn), (int64_t)kPairs) * (bn + kTileCost);
     if (q.bn == 0 || cost < least) q.bn = bn, least = cost;
   }
   p.tiles_m = (int)cdiv(M, (int64_t)2 * kM);
@@ -1061,8 +1121,9 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   float* sums = a->db != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
   __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + l.dz);
   const float *u = a->saved, *g = a->saved + a->rows * Hp;
-  gate_grad_kernel<<<dim3((unsigned)blocks, (unsigned)cdiv(a->H, (int64_t)256)), 256, 0, st>>>(
-      u, g, Hp, a->dh, a->bf16, a->rows, a->H, a->act, dz, Hp, l.parts, sums);
+  const dim3 grid((unsigned)blocks, (unsigned)cdiv(a->H, (int64_t)256));
+  if (a->bf16) gate_grad_kernel<1><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
+  else gate_grad_kernel<kParts><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
   rc = semx::check_launch("gated_linear gate_grad_kernel");
   if (rc != SEMX_OK) return rc;
   Operand x, w;
