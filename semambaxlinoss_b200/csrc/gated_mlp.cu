@@ -39,7 +39,7 @@ constexpr int kGemmT = (kEpi + 2) * 32;  // then one that loads and one that iss
 constexpr int kSms = 148, kPairs = kSms / 2;
 constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
 constexpr int kBufRow = 36;         // floats of a row of a warp's 32 x 32 exchange buffer
-constexpr int kBuf = 32 * kBufRow + 64;  // floats of the buffer, and of u's and g's biases behind it
+constexpr int kBuf = 32 * kBufRow + 128;  // floats of the buffer, and of u's and g's biases (64 columns) behind it
 constexpr int kParts = 3;           // bf16 parts of an fp32 value
 constexpr int kDrain = 2;           // stages whose large products one accumulator takes (fp32)
 
@@ -156,6 +156,28 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) 
 }
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Two runs of 32 columns of this thread's lane of tensor memory, one wait for both.
+__device__ __forceinline__ void tmem_ld32_twice(uint32_t t0, uint32_t t1, float (&v)[32], float (&w)[32]) {
+  uint32_t r[64];
+#define SEMX_R8(o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : SEMX_R8(0), SEMX_R8(8), SEMX_R8(16), SEMX_R8(24), SEMX_R8(32), SEMX_R8(40), SEMX_R8(48), SEMX_R8(56)
+      : "r"(t0), "r"(t1)
+      : "memory");
+#undef SEMX_R8
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    v[i] = __uint_as_float(r[i]);
+    w[i] = __uint_as_float(r[32 + i]);
+  }
 }
 // Descriptor of an operand in 128-byte rows with the 128-byte swizzle. K-major: a row is 64 values of
 // the depth, 8-row groups 1024 bytes apart. MN-major: a row is 64 neighbouring M or N values at one
@@ -437,17 +459,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           return;
         }
         if (p.bias != nullptr) {
-          float* at = buf + 32 * kBufRow;
-          at[lane] = lane < cols ? semx_scan::load(p.bias, col0 + lane, p.bias_bf16) : 0.f;
-          at[32 + lane] = lane < cols ? semx_scan::load(p.bias, p.N + col0 + lane, p.bias_bf16) : 0.f;
-          __syncwarp();
+          const float* at = buf + 32 * kBufRow + c;
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 bu = *reinterpret_cast<const float4*>(at + i), bg = *reinterpret_cast<const float4*>(at + 32 + i);
+            const float4 bu = *reinterpret_cast<const float4*>(at + i), bg = *reinterpret_cast<const float4*>(at + 64 + i);
             v[i] += bu.x; v[i + 1] += bu.y; v[i + 2] += bu.z; v[i + 3] += bu.w;
             g[i] += bg.x; g[i + 1] += bg.y; g[i + 2] += bg.z; g[i + 3] += bg.w;
           }
-          __syncwarp();
         }
         if (p.u != nullptr) {
           write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
@@ -469,6 +487,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
     uint32_t acc = 0, tiles = 0;
     for (int w = pair0; w < works; w += pairs, ++tiles) {
       const Tile t = tile_at(p, w);
+      if (MODE == kFwd && p.bias != nullptr) {  // the tile's biases, while its products run
+        static_assert(MODE != kFwd || WC <= 64, "biases");
+        __syncwarp();
+        for (int c = lane; c < WC; c += 32) {
+          const int64_t col = (int64_t)t.n * CN + side * WC + c;
+          float* at = buf + 32 * kBufRow + c;
+          at[0] = col < p.N ? semx_scan::load(p.bias, col, p.bias_bf16) : 0.f;
+          at[64] = col < p.N ? semx_scan::load(p.bias, p.N + col, p.bias_bf16) : 0.f;
+        }
+        __syncwarp();
+      }
       if constexpr (PARTS == 1) {
         const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
         const bool ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
@@ -478,8 +507,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
 #pragma unroll 1
         for (int c = 0; c < WC && !idle; c += 32) {
           float v[32], g[32];
-          semx::tc::tmem_ld32(d + column(c), v);
-          if (MODE == kFwd) semx::tc::tmem_ld32(d + column(WC + c), g);
+          if (MODE == kFwd) tmem_ld32_twice(d + column(c), d + column(WC + c), v, g);
+          else semx::tc::tmem_ld32(d + column(c), v);
           if (c + 32 >= WC) release(b ? acc_e1 : acc_e0);
           write(t, c, v, g);
         }
@@ -496,11 +525,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           if (!ok) break;
           semx::tc::fence_after_sync();
 #pragma unroll
-          for (int i = 0; i < VALUES; i += 32) {
-            float v[32];
-            semx::tc::tmem_ld32(d + column(i), v);
+          for (int i = 0; i < VALUES; i += 64) {
+            float v[32], y[32];
+            tmem_ld32_twice(d + column(i), d + column(i + 32), v, y);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[i + j] = c0 == k0 ? v[j] : sum[i + j] + v[j];
+            for (int j = 0; j < 32; ++j) {
+              sum[i + j] = c0 == k0 ? v[j] : sum[i + j] + v[j];
+              sum[i + 32 + j] = c0 == k0 ? y[j] : sum[i + 32 + j] + y[j];
+            }
           }
           release(b ? acc_e1 : acc_e0);
         }
@@ -616,18 +648,20 @@ __global__ void __launch_bounds__(256) lay_kernel(const void* src, int64_t ld, i
 }
 
 // du and dg from u, g (fp32, rows of ldu) and dh, as parts (PARTS, 2, rows, ldp); column sums of 64
-// rows each into sums (row blocks, 2 H) where wanted. A thread has 4 columns of every 4th row, four rows
-// on their way at a time.
+// rows each into sums (row blocks, 2 H) where wanted. A thread has 4 columns of every 4th row, two rows
+// on their way at a time; CTAs side by side have columns side by side.
 constexpr int kDzRows = 64;
 template <int PARTS>
-__global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const float* g, int64_t ldu, const void* dh,
+__global__ void __launch_bounds__(256, PARTS == 1 ? 4 : 3) gate_grad_kernel(const float* u, const float* g, int64_t ldu, const void* dh,
                                                         int64_t rows, int64_t H, int gelu, __nv_bfloat16* dz, int64_t ldp,
                                                         float* sums) {
   constexpr bool BF16 = PARTS == 1;
-  constexpr int ACC = BF16 ? semx_scan::kBf16 : semx_scan::kFp32, AHEAD = 4;
+  constexpr int ACC = BF16 ? semx_scan::kBf16 : semx_scan::kFp32, AHEAD = 2;
   __shared__ float red[2][4][256];
   const int lane = threadIdx.x % 64, down = threadIdx.x / 64;
-  const int64_t c = (int64_t)blockIdx.y * 256 + lane * 4, r0 = (int64_t)blockIdx.x * kDzRows;
+  const unsigned across = (unsigned)((H + 255) / 256);
+  const int64_t c0 = (int64_t)(blockIdx.x % across) * 256, block = blockIdx.x / across;
+  const int64_t c = c0 + lane * 4, r0 = block * kDzRows;
   const int nn = (int)max((int64_t)0, min((int64_t)4, H - c)), most = (int)min((int64_t)kDzRows, rows - r0);
   const bool wide = H % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & (BF16 ? 7 : 15)) == 0;
   float su[4] = {}, sg[4] = {};
@@ -693,11 +727,11 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const fl
     red[1][down][lane * 4 + k] = sg[k];
   }
   __syncthreads();
-  const int64_t cc = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  const int64_t cc = c0 + threadIdx.x;
   if (cc < H) {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
-      sums[(int64_t)blockIdx.x * 2 * H + n * H + cc] =
+      sums[block * 2 * H + n * H + cc] =
           red[n][0][threadIdx.x] + red[n][1][threadIdx.x] + red[n][2][threadIdx.x] + red[n][3][threadIdx.x];
   }
 }
@@ -1121,7 +1155,7 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   float* sums = a->db != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
   __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + l.dz);
   const float *u = a->saved, *g = a->saved + a->rows * Hp;
-  const dim3 grid((unsigned)blocks, (unsigned)cdiv(a->H, (int64_t)256));
+  const unsigned grid = (unsigned)(blocks * cdiv(a->H, (int64_t)256));
   if (a->bf16) gate_grad_kernel<1><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
   else gate_grad_kernel<kParts><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
   rc = semx::check_launch("gated_linear gate_grad_kernel");
