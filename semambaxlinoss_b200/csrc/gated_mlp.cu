@@ -11,7 +11,7 @@
 //
 // Products: tcgen05 on pairs of SMs (a cluster of two CTAs has 256 rows of the result, each CTA's tensor
 // memory its 128; each brings its rows of A and half of B's by TMA, and one thread of the pair issues the
-// products for both). Persistent: in each CTA one warp loads and eight write the accumulators out; two
+// products for both). Persistent: in each CTA one warp loads and sixteen write the accumulators out; two
 // accumulators, so that writing a tile overlaps the next one's products.
 // fp32 operands are split into three bf16 parts whose sum is the value up to its last bit; six of the nine
 // products of parts are taken (the others are below 2^-24 of the result). The tensor cores cut where
@@ -34,12 +34,13 @@ using semx::cdiv;
 using semx_scan::sigmoid;
 
 constexpr int kM = 128, kK = 64;    // rows of a CTA's tile, depth of a stage (128 bytes of bf16)
-constexpr int kEpi = 8;             // warps that write out: two for each quarter of the rows
+constexpr int kEpi = 16;            // warps that write out: four for each quarter of the rows
 constexpr int kGemmT = (kEpi + 2) * 32;  // then one that loads and one that issues products
 constexpr int kSms = 148, kPairs = kSms / 2;
 constexpr long long kPatience = 4000000000ll;  // cycles that a wait takes at most
-constexpr int kBufRow = 36;         // floats of a row of a warp's 32 x 32 exchange buffer
-constexpr int kBuf = 32 * kBufRow + 128;  // floats of the buffer, and of u's and g's biases (64 columns) behind it
+constexpr int kCols = 16;           // columns that a warp writes at a time
+constexpr int kBufRow = kCols + 4;  // floats of a row of its exchange buffer
+constexpr int kBuf = 32 * kBufRow + 64;  // floats of the buffer, and of u's and g's biases (32 columns) behind it
 constexpr int kParts = 3;           // bf16 parts of an fp32 value
 constexpr int kDrain = 2;           // stages whose large products one accumulator takes (fp32)
 
@@ -157,26 +158,24 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) 
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// Two runs of 32 columns of this thread's lane of tensor memory, one wait for both.
-__device__ __forceinline__ void tmem_ld32_twice(uint32_t t0, uint32_t t1, float (&v)[32], float (&w)[32]) {
-  uint32_t r[64];
+// 16 columns of this thread's lane of tensor memory from t0 on, and 16 from t1 on; one wait for both.
+__device__ __forceinline__ void tmem_ld16_twice(uint32_t t0, uint32_t t1, float (&v)[16], float (&w)[16]) {
+  uint32_t r[32];
 #define SEMX_R8(o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n"
       "tcgen05.wait::ld.sync.aligned;\n"
-      : SEMX_R8(0), SEMX_R8(8), SEMX_R8(16), SEMX_R8(24), SEMX_R8(32), SEMX_R8(40), SEMX_R8(48), SEMX_R8(56)
+      : SEMX_R8(0), SEMX_R8(8), SEMX_R8(16), SEMX_R8(24)
       : "r"(t0), "r"(t1)
       : "memory");
 #undef SEMX_R8
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < 16; ++i) {
     v[i] = __uint_as_float(r[i]);
-    w[i] = __uint_as_float(r[32 + i]);
+    w[i] = __uint_as_float(r[16 + i]);
   }
 }
 // Descriptor of an operand in 128-byte rows with the 128-byte swizzle. K-major: a row is 64 values of
@@ -240,22 +239,22 @@ __device__ __forceinline__ Tile tile_at(const GemmParams& p, int w) {
   return t;
 }
 
-// 32 x 32 values, a lane's row each, to out[row0 ..][col0 ..] through the warp's buffer, so that a
+// 32 rows of 16 values, a lane's row each, to out[row0 ..][col0 ..] through the warp's buffer, so that a
 // row's values leave as whole sectors. rows, cols: how many of them exist.
-__device__ __forceinline__ void write_block(float* buf, const float (&v)[32], void* out, int64_t ld, int64_t row0, int64_t col0,
+__device__ __forceinline__ void write_block(float* buf, const float (&v)[kCols], void* out, int64_t ld, int64_t row0, int64_t col0,
                                             int rows, int cols, int bf16) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 32; i += 4)
+  for (int i = 0; i < kCols; i += 4)
     *reinterpret_cast<float4*>(&buf[lane * kBufRow + i]) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
   __syncwarp();
   if (bf16) {
     __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(out) + row0 * ld + col0;
-    if (cols >= 32 && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
-      const int c = lane % 4 * 8;
+    if (cols >= kCols && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      const int c = lane % 2 * 8;
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int r = it * 8 + lane / 4;
+      for (int it = 0; it < 2; ++it) {
+        const int r = it * 16 + lane / 2;
         const float4 a = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c]);
         const float4 b = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c + 4]);
         uint4 q;
@@ -267,22 +266,24 @@ __device__ __forceinline__ void write_block(float* buf, const float (&v)[32], vo
         if (r < rows) *reinterpret_cast<uint4*>(to + r * ld + c) = q;
       }
     } else {
-      for (int r = 0; r < rows; ++r)
-        if (lane < cols) to[r * ld + lane] = __float2bfloat16(buf[r * kBufRow + lane]);
+      const int c = lane % kCols;
+      for (int r = lane / kCols; r < rows; r += 2)
+        if (c < cols) to[r * ld + c] = __float2bfloat16(buf[r * kBufRow + c]);
     }
   } else {
     float* to = reinterpret_cast<float*>(out) + row0 * ld + col0;
-    if (cols >= 32 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
-      const int c = lane % 8 * 4;
+    if (cols >= kCols && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      const int c = lane % 4 * 4;
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int r = it * 4 + lane / 8;
+      for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + lane / 4;
         const float4 a = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c]);
         if (r < rows) *reinterpret_cast<float4*>(to + r * ld + c) = a;
       }
     } else {
-      for (int r = 0; r < rows; ++r)
-        if (lane < cols) to[r * ld + lane] = buf[r * kBufRow + lane];
+      const int c = lane % kCols;
+      for (int r = lane / kCols; r < rows; r += 2)
+        if (c < cols) to[r * ld + c] = buf[r * kBufRow + c];
     }
   }
   __syncwarp();
@@ -431,11 +432,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
     }
   } else {
     float* buf = bufs + warp * kBuf;
-    const int quarter = warp % 4, side = warp / 4;  // rows; columns (the first or the second half of u's and g's, or of the tile)
+    const int quarter = warp % 4, side = warp / 4;  // rows; columns (which quarter of u's and g's, or of the tile)
     const uint32_t lanes = (uint32_t)quarter << 21;
-    // Columns of the result that a warp has; of 32 the first four warps have all.
-    constexpr int WC = CN > 32 ? CN / 2 : CN;
-    const bool idle = CN <= 32 && side > 0;
+    // Columns of the result that a warp has; of 32 the first eight warps have all.
+    constexpr int WC = CN > 32 ? CN / 4 : 16;
+    const bool idle = side * WC >= CN;
     constexpr int VALUES = MODE == kFwd ? 2 * WC : WC;  // of the accumulator
     const uint32_t acc_e0 = in_cluster(&acc_empty[0], 0), acc_e1 = in_cluster(&acc_empty[1], 0);
     const uint32_t small_e0 = in_cluster(&small_empty[0], 0), small_e1 = in_cluster(&small_empty[1], 0);
@@ -446,10 +447,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
     };
     // Column (of the accumulator) of value i of this warp.
     auto column = [&](int i) { return MODE == kFwd ? (i / WC) * CN + side * WC + i % WC : side * WC + i; };
-    // What becomes of 32 columns from c of the result on: v (and g, kFwd).
-    auto write = [&](const Tile& t, int c, float (&v)[32], float (&g)[32]) {
+    // What becomes of 16 columns from c of the result on: v (and g, kFwd).
+    auto write = [&](const Tile& t, int c, float (&v)[kCols], float (&g)[kCols]) {
       const int64_t row0 = ((int64_t)t.m * 2 + rank) * kM + quarter * 32, col0 = (int64_t)t.n * CN + side * WC + c;
-      const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0)), cols = (int)max((int64_t)0, min((int64_t)32, p.N - col0));
+      const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0)), cols = (int)max((int64_t)0, min((int64_t)kCols, p.N - col0));
       if (rows == 0 || cols == 0) return;
       if (MODE == kFwd) {
         if (p.splits > 1) {
@@ -461,8 +462,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         if (p.bias != nullptr) {
           const float* at = buf + 32 * kBufRow + c;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 bu = *reinterpret_cast<const float4*>(at + i), bg = *reinterpret_cast<const float4*>(at + 64 + i);
+          for (int i = 0; i < kCols; i += 4) {
+            const float4 bu = *reinterpret_cast<const float4*>(at + i), bg = *reinterpret_cast<const float4*>(at + 32 + i);
             v[i] += bu.x; v[i + 1] += bu.y; v[i + 2] += bu.z; v[i + 3] += bu.w;
             g[i] += bg.x; g[i + 1] += bg.y; g[i + 2] += bg.z; g[i + 3] += bg.w;
           }
@@ -472,7 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           write_block(buf, g, p.g, p.ldu, row0, col0, rows, cols, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= act_of(g[i], p.gelu);
+        for (int i = 0; i < kCols; ++i) v[i] *= act_of(g[i], p.gelu);
         write_block(buf, v, p.out, p.ldo, row0, col0, rows, cols, p.out_bf16);
       } else {
         const int64_t half0 = (int64_t)t.half * p.M;
@@ -488,13 +489,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
     for (int w = pair0; w < works; w += pairs, ++tiles) {
       const Tile t = tile_at(p, w);
       if (MODE == kFwd && p.bias != nullptr) {  // the tile's biases, while its products run
-        static_assert(MODE != kFwd || WC <= 64, "biases");
+        static_assert(MODE != kFwd || WC <= 32, "biases");
         __syncwarp();
-        for (int c = lane; c < WC; c += 32) {
-          const int64_t col = (int64_t)t.n * CN + side * WC + c;
-          float* at = buf + 32 * kBufRow + c;
+        if (lane < WC) {
+          const int64_t col = (int64_t)t.n * CN + side * WC + lane;
+          float* at = buf + 32 * kBufRow + lane;
           at[0] = col < p.N ? semx_scan::load(p.bias, col, p.bias_bf16) : 0.f;
-          at[64] = col < p.N ? semx_scan::load(p.bias, p.N + col, p.bias_bf16) : 0.f;
+          at[32] = col < p.N ? semx_scan::load(p.bias, p.N + col, p.bias_bf16) : 0.f;
         }
         __syncwarp();
       }
@@ -505,12 +506,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         semx::tc::fence_after_sync();
         if (idle) release(b ? acc_e1 : acc_e0);
 #pragma unroll 1
-        for (int c = 0; c < WC && !idle; c += 32) {
-          float v[32], g[32];
-          if (MODE == kFwd) tmem_ld32_twice(d + column(c), d + column(WC + c), v, g);
-          else semx::tc::tmem_ld32(d + column(c), v);
-          if (c + 32 >= WC) release(b ? acc_e1 : acc_e0);
+        for (int c = 0; c < WC && !idle; c += MODE == kFwd ? kCols : 2 * kCols) {
+          float v[kCols], g[kCols];  // of u and g, or of 32 neighbours
+          tmem_ld16_twice(d + column(c), d + column(MODE == kFwd ? WC + c : c + kCols), v, g);
+          if (c + (MODE == kFwd ? 1 : 2) * kCols >= WC) release(b ? acc_e1 : acc_e0);
           write(t, c, v, g);
+          if (MODE != kFwd) write(t, c + kCols, g, v);
         }
         ++acc;
       } else {
@@ -525,13 +526,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           if (!ok) break;
           semx::tc::fence_after_sync();
 #pragma unroll
-          for (int i = 0; i < VALUES; i += 64) {
-            float v[32], y[32];
-            tmem_ld32_twice(d + column(i), d + column(i + 32), v, y);
+          for (int i = 0; i < VALUES; i += 2 * kCols) {
+            float v[kCols], y[kCols];
+            tmem_ld16_twice(d + column(i), d + column(i + kCols), v, y);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < kCols; ++j) {
               sum[i + j] = c0 == k0 ? v[j] : sum[i + j] + v[j];
-              sum[i + 32 + j] = c0 == k0 ? y[j] : sum[i + 32 + j] + y[j];
+              sum[i + kCols + j] = c0 == k0 ? y[j] : sum[i + kCols + j] + y[j];
             }
           }
           release(b ? acc_e1 : acc_e0);
@@ -541,20 +542,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         if (!__all_sync(0xffffffffu, ok)) break;
         semx::tc::fence_after_sync();
 #pragma unroll
-        for (int i = 0; i < VALUES; i += 32) {
-          float v[32];
-          semx::tc::tmem_ld32(tmem + 2 * BN + (tiles & 1) * BN + lanes + column(i), v);
+        for (int i = 0; i < VALUES; i += 2 * kCols) {
+          float v[kCols], y[kCols];
+          const uint32_t small = tmem + 2 * BN + (tiles & 1) * BN + lanes;
+          tmem_ld16_twice(small + column(i), small + column(i + kCols), v, y);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[i + j] += v[j];
+          for (int j = 0; j < kCols; ++j) {
+            sum[i + j] += v[j];
+            sum[i + kCols + j] += y[j];
+          }
         }
         release((tiles & 1) ? small_e1 : small_e0);
 #pragma unroll
-        for (int c = 0; c < WC; c += 32) {
-          float v[32], g[32];
+        for (int c = 0; c < WC; c += kCols) {
+          float v[kCols], g[kCols];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < kCols; ++j) {
             v[j] = sum[c + j];
-            if (MODE == kFwd) g[j] = sum[WC + c + j];
+            g[j] = MODE == kFwd ? sum[WC + c + j] : 0.f;
           }
           write(t, c, v, g);
         }
