@@ -335,55 +335,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
 
   if (warp == kEpi) {
     if (lane == 0) {
-      uint32_t it = 0;
+      // (No divisions in here: a stage is 512 cycles of products, and this is one thread.)
+      const uint32_t bars = in_cluster(&full[0], 0);
+      uint32_t s = 0, phase = 1, issued = 0;
       bool ok = true;
       for (int w = pair0; w < works && ok; w += pairs) {
         const Tile t = tile_at(p, w);
         int k0, k1;
         slice(t, &k0, &k1);
         const int m0 = t.m * 2 * kM + (int)rank * kM, n0 = t.n * BN + (int)rank * (BN / 2);
+        int kh = k0 >= p.khalf ? 1 : 0, kk = (k0 - kh * p.khalf) * kK;
         for (int k = k0; k < k1 && ok; ++k) {
-          const int kh = k / p.khalf, kk = (k % p.khalf) * kK;
-          for (int part = 0; part < PARTS; ++part, ++it) {
-            const int s = it % ST;
-            ok = wait_phase(&empty[s], ((it / ST) & 1) ^ 1, &dead);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            ok = wait_phase(&empty[s], phase, &dead);
             if (!ok) break;
             if (rank == 0) expect_bytes(&full[s], 2 * BYTES);
-            const uint32_t bar = in_cluster(&full[s], 0);
+            const uint32_t bar = bars + 8 * s;
             uint8_t *sa = slot0 + s * BYTES, *sb = sa + ABYTES;
             if (MODE == kDw) {
+#pragma unroll
               for (int b = 0; b < kM / 64; ++b) tma_load(sa + b * 8192, &map_a, m0 + b * 64, kk, t.half, part, bar);
+#pragma unroll
               for (int b = 0; b < BN / 128; ++b) tma_load(sb + b * 8192, &map_b, n0 + b * 64, kk, 0, part, bar);
             } else if (MODE == kDx) {
               tma_load(sa, &map_a, kk, m0, kh, part, bar);
+#pragma unroll
               for (int b = 0; b < BN / 128; ++b) tma_load(sb + b * 8192, &map_b, n0 + b * 64, kk, kh, part, bar);
             } else {  // CTA 0 brings u's rows of W, CTA 1 g's
               tma_load(sa, &map_a, kk, m0, 0, part, bar);
               tma_load(sb, &map_b, kk, t.n * CN, (int)rank, part, bar);
             }
+            ++issued;
+            if (++s == ST) s = 0, phase ^= 1;
           }
+          kk += kK;
+          if (kk >= p.khalf * kK) kk = 0, ++kh;
         }
       }
       // After a wait that gave up: the copies on their way land before the CTAs end (CTA 0 sees both CTAs').
       if (!ok && rank == 0)
-        for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) wait_some(&full[i % ST], (i / ST) & 1, nullptr);
+        for (uint32_t i = issued > ST ? issued - ST : 0; i < issued; ++i) wait_some(&full[i % ST], (i / ST) & 1, nullptr);
     }
   } else if (warp == kEpi + 1) {
     if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc = idesc_bf16(2 * kM, BN, A_MN, B_MN);
       constexpr uint32_t a_step = (A_MN ? 2048 : 32), b_step = (B_MN ? 2048 : 32);  // 16 of the depth
-      uint32_t it = 0, acc = 0, tiles = 0;
+      const uint64_t desc_a = operand_desc<A_MN>(semx::tc::smem_addr(slot0)), desc_b = operand_desc<B_MN>(semx::tc::smem_addr(slot0) + ABYTES);
+      uint32_t acc = 0, tiles = 0, s = 0, phase = 0;
       bool ok = true;
-      auto multiply = [&](uint32_t d, int sa, int sb, bool accumulate) {
-        const uint32_t a = semx::tc::smem_addr(slot0 + sa * BYTES), b = semx::tc::smem_addr(slot0 + sb * BYTES) + ABYTES;
+      auto multiply = [&](uint32_t d, uint32_t sa, uint32_t sb, bool accumulate) {
+        const uint64_t a = desc_a + sa * (BYTES >> 4), b = desc_b + sb * (BYTES >> 4);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          mma_pair(d, operand_desc<A_MN>(a + q * a_step), operand_desc<B_MN>(b + q * b_step), idesc, accumulate || q > 0);
+        for (int q = 0; q < 4; ++q) mma_pair(d, a + q * (a_step >> 4), b + q * (b_step >> 4), idesc, accumulate || q > 0);
       };
-      auto ready = [&](uint32_t i) {
-        ok = ok && wait_phase(&full[i % ST], (i / ST) & 1, &dead);
+      // The next slot, once its copies are there.
+      auto next_slot = [&]() {
+        const uint32_t at = s;
+        ok = wait_phase(&full[at], phase, &dead);
         semx::tc::fence_after_sync();
-        return ok;
+        if (++s == ST) s = 0, phase ^= 1;
+        return at;
       };
       for (int w = pair0; w < works && ok; w += pairs, ++tiles) {
         const Tile t = tile_at(p, w);
@@ -401,17 +413,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           if (!ok) break;
           semx::tc::fence_after_sync();
           const int c1 = min(k1, c0 + drain);
-          for (int k = c0; k < c1; ++k, it += PARTS) {
-            const int s0 = it % ST;
-            if (!ready(it)) break;
+          for (int k = c0; k < c1; ++k) {
+            const uint32_t s0 = next_slot();
+            if (!ok) break;
             multiply(d, s0, s0, k > c0);
             if (PARTS > 1) {
-              const int s1 = (it + 1) % ST, s2 = (it + 2) % ST;
-              if (!ready(it + 1)) break;
+              const uint32_t s1 = next_slot();
+              if (!ok) break;
               multiply(small, s0, s1, k > k0);
               multiply(small, s1, s0, true);
               multiply(small, s1, s1, true);
-              if (!ready(it + 2)) break;
+              const uint32_t s2 = next_slot();
+              if (!ok) break;
               multiply(small, s0, s2, true);
               multiply(small, s2, s0, true);
               commit_pair(&empty[s0]);
