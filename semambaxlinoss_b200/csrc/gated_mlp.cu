@@ -193,6 +193,12 @@ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn, bool b_mn) {
          | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// One lane of the warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
 // Waits for a phase of bar, some two seconds at most.
 __device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity, volatile int* dead) {
   if (semx::tc::mbar_wait(bar, parity, 16)) return true;
@@ -305,7 +311,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
   __shared__ int dead;
   uint8_t* slot0 = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   float* bufs = reinterpret_cast<float*>(slot0 + ST * BYTES);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  // (Of the whole warp, and known to be: the loading and the issuing warp run their loops as one.)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid & 31;
   const uint32_t rank = cluster_rank();
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -326,7 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
   __syncthreads();
   cluster_sync();
   semx::tc::fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   const int works = p.tiles * p.splits, pair0 = blockIdx.x / 2, pairs = gridDim.x / 2;
   auto slice = [&](const Tile& t, int* k0, int* k1) {
     *k0 = (int)((int64_t)p.depth * t.split / p.splits);
@@ -334,25 +341,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
   };
 
   if (warp == kEpi) {
-    if (lane == 0) {
-      // (No divisions in here: a stage is 512 cycles of products, and this is one thread.)
-      const uint32_t bars = in_cluster(&full[0], 0);
-      uint32_t s = 0, phase = 1, issued = 0;
-      bool ok = true;
-      for (int w = pair0; w < works && ok; w += pairs) {
-        const Tile t = tile_at(p, w);
-        int k0, k1;
-        slice(t, &k0, &k1);
-        const int m0 = t.m * 2 * kM + (int)rank * kM, n0 = t.n * BN + (int)rank * (BN / 2);
-        int kh = k0 >= p.khalf ? 1 : 0, kk = (k0 - kh * p.khalf) * kK;
-        for (int k = k0; k < k1 && ok; ++k) {
+    // The warp runs the loop as one and one lane issues, so that what the copies take is in uniform
+    // registers; no divisions in here: a stage is 512 cycles of products.
+    const bool issues = elect_one();
+    const uint32_t bars = in_cluster(&full[0], 0);
+    uint32_t s = 0, phase = 1, issued = 0;
+    bool ok = true;
+    for (int w = pair0; w < works && ok; w += pairs) {
+      const Tile t = tile_at(p, w);
+      int k0, k1;
+      slice(t, &k0, &k1);
+      const int m0 = t.m * 2 * kM + (int)rank * kM, n0 = t.n * BN + (int)rank * (BN / 2);
+      int kh = k0 >= p.khalf ? 1 : 0, kk = (k0 - kh * p.khalf) * kK;
+      for (int k = k0; k < k1 && ok; ++k) {
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            ok = wait_phase(&empty[s], phase, &dead);
-            if (!ok) break;
+        for (int part = 0; part < PARTS; ++part) {
+          ok = __all_sync(0xffffffffu, wait_phase(&empty[s], phase, &dead));
+          if (!ok) break;
+          const uint32_t bar = bars + 8 * s;
+          uint8_t *sa = slot0 + s * BYTES, *sb = sa + ABYTES;
+          if (issues) {
             if (rank == 0) expect_bytes(&full[s], 2 * BYTES);
-            const uint32_t bar = bars + 8 * s;
-            uint8_t *sa = slot0 + s * BYTES, *sb = sa + ABYTES;
             if (MODE == kDw) {
 #pragma unroll
               for (int b = 0; b < kM / 64; ++b) tma_load(sa + b * 8192, &map_a, m0 + b * 64, kk, t.half, part, bar);
@@ -366,34 +375,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
               tma_load(sa, &map_a, kk, m0, 0, part, bar);
               tma_load(sb, &map_b, kk, t.n * CN, (int)rank, part, bar);
             }
-            ++issued;
-            if (++s == ST) s = 0, phase ^= 1;
           }
-          kk += kK;
-          if (kk >= p.khalf * kK) kk = 0, ++kh;
+          __syncwarp();
+          ++issued;
+          if (++s == ST) s = 0, phase ^= 1;
         }
+        kk += kK;
+        if (kk >= p.khalf * kK) kk = 0, ++kh;
       }
-      // After a wait that gave up: the copies on their way land before the CTAs end (CTA 0 sees both CTAs').
-      if (!ok && rank == 0)
-        for (uint32_t i = issued > ST ? issued - ST : 0; i < issued; ++i) wait_some(&full[i % ST], (i / ST) & 1, nullptr);
     }
+    // After a wait that gave up: the copies on their way land before the CTAs end (CTA 0 sees both CTAs').
+    if (!ok && rank == 0)
+      for (uint32_t i = issued > ST ? issued - ST : 0; i < issued; ++i) wait_some(&full[i % ST], (i / ST) & 1, nullptr);
   } else if (warp == kEpi + 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc_bf16(2 * kM, BN, A_MN, B_MN);
       constexpr uint32_t a_step = (A_MN ? 2048 : 32), b_step = (B_MN ? 2048 : 32);  // 16 of the depth
+      const bool issues = elect_one();
       const uint64_t desc_a = operand_desc<A_MN>(semx::tc::smem_addr(slot0)), desc_b = operand_desc<B_MN>(semx::tc::smem_addr(slot0) + ABYTES);
       uint32_t acc = 0, tiles = 0, s = 0, phase = 0;
       bool ok = true;
       auto multiply = [&](uint32_t d, uint32_t sa, uint32_t sb, bool accumulate) {
         const uint64_t a = desc_a + sa * (BYTES >> 4), b = desc_b + sb * (BYTES >> 4);
+        if (issues) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mma_pair(d, a + q * (a_step >> 4), b + q * (b_step >> 4), idesc, accumulate || q > 0);
+          for (int q = 0; q < 4; ++q) mma_pair(d, a + q * (a_step >> 4), b + q * (b_step >> 4), idesc, accumulate || q > 0);
+        }
+      };
+      auto await = [&](uint64_t* bar, uint32_t parity) {
+        ok = __all_sync(0xffffffffu, wait_phase(bar, parity, &dead));
+        semx::tc::fence_after_sync();
+        return ok;
+      };
+      auto done = [&](uint64_t* bar) {
+        if (issues) commit_pair(bar);
+        __syncwarp();
       };
       // The next slot, once its copies are there.
       auto next_slot = [&]() {
         const uint32_t at = s;
-        ok = wait_phase(&full[at], phase, &dead);
-        semx::tc::fence_after_sync();
+        await(&full[at], phase);
         if (++s == ST) s = 0, phase ^= 1;
         return at;
       };
@@ -402,16 +423,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         int k0, k1;
         slice(t, &k0, &k1);
         const uint32_t small = tmem + 2 * BN + (tiles & 1) * BN;
-        if (PARTS > 1) {
-          ok = wait_phase(&small_empty[tiles & 1], ((tiles >> 1) & 1) ^ 1, &dead);
-          if (!ok) break;
-        }
+        if (PARTS > 1 && !await(&small_empty[tiles & 1], ((tiles >> 1) & 1) ^ 1)) break;
         const int drain = PARTS > 1 ? kDrain : k1 - k0;
         for (int c0 = k0; c0 < k1 && ok; c0 += drain, ++acc) {
           const uint32_t b = acc & 1, d = tmem + b * BN;
-          ok = wait_phase(&acc_empty[b], ((acc >> 1) & 1) ^ 1, &dead);
-          if (!ok) break;
-          semx::tc::fence_after_sync();
+          if (!await(&acc_empty[b], ((acc >> 1) & 1) ^ 1)) break;
           const int c1 = min(k1, c0 + drain);
           for (int k = c0; k < c1; ++k) {
             const uint32_t s0 = next_slot();
@@ -427,19 +443,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
               if (!ok) break;
               multiply(small, s0, s2, true);
               multiply(small, s2, s0, true);
-              commit_pair(&empty[s0]);
-              commit_pair(&empty[s1]);
-              commit_pair(&empty[s2]);
+              done(&empty[s0]);
+              done(&empty[s1]);
+              done(&empty[s2]);
             } else {
-              commit_pair(&empty[s0]);
+              done(&empty[s0]);
             }
           }
-          if (ok) commit_pair(&acc_full[b]);
+          if (ok) done(&acc_full[b]);
         }
-        if (PARTS > 1 && ok) commit_pair(&small_full[tiles & 1]);
+        if (PARTS > 1 && ok) done(&small_full[tiles & 1]);
       }
       if (!ok) {  // products on their way end before tensor memory is given back
-        commit_pair(&drained);
+        done(&drained);
         wait_some(&drained, 0, nullptr);
       }
     }
