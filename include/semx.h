@@ -788,8 +788,9 @@ int semx_gated_lru_step(const SemxGatedLruArgs* args, semx_stream_t stream);
  * (2 H, may be NULL) by bias_bf16, db (2 H, may be NULL) fp32. Sums are fp32; fp32 operands keep 2^-24 of each product (as three
  * bf16 parts; an infinity among them gives NaN).
  * A training forward passes saved (semx_gated_linear_saved_bytes(): u and g in fp32, 16-byte
- * aligned); the backward reads it and writes dx, dw and db (each may be NULL), sums in a fixed
- * order. Workspace (16-byte aligned, of this call alone): semx_gated_linear_workspace_bytes() of
+ * aligned; 0 bytes for narrow bf16 rows, whose u and g the backward makes again from x, w and
+ * bias) and the backward reads it. It writes dx, dw and db (each may be NULL), sums in a
+ * fixed order. Workspace (16-byte aligned, of this call alone): semx_gated_linear_workspace_bytes() of
  * the filled struct with `backward` 0 or 1. */
 typedef struct SemxGatedLinearArgs {
   uint32_t struct_size;

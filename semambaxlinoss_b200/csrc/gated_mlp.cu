@@ -46,24 +46,28 @@ constexpr int kDrain = 2;           // stages whose large products one accumulat
 
 __device__ unsigned int g_gemm_timeouts;
 
-enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
+enum Mode { kFwd = 0, kDx = 1, kDw = 2, kGate = 3 };  // kGate (bf16): the forward's products again, for du and dg
 
 struct GemmParams {
   int64_t M, N;           // rows and columns of the result (kFwd: N = H; kDw: M = H, once per half)
   int tiles_m, tiles_n;   // kDw: tiles_m of one half
   int tiles;              // in all
   int depth, khalf;       // stages in all, and of one half of the depth (kDx: u, then g)
-  int splits;             // slices of the depth
+  int whole, splits;      // tiles from number `whole` on run in as many slices of the depth
   void* out;              // kFwd: h
   int64_t ldo;
   int out_bf16;
+  const void* dh;         // kGate: (M, N) of out's type
+  __nv_bfloat16* dz;      // kGate: du and dg (2, M, ldz)
+  int64_t ldz;
+  float* sums;            // kGate: column sums of each warp's 32 rows (8 tiles_m, 2 N), or NULL
   float* u;               // kFwd: u and g in front of the activation, or NULL
   float* g;
   int64_t ldu;
   const void* bias;       // (2 H) or NULL
   int bias_bf16;
   int gelu;
-  float* part;            // with splits: (splits, result) sums, kFwd: (splits, 2, M, N)
+  float* part;            // sums of the sliced tiles: (slices, tiles - whole, 256, accumulator's columns)
 };
 
 // Half of erfc(|g| / sqrt(2)) and e = exp(-g^2 / 2): erfc(z) = t q(t) exp(-z^2) with t = 1 / (1 + z / 2); q is a
@@ -100,6 +104,19 @@ __device__ __forceinline__ void act_and_slope(float g, int gelu, float* act, flo
     *act = g * s;
     *slope = s * fmaf(g, 1.f - s, 1.f);
   }
+}
+
+// Value n of the parts of v: v rounded to bf16, then what is left, each rounded. What no bf16 holds
+// (infinities, NaN) stays in the first; a value that would round to infinity is cut instead.
+__device__ __forceinline__ void parts_of(float v, __nv_bfloat16 (&part)[kParts]) {
+  part[0] = __float2bfloat16(v);
+  float rest = 0.f;
+  if (fabsf(v) <= 3.4028234663852886e38f) {
+    if (fabsf(v) >= 3.3961775292304608e38f) part[0] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16));
+    rest = v - __bfloat162float(part[0]);
+  }
+  part[1] = __float2bfloat16(rest);
+  part[2] = __float2bfloat16(rest - __bfloat162float(part[1]));
 }
 
 // -- tensor core plumbing -----------------------------------------------------------------------
@@ -224,14 +241,18 @@ constexpr size_t gemm_smem(int bn) {
   return 1024 + (size_t)slots_of(bn) * slot_bytes(bn) + kEpi * kBuf * sizeof(float);
 }
 
+// Tile number `index` of the result; slice `split` of `of` of its depth.
 struct Tile {
-  int m, n, half, split;
+  int m, n, half, index, split, of;
 };
-__device__ __forceinline__ Tile tile_at(const GemmParams& p, int w) {
+__host__ __device__ __forceinline__ int works_of(const GemmParams& p) { return p.whole + (p.tiles - p.whole) * p.splits; }
+__device__ __forceinline__ Tile tile_number(const GemmParams& p, int index) {
   Tile t;
-  t.split = w % p.splits;
-  int i = w / p.splits;
+  t.index = index;
+  t.split = 0;
+  t.of = 1;
   t.half = 0;
+  int i = index;
   const int per_half = p.tiles_m * p.tiles_n;
   if (i >= per_half) {
     t.half = 1;
@@ -242,6 +263,14 @@ __device__ __forceinline__ Tile tile_at(const GemmParams& p, int w) {
   const int down = min(8, p.tiles_m - grp * 8);
   t.m = grp * 8 + r % down;
   t.n = r / down;
+  return t;
+}
+__device__ __forceinline__ Tile tile_at(const GemmParams& p, int w) {
+  if (w < p.whole) return tile_number(p, w);
+  const int i = (w - p.whole) / p.splits;
+  Tile t = tile_number(p, p.whole + i);
+  t.split = w - p.whole - i * p.splits;
+  t.of = p.splits;
   return t;
 }
 
@@ -295,14 +324,80 @@ __device__ __forceinline__ void write_block(float* buf, const float (&v)[kCols],
   __syncwarp();
 }
 
+// The other way: 32 rows of 16 bf16 values to a lane's row each, zeros where there are none.
+__device__ __forceinline__ void read_block(float* buf, float (&v)[kCols], const void* src, int64_t ld, int64_t row0, int64_t col0, int rows,
+                                           int cols) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(src) + row0 * ld + col0;
+  if (cols >= kCols && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    const int c = lane % 2 * 8;
+    uint4 q[2];
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      const int r = it * 16 + lane / 2;
+      q[it] = r < rows ? __ldcs(reinterpret_cast<const uint4*>(from + r * ld + c)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      float* to = &buf[(it * 16 + lane / 2) * kBufRow + c];
+      *reinterpret_cast<float4*>(to) = semx_scan::quad_floats<semx_scan::kBf16>(make_uint2(q[it].x, q[it].y), 1);
+      *reinterpret_cast<float4*>(to + 4) = semx_scan::quad_floats<semx_scan::kBf16>(make_uint2(q[it].z, q[it].w), 1);
+    }
+  } else {
+    const int c = lane % kCols;
+    for (int r = lane / kCols; r < 32; r += 2) buf[r * kBufRow + c] = r < rows && c < cols ? __bfloat162float(from[r * ld + c]) : 0.f;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kCols; i += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(&buf[lane * kBufRow + i]);
+    v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+  }
+  __syncwarp();
+}
+
+// 32 rows of 16 values as bf16 to rows of ld, a multiple of 8; columns of a row are written in eights.
+// Their column sums to sums[0 .. 15] where wanted.
+__device__ __forceinline__ void write_summed(float* buf, const float (&v)[kCols], __nv_bfloat16* to, int64_t ld, int rows, int cols,
+                                             float* sums) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kCols; i += 4)
+    *reinterpret_cast<float4*>(&buf[lane * kBufRow + i]) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  __syncwarp();
+  if (sums != nullptr) {  // (Rows that do not exist hold products with gradients of zero.)
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += buf[(2 * r + lane / kCols) * kBufRow + lane % kCols];
+    s += __shfl_xor_sync(0xffffffffu, s, kCols);
+    if (lane < cols) sums[lane] = s;
+  }
+  const int c = lane % 2 * 8;
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    const int r = it * 16 + lane / 2;
+    const float4 a = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c]);
+    const float4 b = *reinterpret_cast<const float4*>(&buf[r * kBufRow + c + 4]);
+    uint4 q;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+    h[0] = __floats2bfloat162_rn(a.x, a.y);
+    h[1] = __floats2bfloat162_rn(a.z, a.w);
+    h[2] = __floats2bfloat162_rn(b.x, b.y);
+    h[3] = __floats2bfloat162_rn(b.z, b.w);
+    if (r < rows && c < cols) *reinterpret_cast<uint4*>(to + r * ld + c) = q;
+  }
+  __syncwarp();
+}
+
 // Result of one mode. BN: columns of the accumulator (kFwd: BN / 2 of u, then as many of g). PARTS: 1
 // (bf16), or 3 (fp32; BN 128).
 template <int MODE, int BN, int PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
   constexpr int ST = slots_of(BN), BYTES = slot_bytes(BN), ABYTES = kM * kK * 2;
-  constexpr bool A_MN = MODE == kDw, B_MN = MODE != kFwd;
-  constexpr int CN = MODE == kFwd ? BN / 2 : BN;        // columns of the result in a tile
+  constexpr bool GATED = MODE == kFwd || MODE == kGate;  // u and g side by side
+  constexpr bool A_MN = MODE == kDw, B_MN = !GATED;
+  constexpr int CN = GATED ? BN / 2 : BN;               // columns of the result in a tile
   constexpr int COLS = (PARTS > 1 ? 4 : 2) * BN;        // of tensor memory: two accumulators, fp32 two more for the small products
   static_assert(COLS <= 512, "tensor memory");
   extern __shared__ uint8_t raw[];
@@ -334,10 +429,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
   cluster_sync();
   semx::tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  const int works = p.tiles * p.splits, pair0 = blockIdx.x / 2, pairs = gridDim.x / 2;
+  const int works = works_of(p), pair0 = blockIdx.x / 2, pairs = gridDim.x / 2;
   auto slice = [&](const Tile& t, int* k0, int* k1) {
-    *k0 = (int)((int64_t)p.depth * t.split / p.splits);
-    *k1 = (int)((int64_t)p.depth * (t.split + 1) / p.splits);
+    *k0 = (int)((int64_t)p.depth * t.split / t.of);
+    *k1 = (int)((int64_t)p.depth * (t.split + 1) / t.of);
   };
 
   if (warp == kEpi) {
@@ -466,7 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
     // Columns of the result that a warp has; of 32 the first eight warps have all.
     constexpr int WC = CN > 32 ? CN / 4 : 16;
     const bool idle = side * WC >= CN;
-    constexpr int VALUES = MODE == kFwd ? 2 * WC : WC;  // of the accumulator
+    constexpr int VALUES = GATED ? 2 * WC : WC;  // of the accumulator
     const uint32_t acc_e0 = in_cluster(&acc_empty[0], 0), acc_e1 = in_cluster(&acc_empty[1], 0);
     const uint32_t small_e0 = in_cluster(&small_empty[0], 0), small_e1 = in_cluster(&small_empty[1], 0);
     auto release = [&](uint32_t bar) {
@@ -475,19 +570,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
       if (lane == 0) arrive_in_cluster(bar);
     };
     // Column (of the accumulator) of value i of this warp.
-    auto column = [&](int i) { return MODE == kFwd ? (i / WC) * CN + side * WC + i % WC : side * WC + i; };
+    auto column = [&](int i) { return GATED ? (i / WC) * CN + side * WC + i % WC : side * WC + i; };
     // What becomes of 16 columns from c of the result on: v (and g, kFwd).
     auto write = [&](const Tile& t, int c, float (&v)[kCols], float (&g)[kCols]) {
       const int64_t row0 = ((int64_t)t.m * 2 + rank) * kM + quarter * 32, col0 = (int64_t)t.n * CN + side * WC + c;
       const int rows = (int)max((int64_t)0, min((int64_t)32, p.M - row0)), cols = (int)max((int64_t)0, min((int64_t)kCols, p.N - col0));
+      if (MODE == kGate && rows == 0 && p.sums != nullptr && lane < cols) {
+        float* to = p.sums + (((int64_t)t.m * 2 + rank) * 4 + quarter) * 2 * p.N + col0 + lane;
+        to[0] = to[p.N] = 0.f;
+      }
       if (rows == 0 || cols == 0) return;
-      if (MODE == kFwd) {
-        if (p.splits > 1) {
-          float* to = p.part + (int64_t)t.split * 2 * p.M * p.N;
-          write_block(buf, v, to, p.N, row0, col0, rows, cols, 0);
-          write_block(buf, g, to + p.M * p.N, p.N, row0, col0, rows, cols, 0);
-          return;
-        }
+      if (t.of > 1) {
+        float* to = p.part + ((int64_t)t.split * (p.tiles - p.whole) + t.index - p.whole) * (2 * kM * BN);
+        const int row = (int)rank * kM + quarter * 32, col = side * WC + c;
+        write_block(buf, v, to, BN, row, col, rows, kCols, 0);
+        if (GATED) write_block(buf, g, to, BN, row, CN + col, rows, kCols, 0);
+        return;
+      }
+      if constexpr (GATED) {
         if (p.bias != nullptr) {
           const float* at = buf + 32 * kBufRow + c;
 #pragma unroll
@@ -497,6 +597,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
             g[i] += bg.x; g[i + 1] += bg.y; g[i + 2] += bg.z; g[i + 3] += bg.w;
           }
         }
+        if constexpr (MODE == kGate) {
+          float d[kCols];
+          read_block(buf, d, p.dh, p.N, row0, col0, rows, cols);
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            float act, slope;
+            act_and_slope(g[i], p.gelu, &act, &slope);
+            g[i] = d[i] * v[i] * slope;
+            v[i] = d[i] * act;
+          }
+          float* to = p.sums == nullptr ? nullptr : p.sums + (((int64_t)t.m * 2 + rank) * 4 + quarter) * 2 * p.N + col0;
+          const int64_t at = row0 * p.ldz + col0;
+          write_summed(buf, v, p.dz + at, p.ldz, rows, cols, to);
+          write_summed(buf, g, p.dz + p.M * p.ldz + at, p.ldz, rows, cols, to == nullptr ? nullptr : to + p.N);
+          return;
+        }
         if (p.u != nullptr) {
           write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
           write_block(buf, g, p.g, p.ldu, row0, col0, rows, cols, 0);
@@ -505,20 +621,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         for (int i = 0; i < kCols; ++i) v[i] *= act_of(g[i], p.gelu);
         write_block(buf, v, p.out, p.ldo, row0, col0, rows, cols, p.out_bf16);
       } else {
-        const int64_t half0 = (int64_t)t.half * p.M;
-        if (p.splits > 1) {
-          const int64_t all = (MODE == kDw ? 2 : 1) * p.M * p.N;
-          write_block(buf, v, p.part + t.split * all + half0 * p.N, p.N, row0, col0, rows, cols, 0);
-        } else {
-          write_block(buf, v, p.out, p.ldo, half0 + row0, col0, rows, cols, p.out_bf16);
-        }
+        write_block(buf, v, p.out, p.ldo, (int64_t)t.half * p.M + row0, col0, rows, cols, p.out_bf16);
       }
     };
     uint32_t acc = 0, tiles = 0;
     for (int w = pair0; w < works; w += pairs, ++tiles) {
       const Tile t = tile_at(p, w);
-      if (MODE == kFwd && p.bias != nullptr) {  // the tile's biases, while its products run
-        static_assert(MODE != kFwd || WC <= 32, "biases");
+      if (GATED && p.bias != nullptr) {  // the tile's biases, while its products run
+        static_assert(!GATED || WC <= 32, "biases");
         __syncwarp();
         if (lane < WC) {
           const int64_t col = (int64_t)t.n * CN + side * WC + lane;
@@ -535,12 +645,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         semx::tc::fence_after_sync();
         if (idle) release(b ? acc_e1 : acc_e0);
 #pragma unroll 1
-        for (int c = 0; c < WC && !idle; c += MODE == kFwd ? kCols : 2 * kCols) {
+        for (int c = 0; c < WC && !idle; c += GATED ? kCols : 2 * kCols) {
           float v[kCols], g[kCols];  // of u and g, or of 32 neighbours
-          tmem_ld16_twice(d + column(c), d + column(MODE == kFwd ? WC + c : c + kCols), v, g);
-          if (c + (MODE == kFwd ? 1 : 2) * kCols >= WC) release(b ? acc_e1 : acc_e0);
+          tmem_ld16_twice(d + column(c), d + column(GATED ? WC + c : c + kCols), v, g);
+          if (c + (GATED ? 1 : 2) * kCols >= WC) release(b ? acc_e1 : acc_e0);
           write(t, c, v, g);
-          if (MODE != kFwd) write(t, c + kCols, g, v);
+          if (!GATED) write(t, c + kCols, g, v);
         }
         ++acc;
       } else {
@@ -588,7 +698,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
 #pragma unroll
           for (int j = 0; j < kCols; ++j) {
             v[j] = sum[c + j];
-            g[j] = MODE == kFwd ? sum[WC + c + j] : 0.f;
+            g[j] = GATED ? sum[WC + c + j] : 0.f;
           }
           write(t, c, v, g);
         }
@@ -602,48 +712,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
   if (warp == 0) tmem_dealloc_pair(tmem, COLS);
 }
 
-// Sums of the slices of the depth, in their order, and what the epilogue does with them.
-__global__ void __launch_bounds__(256) join_plain_kernel(const float* part, int splits, int64_t n, void* out, int bf16) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[k * n + i];
-  semx_scan::store(out, i, bf16, s);
-}
-__global__ void __launch_bounds__(256) join_gated_kernel(const GemmParams p) {
-  const int64_t n = p.M * p.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int64_t row = i / p.N, col = i % p.N;
-  float u = 0.f, g = 0.f;
-  for (int k = 0; k < p.splits; ++k) {
-    u += p.part[2 * k * n + i];
-    g += p.part[(2 * k + 1) * n + i];
+// Sums of the slices of a tile's depth, in their order, and what the epilogue does with them. A thread has
+// four columns of a row of a tile, eight slices on their way at a time.
+template <int MODE>
+__global__ void __launch_bounds__(256) join_kernel(const GemmParams p, int bn) {
+  const int cn = MODE == kFwd ? bn / 2 : bn, across = cn / 4, sliced = p.tiles - p.whole;
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int i = (int)(n / (2 * kM * across)), in = (int)(n % (2 * kM * across)), r = in / across, c = in % across * 4;
+  if (i >= sliced) return;
+  const Tile t = tile_number(p, p.whole + i);
+  const int64_t row = (int64_t)t.m * 2 * kM + r, col = (int64_t)t.n * cn + c;
+  const int nn = (int)min((int64_t)4, p.N - col);
+  if (row >= p.M || nn <= 0) return;
+  float u[4] = {}, g[4] = {};
+  const float* from = p.part + ((int64_t)i * (2 * kM) + r) * bn + c;
+  const int64_t next = (int64_t)sliced * 2 * kM * bn;
+  constexpr int AHEAD = MODE == kFwd ? 4 : 8;
+  for (int k0 = 0; k0 < p.splits; k0 += AHEAD) {
+    float4 a[AHEAD], b[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      a[k] = b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + k >= p.splits) continue;
+      a[k] = __ldcs(reinterpret_cast<const float4*>(from + (k0 + k) * next));
+      if (MODE == kFwd) b[k] = __ldcs(reinterpret_cast<const float4*>(from + (k0 + k) * next + cn));
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      u[0] += a[k].x; u[1] += a[k].y; u[2] += a[k].z; u[3] += a[k].w;
+      g[0] += b[k].x; g[1] += b[k].y; g[2] += b[k].z; g[3] += b[k].w;
+    }
   }
-  if (p.bias != nullptr) {
-    u += semx_scan::load(p.bias, col, p.bias_bf16);
-    g += semx_scan::load(p.bias, p.N + col, p.bias_bf16);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k >= nn || MODE != kFwd) break;
+    if (p.bias != nullptr) {
+      u[k] += semx_scan::load(p.bias, col + k, p.bias_bf16);
+      g[k] += semx_scan::load(p.bias, p.N + col + k, p.bias_bf16);
+    }
+    if (p.u != nullptr) {
+      p.u[row * p.ldu + col + k] = u[k];
+      p.g[row * p.ldu + col + k] = g[k];
+    }
+    u[k] *= act_of(g[k], p.gelu);
   }
-  if (p.u != nullptr) {
-    p.u[row * p.ldu + col] = u;
-    p.g[row * p.ldu + col] = g;
+  const int64_t at = ((int64_t)t.half * p.M + row) * p.ldo + col;
+  const float4 v = make_float4(u[0], u[1], u[2], u[3]);
+  if (nn == 4 && p.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (p.out_bf16 ? 7 : 15)) == 0) {
+    if (p.out_bf16) semx_scan::store_quad<semx_scan::kBf16>(p.out, at, 1, 4, v);
+    else semx_scan::store_quad<semx_scan::kFp32>(p.out, at, 0, 4, v);
+  } else {
+    semx_scan::store_quad<semx_scan::kAny>(p.out, at, p.out_bf16, nn, v);
   }
-  semx_scan::store(p.out, row * p.ldo + col, p.out_bf16, u * act_of(g, p.gelu));
 }
 
 // -- operands as the products read them -----------------------------------------------------------
-
-// Value n of the parts of v: v rounded to bf16, then what is left, each rounded. What no bf16 holds
-// (infinities, NaN) stays in the first; a value that would round to infinity is cut instead.
-__device__ __forceinline__ void parts_of(float v, __nv_bfloat16 (&part)[kParts]) {
-  part[0] = __float2bfloat16(v);
-  float rest = 0.f;
-  if (fabsf(v) <= 3.4028234663852886e38f) {
-    if (fabsf(v) >= 3.3961775292304608e38f) part[0] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16));
-    rest = v - __bfloat162float(part[0]);
-  }
-  part[1] = __float2bfloat16(rest);
-  part[2] = __float2bfloat16(rest - __bfloat162float(part[1]));
-}
 
 // rows x cols values at row stride ld into (parts, rows, ldp) bf16, ldp a multiple of 8; a thread has
 // 8 neighbours. Columns behind the last one are left: the tensor map ends in front of them.
@@ -774,7 +897,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 4 : 3) gate_grad_kernel(cons
 
 // Up to R rows of x. A warp has two columns (four rows of W); x lies in shared memory in fp32, kDepth
 // values of each row at a time. Its lanes take 8 neighbouring weights of every 256.
-constexpr int kDepth = 2048, kFewT = 256, kFew = 8;
+constexpr int kDepth = 2048, kFewT = 256, kFew = 8, kFewBf16 = 16;
 // Place of value k in a row in shared memory: of every 256, the first halves of the lanes' eights, then
 // the second ones, so that lanes side by side read side by side.
 __device__ __forceinline__ int spread(int k) { return (k & ~255) | (k & 4) << 5 | (k & 248) >> 1 | (k & 3); }
@@ -868,6 +991,88 @@ __global__ void __launch_bounds__(kFewT) few_rows_kernel(const void* x, int64_t 
   }
 }
 
+// bf16 rows, up to 8 NT of them: products of 16 rows of W (eight of u, the same eight of g) by 16 of the depth
+// by 8 rows of x. The depth may be taken in any order, so a lane's eight neighbouring weights (16 bytes) are
+// its values of two products, and nothing of W passes through shared memory: each warp streams its rows.
+// (tcgen05 would have tiles of 128 rows of x, nearly all of them empty.) Four warps share the depth of
+// eight columns; their sums meet in shared memory.
+constexpr int kFewWarps = 4;
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int NT>
+__global__ void __launch_bounds__(kFewWarps * 32) few_rows_bf16_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, int64_t D,
+                                                                       int64_t H, int rows, const GemmParams p) {
+  __shared__ float sums[kFewWarps][NT * 8][17];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, q = lane / 4, t = lane % 4;
+  const int64_t h0 = (int64_t)blockIdx.x * 8;
+  // Lane (q, t): row q of u's and of g's eight, values 8 t .. 8 t + 7 of every 32 of the depth; of x row q.
+  const __nv_bfloat16* wu = w + min(h0 + q, H - 1) * D + 8 * t;
+  const __nv_bfloat16* wg = wu + H * D;
+  const __nv_bfloat16* xr[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) xr[n] = x + min(n * 8 + q, rows - 1) * ldx + 8 * t;
+  float c[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+  // D is a multiple of 8: a lane's eight values exist or do not.
+  constexpr int AHEAD = NT > 1 ? 4 : 8;
+  const int blocks = (int)((D + 31) / 32);  // of 32 of the depth; warp k has every fourth run of AHEAD
+  for (int b0 = warp * AHEAD; b0 < blocks; b0 += kFewWarps * AHEAD) {
+    uint4 u[AHEAD], g[AHEAD], v[AHEAD][NT];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int64_t k = (int64_t)(b0 + a) * 32;
+      const bool in = k + 8 * t < D;
+      u[a] = in ? __ldcs(reinterpret_cast<const uint4*>(wu + k)) : make_uint4(0u, 0u, 0u, 0u);
+      g[a] = in ? __ldcs(reinterpret_cast<const uint4*>(wg + k)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) v[a][n] = in ? *reinterpret_cast<const uint4*>(xr[n] + k) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_16x8x16(c[n], u[a].x, g[a].x, u[a].y, g[a].y, v[a][n].x, v[a][n].y);
+        mma_16x8x16(c[n], u[a].z, g[a].z, u[a].w, g[a].w, v[a][n].z, v[a][n].w);
+      }
+  }
+  // c[0], c[1]: u of column q for rows 2 t and 2 t + 1 of x; c[2], c[3]: g.
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      sums[warp][n * 8 + 2 * t + k][q] = c[n][k];
+      sums[warp][n * 8 + 2 * t + k][8 + q] = c[n][2 + k];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NT * 64; i += kFewWarps * 32) {
+    const int r = i / 8, k = i % 8;
+    const int64_t h = h0 + k;
+    if (r >= rows || h >= H) continue;
+    float uu = 0.f, gg = 0.f;
+#pragma unroll
+    for (int a = 0; a < kFewWarps; ++a) {
+      uu += sums[a][r][k];
+      gg += sums[a][r][8 + k];
+    }
+    if (p.bias != nullptr) {
+      uu += semx_scan::load(p.bias, h, p.bias_bf16);
+      gg += semx_scan::load(p.bias, H + h, p.bias_bf16);
+    }
+    if (p.u != nullptr) {
+      p.u[r * p.ldu + h] = uu;
+      p.g[r * p.ldu + h] = gg;
+    }
+    semx_scan::store(p.out, r * p.ldo + h, 1, uu * act_of(gg, p.gelu));
+  }
+}
+
+// Whether the backward makes u and g again.
+bool makes_again(const SemxGatedLinearArgs* a) { return a->bf16 && a->D <= 512; }
+
 // -- host ---------------------------------------------------------------------------------------
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -917,7 +1122,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // What one product needs: tile width, slices of the depth, bytes of their sums.
 struct Plan {
-  int mode, bn, splits;
+  int mode, bn;
   GemmParams p;
   size_t part_bytes;
 };
@@ -935,7 +1140,8 @@ Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   p.N = N;
   p.khalf = (int)cdiv(K, (int64_t)kK);
   p.depth = p.khalf * (mode == kDx ? 2 : 1);
-  const int64_t wide = mode == kFwd ? 2 * N : N;
+  const bool gated = mode == kFwd || mode == kGate;
+  const int64_t wide = gated ? 2 * N : N;
   const int64_t down = cdiv(M, (int64_t)2 * kM) * (mode == kDw ? 2 : 1);
   // The tile width that takes the least time in rounds of all pairs of SMs. (The operands read along the result need 128.)
   int64_t least = 0;
@@ -947,34 +1153,44 @@ Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   p.tiles_m = (int)cdiv(M, (int64_t)2 * kM);
   p.tiles_n = (int)cdiv(wide, (int64_t)q.bn);
   p.tiles = p.tiles_m * p.tiles_n * (mode == kDw ? 2 : 1);
-  // Slices of the depth where tiles alone leave half of the SMs idle, of 8 stages (fp32: 4, each of them
-  // six products) at least.
-  int64_t s = kPairs / p.tiles;
-  const int64_t most = p.depth / (parts > 1 ? 4 : 8);
-  if (s > most) s = most;
-  p.splits = q.splits = s < 2 ? 1 : (int)s;
-  const int64_t result = M * N * (mode == kDx ? 1 : 2);
-  q.part_bytes = p.splits > 1 ? up256((size_t)p.splits * result * sizeof(float)) : 0;
+  // The last round's tiles run in slices of the depth where they leave half of the SMs idle or more, of 8
+  // stages (fp32: 4, each of them six products) at least; behind whole rounds only where that saves more
+  // than the kernel that adds the slices takes (192 x 4096 -> 11008, 172 tiles of 128 columns: 51 and XX us).
+  const int last = p.tiles % kPairs;
+  const int64_t stages = parts > 1 ? 4 : 8;
+  int64_t s = last > 0 ? kPairs / last : 1;
+  if (s > p.depth / stages) s = p.depth / stages;
+  if (s < 1) s = 1;
+  const bool pays = p.tiles < kPairs || p.depth - p.depth / s >= 4 * stages;
+  p.splits = pays && mode != kGate ? (int)s : 1;
+  p.whole = p.splits > 1 ? p.tiles - last : p.tiles;
+  q.part_bytes = up256((size_t)p.splits * (p.tiles - p.whole) * 2 * kM * q.bn * sizeof(float));
   return q;
 }
 
 template <int MODE, int BN, int PARTS>
 int launch_tiles(const Plan& q, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t st) {
   if (!semx::allow_smem(gemm_kernel<MODE, BN, PARTS>, gemm_smem(BN))) return SEMX_ERR_LAUNCH;
-  const int works = q.p.tiles * q.p.splits;
+  const int works = works_of(q.p);
   gemm_kernel<MODE, BN, PARTS><<<2 * (works < kPairs ? works : kPairs), kGemmT, gemm_smem(BN), st>>>(a, b, q.p);
   return semx::check_launch("gated_linear gemm_kernel");
 }
 
 template <int MODE>
 int launch_gemm(const Plan& q, const Operand& A, const Operand& B, cudaStream_t st) {
+  // The driver's call wants a context of this thread, which a new thread (autograd's, say) has only after a
+  // call of the runtime.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+    return semx::fail(SEMX_ERR_DEVICE, "gated_linear: %s", cudaGetErrorString(cudaGetLastError()));
   CUtensorMap a, b;
   int rc = make_map(&a, A, MODE == kDw ? 64 : kM);
   if (rc != SEMX_OK) return rc;
-  rc = make_map(&b, B, MODE == kFwd ? q.bn / 2 : 64);
+  rc = make_map(&b, B, MODE == kFwd || MODE == kGate ? q.bn / 2 : 64);
   if (rc != SEMX_OK) return rc;
   if (A.parts > 1) {
-    rc = launch_tiles<MODE, 128, kParts>(q, a, b, st);
+    if constexpr (MODE != kGate) rc = launch_tiles<MODE, 128, kParts>(q, a, b, st);
+    else rc = semx::fail(SEMX_ERR_UNSUPPORTED, "gated_linear: fp32 keeps u and g");
   } else if (q.bn == 256) {
     rc = launch_tiles<MODE, 256, 1>(q, a, b, st);
   } else if (q.bn == 128) {
@@ -983,12 +1199,10 @@ int launch_gemm(const Plan& q, const Operand& A, const Operand& B, cudaStream_t 
     if constexpr (MODE == kFwd) rc = launch_tiles<MODE, 64, 1>(q, a, b, st);
     else rc = semx::fail(SEMX_ERR_UNSUPPORTED, "gated_linear: tile of %d", q.bn);
   }
-  if (rc != SEMX_OK || q.splits == 1) return rc;
-  const int64_t n = q.p.M * q.p.N * (MODE == kDw ? 2 : 1);
-  const unsigned grid = (unsigned)cdiv(n, (int64_t)256);
-  if (MODE == kFwd) join_gated_kernel<<<grid, 256, 0, st>>>(q.p);
-  else join_plain_kernel<<<grid, 256, 0, st>>>(q.p.part, q.splits, n, q.p.out, q.p.out_bf16);
-  return semx::check_launch("gated_linear join");
+  if (rc != SEMX_OK || q.p.whole == q.p.tiles || MODE == kGate) return rc;
+  const int64_t quads = (int64_t)(q.p.tiles - q.p.whole) * 2 * kM * (MODE == kFwd ? q.bn / 2 : q.bn) / 4;
+  if constexpr (MODE != kGate) join_kernel<MODE><<<(unsigned)cdiv(quads, (int64_t)256), 256, 0, st>>>(q.p, q.bn);
+  return semx::check_launch("gated_linear join_kernel");
 }
 
 int lay(const void* src, int64_t ld, int bf16, int64_t rows, int64_t cols, void* dst, int64_t ldp, int parts, cudaStream_t st) {
@@ -1013,7 +1227,7 @@ int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
   if (a->rows == 0 && !bwd) return SEMX_OK;
   SEMX_REQUIRE(a->w && (a->rows == 0 || a->x), SEMX_ERR_NULL, "gated_linear: x / w is NULL");
   if (!bwd) SEMX_REQUIRE(a->h, SEMX_ERR_NULL, "gated_linear: h is NULL");
-  else SEMX_REQUIRE(a->rows == 0 || (a->dh && a->saved), SEMX_ERR_NULL, "gated_linear bwd: dh / saved is NULL");
+  else SEMX_REQUIRE(a->rows == 0 || (a->dh && (makes_again(a) || a->saved)), SEMX_ERR_NULL, "gated_linear bwd: dh / saved is NULL");
   SEMX_REQUIRE(semx::all_aligned({a->x, a->w, a->h, a->dh, a->dx, a->dw}, a->bf16 ? 2 : 4) &&
                    semx::aligned(a->bias, a->bias_bf16 ? 2 : 4) && semx::aligned(a->db, 4) &&
                    semx::all_aligned({a->saved, a->workspace}, 16),
@@ -1024,19 +1238,31 @@ int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
 // Whether TMA reads rows of n bf16 at stride ld from base.
 bool in_place(const void* base, int64_t ld, int bf16) { return bf16 && ld % 8 == 0 && semx::aligned(base, 16); }
 
+template <int NT>
+int launch_few_bf16(const SemxGatedLinearArgs* a, const GemmParams& p, cudaStream_t st) {
+  few_rows_bf16_kernel<NT><<<(unsigned)cdiv(a->H, (int64_t)8), kFewWarps * 32, 0, st>>>(
+      reinterpret_cast<const __nv_bfloat16*>(a->x), a->ldx, reinterpret_cast<const __nv_bfloat16*>(a->w), a->D, a->H, (int)a->rows, p);
+  return semx::check_launch("gated_linear few_rows_bf16_kernel");
+}
+
 // Workspace of one call: parts of x, of W, of du | dg, sums of slices, column sums.
 struct Layout {
   int parts;
-  bool few, lay_x, lay_w;
+  bool few, few_bf16, lay_x, lay_w;
+  int64_t sum_rows;
   size_t x, w, dz, part, sums, total;
+  bool again;  // backward: u and g are made again
   Plan fwd, dx, dw;
 };
 
 Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
   Layout l = {};
   l.parts = a->bf16 ? 1 : kParts;
-  l.few = !bwd && a->rows <= kFew;
-  if (a->rows == 0 || l.few) return l;
+  // (Rows that the wide loads take.)
+  l.few_bf16 = !bwd && a->bf16 && a->rows <= kFewBf16 && a->D % 8 == 0 && (a->ldx % 8 == 0 || a->rows == 1) &&
+               semx::aligned(a->x, 16) && semx::aligned(a->w, 16);
+  l.few = !bwd && a->rows <= kFew && !l.few_bf16;
+  if (a->rows == 0 || l.few || l.few_bf16) return l;
   // Laid out anew wherever the sizes allow a misaligned base: the query has no addresses that count.
   l.lay_x = !in_place(a->x, a->ldx, a->bf16);
   l.lay_w = !in_place(a->w, a->D, a->bf16);
@@ -1047,7 +1273,8 @@ Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
     at += up256(bytes);
     return was;
   };
-  const bool need_x = !bwd || a->dw != nullptr, need_w = !bwd || a->dx != nullptr;
+  l.again = bwd && makes_again(a);
+  const bool need_x = !bwd || l.again || a->dw != nullptr, need_w = !bwd || l.again || a->dx != nullptr;
   l.x = take(l.lay_x && need_x ? (size_t)l.parts * a->rows * Dp * 2 : 0);
   l.w = take(l.lay_w && need_w ? (size_t)l.parts * 2 * a->H * Dp * 2 : 0);
   if (!bwd) {
@@ -1057,9 +1284,11 @@ Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
     l.dz = take((size_t)l.parts * 2 * a->rows * Hp * 2);
     l.dx = plan_gemm(kDx, a->rows, a->D, a->H, l.parts);
     l.dw = plan_gemm(kDw, a->H, a->D, a->rows, l.parts);
-    const size_t p1 = need_w ? l.dx.part_bytes : 0, p2 = need_x ? l.dw.part_bytes : 0;
+    if (l.again) l.fwd = plan_gemm(kGate, a->rows, a->H, a->D, l.parts);
+    const size_t p1 = a->dx != nullptr ? l.dx.part_bytes : 0, p2 = a->dw != nullptr ? l.dw.part_bytes : 0;
     l.part = take(p1 > p2 ? p1 : p2);
-    l.sums = take(a->db != nullptr ? (size_t)cdiv(a->rows, (int64_t)kDzRows) * 2 * a->H * sizeof(float) : 0);
+    l.sum_rows = l.again ? 8 * l.fwd.p.tiles_m : cdiv(a->rows, (int64_t)kDzRows);
+    l.sums = take(a->db != nullptr ? (size_t)l.sum_rows * 2 * a->H * sizeof(float) : 0);
   }
   l.total = at;
   return l;
@@ -1123,7 +1352,13 @@ extern "C" {
 size_t semx_gated_linear_args_size(void) { return sizeof(SemxGatedLinearArgs); }
 
 size_t semx_gated_linear_saved_bytes(const SemxGatedLinearArgs* a) {
-  return a == nullptr || a->rows < 0 || a->H < 0 ? 0 : (size_t)2 * a->rows * up8(a->H) * sizeof(float);
+  if (a == nullptr || a->rows < 0 || a->H < 0) return 0;
+  // Narrow bf16 rows: the backward makes u and g again in less time than it takes to write and read them
+  // (training passes, kept and made again: 129684 x 64 -> 256 254 and 233 us, 16384 x 512 -> 1408 234 and 223,
+  // 8192 x 1024 -> 2752 299 and 314). In fp32, six times the products and three parts to write, it does not
+  // (129684 x 64 -> 256 462 and 549).
+  if (makes_again(a)) return 0;
+  return (size_t)2 * a->rows * up8(a->H) * sizeof(float);
 }
 
 size_t semx_gated_linear_workspace_bytes(const SemxGatedLinearArgs* a, int32_t backward) {
@@ -1150,6 +1385,11 @@ int semx_gated_linear_fwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   q.p.bias = a->bias;
   q.p.bias_bf16 = a->bias_bf16;
   q.p.gelu = a->act;
+  if (l.few_bf16) {
+    const int tiles = (int)cdiv(a->rows, (int64_t)8);
+    if (tiles == 1) return launch_few_bf16<1>(a, q.p, st);
+    return launch_few_bf16<2>(a, q.p, st);
+  }
   if (l.few) {
     if (a->rows == 1) return launch_few<1>(a, q.p, st);
     if (a->rows == 2) return launch_few<2>(a, q.p, st);
@@ -1185,17 +1425,29 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   const Layout l = layout_of(a, true);
   SEMX_REQUIRE(a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_linear bwd: workspace is NULL");
   char* ws = reinterpret_cast<char*>(a->workspace);
-  const int64_t Hp = up8(a->H), blocks = cdiv(a->rows, (int64_t)kDzRows);
+  const int64_t Hp = up8(a->H);
   float* sums = a->db != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
   __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + l.dz);
-  const float *u = a->saved, *g = a->saved + a->rows * Hp;
-  const unsigned grid = (unsigned)(blocks * cdiv(a->H, (int64_t)256));
-  if (a->bf16) gate_grad_kernel<1><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
-  else gate_grad_kernel<kParts><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
-  rc = semx::check_launch("gated_linear gate_grad_kernel");
-  if (rc != SEMX_OK) return rc;
   Operand x, w;
-  rc = lay_operands(a, l, need_x, need_w, ws, st, &x, &w);
+  rc = lay_operands(a, l, need_x || l.again, need_w || l.again, ws, st, &x, &w);
+  if (rc != SEMX_OK) return rc;
+  if (l.again) {
+    Plan q = l.fwd;
+    q.p.dh = a->dh;
+    q.p.dz = dz;
+    q.p.ldz = Hp;
+    q.p.sums = sums;
+    q.p.bias = a->bias;
+    q.p.bias_bf16 = a->bias_bf16;
+    q.p.gelu = a->act;
+    rc = launch_gemm<kGate>(q, x, w, st);
+  } else {
+    const float *u = a->saved, *g = a->saved + a->rows * Hp;
+    const unsigned grid = (unsigned)(cdiv(a->rows, (int64_t)kDzRows) * cdiv(a->H, (int64_t)256));
+    if (a->bf16) gate_grad_kernel<1><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
+    else gate_grad_kernel<kParts><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
+    rc = semx::check_launch("gated_linear gate_grad_kernel");
+  }
   if (rc != SEMX_OK) return rc;
   const Operand d = {dz, a->H, a->rows, 2, l.parts, Hp, a->rows * Hp, 2 * a->rows * Hp};
   if (need_w) {
@@ -1221,7 +1473,7 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   seg.n = 1;
   seg.out[0] = a->db;
   seg.len[0] = 2 * a->H;
-  return semx::colsum_once(sums, blocks, 2 * a->H, seg, st);
+  return semx::colsum_once(sums, l.sum_rows, 2 * a->H, seg, st);
 }
 
 }  // extern "C"

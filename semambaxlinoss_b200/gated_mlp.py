@@ -43,7 +43,8 @@ def _forward(x, weight, bias, act, keep):
     """(h, u and g in front of the activation where ``keep``)."""
     a = _args(x, weight, bias, act)
     h = x.new_empty((a.rows, a.H))
-    saved = _lib.scratch(_lib.load().semx_gated_linear_saved_bytes(a), x) if keep else None
+    nbytes = _lib.load().semx_gated_linear_saved_bytes(a) if keep else 0
+    saved = _lib.scratch(nbytes, x) if nbytes else None
     a.h, a.saved = h.data_ptr(), _lib.ptr(saved)
     ws = _workspace(a, 0, x)
     _lib.call("semx_gated_linear_fwd", a, x.device)
@@ -54,23 +55,24 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act):
         w = weight.contiguous()
-        h, saved = _forward(x, w, None if bias is None else bias.contiguous(), act, True)
-        ctx.save_for_backward(x, w, saved)
+        b = None if bias is None else bias.contiguous()
+        h, saved = _forward(x, w, b, act, True)
+        ctx.save_for_backward(x, w, b, saved)
         ctx.cfg = (act, None if bias is None else bias.dtype)
         return h
 
     @staticmethod
     @_lib.once_differentiable
     def backward(ctx, dh):
-        x, weight, saved = ctx.saved_tensors
+        x, weight, bias, saved = ctx.saved_tensors
         act, bias_t = ctx.cfg
         need = ctx.needs_input_grad
-        a = _args(x, weight, None, act)
+        a = _args(x, weight, bias, act)
         dh = _lib.as_rows(dh, x.dtype)
         dx = x.new_empty(x.shape) if need[0] else None
         dw = torch.empty_like(weight) if need[1] else None
         db = weight.new_empty(weight.shape[0], dtype=torch.float32) if bias_t is not None and need[2] else None
-        a.saved, a.dh, a.dx, a.dw, a.db = saved.data_ptr(), dh.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db)
+        a.saved, a.dh, a.dx, a.dw, a.db = _lib.ptr(saved), dh.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db)
         ws = _workspace(a, 1, x)
         _lib.call("semx_gated_linear_bwd", a, x.device)
         return dx, dw, _lib.cast(db, bias_t), None
@@ -84,7 +86,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     x and weight are of one type, bf16 or fp32; bf16 autocast casts both. activation: "silu" or "gelu"
     (with the normal distribution). Sums are fp32; fp32 operands keep fp32's precision (an infinity
     among them gives NaN). With gradients wanted the forward keeps u and g in fp32 (8 bytes per element
-    of h)."""
+    of h); in bf16 with x of up to 512 features the backward makes them again instead."""
     op = "gated_linear"
     if not x.is_cuda:
         raise RuntimeError(f"{op} requires CUDA tensors.")

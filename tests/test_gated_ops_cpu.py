@@ -103,8 +103,10 @@ def test_projection_arguments_are_checked_on_the_host():
     assert status("semx_gated_linear_bwd") == _lib.SEMX_ERR_NULL
     assert status(rows=0) == _lib.SEMX_OK
     a = _lib.new_args(_lib.SemxGatedLinearArgs)
-    a.rows, a.D, a.H = 5, 16, 9
+    a.rows, a.D, a.H = 5, 1000, 9
     assert lib.semx_gated_linear_saved_bytes(ctypes.byref(a)) == 2 * 5 * 16 * 4
+    a.D, a.bf16 = 16, 1  # narrow: made again
+    assert lib.semx_gated_linear_saved_bytes(ctypes.byref(a)) == 0
 
 
 def test_factory_and_module():
