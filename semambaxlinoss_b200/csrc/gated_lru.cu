@@ -97,7 +97,7 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
 
 // With m = -la in [0, 0.125] (Chebyshev interpolants of degree 3 in m, at most 2.6e-8 off; fewer
 // coefficients matter because a pair of equal constants takes two instructions to make):
-//   exp(-m), sqrt((1 - exp(-2 m)) / (2 m)), and the latter's inverse.
+//   exp(-m) and sqrt((1 - exp(-2 m)) / (2 m)).
 __device__ __forceinline__ f2 horner3(f2 m, float c0, float c1, float c2, float c3) {
   f2 v = fma2(both(c3), m, both(c2));
   v = fma2(v, m, both(c1));
@@ -109,15 +109,10 @@ __device__ __forceinline__ f2 decay_near(f2 m) {
 __device__ __forceinline__ f2 root_near(f2 m) {
   return horner3(m, 1.0f, -0.49999356269836426f, 0.20807549357414246f, -0.05916960909962654f);
 }
-__device__ __forceinline__ f2 inverse_root_near(f2 m) {
-  return horner3(m, 1.0f, 0.49999943375587463f, 0.04168989136815071f, -0.021152695640921593f);
-}
-
 // What a channel's rates come to, one float per channel of the tile.
 struct Rates {
-  float speed[kCh];  // rate_scale softplus(rate)
+  float speed[kCh], minus[kCh];  // rate_scale softplus(rate), and its negative
   float root[kCh];   // sqrt(2 speed)
-  float inverse[kCh];
   float slope[kCh];  // d speed / d rate
   float r2[kCh], i2[kCh];  // biases, times -log2(e)
 };
@@ -128,9 +123,8 @@ __device__ __forceinline__ void load_rates(const GlParams& p, int c0, int lane, 
   to->slope[lane] = p.scale * softplus_slope(rate, e);
   s = s > 1e37f ? 1e37f : s;  // an infinite one times a closed gate is no number
   to->speed[lane] = s;
-  const float inverse = semx::rsqrt_approx(2.f * s);
-  to->inverse[lane] = inverse;
-  to->root[lane] = s > 0.f ? 2.f * s * inverse : 2.f * s;
+  to->minus[lane] = -s;
+  to->root[lane] = s > 0.f ? 2.f * s * semx::rsqrt_approx(2.f * s) : 2.f * s;
   to->r2[lane] = p.r_bias != nullptr ? -kLog2e * p.r_bias[c] : 0.f;
   to->i2[lane] = p.i_bias != nullptr ? -kLog2e * p.i_bias[c] : 0.f;
 }
@@ -180,10 +174,12 @@ __device__ __forceinline__ f2 least2(f2 gain) {
   const float2 g = unpack2(gain);
   return pack2(fmaxf(g.x, kLeastGain), fmaxf(g.y, kLeastGain));
 }
-// Far up the exponential of a closed gate ends, so that its product with what it closes is 1.
+// Far up the exponential of a closed gate ends, so that its product with what it closes is 1. (A NaN stays.)
 __device__ __forceinline__ f2 end2(f2 v) {
-  const float2 t = unpack2(v);
-  return pack2(t.x > 126.f ? 126.f : t.x, t.y > 126.f ? 126.f : t.y);
+  float2 t = unpack2(v);
+  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.x));  // 126
+  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.y));
+  return pack2(t.x, t.y);
 }
 __device__ __forceinline__ f2 gate_arg(f2 v, f2 bias) { return fma2(v, both(-kLog2e), bias); }
 
@@ -407,10 +403,16 @@ __device__ __forceinline__ void bring(const GlParams& p, const Place& at, const 
   }
 }
 
-// Decay a and input b = gain iota x of the thread's steps.
+// The exponentials exp(-(r + r_bias)) and exp(-(i + i_bias)) of a thread's steps, which the backward takes twice.
+template <int SEG>
+struct Exps {
+  float4 r[SEG][kT], i[SEG][kT];
+};
+
+// Decay a and input b = gain iota x of the thread's steps; the exponentials into `exps` where it is given.
 template <int ACC, int SEG, bool SLOW, int OPS>
 __device__ __forceinline__ void gate_steps(const GlParams& p, const Rates& rt, int lc, const Stage<ACC, SEG, OPS>& st, f2 (&a)[SEG][2],
-                                           f2 (&b)[SEG][2]) {
+                                           f2 (&b)[SEG][2], Exps<SEG>* exps) {
   const int tid = threadIdx.x;
 #pragma unroll
   for (int u = 0; u < SEG; ++u) {
@@ -418,10 +420,16 @@ __device__ __forceinline__ void gate_steps(const GlParams& p, const Rates& rt, i
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = lc + 2 * h;
-      const f2 er = ex2_2(gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, c)));
+      const f2 ar = gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, c));
+      const f2 ai = gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, c));
+      const f2 er = ex2_2(exps != nullptr ? end2(ar) : ar), ei = ex2_2(exps != nullptr ? end2(ai) : ai);
       f2 rho, m, gain;
       decay2<SLOW>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, c), shared_pair(rt.root, c), &rho, &m, &a[u][h], &gain);
-      const f2 iota = rcp_2(add2(ex2_2(gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, c))), both(1.f)));
+      const f2 iota = rcp_2(add2(ei, both(1.f)));
+      if (exps != nullptr) {
+        reinterpret_cast<f2*>(&exps->r[u][tid])[h] = er;
+        reinterpret_cast<f2*>(&exps->i[u][tid])[h] = ei;
+      }
       b[u][h] = mul2(mul2(iota, pair_of<ACC>(rx, h, p.bf16)), least2(gain));
     }
   }
@@ -475,8 +483,8 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
     copies_done();
     const int most = w.n - at.seg * SEG;  // steps of the thread that exist
     if (warp * (kSegs / 4) * SEG < w.n) {
-      if (slow) gate_steps<ACC, SEG, true>(p, rt, at.lc, st, a, b);
-      else gate_steps<ACC, SEG, false>(p, rt, at.lc, st, a, b);
+      if (slow) gate_steps<ACC, SEG, true>(p, rt, at.lc, st, a, b, static_cast<Exps<SEG>*>(nullptr));
+      else gate_steps<ACC, SEG, false>(p, rt, at.lc, st, a, b, static_cast<Exps<SEG>*>(nullptr));
       if (gated) {
 #pragma unroll
         for (int u = 0; u < SEG; ++u) rz[u] = st.v[3][u][tid];
@@ -574,8 +582,8 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
 // gradients that reach h from y; gs: what reaches the last step from behind; sums over the steps of
 // rho dla, dr and di are added to `sum`.
 template <int ACC, int SEG, bool SLOW>
-__device__ __forceinline__ void gradient_steps(const GlParams& p, const Rates& rt, const Place& at, const Stage<ACC, SEG, 5>& st, int most,
-                                               int row0, const f2 (&a)[SEG][2], const f2 (&b)[SEG][2], const f2 (&d)[SEG][2],
+__device__ __forceinline__ void gradient_steps(const GlParams& p, const Rates& rt, const Place& at, const Stage<ACC, SEG, 5>& st,
+                                               const Exps<SEG>& exps, int most, int row0, const f2 (&a)[SEG][2], const f2 (&b)[SEG][2], const f2 (&d)[SEG][2],
                                                f2 (&gs)[2], f2 (&sum)[3][2]) {
   typedef typename RawQuad<ACC>::type Raw;
   const int tid = threadIdx.x;
@@ -585,31 +593,22 @@ __device__ __forceinline__ void gradient_steps(const GlParams& p, const Rates& r
 #pragma unroll
   for (int u = SEG - 1; u >= 0; --u) {
     if (u >= most) continue;
-    const Raw rx = st.v[0][u][tid], rr = st.v[1][u][tid], ri = st.v[2][u][tid], rg = st.v[4][u][tid];
+    const Raw rx = st.v[0][u][tid], rg = st.v[4][u][tid];
+    const f2* er_of = reinterpret_cast<const f2*>(&exps.r[u][tid]);
+    const f2* ei_of = reinterpret_cast<const f2*>(&exps.i[u][tid]);
     f2 dx[2], dr[2], di[2], dz[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int c = at.lc + 2 * k;
       const f2 x = pair_of<ACC>(rx, k, p.bf16), speed = shared_pair(rt.speed, c);
       const f2 gt = add2(d[u][k], gs[k]);
-      const f2 er = ex2_2(end2(gate_arg(pair_of<ACC>(rr, k, p.bf16), shared_pair(rt.r2, c))));
-      const f2 er1 = add2(er, both(1.f)), qr = rsqrt_2(er1);
+      const f2 er = er_of[k], ei = ei_of[k];
       f2 rho, m, same, gain;
-      decay2<SLOW>(qr, speed, shared_pair(rt.root, c), &rho, &m, &same, &gain);
-      // 1 / gain: 1 / q = (1 + er) q.
-      f2 inv = mul2(mul2(mul2(er1, qr), shared_pair(rt.inverse, c)), inverse_root_near(m));
+      decay2<SLOW>(rsqrt_2(add2(er, both(1.f))), speed, shared_pair(rt.root, c), &rho, &m, &same, &gain);
       const float2 gg = unpack2(gain);
-      float2 iv = unpack2(inv);
-      if constexpr (!SLOW) {
-        const float2 mm = unpack2(m);
-        if (mm.x > kNear) iv.x = 1.f / gg.x;
-        if (mm.y > kNear) iv.y = 1.f / gg.y;
-      }
-      iv.x = gg.x > kLeastGain ? iv.x : 0.f;  // at its least value no gradient goes through the gain
-      iv.y = gg.y > kLeastGain ? iv.y : 0.f;
-      inv = pack2(iv.x, iv.y);
+      // -1 / gain; at its least value no gradient goes through the gain
+      const f2 inv = pack2(gg.x > kLeastGain ? semx::rcp_approx(-gg.x) : 0.f, gg.y > kLeastGain ? semx::rcp_approx(-gg.y) : 0.f);
       gain = least2(gain);
-      const f2 ei = ex2_2(end2(gate_arg(pair_of<ACC>(ri, k, p.bf16), shared_pair(rt.i2, c))));
       const f2 iota = rcp_2(add2(ei, both(1.f)));
       const f2 ah = mul2(a[u][k], b[u][k]);
       if (gated) {
@@ -622,10 +621,9 @@ __device__ __forceinline__ void gradient_steps(const GlParams& p, const Rates& r
       const f2 gi = mul2(gt, iota);
       dx[k] = mul2(gi, gain);
       di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
-      const f2 through = mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv));
-      const f2 dla = fma2(gt, ah, mul2(through, both(-1.f)));
+      const f2 dla = fma2(gt, ah, mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv)));
       const f2 rd = mul2(rho, dla);
-      dr[k] = mul2(mul2(rd, mul2(er, rho)), mul2(speed, both(-1.f)));
+      dr[k] = mul2(mul2(rd, mul2(er, rho)), shared_pair(rt.minus, c));
       gs[k] = mul2(a[u][k], gt);
       sum[0][k] = add2(sum[0][k], rd);
       sum[1][k] = add2(sum[1][k], dr[k]);
@@ -702,14 +700,17 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
     if (LINK && tid == 0) drawn = atomicAdd(&p.ticket[at.ct], 1);
     const float entry = warp == 0 && w.live && ok ? p.ckpt[(int64_t)w.unit * p.C + c] : 0.f;
     const Stage<ACC, SEG, 5>& st = stages[buf];
+    // Wide rows' exponentials take the places of the gates that they are made of.
+    static_assert(ACC == kBf16 || sizeof(Exps<SEG>) == 2 * sizeof(st.v[0]), "places");
+    Exps<SEG>& exps = *reinterpret_cast<Exps<SEG>*>(ACC == kBf16 ? raw + 2 * sizeof(Stage<ACC, SEG, 5>) : reinterpret_cast<unsigned char*>(stages[buf].v[1]));
     float(*mA)[kCh] = maps[buf][0], (*mB)[kCh] = maps[buf][1], (*mG)[kCh] = maps[buf][2];
     // b: gain iota x, later the state in front of the step; d: the gradient that reaches h from y.
     f2 a[SEG][2], b[SEG][2], d[SEG][2];
     f2 A[2] = {both(1.f), both(1.f)}, B[2] = {both(0.f), both(0.f)}, G[2] = {both(0.f), both(0.f)};
     copies_done();
     if (busy) {
-      if (slow) gate_steps<ACC, SEG, true>(p, rt, at.lc, st, a, b);
-      else gate_steps<ACC, SEG, false>(p, rt, at.lc, st, a, b);
+      if (slow) gate_steps<ACC, SEG, true>(p, rt, at.lc, st, a, b, &exps);
+      else gate_steps<ACC, SEG, false>(p, rt, at.lc, st, a, b, &exps);
 #pragma unroll
       for (int u = 0; u < SEG; ++u) {
         const Raw rg = st.v[4][u][tid];
@@ -802,8 +803,8 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
           hs[k] = after;
         }
       f2 gs[2] = {shared_pair(mG[at.seg], at.lc), shared_pair(mG[at.seg], at.lc + 2)};
-      if (slow) gradient_steps<ACC, SEG, true>(p, rt, at, st, most, w.row, a, b, d, gs, sum);
-      else gradient_steps<ACC, SEG, false>(p, rt, at, st, most, w.row, a, b, d, gs, sum);
+      if (slow) gradient_steps<ACC, SEG, true>(p, rt, at, st, exps, most, w.row, a, b, d, gs, sum);
+      else gradient_steps<ACC, SEG, false>(p, rt, at, st, exps, most, w.row, a, b, d, gs, sum);
     }
     if (p.part != nullptr && (LINK || w.k == 0)) {
       // The four segments of the warp, then (behind the next barrier) the warps.
@@ -983,7 +984,7 @@ int launch_gl(bool bwd, const GlParams& p, cudaStream_t st) {
     KERNEL<<<n, kT, STAGES, st>>>(p);                                \
     return semx::check_launch("gated_lru kernel");                   \
   } while (0)
-  constexpr size_t fwd = sizeof(Stage<ACC, kFwdSeg, 4>), back = 2 * sizeof(Stage<ACC, kBwdSeg, 5>);
+  constexpr size_t fwd = sizeof(Stage<ACC, kFwdSeg, 4>), back = 2 * sizeof(Stage<ACC, kBwdSeg, 5>) + (ACC == kBf16 ? sizeof(Exps<kBwdSeg>) : 0);
   if (!bwd && linked) SEMX_GL((gated_lru_fwd_kernel<ACC, kFwdSeg, true>), fwd);
   if (!bwd) SEMX_GL((gated_lru_fwd_kernel<ACC, kFwdSeg, false>), fwd);
   if (linked) SEMX_GL((gated_lru_bwd_kernel<ACC, kBwdSeg, true>), back);
