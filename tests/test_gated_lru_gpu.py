@@ -308,6 +308,78 @@ def test_bad_offsets_stay_inside():
     torch.cuda.synchronize()
 
 
+def test_refusals():
+    from semambaxlinoss_b200.gated_lru import gated_lru_scan, gated_lru_step
+
+    C = 8
+    x, rate = torch.zeros(2, 5, C, device=cuda()), torch.zeros(C, device=cuda())
+    state = torch.zeros(3, C, device=cuda())
+    slots, fresh = torch.zeros(2, dtype=torch.int32, device=cuda()), torch.zeros(2, dtype=torch.bool, device=cuda())
+    good = dict(x=x, r=x, i=x, rate=rate, z=x, r_bias=rate, i_bias=rate, state=state, slots=slots, fresh=fresh)
+    gated_lru_scan(**good)
+    for bad, what in ((dict(r=x[:, :4]), "r must"), (dict(i=x.to(torch.bfloat16)), "i must"), (dict(z=x.cpu()), "z must"),
+                      (dict(rate=rate[:7]), "rate must"), (dict(rate=rate.double()), "rate must"),
+                      (dict(r_bias=rate[:3]), "r_bias"), (dict(i_bias=rate.cpu()), "i_bias"), (dict(x=x.double()), "dtype"),
+                      (dict(rate_scale=0.0), "rate_scale"), (dict(rate_scale=float("inf")), "rate_scale"),
+                      (dict(state=state[:, :4]), "state"), (dict(state=state.to(torch.bfloat16)), "state"),
+                      (dict(state=state[:0]), "no entries"), (dict(state=state[:1], slots=None), "entries"),
+                      (dict(slots=slots.long()), "slots"), (dict(fresh=slots), "fresh"), (dict(state=None), "without a state"),
+                      (dict(rate=rate.clone().requires_grad_()), "inference"), (dict(x=x[0]), "batch"),
+                      (dict(cu_seqlens=slots), "packed"), (dict(x=x[0], cu_seqlens=slots.long()), "cu_seqlens")):
+        with pytest.raises(ValueError, match=what):
+            gated_lru_scan(**dict(good, **bad))
+    row = x[:, 0].contiguous()
+    step = dict(x=row, r=row, i=row, rate=rate, state=state, z=row, slots=slots)
+    gated_lru_step(**step)
+    for bad, what in ((dict(x=x), "sequences, channels"), (dict(state=None), "needed"), (dict(r=row[:1]), "r must"),
+                      (dict(z=row.clone().requires_grad_()), "inference"), (dict(state=state[:, :7]), "state")):
+        with pytest.raises(ValueError, match=what):
+            gated_lru_step(**dict(step, **bad))
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        gated_lru_scan(fwad.make_dual(x, torch.ones_like(x)), x, x, rate)
+
+
+def test_broadcast_operands():
+    """Expanded gates and rates: gradients are summed over what they were expanded along."""
+    from semambaxlinoss_b200.gated_lru import gated_lru_scan
+
+    g = gen(17)
+    S, L, C = 3, 70, 24
+    x, dy = (randn((S, L, C), g).float().to(cuda()) for _ in range(2))
+    r, i = randn((1, L, C), g).float().to(cuda()).requires_grad_(), randn((S, 1, C), g).float().to(cuda()).requires_grad_()
+    rate = torch.full((1,), -4.0, device=cuda(), requires_grad=True)
+    got = torch.autograd.grad(gated_lru_scan(x, r.expand(S, L, C), i.expand(S, L, C), rate.expand(C)), (r, i, rate), dy)
+    full = [t.detach().expand(n).contiguous().requires_grad_() for t, n in ((r, (S, L, C)), (i, (S, L, C)), (rate, (C,)))]
+    want = torch.autograd.grad(gated_lru_scan(x, *full), full, dy)
+    assert torch.allclose(got[0], want[0].sum(0, keepdim=True), rtol=1e-5, atol=1e-6)
+    assert torch.allclose(got[1], want[1].sum(1, keepdim=True), rtol=1e-5, atol=1e-6)
+    assert torch.allclose(got[2], want[2].sum(0, keepdim=True), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("C", [8, 24000])
+def test_few_and_many_channel_tiles(C):
+    """One channel tile that all CTAs share, and more of them than CTAs run at once: forward, state and
+    gradients of packed sequences against the walked form of the same rows."""
+    from semambaxlinoss_b200.gated_lru import gated_lru_scan
+
+    g = torch.Generator(device="cuda").manual_seed(C)
+    S, L = (2, 3000) if C == 8 else (3, 100)
+    x, r, i, z, dy = (torch.randn(S, L, C, generator=g, device="cuda") for _ in range(5))
+    rate = torch.rand(C, generator=g, device="cuda") * 4 - 8
+    cu = torch.arange(S + 1, dtype=torch.int32, device="cuda") * L
+
+    def run(packed):
+        f = (lambda t: t.reshape(S * L, C)) if packed else (lambda t: t)
+        v = [f(t).clone().requires_grad_() for t in (x, r, i, z)] + [rate.clone().requires_grad_()]
+        y = gated_lru_scan(v[0], v[1], v[2], v[4], z=v[3], cu_seqlens=cu if packed else None)
+        return [t.reshape(S, L, C) if t.dim() > 1 else t for t in (y,) + torch.autograd.grad(y, v, f(dy))]
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-4 * float(b.abs().max()))
+
+
 def test_empty_batches():
     from semambaxlinoss_b200.gated_lru import gated_lru_scan, gated_lru_step
 

@@ -25,7 +25,7 @@ EPS = 2.0 ** -24
 HALF = {torch.float32: EPS, torch.bfloat16: 2.0 ** -8}
 SHAPES = [(1, 8, 1), (2, 64, 32), (3, 100, 7), (8, 2100, 33), (9, 64, 32), (33, 40, 24), (130, 72, 136), (129, 65, 33),
           (300, 257, 130), (1000, 64, 256), (257, 520, 264), (64, 2048, 40), (5000, 32, 16), (128, 64, 64),
-          (1, 4096, 300), (5, 2056, 1030)]
+          (1, 4096, 300), (5, 2056, 1030), (16, 136, 77), (17, 1000, 90)]
 
 
 def _n(K, dtype):
@@ -88,6 +88,25 @@ def test_training(rows, D, H, dtype, act, bias):
     want = ogm.gated(x.double(), w.double(), b.double() if bias else None, act, dh.double())
     assert all(g.dtype == dtype and g.shape == t.shape for g, t in zip(grads, ins))
     _check(dict(zip(("h", "dx", "dw", "db"), (h,) + grads)), want, rows, D, H, dtype)
+
+
+# Sizes whose oracle runs on the GPU, in 64 bits: tiles of every width, and a last round of tiles that runs in
+# slices of the depth behind whole rounds, in each of the products.
+@pytest.mark.parametrize("rows,D,H", [(600, 2112, 3300), (192, 512, 9472), (2600, 1700, 2000), (3000, 260, 2500),
+                                      (4099, 640, 1000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_tiles(rows, D, H, dtype):
+    from semambaxlinoss_b200.gated_mlp import gated_linear
+
+    x, w, b, dh = (t.to(cuda()) for t in _operands(rows, D, H, dtype, rows + D))
+    ins = [t.requires_grad_() for t in (x, w, b)]
+    h = gated_linear(*ins)
+    grads = torch.autograd.grad(h, ins, dh)
+    want = ogm.gated(x.detach().double(), w.detach().double(), b.detach().double(), "silu", dh.double())
+    want = {k: tuple(t.cpu() for t in v) for k, v in want.items()}
+    _check(dict(zip(("h", "dx", "dw", "db"), (h,) + grads)), want, rows, D, H, dtype)
+    with torch.no_grad():
+        assert torch.equal(gated_linear(x, w, b), h)
 
 
 @pytest.mark.parametrize("wants", [(0,), (1,), (2,), (0, 2), (1, 2), (0, 1)])
@@ -238,6 +257,29 @@ def test_autocast():
     assert torch.equal(h, plain)
     for g, q in zip(grads, want):
         assert g.dtype == torch.float32 and torch.equal(g, q.float())
+
+
+def test_refusals():
+    from semambaxlinoss_b200.gated_mlp import gated_linear
+
+    x, w, b = torch.zeros(4, 16, device=cuda()), torch.zeros(12, 16, device=cuda()), torch.zeros(12, device=cuda())
+    for bad, what in ((dict(weight=w[:11]), "weight"), (dict(weight=w[:, :15]), "weight"), (dict(weight=w[0]), "weight"),
+                      (dict(weight=w.to(torch.bfloat16)), "weight"), (dict(weight=w.cpu()), "weight"),
+                      (dict(bias=b[:6]), "bias"), (dict(bias=b.double()), "bias"), (dict(bias=b.cpu()), "bias"),
+                      (dict(activation="relu"), "activation"), (dict(x=x.double()), "dtype"), (dict(x=x.half()), "dtype"),
+                      (dict(x=x[:, :0], weight=w[:, :0]), "features")):
+        with pytest.raises(ValueError, match=what):
+            gated_linear(**dict(dict(x=x, weight=w, bias=b), **bad))
+    with torch.autocast("cuda", dtype=torch.float16), pytest.raises(ValueError, match="dtype"):
+        gated_linear(x, w, b)
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        gated_linear(fwad.make_dual(x, torch.ones_like(x)), w, b)
+    xr = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(gated_linear(xr, w, b).sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), xr)
 
 
 def test_no_wait_gave_up():
