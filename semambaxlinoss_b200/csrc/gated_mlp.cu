@@ -897,15 +897,19 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 4 : 3) gate_grad_kernel(cons
 
 // Up to R rows of x. A warp has two columns (four rows of W); x lies in shared memory in fp32, kDepth
 // values of each row at a time. Its lanes take 8 neighbouring weights of every 256.
-constexpr int kDepth = 2048, kFewT = 256, kFew = 8, kFewBf16 = 16;
+constexpr int kDepth = 2048, kFewT = 256, kFewBf16 = 16;
+// Rows of fp32 that run so, eight at a time (16 x 2048 -> 5504: 67 us, tiles and the parts of W 89); of bf16 that
+// the kernel below does not take.
+constexpr int kFew = 8, kFewFp32 = 16;
 // Place of value k in a row in shared memory: of every 256, the first halves of the lanes' eights, then
 // the second ones, so that lanes side by side read side by side.
 __device__ __forceinline__ int spread(int k) { return (k & ~255) | (k & 4) << 5 | (k & 248) >> 1 | (k & 3); }
 template <int R, bool BF16, bool VEC>
-__global__ void __launch_bounds__(kFewT) few_rows_kernel(const void* x, int64_t ldx, const void* w, int64_t D, int64_t H, int rows,
+__global__ void __launch_bounds__(kFewT, R > 4 ? 2 : 3) few_rows_kernel(const void* x, int64_t ldx, const void* w, int64_t D, int64_t H, int rows,
                                                          const GemmParams p) {
-  extern __shared__ float xs[];
+  extern __shared__ __align__(16) float xs[];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const bool wide = ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & (BF16 ? 7 : 15)) == 0;
   const int64_t h0 = ((int64_t)blockIdx.x * (kFewT / 32) + warp) * 2;
   semx_scan::f2 acc[4][R];
 #pragma unroll
@@ -918,13 +922,23 @@ __global__ void __launch_bounds__(kFewT) few_rows_kernel(const void* x, int64_t 
   for (int64_t d0 = 0; d0 < D; d0 += kDepth) {
     const int n = (int)min((int64_t)kDepth, D - d0), n8 = (n + 7) / 8 * 8;
     if (d0 > 0) __syncthreads();
-    for (int i = tid; i < R * n8; i += kFewT) {
-      const int r = i / n8, k = i % n8;
-      xs[r * kDepth + spread(k)] = r < rows && k < n ? semx_scan::load(x, r * ldx + d0 + k, BF16) : 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t from = min(r, rows - 1) * ldx + d0;  // (rows that do not exist: the last one, and not written)
+      for (int k = tid * 4; k < n8; k += kFewT * 4) {
+        float4 v;
+        if (k + 4 <= n && wide) {
+          v = BF16 ? semx_scan::quad_floats<semx_scan::kBf16>(semx_scan::load_quad<semx_scan::kBf16>(x, from + k, 1, 4), 1)
+                   : semx_scan::quad_floats<semx_scan::kFp32>(semx_scan::load_quad<semx_scan::kFp32>(x, from + k, 0, 4), 0);
+        } else {
+          v = semx_scan::quad_floats<semx_scan::kAny>(semx_scan::load_quad<semx_scan::kAny>(x, from + k, BF16, n - k), BF16);
+        }
+        *reinterpret_cast<float4*>(&xs[r * kDepth + spread(k)]) = v;
+      }
     }
     __syncthreads();
     if (h0 < H)
-#pragma unroll 2
+#pragma unroll 1
       for (int k = lane * 8; k < n; k += 256) {
         semx_scan::f2 wv[4][4];
 #pragma unroll
@@ -994,17 +1008,20 @@ __global__ void __launch_bounds__(kFewT) few_rows_kernel(const void* x, int64_t 
 // bf16 rows, up to 8 NT of them: products of 16 rows of W (eight of u, the same eight of g) by 16 of the depth
 // by 8 rows of x. The depth may be taken in any order, so a lane's eight neighbouring weights (16 bytes) are
 // its values of two products, and nothing of W passes through shared memory: each warp streams its rows.
-// (tcgen05 would have tiles of 128 rows of x, nearly all of them empty.) Four warps share the depth of
+// (tcgen05 would have tiles of 128 rows of x, nearly all of them empty.) Some warps share the depth of
 // eight columns; their sums meet in shared memory.
-constexpr int kFewWarps = 4;
+// Warps that share the depth (8 rows of 4096 -> 11008, four and eight: 31.8 and 30.7 us, 1 of 2048 -> 5504 11.6
+// and 9.3; 16 rows 45.5 and 42.9, but 2048 -> 5504 11.8 and 15.6).
+constexpr int few_warps(int nt) { return nt == 1 ? 8 : 4; }
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <int NT>
-__global__ void __launch_bounds__(kFewWarps * 32) few_rows_bf16_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, int64_t D,
+__global__ void __launch_bounds__(few_warps(NT) * 32) few_rows_bf16_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* w, int64_t D,
                                                                        int64_t H, int rows, const GemmParams p) {
+  constexpr int kFewWarps = few_warps(NT);
   __shared__ float sums[kFewWarps][NT * 8][17];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, q = lane / 4, t = lane % 4;
   const int64_t h0 = (int64_t)blockIdx.x * 8;
@@ -1018,8 +1035,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) few_rows_bf16_kernel(const __n
 #pragma unroll
   for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
   // D is a multiple of 8: a lane's eight values exist or do not.
-  constexpr int AHEAD = NT > 1 ? 4 : 8;
-  const int blocks = (int)((D + 31) / 32);  // of 32 of the depth; warp k has every fourth run of AHEAD
+  constexpr int AHEAD = 4;
+  const int blocks = (int)((D + 31) / 32);  // of 32 of the depth; warp k has every kFewWarps-th run of AHEAD
   for (int b0 = warp * AHEAD; b0 < blocks; b0 += kFewWarps * AHEAD) {
     uint4 u[AHEAD], g[AHEAD], v[AHEAD][NT];
 #pragma unroll
@@ -1169,8 +1186,14 @@ Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
 }
 
 template <int MODE, int BN, int PARTS>
-int launch_tiles(const Plan& q, const CUtensorMap& a, const CUtensorMap& b, cudaStream_t st) {
-  if (!semx::allow_smem(gemm_kernel<MODE, BN, PARTS>, gemm_smem(BN))) return SEMX_ERR_LAUNCH;
+int launch_tiles(const Plan& q, const CUtensorMap& a, const CUtensorMap& b, int dev, cudaStream_t st) {
+  // The limit stays with the kernel on a device: raised once (a bit for each of 64 devices).
+  static std::atomic<uint64_t> raised{0};
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if ((raised.load(std::memory_order_relaxed) & bit) == 0) {
+    if (!semx::allow_smem(gemm_kernel<MODE, BN, PARTS>, gemm_smem(BN))) return SEMX_ERR_LAUNCH;
+    raised.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int works = works_of(q.p);
   gemm_kernel<MODE, BN, PARTS><<<2 * (works < kPairs ? works : kPairs), kGemmT, gemm_smem(BN), st>>>(a, b, q.p);
   return semx::check_launch("gated_linear gemm_kernel");
@@ -1189,14 +1212,14 @@ int launch_gemm(const Plan& q, const Operand& A, const Operand& B, cudaStream_t 
   rc = make_map(&b, B, MODE == kFwd || MODE == kGate ? q.bn / 2 : 64);
   if (rc != SEMX_OK) return rc;
   if (A.parts > 1) {
-    if constexpr (MODE != kGate) rc = launch_tiles<MODE, 128, kParts>(q, a, b, st);
+    if constexpr (MODE != kGate) rc = launch_tiles<MODE, 128, kParts>(q, a, b, dev, st);
     else rc = semx::fail(SEMX_ERR_UNSUPPORTED, "gated_linear: fp32 keeps u and g");
   } else if (q.bn == 256) {
-    rc = launch_tiles<MODE, 256, 1>(q, a, b, st);
+    rc = launch_tiles<MODE, 256, 1>(q, a, b, dev, st);
   } else if (q.bn == 128) {
-    rc = launch_tiles<MODE, 128, 1>(q, a, b, st);
+    rc = launch_tiles<MODE, 128, 1>(q, a, b, dev, st);
   } else {
-    if constexpr (MODE == kFwd) rc = launch_tiles<MODE, 64, 1>(q, a, b, st);
+    if constexpr (MODE == kFwd) rc = launch_tiles<MODE, 64, 1>(q, a, b, dev, st);
     else rc = semx::fail(SEMX_ERR_UNSUPPORTED, "gated_linear: tile of %d", q.bn);
   }
   if (rc != SEMX_OK || q.p.whole == q.p.tiles || MODE == kGate) return rc;
@@ -1240,7 +1263,7 @@ bool in_place(const void* base, int64_t ld, int bf16) { return bf16 && ld % 8 ==
 
 template <int NT>
 int launch_few_bf16(const SemxGatedLinearArgs* a, const GemmParams& p, cudaStream_t st) {
-  few_rows_bf16_kernel<NT><<<(unsigned)cdiv(a->H, (int64_t)8), kFewWarps * 32, 0, st>>>(
+  few_rows_bf16_kernel<NT><<<(unsigned)cdiv(a->H, (int64_t)8), few_warps(NT) * 32, 0, st>>>(
       reinterpret_cast<const __nv_bfloat16*>(a->x), a->ldx, reinterpret_cast<const __nv_bfloat16*>(a->w), a->D, a->H, (int)a->rows, p);
   return semx::check_launch("gated_linear few_rows_bf16_kernel");
 }
@@ -1261,7 +1284,7 @@ Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
   // (Rows that the wide loads take.)
   l.few_bf16 = !bwd && a->bf16 && a->rows <= kFewBf16 && a->D % 8 == 0 && (a->ldx % 8 == 0 || a->rows == 1) &&
                semx::aligned(a->x, 16) && semx::aligned(a->w, 16);
-  l.few = !bwd && a->rows <= kFew && !l.few_bf16;
+  l.few = !bwd && a->rows <= (a->bf16 ? kFew : kFewFp32) && !l.few_bf16;
   if (a->rows == 0 || l.few || l.few_bf16) return l;
   // Laid out anew wherever the sizes allow a misaligned base: the query has no addresses that count.
   l.lay_x = !in_place(a->x, a->ldx, a->bf16);
@@ -1391,10 +1414,20 @@ int semx_gated_linear_fwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
     return launch_few_bf16<2>(a, q.p, st);
   }
   if (l.few) {
-    if (a->rows == 1) return launch_few<1>(a, q.p, st);
-    if (a->rows == 2) return launch_few<2>(a, q.p, st);
-    if (a->rows <= 4) return launch_few<4>(a, q.p, st);
-    return launch_few<8>(a, q.p, st);
+    SemxGatedLinearArgs part = *a;
+    for (int64_t r = 0; r < a->rows; r += kFew) {
+      const int64_t e = a->bf16 ? 2 : 4;
+      part.rows = a->rows - r < kFew ? a->rows - r : kFew;
+      part.x = reinterpret_cast<const char*>(a->x) + r * a->ldx * e;
+      GemmParams p = q.p;
+      p.out = reinterpret_cast<char*>(a->h) + r * a->H * e;
+      if (p.u != nullptr) p.u += r * p.ldu, p.g += r * p.ldu;
+      rc = part.rows == 1 ? launch_few<1>(&part, p, st)
+           : part.rows == 2 ? launch_few<2>(&part, p, st)
+           : part.rows <= 4 ? launch_few<4>(&part, p, st) : launch_few<8>(&part, p, st);
+      if (rc != SEMX_OK) return rc;
+    }
+    return SEMX_OK;
   }
   SEMX_REQUIRE(l.total == 0 || a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_linear: workspace is NULL");
   char* ws = reinterpret_cast<char*>(a->workspace);
