@@ -16,6 +16,7 @@ that is summed are fp32.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -79,10 +80,25 @@ def _args(x, r, i, rate, z, r_bias, i_bias, scale, S, rows, L, cu):
     return a, (x, r, i, z)
 
 
-def _workspace(a, backward, like):
-    nbytes = _lib.load().semx_gated_lru_workspace_bytes(a, backward)
-    ws = _lib.scratch(nbytes, like) if nbytes else None
-    a.workspace = _lib.ptr(ws)
+@functools.lru_cache(maxsize=256)
+def _sizes(S, rows, L, C, packed):
+    """Bytes of the kept states, and of the workspace forward and backward: the library's, which depend
+    on nothing else."""
+    a = _lib.new_args(_lib.SemxGatedLruArgs)
+    a.rate_scale, a.S, a.rows, a.L, a.C = 1.0, S, rows, L, C
+    a.ldx = a.ldr = a.ldi = a.ldz = C
+    if packed:
+        a.cu_seqlens = 256
+    lib = _lib.load()
+    return (lib.semx_gated_lru_ckpt_bytes(a), lib.semx_gated_lru_workspace_bytes(a, 0),
+            lib.semx_gated_lru_workspace_bytes(a, 1))
+
+
+def _workspace(a, nbytes, like):
+    if not nbytes:
+        return None
+    ws = _lib.scratch(nbytes, like)
+    a.workspace = ws.data_ptr()
     return ws
 
 
@@ -92,20 +108,22 @@ class _GatedLru(torch.autograd.Function):
         rate32, rb32, ib32 = _lib.param32(rate), _lib.param32(r_bias), _lib.param32(i_bias)
         a, kept = _args(x, r, i, rate32, z, rb32, ib32, scale, S, rows, L, cu)
         y = x.new_empty(x.shape)
-        ckpt = _lib.scratch(_lib.load().semx_gated_lru_ckpt_bytes(a), x)
+        kept_bytes, fwd, bwd = _sizes(S, rows, L, rate.shape[0], cu is not None)
+        ckpt = _lib.scratch(kept_bytes, x)
         a.y, a.ckpt = y.data_ptr(), ckpt.data_ptr()
-        ws = _workspace(a, 0, x)
+        ws = _workspace(a, fwd, x)
         _lib.call("semx_gated_lru_fwd", a, x.device)
         xr, rr, ir, zr = kept
         ctx.save_for_backward(xr, rr, ir, rate32, zr, rb32, ib32, ckpt, cu)
-        ctx.cfg = (scale, S, rows, L, [None if t is None else t.dtype for t in (rate, r_bias, i_bias)])
+        ctx.cfg = (scale, S, rows, L, bwd, [None if t is None else t.dtype for t in (rate, r_bias, i_bias)])
         return y
 
     @staticmethod
     @_lib.once_differentiable
     def backward(ctx, dy):
         x, r, i, rate, z, r_bias, i_bias, ckpt, cu = ctx.saved_tensors
-        scale, S, rows, L, (rate_t, rb_t, ib_t) = ctx.cfg
+        scale, S, rows, L, nbytes, (rate_t, rb_t, ib_t) = ctx.cfg
+        # Strides anew: hooks on saved tensors may have brought them back laid out otherwise.
         a, kept = _args(x, r, i, rate, z, r_bias, i_bias, scale, S, rows, L, cu)
         dy = _lib.as_rows(dy, x.dtype)
         dx, dr, di = x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.shape)
@@ -117,7 +135,7 @@ class _GatedLru(torch.autograd.Function):
         a.ckpt, a.dy, a.dx, a.d_r, a.d_i, a.dz = (ckpt.data_ptr(), dy.data_ptr(), dx.data_ptr(), dr.data_ptr(),
                                                   di.data_ptr(), _lib.ptr(dz))
         a.drate, a.dr_bias, a.di_bias = _lib.ptr(drate), _lib.ptr(drb), _lib.ptr(dib)
-        ws = _workspace(a, 1, x)
+        ws = _workspace(a, nbytes, x)
         _lib.call("semx_gated_lru_bwd", a, x.device)
         return (dx, dr, di, _lib.cast(drate, rate_t), dz, _lib.cast(drb, rb_t), _lib.cast(dib, ib_t), None, None, None,
                 None, None)
@@ -153,7 +171,7 @@ def gated_lru_scan(x: torch.Tensor, r: torch.Tensor, i: torch.Tensor, rate: torc
     set_pool(op, a, S, x.get_device(), state, (ch,), torch.float32, slots, fresh)
     y = x.new_empty(x.shape)
     a.y = y.data_ptr()
-    ws = _workspace(a, 0, x)
+    ws = _workspace(a, _sizes(S, rows, L, ch, cu_seqlens is not None)[1], x)
     _lib.call("semx_gated_lru_fwd", a, x.device)
     return y
 

@@ -11,6 +11,8 @@ CUDA tensors only, like the other operators of this package (RuntimeError otherw
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import nn
 
@@ -32,10 +34,27 @@ def _args(x, weight, bias, act):
     return a
 
 
-def _workspace(a, backward, like):
-    nbytes = _lib.load().semx_gated_linear_workspace_bytes(a, backward)
-    ws = _lib.scratch(nbytes, like) if nbytes else None
-    a.workspace = _lib.ptr(ws)
+@functools.lru_cache(maxsize=256)
+def _sizes(rows, D, H, ldx, bf16, x_odd, w_odd, backward, dx, dw, db):
+    """Bytes of what the forward keeps, and of a call's workspace: the library's, by its sizes, whether x
+    and w lie on 16 bytes, and the gradients that are wanted."""
+    a = _lib.new_args(_lib.SemxGatedLinearArgs)
+    a.bf16, a.rows, a.D, a.H, a.ldx = bf16, rows, D, H, ldx
+    a.x, a.w, a.h, a.dh, a.saved = 256 + x_odd, 256 + w_odd, 256, 256, 256
+    a.dx, a.dw, a.db = 256 * dx or None, 256 * dw or None, 256 * db or None
+    lib = _lib.load()
+    return lib.semx_gated_linear_saved_bytes(a), lib.semx_gated_linear_workspace_bytes(a, backward)
+
+
+def _sizes_of(a, backward):
+    return _sizes(a.rows, a.D, a.H, a.ldx, a.bf16, a.x % 16, a.w % 16, backward, bool(a.dx), bool(a.dw), bool(a.db))
+
+
+def _workspace(a, nbytes, like):
+    if not nbytes:
+        return None
+    ws = _lib.scratch(nbytes, like)
+    a.workspace = ws.data_ptr()
     return ws
 
 
@@ -43,10 +62,12 @@ def _forward(x, weight, bias, act, keep):
     """(h, u and g in front of the activation where ``keep``)."""
     a = _args(x, weight, bias, act)
     h = x.new_empty((a.rows, a.H))
-    nbytes = _lib.load().semx_gated_linear_saved_bytes(a) if keep else 0
-    saved = _lib.scratch(nbytes, x) if nbytes else None
+    if a.rows == 0:
+        return h, None
+    kept, nbytes = _sizes_of(a, 0)
+    saved = _lib.scratch(kept, x) if keep and kept else None
     a.h, a.saved = h.data_ptr(), _lib.ptr(saved)
-    ws = _workspace(a, 0, x)
+    ws = _workspace(a, nbytes, x)
     _lib.call("semx_gated_linear_fwd", a, x.device)
     return h, saved
 
@@ -67,13 +88,15 @@ class _GatedLinear(torch.autograd.Function):
         x, weight, bias, saved = ctx.saved_tensors
         act, bias_t = ctx.cfg
         need = ctx.needs_input_grad
+        # Hooks on saved tensors may have brought them back laid out otherwise.
+        x, weight = rows_of(x, x.shape[1])[0], weight.contiguous()
         a = _args(x, weight, bias, act)
         dh = _lib.as_rows(dh, x.dtype)
         dx = x.new_empty(x.shape) if need[0] else None
         dw = torch.empty_like(weight) if need[1] else None
         db = weight.new_empty(weight.shape[0], dtype=torch.float32) if bias_t is not None and need[2] else None
         a.saved, a.dh, a.dx, a.dw, a.db = _lib.ptr(saved), dh.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db)
-        ws = _workspace(a, 1, x)
+        ws = _workspace(a, _sizes_of(a, 1)[1], x) if a.rows else None
         _lib.call("semx_gated_linear_bwd", a, x.device)
         return dx, dw, _lib.cast(db, bias_t), None
 
@@ -116,7 +139,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         rows = rows if rows_of(rows, D)[0] is rows else rows.contiguous()
         h = _GatedLinear.apply(rows, weight, bias, act)
     else:
-        h, _ = _forward(rows_of(rows, D)[0], weight.contiguous(), None if bias is None else bias.contiguous(), act, False)
+        h = _forward(rows_of(rows, D)[0], weight.contiguous(), None if bias is None else bias.contiguous(), act, False)[0]
     return h if x.dim() == 2 else h.view(lead + (h.shape[-1],))
 
 

@@ -380,6 +380,27 @@ def test_few_and_many_channel_tiles(C):
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-4 * float(b.abs().max()))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensors_moved(dtype):
+    """Operands whose rows are strided, kept elsewhere between the passes: they come back dense."""
+    from semambaxlinoss_b200.gated_lru import gated_lru_scan
+
+    rows, params = _operands(170, 40, dtype, gen(6))
+    ins = [_strided(t, 8).requires_grad_() for t in rows] + [p.to(cuda()).requires_grad_() for p in params]
+    dy = randn((170, 40), gen(7)).to(dtype).to(cuda())
+    cu = torch.tensor([0, 70, 70, 165], dtype=torch.int32, device=cuda())
+
+    def run():
+        x, r, i, z, rate, rb, ib = ins
+        return gated_lru_scan(x, r, i, rate, z=z, r_bias=rb, i_bias=ib, cu_seqlens=cu)
+
+    want = torch.autograd.grad(run(), ins, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = run()
+    got = torch.autograd.grad(y, ins, dy)
+    assert all(torch.equal(p[:165], q[:165]) if p.dim() == 2 else torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_empty_batches():
     from semambaxlinoss_b200.gated_lru import gated_lru_scan, gated_lru_step
 

@@ -154,6 +154,39 @@ def test_strides_and_shapes(dtype):
     assert single.shape == (24,)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 5, 8, 9, 12, 16, 17])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_few_strided_rows(rows, dtype):
+    """Few rows of a wider tensor at any offset: the bits of the same rows alone, at two widths of D."""
+    from semambaxlinoss_b200.gated_mlp import gated_linear
+
+    for D, H in ((200, 19), (2308, 36)):
+        x, w, b, _ = (t.to(cuda()) for t in _operands(rows, D, H, dtype, rows + D))
+        for off, ld in ((0, D + 8), (4, D + 4), (3, D + 5)):
+            wide = torch.full((rows, ld + off), float("nan"), dtype=dtype, device=cuda())
+            wide[:, off:off + D] = x
+            h = gated_linear(wide[:, off:off + D], w, b)
+            want = ogm.gated(x.double().cpu(), w.double().cpu(), b.double().cpu(), "silu")
+            _check({"h": h}, want, rows, D, H, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_saved_tensors_moved(dtype):
+    """Operands whose rows are strided, kept elsewhere between the passes: they come back dense."""
+    from semambaxlinoss_b200.gated_mlp import gated_linear
+
+    x, w, b, dh = (t.to(cuda()) for t in _operands(150, 64, 24, dtype, 37))
+    for off in (0, 3):
+        wide = torch.full((150, 160), float("nan"), dtype=dtype, device=cuda())
+        wide[:, off:off + 64] = x
+        ins = [wide[:, off:off + 64].requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+        want = torch.autograd.grad(gated_linear(*ins), ins, dh)
+        with torch.autograd.graph.save_on_cpu():
+            h = gated_linear(*ins)
+        got = torch.autograd.grad(h, ins, dh)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_empty():
     from semambaxlinoss_b200.gated_mlp import gated_linear
 
