@@ -213,25 +213,32 @@ __device__ __forceinline__ void leave_state(const GlParams& p, int64_t j, int c,
 }
 
 // State in front of the tile for channel c (a lane each; ok false: none): the maps of the tiles in
-// front in its group, folded in their order, applied to the state that the group before left (looked for
-// last: it comes last). The first tile of a sequence has its entry state in its map (A = 0).
-__device__ __forceinline__ float link_in(const GlParams& p, const Chain& q, int c, bool ok) {
-  const int g0 = q.at / kGroup * kGroup, n = ok ? q.at - g0 : 0;
-  const long long from = clock64();
-  bool given_up = false;
+// front in its group, folded in their order, applied to the state that the group before left. Three warps fetch
+// five of the maps each while the fourth waits for the state, so that a link is one way to L2 and back
+// (4 x 2047 x 2048 bf16, the fourth warp alone: forward 59 us, backward 135; so: 54 and 126). The first
+// tile of a sequence has its entry state in its map (A = 0).
+constexpr int kAhead = (kGroup - 1) / 3;  // maps of a warp
+static_assert(3 * kAhead == kGroup - 1, "maps in front");
+typedef float Links[3][2][kCh];
+__device__ __forceinline__ float link_failed() {
+  atomicAdd(&g_link_timeouts, 1u);
+  return __int_as_float(0x7fffffff);
+}
+// Warps 1 to 3: the fold of their maps.
+__device__ __forceinline__ void link_maps(const GlParams& p, const Chain& q, int c, bool ok, Links& to) {
+  const int part = threadIdx.x / 32 - 1, g0 = q.at / kGroup * kGroup, e0 = part * kAhead, n = ok ? q.at - g0 - e0 : 0;
   float a = 1.f, b = 0.f;
-  constexpr int kAhead = 5;  // maps on their way
-#pragma unroll 1
-  for (int e0 = 0; e0 < n; e0 += kAhead) {
+  if (n > 0) {
+    const long long from = clock64();
     ulonglong2 m[kAhead];
-    bool done;
+    bool done, given_up;
     do {
       done = true;
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
         const int j = q.j0 + q.dir * (g0 + e0 + e);
         // Offsets that decrease can name a piece that is none.
-        const bool there = e0 + e < n && j >= 0 && j < (int)p.m.pieces;
+        const bool there = e < n && j >= 0 && j < (int)p.m.pieces;
         m[e] = there ? peek_map(&p.maps[(int64_t)j * p.C + c]) : make_ulonglong2(marked(1.f), marked(0.f));
       }
 #pragma unroll
@@ -244,24 +251,32 @@ __device__ __forceinline__ float link_in(const GlParams& p, const Chain& q, int 
       b = fmaf(A, b, B);
       a *= A;
     }
-    if (given_up) break;
+    if (given_up) b = link_failed();
   }
-  const int jb = q.j0 + q.dir * (g0 - 1);
-  if (ok && g0 > 0 && jb >= 0 && jb < (int)p.m.pieces && !given_up) {
-    const unsigned long long* at = &p.left[(int64_t)jb * p.C + c];
-    unsigned long long before;
-    do {
-      before = peek(at);
-      given_up = (before & kHere) == 0 && clock64() - from > kPatience;
-    } while ((before & kHere) == 0 && !given_up);
-    b = fmaf(a, __uint_as_float((unsigned)before), b);
-  }
-  if (given_up) {
-    atomicAdd(&g_link_timeouts, 1u);
-    return __int_as_float(0x7fffffff);
-  }
-  return b;
+  to[part][0][threadIdx.x & 31] = a;
+  to[part][1][threadIdx.x & 31] = b;
 }
+// Warp 0: the state that the group before left.
+__device__ __forceinline__ float link_state(const GlParams& p, const Chain& q, int c, bool ok) {
+  const int g0 = q.at / kGroup * kGroup, jb = q.j0 + q.dir * (g0 - 1);
+  if (!ok || g0 == 0 || jb < 0 || jb >= (int)p.m.pieces) return 0.f;
+  const long long from = clock64();
+  const unsigned long long* at = &p.left[(int64_t)jb * p.C + c];
+  unsigned long long before;
+  do {
+    before = peek(at);
+    if ((before & kHere) == 0 && clock64() - from > kPatience) return link_failed();
+  } while ((before & kHere) == 0);
+  return __uint_as_float((unsigned)before);
+}
+__device__ __forceinline__ float link_all(const Links& from, float h) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) h = fmaf(from[k][0][threadIdx.x & 31], h, from[k][1][threadIdx.x & 31]);
+  return h;
+}
+// Warps 1 to 3 have left their folds; warp 0 waits for them.
+__device__ __forceinline__ void links_left() { asm volatile("bar.arrive 1, %0;" ::"n"(kT) : "memory"); }
+__device__ __forceinline__ void links_await() { asm volatile("bar.sync 1, %0;" ::"n"(kT) : "memory"); }
 
 // -- the order of a CTA's tiles -------------------------------------------------------------------
 
@@ -444,6 +459,8 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
   extern __shared__ __align__(16) unsigned char raw[];
   Stage<ACC, SEG, 4>& st = *reinterpret_cast<Stage<ACC, SEG, 4>*>(raw);
   __shared__ __align__(16) float maps[2][2][kSegs][kCh];  // this tile's and the one's before: A, B
+  __shared__ __align__(16) float entries[2][kCh];          // linked: state in front of the tile
+  __shared__ Links links;
   __shared__ __align__(16) Rates rt;
   __shared__ int ticket;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -515,32 +532,52 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
       step = 0;
       n += at.walk;
     }
-    float h = 0.f, fA = 1.f, fB = 0.f;
-    if (warp == 0) {
-      if (first && ok && slot != semx::kNone) {
-        const bool fresh = p.m.fresh != nullptr && p.m.fresh[w.s] != 0;
-        h = slot == semx::kRefused ? __int_as_float(0x7fffffff) : fresh ? 0.f : p.state[slot * p.C + c];
-      }
-      if (LINK && ok) {
-        fB = h;
-#pragma unroll
-        for (int s = 0; s < kSegs; ++s) {
-          fA *= mA[s][lane];
-          fB = fmaf(mA[s][lane], fB, mB[s][lane]);
-        }
-        leave_map(p, w.j, c, first ? 0.f : fA, fB);
-      }
+    float h = 0.f;
+    if (warp == 0 && first && ok && slot != semx::kNone) {
+      const bool fresh = p.m.fresh != nullptr && p.m.fresh[w.s] != 0;
+      h = slot == semx::kRefused ? __int_as_float(0x7fffffff) : fresh ? 0.f : p.state[slot * p.C + c];
     }
-    // The next tile's rows set out while this one's state is on its way; warp 0 has the state to find
-    // first, unless it waits for others.
+    const bool keeps = p.ckpt != nullptr && ok && w.live;
+    float fA = 1.f, fB = 0.f, uA[Q / kUnit], uB[Q / kUnit];
+    if (LINK && warp == 0) {
+      // Behind this the maps of the steps in front of each segment stand in the segments' places.
+#pragma unroll
+      for (int s = 0; s < kSegs; ++s) {
+        const float A = mA[s][lane], B = mB[s][lane];
+        mA[s][lane] = fA;
+        mB[s][lane] = fB;
+        if (s % (kUnit / SEG) == 0) uA[s * SEG / kUnit] = fA, uB[s * SEG / kUnit] = fB;
+        fA *= A;
+        fB = fmaf(A, fB, B);
+      }
+      if (ok) leave_map(p, w.j, c, first ? 0.f : fA, first ? fmaf(fA, h, fB) : fB);
+    }
+    // The next tile's rows set out while this one's state is on its way; a walked sequence's warp 0 has the state to
+    // find first.
     const Tile next = tile_at<LINK, false, Q>(p, n, step);
     if (LINK || warp != 0) fetch(next);
-    if (warp == 0) {
-      if (!first) h = !LINK ? carry : w.live ? link_in(p, Chain{w.j - w.k, 1, w.k}, c, ok) : 0.f;
-      // Every tile leaves its state, so that nothing waits for long whatever the offsets are; at once, for
-      // the next group waits.
-      if (LINK && ok) leave_state(p, w.j, c, first ? fB : fmaf(fA, h, fB));
-      const bool keeps = p.ckpt != nullptr && ok && w.live;
+    if (LINK) {
+      const bool waits = !first && w.live;  // of the whole CTA
+      const Chain chain{w.j - w.k, 1, w.k};
+      if (warp != 0) {
+        if (waits) link_maps(p, chain, c, ok, links);
+        links_left();
+      }
+      if (warp == 0) {
+        if (waits) h = link_state(p, chain, c, ok);
+        links_await();
+        if (waits) h = link_all(links, h);
+        entries[buf][lane] = h;
+        // Every tile leaves its state, so that nothing waits for long whatever the offsets are.
+        const float after = fmaf(fA, h, fB);
+        if (ok) leave_state(p, w.j, c, after);
+#pragma unroll
+        for (int u = 0; u < Q / kUnit; ++u)
+          if (keeps && (u == 0 || u * kUnit < w.n)) p.ckpt[((int64_t)w.unit + u) * p.C + c] = fmaf(uA[u], h, uB[u]);
+        if (w.live && last && ok && slot >= 0) p.state[slot * p.C + c] = after;
+      }
+    } else if (warp == 0) {
+      if (!first) h = carry;
 #pragma unroll
       for (int s = 0; s < kSegs; ++s) {
         if (s % (kUnit / SEG) == 0 && keeps && (s == 0 || s * SEG < w.n)) p.ckpt[((int64_t)w.unit + s * SEG / kUnit) * p.C + c] = h;
@@ -549,11 +586,15 @@ __global__ void __launch_bounds__(kT, kFwdCtas) gated_lru_fwd_kernel(const GlPar
         h = after;
       }
       carry = h;
-      if (w.live && last && ok && slot >= 0) p.state[slot * p.C + c] = h;
+      if (last && ok && slot >= 0) p.state[slot * p.C + c] = h;
     }
     __syncthreads();
     if (!LINK && warp == 0) fetch(next);
     f2 hs[2] = {shared_pair(mB[at.seg], at.lc), shared_pair(mB[at.seg], at.lc + 2)};
+    if (LINK) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) hs[k] = fma2(shared_pair(mA[at.seg], at.lc + 2 * k), shared_pair(entries[buf], at.lc + 2 * k), hs[k]);
+    }
     char* out = reinterpret_cast<char*>(p.y) + ((int64_t)(w.row + at.seg * SEG) * p.C + at.c0 + at.lc) * element(ACC, p.bf16);
     const int64_t row = (int64_t)p.C * element(ACC, p.bf16);
     const int end = at.nn > 0 ? most : 0;
@@ -650,6 +691,8 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
   extern __shared__ __align__(16) unsigned char raw[];
   Stage<ACC, SEG, 5>* stages = reinterpret_cast<Stage<ACC, SEG, 5>*>(raw);  // this tile's and the next one's
   __shared__ __align__(16) float maps[2][3][kSegs][kCh];  // A, B, and B of the adjoint's map
+  __shared__ __align__(16) float entries[2][kCh];         // linked: what reaches the tile's last step from behind
+  __shared__ Links links;
   __shared__ __align__(16) float sums[4][3][kCh];         // a tile's (or a walked sequence's) sums, one row per warp
   __shared__ __align__(16) Rates rt;
   __shared__ int ticket;
@@ -760,35 +803,52 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
       step = 0;
       n += at.walk;
     }
-    float fA = 1.f, fG = 0.f;
+    float fA = 1.f, fG = 0.f, behind[kSegs];
     if (LINK && warp == 0) {
 #pragma unroll
       for (int s = kSegs - 1; s >= 0; --s) {
-        fA *= mA[s][lane];
-        fG = fmaf(mA[s][lane], fG, mG[s][lane]);
+        const float A = mA[s][lane], G = mG[s][lane];
+        behind[s] = fA;
+        mG[s][lane] = fG;  // from here on the map of the steps behind the segment, A's part still to come
+        fA *= A;
+        fG = fmaf(A, fG, G);
       }
       if (ok) leave_map(p, w.j, c, end ? 0.f : fA, fG);
     }
     const Tile next = tile_at<LINK, true, Q>(p, n, step);
     if (LINK || warp != 0) fetch(next, stages[buf ^ 1]);
+    const bool waits = LINK && !end && w.live;  // of the whole CTA
+    const Chain chain{w.j - w.k + w.tiles - 1, -1, w.tiles - 1 - w.k};
+    if (LINK && warp != 0) {
+      if (waits) link_maps(p, chain, c, ok, links);
+      links_left();
+    }
     if (warp == 0) {
       float h = entry;
 #pragma unroll
       for (int s = 0; s < kSegs; ++s) {
         const float after = fmaf(mA[s][lane], h, mB[s][lane]);
         mB[s][lane] = h;
+        if (LINK) mA[s][lane] = behind[s];
         h = after;
       }
       float g = 0.f;
-      if (!end) g = !LINK ? carry : w.live ? link_in(p, Chain{w.j - w.k + w.tiles - 1, -1, w.tiles - 1 - w.k}, c, ok) : 0.f;
-      if (LINK && ok) leave_state(p, w.j, c, fmaf(fA, g, fG));
+      if (LINK) {
+        if (waits) g = link_state(p, chain, c, ok);
+        links_await();
+        if (waits) g = link_all(links, g);
+        entries[buf][lane] = g;
+        if (ok) leave_state(p, w.j, c, fmaf(fA, g, fG));
+      } else {
+        if (!end) g = carry;
 #pragma unroll
-      for (int s = kSegs - 1; s >= 0; --s) {
-        const float before = fmaf(mA[s][lane], g, mG[s][lane]);
-        mG[s][lane] = g;  // from here on what reaches the segment's last step from behind
-        g = before;
+        for (int s = kSegs - 1; s >= 0; --s) {
+          const float before = fmaf(mA[s][lane], g, mG[s][lane]);
+          mG[s][lane] = g;  // from here on what reaches the segment's last step from behind
+          g = before;
+        }
+        carry = g;
       }
-      carry = g;
     }
     __syncthreads();
     if (!LINK && warp == 0) fetch(next, stages[buf ^ 1]);
@@ -803,6 +863,10 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
           hs[k] = after;
         }
       f2 gs[2] = {shared_pair(mG[at.seg], at.lc), shared_pair(mG[at.seg], at.lc + 2)};
+      if (LINK) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) gs[k] = fma2(shared_pair(mA[at.seg], at.lc + 2 * k), shared_pair(entries[buf], at.lc + 2 * k), gs[k]);
+      }
       if (slow) gradient_steps<ACC, SEG, true>(p, rt, at, st, exps, most, w.row, a, b, d, gs, sum);
       else gradient_steps<ACC, SEG, false>(p, rt, at, st, exps, most, w.row, a, b, d, gs, sum);
     }
@@ -977,7 +1041,7 @@ int launch_gl(bool bwd, const GlParams& p, cudaStream_t st) {
   if (each > works) each = works;
   if (each < 1) each = 1;
   const unsigned n = (unsigned)(each * p.ctiles);
-  constexpr size_t kStatic = 15 * 1024;  // shared memory of fixed size, at most
+  constexpr size_t kStatic = 16 * 1024;  // shared memory of fixed size, at most
 #define SEMX_GL(KERNEL, STAGES)                                      \
   do {                                                               \
     if ((STAGES) + kStatic > 48 * 1024 && !semx::allow_smem(KERNEL, (STAGES) + 48 * 1024)) return SEMX_ERR_LAUNCH; \
