@@ -22,13 +22,14 @@
 // through the legacy tensor products (a tcgen05 tile would be nearly empty), fp32 through packed multiplies.
 //
 // Measured (device time): 8192 x 2048 -> 5504 bf16 forward 272 us (1.36 PFLOP/s; the GPU's power limit is what
-// bounds it), dW 250, dx 237; 4099 x 2048 -> 5461 131 (1.40); 192 x 4096 -> 11008 45 (4.0 TB/s of weights);
-// 129684 x 64 -> 256 fp32, which is its results' bytes: forward 146 (3.0 TB/s; the epilogue's chain of
-// tensor memory, activation and exchange: 0.46 of the issue slots), dx 86, dW 77.
+// bounds it), dW 250, dx 237; 4099 x 2048 -> 5461 131 (1.40); 192 x 4096 -> 11008 43 (4.2 TB/s of weights);
+// 129684 x 64 -> 256 fp32, which is its results' bytes: forward 129 (3.3 TB/s; the epilogue's chain of
+// tensor memory, activation and exchange), dx 85, dW 76; bf16 forward 50, its products again for du and dg 114.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "semx_reduce.cuh"
 #include "semx_tc.cuh"
@@ -92,14 +93,16 @@ __device__ __forceinline__ float normal_tail(float g, float* e) {
   q = fmaf(q, t, 0.14104384183883667f);
   return t * q * *e;
 }
-__device__ __forceinline__ float act_of(float g, int gelu) {
+// (gelu: known to the compiler where many values follow one another. A branch in front of each would keep their
+// special functions apart: 129684 x 64 -> 256 bf16 forward 62 us, so 50.)
+__device__ __forceinline__ float act_of(float g, bool gelu) {
   if (!gelu) return g * sigmoid(g);
   float e;
   const float tail = normal_tail(g, &e);
   return g * (g < 0.f ? tail : 1.f - tail);
 }
 // act(g) and act'(g).
-__device__ __forceinline__ void act_and_slope(float g, int gelu, float* act, float* slope) {
+__device__ __forceinline__ void act_and_slope(float g, bool gelu, float* act, float* slope) {
   if (gelu) {
     float e;
     const float tail = normal_tail(g, &e), cdf = g < 0.f ? tail : 1.f - tail;
@@ -454,6 +457,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
       slice(t, &k0, &k1);
       const int m0 = t.m * 2 * kM + (int)rank * kM, n0 = t.n * BN + (int)rank * (BN / 2);
       int kh = k0 >= p.khalf ? 1 : 0, kk = (k0 - kh * p.khalf) * kK;
+      // Where each row of W is read once, tiles start their depth at different places: in step, all rows' addresses
+      // would be the same but for the row (192 x 4096 -> 11008: 45.1 and 43.2 us).
+      const bool turns = MODE == kFwd && PARTS == 1 && p.tiles_m == 1;
+      if (turns) kk = (k0 + w * 5 % (k1 - k0)) * kK;
       for (int k = k0; k < k1 && ok; ++k) {
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
@@ -482,7 +489,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           if (++s == ST) s = 0, phase ^= 1;
         }
         kk += kK;
-        if (kk >= p.khalf * kK) kk = 0, ++kh;
+        if (turns && kk == k1 * kK) kk = k0 * kK;
+        if (MODE == kDx && kk >= p.khalf * kK) kk = 0, ++kh;
       }
     }
     // After a wait that gave up: the copies on their way land before the CTAs end (CTA 0 sees both CTAs').
@@ -606,13 +614,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         if constexpr (MODE == kGate) {
           float d[kCols];
           read_block(buf, d, p.dh, p.N, row0, col0, rows, cols);
+          auto slopes = [&](auto gelu) {
 #pragma unroll
-          for (int i = 0; i < kCols; ++i) {
-            float act, slope;
-            act_and_slope(g[i], p.gelu, &act, &slope);
-            g[i] = d[i] * v[i] * slope;
-            v[i] = d[i] * act;
-          }
+            for (int i = 0; i < kCols; ++i) {
+              float act, slope;
+              act_and_slope(g[i], decltype(gelu)::value, &act, &slope);
+              g[i] = d[i] * v[i] * slope;
+              v[i] = d[i] * act;
+            }
+          };
+          if (p.gelu) slopes(std::true_type());
+          else slopes(std::false_type());
           float* to = p.sums == nullptr ? nullptr : p.sums + (((int64_t)t.m * 2 + rank) * 4 + quarter) * 2 * p.N + col0;
           const int64_t at = row0 * p.ldz + col0;
           write_summed(buf, v, p.dz + at, p.ldz, rows, cols, to);
@@ -623,8 +635,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           write_block(buf, v, p.u, p.ldu, row0, col0, rows, cols, 0);
           write_block(buf, g, p.g, p.ldu, row0, col0, rows, cols, 0);
         }
+        auto acts = [&](auto gelu) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) v[i] *= act_of(g[i], p.gelu);
+          for (int i = 0; i < kCols; ++i) v[i] *= act_of(g[i], decltype(gelu)::value);
+        };
+        if (p.gelu) acts(std::true_type());
+        else acts(std::false_type());
         write_block(buf, v, p.out, p.ldo, row0, col0, rows, cols, p.out_bf16);
       } else {
         write_block(buf, v, p.out, p.ldo, (int64_t)t.half * p.M + row0, col0, rows, cols, p.out_bf16);
@@ -664,11 +680,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         slice(t, &k0, &k1);
         float sum[VALUES];
         bool ok = true;
-        for (int c0 = k0; c0 < k1; c0 += kDrain, ++acc) {
+        auto drain = [&](auto first) {
           const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
           ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
           ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          if (!ok) return;
           semx::tc::fence_after_sync();
 #pragma unroll
           for (int i = 0; i < VALUES; i += 2 * kCols) {
@@ -676,12 +692,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
             tmem_ld16_twice(d + column(i), d + column(i + kCols), v, y);
 #pragma unroll
             for (int j = 0; j < kCols; ++j) {
-              sum[i + j] = c0 == k0 ? v[j] : sum[i + j] + v[j];
-              sum[i + kCols + j] = c0 == k0 ? y[j] : sum[i + kCols + j] + y[j];
+              sum[i + j] = decltype(first)::value ? v[j] : sum[i + j] + v[j];
+              sum[i + kCols + j] = decltype(first)::value ? y[j] : sum[i + kCols + j] + y[j];
             }
           }
           release(b ? acc_e1 : acc_e0);
-        }
+          ++acc;
+        };
+        drain(std::true_type());
+        for (int c0 = k0 + kDrain; c0 < k1 && ok; c0 += kDrain) drain(std::false_type());
         if (!ok) break;
         ok = wait_phase(&small_full[tiles & 1], (tiles >> 1) & 1, &dead);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -812,13 +831,13 @@ __global__ void __launch_bounds__(256) lay_kernel(const void* src, int64_t ld, i
 }
 
 // du and dg from u, g (fp32, rows of ldu) and dh, as parts (PARTS, 2, rows, ldp). HBM is the bound: 129684 x 256
-// fp32 136 us (5.9 TB/s), 8192 x 5504 bf16 108 (5.8). Column sums of 64
+// fp32 131 us (6.1 TB/s), 8192 x 5504 bf16 107 (5.9). Column sums of 64
 // rows each into sums (row blocks, 2 H) where wanted. A thread has 4 columns of every 4th row, two rows
 // on their way at a time; CTAs side by side have columns side by side.
 constexpr int kDzRows = 64;
-template <int PARTS>
+template <int PARTS, bool GELU>
 __global__ void __launch_bounds__(256, PARTS == 1 ? 4 : 3) gate_grad_kernel(const float* u, const float* g, int64_t ldu, const void* dh,
-                                                        int64_t rows, int64_t H, int gelu, __nv_bfloat16* dz, int64_t ldp,
+                                                        int64_t rows, int64_t H, __nv_bfloat16* dz, int64_t ldp,
                                                         float* sums) {
   constexpr bool BF16 = PARTS == 1;
   constexpr int ACC = BF16 ? semx_scan::kBf16 : semx_scan::kFp32, AHEAD = 2;
@@ -862,7 +881,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 4 : 3) gate_grad_kernel(cons
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float act, slope;
-          act_and_slope(gg[k], gelu, &act, &slope);
+          act_and_slope(gg[k], GELU, &act, &slope);
           const bool in = k < nn;
           const float du = in ? d4[a][k] * act : 0.f, dg = in ? d4[a][k] * uu[k] * slope : 0.f;
           su[k] += du;
@@ -1180,7 +1199,7 @@ Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   p.tiles = p.tiles_m * p.tiles_n * (mode == kDw ? 2 : 1);
   // The last round's tiles run in slices of the depth where they leave half of the SMs idle or more, of 8
   // stages (fp32: 4, each of them six products) at least; behind whole rounds only where that saves more
-  // than the kernel that adds the slices takes (192 x 4096 -> 11008, 172 tiles of 128 columns: 51 us, sliced 45 and 4 of
+  // than the kernel that adds the slices takes (192 x 4096 -> 11008, 172 tiles of 128 columns: 51 us, sliced 45 and 4.5 of
   // adding).
   const int last = p.tiles % kPairs;
   const int64_t stages = parts > 1 ? 4 : 8;
@@ -1486,8 +1505,9 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   } else {
     const float *u = a->saved, *g = a->saved + a->rows * Hp;
     const unsigned grid = (unsigned)(cdiv(a->rows, (int64_t)kDzRows) * cdiv(a->H, (int64_t)256));
-    if (a->bf16) gate_grad_kernel<1><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
-    else gate_grad_kernel<kParts><<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, a->act, dz, Hp, sums);
+    auto* kernel = a->bf16 ? (a->act ? gate_grad_kernel<1, true> : gate_grad_kernel<1, false>)
+                           : (a->act ? gate_grad_kernel<kParts, true> : gate_grad_kernel<kParts, false>);
+    kernel<<<grid, 256, 0, st>>>(u, g, Hp, a->dh, a->rows, a->H, dz, Hp, sums);
     rc = semx::check_launch("gated_linear gate_grad_kernel");
   }
   if (rc != SEMX_OK) return rc;
