@@ -23,8 +23,9 @@
 //
 // Measured (device time): 8192 x 2048 -> 5504 bf16 forward 272 us (1.36 PFLOP/s; the GPU's power limit is what
 // bounds it), dW 250, dx 237; 4099 x 2048 -> 5461 131 (1.40); 192 x 4096 -> 11008 43 (4.2 TB/s of weights);
-// 129684 x 64 -> 256 fp32, which is its results' bytes: forward 129 (3.3 TB/s; the epilogue's chain of
-// tensor memory, activation and exchange), dx 85, dW 76; bf16 forward 50, its products again for du and dg 114.
+// 129684 x 64 -> 256 fp32, which is its results' bytes: forward 118 (3.7 TB/s; the epilogue's chain of
+// tensor memory, activation and exchange), dx 85, dW 76; bf16 forward 49 (without biases 42), its products again for
+// du and dg 112 (88).
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -646,19 +647,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         write_block(buf, v, p.out, p.ldo, (int64_t)t.half * p.M + row0, col0, rows, cols, p.out_bf16);
       }
     };
+    // The biases of a tile, a lane per column: fetched while the tile before is written (when
+    // the tile begins: 129684 x 64 -> 256 fp32 forward 131 us, so 118).
+    static_assert(!GATED || WC <= 32, "biases");
+    uint32_t bias_u = 0, bias_g = 0;
+    auto fetch_bias = [&](const Tile& t) {
+      const int64_t col = (int64_t)t.n * CN + side * WC + lane;
+      const bool any = lane < WC && col < p.N;
+      bias_u = any ? semx_scan::load_raw(p.bias, col, p.bias_bf16) : 0;
+      bias_g = any ? semx_scan::load_raw(p.bias, p.N + col, p.bias_bf16) : 0;
+    };
     uint32_t acc = 0, tiles = 0;
+    if (GATED && p.bias != nullptr && pair0 < works) fetch_bias(tile_at(p, pair0));
     for (int w = pair0; w < works; w += pairs, ++tiles) {
       const Tile t = tile_at(p, w);
-      if (GATED && p.bias != nullptr) {  // the tile's biases, while its products run
-        static_assert(!GATED || WC <= 32, "biases");
+      if (GATED && p.bias != nullptr) {
         __syncwarp();
-        if (lane < WC) {
-          const int64_t col = (int64_t)t.n * CN + side * WC + lane;
-          float* at = buf + 32 * kBufRow + lane;
-          at[0] = col < p.N ? semx_scan::load(p.bias, col, p.bias_bf16) : 0.f;
-          at[32] = col < p.N ? semx_scan::load(p.bias, p.N + col, p.bias_bf16) : 0.f;
-        }
+        buf[32 * kBufRow + lane] = semx_scan::as_float(bias_u, p.bias_bf16);
+        buf[32 * kBufRow + 32 + lane] = semx_scan::as_float(bias_g, p.bias_bf16);
         __syncwarp();
+        if (w + pairs < works) fetch_bias(tile_at(p, w + pairs));
       }
       if constexpr (PARTS == 1) {
         const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
@@ -1405,7 +1413,7 @@ size_t semx_gated_linear_args_size(void) { return sizeof(SemxGatedLinearArgs); }
 size_t semx_gated_linear_saved_bytes(const SemxGatedLinearArgs* a) {
   if (a == nullptr || a->rows < 0 || a->H < 0) return 0;
   // Narrow bf16 rows: the backward makes u and g again in less time than it takes to write and read them
-  // (training passes, kept and made again: 129684 x 64 -> 256 254 and 233 us, 16384 x 512 -> 1408 234 and 223,
+  // (training passes, kept and made again: 129684 x 64 -> 256 241 and 199 us, 16384 x 512 -> 1408 226 and 213,
   // 8192 x 1024 -> 2752 299 and 314). In fp32, six times the products and three parts to write, it does not
   // (129684 x 64 -> 256 462 and 549).
   if (makes_again(a)) return 0;
