@@ -785,8 +785,8 @@ int semx_gated_lru_step(const SemxGatedLruArgs* args, semx_stream_t stream);
  *   [u | g] = x W^T + bias;  h = u act(g)   (act 0: silu, 1: gelu with the normal distribution)
  * x (rows, D) at row stride ldx, w (2 H, D) contiguous (the value's rows, then the gate's), h, dh
  * (rows, H), dx (rows, D) and dw contiguous; all bf16 when `bf16` is set, else fp32. bias
- * (2 H, may be NULL) by bias_bf16, db (2 H, may be NULL) fp32. Sums are fp32; fp32 operands keep 2^-24 of each product (as three
- * bf16 parts; an infinity among them gives NaN).
+ * (2 H, may be NULL) bf16 when bias_bf16 is set, else fp32, db (2 H, may be NULL) fp32. Sums are fp32; fp32
+ * operands keep 2^-24 of each product (as three bf16 parts; an infinity among them gives NaN).
  * A training forward passes saved (semx_gated_linear_saved_bytes(): u and g in fp32, 16-byte
  * aligned; 0 bytes for narrow bf16 rows, whose u and g the backward makes again from x, w and
  * bias) and the backward reads it. It writes dx, dw and db (each may be NULL), sums in a

@@ -10,7 +10,9 @@
 // with speed = rate_scale softplus(rate).
 //
 // Bound: HBM (5 values per element forward, 9 backward); the special-function unit (6 operations per
-// element forward) comes next.
+// element forward, 11 backward) comes next. Measured (device time): many sequences, 404 x 321 x 256 fp32 forward
+// 113 us (5.9 TB/s) and backward 209 (5.7), bf16 84 and 184 (instructions); linked, 8191 x 2048 bf16 54 (3.1 TB/s: the
+// links' way to L2 and back on top), 4 x 2047 x 2048 bf16 backward 126 (2.4).
 //
 // Split: a tile is 64 steps (backward 32) of one sequence by 32 channels; a CTA of four warps reads
 // it once. A thread has a segment of 4 (2) neighbouring steps of four neighbouring channels: it folds
@@ -23,8 +25,8 @@
 // state behind it, and takes the maps of the tiles in front of it in its group of 16 and the state that
 // the group before left. Which maps are folded in which order depends on the numbers alone, so
 // results do not change from run to run. Tickets number the tiles in the order in which CTAs take
-// them, one count for each 32 channels, so a tile only waits for tiles that are under way. The backward runs the same from the last
-// tile on.
+// them, one count for each 32 channels, so a tile only waits for tiles that are under way. The backward runs the
+// same from the last tile on.
 #include "semx_reduce.cuh"
 #include "state_scan.cuh"
 
@@ -895,7 +897,8 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
 }
 
 // One token per sequence: a thread has four channels of one, a CTA a run of sequences (their slots
-// are looked up together, the parameters read once).
+// are looked up together, the parameters read once). Bound by its chain of slots, rows and state: 192 x 4096 fp32
+// 6.2 us (22 MB), one row of 2048 3.5.
 constexpr int kStepT = 128, kStepRows = 8;
 template <int ACC>
 __global__ void __launch_bounds__(kStepT) gated_lru_step_kernel(const GlParams p, int rows) {
