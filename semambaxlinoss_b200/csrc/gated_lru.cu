@@ -228,20 +228,23 @@ __device__ __forceinline__ float link_failed() {
 }
 // Warps 1 to 3: the fold of their maps.
 __device__ __forceinline__ void link_maps(const GlParams& p, const Chain& q, int c, bool ok, Links& to) {
-  const int part = threadIdx.x / 32 - 1, g0 = q.at / kGroup * kGroup, e0 = part * kAhead, n = ok ? q.at - g0 - e0 : 0;
+  const int part = threadIdx.x / 32 - 1, e0 = q.at / kGroup * kGroup + part * kAhead, j = q.j0 + q.dir * e0;
+  // Offsets that decrease can name pieces that are none.
+  const int there = j < 0 || j >= (int)p.m.pieces ? 0 : q.dir > 0 ? (int)p.m.pieces - j : j + 1;
+  const int n = ok ? min(q.at - e0, there) : 0;
   float a = 1.f, b = 0.f;
   if (n > 0) {
     const long long from = clock64();
+    const ulonglong2* at = p.maps + (int64_t)j * p.C + c;
+    const int64_t step = (int64_t)q.dir * p.C;
     ulonglong2 m[kAhead];
     bool done, given_up;
     do {
       done = true;
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
-        const int j = q.j0 + q.dir * (g0 + e0 + e);
-        // Offsets that decrease can name a piece that is none.
-        const bool there = e < n && j >= 0 && j < (int)p.m.pieces;
-        m[e] = there ? peek_map(&p.maps[(int64_t)j * p.C + c]) : make_ulonglong2(marked(1.f), marked(0.f));
+        m[e] = make_ulonglong2(marked(1.f), marked(0.f));
+        if (e < n) m[e] = peek_map(at + e * step);
       }
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) done = done && (m[e].x & kHere) != 0 && (m[e].y & kHere) != 0;
@@ -695,7 +698,6 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
   __shared__ __align__(16) float maps[2][3][kSegs][kCh];  // A, B, and B of the adjoint's map
   __shared__ __align__(16) float entries[2][kCh];         // linked: what reaches the tile's last step from behind
   __shared__ Links links;
-  __shared__ __align__(16) float sums[4][3][kCh];         // a tile's (or a walked sequence's) sums, one row per warp
   __shared__ __align__(16) Rates rt;
   __shared__ int ticket;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -731,7 +733,9 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
   auto write_sums = [&]() {
     if (summed < 0 || warp == 0 || !ok) return;
     const int k = warp - 1;
-    const float v = sums[0][k][lane] + sums[1][k][lane] + sums[2][k][lane] + sums[3][k][lane];
+    float v = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSegs; ++s) v += maps[buf ^ 1][k][s][lane];
     p.part[((int64_t)summed * 3 + k) * p.C + c] = k == 0 ? -rt.slope[lane] * v : v;
   };
   f2 sum[3][2];
@@ -873,18 +877,13 @@ __global__ void __launch_bounds__(kT, kBwdCtas) gated_lru_bwd_kernel(const GlPar
       else gradient_steps<ACC, SEG, false>(p, rt, at, st, exps, most, w.row, a, b, d, gs, sum);
     }
     if (p.part != nullptr && (LINK || w.k == 0)) {
-      // The four segments of the warp, then (behind the next barrier) the warps.
+      // Into the segment's places among the maps, which only this thread has read since the barrier; behind the next
+      // one the segments are added (exchanged between lanes first, 4 x 2047 x 2048 bf16 took 126 us, so 123).
 #pragma unroll
       for (int k = 0; k < 3; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float2 v = unpack2(sum[k][h]);
-#pragma unroll
-          for (int m = kCh / 4; m < 32; m *= 2) {
-            v.x += __shfl_xor_sync(0xffffffffu, v.x, m);
-            v.y += __shfl_xor_sync(0xffffffffu, v.y, m);
-          }
-          if (lane < kCh / 4) *reinterpret_cast<float2*>(&sums[warp][k][at.lc + 2 * h]) = v;
+          *reinterpret_cast<f2*>(&maps[buf][k][at.seg][at.lc + 2 * h]) = sum[k][h];
           sum[k][h] = both(0.f);
         }
       summed = LINK ? w.j : w.s;
