@@ -12,7 +12,7 @@
 // Bound: HBM (5 values per element forward, 9 backward); the special-function unit (6 operations per
 // element forward, 11 backward) comes next. Measured (device time): many sequences, 404 x 321 x 256 fp32 forward
 // 113 us (5.9 TB/s) and backward 209 (5.7), bf16 84 and 184 (instructions); linked, 8191 x 2048 bf16 54 (3.1 TB/s: the
-// links' way to L2 and back on top), 4 x 2047 x 2048 bf16 backward 126 (2.4).
+// links' way to L2 and back on top), 4 x 2047 x 2048 bf16 backward 123 (2.5).
 //
 // Split: a tile is 64 steps (backward 32) of one sequence by 32 channels; a CTA of four warps reads
 // it once. A thread has a segment of 4 (2) neighbouring steps of four neighbouring channels: it folds
@@ -217,7 +217,7 @@ __device__ __forceinline__ void leave_state(const GlParams& p, int64_t j, int c,
 // State in front of the tile for channel c (a lane each; ok false: none): the maps of the tiles in
 // front in its group, folded in their order, applied to the state that the group before left. Three warps fetch
 // five of the maps each while the fourth waits for the state, so that a link is one way to L2 and back
-// (4 x 2047 x 2048 bf16, the fourth warp alone: forward 59 us, backward 135; so: 54 and 126). The first
+// (4 x 2047 x 2048 bf16, the fourth warp alone: forward 59 us, backward 135; so: 54 and 126, with the sums as below 123). The first
 // tile of a sequence has its entry state in its map (A = 0).
 constexpr int kAhead = (kGroup - 1) / 3;  // maps of a warp
 static_assert(3 * kAhead == kGroup - 1, "maps in front");
