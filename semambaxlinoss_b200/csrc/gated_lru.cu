@@ -217,8 +217,8 @@ __device__ __forceinline__ void leave_state(const GlParams& p, int64_t j, int c,
 // State in front of the tile for channel c (a lane each; ok false: none): the maps of the tiles in
 // front in its group, folded in their order, applied to the state that the group before left. Three warps fetch
 // five of the maps each while the fourth waits for the state, so that a link is one way to L2 and back
-// (4 x 2047 x 2048 bf16, the fourth warp alone: forward 59 us, backward 135; so: 54 and 126, with the sums as below 123). The first
-// tile of a sequence has its entry state in its map (A = 0).
+// (4 x 2047 x 2048 bf16, the fourth warp alone: forward 59 us, backward 135; so: 54 and 126, with a tile's sums as
+// they are added now 123). The first tile of a sequence has its entry state in its map (A = 0).
 constexpr int kAhead = (kGroup - 1) / 3;  // maps of a warp
 static_assert(3 * kAhead == kGroup - 1, "maps in front");
 typedef float Links[3][2][kCh];
@@ -379,11 +379,6 @@ __device__ __forceinline__ void bring_quad(typename RawQuad<ACC>::type* to, cons
   else
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(any ? 16 : 0) : "memory");
 }
-
-template <bool V>
-struct Is {
-  static constexpr bool value = V;
-};
 
 template <int ACC, int SEG, int OPS>
 struct Stage {

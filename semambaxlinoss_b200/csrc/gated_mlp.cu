@@ -941,7 +941,8 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 4 : 3) gate_grad_kernel(cons
 // -- few rows ---------------------------------------------------------------------------------
 
 // Up to R rows of x. A warp has two columns (four rows of W); x lies in shared memory in fp32, kDepth
-// values of each row at a time. Its lanes take 8 neighbouring weights of every 256.
+// values of each row at a time. Its lanes take 8 neighbouring weights of every 256. Bound by W's bytes for one or two
+// rows, then by reading x from shared memory (fp32 2048 -> 5504: 1 row 15.2 us, 5.9 TB/s; 2 rows 16.3, 4 19.4, 8 33).
 constexpr int kDepth = 2048, kFewT = 256, kFewBf16 = 16;
 // Rows of fp32 that run so, eight at a time (16 x 2048 -> 5504: 67 us, tiles and the parts of W 89); of bf16 that
 // the kernel below does not take.
@@ -1055,6 +1056,7 @@ __global__ void __launch_bounds__(kFewT, R > 4 ? 2 : 3) few_rows_kernel(const vo
 // its values of two products, and nothing of W passes through shared memory: each warp streams its rows.
 // (tcgen05 would have tiles of 128 rows of x, nearly all of them empty.) Some warps share the depth of
 // eight columns; their sums meet in shared memory.
+// Bound by W's bytes: 1 row of 2048 -> 5504 9.2 us (4.9 TB/s), 8 of 4096 -> 11008 30.7 (5.9).
 // Warps that share the depth (8 rows of 4096 -> 11008, four and eight: 31.8 and 30.7 us, 1 of 2048 -> 5504 11.6
 // and 9.3; 16 rows 45.5 and 42.9, but 2048 -> 5504 11.8 and 15.6).
 constexpr int few_warps(int nt) { return nt == 1 ? 8 : 4; }
