@@ -176,12 +176,11 @@ __device__ __forceinline__ f2 least2(f2 gain) {
   const float2 g = unpack2(gain);
   return pack2(fmaxf(g.x, kLeastGain), fmaxf(g.y, kLeastGain));
 }
-// Far up the exponential of a closed gate ends, so that its product with what it closes is 1. (A NaN stays.)
-__device__ __forceinline__ f2 end2(f2 v) {
-  float2 t = unpack2(v);
-  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.x));  // 126
-  asm("min.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(t.y));
-  return pack2(t.x, t.y);
+// 1 - s of a sigmoid s = 1 / (1 + e): e s, which nothing cancels in, and 1 where e is infinite (a shut gate: s is 0,
+// and so is what it multiplies, however large the rest is; the gradient of a gate that is no number has s in it too).
+__device__ __forceinline__ f2 rest2(f2 e, f2 s) {
+  const float2 t = unpack2(mul2(e, s));
+  return pack2(fminf(t.x, 1.f), fminf(t.y, 1.f));
 }
 __device__ __forceinline__ f2 gate_arg(f2 v, f2 bias) { return fma2(v, both(-kLog2e), bias); }
 
@@ -437,7 +436,7 @@ __device__ __forceinline__ void gate_steps(const GlParams& p, const Rates& rt, i
       const int c = lc + 2 * h;
       const f2 ar = gate_arg(pair_of<ACC>(rr, h, p.bf16), shared_pair(rt.r2, c));
       const f2 ai = gate_arg(pair_of<ACC>(ri, h, p.bf16), shared_pair(rt.i2, c));
-      const f2 er = ex2_2(exps != nullptr ? end2(ar) : ar), ei = ex2_2(exps != nullptr ? end2(ai) : ai);
+      const f2 er = ex2_2(ar), ei = ex2_2(ai);
       f2 rho, m, gain;
       decay2<SLOW>(rsqrt_2(add2(er, both(1.f))), shared_pair(rt.speed, c), shared_pair(rt.root, c), &rho, &m, &a[u][h], &gain);
       const f2 iota = rcp_2(add2(ei, both(1.f)));
@@ -654,17 +653,17 @@ __device__ __forceinline__ void gradient_steps(const GlParams& p, const Rates& r
       const f2 ah = mul2(a[u][k], b[u][k]);
       if (gated) {
         const f2 z = pair_of<ACC>(st.v[3][u][tid], k, p.bf16);
-        const f2 ez = ex2_2(end2(mul2(z, both(-kLog2e)))), s = rcp_2(add2(ez, both(1.f)));
+        const f2 ez = ex2_2(mul2(z, both(-kLog2e))), s = rcp_2(add2(ez, both(1.f)));
         const f2 h = fma2(mul2(gain, iota), x, ah);
-        // silu'(z) = s (1 + z (1 - s)), 1 - s = ez s
-        dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, mul2(ez, s), both(1.f))));
+        // silu'(z) = s (1 + z (1 - s))
+        dz[k] = mul2(mul2(pair_of<ACC>(rg, k, p.bf16), h), mul2(s, fma2(z, rest2(ez, s), both(1.f))));
       }
       const f2 gi = mul2(gt, iota);
       dx[k] = mul2(gi, gain);
-      di[k] = mul2(mul2(dx[k], x), mul2(ei, iota));
+      di[k] = mul2(mul2(dx[k], x), rest2(ei, iota));
       const f2 dla = fma2(gt, ah, mul2(mul2(gi, x), mul2(mul2(a[u][k], a[u][k]), inv)));
       const f2 rd = mul2(rho, dla);
-      dr[k] = mul2(mul2(rd, mul2(er, rho)), shared_pair(rt.minus, c));
+      dr[k] = mul2(mul2(rd, rest2(er, rho)), shared_pair(rt.minus, c));
       gs[k] = mul2(a[u][k], gt);
       sum[0][k] = add2(sum[0][k], rd);
       sum[1][k] = add2(sum[1][k], dr[k]);
