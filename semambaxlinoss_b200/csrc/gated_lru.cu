@@ -126,7 +126,7 @@ __device__ __forceinline__ void load_rates(const GlParams& p, int c0, int lane, 
   s = s > 1e37f ? 1e37f : s;  // an infinite one times a closed gate is no number
   to->speed[lane] = s;
   to->minus[lane] = -s;
-  to->root[lane] = s > 0.f ? 2.f * s * semx::rsqrt_approx(2.f * s) : 2.f * s;
+  to->root[lane] = sqrtf(2.f * s);  // (not by the reciprocal root, which takes a speed below the normal numbers for 0)
   to->r2[lane] = p.r_bias != nullptr ? -kLog2e * p.r_bias[c] : 0.f;
   to->i2[lane] = p.i_bias != nullptr ? -kLog2e * p.i_bias[c] : 0.f;
 }

@@ -49,3 +49,31 @@ def test_shut_gates_pass_nothing_back(packed, dtype):
         assert torch.isfinite(got).all(), name
         over = (got - want[name]).abs() - tol
         assert bool((over <= 0).all()), (name, over.max().item(), int(over.argmax()) % C)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_speeds_below_the_normal_numbers(packed):
+    """rate_scale softplus(rate) among fp32's subnormal numbers, or 0: the decay is 1 and the gain its least
+    value, 1e-3, for whole sequences, their gradients and single tokens. Sums over three steps in fp32, each of
+    at most 8 roundings: 24 eps of terms that do not cancel here, 2e-6 allowed."""
+    from semambaxlinoss_b200.gated_lru import gated_lru_scan, gated_lru_step
+
+    rate = torch.linspace(-92, -82, 41, dtype=torch.float64).repeat(2)[:72]
+    C, L, scale = rate.numel(), 3, 0.1
+    g = gen(52)
+    x, dy = randn((L, C), g).abs().float().double(), randn((L, C), g).abs().float().double()
+    r, i = torch.full((L, C), 3.0, dtype=torch.float64), torch.full((L, C), 0.5, dtype=torch.float64)
+    want = ogl.scan(x, r, i, rate.float().double(), [0, L], scale=scale, dy=dy)
+    cu = torch.tensor([0, L], dtype=torch.int32, device=cuda()) if packed else None
+    d = [t.float().to(cuda()) for t in (x, r, i)]
+    d = [(t if packed else t[None]).requires_grad_() for t in d]
+    rd = rate.float().to(cuda()).requires_grad_()
+    y = gated_lru_scan(d[0], d[1], d[2], rd, rate_scale=scale, cu_seqlens=cu)
+    grads = torch.autograd.grad(y, d + [rd], dy.float().to(cuda()).reshape(y.shape))
+    state = torch.zeros(1, C, device=cuda())
+    toks = torch.cat([gated_lru_step(*(t.detach().reshape(L, C)[k:k + 1] for t in d), rd.detach(), state, rate_scale=scale)
+                      for k in range(L)])
+    for name, got in zip(("y", "dx", "dr", "di", "drate", "y"), (y,) + grads + (toks,)):
+        got = got.detach().double().cpu().reshape(want[name].shape)
+        assert torch.isfinite(got).all(), name
+        assert torch.allclose(got, want[name], rtol=2e-6, atol=1e-30), (name, (got - want[name]).abs().max())
