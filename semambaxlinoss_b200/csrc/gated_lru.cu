@@ -172,9 +172,12 @@ __device__ __forceinline__ void decay2(f2 q, f2 speed, f2 root, f2* rho, f2* m, 
     *gain = pack2(gg.x, gg.y);
   }
 }
+// The gain, its least value at least. (A NaN stays: the gradient of x has no other trace of it.)
 __device__ __forceinline__ f2 least2(f2 gain) {
-  const float2 g = unpack2(gain);
-  return pack2(fmaxf(g.x, kLeastGain), fmaxf(g.y, kLeastGain));
+  float2 g = unpack2(gain);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.x) : "f"(kLeastGain));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.y) : "f"(kLeastGain));
+  return pack2(g.x, g.y);
 }
 // 1 - s of a sigmoid s = 1 / (1 + e): e s, which nothing cancels in, and 1 where e is infinite (a shut gate: s is 0,
 // and so is what it multiplies, however large the rest is; the gradient of a gate that is no number has s in it too).

@@ -77,3 +77,30 @@ def test_speeds_below_the_normal_numbers(packed):
         got = got.detach().double().cpu().reshape(want[name].shape)
         assert torch.isfinite(got).all(), name
         assert torch.allclose(got, want[name], rtol=2e-6, atol=1e-30), (name, (got - want[name]).abs().max())
+
+
+@pytest.mark.parametrize("gate", ["r", "i"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gates_that_are_no_number(gate, dtype):
+    """A NaN among the gates of one step: NaN where the formulas have it, and the other channels as without it."""
+    from semambaxlinoss_b200.gated_lru import gated_lru_scan
+
+    g = gen(53)
+    L, C, at, ch = 150, 40, 70, 9
+    tok = {n: randn((L, C), g).to(dtype) for n in ("x", "r", "i", "z")}
+    rate, dy = torch.full((C,), -5.0), randn((L, C), g).to(dtype)
+
+    def run(tok):
+        d = [tok[n].to(cuda())[None].requires_grad_() for n in ("x", "r", "i", "z")]
+        rd = rate.to(cuda()).requires_grad_()
+        y = gated_lru_scan(d[0], d[1], d[2], rd, z=d[3])
+        return [t.detach().cpu().reshape(-1, C) for t in (y,) + torch.autograd.grad(y, d + [rd], dy.to(cuda())[None])]
+
+    clean = run(tok)
+    tok[gate][at, ch] = float("nan")
+    t64 = {n: t.double() for n, t in tok.items()}
+    want = ogl.scan(t64["x"], t64["r"], t64["i"], rate.double(), [0, L], t64["z"], dy=dy.double())
+    others = torch.arange(C) != ch
+    for name, got, was in zip(NAMES + ("drate",), run(tok), clean):
+        assert torch.equal(torch.isnan(got), torch.isnan(want[name].reshape(got.shape))), name
+        assert torch.equal(got[:, others], was[:, others]), name
