@@ -17,7 +17,7 @@ checkout. Their documented behaviour is restated here:
   the kernel does not take (CPU, other types, rows above 8192 elements) run as nn.LayerNorm behind an addition.
 * ``_init_weights(module, n_layer)``: zero every Linear bias not tagged ``_no_reinit``;
   re-draw every ``out_proj.weight`` / ``fc2.weight`` Kaiming-uniform (a = sqrt(5)) and
-  divide it by sqrt(n_layer).
+  divide it by the root of the residual branches, n_layer, or 2 n_layer with a feed-forward half.
 
 Token layouts (:mod:`semambaxlinoss_b200.layout`): a TF-block keeps its activations as
 one (batch, frames, bins, channels) tensor. The frequency-axis scans read it as
@@ -33,8 +33,8 @@ this package's scan path), ``selective_state`` (the Mamba layer's formulas) and 
 (one gated real mode per channel). The last two take packed sequences, prompts and single
 tokens (``ssm_params``: the mixer's own keyword arguments; ``cu_seqlens``, ``cache``, ``slots``
 and ``fresh`` pass through ``Block.forward``). With ``mlp`` (the keyword arguments of
-``GatedMLP``, an empty dict for its defaults) in the configuration the block has a gated
-feed-forward half behind a second norm. The
+``GatedMLP``, an empty dict for its defaults; None or False for none) in the configuration the
+block has a gated feed-forward half behind a second norm; a hybrid block has none, and refuses it. The
 reference's other backbones (``mamba``, ``mamba2``, ``mamba3`` from mamba_ssm, ``s4d``,
 ``s5``, and ``selective_linoss``, whose source the reference does not contain) raise
 NotImplementedError.
@@ -42,6 +42,7 @@ NotImplementedError.
 from __future__ import annotations
 
 import math
+from collections.abc import Mapping
 from functools import partial
 from typing import Literal
 
@@ -287,14 +288,25 @@ def _build_mixer_cls(d_model, model_cfg, layer_idx=0):
     return partial(MambaStyleMixer, ssm=layer, expand=expand, d_conv=d_conv, causal_conv=causal)
 
 
+def _mlp_cfg(model_cfg):
+    """Keyword arguments of the block's feed-forward half, None without one (``mlp`` absent, None or False)."""
+    mlp = model_cfg.get("mlp", None)
+    if mlp is None or mlp is False:
+        return None
+    if not isinstance(mlp, Mapping):
+        raise ValueError("mlp must be GatedMLP's keyword arguments (an empty dict for its defaults), or None or False "
+                         f"for no feed-forward half, got {mlp!r}")
+    return mlp
+
+
 def create_block(d_model, model_cfg, layer_idx=0, rms_norm=True, fused_add_norm=False,
                  residual_in_fp32=False):
     norm_eps = model_cfg.get("norm_epsilon", 1e-5)
     layer_norm_cls = LayerNorm if fused_add_norm else nn.LayerNorm
     norm_cls = partial(layer_norm_cls if not rms_norm else RMSNorm, eps=norm_eps)
     if model_cfg["ssm"] == "hybrid":
-        if model_cfg.get("mlp", None) is not None:
-            raise ValueError("a hybrid block has no feed-forward half; mlp must be absent")
+        if any(_mlp_cfg(cfg) is not None for cfg in (model_cfg, model_cfg["backbone_1"], model_cfg["backbone_2"])):
+            raise ValueError("a hybrid block and its backbones have no feed-forward half; mlp must be absent")
         hybrid_cfg = model_cfg.get("hybrid", {})
         b1 = _build_mixer_cls(d_model, model_cfg["backbone_1"], layer_idx)(d_model)
         b2 = _build_mixer_cls(d_model, model_cfg["backbone_2"], layer_idx)(d_model)
@@ -304,7 +316,7 @@ def create_block(d_model, model_cfg, layer_idx=0, rms_norm=True, fused_add_norm=
         block.layer_idx = layer_idx
         return block
     mixer_cls = _build_mixer_cls(d_model, model_cfg, layer_idx)
-    mlp = model_cfg.get("mlp", None)
+    mlp = _mlp_cfg(model_cfg)
     mlp_cls = nn.Identity if mlp is None else partial(GatedMLP, **mlp)
     block = Block(d_model, mixer_cls, mlp_cls, norm_cls=norm_cls,
                   fused_add_norm=fused_add_norm, residual_in_fp32=residual_in_fp32)
@@ -327,7 +339,7 @@ class MambaBlock(nn.Module):
         if self.bidirectional:
             self.backward_blocks = nn.ModuleList(create_block(in_channels, cfg) for _ in range(n_layer))
         self.apply(partial(_init_weights, n_layer=n_layer,
-                           n_residuals_per_layer=1 if cfg.get("mlp", None) is None else 2))
+                           n_residuals_per_layer=1 if _mlp_cfg(cfg) is None else 2))
 
     def accepts_layout(self, layout: TokenLayout) -> bool:
         """Whether forward(x, layout=layout) reads x in place: the forward blocks take
