@@ -791,7 +791,9 @@ int semx_gated_lru_step(const SemxGatedLruArgs* args, semx_stream_t stream);
  * aligned; 0 bytes for narrow bf16 rows, whose u and g the backward makes again from x, w and
  * bias) and the backward reads it. It writes dx, dw and db (each may be NULL), sums in a
  * fixed order. Workspace (16-byte aligned, of this call alone): semx_gated_linear_workspace_bytes() of
- * the filled struct with `backward` 0 or 1. */
+ * the filled struct with `backward` 0 or 1. That depends on all sizes, on whether x and w lie on 16 bytes
+ * (a query with x or w NULL counts for any address of it) and, backward, on which of dx, dw and db are
+ * set; workspace_bytes says what workspace holds, and a call that needs more is refused. */
 typedef struct SemxGatedLinearArgs {
   uint32_t struct_size;
   int32_t bf16;
@@ -808,6 +810,7 @@ typedef struct SemxGatedLinearArgs {
   void* dw;
   float* db;
   void* workspace;
+  int64_t workspace_bytes;
 } SemxGatedLinearArgs;
 
 size_t semx_gated_linear_args_size(void);

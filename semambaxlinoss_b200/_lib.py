@@ -294,7 +294,8 @@ class SemxGatedLinearArgs(ctypes.Structure):
         ("act", ctypes.c_int32),
         ("bias_bf16", ctypes.c_int32),
     ] + [(name, ctypes.c_int64) for name in ("rows", "D", "H", "ldx")] + [
-        (name, ctypes.c_void_p) for name in ("x", "w", "bias", "h", "saved", "dh", "dx", "dw", "db", "workspace")]
+        (name, ctypes.c_void_p) for name in ("x", "w", "bias", "h", "saved", "dh", "dx", "dw", "db", "workspace")] + [
+        ("workspace_bytes", ctypes.c_int64)]
 
 
 # (python struct, C size query) for every argument struct in semx.h.

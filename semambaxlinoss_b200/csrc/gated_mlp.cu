@@ -1278,7 +1278,7 @@ int launch_gemm(const Plan& q, const Operand& A, const Operand& B, cudaStream_t 
   return semx::check_launch("gated_linear join_kernel");
 }
 
-int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
+int gl_check_sizes(const SemxGatedLinearArgs* a) {
   const int64_t top = (int64_t)1 << 31;
   SEMX_REQUIRE(a->rows >= 0 && a->rows < top && a->D >= 1 && a->D < (1 << 23) && a->H >= 1 && a->H < (1 << 23),
                SEMX_ERR_SHAPE, "gated_linear: rows=%lld, D=%lld, H=%lld", (long long)a->rows, (long long)a->D, (long long)a->H);
@@ -1290,6 +1290,11 @@ int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
                    cdiv(a->D, (int64_t)64) * cdiv(a->H, (int64_t)32) < ((int64_t)1 << 30) &&
                    cdiv(a->rows, (int64_t)kK) * 6 < top,
                SEMX_ERR_SHAPE, "gated_linear: rows=%lld, D=%lld, H=%lld", (long long)a->rows, (long long)a->D, (long long)a->H);
+  return SEMX_OK;
+}
+int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
+  const int rc = gl_check_sizes(a);
+  if (rc != SEMX_OK) return rc;
   if (a->rows == 0 && !bwd) return SEMX_OK;
   SEMX_REQUIRE(a->w && (a->rows == 0 || a->x), SEMX_ERR_NULL, "gated_linear: x / w is NULL");
   if (!bwd) SEMX_REQUIRE(a->h, SEMX_ERR_NULL, "gated_linear: h is NULL");
@@ -1301,8 +1306,9 @@ int gl_check(const SemxGatedLinearArgs* a, bool bwd) {
   return SEMX_OK;
 }
 
-// Whether TMA reads rows of n bf16 at stride ld from base.
-bool in_place(const void* base, int64_t ld, int bf16) { return bf16 && ld % 8 == 0 && semx::aligned(base, 16); }
+// Whether TMA reads rows of n bf16 at stride ld from base. (A size query may leave a base open: it could be anywhere.)
+bool on_16(const void* base) { return base != nullptr && semx::aligned(base, 16); }
+bool in_place(const void* base, int64_t ld, int bf16) { return bf16 && ld % 8 == 0 && on_16(base); }
 
 template <int NT>
 int launch_few_bf16(const SemxGatedLinearArgs* a, const GemmParams& p, cudaStream_t st) {
@@ -1326,10 +1332,10 @@ Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
   l.parts = a->bf16 ? 1 : kParts;
   // (Rows that the wide loads take.)
   l.few_bf16 = !bwd && a->bf16 && a->rows <= kFewBf16 && a->D % 8 == 0 && (a->ldx % 8 == 0 || a->rows == 1) &&
-               semx::aligned(a->x, 16) && semx::aligned(a->w, 16);
+               on_16(a->x) && on_16(a->w);
   l.few = !bwd && a->rows <= (a->bf16 ? kFew : kFewFp32) && !l.few_bf16;
   if (a->rows == 0 || l.few || l.few_bf16) return l;
-  // Laid out anew wherever the sizes allow a misaligned base: the query has no addresses that count.
+  // Laid out anew where TMA cannot read them, which depends on the addresses too: hence workspace_bytes.
   l.lay_x = !in_place(a->x, a->ldx, a->bf16);
   l.lay_w = !in_place(a->w, a->D, a->bf16);
   const int64_t Dp = up8(a->D), Hp = up8(a->H);
@@ -1358,6 +1364,13 @@ Layout layout_of(const SemxGatedLinearArgs* a, bool bwd) {
   }
   l.total = at;
   return l;
+}
+
+int gl_check_workspace(const SemxGatedLinearArgs* a, const Layout& l) {
+  SEMX_REQUIRE(l.total == 0 || (a->workspace != nullptr && a->workspace_bytes >= (int64_t)l.total), SEMX_ERR_WORKSPACE,
+               "gated_linear: a workspace of %lld bytes where the call needs %zu", (long long)(a->workspace ? a->workspace_bytes : 0),
+               l.total);
+  return SEMX_OK;
 }
 
 template <int R>
@@ -1430,7 +1443,7 @@ size_t semx_gated_linear_saved_bytes(const SemxGatedLinearArgs* a) {
 }
 
 size_t semx_gated_linear_workspace_bytes(const SemxGatedLinearArgs* a, int32_t backward) {
-  if (a == nullptr || a->rows < 0 || a->D < 1 || a->H < 1) return 0;
+  if (a == nullptr || gl_check_sizes(a) != SEMX_OK) return 0;
   return layout_of(a, backward != 0).total;
 }
 
@@ -1438,11 +1451,13 @@ int semx_gated_linear_fwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   SEMX_CHECK_ARGS(a, SemxGatedLinearArgs);
   int rc = gl_check(a, false);
   if (rc != SEMX_OK || a->rows == 0) return rc;
+  const Layout l = layout_of(a, false);
+  rc = gl_check_workspace(a, l);
+  if (rc != SEMX_OK) return rc;
   semx::DeviceScope scope;
   rc = scope.bind({a->h});
   if (rc != SEMX_OK) return rc;
   cudaStream_t st = semx::as_stream(stream);
-  const Layout l = layout_of(a, false);
   Plan q = l.fwd;
   q.p.out = a->h;
   q.p.ldo = a->H;
@@ -1474,7 +1489,6 @@ int semx_gated_linear_fwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
     }
     return SEMX_OK;
   }
-  SEMX_REQUIRE(l.total == 0 || a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_linear: workspace is NULL");
   char* ws = reinterpret_cast<char*>(a->workspace);
   q.p.part = reinterpret_cast<float*>(ws + l.part);
   Operand x, w;
@@ -1487,6 +1501,11 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
   SEMX_CHECK_ARGS(a, SemxGatedLinearArgs);
   int rc = gl_check(a, true);
   if (rc != SEMX_OK) return rc;
+  const bool need_x = a->dw != nullptr, need_w = a->dx != nullptr;
+  if (!need_x && !need_w && a->db == nullptr) return SEMX_OK;
+  const Layout l = layout_of(a, true);
+  rc = gl_check_workspace(a, l);
+  if (rc != SEMX_OK) return rc;
   semx::DeviceScope scope;
   rc = scope.bind({a->dw, a->dx, a->db});
   if (rc != SEMX_OK) return rc;
@@ -1498,10 +1517,6 @@ int semx_gated_linear_bwd(const SemxGatedLinearArgs* a, semx_stream_t stream) {
     SEMX_REQUIRE(e == cudaSuccess, SEMX_ERR_LAUNCH, "gated_linear bwd: cudaMemsetAsync: %s", cudaGetErrorString(e));
     return SEMX_OK;
   }
-  const bool need_x = a->dw != nullptr, need_w = a->dx != nullptr;
-  if (!need_x && !need_w && a->db == nullptr) return SEMX_OK;
-  const Layout l = layout_of(a, true);
-  SEMX_REQUIRE(a->workspace != nullptr, SEMX_ERR_WORKSPACE, "gated_linear bwd: workspace is NULL");
   char* ws = reinterpret_cast<char*>(a->workspace);
   const int64_t Hp = up8(a->H);
   float* sums = a->db != nullptr ? reinterpret_cast<float*>(ws + l.sums) : nullptr;

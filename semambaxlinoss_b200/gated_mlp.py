@@ -54,7 +54,7 @@ def _workspace(a, nbytes, like):
     if not nbytes:
         return None
     ws = _lib.scratch(nbytes, like)
-    a.workspace = ws.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     return ws
 
 
