@@ -1188,7 +1188,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // What one product needs: tile width, slices of the depth, bytes of their sums.
 struct Plan {
-  int mode, bn;
+  int bn;
   GemmParams p;
   size_t part_bytes;
 };
@@ -1200,7 +1200,6 @@ constexpr int kTileCost = 96;
 // M, N: the result; K: the depth of one half.
 Plan plan_gemm(int mode, int64_t M, int64_t N, int64_t K, int parts) {
   Plan q = {};
-  q.mode = mode;
   GemmParams& p = q.p;
   p.M = M;
   p.N = N;
