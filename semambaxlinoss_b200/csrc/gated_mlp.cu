@@ -17,7 +17,8 @@
 // products of parts are taken (the others are below 2^-24 of the result). The tensor cores cut where
 // an addition rounds, which shows over thousands of additions: so the large products (first parts) are
 // summed in tensor memory over 128 of the depth at a time, and those sums in registers; the small ones
-// have an accumulator of their own.
+// have an accumulator of their own. bf16 sums over rows (dW) leave tensor memory every 4096 rows; h and dx, whose depth
+// is a width, stay there (9e-8 of a sum per 16 of the depth at most, where terms have one sign).
 // Few rows (bf16 up to 16, fp32 16 by eights): the weights' bytes are the bound, and warps stream them, bf16
 // through the legacy tensor products (a tcgen05 tile would be nearly empty), fp32 through packed multiplies.
 //
@@ -50,7 +51,11 @@ constexpr int kCols = 16;           // columns that a warp writes at a time
 constexpr int kBufRow = kCols + 4;  // floats of a row of its exchange buffer
 constexpr int kBuf = 32 * kBufRow + 64;  // floats of the buffer, and of u's and g's biases (32 columns) behind it
 constexpr int kParts = 3;           // bf16 parts of an fp32 value
-constexpr int kDrain = 2;           // stages whose large products one accumulator takes (fp32)
+// Stages whose large products one accumulator takes: of fp32; and of bf16 where the depth is the rows, which have no
+// end (dW of 131072 x 1024 -> 2752, terms of one sign: in one sum 7.1e-4 too small, of 524288 rows 3.0e-3, where the
+// results' own rounding is 1.4e-3; in runs of 64 stages 1.2e-5 for the former. dW of 8192 x 2048 -> 5504
+// 246.7 us in one sum, 249.8, 248.9 and 248.5 in runs of 16, 32 and 64; 16384 x 1024 -> 2752 131.8, and 139.6, 136.3, 134.6).
+constexpr int kDrain = 2, kRun = 64;
 
 __device__ unsigned int g_gemm_timeouts;
 
@@ -410,6 +415,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
   constexpr bool GATED = MODE == kFwd || MODE == kGate;  // u and g side by side
   constexpr bool A_MN = MODE == kDw, B_MN = !GATED;
   constexpr int CN = GATED ? BN / 2 : BN;               // columns of the result in a tile
+  constexpr bool DRAINED = PARTS > 1 || MODE == kDw;    // sums leave tensor memory every RUN stages
+  constexpr int RUN = PARTS > 1 ? kDrain : kRun;
   constexpr int COLS = (PARTS > 1 ? 4 : 2) * BN;        // of tensor memory: two accumulators, fp32 two more for the small products
   static_assert(COLS <= 512, "tensor memory");
   extern __shared__ uint8_t raw[];
@@ -536,7 +543,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         slice(t, &k0, &k1);
         const uint32_t small = tmem + 2 * BN + (tiles & 1) * BN;
         if (PARTS > 1 && !await(&small_empty[tiles & 1], ((tiles >> 1) & 1) ^ 1)) break;
-        const int drain = PARTS > 1 ? kDrain : k1 - k0;
+        const int drain = DRAINED ? RUN : k1 - k0;
         for (int c0 = k0; c0 < k1 && ok; c0 += drain, ++acc) {
           const uint32_t b = acc & 1, d = tmem + b * BN;
           if (!await(&acc_empty[b], ((acc >> 1) & 1) ^ 1)) break;
@@ -670,7 +677,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
         __syncwarp();
         if (w + pairs < works) fetch_bias(tile_at(p, w + pairs));
       }
-      if constexpr (PARTS == 1) {
+      if constexpr (!DRAINED) {
         const uint32_t b = acc & 1, d = tmem + b * BN + lanes;
         const bool ok = wait_phase(&acc_full[b], (acc >> 1) & 1, &dead);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -710,23 +717,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmT, 1)
           ++acc;
         };
         drain(std::true_type());
-        for (int c0 = k0 + kDrain; c0 < k1 && ok; c0 += kDrain) drain(std::false_type());
+        for (int c0 = k0 + RUN; c0 < k1 && ok; c0 += RUN) drain(std::false_type());
         if (!ok) break;
-        ok = wait_phase(&small_full[tiles & 1], (tiles >> 1) & 1, &dead);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        semx::tc::fence_after_sync();
+        if constexpr (PARTS > 1) {
+          ok = wait_phase(&small_full[tiles & 1], (tiles >> 1) & 1, &dead);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          semx::tc::fence_after_sync();
 #pragma unroll
-        for (int i = 0; i < VALUES; i += 2 * kCols) {
-          float v[kCols], y[kCols];
-          const uint32_t small = tmem + 2 * BN + (tiles & 1) * BN + lanes;
-          tmem_ld16_twice(small + column(i), small + column(i + kCols), v, y);
+          for (int i = 0; i < VALUES; i += 2 * kCols) {
+            float v[kCols], y[kCols];
+            const uint32_t small = tmem + 2 * BN + (tiles & 1) * BN + lanes;
+            tmem_ld16_twice(small + column(i), small + column(i + kCols), v, y);
 #pragma unroll
-          for (int j = 0; j < kCols; ++j) {
-            sum[i + j] += v[j];
-            sum[i + kCols + j] += y[j];
+            for (int j = 0; j < kCols; ++j) {
+              sum[i + j] += v[j];
+              sum[i + kCols + j] += y[j];
+            }
           }
+          release((tiles & 1) ? small_e1 : small_e0);
         }
-        release((tiles & 1) ? small_e1 : small_e0);
 #pragma unroll
         for (int c = 0; c < WC; c += kCols) {
           float v[kCols], g[kCols];
