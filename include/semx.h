@@ -786,7 +786,9 @@ int semx_gated_lru_step(const SemxGatedLruArgs* args, semx_stream_t stream);
  * x (rows, D) at row stride ldx, w (2 H, D) contiguous (the value's rows, then the gate's), h, dh
  * (rows, H), dx (rows, D) and dw contiguous; all bf16 when `bf16` is set, else fp32. bias
  * (2 H, may be NULL) bf16 when bias_bf16 is set, else fp32, db (2 H, may be NULL) fp32. Sums are fp32; fp32
- * operands keep 2^-24 of each product (as three bf16 parts; an infinity among them gives NaN).
+ * operands keep 2^-24 of each product (as three bf16 parts; an infinity among them makes what depends on
+ * it infinite or NaN, from 17 rows on NaN). With bf16 operands the gradients of u and g are rounded to
+ * bf16 for the products that give dx and dw (db is their sum before that).
  * A training forward passes saved (semx_gated_linear_saved_bytes(): u and g in fp32, 16-byte
  * aligned; 0 bytes for narrow bf16 rows, whose u and g the backward makes again from x, w and
  * bias) and the backward reads it. It writes dx, dw and db (each may be NULL), sums in a

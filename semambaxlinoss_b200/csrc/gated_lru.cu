@@ -11,8 +11,12 @@
 //
 // Bound: HBM (5 values per element forward, 9 backward); the special-function unit (6 operations per
 // element forward, 11 backward) comes next. Measured (device time): many sequences, 404 x 321 x 256 fp32 forward
-// 113 us (5.9 TB/s) and backward 209 (5.7), bf16 84 and 184 (instructions); linked, 8191 x 2048 bf16 54 (3.1 TB/s: the
-// links' way to L2 and back on top), 4 x 2047 x 2048 bf16 backward 123 (2.5).
+// 113 us (5.9 TB/s) and backward 210 (5.7), bf16 84 and 183 (no unit is full: issue slots 58 %, special functions 56 and
+// 47 %, memory 43 and 33 %, 28 and 24 % of the warps; they wait for one another at the barriers and for results); linked,
+// 8191 x 2048 bf16 54 (3.1 TB/s: the links' way to L2 and back on top) and backward 123, fp32 72 and 144, 4 x 2047 x 2048
+// bf16 backward 123 (2.5). These have decays above 0.883 (kNear); one below among four neighbouring channels takes
+// their thread through decay2's other branch: 404 x 321 x 256 fp32 131 and 257, bf16 118 and 257, 8191 x 2048 bf16 70
+// and 158, fp32 86 and 175.
 //
 // Split: a tile is 64 steps (backward 32) of one sequence by 32 channels; a CTA of four warps reads
 // it once. A thread has a segment of 4 (2) neighbouring steps of four neighbouring channels: it folds
@@ -1005,7 +1009,11 @@ int gl_validate(const SemxGatedLruArgs* a, bool bwd, GlParams* p) {
 }
 
 // Whether tiles are linked: packed sequences, whose lengths the host does not know, and sequences too
-// few to give each SM four CTAs that walk them.
+// few to give each SM four CTAs that walk them. Sequences of 1000 steps, linked (with the clearing) and walked, us:
+//   pairs of a sequence and a channel tile      128          256          384          512          768         3232 (321 steps)
+//   forward bf16                             21 and 30    34 and 39    46 and 44    59 and 49    83 and 80    115 and 86
+//   backward bf16                            39 and 55    72 and 67   105 and 84   138 and 103  205 and 176   281 and 186
+// fp32 is alike. (By these figures a walk would pay from 384 pairs on, in the backward from 256.)
 bool gl_linked(const GlParams& p) {
   if (p.m.cu != nullptr) return true;
   return p.m.per > 1 && p.m.S * p.ctiles < kSms * 4;
